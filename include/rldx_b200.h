@@ -295,6 +295,72 @@ int rldx_qk_rmsnorm_rope(const void* x, void* y, const void* w, const int32_t* p
                          int head_dim, float eps, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Token decoding over a paged 4-bit cache of keys and values (no counterpart in the reference,
+ * whose backbone only prefills).
+ *
+ * Pool `data`: [pages, kv_heads, page_size / 32, 40 head_dim] bytes, 16-byte aligned; a unit of
+ * 40 head_dim bytes holds K and V of 32 consecutive tokens of a head as 4-bit codes with an fp16
+ * scale and low per token and 32 channels (value = scale * code + low).  Token i of sequence s
+ * stands in page table[s * table_ld + i / page_size].  lengths[s] is the number of tokens that
+ * sequence s holds, its new ones included; cu_seqlens[s] .. cu_seqlens[s + 1] are the rows of its
+ * new tokens, which are the last tokens it holds.  head_dim is 64 or 128, page_size a multiple
+ * of 32.  Table entries past a sequence's length are never read.
+ *
+ * What the host cannot see is checked on the device: an entry that names no page of the pool, a
+ * RoPE row outside the table, a sequence with more tokens than max_len or max_new says records
+ * a device error (0x500, 0x501, 0x502) and the access is skipped.
+ * ------------------------------------------------------------------------------------------ */
+typedef struct rldx_kv4_cache {
+  void* data;
+  const int32_t* table;
+  const int32_t* lengths;
+  const int32_t* cu_seqlens;
+  int64_t pages;
+  int page_size;
+  int kv_heads;
+  int head_dim;
+  int table_width;
+  int table_ld;
+  int seqs;
+} rldx_kv4_cache;
+
+/* q = rope(rms(q) * q_norm), k = rope(rms(k) * k_norm) per head (rotate-half RoPE, eps inside the
+ * mean's root), all in fp32: q to bf16 [tokens, q_heads, head_dim], k and v into the cache.
+ * qkv: bf16 rows [q | k | v] with stride ld (a multiple of 8); q_norm, k_norm bf16 [head_dim];
+ * rope_cos / rope_sin [rope_rows, head_dim] bf16, or fp32 with rope_fp32; rope_pos [tokens] rows
+ * of them. */
+int rldx_kv4_append(const rldx_kv4_cache* cache, const void* qkv, int64_t ld, int tokens, int q_heads,
+                    const void* q_norm, const void* k_norm, const void* rope_cos, const void* rope_sin,
+                    int rope_fp32, int rope_rows, const int32_t* rope_pos, void* q_out, float eps, void* stream);
+
+/* The values that the cache holds for the new tokens: k, v bf16 [tokens, kv_heads, head_dim]. */
+int rldx_kv4_read(const rldx_kv4_cache* cache, int tokens, void* k, void* v, void* stream);
+
+/* Softmax attention of the new tokens' queries over the cache: the token at position p sees key
+ * j <= p, with window > 0 only j > p - window or j < sinks.  A row that sees no key is zero.
+ * q, out bf16 [tokens, q_heads, head_dim], q with token stride ldq (a multiple of 8); query head
+ * h reads kv head h / (q_heads / kv_heads).  max_new / max_len bound the new tokens and the
+ * length of a sequence (they size the launch; values on the device may be smaller). */
+typedef struct rldx_kv4_attention_desc {
+  const void* q;
+  void* out;
+  int64_t ldq;
+  int tokens;
+  int q_heads;
+  int max_new;
+  int max_len;
+  int window;
+  int sinks;
+  float scale;
+} rldx_kv4_attention_desc;
+
+/* Bytes of workspace (16-byte aligned, any contents) that rldx_kv4_attention needs; 0: none. */
+int rldx_kv4_attention_workspace_size(const rldx_kv4_cache* cache, const rldx_kv4_attention_desc* a,
+                                      uint64_t* bytes);
+int rldx_kv4_attention(const rldx_kv4_cache* cache, const rldx_kv4_attention_desc* a, void* workspace,
+                       uint64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * SwiGLU activation out[t,i] = silu(gate[t,i]) * up[t,i]  (H % 8 == 0).
  * Replaces ds::grouped_swiglu's activation
  * (rldx/inference/action_model/double_stream/engine/kernels/grouped_swiglu.py:108) and

@@ -154,6 +154,18 @@ class LlmWeights(C.Structure):
                 ("rope_sin", vp), ("deepstack_row_index", C.POINTER(C.c_int))]
 
 
+class Kv4Cache(C.Structure):
+    _fields_ = [("data", vp), ("table", vp), ("lengths", vp), ("cu_seqlens", vp), ("pages", i64),
+                ("page_size", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int), ("table_width", C.c_int),
+                ("table_ld", C.c_int), ("seqs", C.c_int)]
+
+
+class Kv4AttentionDesc(C.Structure):
+    _fields_ = [("q", vp), ("out", vp), ("ldq", i64), ("tokens", C.c_int), ("q_heads", C.c_int),
+                ("max_new", C.c_int), ("max_len", C.c_int), ("window", C.c_int), ("sinks", C.c_int),
+                ("scale", C.c_float)]
+
+
 class MsatIO(C.Structure):
     _fields_ = [("vl", vp), ("state", vp), ("emb_id", vp), ("init_noise", vp),
                 ("physics_hist", vp), ("physics_noise", vp), ("actions", vp),
@@ -188,6 +200,12 @@ SIGNATURES = {
     "rldx_swiglu_bias": (C.c_int, [C.POINTER(SwigluBiasSegment), C.c_int, vp]),
     "rldx_qk_rmsnorm_rope": (C.c_int, [vp, vp, vp, vp, vp, vp, i64, C.c_int, C.c_int,
                                        C.c_float, vp]),
+    "rldx_kv4_append": (C.c_int, [C.POINTER(Kv4Cache), vp, i64, C.c_int, C.c_int, vp, vp, vp, vp, C.c_int,
+                                  C.c_int, vp, vp, C.c_float, vp]),
+    "rldx_kv4_read": (C.c_int, [C.POINTER(Kv4Cache), C.c_int, vp, vp, vp]),
+    "rldx_kv4_attention_workspace_size": (C.c_int, [C.POINTER(Kv4Cache), C.POINTER(Kv4AttentionDesc),
+                                                    C.POINTER(C.c_uint64)]),
+    "rldx_kv4_attention": (C.c_int, [C.POINTER(Kv4Cache), C.POINTER(Kv4AttentionDesc), vp, C.c_uint64, vp]),
     "rldx_swiglu": (C.c_int, [vp, vp, i64, vp, i64, i64, C.c_int, vp]),
     "rldx_msat_create": (C.c_int, [C.POINTER(MsatConfig), C.POINTER(MsatWeights), C.POINTER(vp)]),
     "rldx_msat_destroy": (C.c_int, [vp]),

@@ -72,7 +72,8 @@ int ensure_device() {
       return;
     }
     g_dev_sms[dev] = prop.multiProcessorCount;
-    if (gemm_prepare_device() != cudaSuccess || attention_prepare_device() != cudaSuccess) {
+    if (gemm_prepare_device() != cudaSuccess || attention_prepare_device() != cudaSuccess ||
+        kv4_prepare_device() != cudaSuccess) {
       g_dev_status[dev] = -3;
       return;
     }

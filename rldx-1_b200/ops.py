@@ -334,3 +334,126 @@ def wait_selftest(limit_cycles: int) -> None:
     """Launches the bounded-wait self-test on the current stream: a wait on a barrier nothing
     arrives on runs out after `limit_cycles` and records device error 0x400."""
     check(load().rldx_wait_selftest(int(limit_cycles), _stream()))
+
+
+# ------------------------------------------------------------------------------------------------
+# token decoding: 4-bit key / value cache
+# ------------------------------------------------------------------------------------------------
+def _on_one_device(*tensors) -> int:
+    """Index of the device that holds every tensor; it has to be the current one, whose stream the
+    launch goes to."""
+    index = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"every tensor must be on the current CUDA device {index}, got {t.device} (no CPU path exists)")
+    return index
+
+
+def _raw_stream(index: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def kv4_cache(pages: int, kv_heads: int, head_dim: int, page_size: int = 64, device="cuda") -> torch.Tensor:
+    """An empty pool of `pages` pages for the 4-bit cache: uint8 [pages, kv_heads, page_size / 32,
+    40 head_dim] (5 bits a value).  Its contents may be anything: only appended tokens are read."""
+    if head_dim not in (64, 128) or page_size <= 0 or page_size % 32 or pages <= 0 or kv_heads <= 0:
+        raise ValueError("head_dim must be 64 or 128, page_size a multiple of 32, pages and kv_heads positive")
+    return torch.empty(pages, kv_heads, page_size // 32, 40 * head_dim, dtype=torch.uint8, device=device)
+
+
+def _kv4_desc(cache, table, lengths, cu_seqlens) -> "_lib.Kv4Cache":
+    if cache.dtype != torch.uint8 or cache.dim() != 4 or not cache.is_contiguous():
+        raise ValueError("cache must be a contiguous uint8 tensor [pages, kv_heads, page_size / 32, 40 head_dim]")
+    pages, kv_heads, units, unit_bytes = cache.shape
+    if unit_bytes not in (2560, 5120):
+        raise ValueError("the cache's last dimension must be 40 head_dim with head_dim 64 or 128")
+    if table.dtype != torch.int32 or table.dim() != 2 or table.stride(1) != 1:
+        raise ValueError("table must be a row-major int32 tensor [seqs, pages of a sequence]")
+    seqs, width = table.shape
+    for t, n, name in ((lengths, seqs, "lengths"), (cu_seqlens, seqs + 1, "cu_seqlens")):
+        if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 tensor [{n}]")
+    return _lib.Kv4Cache(cache.data_ptr(), table.data_ptr(), lengths.data_ptr(), cu_seqlens.data_ptr(), pages,
+                         32 * units, kv_heads, unit_bytes // 40, width, max(width, table.stride(0)), seqs)
+
+
+def qkv_rope_append(qkv, q_norm, k_norm, cos, sin, rope_pos, cache, table, lengths, cu_seqlens, *, q_heads: int,
+                    eps: float = 1e-6, out=None) -> torch.Tensor:
+    """Per-head RMSNorm and rotate-half RoPE of q and k, and the write of k and v into the 4-bit
+    cache, in one pass over projected rows qkv [tokens, (q_heads + 2 kv_heads) head_dim] (bf16, any
+    row stride).  Rows cu_seqlens[s] .. cu_seqlens[s + 1] are the new tokens of sequence s, the last
+    of its lengths[s] tokens; table [seqs, n] int32 gives its pages.  q_norm, k_norm [head_dim] bf16;
+    cos, sin [rows, head_dim] bf16 or fp32, rope_pos [tokens] int32 their rows.  Returns q
+    [tokens, q_heads, head_dim]: fp32 arithmetic, one rounding to bf16."""
+    _need(qkv, "qkv")
+    _need(q_norm, "q_norm")
+    _need(k_norm, "k_norm")
+    index = _on_one_device(qkv, q_norm, k_norm, cos, sin, rope_pos, cache, table, lengths, cu_seqlens, out)
+    d = _kv4_desc(cache, table, lengths, cu_seqlens)
+    ld, hd = _row_major(qkv, "qkv"), d.head_dim
+    tokens, width = qkv.shape
+    if width != (q_heads + 2 * d.kv_heads) * hd:
+        raise ValueError(f"qkv rows must hold (q_heads + 2 kv_heads) head_dim = {(q_heads + 2 * d.kv_heads) * hd} values, got {width}")
+    if q_norm.shape != (hd,) or k_norm.shape != (hd,) or q_norm.stride(0) != 1 or k_norm.stride(0) != 1:
+        raise ValueError(f"q_norm and k_norm must be contiguous [{hd}]")
+    if cos.dtype not in (torch.bfloat16, torch.float32) or sin.dtype != cos.dtype:
+        raise TypeError("cos and sin must both be bfloat16 or both float32")
+    if cos.dim() != 2 or cos.shape[1] != hd or sin.shape != cos.shape or not cos.is_contiguous() or not sin.is_contiguous():
+        raise ValueError(f"cos and sin must be contiguous [rows, {hd}]")
+    _need(rope_pos, "rope_pos", torch.int32)
+    if rope_pos.shape != (tokens,) or not rope_pos.is_contiguous():
+        raise ValueError(f"rope_pos must be a contiguous tensor [{tokens}]")
+    if out is None:
+        out = torch.empty(tokens, q_heads, hd, dtype=torch.bfloat16, device=qkv.device)
+    elif out.dtype != torch.bfloat16 or out.shape != (tokens, q_heads, hd) or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous bfloat16 tensor [{tokens}, {q_heads}, {hd}]")
+    if tokens == 0:
+        return out
+    check(load().rldx_kv4_append(C.byref(d), qkv.data_ptr(), max(ld, width), tokens, q_heads, q_norm.data_ptr(), k_norm.data_ptr(),
+                                 cos.data_ptr(), sin.data_ptr(), cos.dtype == torch.float32, cos.shape[0],
+                                 rope_pos.data_ptr(), out.data_ptr(), eps, _raw_stream(index)))
+    return out
+
+
+def kv4_read(cache, table, lengths, cu_seqlens, *, tokens: int):
+    """The values that the cache holds for the `tokens` new tokens: k, v [tokens, kv_heads, head_dim]
+    bf16.  With lengths and cu_seqlens that call every token new, the whole of the sequences."""
+    index = _on_one_device(cache, table, lengths, cu_seqlens)
+    d = _kv4_desc(cache, table, lengths, cu_seqlens)
+    if tokens < 0:
+        raise ValueError("tokens must not be negative")
+    kv = torch.empty(2, tokens, d.kv_heads, d.head_dim, dtype=torch.bfloat16, device=cache.device)
+    k, v = kv.unbind(0)
+    if tokens:
+        check(load().rldx_kv4_read(C.byref(d), tokens, k.data_ptr(), v.data_ptr(), _raw_stream(index)))
+    return k, v
+
+
+def kv4_attention(q, cache, table, lengths, cu_seqlens, *, max_new: int, max_len: int, window: int = 0,
+                  sinks: int = 0, scale: Optional[float] = None, out=None) -> torch.Tensor:
+    """Softmax attention of the new tokens' queries q [tokens, q_heads, head_dim] (bf16, any token
+    stride) over the 4-bit cache, grouped-query heads: the token at position p of its sequence sees
+    key j <= p, with window > 0 only j > p - window or j < sinks.  A token that sees no key gives
+    zeros.  max_new and max_len bound the new tokens and the length of any sequence (a launch is
+    sized by them; the device's values may be smaller, larger ones record device error 0x502).
+    scale defaults to head_dim ** -0.5.  Returns [tokens, q_heads, head_dim]."""
+    _need(q, "q")
+    index = _on_one_device(q, cache, table, lengths, cu_seqlens, out)
+    d = _kv4_desc(cache, table, lengths, cu_seqlens)
+    if q.dim() != 3 or q.shape[2] != d.head_dim or q.stride(2) != 1 or (q.shape[1] > 1 and q.stride(1) != d.head_dim):
+        raise ValueError(f"q must be [tokens, q_heads, {d.head_dim}] with the heads of a token side by side")
+    tokens, q_heads, hd = q.shape
+    if out is None:
+        out = torch.empty(tokens, q_heads, hd, dtype=torch.bfloat16, device=q.device)
+    elif out.dtype != torch.bfloat16 or out.shape != q.shape or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous bfloat16 tensor {tuple(q.shape)}")
+    if tokens == 0:
+        return out
+    a = _lib.Kv4AttentionDesc(q.data_ptr(), out.data_ptr(), max(q.stride(0), q_heads * hd), tokens, q_heads, max_new, max_len,
+                              window, sinks, hd ** -0.5 if scale is None else scale)
+    lib, need = load(), C.c_uint64(0)
+    check(lib.rldx_kv4_attention_workspace_size(C.byref(d), C.byref(a), C.byref(need)))
+    ws = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
+    check(lib.rldx_kv4_attention(C.byref(d), C.byref(a), None if ws is None else ws.data_ptr(), need.value,
+                                 _raw_stream(index)))
+    return out
