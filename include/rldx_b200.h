@@ -361,6 +361,24 @@ int rldx_kv4_attention(const rldx_kv4_cache* cache, const rldx_kv4_attention_des
                        uint64_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * One token per row of logits [rows, vocab] (bf16, or fp32 with logits_fp32; row stride ld) from a
+ * given number u[row] in [0, 1).  With M the row's maximum and T its temperature a token's weight
+ * is the whole number floor(2^32 exp((x - M) / T)); in the order of descending logits (equal ones
+ * by ascending id) the kept tokens are the first top_k, those with less than top_p of the weight
+ * that top_k left before them (the first always), and those of weight >= min_p 2^32.  The draw
+ * is the first kept token, in the order of ids, whose inclusive sum of weights passes u times
+ * the whole.  All sums are exact: the result depends on no launch shape or order.
+ * temperature, top_k, top_p, min_p: [rows] or NULL (1, off, off, off); T <= 0 (or NaN) takes the
+ * largest logit; top_k <= 0 or >= vocab, top_p >= 1, min_p <= 0 are off.  NaN logits are never
+ * drawn; a row without any other gives token -1, logprob -inf, kept 0.
+ * token [rows] int64, logprob [rows] fp32: log of the token's share of the kept weight, kept
+ * [rows] int32: tokens kept.  vocab <= 393216.
+ * ------------------------------------------------------------------------------------------ */
+int rldx_sample(const void* logits, int64_t ld, int rows, int vocab, int logits_fp32, const float* u,
+                const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                int64_t* token, float* logprob, int32_t* kept, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * SwiGLU activation out[t,i] = silu(gate[t,i]) * up[t,i]  (H % 8 == 0).
  * Replaces ds::grouped_swiglu's activation
  * (rldx/inference/action_model/double_stream/engine/kernels/grouped_swiglu.py:108) and

@@ -206,6 +206,7 @@ SIGNATURES = {
     "rldx_kv4_attention_workspace_size": (C.c_int, [C.POINTER(Kv4Cache), C.POINTER(Kv4AttentionDesc),
                                                     C.POINTER(C.c_uint64)]),
     "rldx_kv4_attention": (C.c_int, [C.POINTER(Kv4Cache), C.POINTER(Kv4AttentionDesc), vp, C.c_uint64, vp]),
+    "rldx_sample": (C.c_int, [vp, i64, C.c_int, C.c_int, C.c_int, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
     "rldx_swiglu": (C.c_int, [vp, vp, i64, vp, i64, i64, C.c_int, vp]),
     "rldx_msat_create": (C.c_int, [C.POINTER(MsatConfig), C.POINTER(MsatWeights), C.POINTER(vp)]),
     "rldx_msat_destroy": (C.c_int, [vp]),

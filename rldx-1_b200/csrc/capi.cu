@@ -73,7 +73,7 @@ int ensure_device() {
     }
     g_dev_sms[dev] = prop.multiProcessorCount;
     if (gemm_prepare_device() != cudaSuccess || attention_prepare_device() != cudaSuccess ||
-        kv4_prepare_device() != cudaSuccess) {
+        kv4_prepare_device() != cudaSuccess || sample_prepare_device() != cudaSuccess) {
       g_dev_status[dev] = -3;
       return;
     }

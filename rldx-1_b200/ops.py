@@ -457,3 +457,37 @@ def kv4_attention(q, cache, table, lengths, cu_seqlens, *, max_new: int, max_len
     check(lib.rldx_kv4_attention(C.byref(d), C.byref(a), None if ws is None else ws.data_ptr(), need.value,
                                  _raw_stream(index)))
     return out
+
+
+# ------------------------------------------------------------------------------------------------
+# token decoding: sampling
+# ------------------------------------------------------------------------------------------------
+def sample(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=None):
+    """One token per row of logits [rows, vocab] (bf16 or fp32, any row stride) from the given numbers
+    u [rows] fp32 in [0, 1), after temperature, top-k, top-p (of the weight that top-k leaves) and
+    min-p ([rows] tensors, fp32 and int32 for top_k, or None).  Temperature 0 takes the largest
+    logit; ties go to the lowest id.  Weights are whole numbers, floor(2^32 exp((x - max) / T)), so
+    a row's draw is the same in every batch.  Returns token [rows] int64, logprob [rows] fp32 (of the
+    kept distribution) and kept [rows] int32, the number of tokens that the filters left."""
+    if logits.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"logits must be bfloat16 or float32, got {logits.dtype}")
+    index = _on_one_device(logits, u, temperature, top_k, top_p, min_p)
+    ld = _row_major(logits, "logits")
+    rows, vocab = logits.shape
+    ptr = []
+    for t, name, dtype in ((u, "u", torch.float32), (temperature, "temperature", torch.float32), (top_k, "top_k", torch.int32),
+                           (top_p, "top_p", torch.float32), (min_p, "min_p", torch.float32)):
+        if t is None and name != "u":
+            ptr.append(None)
+            continue
+        if t.dtype != dtype or t.shape != (rows,) or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {dtype} tensor [{rows}]")
+        ptr.append(t.data_ptr())
+    dev = logits.device
+    token = torch.empty(rows, dtype=torch.int64, device=dev)
+    logprob = torch.empty(rows, dtype=torch.float32, device=dev)
+    kept = torch.empty(rows, dtype=torch.int32, device=dev)
+    if rows:
+        check(load().rldx_sample(logits.data_ptr(), max(ld, vocab), rows, vocab, logits.dtype == torch.float32, *ptr,
+                                 token.data_ptr(), logprob.data_ptr(), kept.data_ptr(), _raw_stream(index)))
+    return token, logprob, kept
