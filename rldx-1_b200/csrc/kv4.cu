@@ -61,12 +61,12 @@ __device__ __forceinline__ uint8_t* kv4_token_unit(const Kv4Cache& c, const int*
   const int b = seq_of_row(cu, c.seqs, row);
   const int pos = lengths[b] - cu[b + 1] + row;
   *tau = pos & (kKv4Unit - 1);
-  const long long off = pos >= 0 ? kv4_unit_offset(c, b, head, pos / kKv4Unit, unit_bytes) : -1;
-  if (off < 0) {
+  const int index = pos >= 0 ? kv4_unit_index(c, b, head, pos / kKv4Unit) : -1;
+  if (index < 0) {
     record_error(kErrKv4Table);
     return nullptr;
   }
-  return c.data + off;
+  return c.data + static_cast<long long>(index) * unit_bytes;
 }
 
 // Copies cu and lengths to shared memory where they fit and returns where to read them.
@@ -295,6 +295,8 @@ int kv4_cache(const rldx_kv4_cache* d, int tokens, const char* what, Kv4Cache* c
     return set_error(RLDX_ERR_ARG, w + ": pages, kv_heads, seqs and table_width must be positive, table_ld >= table_width");
   if (static_cast<long long>(d->table_width) * d->page_size >= (1LL << 31))
     return set_error(RLDX_ERR_UNSUPPORTED, w + ": a sequence holds less than 2^31 tokens");
+  if (d->pages * d->kv_heads * (d->page_size / kKv4Unit) >= (1LL << 31))
+    return set_error(RLDX_ERR_UNSUPPORTED, w + ": a pool has fewer than 2^31 units of 32 tokens of a head");
   if (tokens < 0) return set_error(RLDX_ERR_ARG, w + ": negative token count");
   if (!aligned_to(d->data, 16)) return set_error(RLDX_ERR_ARG, w + ": the cache must be 16-byte aligned");
   c->data = static_cast<uint8_t*>(d->data);

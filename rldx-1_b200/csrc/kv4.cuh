@@ -54,14 +54,14 @@ struct Kv4Cache {
   int seqs, tokens;
 };
 
-// Byte offset of unit `unit` (of sequence b, head h) in the pool, or -1 when the table names no page.
-__device__ __forceinline__ long long kv4_unit_offset(const Kv4Cache& c, int b, int h, int unit, int unit_bytes) {
+// Index of unit `unit` (of sequence b, head h) in the pool, or -1 when the table names no page.  The
+// host checks that a pool has fewer than 2^31 units.
+__device__ __forceinline__ int kv4_unit_index(const Kv4Cache& c, int b, int h, int unit) {
   const int pg = unit / c.units_per_page;
   if (pg < 0 || pg >= c.table_width) return -1;
   const int id = __ldg(c.table + static_cast<long long>(b) * c.table_ld + pg);
   if (id < 0 || id >= c.pages) return -1;
-  return ((static_cast<long long>(id) * c.kv_heads + h) * c.units_per_page + (unit - pg * c.units_per_page)) *
-         unit_bytes;
+  return (id * c.kv_heads + h) * c.units_per_page + (unit - pg * c.units_per_page);
 }
 
 struct Kv4AppendParams {
@@ -96,9 +96,10 @@ struct Kv4AttnParams {
   int window, sinks;
   float scale_log2;
   int max_new, max_len;
-  int chunk_units, chunks;  // units of one split, splits of the longest sequence
-  float* part_o;            // [tokens Hq, chunks, d]
-  float2* part_ml;          // [tokens Hq, chunks] reference maximum (log2 units), sum
+  int whole;        // no segment is cut between CTAs
+  float* part_o;    // [CTAs, 2, columns, d] unfinished results of a CTA's first and last segment
+  float2* part_ml;  // [CTAs, 2, columns] their reference maximum (log2 units) and sum
+  int4* part_head;  // [CTAs] first row, columns, kv head and parts of the segment that a CTA begins
 };
 
 // The units that the rows [row0, row0 + rows) of a sequence (row = new token * group + head of the
@@ -123,6 +124,6 @@ __device__ __forceinline__ Kv4Span kv4_span(int length, int nq, int tok_lo, int 
   return s;
 }
 
-cudaError_t launch_kv4_decode(const Kv4AttnParams& p, int head_dim, int cols_per_cta, cudaStream_t stream);
+cudaError_t launch_kv4_decode(const Kv4AttnParams& p, int head_dim, int cols, int ctas, cudaStream_t stream);
 
 }  // namespace rldx

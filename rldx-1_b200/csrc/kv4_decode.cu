@@ -17,19 +17,34 @@
 // moves when a score passes it by more than 2 (log2 units), so p <= 4 and p scale <= 4 x 8735
 // stays finite for every scale that the append kernel writes.
 //
-// A CTA of 8 warps takes one split of one (sequence, kv head); each warp takes every eighth unit of
-// 32 tokens with its own bulk-copy ring, running maximum, sum and accumulator, so nothing is
-// exchanged until the warps' results meet in shared memory at the end.  Splits meet in a second
-// kernel, in order, so the result does not depend on timing.
+// Work is split evenly over one wave of CTAs, whatever the lengths: a segment is one (sequence, kv
+// head, tile of columns) with the units that it can see, all segments stand in one line and each
+// CTA takes the same share of it, found by a prefix sum over the sequences that every CTA makes
+// for itself.  Inside a CTA each of 8 warps takes every eighth unit with its own bulk-copy ring,
+// running maximum, sum and accumulator, so nothing is exchanged until the warps' results meet in
+// shared memory at a segment's end.  A segment cut between CTAs is joined by a second kernel, in
+// the CTAs' order, so the result does not depend on timing.
+#include <type_traits>
+
 #include "host_util.h"
 #include "kv4.cuh"
 
 namespace rldx {
 
 namespace {
-constexpr int kDecWarps = 8;
+constexpr int kDecWarps = 4;
+constexpr int kDecResident = 16 / kDecWarps;  // CTAs of 8 columns per SM (128 registers a thread)
 constexpr int kDecStages = 2;
 constexpr float kDecGrow = 2.0f;  // lazy move of the reference maximum (log2 units)
+
+constexpr int kDecMaxSeqs = 1024;  // sequences of one launch (their prefix sums stand in shared memory)
+
+// What a CTA works on: units [u0, u0 + m) of the n that columns [c0, c0 + ncols) of kv head kvh of a
+// sequence can see.
+struct DecSegment {
+  int b, q0, kvh, c0, ncols, n, u0, m, line, at;
+  Kv4Span span;
+};
 
 template <int D, int NT>
 struct DecShape {
@@ -39,20 +54,28 @@ struct DecShape {
   static constexpr int kMerge = kDecWarps * kCols * kOLd * 4;
   static constexpr int kBody = kRing > kMerge ? kRing : kMerge;
   static constexpr int kMl = kDecWarps * kCols * 8;  // (reference maximum, sum)
-  static constexpr size_t kSmem = kBody + kMl + 8 * kDecWarps * kDecStages + 16;
+  static constexpr int kQWords = 4 * Kv4Unit<D>::kG + 3;  // a lane's fragments, sums, factors of 8 columns
+  static constexpr int kQ = NT * kQWords * 32 * 4;
+  static constexpr size_t kSmem = kBody + kMl + kQ + 8 * kDecWarps * kDecStages + sizeof(DecSegment) + 4 * (kDecMaxSeqs + 1) + 12;
 };
 
+// d += a b, and d = a b (no accumulator to clear).
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                           uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_1688(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
-  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a0), "r"(a1), "r"(b0));
+__device__ __forceinline__ void mma_16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ __forceinline__ void mma_1688_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(b0), "f"(0.0f));
 }
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   uint32_t y;
@@ -84,10 +107,25 @@ __device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[G]) {
 }
 }  // namespace
 
-// Rows of a CTA's columns: column c of tile `tile` is new token (tile * kCols + c) / group, head
-// (tile * kCols + c) % group of the kv head's group.
+// Units of all segments of sequence b: at least one per segment with a row, so that rows which see
+// no key are written too.  In a launch that cuts no segment (P.whole) a segment counts as one.
+__device__ __forceinline__ int tile_units(const Kv4AttnParams& P, int len, int nq, int c0, int cols) {
+  const int c1 = min(c0 + cols, nq * P.group) - 1;
+  return max(1, kv4_span(len, nq, c0 / P.group, c1 / P.group, P.window, P.sinks).count);
+}
+__device__ __forceinline__ int sequence_units(const Kv4AttnParams& P, int b, int cols) {
+  const int q0 = P.c.cu[b], nq = P.c.cu[b + 1] - q0, len = P.c.lengths[b];
+  if (nq <= 0 || q0 < 0 || nq > P.max_new || len > P.max_len || q0 + nq > P.c.tokens) {
+    if (nq != 0) record_error(kErrKv4Bound);
+    return 0;
+  }
+  int n = 0;
+  for (int c0 = 0; c0 < nq * P.group; c0 += cols) n += P.whole ? 1 : tile_units(P, len, nq, c0, cols);
+  return n * P.c.kv_heads;
+}
+
 template <int D, int NT>
-__global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? 2 : 1)
+__global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? kDecResident : kDecResident / 2)
     kv4_decode_kernel(const __grid_constant__ Kv4AttnParams P) {
   using U = Kv4Unit<D>;
   using Sh = DecShape<D, NT>;
@@ -96,379 +134,512 @@ __global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? 2 : 1)
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* body = smem;
   float2* s_ml = reinterpret_cast<float2*>(smem + Sh::kBody);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Sh::kBody + Sh::kMl);
+  uint32_t* s_q = reinterpret_cast<uint32_t*>(smem + Sh::kBody + Sh::kMl);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Sh::kBody + Sh::kMl + Sh::kQ);
+  DecSegment& sg = *reinterpret_cast<DecSegment*>(bars + kDecWarps * kDecStages);
+  int* s_before = reinterpret_cast<int*>(&sg + 1);  // [seqs + 1] units before a sequence
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  const int tile = blockIdx.y / P.c.kv_heads, kvh = blockIdx.y - tile * P.c.kv_heads;
-  const int b = blockIdx.z, split = blockIdx.x;
 
   if (threadIdx.x < kDecWarps * kDecStages) mbar_init(&bars[threadIdx.x], 1);
   if (threadIdx.x == 0) fence_mbar_init();
   griddep_wait();
   griddep_launch();
-  const int q0 = P.c.cu[b], nq = P.c.cu[b + 1] - q0;
-  const int c0 = tile * kCols, ncols = min(kCols, nq * P.group - c0);
-  if (ncols <= 0) return;  // the whole CTA
-  if (q0 < 0 || q0 + nq > P.c.tokens) {
-    if (threadIdx.x == 0) record_error(kErrKv4Table);
-    return;
+  // ---- prefix sums of the sequences' units ----
+  {
+    int* s_warp = reinterpret_cast<int*>(s_ml);
+    int before = 0;
+    for (int b0 = 0; b0 < P.c.seqs; b0 += 32 * kDecWarps) {
+      const int b = b0 + threadIdx.x;
+      const int n = b < P.c.seqs ? sequence_units(P, b, kCols) : 0;
+      int inc = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += x;
+      }
+      if (lane == 31) s_warp[warp] = inc;
+      __syncthreads();
+      int mine = before + inc - n;
+#pragma unroll
+      for (int w = 0; w < kDecWarps; ++w) {
+        if (w < warp) mine += s_warp[w];
+        before += s_warp[w];
+      }
+      if (b < P.c.seqs) s_before[b] = mine;
+      if (threadIdx.x == 0) s_before[P.c.seqs] = before;  // the last round's is the whole
+      __syncthreads();
+    }
   }
-  const int len = P.c.lengths[b];
-  const Kv4Span span = kv4_span(len, nq, c0 / P.group, (c0 + ncols - 1) / P.group, P.window, P.sinks);
-  if (threadIdx.x == 0 && (nq > P.max_new || len > P.max_len)) record_error(kErrKv4Bound);
-  const int u_begin = split * P.chunk_units, u_end = min(span.count, u_begin + P.chunk_units);
-  if (split > 0 && u_begin >= u_end) return;  // the combine kernel counts the splits the same way
-
-  // ---- this warp's units: lane i holds the place of the i-th (u_begin + warp + 8 i) ----
-  const int mine = max(0, (u_end - u_begin - warp + kDecWarps - 1) / kDecWarps);  // <= 32
-  long long my_off = -1;
-  if (lane < mine) {
-    my_off = kv4_unit_offset(P.c, b, kvh, span.unit(u_begin + warp + kDecWarps * lane), U::kBytes);
-    if (my_off < 0) record_error(kErrKv4Table);
-  }
+  const int total = s_before[P.c.seqs];
+  const int quota = max(P.whole ? 1 : kDecWarps, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
+  const int cta = blockIdx.x;
+  const int begin = min(total, cta * quota), end = min(total, begin + quota);
+  const uint64_t policy = l2_policy_evict_first();
   uint8_t* ring = body + warp * kDecStages * U::kBytes;
   uint64_t* bar = bars + warp * kDecStages;
-  __syncthreads();
-  const uint64_t policy = l2_policy_evict_first();
-  auto fetch = [&](int i) {  // every lane calls it; a unit without a page is not fetched
-    const long long off = __shfl_sync(0xffffffffu, my_off, i);
-    if (lane == 0) {
-      uint64_t* bb = &bar[i % kDecStages];
-      if (off >= 0) {
-        mbar_arrive_expect_tx(bb, U::kBytes);
-        bulk_load(ring + (i % kDecStages) * U::kBytes, P.c.data + off, U::kBytes, bb, policy);
-      } else {
-        mbar_arrive(bb);
-      }
-    }
-  };
-  for (int i = 0; i < kDecStages && i < mine; ++i) fetch(i);
-
-  // ---- q: B fragments of column 8 nt + g, channels 32 j + 8 t + 0..7 ----
-  uint32_t qf[NT][G][4], qsum[NT];
-  float colfac[NT][2];  // log2 score per unit of the products, for columns 2t, 2t + 1
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int col = 8 * nt + g;
-    const int row = c0 + col, tok = row / P.group;
-    float v[G][8], mx = 0.0f;
-#pragma unroll
-    for (int j = 0; j < G; ++j) {
-      uint4 u = make_uint4(0u, 0u, 0u, 0u);
-      if (col < ncols)
-        u = *reinterpret_cast<const uint4*>(P.q + (q0 + tok) * P.ldq +
-                                            static_cast<long long>(kvh * P.group + row - tok * P.group) * D + 32 * j + 8 * t);
-      unpack_bf16x2(u.x, v[j][0], v[j][1]);
-      unpack_bf16x2(u.y, v[j][2], v[j][3]);
-      unpack_bf16x2(u.z, v[j][4], v[j][5]);
-      unpack_bf16x2(u.w, v[j][6], v[j][7]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(v[j][e]));
-    }
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    // 2^e with e = 8 - exponent(mx), kept a normal number; a row of zeros keeps 1
-    const int ex = static_cast<int>(__float_as_uint(mx) >> 23);
-    const int e2 = mx > 0.0f ? min(max(262 - ex, 1), 253) : 127;
-    const float up = __uint_as_float(static_cast<uint32_t>(e2) << 23);
-    const float down = __uint_as_float(static_cast<uint32_t>(254 - e2) << 23);
-    float part[G];
-#pragma unroll
-    for (int j = 0; j < G; ++j) {
-      part[j] = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v[j][e] *= up;
-        part[j] += v[j][e];
-      }
-      part[j] += __shfl_xor_sync(0xffffffffu, part[j], 1);
-      part[j] += __shfl_xor_sync(0xffffffffu, part[j], 2);
-      // nibbles 0, 4 | 1, 5 (sixteen times their code) | 2, 6 | 3, 7
-      qf[nt][j][0] = h2_bits(__floats2half2_rn(v[j][0], v[j][4]));
-      qf[nt][j][1] = h2_bits(__floats2half2_rn(v[j][1] * 0.0625f, v[j][5] * 0.0625f));
-      qf[nt][j][2] = h2_bits(__floats2half2_rn(v[j][2], v[j][6]));
-      qf[nt][j][3] = h2_bits(__floats2half2_rn(v[j][3] * 0.0625f, v[j][7] * 0.0625f));
-    }
-    // sums of q for the lows: lanes t = 0, 1 hold the fp16 high halves of groups 0, 1 | 2, 3, lanes
-    // t = 2, 3 what those leave
-    float sa = part[0], sb = part[1];
-    if constexpr (G == 4) {
-      if (t & 1) sa = part[2], sb = part[3];
-    } else {
-      if (t & 1) sa = sb = 0.0f;
-    }
-    const __half2 hi = __floats2half2_rn(sa, sb);
-    const float2 hf = __half22float2(hi);
-    qsum[nt] = h2_bits(t < 2 ? hi : __floats2half2_rn(sa - hf.x, sb - hf.y));
-    const float cf = P.scale_log2 * down;
-    colfac[nt][0] = __shfl_sync(0xffffffffu, cf, 8 * t);
-    colfac[nt][1] = __shfl_sync(0xffffffffu, cf, 8 * t + 4);
-  }
-  int pos[NT][2];  // position of columns 2t, 2t + 1 of each tile
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) pos[nt][i] = span.pos_lo + min(c0 + 8 * nt + 2 * t + i, c0 + ncols - 1) / P.group - c0 / P.group;
-
-  float acc[NT][G][2][4], low[NT][4];  // O of channels 32 j + 4 g + 2 s (and + 1), low sums and row sum
-  float m_ref[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-    for (int j = 0; j < G; ++j)
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[nt][j][s][i] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) low[nt][i] = 0.0f;
-    m_ref[nt][0] = m_ref[nt][1] = -INFINITY;
-  }
-
+  bool began = false;  // thread 0: a segment begins here and goes on
+  int turn = 0;  // units this warp has fetched into its ring and consumed, over all segments
   bool ok = true;
-  for (int i = 0; i < mine; ++i) {
-    const int st = i % kDecStages;
-    ok = mbar_wait(&bar[st], static_cast<uint32_t>(i / kDecStages) & 1u, kErrKv4Timeout);
-    ok = __all_sync(0xffffffffu, ok);
-    if (!ok) break;
-    const uint8_t* un = ring + st * U::kBytes;
-    const bool have = __shfl_sync(0xffffffffu, my_off, i) >= 0;
-    const int key0 = kKv4Unit * span.unit(u_begin + warp + kDecWarps * i);
-    const int key_hi = key0 + kKv4Unit - 1;
-    const bool plain = have && key_hi <= span.pos_lo &&
-                       (P.window <= 0 || span.pos_hi - key0 < P.window || key_hi < P.sinks);
 
-    // ---- scores of 32 tokens (two tiles of 16) ----
-    float sc[2][NT][4];
-#pragma unroll
-    for (int blk = 0; blk < 2; ++blk) {
-      uint32_t ka[G], kb[G], ma[G], mb[G];
-      lds_words<G>(un + blk * 16 * U::kRow + lane * 4 * G, ka);
-      lds_words<G>(un + blk * 16 * U::kRow + 8 * U::kRow + lane * 4 * G, kb);
-      lds_words<G>(un + U::kKMeta + (blk * 16 + g) * 4 * G, ma);
-      lds_words<G>(un + U::kKMeta + (blk * 16 + 8 + g) * 4 * G, mb);
-      float sa[G], sb[G];
-#pragma unroll
-      for (int j = 0; j < G; j += 2) {
-        const float2 a = h2_floats(ma[j / 2]), c = h2_floats(mb[j / 2]);
-        sa[j] = a.x, sa[j + 1] = a.y, sb[j] = c.x, sb[j + 1] = c.y;
+  for (int at = begin; at < end;) {
+    // ---- the segment that unit `at` of the line belongs to ----
+    if (warp == 0) {
+      int lo = 0, hi = P.c.seqs;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s_before[mid] <= at) lo = mid; else hi = mid;
       }
-      uint32_t la = ma[G / 2], lb = mb[G / 2];
-      if constexpr (G == 4) {
-        if (t & 1) la = ma[3], lb = mb[3];
-      } else {
-        if (t & 1) la = lb = 0u;
+      const int b = lo;  // the last sequence that begins at or before `at`: it has units
+      const int q0 = P.c.cu[b], nq = P.c.cu[b + 1] - q0, len = P.c.lengths[b];
+      int rest = at - s_before[b], c0 = 0, n = 0, line = 0;
+      for (;; c0 += kCols) {  // tiles of columns, each with all kv heads
+        n = tile_units(P, len, nq, c0, kCols);
+        line = P.whole ? 1 : n;
+        if (rest < line * P.c.kv_heads) break;
+        rest -= line * P.c.kv_heads;
       }
-      float sm[NT][4], sum[NT][4];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sm[nt][e] = sum[nt][e] = 0.0f;
-        mma_1688(sm[nt], la, lb, qsum[nt]);
+      const int kvh = rest / line, u0 = P.whole ? 0 : rest - kvh * line;
+      const int m = P.whole ? n : min(n - u0, end - at);
+      if (lane == 0) {
+        sg.b = b, sg.q0 = q0, sg.kvh = kvh, sg.c0 = c0, sg.ncols = min(kCols, nq * P.group - c0);
+        sg.n = n, sg.u0 = u0, sg.m = m, sg.line = at - u0, sg.at = at + (P.whole ? 1 : m);
+        sg.span = kv4_span(len, nq, c0 / P.group, (c0 + sg.ncols - 1) / P.group, P.window, P.sinks);
       }
-#pragma unroll
-      for (int j = 0; j < G; ++j) {
-        const uint32_t wa = ka[j], wb = kb[j], va = wa >> 8, vb = wb >> 8;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          mma_16816(d, wa & 0x000f000fu, wb & 0x000f000fu, wa & 0x00f000f0u, wb & 0x00f000f0u, qf[nt][j][0], qf[nt][j][1]);
-          mma_16816(d, va & 0x000f000fu, vb & 0x000f000fu, va & 0x00f000f0u, vb & 0x00f000f0u, qf[nt][j][2], qf[nt][j][3]);
-          sum[nt][0] = fmaf(sa[j], d[0], sum[nt][0]);
-          sum[nt][1] = fmaf(sa[j], d[1], sum[nt][1]);
-          sum[nt][2] = fmaf(sb[j], d[2], sum[nt][2]);
-          sum[nt][3] = fmaf(sb[j], d[3], sum[nt][3]);
+    }
+    __syncthreads();
+    const int b = sg.b, q0 = sg.q0, kvh = sg.kvh, c0 = sg.c0, ncols = sg.ncols, n = sg.n, u0 = sg.u0, m = sg.m;
+    const Kv4Span span = sg.span;
+    at = sg.at;
+
+    // lane i holds the i-th of this warp's next 32 units: its index in the pool, and in a ballot
+    // whether every column sees every token of it
+    const int mine = (m - warp + kDecWarps - 1) / kDecWarps;
+    int index = -1;
+    unsigned clear = 0u;
+    auto look = [&](int round) {
+      const int i = 32 * round + lane;
+      index = -1;
+      bool all = false;
+      if (i < mine) {
+        const int u = span.unit(u0 + warp + kDecWarps * i), key0 = kKv4Unit * u, key1 = key0 + kKv4Unit - 1;
+        if (span.count > 0) {
+          index = kv4_unit_index(P.c, b, kvh, u);
+          if (index < 0) record_error(kErrKv4Table);
+        }
+        all = index >= 0 && key1 <= span.pos_lo && (P.window <= 0 || span.pos_hi - key0 < P.window || key1 < P.sinks);
+      }
+      clear = __ballot_sync(0xffffffffu, all);
+    };
+    auto fetch = [&](int i, int slot) {  // every lane calls it; a unit without a page is not fetched
+      const int x = __shfl_sync(0xffffffffu, index, i & 31);
+      if (lane == 0) {
+        if (x >= 0) {
+          mbar_arrive_expect_tx(&bar[slot], U::kBytes);
+          bulk_load(ring + slot * U::kBytes, P.c.data + static_cast<long long>(x) * U::kBytes, U::kBytes, &bar[slot], policy);
+        } else {
+          mbar_arrive(&bar[slot]);
         }
       }
+    };
+    look(0);
+    for (int i = 0; i < kDecStages && i < mine; ++i) fetch(i, (turn + i) % kDecStages);
+
+    // ---- q: B fragments of column 8 nt + g, channels 32 j + 8 t + 0..7, made by warp nt ----
+    if (warp < NT) {
+      const int nt = warp, col = 8 * nt + g;
+      const int row = c0 + col, tok = row / P.group;
+      uint32_t* dst = s_q + nt * Sh::kQWords * 32 + lane;
+      float v[G][8], mx = 0.0f;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int j = 0; j < G; ++j) {
+        uint4 u = make_uint4(0u, 0u, 0u, 0u);
+        if (col < ncols)
+          u = *reinterpret_cast<const uint4*>(P.q + (q0 + tok) * P.ldq +
+                                              static_cast<long long>(kvh * P.group + row - tok * P.group) * D + 32 * j + 8 * t);
+        unpack_bf16x2(u.x, v[j][0], v[j][1]);
+        unpack_bf16x2(u.y, v[j][2], v[j][3]);
+        unpack_bf16x2(u.z, v[j][4], v[j][5]);
+        unpack_bf16x2(u.w, v[j][6], v[j][7]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[blk][nt][e] = fmaf(16777216.0f, sum[nt][e], sm[nt][e]) * colfac[nt][e & 1];
+        for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(v[j][e]));
+      }
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      // 2^e with e = 8 - exponent(mx), kept a normal number; a row of zeros keeps 1
+      const int ex = static_cast<int>(__float_as_uint(mx) >> 23);
+      const int e2 = mx > 0.0f ? min(max(262 - ex, 1), 253) : 127;
+      const float up = __uint_as_float(static_cast<uint32_t>(e2) << 23);
+      const float down = __uint_as_float(static_cast<uint32_t>(254 - e2) << 23);
+      float part[G];
+#pragma unroll
+      for (int j = 0; j < G; ++j) {
+        part[j] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          v[j][e] *= up;
+          part[j] += v[j][e];
+        }
+        part[j] += __shfl_xor_sync(0xffffffffu, part[j], 1);
+        part[j] += __shfl_xor_sync(0xffffffffu, part[j], 2);
+        // nibbles 0, 4 | 1, 5 (sixteen times their code) | 2, 6 | 3, 7
+        dst[(4 * j + 0) * 32] = h2_bits(__floats2half2_rn(v[j][0], v[j][4]));
+        dst[(4 * j + 1) * 32] = h2_bits(__floats2half2_rn(v[j][1] * 0.0625f, v[j][5] * 0.0625f));
+        dst[(4 * j + 2) * 32] = h2_bits(__floats2half2_rn(v[j][2], v[j][6]));
+        dst[(4 * j + 3) * 32] = h2_bits(__floats2half2_rn(v[j][3] * 0.0625f, v[j][7] * 0.0625f));
+      }
+      // sums of q for the lows: lanes t = 0, 1 hold the fp16 high halves of groups 0, 1 | 2, 3, lanes
+      // t = 2, 3 what those leave
+      float sa = part[0], sb = part[1];
+      if constexpr (G == 4) {
+        if (t & 1) sa = part[2], sb = part[3];
+      } else {
+        if (t & 1) sa = sb = 0.0f;
+      }
+      const __half2 hi2 = __floats2half2_rn(sa, sb);
+      const float2 hf = __half22float2(hi2);
+      dst[4 * G * 32] = h2_bits(t < 2 ? hi2 : __floats2half2_rn(sa - hf.x, sb - hf.y));
+      const float cf = P.scale_log2 * down;  // log2 score per unit of the products, of columns 2t, 2t + 1
+      dst[(4 * G + 1) * 32] = __float_as_uint(__shfl_sync(0xffffffffu, cf, 8 * t));
+      dst[(4 * G + 2) * 32] = __float_as_uint(__shfl_sync(0xffffffffu, cf, 8 * t + 4));
     }
-    if (!plain) {
+    __syncthreads();
+    uint32_t qf[NT][G][4], qsum[NT];
+    float colfac[NT][2];
 #pragma unroll
-      for (int blk = 0; blk < 2; ++blk)
+    for (int nt = 0; nt < NT; ++nt) {
+      const uint32_t* src = s_q + nt * Sh::kQWords * 32 + lane;
+#pragma unroll
+      for (int j = 0; j < G; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) qf[nt][j][i] = src[(4 * j + i) * 32];
+      qsum[nt] = src[4 * G * 32];
+      colfac[nt][0] = __uint_as_float(src[(4 * G + 1) * 32]);
+      colfac[nt][1] = __uint_as_float(src[(4 * G + 2) * 32]);
+    }
+
+    float acc[NT][G][2][4], low[NT][4];  // O of channels 32 j + 4 g + 2 s (and + 1), low sums and row sum
+    float m_ref[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int j = 0; j < G; ++j)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[nt][j][s][i] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) low[nt][i] = 0.0f;
+      m_ref[nt][0] = m_ref[nt][1] = -INFINITY;
+    }
+
+    // One unit; kPlain: every column sees every token of it.  The two forms are separate code, so that
+    // the plain one carries no masking.
+    auto attend = [&](const uint8_t* un, int i, auto flag) {
+      constexpr bool kPlain = decltype(flag)::value;
+      // ---- products of 32 tokens (two tiles of 16), before the column's factor ----
+      float sc[2][NT][4];
+#pragma unroll
+      for (int blk = 0; blk < 2; ++blk) {
+        uint32_t ka[G], kb[G], ma[G], mb[G];
+        lds_words<G>(un + blk * 16 * U::kRow + lane * 4 * G, ka);
+        lds_words<G>(un + blk * 16 * U::kRow + 8 * U::kRow + lane * 4 * G, kb);
+        lds_words<G>(un + U::kKMeta + (blk * 16 + g) * 4 * G, ma);
+        lds_words<G>(un + U::kKMeta + (blk * 16 + 8 + g) * 4 * G, mb);
+        float sa[G], sb[G];
+#pragma unroll
+        for (int j = 0; j < G; j += 2) {
+          const float2 a = h2_floats(ma[j / 2]), c = h2_floats(mb[j / 2]);
+          sa[j] = a.x, sa[j + 1] = a.y, sb[j] = c.x, sb[j + 1] = c.y;
+        }
+        uint32_t la = ma[G / 2], lb = mb[G / 2];
+        if constexpr (G == 4) {
+          if (t & 1) la = ma[3], lb = mb[3];
+        } else {
+          if (t & 1) la = lb = 0u;
+        }
+        float sum[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int key = key0 + 16 * blk + 8 * (e >> 1) + g, ps = pos[nt][e & 1];
-            const bool seen = have && key <= ps && (P.window <= 0 || ps - key < P.window || key < P.sinks);
-            sc[blk][nt][e] = seen ? sc[blk][nt][e] : -INFINITY;
+          for (int e = 0; e < 4; ++e) sum[nt][e] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+          const uint32_t wa = ka[j], wb = kb[j], va = wa >> 8, vb = wb >> 8;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float d[4];
+            mma_16816_first(d, wa & 0x000f000fu, wb & 0x000f000fu, wa & 0x00f000f0u, wb & 0x00f000f0u, qf[nt][j][0], qf[nt][j][1]);
+            mma_16816(d, va & 0x000f000fu, vb & 0x000f000fu, va & 0x00f000f0u, vb & 0x00f000f0u, qf[nt][j][2], qf[nt][j][3]);
+            sum[nt][0] = fmaf(sa[j], d[0], sum[nt][0]);
+            sum[nt][1] = fmaf(sa[j], d[1], sum[nt][1]);
+            sum[nt][2] = fmaf(sb[j], d[2], sum[nt][2]);
+            sum[nt][3] = fmaf(sb[j], d[3], sum[nt][3]);
           }
-    }
-    // ---- running maximum ----
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float mx[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) mx[e] = fmaxf(fmaxf(sc[0][nt][e], sc[0][nt][e + 2]), fmaxf(sc[1][nt][e], sc[1][nt][e + 2]));
-      if (__any_sync(0xffffffffu, mx[0] > m_ref[nt][0] + kDecGrow || mx[1] > m_ref[nt][1] + kDecGrow)) {
-        float al[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-#pragma unroll
-          for (int o = 4; o <= 16; o <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], o));
-          const float m = fmaxf(m_ref[nt][e], mx[e]);
-          al[e] = m_ref[nt][e] == -INFINITY ? 0.0f : ex2_approx(m_ref[nt][e] - m);
-          m_ref[nt][e] = m;
         }
-#pragma unroll
-        for (int j = 0; j < G; ++j)
-#pragma unroll
-          for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[nt][j][s][e] *= al[e & 1];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) low[nt][e] *= al[e & 1];
-      }
-    }
-    // ---- O += P V ----
-#pragma unroll
-    for (int blk = 0; blk < 2; ++blk) {
-      uint32_t pb[NT][2];  // B fragments of p: tokens 2t, 2t + 1 of each half, column g
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const float m0 = m_ref[nt][0] == -INFINITY ? 0.0f : m_ref[nt][0];
-        const float m1 = m_ref[nt][1] == -INFINITY ? 0.0f : m_ref[nt][1];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          pb[nt][h] = transpose_8x8(h2_bits(
-              __floats2half2_rn(ex2_approx(sc[blk][nt][2 * h] - m0), ex2_approx(sc[blk][nt][2 * h + 1] - m1))));
-      }
-      uint32_t v0[G], v1[G], s0[G], s1[G];
-      lds_words<G>(un + U::kV + blk * 8 * D + lane * 4 * G, v0);
-      lds_words<G>(un + U::kV + blk * 8 * D + 4 * D + lane * 4 * G, v1);
-      lds_words<G>(un + U::kVScale + blk * 32 * G + t * 4 * G, s0);
-      lds_words<G>(un + U::kVScale + blk * 32 * G + 16 * G + t * 4 * G, s1);
-      uint32_t l0 = g == 4 ? 0x3c003c00u : 0u, l1 = l0;  // rows 0..G-1: lows of a group; row 4: ones
-      if (g < G) {
-        l0 = *reinterpret_cast<const uint32_t*>(un + U::kVLow + blk * 32 * G + t * 4 * G + 4 * g);
-        l1 = *reinterpret_cast<const uint32_t*>(un + U::kVLow + blk * 32 * G + 16 * G + t * 4 * G + 4 * g);
-        if (!plain) {  // a NaN low comes with a NaN scale, which reaches the columns that see the token
-          l0 &= __hlt2_mask(__habs2(bits_h2(l0)), bits_h2(0x7c007c00u));
-          l1 &= __hlt2_mask(__habs2(bits_h2(l1)), bits_h2(0x7c007c00u));
-        }
-      }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) mma_16816(low[nt], l0, 0u, l1, 0u, pb[nt][0], pb[nt][1]);
-#pragma unroll
-      for (int j = 0; j < G; ++j) {
-        // half-words of group j of tokens 2t | 2t + 1
-        const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
-        const uint32_t x0 = __byte_perm(v0[j / 2], v0[G / 2 + j / 2], sel), x1 = __byte_perm(v1[j / 2], v1[G / 2 + j / 2], sel);
-        const uint32_t y0 = x0 >> 8, y1 = x1 >> 8;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          uint32_t b0 = h2_bits(__hmul2(bits_h2(pb[nt][0]), bits_h2(s0[j])));
-          uint32_t b1 = h2_bits(__hmul2(bits_h2(pb[nt][1]), bits_h2(s1[j])));
-          if (!plain) {  // p = 0 stays 0 beside whatever stands in a hidden token's scale
-            b0 &= __hneu2_mask(bits_h2(pb[nt][0]), bits_h2(0u));
-            b1 &= __hneu2_mask(bits_h2(pb[nt][1]), bits_h2(0u));
+          float sm[4];
+          mma_1688_first(sm, la, lb, qsum[nt]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[blk][nt][e] = fmaf(16777216.0f, sum[nt][e], sm[e]);
+        }
+      }
+      if constexpr (!kPlain) {
+        const int key0 = kKv4Unit * span.unit(u0 + warp + kDecWarps * i);
+        const bool have = __shfl_sync(0xffffffffu, index, i & 31) >= 0;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            // position of column 2t + e (columns past the rows repeat the last one)
+            const int ps = span.pos_lo + min(c0 + 8 * nt + 2 * t + e, c0 + ncols - 1) / P.group - c0 / P.group;
+#pragma unroll
+            for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int key = key0 + 16 * blk + 8 * h + g;
+                const bool seen = have && key <= ps && (P.window <= 0 || ps - key < P.window || key < P.sinks);
+                if (!seen) sc[blk][nt][2 * h + e] = -INFINITY;
+              }
           }
-          mma_16816(acc[nt][j][0], x0 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x000f000fu, x1 & 0x00f000f0u, b0, b1);
-          mma_16816(acc[nt][j][1], y0 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x000f000fu, y1 & 0x00f000f0u, b0, b1);
+      }
+      // ---- running maximum ----
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float mx[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          mx[e] = fmaxf(fmaxf(sc[0][nt][e], sc[0][nt][e + 2]), fmaxf(sc[1][nt][e], sc[1][nt][e + 2])) * colfac[nt][e];
+        if (__any_sync(0xffffffffu, mx[0] > m_ref[nt][0] + kDecGrow || mx[1] > m_ref[nt][1] + kDecGrow)) {
+          float al[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int o = 4; o <= 16; o <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], o));
+            const float mm = mx[e] > m_ref[nt][e] ? mx[e] + kDecGrow : m_ref[nt][e];
+            al[e] = m_ref[nt][e] == -INFINITY ? 0.0f : ex2_approx(m_ref[nt][e] - mm);
+            m_ref[nt][e] = mm;
+          }
+#pragma unroll
+          for (int j = 0; j < G; ++j)
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[nt][j][s][e] *= al[e & 1];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) low[nt][e] *= al[e & 1];
+        }
+      }
+      // ---- O += P V ----
+      float neg[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) neg[nt][e] = m_ref[nt][e] == -INFINITY ? 0.0f : -m_ref[nt][e];
+#pragma unroll
+      for (int blk = 0; blk < 2; ++blk) {
+        uint32_t pb[NT][2];  // B fragments of p: tokens 2t, 2t + 1 of each half, column g
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            pb[nt][h] = transpose_8x8(h2_bits(__floats2half2_rn(ex2_approx(fmaf(sc[blk][nt][2 * h], colfac[nt][0], neg[nt][0])),
+                                                                ex2_approx(fmaf(sc[blk][nt][2 * h + 1], colfac[nt][1], neg[nt][1])))));
+        uint32_t v0[G], v1[G], s0[G], s1[G];
+        lds_words<G>(un + U::kV + blk * 8 * D + lane * 4 * G, v0);
+        lds_words<G>(un + U::kV + blk * 8 * D + 4 * D + lane * 4 * G, v1);
+        lds_words<G>(un + U::kVScale + blk * 32 * G + t * 4 * G, s0);
+        lds_words<G>(un + U::kVScale + blk * 32 * G + 16 * G + t * 4 * G, s1);
+        uint32_t l0 = g == 4 ? 0x3c003c00u : 0u, l1 = l0;  // rows 0..G-1: lows of a group; row 4: ones
+        if (g < G) {
+          l0 = *reinterpret_cast<const uint32_t*>(un + U::kVLow + blk * 32 * G + t * 4 * G + 4 * g);
+          l1 = *reinterpret_cast<const uint32_t*>(un + U::kVLow + blk * 32 * G + 16 * G + t * 4 * G + 4 * g);
+          if constexpr (!kPlain) {  // a NaN low comes with a NaN scale, which reaches the columns that see the token
+            l0 &= __hlt2_mask(__habs2(bits_h2(l0)), bits_h2(0x7c007c00u));
+            l1 &= __hlt2_mask(__habs2(bits_h2(l1)), bits_h2(0x7c007c00u));
+          }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma_16816(low[nt], l0, 0u, l1, 0u, pb[nt][0], pb[nt][1]);
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+          // half-words of group j of tokens 2t | 2t + 1
+          const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
+          const uint32_t x0 = __byte_perm(v0[j / 2], v0[G / 2 + j / 2], sel), x1 = __byte_perm(v1[j / 2], v1[G / 2 + j / 2], sel);
+          const uint32_t y0 = x0 >> 8, y1 = x1 >> 8;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            uint32_t b0 = h2_bits(__hmul2(bits_h2(pb[nt][0]), bits_h2(s0[j])));
+            uint32_t b1 = h2_bits(__hmul2(bits_h2(pb[nt][1]), bits_h2(s1[j])));
+            if constexpr (!kPlain) {  // p = 0 stays 0 beside whatever stands in a hidden token's scale
+              b0 &= __hneu2_mask(bits_h2(pb[nt][0]), bits_h2(0u));
+              b1 &= __hneu2_mask(bits_h2(pb[nt][1]), bits_h2(0u));
+            }
+            mma_16816(acc[nt][j][0], x0 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x000f000fu, x1 & 0x00f000f0u, b0, b1);
+            mma_16816(acc[nt][j][1], y0 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x000f000fu, y1 & 0x00f000f0u, b0, b1);
+          }
+        }
+      }
+    };
+    for (int i = 0; i < mine; ++i, ++turn) {
+      const int st = turn % kDecStages;
+      ok = mbar_wait(&bar[st], static_cast<uint32_t>(turn / kDecStages) & 1u, kErrKv4Timeout);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if ((clear >> (i & 31)) & 1u)
+        attend(ring + st * U::kBytes, i, std::true_type{});
+      else
+        attend(ring + st * U::kBytes, i, std::false_type{});
+      __syncwarp();  // every lane has read the unit
+      if ((i & 31) == 31) {  // the next 32 places; those of the ring's units ahead are in the same round
+        look((i + 1) >> 5);
+        for (int k = 1; k <= kDecStages && i + k < mine; ++k) fetch(i + k, (turn + k) % kDecStages);
+      } else if (i + kDecStages < mine && ((i + kDecStages) >> 5) == (i >> 5)) {
+        fetch(i + kDecStages, st);
+      }
+    }
+    if (!ok) settle_issued_copies();
+
+    // ---- the warps' results meet in shared memory ----
+    __syncthreads();  // every ring is idle
+    float* so = reinterpret_cast<float*>(body);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int col = 8 * nt + 2 * t + e;
+        const float l = __shfl_sync(0xffffffffu, low[nt][e], 16 + t);
+        if (g == 0) s_ml[warp * kCols + col] = make_float2(m_ref[nt][e], l);
+        float* dst = so + (warp * kCols + col) * Sh::kOLd + 4 * g;
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+          const float lw = __shfl_sync(0xffffffffu, low[nt][e], 4 * j + t);
+          float4 o;
+          o.x = fmaf(16777216.0f, acc[nt][j][0][e], lw);
+          o.y = fmaf(1048576.0f, acc[nt][j][0][e + 2], lw);
+          o.z = fmaf(16777216.0f, acc[nt][j][1][e], lw);
+          o.w = fmaf(1048576.0f, acc[nt][j][1][e + 2], lw);
+          *reinterpret_cast<float4*>(dst + 32 * j) = o;
         }
       }
     }
-    __syncwarp();  // every lane has read the unit
-    if (i + kDecStages < mine) fetch(i + kDecStages);
-  }
-  if (!ok) settle_issued_copies();
-
-  // ---- the warps' results meet in shared memory ----
-  __syncthreads();  // every ring is idle
-  float* so = reinterpret_cast<float*>(body);
+    __syncthreads();
+    const bool whole = m == n;
+    if (!whole && u0 == 0 && threadIdx.x == 0) {  // for the join: what begins here, and how many CTAs have a part
+      const int last = (sg.line + n - 1) / quota;
+      P.part_head[cta] = make_int4(q0, c0 | (ncols << 24), kvh, last - cta + 1);
+      began = true;
+    }
+    const long long slot = 2LL * cta + (u0 == 0 ? 1 : 0);  // 0: began in an earlier CTA; 1: goes on in the next
+    for (int i = threadIdx.x; i < ncols * (D / 4); i += 32 * kDecWarps) {
+      const int col = i / (D / 4), ch = i % (D / 4) * 4;
+      float mm = -INFINITY;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
+      for (int w = 0; w < kDecWarps; ++w) mm = fmaxf(mm, s_ml[w * kCols + col].x);
+      const float m_use = mm == -INFINITY ? 0.0f : mm;
+      float l = 0.0f;
+      float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int col = 8 * nt + 2 * t + e;
-      const float l = __shfl_sync(0xffffffffu, low[nt][e], 16 + t);
-      if (g == 0) s_ml[warp * kCols + col] = make_float2(m_ref[nt][e], l);
-      float* dst = so + (warp * kCols + col) * Sh::kOLd + 4 * g;
-#pragma unroll
-      for (int j = 0; j < G; ++j) {
-        const float lw = __shfl_sync(0xffffffffu, low[nt][e], 4 * j + t);
-        float4 o;
-        o.x = fmaf(16777216.0f, acc[nt][j][0][e], lw);
-        o.y = fmaf(1048576.0f, acc[nt][j][0][e + 2], lw);
-        o.z = fmaf(16777216.0f, acc[nt][j][1][e], lw);
-        o.w = fmaf(1048576.0f, acc[nt][j][1][e + 2], lw);
-        *reinterpret_cast<float4*>(dst + 32 * j) = o;
+      for (int w = 0; w < kDecWarps; ++w) {
+        const float2 ml = s_ml[w * kCols + col];
+        if (ml.x == -INFINITY && ml.y == 0.0f) continue;  // saw no visible token
+        const float f = ex2_approx(ml.x - m_use);
+        const float4 x = *reinterpret_cast<const float4*>(so + (w * kCols + col) * Sh::kOLd + ch);
+        l = fmaf(f, ml.y, l);
+        o.x = fmaf(f, x.x, o.x), o.y = fmaf(f, x.y, o.y), o.z = fmaf(f, x.z, o.z), o.w = fmaf(f, x.w, o.w);
+      }
+      if (whole) {
+        const int row = c0 + col, tok = row / P.group;
+        const long long orow = static_cast<long long>(q0 + tok) * P.q_heads + kvh * P.group + row - tok * P.group;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no visible token: zeros
+        uint2 u;
+        u.x = pack_bf16x2(o.x * inv, o.y * inv);
+        u.y = pack_bf16x2(o.z * inv, o.w * inv);
+        *reinterpret_cast<uint2*>(P.out + orow * D + ch) = u;
+      } else {
+        *reinterpret_cast<float4*>(P.part_o + (slot * kCols + col) * D + ch) = o;
+        if (ch == 0) P.part_ml[slot * kCols + col] = make_float2(mm, l);
       }
     }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < ncols * (D / 4); i += 32 * kDecWarps) {
-    const int col = i / (D / 4), ch = i % (D / 4) * 4;
-    float m = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kDecWarps; ++w) m = fmaxf(m, s_ml[w * kCols + col].x);
-    const float m_use = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-    for (int w = 0; w < kDecWarps; ++w) {
-      const float2 ml = s_ml[w * kCols + col];
-      if (ml.x == -INFINITY && ml.y == 0.0f) continue;  // saw no visible token
-      const float f = ex2_approx(ml.x - m_use);
-      const float4 x = *reinterpret_cast<const float4*>(so + (w * kCols + col) * Sh::kOLd + ch);
-      l = fmaf(f, ml.y, l);
-      o.x = fmaf(f, x.x, o.x), o.y = fmaf(f, x.y, o.y), o.z = fmaf(f, x.z, o.z), o.w = fmaf(f, x.w, o.w);
-    }
-    const int row = c0 + col, tok = row / P.group;
-    const long long orow = static_cast<long long>(q0 + tok) * P.q_heads + kvh * P.group + row - tok * P.group;
-    if (P.chunks == 1) {
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no visible token: zeros
-      uint2 u;
-      u.x = pack_bf16x2(o.x * inv, o.y * inv);
-      u.y = pack_bf16x2(o.z * inv, o.w * inv);
-      *reinterpret_cast<uint2*>(P.out + orow * D + ch) = u;
-    } else {
-      *reinterpret_cast<float4*>(P.part_o + (orow * P.chunks + split) * D + ch) = o;
-      if (ch == 0) P.part_ml[orow * P.chunks + split] = make_float2(m, l);
+    if (at < end) {
+      fence_proxy_async_smem();  // the rings are written by bulk copies again
+      __syncthreads();
     }
   }
+  if (threadIdx.x == 0 && !P.whole && !began) P.part_head[cta] = make_int4(0, 0, 0, 0);
 }
 
-// out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s over a row's splits; D / 4 lanes per row.
+// Joins the segments that were cut between CTAs: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s
+// over the parts.  CTA (i, y) takes the segment that begins in CTA i and goes on: a column per warp
+// (kCols warps), or with gridDim.y > 1 column y, of which each of 8 warps takes every eighth part.
 template <int D>
-__global__ void __launch_bounds__(128) kv4_combine_kernel(const __grid_constant__ Kv4AttnParams P, int cols_per_cta) {
-  constexpr int kLanes = D / 4;
+__global__ void __launch_bounds__(512) kv4_combine_kernel(const __grid_constant__ Kv4AttnParams P, int cols) {
+  constexpr int kVec = D / 32;  // channels of a lane
+  __shared__ float s_o[8][D], s_l[8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   griddep_wait();
   griddep_launch();
-  const int b = blockIdx.y;
-  const int q0 = P.c.cu[b], nq = P.c.cu[b + 1] - q0;
-  if (q0 < 0 || q0 + nq > P.c.tokens) return;
-  const int r = (blockIdx.x * blockDim.x + threadIdx.x) / kLanes, ch = threadIdx.x % kLanes * 4;
-  if (r >= nq * P.q_heads) return;
-  const int tok = r / P.q_heads, head = r - tok * P.q_heads;
-  const int col = tok * P.group + head % P.group;  // column of its kv head
-  const int c0 = col / cols_per_cta * cols_per_cta, c1 = min(c0 + cols_per_cta, nq * P.group) - 1;
-  const Kv4Span span = kv4_span(P.c.lengths[b], nq, c0 / P.group, c1 / P.group, P.window, P.sinks);
-  const int n = min(P.chunks, max(1, (span.count + P.chunk_units - 1) / P.chunk_units));
-  const long long row = static_cast<long long>(q0) * P.q_heads + r;
-  const float2* ml = P.part_ml + row * P.chunks;
-  const float* po = P.part_o + row * P.chunks * D + ch;
-  float m = -INFINITY;
-  for (int s = 0; s < n; ++s) m = fmaxf(m, ml[s].x);
-  const float m_use = m == -INFINITY ? 0.0f : m;
-  float l = 0.0f;
-  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  const int cta = blockIdx.x;
+  const int4 head = P.part_head[cta];
+  const int parts = head.w, c0 = head.y & 0xffffff, ncols = head.y >> 24;
+  if (parts == 0) return;
+  // the first CTA kept its part as one that goes on, the others as one that began earlier
+  const int split = gridDim.y == 1 ? 1 : 8;  // warps that share a column
+  const int col = gridDim.y == 1 ? warp : blockIdx.y, from = gridDim.y == 1 ? 0 : warp;
+  auto slot = [&](int i) { return (2LL * (cta + i) + (i == 0 ? 1 : 0)) * cols + col; };
+  float l = 0.0f, o[kVec];
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) o[e] = 0.0f;
+  if (col < ncols) {
+    float m = -INFINITY;
+    for (int i = lane; i < parts; i += 32) m = fmaxf(m, P.part_ml[slot(i)].x);
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+    const float m_use = m == -INFINITY ? 0.0f : m;
 #pragma unroll 4
-  for (int s = 0; s < n; ++s) {
-    const float2 x = ml[s];
-    const float4 v = *reinterpret_cast<const float4*>(po + static_cast<long long>(s) * D);
-    const float f = x.x == -INFINITY && x.y == 0.0f ? 0.0f : ex2_approx(x.x - m_use);
-    l = fmaf(f, x.y, l);
-    o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
+    for (int i = from; i < parts; i += split) {
+      const float2 x = P.part_ml[slot(i)];
+      float v[kVec];
+      const float* src = P.part_o + slot(i) * D + lane * kVec;
+      if constexpr (kVec == 4) {
+        const float4 u = *reinterpret_cast<const float4*>(src);
+        v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
+      } else {
+        const float2 u = *reinterpret_cast<const float2*>(src);
+        v[0] = u.x, v[1] = u.y;
+      }
+      const float f = x.x == -INFINITY && x.y == 0.0f ? 0.0f : ex2_approx(x.x - m_use);
+      l = fmaf(f, x.y, l);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) o[e] = fmaf(f, v[e], o[e]);
+    }
   }
+  if (split > 1) {
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) s_o[warp][lane * kVec + e] = o[e];
+    if (lane == 0) s_l[warp] = l;
+    __syncthreads();
+    if (warp > 0) return;
+    l = 0.0f;
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) o[e] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      l += s_l[w];
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) o[e] += s_o[w][lane * kVec + e];
+    }
+  }
+  if (col >= ncols) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  uint2 u;
-  u.x = pack_bf16x2(o.x * inv, o.y * inv);
-  u.y = pack_bf16x2(o.z * inv, o.w * inv);
-  *reinterpret_cast<uint2*>(P.out + row * D + ch) = u;
+  const int row = c0 + col, tok = row / P.group;
+  const long long orow = static_cast<long long>(head.x + tok) * P.q_heads + head.z * P.group + row - tok * P.group;
+  __nv_bfloat16* dst = P.out + orow * D + lane * kVec;
+  if constexpr (kVec == 4)
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
+  else
+    *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(o[0] * inv, o[1] * inv);
 }
 
 namespace {
@@ -488,15 +659,23 @@ cudaError_t launch_pdl(K kernel, dim3 grid, int threads, size_t smem, cudaStream
 }
 
 template <int D, int NT>
-cudaError_t launch_decode(const Kv4AttnParams& p, cudaStream_t stream) {
-  const int tiles = (p.max_new * p.group + 8 * NT - 1) / (8 * NT);
-  cudaError_t e = launch_pdl(kv4_decode_kernel<D, NT>, dim3(p.chunks, tiles * p.c.kv_heads, p.c.seqs), 32 * kDecWarps,
-                             DecShape<D, NT>::kSmem, stream, p);
-  if (e != cudaSuccess || p.chunks == 1) return e;
-  const int rows_per_block = 128 / (D / 4);
-  return launch_pdl(kv4_combine_kernel<D>,
-                    dim3((p.max_new * p.q_heads + rows_per_block - 1) / rows_per_block, p.c.seqs, 1), 128, 0, stream, p,
-                    8 * NT);
+cudaError_t launch_decode(const Kv4AttnParams& whole, int ctas, cudaStream_t stream) {
+  for (int b0 = 0; b0 < whole.c.seqs; b0 += kDecMaxSeqs) {
+    Kv4AttnParams p = whole;
+    p.c.seqs = std::min(kDecMaxSeqs, whole.c.seqs - b0);
+    p.c.cu += b0;
+    p.c.lengths += b0;
+    p.c.table += static_cast<long long>(b0) * p.c.table_ld;
+    cudaError_t e = launch_pdl(kv4_decode_kernel<D, NT>, dim3(ctas, 1, 1), 32 * kDecWarps, DecShape<D, NT>::kSmem, stream, p);
+    if (e != cudaSuccess) return e;
+    if (ctas == 1 || p.whole) continue;
+    // few segments have many parts each: then a CTA per column
+    const long long segments = (static_cast<long long>(p.max_new) * p.group + 8 * NT - 1) / (8 * NT) * p.c.kv_heads * p.c.seqs;
+    const bool many = ctas > 16 * segments;
+    e = launch_pdl(kv4_combine_kernel<D>, dim3(ctas, many ? 8 * NT : 1, 1), many ? 256 : 256 * NT, 0, stream, p, 8 * NT);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
 }
 
 template <int D, int NT>
@@ -506,10 +685,9 @@ cudaError_t decode_smem() {
 }
 }  // namespace
 
-cudaError_t launch_kv4_decode(const Kv4AttnParams& p, int head_dim, int cols_per_cta, cudaStream_t stream) {
-  if (head_dim == 128)
-    return cols_per_cta == 8 ? launch_decode<128, 1>(p, stream) : launch_decode<128, 2>(p, stream);
-  return cols_per_cta == 8 ? launch_decode<64, 1>(p, stream) : launch_decode<64, 2>(p, stream);
+cudaError_t launch_kv4_decode(const Kv4AttnParams& p, int head_dim, int cols, int ctas, cudaStream_t stream) {
+  if (head_dim == 128) return cols == 8 ? launch_decode<128, 1>(p, ctas, stream) : launch_decode<128, 2>(p, ctas, stream);
+  return cols == 8 ? launch_decode<64, 1>(p, ctas, stream) : launch_decode<64, 2>(p, ctas, stream);
 }
 
 cudaError_t kv4_prepare_device() {
@@ -522,29 +700,28 @@ cudaError_t kv4_prepare_device() {
 
 namespace {
 struct DecodePlan {
-  int cols, chunk_units, chunks;
-  uint64_t bytes;  // workspace of the splits' results
+  int cols, ctas, whole;
+  uint64_t part_rows, bytes;  // workspace of unfinished segments
 };
 
-// Columns per CTA and the split over the length.  Splits until two rounds of the resident CTAs
-// (two per SM) are full or a warp is left with one unit; a split has at most 256 units (each
-// warp holds the places of its units in its 32 lanes).
-DecodePlan decode_plan(const rldx_kv4_cache& c, int tokens, int q_heads, int max_new, int max_len, int window, int sinks) {
+// Columns per CTA, and one wave of resident CTAs (two per SM with 8 columns, one with 16), or
+// fewer when not every warp could have a unit.  Up to kDecWholeUnits units a segment is left
+// whole: the few rounds that a warp then takes cost less than the join's launch.
+constexpr int kDecWholeUnits = 48;
+DecodePlan decode_plan(const rldx_kv4_cache& c, int q_heads, int max_new, int max_len, int window, int sinks) {
   DecodePlan p;
   const int group = q_heads / c.kv_heads;
   p.cols = max_new * group <= 8 ? 8 : 16;
   const long long tiles = (static_cast<long long>(max_new) * group + p.cols - 1) / p.cols;
-  const long long base = tiles * c.kv_heads * c.seqs;
   long long keys = max_len;
   if (window > 0) keys = std::min<long long>(keys, static_cast<long long>(window) + max_new + std::min(sinks, max_len) + 3 * kKv4Unit);
-  const long long units = std::max<long long>(1, (keys + kKv4Unit - 1) / kKv4Unit);
-  const long long want = std::max<long long>(1, 4LL * sm_count() / base);
-  long long per = std::max<long long>(kDecWarps, (units + want - 1) / want);
-  per = std::min<long long>((per + kDecWarps - 1) / kDecWarps * kDecWarps, 32 * kDecWarps);
-  p.chunk_units = static_cast<int>(per);
-  p.chunks = static_cast<int>((units + per - 1) / per);
-  const uint64_t rows = static_cast<uint64_t>(tokens) * q_heads;
-  p.bytes = p.chunks == 1 ? 0 : rows * p.chunks * (static_cast<uint64_t>(c.head_dim) * 4 + 8);
+  const long long units = (keys + kKv4Unit - 1) / kKv4Unit;
+  const long long segments = tiles * c.kv_heads * std::min(c.seqs, kDecMaxSeqs);
+  const int wave = (p.cols == 8 ? kDecResident : kDecResident / 2) * sm_count();
+  p.whole = units <= kDecWholeUnits;
+  p.ctas = static_cast<int>(std::min<long long>(wave, p.whole ? segments : (units * segments + kDecWarps - 1) / kDecWarps));
+  p.part_rows = (p.ctas == 1 || p.whole) ? 0 : 2ull * p.ctas * p.cols;
+  p.bytes = p.part_rows * (static_cast<uint64_t>(c.head_dim) * 4 + 8) + (p.part_rows ? 16ull * p.ctas : 0);
   return p;
 }
 
@@ -559,6 +736,7 @@ int attention_args(const rldx_kv4_cache* cache, const rldx_kv4_attention_desc* a
   if (cache->seqs > 65535) return set_error(RLDX_ERR_UNSUPPORTED, "kv4_attention: more than 65535 sequences");
   if (static_cast<long long>(a->tokens) * a->q_heads >= (1LL << 31) || static_cast<long long>(a->max_new) * a->q_heads >= (1LL << 19))
     return set_error(RLDX_ERR_UNSUPPORTED, "kv4_attention: too many rows");
+  p->max_len = static_cast<int>(std::min<long long>(a->max_len, static_cast<long long>(cache->table_width) * cache->page_size));
   return RLDX_OK;
 }
 }  // namespace
@@ -575,7 +753,7 @@ int rldx_kv4_attention_workspace_size(const rldx_kv4_cache* cache, const rldx_kv
   Kv4AttnParams p;
   int rc = attention_args(cache, a, &p);
   if (rc != RLDX_OK) return rc;
-  *bytes = decode_plan(*cache, a->tokens, a->q_heads, a->max_new, std::min<long long>(a->max_len, static_cast<long long>(cache->table_width) * cache->page_size), a->window, a->sinks).bytes;
+  *bytes = decode_plan(*cache, a->q_heads, a->max_new, p.max_len, a->window, a->sinks).bytes;
   return RLDX_OK;
 }
 
@@ -592,8 +770,7 @@ int rldx_kv4_attention(const rldx_kv4_cache* cache, const rldx_kv4_attention_des
   if (a->ldq < static_cast<int64_t>(a->q_heads) * d || a->ldq % 8)
     return set_error(RLDX_ERR_ARG, "kv4_attention: q rows must be 16-byte aligned and hold every head");
   if (a->tokens == 0) return RLDX_OK;
-  const int max_len = static_cast<int>(std::min<long long>(a->max_len, static_cast<long long>(cache->table_width) * cache->page_size));
-  const DecodePlan plan = decode_plan(*cache, a->tokens, a->q_heads, a->max_new, max_len, a->window, a->sinks);
+  const DecodePlan plan = decode_plan(*cache, a->q_heads, a->max_new, p.max_len, a->window, a->sinks);
   if (plan.bytes > workspace_bytes || (plan.bytes > 0 && (!workspace || !aligned_to(workspace, 16))))
     return set_error(RLDX_ERR_ARG, "kv4_attention: needs a 16-byte aligned workspace of " + std::to_string(plan.bytes) + " bytes");
   p.q = static_cast<const __nv_bfloat16*>(a->q);
@@ -605,12 +782,11 @@ int rldx_kv4_attention(const rldx_kv4_cache* cache, const rldx_kv4_attention_des
   p.sinks = a->window > 0 ? a->sinks : 0;
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.max_new = a->max_new;
-  p.max_len = max_len;
-  p.chunk_units = plan.chunk_units;
-  p.chunks = plan.chunks;
+  p.whole = plan.whole;
   p.part_o = static_cast<float*>(workspace);
-  p.part_ml = reinterpret_cast<float2*>(p.part_o + (plan.chunks > 1 ? static_cast<size_t>(a->tokens) * a->q_heads * plan.chunks * d : 0));
-  cudaError_t e = launch_kv4_decode(p, d, plan.cols, static_cast<cudaStream_t>(stream));
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + plan.part_rows * d);
+  p.part_head = reinterpret_cast<int4*>(p.part_ml + plan.part_rows);
+  cudaError_t e = launch_kv4_decode(p, d, plan.cols, plan.ctas, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "kv4_attention launch");
   return RLDX_OK;
 }
