@@ -124,6 +124,8 @@ __device__ __forceinline__ Kv4Span kv4_span(int length, int nq, int tok_lo, int 
   return s;
 }
 
+cudaError_t launch_kv4_chunk(const Kv4AttnParams& p, int head_dim, cudaStream_t stream);
+cudaError_t kv4_chunk_prepare_device();
 cudaError_t launch_kv4_decode(const Kv4AttnParams& p, int head_dim, int cols, int ctas, cudaStream_t stream);
 
 }  // namespace rldx

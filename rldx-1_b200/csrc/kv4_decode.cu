@@ -695,12 +695,13 @@ cudaError_t kv4_prepare_device() {
   if (e == cudaSuccess) e = decode_smem<128, 2>();
   if (e == cudaSuccess) e = decode_smem<64, 1>();
   if (e == cudaSuccess) e = decode_smem<64, 2>();
+  if (e == cudaSuccess) e = kv4_chunk_prepare_device();
   return e;
 }
 
 namespace {
 struct DecodePlan {
-  int cols, ctas, whole;
+  int cols, ctas, whole;  // cols 0: kv4_chunk_kernel
   uint64_t part_rows, bytes;  // workspace of unfinished segments
 };
 
@@ -708,9 +709,12 @@ struct DecodePlan {
 // fewer when not every warp could have a unit.  Up to kDecWholeUnits units a segment is left
 // whole: the few rounds that a warp then takes cost less than the join's launch.
 constexpr int kDecWholeUnits = 48;
+constexpr int kDecMaxRows = 32;  // rows of a kv head and sequence beyond which kv4_chunk_kernel takes over
 DecodePlan decode_plan(const rldx_kv4_cache& c, int q_heads, int max_new, int max_len, int window, int sinks) {
   DecodePlan p;
   const int group = q_heads / c.kv_heads;
+  p = {};
+  if (max_new * group > kDecMaxRows) return p;
   p.cols = max_new * group <= 8 ? 8 : 16;
   const long long tiles = (static_cast<long long>(max_new) * group + p.cols - 1) / p.cols;
   long long keys = max_len;
@@ -786,7 +790,8 @@ int rldx_kv4_attention(const rldx_kv4_cache* cache, const rldx_kv4_attention_des
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + plan.part_rows * d);
   p.part_head = reinterpret_cast<int4*>(p.part_ml + plan.part_rows);
-  cudaError_t e = launch_kv4_decode(p, d, plan.cols, plan.ctas, static_cast<cudaStream_t>(stream));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = plan.cols == 0 ? launch_kv4_chunk(p, d, st) : launch_kv4_decode(p, d, plan.cols, plan.ctas, st);
   if (e != cudaSuccess) return cuda_fail(e, "kv4_attention launch");
   return RLDX_OK;
 }
