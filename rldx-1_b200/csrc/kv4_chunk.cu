@@ -7,8 +7,8 @@
 // fp16 scaled by a power of two per row (largest in [2^14, 2^15)), p is at most 2^8 by the lazy
 // reference maximum of joint_attention_kernel; sums and maxima are fp32.
 //
-// Warps: 0 fetches units by bulk copies, 1 issues the MMAs, 2-9 do the softmax (one row a thread),
-// 10-11 rebuild K, 12-13 rebuild V^T.  The order of channels inside 16 bytes of K (and q) is that of
+// Warps: 0 fetches units by bulk copies, 1 issues the MMAs, 4-11 do the softmax (one row a thread),
+// 12-13 rebuild K, 14-15 rebuild V^T; registers move from the first four to the softmax.  The order of channels inside 16 bytes of K (and q) is that of
 // the nibbles under the masks (0 4 1 5 2 6 3 7), and tokens stand inside each group of eight in
 // an order rotated by the group (chunk_token), so that neither side needs a shuffle and both the
 // reads of the units and the writes of the swizzled tiles are free of bank conflicts.
@@ -39,11 +39,11 @@ struct ChunkShape {
   static constexpr int kRaw = 2 * Kv4Unit<D>::kBytes;
   static constexpr int kStages = 3;     // of K and of V^T
   static constexpr int kRawStages = 4;  // of unit pairs
-  static constexpr int kThreads = 32 * 14;
+  static constexpr int kThreads = 32 * 16;
   static constexpr uint32_t kOCol = 256;  // S / P: (2 g + buffer) 64 columns; O of tile g: 256 + g d
   static constexpr uint32_t kTmemCols = 512;
   static constexpr int kBars = 1 + 2 * kRawStages + 4 * kStages + 2 * 7 + 1;
-  static constexpr int kBad = kStages * (kG + 1) * 8;  // marks of what is not finite, a bit per token: V's groups, K
+  static constexpr int kBad = kStages * (kG + 2) * 8;  // marks of what is not finite, a bit per token: V's groups, K; any
   static constexpr size_t kSmem = 1024 + 2 * kQTile + kStages * (kKTile + kVTile) + kRawStages * kRaw + kBad + 8 * kBars + 16;
 };
 
@@ -69,11 +69,75 @@ __device__ __forceinline__ void codes_f16(uint32_t w, __half2 (&c)[4]) {
   c[2] = __hsub2(bits_h2((v & 0x000f000fu) | 0x64006400u), bias);
   c[3] = __hfma2(bits_h2((v & 0x00f000f0u) | 0x64006400u), sixteenth, shift);
 }
-__device__ __forceinline__ __half2 clamp_finite(__half2 x) {  // NaN stays
+__device__ __forceinline__ void clamp_words(uint4* at) {  // NaN stays
   const __half2 top = bits_h2(0x7bff7bffu), bottom = bits_h2(0xfbfffbffu);
-  return __hmax2_nan(__hmin2_nan(x, top), bottom);
+  uint32_t* w = reinterpret_cast<uint32_t*>(at);
+#pragma unroll 1
+  for (int i = 0; i < 4; ++i) w[i] = h2_bits(__hmax2_nan(__hmin2_nan(bits_h2(w[i]), top), bottom));
 }
 }  // namespace
+
+// MMAs and commits that a converged warp reaches and the lane with `lead` issues.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+  return e;
+}
+__device__ __forceinline__ void umma_f16_lead(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 e, %5, 0;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate),
+      "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void umma_f16_ts_lead(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 e, %5, 0;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate),
+      "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void umma_commit_lead(uint32_t lead, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)), "r"(lead)
+      : "memory");
+}
+
+// 16 consecutive 32-bit columns of one TMEM lane per thread.
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const float (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3])),
+      "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])), "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7])),
+      "r"(__float_as_uint(v[8])), "r"(__float_as_uint(v[9])), "r"(__float_as_uint(v[10])), "r"(__float_as_uint(v[11])),
+      "r"(__float_as_uint(v[12])), "r"(__float_as_uint(v[13])), "r"(__float_as_uint(v[14])), "r"(__float_as_uint(v[15]))
+      : "memory");
+}
+template <int N>
+__device__ __forceinline__ void reg_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void reg_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+// Registers a thread of the four warpgroups: 72 + 160 + 160 + 120 = 4 x 128, what the block starts with.
+constexpr int kChunkRegsIssue = 72, kChunkRegsSoftmax = 160, kChunkRegsRebuild = 120;
+
+// What a row sees of a unit of 32 tokens: tau < hi and (tau > lo or tau < sinks), a bit per key position.
+__device__ __forceinline__ uint32_t chunk_seen(int hi, int lo, int sinks) {
+  auto below = [](int n) -> uint32_t { return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u); };
+  const uint32_t m = below(hi) & (~below(lo + 1) | below(sinks));
+  // token pair p of group o stands at pair (p - o) & 3: byte o turns right by 2 o bits
+  uint32_t r = m & 0xffu;
+#pragma unroll
+  for (int o = 1; o < 4; ++o) {
+    const uint32_t x = m >> (8 * o) & 0xffu;
+    r |= ((x >> (2 * o) | x << (8 - 2 * o)) & 0xffu) << (8 * o);
+  }
+  return r;
+}
 
 template <int D>
 __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(const __grid_constant__ Kv4AttnParams P) {
@@ -87,7 +151,7 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
   uint8_t* sK = sQ + 2 * Sh::kQTile;
   uint8_t* sV = sK + kS * Sh::kKTile;
   uint8_t* sRaw = sV + kS * Sh::kVTile;
-  uint8_t* sBad = sRaw + kR * Sh::kRaw;  // [stage][group of V, then K][8] bytes
+  uint8_t* sBad = sRaw + kR * Sh::kRaw;  // [stage][group of V, then K, then any][8] bytes
   uint64_t* bars = reinterpret_cast<uint64_t*>(sBad + Sh::kBad);
   uint64_t* q_full = bars;
   uint64_t* raw_full = bars + 1;
@@ -142,6 +206,8 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
+  if (warp < 4) {
+    reg_dec<kChunkRegsIssue>();
   if (warp == 0) {
     // ---------------- units: bulk copies; lane i looks up the i-th of the next 32 ----------------
     bool ok = true;
@@ -174,57 +240,66 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
     if (!ok) settle_issued_copies();
   } else if (warp == 1) {
     // ---------------- MMAs ----------------
-    if (lane == 0 && nt > 0) {
-      const uint32_t idesc_s = umma_idesc_f16(128, 64), idesc_o = umma_idesc_f16(128, D);
-      bool ok = mbar_wait(q_full, 0u, kErrKv4Chunk + 1);
-      tc_fence_after();
-      auto issue_s = [&](int j) -> bool {
-        const int s = j % kS;
-        if (!mbar_wait(&k_full[s], static_cast<uint32_t>(j / kS) & 1u, kErrKv4Chunk + 1)) return false;
-        const uint32_t k_addr = smem_u32(sK + s * Sh::kKTile);
-        for (int g = 0; g < ng; ++g) {
-          // the buffer holds P_{j-2} until its product is done
-          if (j >= 2 && !mbar_wait(&o_done(g)[j & 1], static_cast<uint32_t>((j - 2) >> 1) & 1u, kErrKv4Chunk + 1)) return false;
+    // the whole warp runs the loop, so that descriptors stay in uniform registers; one elected lane
+    // issues
+    const uint32_t lead = elect_one();
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const int tiles_k = __shfl_sync(0xffffffffu, nt, 0), groups = __shfl_sync(0xffffffffu, ng, 0);
+    constexpr uint32_t idesc_s = umma_idesc_f16(128, 64), idesc_o = umma_idesc_f16(128, D);
+    const uint64_t q_desc = umma_desc_sw128(smem_u32(sQ)), k_desc = umma_desc_sw128(smem_u32(sK)), v_desc = umma_desc_sw128(smem_u32(sV));
+    bool ok = tiles_k > 0 && __all_sync(0xffffffffu, mbar_wait(q_full, 0u, kErrKv4Chunk + 1));
+    tc_fence_after();
+    // S runs two tiles ahead of PV
+    int ks = 0, vs = 0;  // stages of S_{j+2} and PV_j, and their rounds' parity
+    uint32_t kp = 0u, vp = 0u;
+    for (int j = -2; ok && j < tiles_k; ++j) {
+      const int b2 = j & 1;  // buffer of tiles j and j + 2
+      if (j >= 0) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&v_full[vs], vp, kErrKv4Chunk + 1));
+        for (int g = 0; ok && g < groups; ++g) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&p_full(g)[b2], static_cast<uint32_t>(j >> 1) & 1u, kErrKv4Chunk + 1));
+          if (!ok) break;
           tc_fence_after();
-          const uint32_t q_addr = smem_u32(sQ + g * Sh::kQTile);
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            umma_f16(tmem + (2 * g + (j & 1)) * 64, umma_desc_sw128(q_addr + (k >> 2) * Sh::kQChunk + 32 * (k & 3)),
-                     umma_desc_sw128(k_addr + (k >> 2) * Sh::kKChunk + 32 * (k & 3)), idesc_s, k != 0 ? 1u : 0u);
-          umma_commit(&s_full(g)[j & 1]);
-        }
-        umma_commit(&k_empty[s]);
-        return true;
-      };
-      if (ok) ok = issue_s(0);
-      if (ok && nt > 1) ok = issue_s(1);
-      for (int j = 0; ok && j < nt; ++j) {
-        const int s = j % kS;
-        if (!(ok = mbar_wait(&v_full[s], static_cast<uint32_t>(j / kS) & 1u, kErrKv4Chunk + 1))) break;
-        const uint32_t v_addr = smem_u32(sV + s * Sh::kVTile);
-        for (int g = 0; ok && g < ng; ++g) {
-          if (!(ok = mbar_wait(&p_full(g)[j & 1], static_cast<uint32_t>(j >> 1) & 1u, kErrKv4Chunk + 1))) break;
-          tc_fence_after();
+          const uint64_t vd = v_desc + static_cast<uint32_t>(vs) * (Sh::kVTile >> 4);
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            umma_f16_ts(tmem + Sh::kOCol + g * D, tmem + (2 * g + (j & 1)) * 64 + 8 * k, umma_desc_sw128(v_addr + 32 * k),
-                        idesc_o, (j | k) != 0 ? 1u : 0u);
-          umma_commit(&o_done(g)[j & 1]);
-          if (j == nt - 1) umma_commit(o_final(g));
+            umma_f16_ts_lead(lead, tm + Sh::kOCol + g * D, tm + (2 * g + b2) * 64 + 8 * k, vd + 2 * k, idesc_o, (j | k) != 0);
+          umma_commit_lead(lead, &o_done(g)[b2]);
+          if (j == tiles_k - 1) umma_commit_lead(lead, o_final(g));
         }
         if (!ok) break;
-        umma_commit(&v_empty[s]);
-        if (j + 2 < nt) ok = issue_s(j + 2);
+        umma_commit_lead(lead, &v_empty[vs]);
+        if (++vs == kS) vs = 0, vp ^= 1u;
       }
-      if (!ok) {  // the MMAs already issued finish before tensor memory is released
-        umma_commit(drain);
-        mbar_wait_teardown(drain, 0u);
+      if (j + 2 < tiles_k) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&k_full[ks], kp, kErrKv4Chunk + 1));
+        for (int g = 0; ok && g < groups; ++g) {
+          // the buffer holds P_j until its product is done
+          if (j >= 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_done(g)[b2], static_cast<uint32_t>(j >> 1) & 1u, kErrKv4Chunk + 1));
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t qd = q_desc + static_cast<uint32_t>(g) * (Sh::kQTile >> 4), kd = k_desc + static_cast<uint32_t>(ks) * (Sh::kKTile >> 4);
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            umma_f16_lead(lead, tm + (2 * g + b2) * 64, qd + (((k >> 2) * Sh::kQChunk + 32 * (k & 3)) >> 4),
+                          kd + (((k >> 2) * Sh::kKChunk + 32 * (k & 3)) >> 4), idesc_s, k != 0);
+          umma_commit_lead(lead, &s_full(g)[b2]);
+        }
+        if (!ok) break;
+        umma_commit_lead(lead, &k_empty[ks]);
+        if (++ks == kS) ks = 0, kp ^= 1u;
       }
     }
-  } else if (warp >= 10) {
-    // ---------------- rebuild K (warps 10, 11) and V^T (warps 12, 13) ----------------
-    const bool is_v = warp >= 12;
-    const int w = (warp - 10) & 1;
+    if (!ok && tiles_k > 0) {  // the MMAs already issued finish before tensor memory is released
+      umma_commit_lead(lead, drain);
+      mbar_wait_teardown(drain, 0u);
+    }
+  }
+  } else if (warp >= 12) {
+    // ---------------- rebuild K (warps 12, 13) and V^T (warps 14, 15) ----------------
+    reg_dec<kChunkRegsRebuild>();
+    const bool is_v = warp >= 14;
+    const int w = warp & 1;
     bool ok = true;
     for (int j = 0; ok && j < nt; ++j) {
       const int s = j % kS, rs = j % kR;
@@ -238,7 +313,7 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
         // keeps both the loads (64-byte rows) and the swizzled stores free of conflicts
         const int t = lane & 3, r = (lane >> 3) ^ ((lane & 4) ? 5 : 0);
         uint8_t* dst = sK + s * Sh::kKTile;
-#pragma unroll 2
+#pragma unroll 1
         for (int p = 0; p < 4; ++p) {
           const int token = 8 * (4 * w + p) + r, tau = token & 31;
           const uint8_t* un = raw + (token >> 5) * U::kBytes;
@@ -249,8 +324,8 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
 #pragma unroll
           for (int i = 0; i < G / 2; ++i)
             z = __hfma2(__hfma2(bits_h2(0x4b804b80u), bits_h2(meta[i]), bits_h2(meta[G / 2 + i])), bits_h2(0u), z);
-          const bool odd = __any_sync(0xffffffffu, h2_bits(z) & 0x7fff7fffu);
           const int row = chunk_row(token);
+          uint8_t* at = dst + row * 128;
 #pragma unroll
           for (int gi = 0; gi < G; ++gi) {
             const uint32_t sel = (gi & 1) ? 0x3232u : 0x1010u;
@@ -258,11 +333,14 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
             __half2 c[4];
             codes_f16(code[gi], c);
             uint4 u;
-            __half2 x0 = __hfma2(c[0], sc, lo), x1 = __hfma2(c[1], sc, lo), x2 = __hfma2(c[2], sc, lo), x3 = __hfma2(c[3], sc, lo);
-            if (odd) x0 = clamp_finite(x0), x1 = clamp_finite(x1), x2 = clamp_finite(x2), x3 = clamp_finite(x3);
-            u.x = h2_bits(x0), u.y = h2_bits(x1), u.z = h2_bits(x2), u.w = h2_bits(x3);
-            const int unit = 4 * (gi & 1) + t;
-            *reinterpret_cast<uint4*>(dst + (gi >> 1) * Sh::kKChunk + row * 128 + ((unit ^ (row & 7)) << 4)) = u;
+            u.x = h2_bits(__hfma2(c[0], sc, lo)), u.y = h2_bits(__hfma2(c[1], sc, lo));
+            u.z = h2_bits(__hfma2(c[2], sc, lo)), u.w = h2_bits(__hfma2(c[3], sc, lo));
+            *reinterpret_cast<uint4*>(at + (gi >> 1) * Sh::kKChunk + (((4 * (gi & 1) + t) ^ (row & 7)) << 4)) = u;
+          }
+          if (h2_bits(z) & 0x7fff7fffu) {  // a value outside fp16's range becomes its largest
+#pragma unroll 1
+            for (int gi = 0; gi < G; ++gi)
+              clamp_words(reinterpret_cast<uint4*>(at + (gi >> 1) * Sh::kKChunk + (((4 * (gi & 1) + t) ^ (row & 7)) << 4)));
           }
         }
       } else {
@@ -289,13 +367,7 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
 #pragma unroll
         for (int i = 0; i < G; ++i) zk = __hfma2(bits_h2(meta[i]), bits_h2(0u), zk);
         const unsigned bad_k = __ballot_sync(0xffffffffu, h2_bits(zk) & 0x7fff7fffu);
-        if (g == 0) {
-          uint32_t byte = 0u;
-          if (bad_k != 0u)
-            for (int i = 0; i < 8; ++i) byte |= (bad_k >> (4 * i + lane) & 1u) << (chunk_row(8 * o + i) & 7);
-          sBad[(s * (G + 1) + G) * 8 + o] = static_cast<uint8_t>(byte);
-        }
-        const bool odd = __any_sync(0xffffffffu, h2_bits(z) & 0x7fff7fffu);
+        const bool odd = (h2_bits(z) & 0x7fff7fffu) != 0u;  // a value would not be finite
         uint32_t bad[G];
 #pragma unroll
         for (int gi = 0; gi < G; ++gi) bad[gi] = 0u;
@@ -310,6 +382,22 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
               bad[gi] |= ((~fine & 1u) | (~fine >> 15 & 2u)) << (2 * k);
             }
         }
+        if (__any_sync(0xffffffffu, odd || bad_k != 0u)) {
+          if (g == 0) {
+#pragma unroll
+            for (int gi = 0; gi < G; ++gi) sBad[(s * (G + 2) + gi) * 8 + o] = static_cast<uint8_t>(bad[gi]);
+            uint32_t byte = 0u;
+#pragma unroll 1
+            for (int i = 0; i < 8; ++i) byte |= (bad_k >> (4 * i + lane) & 1u) << (chunk_row(8 * o + i) & 7);
+            sBad[(s * (G + 2) + G) * 8 + o] = static_cast<uint8_t>(byte);
+            sBad[(s * (G + 2) + G + 1) * 8 + o] = 1u;
+          }
+          __syncwarp();
+        } else if (g == 0) {
+          // the other warp's groups may be marked: then these are read too
+#pragma unroll
+          for (int gi = 0; gi <= G + 1; ++gi) sBad[(s * (G + 2) + gi) * 8 + o] = 0u;
+        }
         uint8_t* dst = sV + s * Sh::kVTile;
 #pragma unroll
         for (int gi = 0; gi < G; ++gi) {
@@ -321,9 +409,7 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
             codes_f16(x, c);  // channels 0..3 of tokens 2t | 2t + 1
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              __half2 v = __hfma2(c[i], bits_h2(sc[k][gi]), bits_h2(lo[k][gi]));
-              if (odd) v = clamp_finite(v);
-              out[i][k] = h2_bits(v);
+              out[i][k] = h2_bits(__hfma2(c[i], bits_h2(sc[k][gi]), bits_h2(lo[k][gi])));
             }
           }
 #pragma unroll
@@ -331,7 +417,13 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
             const int row = 32 * gi + 4 * g + i;
             *reinterpret_cast<uint4*>(dst + row * 128 + ((o ^ (row & 7)) << 4)) = make_uint4(out[i][0], out[i][1], out[i][2], out[i][3]);
           }
-          if (g == 0) sBad[(s * (G + 1) + gi) * 8 + o] = static_cast<uint8_t>(bad[gi]);
+        }
+        if (odd) {
+#pragma unroll 1
+          for (int i = 0; i < 4 * G; ++i) {
+            const int row = 32 * (i >> 2) + 4 * g + (i & 3);
+            clamp_words(reinterpret_cast<uint4*>(dst + row * 128 + ((o ^ (row & 7)) << 4)));
+          }
         }
       }
       fence_proxy_async_smem();
@@ -343,7 +435,8 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
     }
   } else {
     // ---------------- softmax: one row a thread ----------------
-    const int g = (warp - 2) >> 2, quad = warp & 3, r = quad * 32 + lane;
+    reg_inc<kChunkRegsSoftmax>();
+    const int g = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane;
     const int row = c0 + 128 * g + r;  // among the kv head's rows
     const bool live = 128 * g + r < nrows;
     const int tok = row / P.group, head = kvh * P.group + row - tok * P.group;
@@ -401,34 +494,37 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
       ok = __all_sync(0xffffffffu, mbar_wait(&s_full(g)[sb], ph, kErrKv4Chunk + 3));
       if (!ok) break;
       tc_fence_after();
-      float sv[64];
-      tmem_ld32(s_col, *reinterpret_cast<float(*)[32]>(&sv[0]));
-      tmem_ld32(s_col + 32, *reinterpret_cast<float(*)[32]>(&sv[32]));
-      tmem_wait_ld();
-      // ---- masks: keys of the two units; a unit past the span or without a page is hidden ----
+      // ---- masks: keys of the two units; a unit past the span is hidden ----
       bool plain = true;
-      int hi[2], lo[2], sk[2];  // token tau of unit i is seen iff tau < hi and (tau > lo or tau < sk)
+      int key0[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int u = 2 * j + i;
-        const bool have = u < span.count;
-        const int key0 = have ? kKv4Unit * span.unit(u) : 0;
-        hi[i] = have ? ps - key0 + 1 : 0;
-        lo[i] = P.window > 0 ? ps - P.window - key0 : -1;
-        sk[i] = P.window > 0 ? P.sinks - key0 : 0;
-        plain &= have && key0 + 31 <= pos_lo && (P.window <= 0 || pos_hi - key0 < P.window || key0 + 31 < P.sinks);
+        const bool have = 2 * j + i < span.count;
+        key0[i] = have ? kKv4Unit * span.unit(2 * j + i) : 0x40000000;
+        plain &= key0[i] + 31 <= pos_lo && (P.window <= 0 || pos_hi - key0[i] < P.window || key0[i] + 31 < P.sinks);
       }
+      uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
+      if (!plain) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          seen[i] = P.window > 0 ? chunk_seen(ps - key0[i] + 1, ps - P.window - key0[i], P.sinks - key0[i])
+                                 : chunk_seen(ps - key0[i] + 1, -1, 0);
+      }
+      // the scores are read twice, 32 at a time: for the maximum, then for the exponentials
       float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      if (plain) {
+#pragma unroll 1
+      for (int i = 0; i < 2; ++i) {
+        float sv[32];
+        tmem_ld32(s_col + 32 * i, sv);
+        const uint32_t see = seen[i];
+        tmem_wait_ld();
+        if (!plain) {
 #pragma unroll
-        for (int c = 0; c < 64; ++c) mx4[c & 3] = fmaxf(mx4[c & 3], sv[c]);
-      } else {
-#pragma unroll
-        for (int c = 0; c < 64; ++c) {
-          const int tau = chunk_token(c) & 31, i = c >> 5;
-          sv[c] = (tau < hi[i] && (tau > lo[i] || tau < sk[i])) ? sv[c] : -INFINITY;
-          mx4[c & 3] = fmaxf(mx4[c & 3], sv[c]);
+          for (int c = 0; c < 32; ++c)
+            if (!(see >> c & 1u)) sv[c] = -INFINITY;
         }
+#pragma unroll
+        for (int c = 0; c < 32; ++c) mx4[c & 3] = fmaxf(mx4[c & 3], sv[c]);
       }
       const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * fac;
       const bool grow = mx > m_ref + kRescaleLog2;
@@ -442,7 +538,7 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
         ok = __all_sync(0xffffffffu, mbar_wait(&o_done(g)[sb ^ 1], static_cast<uint32_t>((j - 1) >> 1) & 1u, kErrKv4Chunk + 3));
         if (!ok) break;
         tc_fence_after();
-#pragma unroll
+#pragma unroll 1
         for (int h = 0; h < D / 32; ++h) {
           float o[32];
           tmem_ld32(tmem + lane_off + Sh::kOCol + g * D + 32 * h, o);
@@ -455,40 +551,41 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
       }
       const float m_use = m_ref == -INFINITY ? 0.0f : m_ref;
       const float2 f2 = make_float2(fac, fac), n2 = make_float2(-m_use, -m_use);
-      float pk[32];
       float2 sum0 = make_float2(0.0f, 0.0f), sum1 = make_float2(0.0f, 0.0f);
+#pragma unroll 1
+      for (int i = 0; i < 2; ++i) {
+        float sv[32], pk[16];
+        tmem_ld32(s_col + 32 * i, sv);
+        const uint32_t see = seen[i];
+        tmem_wait_ld();
+        if (!plain) {
 #pragma unroll
-      for (int c = 0; c < 64; c += 2) {
-        const float2 x = fma_f32x2(make_float2(sv[c], sv[c + 1]), f2, n2);
-        float2 e;
-        if (((c >> 1) & 3) < kExpFmaPairs)
-          e = exp2_fma_x2(x);
-        else
-          e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-        if (c & 2) sum1 = add_f32x2(sum1, e); else sum0 = add_f32x2(sum0, e);
-        pk[c >> 1] = __uint_as_float(h2_bits(__floats2half2_rn(e.x, e.y)));
+          for (int c = 0; c < 32; ++c)
+            if (!(see >> c & 1u)) sv[c] = -INFINITY;
+        }
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) {
+          const float2 x = fma_f32x2(make_float2(sv[c], sv[c + 1]), f2, n2);
+          float2 e;
+          if (((c >> 1) & 3) < kExpFmaPairs)
+            e = exp2_fma_x2(x);
+          else
+            e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+          if (c & 2) sum1 = add_f32x2(sum1, e); else sum0 = add_f32x2(sum0, e);
+          pk[c >> 1] = __uint_as_float(h2_bits(__floats2half2_rn(e.x, e.y)));
+        }
+        tmem_st16(s_col + 16 * i, pk);  // P_j over S_j, two keys a column: behind what is still to be read
       }
       l_run += (sum0.x + sum0.y) + (sum1.x + sum1.y);
-      tmem_st32(s_col, pk);  // P_j over S_j: two keys a column
       tmem_wait_st();
       // ---- values that are not finite (the marks are there once V_j is) ----
       ok = __all_sync(0xffffffffu, mbar_wait(&v_full[j % kS], static_cast<uint32_t>(j / kS) & 1u, kErrKv4Chunk + 3));
       if (!ok) break;
-      const uint32_t* marks = reinterpret_cast<const uint32_t*>(sBad + (j % kS) * (G + 1) * 8);
-      uint32_t any = 0u;
-#pragma unroll
-      for (int i = 0; i < 2 * G + 2; ++i) any |= marks[i];
-      if (any) {
-        uint32_t seen[2] = {0u, 0u};
-#pragma unroll
-        for (int c = 0; c < 64; ++c) {
-          const int tau = chunk_token(c) & 31, i = c >> 5;
-          if (tau < hi[i] && (tau > lo[i] || tau < sk[i])) seen[i] |= 1u << (c & 31);
-        }
-#pragma unroll
-        for (int gi = 0; gi < G; ++gi)
-          if ((seen[0] & marks[2 * gi]) | (seen[1] & marks[2 * gi + 1])) poison |= 1u << gi;
-        if ((seen[0] & marks[2 * G]) | (seen[1] & marks[2 * G + 1])) poison = 0xffffffffu;
+      const uint32_t* marks = reinterpret_cast<const uint32_t*>(sBad + (j % kS) * (G + 2) * 8);
+      if (marks[2 * G + 2] | marks[2 * G + 3]) {
+#pragma unroll 1
+        for (int gi = 0; gi <= G; ++gi)
+          if ((seen[0] & marks[2 * gi]) | (seen[1] & marks[2 * gi + 1])) poison |= gi < G ? 1u << gi : 0xffffffffu;
       }
       tc_fence_before();
       __syncwarp();
