@@ -510,22 +510,18 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
           seen[i] = P.window > 0 ? chunk_seen(ps - key0[i] + 1, ps - P.window - key0[i], P.sinks - key0[i])
                                  : chunk_seen(ps - key0[i] + 1, -1, 0);
       }
-      // the scores are read twice, 32 at a time: for the maximum, then for the exponentials
       float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-      for (int i = 0; i < 2; ++i) {
-        float sv[32];
-        tmem_ld32(s_col + 32 * i, sv);
-        const uint32_t see = seen[i];
-        tmem_wait_ld();
-        if (!plain) {
+      float sv[64];
+      tmem_ld32(s_col, *reinterpret_cast<float(*)[32]>(&sv[0]));
+      tmem_ld32(s_col + 32, *reinterpret_cast<float(*)[32]>(&sv[32]));
+      tmem_wait_ld();
+      if (!plain) {
 #pragma unroll
-          for (int c = 0; c < 32; ++c)
-            if (!(see >> c & 1u)) sv[c] = -INFINITY;
-        }
-#pragma unroll
-        for (int c = 0; c < 32; ++c) mx4[c & 3] = fmaxf(mx4[c & 3], sv[c]);
+        for (int c = 0; c < 64; ++c)
+          if (!(seen[c >> 5] >> (c & 31) & 1u)) sv[c] = -INFINITY;
       }
+#pragma unroll
+      for (int c = 0; c < 64; ++c) mx4[c & 3] = fmaxf(mx4[c & 3], sv[c]);
       const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * fac;
       const bool grow = mx > m_ref + kRescaleLog2;
       float alpha = 1.0f;
@@ -552,29 +548,17 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
       const float m_use = m_ref == -INFINITY ? 0.0f : m_ref;
       const float2 f2 = make_float2(fac, fac), n2 = make_float2(-m_use, -m_use);
       float2 sum0 = make_float2(0.0f, 0.0f), sum1 = make_float2(0.0f, 0.0f);
-#pragma unroll 1
-      for (int i = 0; i < 2; ++i) {
-        float sv[32], pk[16];
-        tmem_ld32(s_col + 32 * i, sv);
-        const uint32_t see = seen[i];
-        tmem_wait_ld();
-        if (!plain) {
 #pragma unroll
-          for (int c = 0; c < 32; ++c)
-            if (!(see >> c & 1u)) sv[c] = -INFINITY;
-        }
+      for (int i = 0; i < 2; ++i) {
+        float pk[16];
 #pragma unroll
         for (int c = 0; c < 32; c += 2) {
-          const float2 x = fma_f32x2(make_float2(sv[c], sv[c + 1]), f2, n2);
-          float2 e;
-          if (((c >> 1) & 3) < kExpFmaPairs)
-            e = exp2_fma_x2(x);
-          else
-            e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+          const float2 x = fma_f32x2(make_float2(sv[32 * i + c], sv[32 * i + c + 1]), f2, n2);
+          const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
           if (c & 2) sum1 = add_f32x2(sum1, e); else sum0 = add_f32x2(sum0, e);
           pk[c >> 1] = __uint_as_float(h2_bits(__floats2half2_rn(e.x, e.y)));
         }
-        tmem_st16(s_col + 16 * i, pk);  // P_j over S_j, two keys a column: behind what is still to be read
+        tmem_st16(s_col + 16 * i, pk);  // P_j over S_j, two keys a column
       }
       l_run += (sum0.x + sum0.y) + (sum1.x + sum1.y);
       tmem_wait_st();
