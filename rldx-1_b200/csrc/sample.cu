@@ -13,8 +13,9 @@
 // The last token kept is found in one of two ways:
 //   - top-k up to about a thousand: each CTA finds the k / CTAs-th largest of its threads' maxima (four a
 //     thread), by bisection of the ordered bits; the least of these is a lower bound of the k-th
-//     largest logit.  The tokens that reach it, a little more than k, go to rank 0's list, which sorts
-//     them (bitonic, ordered bits and id in one word), scans the weights and draws alone.
+//     largest logit.  The tokens that reach it, a little more than k, go to rank 0's list.  Up to 128 one
+//     of its warps sorts (bitonic, ordered bits and id in one word), scans and draws from alone; of more
+//     it finds the cut as below and tells the others.
 //   - otherwise by histogram: 1024 bins linear in -d (every bin holds a run of the order), then by the
 //     ordered bits of the logit inside the bin where count or weight crosses, until one value is left;
 //     of the tokens that share it the first few by id stay.  Bins hold counts (top-k) or weights
@@ -67,7 +68,7 @@ struct SampleShared {
   u64 found[4];                      // rank 0's answer, written to every CTA
   u64 red[32][2];
   uint32_t red32[32];
-  uint32_t flag, kept;
+  uint32_t flag;
   uint64_t loaded;  // the bulk copy
 };
 
@@ -106,8 +107,7 @@ struct Sampler {
   const uint4* row;    // this CTA's vectors in shared memory
   int nvec, first_id;  // vectors held, id of the first one's first token (negative: padding)
   int rank, cluster, phase;
-  float top, temp, inv;  // maximum, temperature and its reciprocal
-  bool quick;            // a quotient's remainder stays a normal number
+  float top, temp, inv, scale;  // maximum; scaled temperature, its reciprocal and the scale
 
   __device__ __forceinline__ void load(int v, float (&x)[kVec]) const { unpack(row[v], static_cast<const T*>(nullptr), x); }
   template <typename F>
@@ -164,19 +164,18 @@ struct Sampler {
 
   // ---- tokens ----
   // d = (x - top) / temp, correctly rounded: an approximate quotient improved twice by its exact
-  // remainder (Markstein's division with a rounded reciprocal), or divided where a remainder could leave
-  // the normal numbers.  Below -22.2 the weight is 0: -inf.
+  // remainder (Markstein's division with a rounded reciprocal); both sides are scaled by a power of two
+  // that keeps the remainders normal numbers.  -inf and NaN logits, and quotients that overflow, give NaN
+  // or -inf, which weighs 0 below.
   __device__ __forceinline__ float distance(float x) const {
-    const float n = x - top;
-    if (!quick) return x == top ? 0.0f : __fdiv_rn(n, temp);
+    const float n = (x - top) * scale;
     const float q0 = n * inv, q1 = fmaf(fmaf(-q0, temp, n), inv, q0);
-    return q0 > -22.2f ? fmaf(fmaf(-q1, temp, n), inv, q1) : -INFINITY;
+    return fmaf(fmaf(-q1, temp, n), inv, q1);
   }
-  __device__ __forceinline__ static u64 weight_of(float d) {
-    const float f = expf(d) * 4294967296.0f;
-    const u64 w = static_cast<u64>(__float2uint_rz(f)) + (f >= 4294967296.0f ? 1u : 0u);
-    return d > -22.2f ? w : 0;
-  }
+  // The weight, with 2^32 - 1 for 2^32 (exponentials below 1 give at most 2^32 - 256); 0 for NaN.
+  __device__ __forceinline__ static uint32_t weight32(float d) { return __float2uint_rz(expf(d) * 4294967296.0f); }
+  __device__ __forceinline__ static u64 widen(uint32_t t) { return static_cast<u64>(t) + (t == 0xffffffffu ? 1u : 0u); }
+  __device__ __forceinline__ static u64 weight_of(float d) { return widen(weight32(d)); }
   __device__ __forceinline__ u64 weight(float x) const { return weight_of(distance(x)); }
   __device__ __forceinline__ static bool weighs(float d) { return d > -22.17f || (d > -22.2f && weight_of(d) > 0); }
   __device__ __forceinline__ static int bin_of(float d) {
@@ -201,6 +200,8 @@ struct Sampler {
   // The first bin where the running sum passes `level`; found = {bin or ~0, sum before, sum of the
   // bin, whole}.  With `share` >= 0 the level is the last one below share x whole.  rank 0's sums are
   // zero before and after.
+  // kAlone: rank 0 works without the others.
+  template <bool kAlone>
   __device__ __forceinline__ bool crossing(u64 level, float share) {
     __syncthreads();
     const uint32_t g = mapa_shared(smem_u32(s.g), 0);
@@ -208,8 +209,12 @@ struct Sampler {
       const u64 v = (static_cast<u64>(s.hi[i]) << 16) + s.lo[i];
       if (v) red_cluster_u64(g + 8 * i, v);
     }
-    cluster_sync();
+    if constexpr (kAlone)
+      __syncthreads();
+    else
+      cluster_sync();
     if (rank == 0) {
+      const int told = kAlone ? 1 : cluster;  // rank 0 itself is the first
       constexpr int kPer = kSampBins / NT;
       u64 w[kPer], ws = 0;
       const int b0 = threadIdx.x * kPer;
@@ -229,26 +234,30 @@ struct Sampler {
         if (wb <= level && level < wb + w[i]) {
           s.flag = 1u;
           const u64 v[4] = {static_cast<u64>(b0 + i), wb, w[i], whole};
-          for (int r = 0; r < cluster; ++r)
+          for (int r = 0; r < told; ++r)
             for (int k = 0; k < 4; ++k) st_cluster_u64(mapa_shared(smem_u32(&s.found[k]), r), v[k]);
         }
         wb += w[i];
       }
       __syncthreads();
       if (threadIdx.x == 0 && s.flag == 0u)
-        for (int r = 0; r < cluster; ++r) {
+        for (int r = 0; r < told; ++r) {
           st_cluster_u64(mapa_shared(smem_u32(&s.found[0]), r), ~0ull);
           st_cluster_u64(mapa_shared(smem_u32(&s.found[3]), r), whole);
         }
     }
-    cluster_sync();
+    if constexpr (kAlone)
+      __syncthreads();
+    else
+      cluster_sync();
     return s.found[0] != ~0ull;
   }
 
   // Finds the cut where the count (or weight) of the order passes `level` among the tokens of positive
   // weight above `from` and its ties.  With `share` >= 0 the level comes from the whole weight, which
-  // is returned in *whole.  False: never.
-  __device__ __forceinline__ bool find(bool by_count, u64 level, float share, const Cut& from, Cut* out, u64* whole) {
+  // is returned in *whole.  False: never.  `each` visits the CTA's tokens.
+  template <bool kAlone, typename Each>
+  __device__ __forceinline__ bool find(Each each, bool by_count, u64 level, float share, const Cut& from, Cut* out, u64* whole) {
     clear();
     if (by_count) {
       each([&](float x) {
@@ -268,8 +277,8 @@ struct Sampler {
     const u64 tie_sum = by_count ? from.ties : from.ties * from.weight;
     __syncthreads();
     if (rank == 0 && threadIdx.x == 0 && has_ties) s.g[tie_bin] += tie_sum;
-    if (has_ties) cluster_sync();  // before the others add to the same bin
-    const bool hit = crossing(level, share);
+    if (has_ties && !kAlone) cluster_sync();  // before the others add to the same bin
+    const bool hit = crossing<kAlone>(level, share);
     *whole = s.found[3];
     if (!hit) return false;
     if (share >= 0.0f) level = last_below(share, *whole);
@@ -279,8 +288,8 @@ struct Sampler {
     const float q_hi = -bin * (kSampReach / kSampBins) * 0.9999f + 1e-6f, q_lo = -(bin + 1) * (kSampReach / kSampBins) * 1.0001f - 1e-6f;
     uint32_t lo = 0xffffffffu, hi = 0u;
     each([&](float x) {
-      const float q = (x - top) * inv;
-      if (quick && !(q >= q_lo && q <= q_hi)) return;
+      const float q = (x - top) * scale * inv;
+      if (!(q >= q_lo && q <= q_hi)) return;
       if (!(x > from.x)) return;
       const float d = distance(x);
       if (bin_of(d) != bin || !weighs(d)) return;
@@ -295,8 +304,10 @@ struct Sampler {
     if ((threadIdx.x & 31) == 0) s.red[threadIdx.x >> 5][0] = lo, s.red[threadIdx.x >> 5][1] = hi;
     __syncthreads();
     for (int w = 0; w < kWarps; ++w) lo = min(lo, static_cast<uint32_t>(s.red[w][0])), hi = max(hi, static_cast<uint32_t>(s.red[w][1]));
-    all_gather(lo, hi);
-    for (int r = 0; r < cluster; ++r) lo = min(lo, static_cast<uint32_t>(slot(r, 0))), hi = max(hi, static_cast<uint32_t>(slot(r, 1)));
+    if constexpr (!kAlone) {
+      all_gather(lo, hi);
+      for (int r = 0; r < cluster; ++r) lo = min(lo, static_cast<uint32_t>(slot(r, 0))), hi = max(hi, static_cast<uint32_t>(slot(r, 1)));
+    }
     while (lo != hi) {
       const int shift = max(0, 32 - __clz(hi - lo) - 10);
       const float x_lo = order_value(lo), x_hi = order_value(hi);
@@ -314,8 +325,8 @@ struct Sampler {
       const bool tie_in = has_ties && from_key >= lo && from_key <= hi;
       __syncthreads();
       if (rank == 0 && threadIdx.x == 0 && tie_in) s.g[(hi - from_key) >> shift] += tie_sum;
-      if (tie_in) cluster_sync();
-      if (!crossing(level - before, -1.0f)) return false;  // (a bin holds its crossing)
+      if (tie_in && !kAlone) cluster_sync();
+      if (!crossing<kAlone>(level - before, -1.0f)) return false;  // (a bin holds its crossing)
       const uint32_t b = static_cast<uint32_t>(s.found[0]);
       before += s.found[1], sum = s.found[2];
       hi -= b << shift;
@@ -325,46 +336,109 @@ struct Sampler {
     out->x = order_value(lo);
     out->weight = weight(out->x);
     out->before = before;
-    out->ties = static_cast<uint32_t>(by_count ? sum : sum / out->weight);  // the caller keeps as many as fit
+    out->ties = static_cast<uint32_t>(by_count ? sum : sum / out->weight);  // find_cut keeps as many as fit
     return true;
+  }
+  // The cut of top_k (0: off), then of top_p.
+  template <bool kAlone, typename Each>
+  __device__ __forceinline__ Cut find_cut(Each each, int top_k, float top_p) {
+    Cut cut{}, c;  // below every logit
+    cut.x = -INFINITY;
+    u64 whole;
+    if (top_k > 0 && find<kAlone>(each, true, static_cast<u64>(top_k) - 1, -1.0f, cut, &c, &whole)) {
+      c.ties = min(c.ties, static_cast<uint32_t>(static_cast<u64>(top_k) - c.before));
+      cut = c;
+    }
+    const float share = fmaxf(top_p, 0.0f);
+    if (top_p < 1.0f && find<kAlone>(each, false, 0, share, cut, &c, &whole)) {
+      const u64 fit = (last_below(share, whole) - c.before) / c.weight + 1;
+      c.ties = static_cast<uint32_t>(min(static_cast<u64>(c.ties), fit));
+      cut = c;
+    }
+    return cut;
   }
 
   // ---- a few candidates ----
-  // Sorts s.list[0, n) of this CTA descending, n a power of two.
-  __device__ __forceinline__ void sort(int n) {
+  // Sorts the first n (a power of two) of a warp's 128 values descending: lane i holds places 4 i .. 4 i + 3.
+  __device__ __forceinline__ static void sort(u64 (&v)[4], int n) {
+    const int i0 = 4 * (threadIdx.x & 31);
+    // of a pair of places a < b, a takes the larger where (a & k) == 0
+    auto meet = [](u64& x, u64& y, bool larger_first) {
+      if ((x < y) == larger_first) {
+        const u64 z = x;
+        x = y, y = z;
+      }
+    };
+#pragma unroll 1
     for (int k = 2; k <= n; k <<= 1)
+#pragma unroll 1
       for (int j = k >> 1; j > 0; j >>= 1) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < n / 2; i += NT) {
-          const int a = 2 * i - (i & (j - 1)), b = a + j;  // a has bit j clear
-          const u64 x = s.list[a], y = s.list[b];
-          if ((x < y) == ((a & k) == 0)) s.list[a] = y, s.list[b] = x;
+        if (j >= 4) {
+          const bool take_max = ((i0 & k) == 0) == ((i0 & j) == 0);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const u64 other = __shfl_xor_sync(0xffffffffu, v[e], j >> 2);
+            v[e] = (v[e] < other) == take_max ? other : v[e];
+          }
+        } else if (j == 2) {
+          meet(v[0], v[2], (i0 & k) == 0);
+          meet(v[1], v[3], (i0 & k) == 0);
+        } else {
+          meet(v[0], v[1], (i0 & k) == 0);
+          meet(v[2], v[3], ((i0 + 2) & k) == 0);
         }
       }
-    __syncthreads();
   }
 
-  // A value that at least `want` of the CTA's tokens reach (-inf: not found): the want-th largest of the
-  // threads' maxima, its low bits dropped.
+  // A value that at least `want` of the CTA's tokens reach (-inf: not found), its low bits dropped.
   __device__ __forceinline__ float reached_by(int want, const float (&best)[4]) {
     uint32_t b[4], at = 0u;
 #pragma unroll
     for (int i = 0; i < 4; ++i) b[i] = order_bits(best[i]);
-    // 16 bits: exponent and 7 bits of the mantissa, all that bf16 has
-#pragma unroll 1
-    for (int bit = 31; bit >= 16; --bit) {
-      const uint32_t trial = at | (1u << bit);
-      int n = 0;
+    if (2 * want <= 4 * kWarps) {
+      // few: the want-th largest of the warps' four maxima each
 #pragma unroll
-      for (int i = 0; i < 4; ++i) n += b[i] >= trial;
-      n = __reduce_add_sync(0xffffffffu, n);
-      uint32_t* red = s.red32 + 16 * (bit & 1);  // (NT <= 512: 16 warps)
-      if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = n;
+      for (int i = 0; i < 4; ++i) b[i] = __reduce_max_sync(0xffffffffu, b[i]);
+      if ((threadIdx.x & 31) == 0)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) reinterpret_cast<uint32_t*>(s.list)[4 * (threadIdx.x >> 5) + i] = b[i];
       __syncthreads();
-      int all = 0;
+      // every warp ranks the 4 kWarps <= 64 values, two a lane, by (value, place)
+      const uint32_t* all = reinterpret_cast<const uint32_t*>(s.list);
+      const int lane = threadIdx.x & 31;
+      uint32_t found = 0u;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) all += red[w];
-      if (all >= want) at = trial;
+      for (int h = 0; h < (4 * kWarps + 31) / 32; ++h) {
+        const int place = lane + 32 * h;
+        const uint32_t mine = all[place];
+        int rank_of = 0;
+#pragma unroll 8
+        for (int i = 0; i < 4 * kWarps; ++i) rank_of += all[i] > mine || (all[i] == mine && i < place);
+        if (rank_of == want - 1) found = mine;
+      }
+      at = __reduce_max_sync(0xffffffffu, found);
+      __syncthreads();  // the list's place is used again
+    } else {
+      // the want-th largest of the threads' four, 16 bits (exponent and 7 of the mantissa: all that bf16
+      // has), two a round: a warp counts up to 128 for each of three trial values
+#pragma unroll 1
+      for (int bit = 30; bit >= 16; bit -= 2) {
+        uint32_t n = 0u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          n += (b[i] >= (at | 1u << bit) ? 1u : 0u) + (b[i] >= (at | 2u << bit) ? 1u << 8 : 0u) + (b[i] >= (at | 3u << bit) ? 1u << 16 : 0u);
+        n = __reduce_add_sync(0xffffffffu, n & 0x00ff00ffu) | __reduce_add_sync(0xffffffffu, n & 0x0000ff00u);
+        uint32_t* red = s.red32 + 16 * (bit >> 1 & 1);  // (NT <= 512: 16 warps)
+        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = n;
+        __syncthreads();
+        int n1 = 0, n2 = 0, n3 = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const uint32_t x = red[w];
+          n1 += x & 0xffu, n2 += x >> 8 & 0xffu, n3 += x >> 16;
+        }
+        at |= (n3 >= want ? 3u : n2 >= want ? 2u : n1 >= want ? 1u : 0u) << bit;
+      }
     }
     return at <= order_bits(-INFINITY) ? -INFINITY : order_value(at);
   }
@@ -387,70 +461,75 @@ struct Sampler {
       for (int v = threadIdx.x; v < nvec; v += NT) {
         float x[kVec];
         load(v, x);
+        bool any = false;
 #pragma unroll
-        for (int e = 0; e < kVec; ++e)
-          if (x[e] >= bound && x[e] > -INFINITY) {
-            st_cluster_u64(at, (static_cast<u64>(order_bits(x[e])) << 32) | static_cast<uint32_t>(~(first_id + v * kVec + e)));
-            at += 8;
-          }
+        for (int e = 0; e < kVec; ++e) any |= x[e] >= bound;
+        if (any) {
+#pragma unroll
+          for (int e = 0; e < kVec; ++e)
+            if (x[e] >= bound && x[e] > -INFINITY) {
+              st_cluster_u64(at, (static_cast<u64>(order_bits(x[e])) << 32) | static_cast<uint32_t>(~(first_id + v * kVec + e)));
+              at += 8;
+            }
+        }
       }
     }
     cluster_sync();
     return static_cast<int>(total);
   }
 
-  // The whole draw from rank 0's n candidates, which contain the first top_k tokens of positive weight.
+  // The whole draw by one warp from rank 0's n <= 128 candidates, which contain the first top_k tokens of
+  // positive weight.
   __device__ __forceinline__ void draw_from_list(const SampleParams& P, int r, int n, int top_k, float top_p, u64 least) {
-    int size = 2;
-    while (size < n) size <<= 1;
-    for (int i = n + threadIdx.x; i < size; i += NT) s.list[i] = 0;
-    if (threadIdx.x == 0) s.kept = 0u;
-    sort(size);
+    constexpr int kE = 4;
+    const int lane = threadIdx.x & 31, p0 = kE * lane;
+    auto power = [](int m) { return m <= 2 ? 2 : 1 << (32 - __clz(m - 1)); };
+    // inclusive sums in the order of places, and of all
+    auto scan = [&](u64 x, u64* all) {
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const u64 y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      *all = __shfl_sync(0xffffffffu, x, 31);
+      return x;
+    };
+    u64 v[kE], w[kE], sum = 0, whole;
+#pragma unroll
+    for (int e = 0; e < kE; ++e) v[e] = p0 + e < n ? s.list[p0 + e] : 0;
+    sort(v, power(n));
     n = min(n, top_k);
-    constexpr int kPer = kSampList / NT;  // consecutive places of the order a thread
-    const int p0 = kPer * threadIdx.x;
-    u64 w[kPer], sum = 0, none = 0, whole, other;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      w[i] = p0 + i < n ? weight(order_value(static_cast<uint32_t>(s.list[p0 + i] >> 32))) : 0;
-      sum += w[i];
+    for (int e = 0; e < kE; ++e) {
+      w[e] = p0 + e < n ? weight(order_value(static_cast<uint32_t>(v[e] >> 32))) : 0;
+      sum += w[e];
     }
-    u64 before = sum;
-    block_scan(before, none, &whole, &other);
-    before -= sum;
+    u64 before = scan(sum, &whole) - sum;
     const u64 level = top_p < 1.0f ? last_below(fmaxf(top_p, 0.0f), whole) : ~0ull;
-    uint32_t mine = 0;
-    u64 kept_sum = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      if (w[i] > 0 && before <= level && w[i] >= least) ++mine, kept_sum += w[i];
-      before += w[i];
-    }
-    mine = __reduce_add_sync(0xffffffffu, mine);
-    if ((threadIdx.x & 31) == 0) atomicAdd(&s.kept, mine);
-    kept_sum = block_sum(kept_sum);  // (its barriers also order s.kept)
-    const int kept = static_cast<int>(s.kept);  // a prefix of the order
-    // the kept ones by id
-    size = 2;
-    while (size < kept) size <<= 1;
-    for (int i = threadIdx.x; i < size; i += NT)
-      s.list[i] = i < kept ? (s.list[i] << 32) | (s.list[i] >> 32) : 0;  // ~id, ordered bits: descending is ascending id
-    sort(size);
+    u64 mine = 0, kept, kept_sum;  // the kept ones are a prefix of the order
     sum = 0;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      w[i] = p0 + i < kept ? weight(order_value(static_cast<uint32_t>(s.list[p0 + i]))) : 0;
-      sum += w[i];
+    for (int e = 0; e < kE; ++e) {
+      const bool keep = w[e] > 0 && before <= level && w[e] >= least;
+      before += w[e];
+      if (keep) ++mine, sum += w[e];
+      v[e] = keep ? (v[e] << 32) | (v[e] >> 32) : 0;  // ~id, ordered bits: descending is ascending id
     }
-    before = sum;
-    block_scan(before, none, &whole, &other);
-    before -= sum;
+    scan(mine, &kept);
+    scan(sum, &kept_sum);
+    sort(v, power(static_cast<int>(kept)));
+    sum = 0;
+#pragma unroll
+    for (int e = 0; e < kE; ++e) {
+      w[e] = p0 + e < static_cast<int>(kept) ? weight(order_value(static_cast<uint32_t>(v[e]))) : 0;
+      sum += w[e];
+    }
+    before = scan(sum, &whole) - sum;
     const u64 goal = goal_of(P.u[r], kept_sum);
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      if (before <= goal && goal < before + w[i])
-        write(P, r, static_cast<int>(~static_cast<uint32_t>(s.list[p0 + i] >> 32)), w[i], kept_sum, kept);
-      before += w[i];
+    for (int e = 0; e < kE; ++e) {
+      if (before <= goal && goal < before + w[e]) write(P, r, static_cast<int>(~static_cast<uint32_t>(v[e] >> 32)), w[e], kept_sum, kept);
+      before += w[e];
     }
   }
 
@@ -469,29 +548,34 @@ struct Sampler {
   __device__ __forceinline__ void draw_from_row(const SampleParams& P, int r, const Cut& cut, u64 least) {
     const u64 tie_weight = (cut.ties > 0 && cut.weight >= least) ? cut.weight : 0;
     const uint32_t ties = tie_weight ? cut.ties : 0;
-    // of one vector: weight and number of the kept tokens above the cut, number of those that equal it;
-    // most vectors have none where the cut is high
-    auto kept_of = [&](const float (&x)[kVec], u64 (&k)[kVec]) {
+    const uint32_t least32 = static_cast<uint32_t>(max(1ull, min(least, 0xffffffffull)));
+    // weights of one vector's kept tokens above the cut; most vectors have none where the cut is high
+    auto kept_of = [&](const float (&x)[kVec], uint32_t (&k)[kVec]) {
       bool any = false;
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) k[e] = 0, any |= x[e] > cut.x;
+      for (int e = 0; e < kVec; ++e) k[e] = 0u, any |= x[e] > cut.x;
       if (any) {
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
-          const u64 w = x[e] > cut.x ? weight(x[e]) : 0;
-          k[e] = w >= least ? w : 0;
+          const uint32_t t = weight32(distance(x[e]));
+          k[e] = x[e] > cut.x && t >= least32 ? t : 0u;
         }
       }
     };
     u64 sum = 0, num = 0;  // num: count above, and ties in the low half
+    uint32_t above = 0u, tied = 0u;
     for (int v = threadIdx.x; v < nvec; v += NT) {
       float x[kVec];
-      u64 k[kVec];
+      uint32_t k[kVec];
       load(v, x);
       kept_of(x, k);
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) sum += k[e], num += (k[e] > 0 ? 1ull << 32 : 0ull) + (x[e] == cut.x ? 1u : 0u);
+      for (int e = 0; e < kVec; ++e) sum += widen(k[e]), above += k[e] > 0u;
+      if (ties)
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) tied += x[e] == cut.x;
     }
+    num = (static_cast<u64>(above) << 32) | tied;
     sum = block_sum(sum);
     num = block_sum(num);
     all_gather(sum, num);
@@ -511,12 +595,13 @@ struct Sampler {
     for (int base = 0; base < nvec; base += NT) {
       const int v = base + threadIdx.x;
       float x[kVec];
-      u64 k[kVec], ws = 0, ts = 0, all_w, all_t;
+      uint32_t k[kVec];
+      u64 ws = 0, ts = 0, all_w, all_t;
       if (v < nvec) {
         load(v, x);
         kept_of(x, k);
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) ws += k[e], ts += x[e] == cut.x;
+        for (int e = 0; e < kVec; ++e) ws += widen(k[e]), ts += ties > 0u && x[e] == cut.x;
       }
       u64 wi = ws, ti = ts;
       block_scan(wi, ti, &all_w, &all_t);
@@ -525,11 +610,11 @@ struct Sampler {
         bool done = false;
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
-          const bool tie = x[e] == cut.x;
-          wi += k[e], ti += tie;
+          const bool tie = ties > 0u && x[e] == cut.x;
+          wi += widen(k[e]), ti += tie;
           if (!done && reach(wi, ti) > goal) {
             done = true;
-            write(P, r, first_id + v * kVec + e, tie ? tie_weight : k[e], whole, count);
+            write(P, r, first_id + v * kVec + e, tie ? tie_weight : widen(k[e]), whole, count);
           }
         }
       }
@@ -585,7 +670,7 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 1 : 4) sample_kernel(const __g
   // the list holds what the bound lets through, a little more than top_k
   const bool few = !greedy && top_k > 0 && top_k < P.vocab && top_k <= kSampList * 3 / 4;
   for (int i = threadIdx.x; i < kSampBins; i += NT) s.g[i] = 0;
-  Sampler<T, NT> S{s, vecs, nvec, first_id, rank, cluster, 0, 0.0f, 0.0f, 0.0f, false};
+  Sampler<T, NT> S{s, vecs, nvec, first_id, rank, cluster, 0, 0.0f, 0.0f, 0.0f, 1.0f};
   __syncthreads();  // the barrier is set up, the edges are written
   const bool ok = mbar_wait(&s.loaded, 0u, kErrSampleTimeout);
   // ---- maximum (NaN is passed over here and weighs nothing below) and, for a greedy row, its first id ----
@@ -641,35 +726,62 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 1 : 4) sample_kernel(const __g
     }
     return;  // nothing is written to another CTA after the last barrier: so at every return here
   }
-  S.temp = fmaxf(temp, 1e-30f);
+  if (S.top == INFINITY) {  // the infinite ones share the draw: as logits 0 and -inf
+    for (int v = threadIdx.x; v < nvec; v += NT) {
+      T* e = reinterpret_cast<T*>(vecs + v);
+#pragma unroll 1
+      for (int i = 0; i < kVec; ++i) e[i] = static_cast<T>(static_cast<float>(e[i]) == INFINITY ? 0.0f : -INFINITY);
+    }
+    __syncthreads();
+    S.top = 0.0f;
+    least_bound = order_bits(-INFINITY);
+  }
+  // temperatures of [1e-30, 3e38] at a scale where neither a quotient's remainder nor the reciprocal leaves
+  // the normal numbers
+  S.temp = fminf(fmaxf(temp, 1e-30f), 3e38f);
+  S.scale = S.temp < 1e-20f ? 18446744073709551616.0f : S.temp > 1e20f ? 5.4210108624275222e-20f : 1.0f;  // 2^64, 2^-64
+  S.temp *= S.scale;
   S.inv = __fdiv_rn(1.0f, S.temp);
-  S.quick = S.temp > 1e-20f && S.temp < 1e20f && S.top < INFINITY;
 
   // w >= min_p 2^32 for whole w
   const u64 least = static_cast<u64>(ceil(static_cast<double>(min_p > 0.0f ? fminf(min_p, 1.0f) : 0.0f) * 4294967296.0));
-  Cut cut{};  // below every logit
-  cut.x = -INFINITY;
-  u64 whole;
-  if (top_k > 0 && top_k < P.vocab) {
-    const int n = few ? S.gather_candidates(order_value(least_bound)) : -1;
-    if (n >= 0) {
-      if (rank == 0) S.draw_from_list(P, r, n, top_k, top_p, least);
-      return;
+  auto in_row = [&](auto f) { S.each(f); };
+  const int n = few ? S.gather_candidates(order_value(least_bound)) : -1;
+  Cut cut{};
+  if (n < 0) {
+    cut = S.template find_cut<false>(in_row, top_k < P.vocab ? top_k : 0, top_p);
+  } else if (n <= 128) {
+    if (rank == 0 && threadIdx.x < 32) S.draw_from_list(P, r, n, top_k, top_p, least);
+    return;
+  } else {
+    // rank 0 finds the cut among the candidates, a few in each thread's registers, and tells the others
+    if (rank == 0) {
+      constexpr int kE = kSampList / NT;
+      float x[kE];
+#pragma unroll
+      for (int e = 0; e < kE; ++e) {
+        const int i = threadIdx.x + e * NT;
+        x[e] = i < n ? order_value(static_cast<uint32_t>(s.list[i] >> 32)) : -INFINITY;
+      }
+      __syncthreads();
+      for (int i = threadIdx.x; i < kSampBins; i += NT) s.g[i] = 0;
+      cut = S.template find_cut<true>(
+          [&](auto f) {
+#pragma unroll
+            for (int e = 0; e < kE; ++e) f(x[e]);
+          },
+          top_k, top_p);
+      if (threadIdx.x < cluster) {
+        const uint32_t at = mapa_shared(smem_u32(s.found), threadIdx.x);
+        st_cluster_u64(at, __float_as_uint(cut.x));
+        st_cluster_u64(at + 8, cut.ties);
+        st_cluster_u64(at + 16, cut.weight);
+      }
     }
-    Cut c;
-    if (S.find(true, static_cast<u64>(top_k) - 1, -1.0f, cut, &c, &whole)) {
-      c.ties = min(c.ties, static_cast<uint32_t>(static_cast<u64>(top_k) - c.before));
-      cut = c;
-    }
-  }
-  if (top_p < 1.0f) {
-    const float share = fmaxf(top_p, 0.0f);
-    Cut c;
-    if (S.find(false, 0, share, cut, &c, &whole)) {
-      const u64 fit = (Sampler<T, NT>::last_below(share, whole) - c.before) / c.weight + 1;
-      c.ties = static_cast<uint32_t>(min(static_cast<u64>(c.ties), fit));
-      cut = c;
-    }
+    cluster_sync();
+    cut.x = __uint_as_float(static_cast<uint32_t>(s.found[0]));
+    cut.ties = static_cast<uint32_t>(s.found[1]);
+    cut.weight = s.found[2];
   }
   S.draw_from_row(P, r, cut, least);
 }
