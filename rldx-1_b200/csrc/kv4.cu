@@ -55,18 +55,15 @@ __device__ __forceinline__ int seq_of_row(const int* cu, int seqs, int row) {
 
 constexpr int kKv4SmemSeqs = 1024;  // batches up to this size keep cu and lengths in shared memory
 
-// Unit of the cache (start, or null) and token in the unit of new-token row `row`.
-__device__ __forceinline__ uint8_t* kv4_token_unit(const Kv4Cache& c, const int* cu, const int* lengths, int row,
-                                                   int head, int unit_bytes, int* tau) {
+// Where new-token row `row` stands in the cache: index of its unit for head 0 (-1: nowhere, recorded) and
+// its token in the unit; head h's unit is units_per_page h further.
+__device__ __forceinline__ int kv4_token_place(const Kv4Cache& c, const int* cu, const int* lengths, int row, int* tau) {
   const int b = seq_of_row(cu, c.seqs, row);
   const int pos = lengths[b] - cu[b + 1] + row;
   *tau = pos & (kKv4Unit - 1);
-  const int index = pos >= 0 ? kv4_unit_index(c, b, head, pos / kKv4Unit) : -1;
-  if (index < 0) {
-    record_error(kErrKv4Table);
-    return nullptr;
-  }
-  return c.data + static_cast<long long>(index) * unit_bytes;
+  const int index = pos >= 0 ? kv4_unit_index(c, b, 0, pos / kKv4Unit) : -1;
+  if (index < 0) record_error(kErrKv4Table);
+  return index;
 }
 
 // Copies cu and lengths to shared memory where they fit and returns where to read them.
@@ -81,118 +78,154 @@ __device__ __forceinline__ void stage_seqs(const Kv4Cache& c, int* smem, const i
   }
 }
 
-// D / 8 lanes own a (token, head) row, 8 channels each; kRows rows per lane group, their loads
-// issued before any arithmetic.  Heads of a token are ordered [q | k | v].
-template <int D, int kRows, typename Rope>
-__global__ void __launch_bounds__(128) kv4_append_kernel(const __grid_constant__ Kv4AppendParams P) {
+__device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8]) {
+  unpack_bf16x2(u.x, v[0], v[1]);
+  unpack_bf16x2(u.y, v[2], v[3]);
+  unpack_bf16x2(u.z, v[4], v[5]);
+  unpack_bf16x2(u.w, v[6], v[7]);
+}
+
+// kN heads of one token, D / 8 lanes with 8 channels of each: v = rope(rms(v) w).  c, s: this lane's part
+// of the rotation's row, s with the sign of rotate_half = cat(-x2, x1).  The heads' steps are
+// independent of one another, so their shuffles overlap.
+template <int D, int kN>
+__device__ __forceinline__ void norm_rope(float (&v)[kN][8], const float (&w)[8], const float (&c)[8], const float (&s)[8],
+                                          float eps) {
+  constexpr int kLanes = D / 8;
+  float ss[kN];
+#pragma unroll
+  for (int r = 0; r < kN; ++r) {
+    ss[r] = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss[r] = fmaf(v[r][e], v[r][e], ss[r]);
+  }
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int r = 0; r < kN; ++r) ss[r] += __shfl_xor_sync(0xffffffffu, ss[r], o);
+#pragma unroll
+  for (int r = 0; r < kN; ++r) {
+    const float rstd = rsqrtf(ss[r] * (1.0f / D) + eps);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float y = __fmul_rn(__fmul_rn(v[r][e], rstd), w[e]);
+      const float o = __shfl_xor_sync(0xffffffffu, y, kLanes / 2);  // the channel half a head away
+      v[r][e] = __fadd_rn(__fmul_rn(y, c[e]), __fmul_rn(o, s[e]));
+    }
+  }
+}
+
+// Codes of this lane's 8 channels (lowest first), and scale and low of the group that four lanes share.
+__device__ __forceinline__ uint32_t quantise8(const float (&v)[8], __half* scale_h, __half* low_h) {
+  float mn = v[0], mx = v[0];
+#pragma unroll
+  for (int e = 1; e < 8; ++e) mn = min_nan(mn, v[e]), mx = max_nan(mx, v[e]);
+#pragma unroll
+  for (int o = 1; o <= 2; o <<= 1) {
+    mn = min_nan(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+    mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  }
+  mn = max_nan(min_nan(mn, 65504.0f), -65504.0f);
+  mx = max_nan(min_nan(mx, 65504.0f), -65504.0f);
+  *low_h = __float2half_rn(mn);
+  *scale_h = __float2half_rn(__fmul_rn(mx - mn, 1.0f / 15.0f));
+  const float low = __half2float(*low_h), scale = __half2float(*scale_h);
+  const float inv = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
+  uint32_t codes = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float q = fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(v[e], low), inv)), 0.0f), 15.0f);  // NaN: 0
+    codes |= static_cast<uint32_t>(q) << (4 * e);
+  }
+  return codes;
+}
+
+// D / 8 lanes own an item: four query heads of a token, or (blocks from q_blocks on) k and v of one kv
+// head.  The rotation's row is read once for an item, all loads are issued before any arithmetic, and
+// every block runs straight-line code of one kind.
+constexpr int kAppendHeads = 4;
+
+template <int D, typename Rope>
+__global__ void __launch_bounds__(128) kv4_append_kernel(const __grid_constant__ Kv4AppendParams P, unsigned q_blocks) {
   using U = Kv4Unit<D>;
   constexpr int kLanes = D / 8;
   __shared__ int s_seq[2 * kKv4SmemSeqs + 1];
   griddep_wait();
-  const int hq = P.q_heads, hkv = P.c.kv_heads, heads = hq + 2 * hkv;
-  const long long nrows = static_cast<long long>(P.c.tokens) * heads;
-  const long long group = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) / kLanes;
-  const int l = threadIdx.x % kLanes;
-  const long long row0 = group * kRows;
-  float x[kRows][8];
-  int tok[kRows], head[kRows], rp[kRows];
+  const int hq = P.q_heads, hkv = P.c.kv_heads, l = threadIdx.x % kLanes;
+  const bool of_q = blockIdx.x < q_blocks;
+  const unsigned item = ((of_q ? blockIdx.x : blockIdx.x - q_blocks) * 128u + threadIdx.x) / kLanes;
+  const unsigned per_token = of_q ? (hq + kAppendHeads - 1) / kAppendHeads : hkv;
+  const bool live = item < static_cast<unsigned>(P.c.tokens) * per_token;  // (an item past the end repeats the last token)
+  const int tok = live ? static_cast<int>(item / per_token) : P.c.tokens - 1;
+  const int at = static_cast<int>(item % per_token);
+  const __nv_bfloat16* src = P.qkv + tok * P.ld + 8 * l;
+  int rp = __ldg(P.rope_pos + tok);
+  float w[8], c[8], s[8];
+  load8((of_q ? P.wq : P.wk) + 8 * l, w);
+  auto rotation = [&] {
+    if (static_cast<unsigned>(rp) >= static_cast<unsigned>(P.rope_rows)) {
+      if (live) record_error(kErrKv4Rope);
+      rp = 0;
+    }
+    load8(static_cast<const Rope*>(P.cos) + static_cast<long long>(rp) * D + 8 * l, c);
+    load8(static_cast<const Rope*>(P.sin) + static_cast<long long>(rp) * D + 8 * l, s);
+    if (l < kLanes / 2)
 #pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    const long long row = min(row0 + r, nrows - 1);  // clamped: rows past the end are not stored
-    tok[r] = static_cast<int>(row / heads);
-    head[r] = static_cast<int>(row - static_cast<long long>(tok[r]) * heads);
-    load8(P.qkv + tok[r] * P.ld + head[r] * D + 8 * l, x[r]);
-    rp[r] = __ldg(P.rope_pos + tok[r]);
+      for (int e = 0; e < 8; ++e) s[e] = -s[e];
+  };
+  if (of_q) {
+    uint4 x[kAppendHeads];
+    float v[kAppendHeads][8];
+    const int h0 = at * kAppendHeads;
+#pragma unroll
+    for (int r = 0; r < kAppendHeads; ++r) x[r] = __ldcs(reinterpret_cast<const uint4*>(src + min(h0 + r, hq - 1) * D));
+    rotation();
+    griddep_launch();
+#pragma unroll
+    for (int r = 0; r < kAppendHeads; ++r) unpack8(x[r], v[r]);
+    norm_rope<D, kAppendHeads>(v, w, c, s, P.eps);
+#pragma unroll
+    for (int r = 0; r < kAppendHeads; ++r)
+      if (live && h0 + r < hq) {
+        uint4 u;
+        u.x = pack_bf16x2(v[r][0], v[r][1]);
+        u.y = pack_bf16x2(v[r][2], v[r][3]);
+        u.z = pack_bf16x2(v[r][4], v[r][5]);
+        u.w = pack_bf16x2(v[r][6], v[r][7]);
+        *reinterpret_cast<uint4*>(P.q + (static_cast<long long>(tok) * hq + h0 + r) * D + 8 * l) = u;
+      }
+    return;
   }
-  const int *cu, *lengths;
+  const uint4 xk = __ldcs(reinterpret_cast<const uint4*>(src + (hq + at) * D));
+  const uint4 xv = __ldcs(reinterpret_cast<const uint4*>(src + (hq + hkv + at) * D));
+  const int *cu = P.c.cu, *lengths = P.c.lengths;
   stage_seqs(P.c, s_seq, &cu, &lengths);
+  rotation();
   __syncthreads();
   griddep_launch();
-#pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    const bool live = row0 + r < nrows;
-    const bool is_v = head[r] >= hq + hkv;
-    if (!is_v) {
-      float ss = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(x[r][e], x[r][e], ss);
-      // rows of one warp may be q / k in one lane group and v in another: the mask names the group
-      const unsigned lanes = (kLanes == 16 ? 0xffffu : 0xffu) << ((threadIdx.x & 31) / kLanes * kLanes);
-#pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(lanes, ss, o);
-      const float rstd = rsqrtf(ss * (1.0f / D) + P.eps);
-      float w[8], c[8], s[8];
-      load8((head[r] < hq ? P.wq : P.wk) + 8 * l, w);
-      if (static_cast<unsigned>(rp[r]) >= static_cast<unsigned>(P.rope_rows)) {
-        if (live) record_error(kErrKv4Rope);
-        rp[r] = 0;
-      }
-      load8(static_cast<const Rope*>(P.cos) + static_cast<long long>(rp[r]) * D + 8 * l, c);
-      load8(static_cast<const Rope*>(P.sin) + static_cast<long long>(rp[r]) * D + 8 * l, s);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float y = __fmul_rn(__fmul_rn(x[r][e], rstd), w[e]);
-        const float o = __shfl_xor_sync(lanes, y, kLanes / 2);  // the channel half a head away
-        x[r][e] = __fadd_rn(__fmul_rn(y, c[e]), __fmul_rn(l < kLanes / 2 ? -o : o, s[e]));
-      }
-    }
-    if (head[r] < hq) {
-      if (live) {
-        uint4 u;
-        u.x = pack_bf16x2(x[r][0], x[r][1]);
-        u.y = pack_bf16x2(x[r][2], x[r][3]);
-        u.z = pack_bf16x2(x[r][4], x[r][5]);
-        u.w = pack_bf16x2(x[r][6], x[r][7]);
-        *reinterpret_cast<uint4*>(P.q + (static_cast<long long>(tok[r]) * hq + head[r]) * D + 8 * l) = u;
-      }
-      continue;
-    }
-    // four lanes share a group of 32 channels
-    const unsigned quad = 0xfu << (threadIdx.x & 28);
-    float mn = x[r][0], mx = x[r][0];
-#pragma unroll
-    for (int e = 1; e < 8; ++e) mn = min_nan(mn, x[r][e]), mx = max_nan(mx, x[r][e]);
-#pragma unroll
-    for (int o = 1; o <= 2; o <<= 1) {
-      mn = min_nan(mn, __shfl_xor_sync(quad, mn, o));
-      mx = max_nan(mx, __shfl_xor_sync(quad, mx, o));
-    }
-    mn = max_nan(min_nan(mn, 65504.0f), -65504.0f);
-    mx = max_nan(min_nan(mx, 65504.0f), -65504.0f);
-    const __half low_h = __float2half_rn(mn);
-    const __half scale_h = __float2half_rn(__fmul_rn(mx - mn, 1.0f / 15.0f));
-    const float low = __half2float(low_h), scale = __half2float(scale_h);
-    const float inv = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
-    uint32_t codes = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float c = fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(x[r][e], low), inv)), 0.0f), 15.0f);  // NaN: 0
-      codes |= static_cast<uint32_t>(c) << (4 * e);
-    }
-    if (!live) continue;
-    const int h = head[r] - hq - (is_v ? hkv : 0);
-    int tau;
-    uint8_t* unit = kv4_token_unit(P.c, cu, lengths, tok[r], h, U::kBytes, &tau);
-    if (unit == nullptr) continue;
-    const int j = l / 4, t4 = l % 4;  // group, position in the group
-    if (!is_v) {
-      *reinterpret_cast<uint32_t*>(unit + tau * U::kRow + 4 * (t4 * U::kG + j)) = codes;
-      if (t4 == 0) {
-        __half* meta = reinterpret_cast<__half*>(unit + U::kKMeta + 4 * U::kG * tau);
-        meta[j] = scale_h;
-        meta[U::kG + j] = low_h;
-      }
-    } else {
-      const int blk = tau / 16, hh = tau / 8 % 2, t = tau / 2 % 4, e = tau % 2;
-      uint8_t* at = unit + U::kV + 8 * D * blk + 4 * D * hh + 4 * U::kG * t + 2 * U::kG * e + 2 * j;
-      *reinterpret_cast<uint16_t*>(at + 16 * U::kG * (2 * t4)) = static_cast<uint16_t>(codes);
-      *reinterpret_cast<uint16_t*>(at + 16 * U::kG * (2 * t4 + 1)) = static_cast<uint16_t>(codes >> 16);
-      if (t4 == 0) {
-        const int m = 32 * U::kG * blk + 16 * U::kG * hh + 4 * U::kG * t + 4 * j + 2 * e;
-        *reinterpret_cast<__half*>(unit + U::kVScale + m) = scale_h;
-        *reinterpret_cast<__half*>(unit + U::kVLow + m) = low_h;
-      }
-    }
+  int tau = 0;
+  const int place = live ? kv4_token_place(P.c, cu, lengths, tok, &tau) : -1;
+  float k[1][8], v[8];
+  unpack8(xk, k[0]);
+  unpack8(xv, v);
+  norm_rope<D, 1>(k, w, c, s, P.eps);
+  __half k_scale, k_low, v_scale, v_low;
+  const uint32_t kc = quantise8(k[0], &k_scale, &k_low), vc = quantise8(v, &v_scale, &v_low);
+  if (place < 0) return;
+  uint8_t* unit = P.c.data + static_cast<long long>(place + at * P.c.units_per_page) * U::kBytes;
+  const int j = l / 4, t4 = l % 4;  // group, position in the group
+  const int blk = tau / 16, hh = tau / 8 % 2, t = tau / 2 % 4, e = tau % 2;
+  *reinterpret_cast<uint32_t*>(unit + tau * U::kRow + 4 * (t4 * U::kG + j)) = kc;
+  uint8_t* va = unit + U::kV + 8 * D * blk + 4 * D * hh + 4 * U::kG * t + 2 * U::kG * e + 2 * j;
+  *reinterpret_cast<uint16_t*>(va + 16 * U::kG * (2 * t4)) = static_cast<uint16_t>(vc);
+  *reinterpret_cast<uint16_t*>(va + 16 * U::kG * (2 * t4 + 1)) = static_cast<uint16_t>(vc >> 16);
+  if (t4 == 0) {
+    __half* meta = reinterpret_cast<__half*>(unit + U::kKMeta + 4 * U::kG * tau);
+    meta[j] = k_scale;
+    meta[U::kG + j] = k_low;
+    const int m = 32 * U::kG * blk + 16 * U::kG * hh + 4 * U::kG * t + 4 * j + 2 * e;
+    *reinterpret_cast<__half*>(unit + U::kVScale + m) = v_scale;
+    *reinterpret_cast<__half*>(unit + U::kVLow + m) = v_low;
   }
 }
 
@@ -215,9 +248,10 @@ __global__ void __launch_bounds__(128) kv4_read_kernel(const __grid_constant__ K
   const bool is_v = which >= hkv;
   const int h = is_v ? which - hkv : which;
   int tau;
-  const uint8_t* unit = kv4_token_unit(P.c, cu, lengths, tok, h, U::kBytes, &tau);
+  const int place = kv4_token_place(P.c, cu, lengths, tok, &tau);
   uint4 o = make_uint4(0u, 0u, 0u, 0u);
-  if (unit != nullptr) {
+  if (place >= 0) {
+    const uint8_t* unit = P.c.data + static_cast<long long>(place + h * P.c.units_per_page) * U::kBytes;
     uint32_t codes;
     float scale, low;
     if (!is_v) {
@@ -247,10 +281,10 @@ __global__ void __launch_bounds__(128) kv4_read_kernel(const __grid_constant__ K
 }
 
 namespace {
-template <typename Params>
-cudaError_t launch_rows(void (*kernel)(Params), const Params& p, long long groups, int lanes, cudaStream_t stream) {
+template <typename... Args>
+cudaError_t launch_blocks(void (*kernel)(Args...), unsigned blocks, cudaStream_t stream, Args... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((groups * lanes + 127) / 128), 1, 1);
+  cfg.gridDim = dim3(blocks, 1, 1);
   cfg.blockDim = dim3(128, 1, 1);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -258,26 +292,28 @@ cudaError_t launch_rows(void (*kernel)(Params), const Params& p, long long group
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, p);
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
+// blocks of 128 threads for `items` of `lanes` threads
+unsigned blocks_of(long long items, int lanes) { return static_cast<unsigned>((items * lanes + 127) / 128); }
 
-template <int D, int kRows>
-cudaError_t launch_append(const Kv4AppendParams& p, long long rows, cudaStream_t stream) {
-  const long long groups = (rows + kRows - 1) / kRows;
-  return p.rope_f32 ? launch_rows<Kv4AppendParams>(kv4_append_kernel<D, kRows, float>, p, groups, D / 8, stream)
-                    : launch_rows<Kv4AppendParams>(kv4_append_kernel<D, kRows, __nv_bfloat16>, p, groups, D / 8, stream);
+template <int D>
+cudaError_t launch_append(const Kv4AppendParams& p, cudaStream_t stream) {
+  const unsigned q_blocks = blocks_of(static_cast<long long>(p.c.tokens) * ((p.q_heads + kAppendHeads - 1) / kAppendHeads), D / 8);
+  const unsigned kv_blocks = blocks_of(static_cast<long long>(p.c.tokens) * p.c.kv_heads, D / 8);
+  return p.rope_f32 ? launch_blocks<Kv4AppendParams, unsigned>(kv4_append_kernel<D, float>, q_blocks + kv_blocks, stream, p, q_blocks)
+                    : launch_blocks<Kv4AppendParams, unsigned>(kv4_append_kernel<D, __nv_bfloat16>, q_blocks + kv_blocks, stream, p, q_blocks);
 }
 }  // namespace
 
 cudaError_t launch_kv4_append(const Kv4AppendParams& p, int head_dim, cudaStream_t stream) {
-  const long long rows = static_cast<long long>(p.c.tokens) * (p.q_heads + 2 * p.c.kv_heads);
-  return head_dim == 128 ? launch_append<128, 1>(p, rows, stream) : launch_append<64, 1>(p, rows, stream);
+  return head_dim == 128 ? launch_append<128>(p, stream) : launch_append<64>(p, stream);
 }
 
 cudaError_t launch_kv4_read(const Kv4ReadParams& p, int head_dim, cudaStream_t stream) {
-  const long long rows = static_cast<long long>(p.c.tokens) * p.c.kv_heads * 2;
-  return head_dim == 128 ? launch_rows<Kv4ReadParams>(kv4_read_kernel<128>, p, rows, 16, stream)
-                         : launch_rows<Kv4ReadParams>(kv4_read_kernel<64>, p, rows, 8, stream);
+  const unsigned blocks = blocks_of(static_cast<long long>(p.c.tokens) * p.c.kv_heads * 2, head_dim / 8);
+  return head_dim == 128 ? launch_blocks<Kv4ReadParams>(kv4_read_kernel<128>, blocks, stream, p)
+                         : launch_blocks<Kv4ReadParams>(kv4_read_kernel<64>, blocks, stream, p);
 }
 
 namespace {
@@ -337,7 +373,7 @@ int rldx_kv4_append(const rldx_kv4_cache* cache, const void* qkv, int64_t ld, in
   if (rope_rows <= 0) return set_error(RLDX_ERR_ARG, "kv4_append: empty RoPE table");
   for (const void* x : {qkv, q_norm, k_norm, rope_cos, rope_sin, static_cast<const void*>(q_out)})
     if (!aligned_to(x, 16)) return set_error(RLDX_ERR_ARG, "kv4_append: pointers must be 16-byte aligned");
-  if (static_cast<long long>(tokens) * (q_heads + 2 * cache->kv_heads) >= (1LL << 31))
+  if (static_cast<long long>(tokens) * (q_heads + 2 * cache->kv_heads) >= (1LL << 27))
     return set_error(RLDX_ERR_UNSUPPORTED, "kv4_append: too many rows");
   if (tokens == 0) return RLDX_OK;
   p.qkv = static_cast<const __nv_bfloat16*>(qkv);
