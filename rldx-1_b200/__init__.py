@@ -7,6 +7,8 @@ VLM-backbone prefill and memory module that feed them in batched serving.
   rldx_b200.llm.B200LLMChain                    drop-in for CustomLLMChain (Qwen3 decoder prefill)
   rldx_b200.llm.B200MemoryChain                 drop-in for CustomMemoryChain (TransformerMemory)
   rldx_b200.llm.B200MemoryCache                 GraphSafeVLA's memory window + _process_memory
+  rldx_b200.decoder.B200TextDecoder            token decoding with the backbone's layers over a 4-bit cache
+  rldx_b200.decoder.B200KV4Cache               its pages, table and lengths
   rldx_b200.serve.apply_optimization            installs the native head behind model.get_action
   rldx_b200.torch_ops                           torch.ops.b200msat.* (the reference's ds::/ss:: ops)
   rldx_b200.ops                                 per-kernel wrappers (tests, op-level use)

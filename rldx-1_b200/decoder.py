@@ -1,0 +1,229 @@
+"""Text decoding with the VLM backbone's layers over a 4-bit key / value cache.
+
+The backbone chains (`rldx_b200.llm`) prefill a fixed sequence; this module keeps the keys and values
+and produces tokens, one path through the decoding operators of `rldx_b200.ops`:
+
+    n = rmsnorm(h); qkv = n Wqkv^T
+    q = qkv_rope_append(qkv, ...)      per-head norms, rotation, 4-bit write into the cache
+    a = kv4_attention(q, cache, ...)   over the whole sequence, or a sliding window and sinks
+    h = h + a Wo^T; h = h + swiglu(rmsnorm(h) [Wg; Wu]^T) Wd^T
+    token = sample(logits of the last rows, u, temperature, top_k, top_p, min_p)
+
+    cache = B200KV4Cache(layers, kv_heads, head_dim, seqs=4, max_tokens=4096)
+    decoder = B200TextDecoder(decoder_layers, norm, embed, lm_head, cos, sin)
+    out = decoder.generate(prompts, 64, cache=cache, u=torch.rand(64, 4), temperature=0.7, top_p=0.9)
+
+`decoder_layers` are Qwen3 text decoder layers (the attribute names that B200LLMChain takes), `cos` and
+`sin` their RoPE tables [positions, head_dim].  `python -m rldx_b200.decoder` decodes with random
+weights.
+"""
+
+from __future__ import annotations
+
+import argparse
+import ctypes as C
+from typing import Optional, Sequence
+
+import torch
+
+from . import _lib, ops
+from .llm import _raw_layer
+
+BF = torch.bfloat16
+
+
+class B200KV4Cache:
+    """Pages of the 4-bit cache of `layers` layers for `seqs` sequences: a pool per layer, one page
+    table, the lengths, and the list of free pages (on the host).  `max_tokens` bounds all
+    sequences together, rounded up to pages."""
+
+    def __init__(self, layers: int, kv_heads: int, head_dim: int, seqs: int, max_tokens: int, page_size: int = 64,
+                 device="cuda"):
+        if layers <= 0 or seqs <= 0 or max_tokens <= 0:
+            raise ValueError("layers, seqs and max_tokens must be positive")
+        self.page_size, self.seqs = int(page_size), int(seqs)
+        self.pages = -(-int(max_tokens) // self.page_size) + seqs  # a sequence's last page may be part empty
+        self.device = torch.device(device)
+        self.pools = [ops.kv4_cache(self.pages, kv_heads, head_dim, page_size, device=self.device) for _ in range(layers)]
+        self.table = torch.full((seqs, self.pages), -1, dtype=torch.int32, device=self.device)
+        self.lengths = torch.zeros(seqs, dtype=torch.int32, device=self.device)
+        self.tokens = [0] * seqs  # host copies
+        self._held = [[] for _ in range(seqs)]
+        self._free = list(range(self.pages - 1, -1, -1))
+
+    @property
+    def free_tokens(self) -> int:
+        return len(self._free) * self.page_size
+
+    def extend(self, new: Sequence[int]) -> None:
+        """Makes room for new[s] more tokens of each sequence: lengths and pages cover them after."""
+        if len(new) != self.seqs or any(n < 0 for n in new):
+            raise ValueError(f"new must give a count for each of the {self.seqs} sequences")
+        need = [-(-(t + n) // self.page_size) - len(h) for t, n, h in zip(self.tokens, new, self._held)]
+        if sum(need) > len(self._free):
+            raise RuntimeError(f"the cache has {len(self._free)} free pages, {sum(need)} are needed")
+        seq, col, page = [], [], []
+        for s, n in enumerate(need):
+            for _ in range(n):
+                seq.append(s)
+                col.append(len(self._held[s]))
+                page.append(self._free.pop())
+                self._held[s].append(page[-1])
+        if page:
+            at = torch.tensor([seq, col, page], device=self.device)
+            self.table[at[0], at[1]] = at[2].to(torch.int32)
+        self.tokens = [t + n for t, n in zip(self.tokens, new)]
+        self.lengths.copy_(torch.tensor(self.tokens, dtype=torch.int32))
+
+    def release(self, seq: int) -> None:
+        """Forgets a sequence; its pages are free again."""
+        self._free.extend(reversed(self._held[seq]))
+        self._held[seq] = []
+        self.tokens[seq] = 0
+        self.table[seq] = -1
+        self.lengths[seq] = 0
+
+
+class B200TextDecoder:
+    """Qwen3 decoder layers, embedding and output projection over a B200KV4Cache."""
+
+    def __init__(self, layers, norm, embed: torch.Tensor, lm_head: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *,
+                 window: int = 0, sinks: int = 0, device=None):
+        self.device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+        layers = [_raw_layer(layer) for layer in layers]
+        a0 = layers[0].self_attn
+        self.head_dim = a0.q_norm.weight.shape[0]
+        self.q_heads = a0.q_proj.weight.shape[0] // self.head_dim
+        self.kv_heads = a0.k_proj.weight.shape[0] // self.head_dim
+        self.hidden = embed.shape[1]
+        self.window, self.sinks = int(window), int(sinks)
+        ln = layers[0].input_layernorm
+        self.eps = float(getattr(ln, "variance_epsilon", getattr(ln, "eps", 1e-6)))
+
+        def put(*w):
+            return torch.cat([t.detach() for t in w]).to(self.device, BF).contiguous()
+
+        self.layers = [dict(norm1=put(m.input_layernorm.weight), norm2=put(m.post_attention_layernorm.weight),
+                            qkv=put(m.self_attn.q_proj.weight, m.self_attn.k_proj.weight, m.self_attn.v_proj.weight),
+                            q_norm=put(m.self_attn.q_norm.weight), k_norm=put(m.self_attn.k_norm.weight),
+                            o=put(m.self_attn.o_proj.weight), gate_up=put(m.mlp.gate_proj.weight, m.mlp.up_proj.weight),
+                            down=put(m.mlp.down_proj.weight)) for m in layers]
+        self.norm, self.embed, self.lm_head = put(norm.weight), put(embed), put(lm_head)
+        self.cos, self.sin = (t.detach().to(self.device).contiguous() for t in (cos, sin))
+
+    def new_cache(self, seqs: int, max_tokens: int, page_size: int = 64) -> B200KV4Cache:
+        return B200KV4Cache(len(self.layers), self.kv_heads, self.head_dim, seqs, max_tokens, page_size, self.device)
+
+    def _rmsnorm(self, x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
+        out = torch.empty_like(x)
+        seg = _lib.ResLnSegment(x.data_ptr(), None, None, None, None, out.data_ptr(), x.shape[0], x.shape[1], x.stride(0),
+                                weight.data_ptr())
+        _lib.check(_lib.load().rldx_res_rmsnorm(C.byref(seg), 1, self.eps, C.c_void_p(torch.cuda.current_stream().cuda_stream)))
+        return out
+
+    def forward(self, hidden: torch.Tensor, cache: B200KV4Cache, new: Sequence[int],
+                positions: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Runs the rows `hidden` [sum(new), hidden] (the new tokens of every sequence, in order)
+        through the layers; keys and values join the cache.  positions [sum(new)]: RoPE rows, the
+        tokens' places in their sequences by default.  Returns logits [seqs with new tokens, vocab]
+        of each sequence's last new token."""
+        if hidden.shape != (sum(new), self.hidden) or hidden.dtype != BF:
+            raise ValueError(f"hidden must be bfloat16 [{sum(new)}, {self.hidden}], got {hidden.dtype} {tuple(hidden.shape)}")
+        start = list(cache.tokens)
+        cache.extend(new)
+        if positions is None:
+            if max(cache.tokens) > self.cos.shape[0]:
+                raise ValueError(f"a sequence of {max(cache.tokens)} tokens is longer than the RoPE tables ({self.cos.shape[0]})")
+            positions = torch.cat([torch.arange(s, s + n, dtype=torch.int32) for s, n in zip(start, new)])
+        positions = positions.to(self.device, torch.int32)
+        cu = torch.tensor([0, *new], dtype=torch.int32).cumsum(0).to(torch.int32).to(self.device)
+        max_new, max_len = max(new), max(cache.tokens)
+        h = hidden
+        for w, pool in zip(self.layers, cache.pools):
+            qkv = ops.linear(self._rmsnorm(h, w["norm1"]), w["qkv"])
+            q = ops.qkv_rope_append(qkv, w["q_norm"], w["k_norm"], self.cos, self.sin, positions, pool, cache.table,
+                                    cache.lengths, cu, q_heads=self.q_heads, eps=self.eps)
+            a = ops.kv4_attention(q, pool, cache.table, cache.lengths, cu, max_new=max_new, max_len=max_len,
+                                  window=self.window, sinks=self.sinks)
+            h = ops.linear(a.flatten(1), w["o"], add=h)
+            gate, up = ops.linear(self._rmsnorm(h, w["norm2"]), w["gate_up"]).chunk(2, 1)
+            h = ops.linear(ops.swiglu(gate, up), w["down"], add=h)
+        last = torch.tensor([e - 1 for n, e in zip(new, torch.tensor(new).cumsum(0).tolist()) if n], device=self.device)
+        return ops.linear(self._rmsnorm(h[last].contiguous(), self.norm), self.lm_head)
+
+    def generate(self, prompts, max_new_tokens: int, *, u: torch.Tensor, cache: Optional[B200KV4Cache] = None,
+                 temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, stop_ids: Sequence[int] = ()):
+        """Appends max_new_tokens tokens to each of the prompts (lists of ids, or rows [n, hidden] of
+        embeddings that a vision tower has filled in).  u [max_new_tokens, prompts] are the draws'
+        numbers in [0, 1).  Returns a list of id lists; a sequence ends after one of stop_ids."""
+        n = len(prompts)
+        if tuple(u.shape) != (max_new_tokens, n):
+            raise ValueError(f"u must be [{max_new_tokens}, {n}], got {tuple(u.shape)}")
+        rows = [self.embed[torch.as_tensor(p, device=self.device)] if not torch.is_tensor(p) or p.dim() == 1 else
+                p.to(self.device, BF) for p in prompts]
+        cache = cache or self.new_cache(n, sum(r.shape[0] for r in rows) + n * max_new_tokens)
+        u = u.to(self.device, torch.float32).contiguous()
+
+        def full(v, dtype):
+            return torch.full((n,), v, dtype=dtype, device=self.device)
+
+        limits = dict(temperature=full(temperature, torch.float32), top_k=full(top_k, torch.int32),
+                      top_p=full(top_p, torch.float32), min_p=full(min_p, torch.float32))
+        hidden, new, tokens = torch.cat(rows), [r.shape[0] for r in rows], []
+        for i in range(max_new_tokens):
+            token, _, _ = ops.sample(self.forward(hidden, cache, new), u[i], **limits)
+            tokens.append(token)
+            hidden, new = self.embed[token], [1] * n
+        out = torch.stack(tokens, 1).tolist() if tokens else [[] for _ in prompts]
+        for ids in out:
+            end = next((k for k, t in enumerate(ids) if t in stop_ids), None)
+            if end is not None:
+                del ids[end + 1:]
+        return out
+
+
+def main() -> None:
+    from types import SimpleNamespace as NS
+
+    ap = argparse.ArgumentParser(description="Decodes tokens with random weights of a Qwen3-shaped decoder.")
+    ap.add_argument("--layers", type=int, default=4)
+    ap.add_argument("--hidden", type=int, default=2048)
+    ap.add_argument("--vocab", type=int, default=32000)
+    ap.add_argument("--prompt", type=int, default=1104)
+    ap.add_argument("--seqs", type=int, default=4)
+    ap.add_argument("--tokens", type=int, default=32)
+    ap.add_argument("--window", type=int, default=0)
+    ap.add_argument("--sinks", type=int, default=0)
+    a = ap.parse_args()
+    g = torch.Generator(device="cuda").manual_seed(0)
+
+    def w(*shape):
+        return NS(weight=torch.randn(*shape, device="cuda", generator=g) * 0.02)
+
+    d, hq, hkv, ffn = 128, 16, 2, 11008
+    one = NS(weight=torch.ones(a.hidden, device="cuda"))
+    head = NS(weight=torch.ones(d, device="cuda"))
+    layers = [NS(input_layernorm=one, post_attention_layernorm=one,
+                 self_attn=NS(q_proj=w(hq * d, a.hidden), k_proj=w(hkv * d, a.hidden), v_proj=w(hkv * d, a.hidden),
+                              o_proj=w(a.hidden, hq * d), q_norm=head, k_norm=head),
+                 mlp=NS(gate_proj=w(ffn, a.hidden), up_proj=w(ffn, a.hidden), down_proj=w(a.hidden, ffn)))
+              for _ in range(a.layers)]
+    inv = 1.0 / (1e6 ** (torch.arange(0, d, 2, device="cuda").float() / d))
+    ang = torch.outer(torch.arange(a.prompt + a.tokens, device="cuda").float(), inv).repeat(1, 2)
+    dec = B200TextDecoder(layers, one, w(a.vocab, a.hidden).weight * 50, w(a.vocab, a.hidden).weight, ang.cos(), ang.sin(),
+                          window=a.window, sinks=a.sinks)
+    prompts = [torch.randint(a.vocab, (a.prompt - 7 * s,), device="cuda", generator=g).tolist() for s in range(a.seqs)]
+    u = torch.rand(a.tokens, a.seqs, generator=torch.Generator().manual_seed(0))
+    dec.generate(prompts, 2, u=u[:2], temperature=0.8, top_p=0.95)  # loads the kernels
+    torch.cuda.synchronize()
+    e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    e0.record()
+    out = dec.generate(prompts, a.tokens, u=u, temperature=0.8, top_k=50, top_p=0.95)
+    e1.record()
+    torch.cuda.synchronize()
+    print(f"{a.seqs} sequences, prompts of {a.prompt}: {a.tokens} tokens each in {e0.elapsed_time(e1):.1f} ms; first ids "
+          f"{[ids[:6] for ids in out]}")
+
+
+if __name__ == "__main__":
+    main()

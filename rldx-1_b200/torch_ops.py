@@ -16,7 +16,8 @@ torch.ops.b200msat.ds_X instead (or rebind the name):
     ss::fused_mlp_swiglu               -> b200msat::ss_fused_mlp_swiglu
 
 plus the kernels themselves (b200msat::linear, ::joint_attention, ::layernorm,
-::qk_rmsnorm_rope, ::swiglu).  Unlike the reference ops (which hard-code 24 heads x 64 and
+::qk_rmsnorm_rope, ::swiglu) and the token-decoding operators (::qkv_rope_append, ::kv4_read,
+::kv4_attention, ::sample), which the reference has no counterpart of.  Unlike the reference ops (which hard-code 24 heads x 64 and
 batch 1), the head count comes from the shapes.  Every op runs the sm_100a kernels of
 librldx_b200.so on the current stream; there is no CPU implementation.
 
@@ -303,3 +304,59 @@ def swiglu(gate: Tensor, up: Tensor) -> Tensor:
 @swiglu.register_fake
 def _(gate, up):
     return gate.new_empty(gate.shape)
+
+
+# ---------------------------------------------------------------------------------------------
+# token decoding
+# ---------------------------------------------------------------------------------------------
+@torch.library.custom_op("b200msat::qkv_rope_append", mutates_args=("cache",))
+def qkv_rope_append(qkv: Tensor, q_norm: Tensor, k_norm: Tensor, cos: Tensor, sin: Tensor, rope_pos: Tensor, cache: Tensor,
+                    table: Tensor, lengths: Tensor, cu_seqlens: Tensor, q_heads: int, eps: float = 1e-6) -> Tensor:
+    """Per-head norms and rotation of q and k, k and v into the 4-bit cache; q [tokens, q_heads, d]."""
+    return ops.qkv_rope_append(qkv, q_norm, k_norm, cos, sin, rope_pos, cache, table, lengths, cu_seqlens, q_heads=q_heads,
+                               eps=eps)
+
+
+@qkv_rope_append.register_fake
+def _(qkv, q_norm, k_norm, cos, sin, rope_pos, cache, table, lengths, cu_seqlens, q_heads, eps=1e-6):
+    return qkv.new_empty((qkv.shape[0], q_heads, cache.shape[3] // 40))
+
+
+@torch.library.custom_op("b200msat::kv4_read", mutates_args=())
+def kv4_read(cache: Tensor, table: Tensor, lengths: Tensor, cu_seqlens: Tensor, tokens: int) -> Tuple[Tensor, Tensor]:
+    """The values that the 4-bit cache holds for the new tokens: k, v [tokens, kv_heads, d]."""
+    k, v = ops.kv4_read(cache, table, lengths, cu_seqlens, tokens=tokens)
+    return k.clone(), v.clone()  # (outputs of an op must not share storage)
+
+
+@kv4_read.register_fake
+def _(cache, table, lengths, cu_seqlens, tokens):
+    shape = (tokens, cache.shape[1], cache.shape[3] // 40)
+    return cache.new_empty(shape, dtype=BF), cache.new_empty(shape, dtype=BF)
+
+
+@torch.library.custom_op("b200msat::kv4_attention", mutates_args=())
+def kv4_attention(q: Tensor, cache: Tensor, table: Tensor, lengths: Tensor, cu_seqlens: Tensor, max_new: int, max_len: int,
+                  window: int = 0, sinks: int = 0, scale: Optional[float] = None) -> Tensor:
+    """Attention of the new tokens over the 4-bit cache (causal, optional sliding window and sinks)."""
+    return ops.kv4_attention(q, cache, table, lengths, cu_seqlens, max_new=max_new, max_len=max_len, window=window,
+                             sinks=sinks, scale=scale)
+
+
+@kv4_attention.register_fake
+def _(q, cache, table, lengths, cu_seqlens, max_new, max_len, window=0, sinks=0, scale=None):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("b200msat::sample", mutates_args=())
+def sample(logits: Tensor, u: Tensor, temperature: Optional[Tensor] = None, top_k: Optional[Tensor] = None,
+           top_p: Optional[Tensor] = None, min_p: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor]:
+    """One token per row from given numbers: token, logprob, kept."""
+    return ops.sample(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+
+
+@sample.register_fake
+def _(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
+    rows = logits.shape[0]
+    return (logits.new_empty((rows,), dtype=torch.int64), logits.new_empty((rows,), dtype=torch.float32),
+            logits.new_empty((rows,), dtype=torch.int32))
