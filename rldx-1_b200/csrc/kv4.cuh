@@ -99,7 +99,9 @@ struct Kv4AttnParams {
   int whole;        // no segment is cut between CTAs
   float* part_o;    // [CTAs, 2, columns, d] unfinished results of a CTA's first and last segment
   float2* part_ml;  // [CTAs, 2, columns] their reference maximum (log2 units) and sum
-  int4* part_head;  // [CTAs] first row, columns, kv head and parts of the segment that a CTA begins
+  int4* part_head;  // [CTAs] first row, columns, kv head, parts and first CTA of the segment that a CTA begins,
+                    // or (by_segment) of each segment: sequence, tile of columns, kv head
+  int by_segment, tiles;
 };
 
 // The units that the rows [row0, row0 + rows) of a sequence (row = new token * group + head of the

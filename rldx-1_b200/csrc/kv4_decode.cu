@@ -39,6 +39,10 @@ constexpr float kDecGrow = 2.0f;  // lazy move of the reference maximum (log2 un
 
 constexpr int kDecMaxSeqs = 1024;  // sequences of one launch (their prefix sums stand in shared memory)
 
+// A segment's start counts as this many units of a CTA's share: its lookups, the wait for its first units
+// and the merge of the one before.
+constexpr int kDecStart = 12;
+
 // What a CTA works on: units [u0, u0 + m) of the n that columns [c0, c0 + ncols) of kv head kvh of a
 // sequence can see.
 struct DecSegment {
@@ -120,7 +124,7 @@ __device__ __forceinline__ int sequence_units(const Kv4AttnParams& P, int b, int
     return 0;
   }
   int n = 0;
-  for (int c0 = 0; c0 < nq * P.group; c0 += cols) n += P.whole ? 1 : tile_units(P, len, nq, c0, cols);
+  for (int c0 = 0; c0 < nq * P.group; c0 += cols) n += P.whole ? 1 : kDecStart + tile_units(P, len, nq, c0, cols);
   return n * P.c.kv_heads;
 }
 
@@ -195,15 +199,16 @@ __global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? kDecResident : kDecR
       int rest = at - s_before[b], c0 = 0, n = 0, line = 0;
       for (;; c0 += kCols) {  // tiles of columns, each with all kv heads
         n = tile_units(P, len, nq, c0, kCols);
-        line = P.whole ? 1 : n;
+        line = P.whole ? 1 : kDecStart + n;
         if (rest < line * P.c.kv_heads) break;
         rest -= line * P.c.kv_heads;
       }
-      const int kvh = rest / line, u0 = P.whole ? 0 : rest - kvh * line;
-      const int m = P.whole ? n : min(n - u0, end - at);
+      const int kvh = rest / line, off = rest - kvh * line;  // units of the segment stand from kDecStart on
+      const int here = min(line - off, end - at);
+      const int u0 = P.whole ? 0 : max(0, off - kDecStart), m = P.whole ? n : max(0, off + here - kDecStart) - u0;
       if (lane == 0) {
         sg.b = b, sg.q0 = q0, sg.kvh = kvh, sg.c0 = c0, sg.ncols = min(kCols, nq * P.group - c0);
-        sg.n = n, sg.u0 = u0, sg.m = m, sg.line = at - u0, sg.at = at + (P.whole ? 1 : m);
+        sg.n = n, sg.u0 = u0, sg.m = m, sg.line = at - off + kDecStart, sg.at = at + here;
         sg.span = kv4_span(len, nq, c0 / P.group, (c0 + sg.ncols - 1) / P.group, P.window, P.sinks);
       }
     }
@@ -211,6 +216,10 @@ __global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? kDecResident : kDecR
     const int b = sg.b, q0 = sg.q0, kvh = sg.kvh, c0 = sg.c0, ncols = sg.ncols, n = sg.n, u0 = sg.u0, m = sg.m;
     const Kv4Span span = sg.span;
     at = sg.at;
+    if (m == 0) {  // the CTA's share ends before the segment's first unit
+      __syncthreads();
+      continue;
+    }
 
     // lane i holds the i-th of this warp's next 32 units: its index in the pool, and in a ballot
     // whether every column sees every token of it
@@ -526,10 +535,11 @@ __global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? kDecResident : kDecR
     }
     __syncthreads();
     const bool whole = m == n;
-    if (!whole && u0 == 0 && threadIdx.x == 0) {  // for the join: what begins here, and how many CTAs have a part
-      const int last = (sg.line + n - 1) / quota;
-      P.part_head[cta] = make_int4(q0, c0 | (ncols << 24), kvh, last - cta + 1);
-      began = true;
+    if (u0 == 0 && threadIdx.x == 0 && (P.by_segment || !whole)) {  // for the join: who has a part of what begins here
+      const int parts = (sg.line + n - 1) / quota - cta + 1;
+      P.part_head[P.by_segment ? (b * P.tiles + c0 / kCols) * P.c.kv_heads + kvh : cta] =
+          make_int4(q0, c0 | (ncols << 24), kvh, parts | cta << 16);
+      began = !whole;
     }
     const long long slot = 2LL * cta + (u0 == 0 ? 1 : 0);  // 0: began in an earlier CTA; 1: goes on in the next
     for (int i = threadIdx.x; i < ncols * (D / 4); i += 32 * kDecWarps) {
@@ -567,71 +577,93 @@ __global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? kDecResident : kDecR
       __syncthreads();
     }
   }
-  if (threadIdx.x == 0 && !P.whole && !began) P.part_head[cta] = make_int4(0, 0, 0, 0);
+  if (threadIdx.x == 0 && !P.whole && !P.by_segment && !began) P.part_head[cta] = make_int4(0, 0, 0, 1);
 }
 
 // Joins the segments that were cut between CTAs: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s
-// over the parts.  CTA (i, y) takes the segment that begins in CTA i and goes on: a column per warp
-// (kCols warps), or with gridDim.y > 1 column y, of which each of 8 warps takes every eighth part.
+// over the parts, eight at a time so that their loads overlap.  Few segments with many parts
+// (P.by_segment): CTA (i, y) takes column y of segment i, its 16 warps every 16th part.  Otherwise CTA i
+// takes the segment that begins in CTA i of the decode kernel and goes on, a warp per column.
 template <int D>
 __global__ void __launch_bounds__(512) kv4_combine_kernel(const __grid_constant__ Kv4AttnParams P, int cols) {
-  constexpr int kVec = D / 32;  // channels of a lane
-  __shared__ float s_o[8][D], s_l[8];
+  constexpr int kVec = D / 32, kBatch = 8;  // channels of a lane, parts loaded at once
+  __shared__ float s_o[16][D], s_l[16], s_m[16];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   griddep_wait();
   griddep_launch();
-  const int cta = blockIdx.x;
-  const int4 head = P.part_head[cta];
-  const int parts = head.w, c0 = head.y & 0xffffff, ncols = head.y >> 24;
-  if (parts == 0) return;
+  if (P.by_segment) {  // a segment without rows has no entry
+    const int rest = blockIdx.x / P.c.kv_heads, b = rest / P.tiles, c0 = (rest - b * P.tiles) * cols;
+    const int q0 = P.c.cu[b], nq = P.c.cu[b + 1] - q0;
+    if (nq <= 0 || q0 < 0 || nq > P.max_new || P.c.lengths[b] > P.max_len || q0 + nq > P.c.tokens || c0 >= nq * P.group) return;
+  }
+  const int4 head = P.part_head[blockIdx.x];
+  const int parts = head.w & 0xffff, cta = head.w >> 16, c0 = head.y & 0xffffff, ncols = head.y >> 24;
+  if (parts <= 1) return;  // written by its CTA
+  const int split = P.by_segment ? 16 : 1;
+  const int col = P.by_segment ? blockIdx.y : warp, from = P.by_segment ? warp : 0;
+  if (col >= ncols) return;
   // the first CTA kept its part as one that goes on, the others as one that began earlier
-  const int split = gridDim.y == 1 ? 1 : 8;  // warps that share a column
-  const int col = gridDim.y == 1 ? warp : blockIdx.y, from = gridDim.y == 1 ? 0 : warp;
   auto slot = [&](int i) { return (2LL * (cta + i) + (i == 0 ? 1 : 0)) * cols + col; };
-  float l = 0.0f, o[kVec];
+  auto factor = [](float2 x, float m) { return x.x == -INFINITY && x.y == 0.0f ? 0.0f : ex2_approx(x.x - (m == -INFINITY ? 0.0f : m)); };
+  float m = -INFINITY, l = 0.0f, o[kVec];
 #pragma unroll
   for (int e = 0; e < kVec; ++e) o[e] = 0.0f;
-  if (col < ncols) {
-    float m = -INFINITY;
-    for (int i = lane; i < parts; i += 32) m = fmaxf(m, P.part_ml[slot(i)].x);
+  for (int i0 = from; i0 < parts; i0 += kBatch * split) {
+    float2 x[kBatch];
+    float v[kBatch][kVec];
 #pragma unroll
-    for (int k = 16; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
-    const float m_use = m == -INFINITY ? 0.0f : m;
-#pragma unroll 4
-    for (int i = from; i < parts; i += split) {
-      const float2 x = P.part_ml[slot(i)];
-      float v[kVec];
-      const float* src = P.part_o + slot(i) * D + lane * kVec;
-      if constexpr (kVec == 4) {
-        const float4 u = *reinterpret_cast<const float4*>(src);
-        v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
-      } else {
-        const float2 u = *reinterpret_cast<const float2*>(src);
-        v[0] = u.x, v[1] = u.y;
+    for (int u = 0; u < kBatch; ++u) {
+      const int i = i0 + u * split;
+      x[u] = make_float2(-INFINITY, 0.0f);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) v[u][e] = 0.0f;
+      if (i < parts) {
+        x[u] = P.part_ml[slot(i)];
+        const float* src = P.part_o + slot(i) * D + lane * kVec;
+        if constexpr (kVec == 4) {
+          const float4 y = *reinterpret_cast<const float4*>(src);
+          v[u][0] = y.x, v[u][1] = y.y, v[u][2] = y.z, v[u][3] = y.w;
+        } else {
+          const float2 y = *reinterpret_cast<const float2*>(src);
+          v[u][0] = y.x, v[u][1] = y.y;
+        }
       }
-      const float f = x.x == -INFINITY && x.y == 0.0f ? 0.0f : ex2_approx(x.x - m_use);
-      l = fmaf(f, x.y, l);
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) o[e] = fmaf(f, v[e], o[e]);
     }
+    float mb = m;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) mb = fmaxf(mb, x[u].x);
+    const float back = factor(make_float2(m, l), mb);
+    l *= back;
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) o[e] *= back;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const float f = factor(x[u], mb);
+      l = fmaf(f, x[u].y, l);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) o[e] = fmaf(f, v[u][e], o[e]);
+    }
+    m = mb;
   }
-  if (split > 1) {
+  if (P.by_segment) {  // the warps' sums meet
 #pragma unroll
     for (int e = 0; e < kVec; ++e) s_o[warp][lane * kVec + e] = o[e];
-    if (lane == 0) s_l[warp] = l;
+    if (lane == 0) s_l[warp] = l, s_m[warp] = m;
     __syncthreads();
     if (warp > 0) return;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) m = fmaxf(m, s_m[w]);
     l = 0.0f;
 #pragma unroll
     for (int e = 0; e < kVec; ++e) o[e] = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) {
-      l += s_l[w];
+    for (int w = 0; w < 16; ++w) {
+      const float f = factor(make_float2(s_m[w], s_l[w]), m);
+      l = fmaf(f, s_l[w], l);
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) o[e] += s_o[w][lane * kVec + e];
+      for (int e = 0; e < kVec; ++e) o[e] = fmaf(f, s_o[w][lane * kVec + e], o[e]);
     }
   }
-  if (col >= ncols) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const int row = c0 + col, tok = row / P.group;
   const long long orow = static_cast<long long>(head.x + tok) * P.q_heads + head.z * P.group + row - tok * P.group;
@@ -666,13 +698,14 @@ cudaError_t launch_decode(const Kv4AttnParams& whole, int ctas, cudaStream_t str
     p.c.cu += b0;
     p.c.lengths += b0;
     p.c.table += static_cast<long long>(b0) * p.c.table_ld;
+    p.tiles = (p.max_new * p.group + 8 * NT - 1) / (8 * NT);
+    // a few segments are cut into many parts each: then a CTA of the join per segment and column
+    p.by_segment = 16LL * p.tiles * p.c.kv_heads * p.c.seqs < ctas;
     cudaError_t e = launch_pdl(kv4_decode_kernel<D, NT>, dim3(ctas, 1, 1), 32 * kDecWarps, DecShape<D, NT>::kSmem, stream, p);
     if (e != cudaSuccess) return e;
     if (ctas == 1 || p.whole) continue;
-    // few segments have many parts each: then a CTA per column
-    const long long segments = (static_cast<long long>(p.max_new) * p.group + 8 * NT - 1) / (8 * NT) * p.c.kv_heads * p.c.seqs;
-    const bool many = ctas > 16 * segments;
-    e = launch_pdl(kv4_combine_kernel<D>, dim3(ctas, many ? 8 * NT : 1, 1), many ? 256 : 256 * NT, 0, stream, p, 8 * NT);
+    e = p.by_segment ? launch_pdl(kv4_combine_kernel<D>, dim3(p.tiles * p.c.kv_heads * p.c.seqs, 8 * NT, 1), 512, 0, stream, p, 8 * NT)
+                     : launch_pdl(kv4_combine_kernel<D>, dim3(ctas, 1, 1), 256 * NT, 0, stream, p, 8 * NT);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
