@@ -7,6 +7,8 @@ fallback implementation anywhere in this package.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.machinery
+import importlib.util
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -249,6 +251,31 @@ def load(path: Path | None = None) -> C.CDLL:
         fn.argtypes = args
     _LIB = lib
     return lib
+
+
+_BINDING = None
+
+
+def load_binding():
+    """The Python binding of the token-decoding operators (csrc/torch_binding.cpp), bound to the loaded
+    library; built first when its source is newer."""
+    global _BINDING
+    if _BINDING is not None:
+        return _BINDING
+    import torch  # noqa: F401, PLC0415  (the binding links against its libraries)
+
+    from . import build as _build  # noqa: PLC0415
+
+    path = _build.build_binding()
+    loader = importlib.machinery.ExtensionFileLoader("_torch_binding", str(path))
+    mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("_torch_binding", loader))
+    loader.exec_module(mod)
+    lib = load()
+    mod.bind(RldxError, *(C.cast(getattr(lib, name), C.c_void_p).value for name in (
+        "rldx_last_error", "rldx_kv4_append", "rldx_kv4_read", "rldx_kv4_attention_workspace_size", "rldx_kv4_attention",
+        "rldx_sample")))
+    _BINDING = mod
+    return mod
 
 
 class RldxError(RuntimeError):

@@ -1,21 +1,27 @@
-"""Builds librldx_b200.so (all sm_100a kernels + the C ABI) in this package directory.
+"""Builds librldx_b200.so (all sm_100a kernels + the C ABI) and _torch_binding.so (the Python binding of
+the token-decoding operators) in this package directory.
 
 The library is one nvcc translation unit (csrc/rldx_b200.cu) compiled for sm_100a only:
-no PTX for other architectures is embedded, so it loads only on B200-class GPUs.
+no PTX for other architectures is embedded, so it loads only on B200-class GPUs.  The binding is
+host C++ against the installed torch's headers.
 """
 
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_NAME = "librldx_b200.so"
 LIB_PATH = PKG_DIR / LIB_NAME
+BINDING_PATH = PKG_DIR / "_torch_binding.so"
+BINDING_SOURCES = [CSRC / "torch_binding.cpp", PKG_DIR.parent / "include" / "rldx_b200.h"]
 
 NVCC_FLAGS = [
     "-gencode",
@@ -47,8 +53,38 @@ def needs_build() -> bool:
     return any(p.stat().st_mtime > lib_mtime for p in _sources() if p.exists())
 
 
+def binding_needs_build() -> bool:
+    if not BINDING_PATH.exists():
+        return True
+    mtime = BINDING_PATH.stat().st_mtime
+    return any(p.stat().st_mtime > mtime for p in BINDING_SOURCES if p.exists())
+
+
+def build_binding(force: bool = False) -> Path:
+    """Compiles the Python binding if a source is newer than it (or when forced)."""
+    if not force and not binding_needs_build():
+        return BINDING_PATH
+    spec = importlib.util.find_spec("torch")
+    if spec is None or spec.origin is None:
+        raise RuntimeError("torch is not installed: its headers are needed to build the binding")
+    torch_dir = Path(spec.origin).parent
+    nvcc = Path(_nvcc()).resolve()
+    include = [torch_dir / "include", torch_dir / "include" / "torch" / "csrc" / "api" / "include",
+               Path(sysconfig.get_paths()["include"]), nvcc.parents[1] / "include"]
+    tmp = BINDING_PATH.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", *[f"-I{p}" for p in include],
+           str(BINDING_SOURCES[0]), "-o", str(tmp), f"-L{torch_dir / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
+           "-ltorch_cuda", "-ltorch_python", "-ltorch"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, BINDING_PATH)
+    return BINDING_PATH
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compiles the library if a source is newer than the .so (or when forced)."""
+    """Compiles the library and the binding if a source is newer than the .so (or when forced)."""
+    build_binding(force)
     if not force and not needs_build():
         return LIB_PATH
     tmp = LIB_PATH.with_suffix(".so.tmp")

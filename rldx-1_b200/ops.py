@@ -9,7 +9,6 @@ runtime (chain.py) instead.
 from __future__ import annotations
 
 import ctypes as C
-import functools
 from typing import Optional, Sequence
 
 import torch
@@ -339,20 +338,11 @@ def wait_selftest(limit_cycles: int) -> None:
 
 # ------------------------------------------------------------------------------------------------
 # token decoding: 4-bit key / value cache
+#
+# These operators check their tensors, allocate and launch in csrc/torch_binding.cpp: TypeError for a
+# wrong type, ValueError for a wrong shape, layout or device, RldxError for what the library refuses.
 # ------------------------------------------------------------------------------------------------
-def _on_one_device(*tensors) -> int:
-    """Index of the device that holds every tensor; it has to be the current one, whose stream the
-    launch goes to."""
-    index = tensors[0].get_device()
-    for t in tensors:
-        if t is not None and t.get_device() != index:
-            raise ValueError(f"the tensors are on different devices: {index} and {t.device}")
-    if index < 0 or index != torch._C._cuda_getDevice():
-        raise ValueError(f"every tensor must be on the current CUDA device, got {tensors[0].device} (no CPU path exists)")
-    return index
-
-
-_raw_stream = torch._C._cuda_getCurrentRawStream  # of a device index
+_native = _lib.load_binding
 
 
 def kv4_cache(pages: int, kv_heads: int, head_dim: int, page_size: int = 64, device="cuda") -> torch.Tensor:
@@ -363,36 +353,6 @@ def kv4_cache(pages: int, kv_heads: int, head_dim: int, page_size: int = 64, dev
     return torch.empty(pages, kv_heads, page_size // 32, 40 * head_dim, dtype=torch.uint8, device=device)
 
 
-def _kv4_desc(cache, table, lengths, cu_seqlens) -> "_lib.Kv4Cache":
-    shape = cache.shape
-    if cache.dtype is not torch.uint8 or len(shape) != 4 or not cache.is_contiguous() or shape[3] not in (2560, 5120):
-        raise ValueError("cache must be a contiguous uint8 tensor [pages, kv_heads, page_size / 32, 40 head_dim], "
-                         "head_dim 64 or 128")
-    if table.dtype is not torch.int32 or table.dim() != 2 or table.stride(1) != 1:
-        raise ValueError("table must be a row-major int32 tensor [seqs, pages of a sequence]")
-    seqs, width = table.shape
-    if lengths.dtype is not torch.int32 or lengths.shape != (seqs,) or not lengths.is_contiguous():
-        raise ValueError(f"lengths must be a contiguous int32 tensor [{seqs}]")
-    if cu_seqlens.dtype is not torch.int32 or cu_seqlens.shape != (seqs + 1,) or not cu_seqlens.is_contiguous():
-        raise ValueError(f"cu_seqlens must be a contiguous int32 tensor [{seqs + 1}]")
-    pages, kv_heads, units, unit_bytes = shape
-    return _lib.Kv4Cache(cache.data_ptr(), table.data_ptr(), lengths.data_ptr(), cu_seqlens.data_ptr(), pages,
-                         32 * units, kv_heads, unit_bytes // 40, width, max(width, table.stride(0)), seqs)
-
-
-@functools.lru_cache(maxsize=None)
-def _kv4_workspace(index: int, head_dim: int) -> int:
-    """Bytes that hold the unfinished results of any kv4_attention launch on the device."""
-    d = _lib.Kv4Cache(256, 256, 256, 256, 1 << 20, 64, 1, head_dim, 1 << 20, 1 << 20, 1)  # (only sizes are looked at)
-    need = 0
-    for q_heads in (8, 16):
-        n = C.c_uint64(0)
-        a = _lib.Kv4AttentionDesc(None, None, 0, 1, q_heads, 1, 1 << 25, 0, 0, 1.0)
-        check(load().rldx_kv4_attention_workspace_size(C.byref(d), C.byref(a), C.byref(n)))
-        need = max(need, n.value)
-    return need
-
-
 def qkv_rope_append(qkv, q_norm, k_norm, cos, sin, rope_pos, cache, table, lengths, cu_seqlens, *, q_heads: int,
                     eps: float = 1e-6, out=None) -> torch.Tensor:
     """Per-head RMSNorm and rotate-half RoPE of q and k, and the write of k and v into the 4-bit
@@ -401,46 +361,13 @@ def qkv_rope_append(qkv, q_norm, k_norm, cos, sin, rope_pos, cache, table, lengt
     of its lengths[s] tokens; table [seqs, n] int32 gives its pages.  q_norm, k_norm [head_dim] bf16;
     cos, sin [rows, head_dim] bf16 or fp32, rope_pos [tokens] int32 their rows.  Returns q
     [tokens, q_heads, head_dim]: fp32 arithmetic, one rounding to bf16."""
-    if not (qkv.dtype is q_norm.dtype is k_norm.dtype is torch.bfloat16) or rope_pos.dtype is not torch.int32:
-        raise TypeError("qkv, q_norm and k_norm must be bfloat16, rope_pos int32")
-    index = _on_one_device(qkv, q_norm, k_norm, cos, sin, rope_pos, cache, table, lengths, cu_seqlens, out)
-    d = _kv4_desc(cache, table, lengths, cu_seqlens)
-    ld, hd = _row_major(qkv, "qkv"), d.head_dim
-    tokens, width = qkv.shape
-    if width != (q_heads + 2 * d.kv_heads) * hd:
-        raise ValueError(f"qkv rows must hold (q_heads + 2 kv_heads) head_dim = {(q_heads + 2 * d.kv_heads) * hd} values, got {width}")
-    if q_norm.shape != (hd,) or k_norm.shape != (hd,) or q_norm.stride(0) != 1 or k_norm.stride(0) != 1:
-        raise ValueError(f"q_norm and k_norm must be contiguous [{hd}]")
-    rope_fp32 = cos.dtype is torch.float32
-    if not rope_fp32 and cos.dtype is not torch.bfloat16 or sin.dtype is not cos.dtype:
-        raise TypeError("cos and sin must both be bfloat16 or both float32")
-    if cos.dim() != 2 or cos.shape[1] != hd or sin.shape != cos.shape or not cos.is_contiguous() or not sin.is_contiguous():
-        raise ValueError(f"cos and sin must be contiguous [rows, {hd}]")
-    if rope_pos.shape != (tokens,) or not rope_pos.is_contiguous():
-        raise ValueError(f"rope_pos must be a contiguous tensor [{tokens}]")
-    if out is None:
-        out = torch.empty(tokens, q_heads, hd, dtype=torch.bfloat16, device=qkv.device)
-    elif out.dtype != torch.bfloat16 or out.shape != (tokens, q_heads, hd) or not out.is_contiguous():
-        raise ValueError(f"out must be a contiguous bfloat16 tensor [{tokens}, {q_heads}, {hd}]")
-    if tokens == 0:
-        return out
-    check(load().rldx_kv4_append(C.byref(d), qkv.data_ptr(), max(ld, width), tokens, q_heads, q_norm.data_ptr(), k_norm.data_ptr(),
-                                 cos.data_ptr(), sin.data_ptr(), rope_fp32, cos.shape[0],
-                                 rope_pos.data_ptr(), out.data_ptr(), eps, _raw_stream(index)))
-    return out
+    return _native().qkv_rope_append(qkv, q_norm, k_norm, cos, sin, rope_pos, cache, table, lengths, cu_seqlens, q_heads, eps, out)
 
 
 def kv4_read(cache, table, lengths, cu_seqlens, *, tokens: int):
     """The values that the cache holds for the `tokens` new tokens: k, v [tokens, kv_heads, head_dim]
     bf16.  With lengths and cu_seqlens that call every token new, the whole of the sequences."""
-    index = _on_one_device(cache, table, lengths, cu_seqlens)
-    d = _kv4_desc(cache, table, lengths, cu_seqlens)
-    if tokens < 0:
-        raise ValueError("tokens must not be negative")
-    k, v = torch.empty(2, tokens, d.kv_heads, d.head_dim, dtype=torch.bfloat16, device=cache.device).unbind(0)
-    if tokens:
-        check(load().rldx_kv4_read(C.byref(d), tokens, k.data_ptr(), v.data_ptr(), _raw_stream(index)))
-    return k, v
+    return _native().kv4_read(cache, table, lengths, cu_seqlens, tokens)
 
 
 def kv4_attention(q, cache, table, lengths, cu_seqlens, *, max_new: int, max_len: int, window: int = 0,
@@ -451,26 +378,7 @@ def kv4_attention(q, cache, table, lengths, cu_seqlens, *, max_new: int, max_len
     zeros.  max_new and max_len bound the new tokens and the length of any sequence (a launch is
     sized by them; the device's values may be smaller, larger ones record device error 0x502).
     scale defaults to head_dim ** -0.5.  Returns [tokens, q_heads, head_dim]."""
-    if q.dtype is not torch.bfloat16:
-        raise TypeError(f"q must be bfloat16, got {q.dtype}")
-    index = _on_one_device(q, cache, table, lengths, cu_seqlens, out)
-    d = _kv4_desc(cache, table, lengths, cu_seqlens)
-    hd = d.head_dim
-    if q.dim() != 3 or q.shape[2] != hd or q.stride(2) != 1 or (q.shape[1] > 1 and q.stride(1) != hd):
-        raise ValueError(f"q must be [tokens, q_heads, {hd}] with the heads of a token side by side")
-    tokens, q_heads, _ = q.shape
-    if out is None:
-        out = torch.empty(tokens, q_heads, hd, dtype=torch.bfloat16, device=q.device)
-    elif out.dtype != torch.bfloat16 or out.shape != q.shape or not out.is_contiguous():
-        raise ValueError(f"out must be a contiguous bfloat16 tensor {tuple(q.shape)}")
-    if tokens == 0:
-        return out
-    a = _lib.Kv4AttentionDesc(q.data_ptr(), out.data_ptr(), max(q.stride(0), q_heads * hd), tokens, q_heads, max_new, max_len,
-                              window, sinks, hd ** -0.5 if scale is None else scale)
-    need = _kv4_workspace(index, hd)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-    check(load().rldx_kv4_attention(C.byref(d), C.byref(a), ws.data_ptr(), need, _raw_stream(index)))
-    return out
+    return _native().kv4_attention(q, cache, table, lengths, cu_seqlens, max_new, max_len, window, sinks, scale, out)
 
 
 # ------------------------------------------------------------------------------------------------
@@ -483,25 +391,4 @@ def sample(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=None):
     logit; ties go to the lowest id.  Weights are whole numbers, floor(2^32 exp((x - max) / T)), so
     a row's draw is the same in every batch.  Returns token [rows] int64, logprob [rows] fp32 (of the
     kept distribution) and kept [rows] int32, the number of tokens that the filters left."""
-    fp32 = logits.dtype is torch.float32
-    if not fp32 and logits.dtype is not torch.bfloat16:
-        raise TypeError(f"logits must be bfloat16 or float32, got {logits.dtype}")
-    index = _on_one_device(logits, u, temperature, top_k, top_p, min_p)
-    ld = _row_major(logits, "logits")
-    rows, vocab = logits.shape
-    if u.dtype is not torch.float32 or u.shape != (rows,) or not u.is_contiguous():
-        raise ValueError(f"u must be a contiguous float32 tensor [{rows}]")
-    ptr = []
-    for t, name, dtype in ((temperature, "temperature", torch.float32), (top_k, "top_k", torch.int32),
-                           (top_p, "top_p", torch.float32), (min_p, "min_p", torch.float32)):
-        if t is not None and (t.dtype is not dtype or t.shape != (rows,) or not t.is_contiguous()):
-            raise ValueError(f"{name} must be a contiguous {dtype} tensor [{rows}]")
-        ptr.append(None if t is None else t.data_ptr())
-    dev = logits.device
-    token = torch.empty(rows, dtype=torch.int64, device=dev)
-    logprob = torch.empty(rows, dtype=torch.float32, device=dev)
-    kept = torch.empty(rows, dtype=torch.int32, device=dev)
-    if rows:
-        check(load().rldx_sample(logits.data_ptr(), max(ld, vocab), rows, vocab, fp32, u.data_ptr(), *ptr,
-                                 token.data_ptr(), logprob.data_ptr(), kept.data_ptr(), _raw_stream(index)))
-    return token, logprob, kept
+    return _native().sample(logits, u, temperature, top_k, top_p, min_p)

@@ -325,8 +325,7 @@ def _(qkv, q_norm, k_norm, cos, sin, rope_pos, cache, table, lengths, cu_seqlens
 @torch.library.custom_op("b200msat::kv4_read", mutates_args=())
 def kv4_read(cache: Tensor, table: Tensor, lengths: Tensor, cu_seqlens: Tensor, tokens: int) -> Tuple[Tensor, Tensor]:
     """The values that the 4-bit cache holds for the new tokens: k, v [tokens, kv_heads, d]."""
-    k, v = ops.kv4_read(cache, table, lengths, cu_seqlens, tokens=tokens)
-    return k.clone(), v.clone()  # (outputs of an op must not share storage)
+    return ops.kv4_read(cache, table, lengths, cu_seqlens, tokens=tokens)
 
 
 @kv4_read.register_fake
