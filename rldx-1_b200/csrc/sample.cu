@@ -197,6 +197,19 @@ struct Sampler {
     const double bound = static_cast<double>(share) * static_cast<double>(whole);
     return bound > 1.0 ? static_cast<u64>(ceil(bound)) - 1 : 0;
   }
+  __device__ __forceinline__ u64 bin_sum(int i) const { return (static_cast<u64>(s.hi[i]) << 16) + s.lo[i]; }
+  // One thread of rank 0 writes `found`, of every CTA or (kAlone) its own.
+  template <bool kAlone>
+  __device__ __forceinline__ void tell(const u64 (&v)[4]) {
+    if constexpr (kAlone) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s.found[k] = v[k];
+    } else {
+      for (int r = 0; r < cluster; ++r)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) st_cluster_u64(mapa_shared(smem_u32(&s.found[k]), r), v[k]);
+    }
+  }
   // The first bin where the running sum passes `level`; found = {bin or ~0, sum before, sum of the
   // bin, whole}.  With `share` >= 0 the level is the last one below share x whole.  rank 0's sums are
   // zero before and after.
@@ -204,23 +217,21 @@ struct Sampler {
   template <bool kAlone>
   __device__ __forceinline__ bool crossing(u64 level, float share) {
     __syncthreads();
-    const uint32_t g = mapa_shared(smem_u32(s.g), 0);
-    for (int i = threadIdx.x; i < kSampBins; i += NT) {
-      const u64 v = (static_cast<u64>(s.hi[i]) << 16) + s.lo[i];
-      if (v) red_cluster_u64(g + 8 * i, v);
-    }
-    if constexpr (kAlone)
-      __syncthreads();
-    else
+    if constexpr (!kAlone) {
+      const uint32_t g = mapa_shared(smem_u32(s.g), 0);
+      for (int i = threadIdx.x; i < kSampBins; i += NT) {
+        const u64 v = bin_sum(i);
+        if (v) red_cluster_u64(g + 8 * i, v);
+      }
       cluster_sync();
+    }
     if (rank == 0) {
-      const int told = kAlone ? 1 : cluster;  // rank 0 itself is the first
       constexpr int kPer = kSampBins / NT;
       u64 w[kPer], ws = 0;
       const int b0 = threadIdx.x * kPer;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        w[i] = s.g[b0 + i];
+        w[i] = s.g[b0 + i] + (kAlone ? bin_sum(b0 + i) : 0);
         s.g[b0 + i] = 0;
         ws += w[i];
       }
@@ -234,17 +245,15 @@ struct Sampler {
         if (wb <= level && level < wb + w[i]) {
           s.flag = 1u;
           const u64 v[4] = {static_cast<u64>(b0 + i), wb, w[i], whole};
-          for (int r = 0; r < told; ++r)
-            for (int k = 0; k < 4; ++k) st_cluster_u64(mapa_shared(smem_u32(&s.found[k]), r), v[k]);
+          tell<kAlone>(v);
         }
         wb += w[i];
       }
       __syncthreads();
-      if (threadIdx.x == 0 && s.flag == 0u)
-        for (int r = 0; r < told; ++r) {
-          st_cluster_u64(mapa_shared(smem_u32(&s.found[0]), r), ~0ull);
-          st_cluster_u64(mapa_shared(smem_u32(&s.found[3]), r), whole);
-        }
+      if (threadIdx.x == 0 && s.flag == 0u) {
+        const u64 v[4] = {~0ull, 0, 0, whole};
+        tell<kAlone>(v);
+      }
     }
     if constexpr (kAlone)
       __syncthreads();
@@ -771,6 +780,7 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 1 : 4) sample_kernel(const __g
             for (int e = 0; e < kE; ++e) f(x[e]);
           },
           top_k, top_p);
+      __syncthreads();  // every warp has read the last answer in `found`
       if (threadIdx.x < cluster) {
         const uint32_t at = mapa_shared(smem_u32(s.found), threadIdx.x);
         st_cluster_u64(at, __float_as_uint(cut.x));
