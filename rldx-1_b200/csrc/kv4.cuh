@@ -98,10 +98,12 @@ struct Kv4AttnParams {
   int max_new, max_len;
   int whole;        // no segment is cut between CTAs
   float* part_o;    // [CTAs, 2, columns, d] unfinished results of a CTA's first and last segment
-  float2* part_ml;  // [CTAs, 2, columns] their reference maximum (log2 units) and sum
+                    // (kv4_chunk_kernel: [CTAs, d / 4, 256, 4])
+  float2* part_ml;  // [CTAs, 2, columns] their reference maximum (log2 units) and sum ([CTAs, 256])
   int4* part_head;  // [CTAs] first row, columns, kv head, parts and first CTA of the segment that a CTA begins,
                     // or (by_segment) of each segment: sequence, tile of columns, kv head
   int by_segment, tiles;
+  int split, ordered;  // kv4_chunk_kernel: CTAs that share the keys of a tile of rows; longest tiles first
 };
 
 // The units that the rows [row0, row0 + rows) of a sequence (row = new token * group + head of the
@@ -126,7 +128,7 @@ __device__ __forceinline__ Kv4Span kv4_span(int length, int nq, int tok_lo, int 
   return s;
 }
 
-cudaError_t launch_kv4_chunk(const Kv4AttnParams& p, int head_dim, cudaStream_t stream);
+cudaError_t launch_kv4_chunk(Kv4AttnParams p, int head_dim, cudaStream_t stream);
 cudaError_t kv4_chunk_prepare_device();
 cudaError_t launch_kv4_decode(const Kv4AttnParams& p, int head_dim, int cols, int ctas, cudaStream_t stream);
 

@@ -7,11 +7,12 @@
 // fp16 scaled by a power of two per row (largest in [2^14, 2^15)), p is at most 2^8 by the lazy
 // reference maximum of joint_attention_kernel; sums and maxima are fp32.
 //
-// Warps: 0 fetches units by bulk copies, 1 issues the MMAs, 4-11 do the softmax (one row a thread),
-// 12-13 rebuild K, 14-15 rebuild V^T; registers move from the first four to the softmax.  The order of channels inside 16 bytes of K (and q) is that of
-// the nibbles under the masks (0 4 1 5 2 6 3 7), and tokens stand inside each group of eight in
-// an order rotated by the group (chunk_token), so that neither side needs a shuffle and both the
-// reads of the units and the writes of the swizzled tiles are free of bank conflicts.
+// Warps: 0 fetches units by bulk copies, 1 issues the MMAs, 2-3 rebuild K, 4-11 do the softmax (one row a
+// thread), 12-15 rebuild V^T; registers move from the first four to the softmax.  The order of
+// channels inside 16 bytes of K (and q) is that of the nibbles under the masks (0 4 1 5 2 6 3 7), and tokens
+// stand inside each group of eight in an order rotated by the group (chunk_token), so that neither
+// side needs a shuffle and both the reads of the units and the writes of the swizzled tiles are free
+// of bank conflicts.
 //
 // P_j takes the place of S_j in tensor memory, so S_{j+2} is issued once PV_j has finished; the
 // other query tile's products keep the tensor cores busy meanwhile.
@@ -19,6 +20,14 @@
 // A value of V that is not finite, of a token that some rows must not see, cannot go through a
 // product with p = 0: it is rebuilt as 0, its place marked, and the rows that do see the token
 // give NaN in the channels of its group (in every channel where K is not finite).
+// Few tiles of rows would leave most SMs idle, so up to two waves' worth of CTAs share a tile's keys evenly
+// and a second kernel joins their parts (the rule and both sides' times: decode_plan).  With more than
+// a wave of tiles each CTA has its own, longest first.
+//
+// Measured: 8 sequences of up to 2300 tokens, up to 1104 of them new, 16 / 2 heads, d = 128: 139 us, 31 % of
+// cuBLAS's bf16 rate (44 us).  No role bounds it alone: without three quarters of K's rebuilding, of V's, or
+// of the exponentials it takes 137, 132 and 130 us.  K's tiles of 64 keys give an MMA of N = 64, P takes S's
+// place, and the chain S, softmax, P V of the two query tiles covers each other's waits only in part.
 #include "host_util.h"
 #include "kv4.cuh"
 
@@ -44,7 +53,7 @@ struct ChunkShape {
   static constexpr uint32_t kTmemCols = 512;
   static constexpr int kBars = 1 + 2 * kRawStages + 4 * kStages + 2 * 7 + 1;
   static constexpr int kBad = kStages * (kG + 2) * 8;  // marks of what is not finite, a bit per token: V's groups, K; any
-  static constexpr size_t kSmem = 1024 + 2 * kQTile + kStages * (kKTile + kVTile) + kRawStages * kRaw + kBad + 8 * kBars + 16;
+  static constexpr size_t kSmem = 1024 + 2 * kQTile + kStages * (kKTile + kVTile) + kRawStages * kRaw + kBad + 8 * kBars + 16 + 64;
 };
 
 __host__ __device__ constexpr uint32_t umma_idesc_f16(int M, int N) {  // fp16 operands, fp32 accumulator, both K-major
@@ -59,15 +68,14 @@ __device__ __forceinline__ int chunk_row(int token) {
   return (o << 3) + 2 * (((token >> 1) - o) & 3) + (token & 1);
 }
 
-// Codes of one word as fp16 pairs (nibbles 0 4 | 1 5 | 2 6 | 3 7).
+// Codes of one word as fp16 pairs: its nibbles 0 4 | 1 5, and with those of word >> 8 also 2 6 | 3 7.
+__device__ __forceinline__ void codes_f16_low(uint32_t w, __half2 (&c)[2]) {
+  c[0] = __hsub2(bits_h2((w & 0x000f000fu) | 0x64006400u), bits_h2(0x64006400u));                                // 1024
+  c[1] = __hfma2(bits_h2((w & 0x00f000f0u) | 0x64006400u), bits_h2(0x2c002c00u), bits_h2(0xd400d400u));  // 1/16, -64
+}
 __device__ __forceinline__ void codes_f16(uint32_t w, __half2 (&c)[4]) {
-  const uint32_t v = w >> 8;
-  const __half2 bias = bits_h2(0x64006400u);  // 1024
-  const __half2 sixteenth = bits_h2(0x2c002c00u), shift = bits_h2(0xd400d400u);  // 1/16, -64
-  c[0] = __hsub2(bits_h2((w & 0x000f000fu) | 0x64006400u), bias);
-  c[1] = __hfma2(bits_h2((w & 0x00f000f0u) | 0x64006400u), sixteenth, shift);
-  c[2] = __hsub2(bits_h2((v & 0x000f000fu) | 0x64006400u), bias);
-  c[3] = __hfma2(bits_h2((v & 0x00f000f0u) | 0x64006400u), sixteenth, shift);
+  codes_f16_low(w, *reinterpret_cast<__half2(*)[2]>(&c[0]));
+  codes_f16_low(w >> 8, *reinterpret_cast<__half2(*)[2]>(&c[2]));
 }
 __device__ __forceinline__ void clamp_words(uint4* at) {  // NaN stays
   const __half2 top = bits_h2(0x7bff7bffu), bottom = bits_h2(0xfbfffbffu);
@@ -139,6 +147,47 @@ __device__ __forceinline__ uint32_t chunk_seen(int hi, int lo, int sinks) {
   return r;
 }
 
+__device__ __forceinline__ bool chunk_in_bounds(const Kv4AttnParams& P, int q0, int nq, int len) {
+  return nq > 0 && q0 >= 0 && nq <= P.max_new && len <= P.max_len && q0 + nq <= P.c.tokens;
+}
+
+// What a CTA works on, in shared memory, so that each role keeps no more of it in registers than it needs.
+struct alignas(16) ChunkShare {
+  int u0, sink_units, gap, count;  // unit i of the share stands at i + u0 among the span's `count`; kv4_span's unit()
+  int q0, kvh, c0, nrows;          // first query row, kv head, first of the kv head's rows, rows
+  int nt, ng, base, b;             // tiles of 64 keys, of 128 rows; position of the first new token; sequence
+  __device__ __forceinline__ static int unit(const int4& span, int u) { return u < span.y ? u : span.z + u; }
+  __device__ __forceinline__ int4 span() const { return *reinterpret_cast<const int4*>(this); }
+};
+
+// The (sequence, tile of rows) that comes at place `rank` when they stand by descending units, equal ones by
+// ascending number; at most kChunkOrdered of them.  CTAs that run long start first, which evens out the last wave: 4 sequences of
+// 2048 tokens, 1104 of them new, 32 / 8 heads, 184 us against 204 in their own order.
+constexpr int kChunkOrdered = 512;
+__device__ __forceinline__ int chunk_item_of_rank(const Kv4AttnParams& P, int rank, int max_tiles, int* s_units) {
+  const int n = P.c.seqs * max_tiles, i = threadIdx.x;
+  int mine = -1;
+  if (i < n) {
+    const int b = i / max_tiles, c0 = (i - b * max_tiles) * 256;
+    const int q0 = P.c.cu[b], nq = P.c.cu[b + 1] - q0, len = P.c.lengths[b];
+    mine = 0;
+    if (chunk_in_bounds(P, q0, nq, len) && c0 < nq * P.group)
+      mine = 1 + kv4_span(len, nq, c0 / P.group, (min(c0 + 256, nq * P.group) - 1) / P.group, P.window, P.sinks).count;
+  }
+  s_units[i] = mine;
+  __syncthreads();
+  if (i < n) {
+    int before = 0;
+#pragma unroll 8
+    for (int k = 0; k < n; ++k) before += s_units[k] > mine || (s_units[k] == mine && k < i);
+    if (before == rank) s_units[kChunkOrdered] = i;
+  }
+  __syncthreads();
+  const int item = s_units[kChunkOrdered];
+  __syncthreads();
+  return item;
+}
+
 template <int D>
 __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(const __grid_constant__ Kv4AttnParams P) {
   using U = Kv4Unit<D>;
@@ -167,14 +216,15 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
   auto o_final = [&](int g) { return gbar + 7 * g + 6; };
   uint64_t* drain = gbar + 14;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  ChunkShare& share = *reinterpret_cast<ChunkShare*>((reinterpret_cast<uintptr_t>(tmem_slot) + 19) & ~static_cast<uintptr_t>(15));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 8);
-    for (int s = 0; s < kR; ++s) mbar_init(&raw_full[s], 1), mbar_init(&raw_empty[s], 4);
+    for (int s = 0; s < kR; ++s) mbar_init(&raw_full[s], 1), mbar_init(&raw_empty[s], 6);
     for (int s = 0; s < kS; ++s) {
       mbar_init(&k_full[s], 2), mbar_init(&k_empty[s], 1);
-      mbar_init(&v_full[s], 2), mbar_init(&v_empty[s], 1);
+      mbar_init(&v_full[s], 4), mbar_init(&v_empty[s], 1);
     }
     for (int g = 0; g < 2; ++g) {
       for (int i = 0; i < 2; ++i) mbar_init(&s_full(g)[i], 1), mbar_init(&p_full(g)[i], 4), mbar_init(&o_done(g)[i], 1);
@@ -185,20 +235,34 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
   }
   griddep_wait();
   griddep_launch();
-  // ---- this CTA's rows: the last tile of a sequence, which sees most keys, first ----
-  const int b = blockIdx.z, kvh = blockIdx.y;
-  const int q0 = P.c.cu[b], nq = P.c.cu[b + 1] - q0, len = P.c.lengths[b];
-  if (nq <= 0 || q0 < 0 || nq > P.max_new || len > P.max_len || q0 + nq > P.c.tokens) {
-    if (nq != 0 && threadIdx.x == 0) record_error(kErrKv4Bound);
-    return;
+  // ---- this CTA's rows and its share of their keys ----
+  {
+    const int max_tiles = (P.max_new * P.group + 255) / 256;
+    const int part = static_cast<int>(blockIdx.x % P.split), unsplit = static_cast<int>(blockIdx.x / P.split);
+    int item = unsplit / P.c.kv_heads;  // sequence, tile
+    if (P.ordered) item = chunk_item_of_rank(P, item, max_tiles, reinterpret_cast<int*>(smem));
+    const int b = item / max_tiles, c0 = (item - b * max_tiles) * 256;
+    const int q0 = P.c.cu[b], nq = P.c.cu[b + 1] - q0, len = P.c.lengths[b];
+    if (!chunk_in_bounds(P, q0, nq, len)) {
+      if (nq != 0 && threadIdx.x == 0) record_error(kErrKv4Bound);
+      return;
+    }
+    const int nrows = min(256, nq * P.group - c0);
+    if (nrows <= 0) return;
+    if (threadIdx.x == 0) {
+      const Kv4Span span = kv4_span(len, nq, c0 / P.group, (c0 + nrows - 1) / P.group, P.window, P.sinks);
+      const int all = (span.count + 1) / 2;
+      int t0 = 0, t1 = all;
+      if (P.split > 1) {
+        t0 = static_cast<int>(static_cast<long long>(all) * part / P.split);
+        t1 = static_cast<int>(static_cast<long long>(all) * (part + 1) / P.split);
+      }
+      share.u0 = 2 * t0, share.sink_units = span.sink_units, share.gap = span.first - span.sink_units, share.count = span.count;
+      share.q0 = q0, share.kvh = unsplit % P.c.kv_heads, share.c0 = c0, share.nrows = nrows;
+      share.nt = t1 - t0, share.ng = nrows > 128 ? 2 : 1;
+      share.base = len - nq, share.b = b;
+    }
   }
-  const int tiles = (nq * P.group + 255) / 256;
-  const int tile = tiles - 1 - static_cast<int>(blockIdx.x);
-  if (tile < 0) return;
-  const int c0 = tile * 256, nrows = min(256, nq * P.group - c0);
-  const int ng = nrows > 128 ? 2 : 1;
-  const Kv4Span span = kv4_span(len, nq, c0 / P.group, (c0 + nrows - 1) / P.group, P.window, P.sinks);
-  const int nt = (span.count + 1) / 2;  // key tiles
 
   if (warp == 1) tmem_alloc(tmem_slot, Sh::kTmemCols);
   tc_fence_before();
@@ -213,11 +277,13 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
     bool ok = true;
     int index = -1;
     const uint64_t policy = l2_policy_evict_last();
+    const int4 span = share.span();
+    const int nt = share.nt, kvh = share.kvh, b = share.b;
     for (int j = 0; j < nt; ++j) {
       if ((j & 15) == 0) {
-        const int i = 2 * j + lane;
-        index = i < span.count ? kv4_unit_index(P.c, b, kvh, span.unit(i)) : -1;
-        if (i < span.count && index < 0) record_error(kErrKv4Table);
+        const int u = span.x + 2 * j + lane;
+        index = u < span.w ? kv4_unit_index(P.c, b, kvh, ChunkShare::unit(span, u)) : -1;
+        if (u < span.w && index < 0) record_error(kErrKv4Table);
       }
       const int a = __shfl_sync(0xffffffffu, index, 2 * (j & 15)), c = __shfl_sync(0xffffffffu, index, 2 * (j & 15) + 1);
       const int s = j % kR;
@@ -244,7 +310,7 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
     // issues
     const uint32_t lead = elect_one();
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-    const int tiles_k = __shfl_sync(0xffffffffu, nt, 0), groups = __shfl_sync(0xffffffffu, ng, 0);
+    const int tiles_k = __shfl_sync(0xffffffffu, share.nt, 0), groups = __shfl_sync(0xffffffffu, share.ng, 0);
     constexpr uint32_t idesc_s = umma_idesc_f16(128, 64), idesc_o = umma_idesc_f16(128, D);
     const uint64_t q_desc = umma_desc_sw128(smem_u32(sQ)), k_desc = umma_desc_sw128(smem_u32(sK)), v_desc = umma_desc_sw128(smem_u32(sV));
     bool ok = tiles_k > 0 && __all_sync(0xffffffffu, mbar_wait(q_full, 0u, kErrKv4Chunk + 1));
@@ -294,142 +360,154 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
       umma_commit_lead(lead, drain);
       mbar_wait_teardown(drain, 0u);
     }
-  }
-  } else if (warp >= 12) {
-    // ---------------- rebuild K (warps 12, 13) and V^T (warps 14, 15) ----------------
-    reg_dec<kChunkRegsRebuild>();
-    const bool is_v = warp >= 14;
-    const int w = warp & 1;
+  } else {
+    // ---------------- rebuild K (warps 2, 3) ----------------
+    const int w = warp & 1, nt = share.nt;
     bool ok = true;
     for (int j = 0; ok && j < nt; ++j) {
       const int s = j % kS, rs = j % kR;
       ok = mbar_wait(&raw_full[rs], static_cast<uint32_t>(j / kR) & 1u, kErrKv4Chunk + 2) &&
-           mbar_wait(is_v ? &v_empty[s] : &k_empty[s], (static_cast<uint32_t>(j / kS) & 1u) ^ 1u, kErrKv4Chunk + 2);
+           mbar_wait(&k_empty[s], (static_cast<uint32_t>(j / kS) & 1u) ^ 1u, kErrKv4Chunk + 2);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       const uint8_t* raw = sRaw + rs * Sh::kRaw;
-      if (!is_v) {
-        // lane (quarter q, upper u, t): tokens r and r ^ 5 of a group of eight share a quarter, which
-        // keeps both the loads (64-byte rows) and the swizzled stores free of conflicts
-        const int t = lane & 3, r = (lane >> 3) ^ ((lane & 4) ? 5 : 0);
-        uint8_t* dst = sK + s * Sh::kKTile;
+      // lane (quarter q, upper u, t): tokens r and r ^ 5 of a group of eight share a quarter, which
+      // keeps both the loads (64-byte rows) and the swizzled stores free of conflicts
+      const int t = lane & 3, r = (lane >> 3) ^ ((lane & 4) ? 5 : 0);
+      uint8_t* dst = sK + s * Sh::kKTile;
 #pragma unroll 1
-        for (int p = 0; p < 4; ++p) {
-          const int token = 8 * (4 * w + p) + r, tau = token & 31;
-          const uint8_t* un = raw + (token >> 5) * U::kBytes;
-          uint32_t code[G], meta[G];
-          lds_words<G>(un + tau * U::kRow + t * 4 * G, code);
-          lds_words<G>(un + U::kKMeta + 4 * G * tau, meta);
-          __half2 z = bits_h2(0u);  // NaN once a value would not be finite
+      for (int p = 0; p < 4; ++p) {
+        const int token = 8 * (4 * w + p) + r, tau = token & 31;
+        const uint8_t* un = raw + (token >> 5) * U::kBytes;
+        uint32_t code[G], meta[G];
+        lds_words<G>(un + tau * U::kRow + t * 4 * G, code);
+        lds_words<G>(un + U::kKMeta + 4 * G * tau, meta);
+        __half2 z = bits_h2(0u);  // NaN once a value would not be finite
 #pragma unroll
-          for (int i = 0; i < G / 2; ++i)
-            z = __hfma2(__hfma2(bits_h2(0x4b804b80u), bits_h2(meta[i]), bits_h2(meta[G / 2 + i])), bits_h2(0u), z);
-          const int row = chunk_row(token);
-          uint8_t* at = dst + row * 128;
-#pragma unroll
-          for (int gi = 0; gi < G; ++gi) {
-            const uint32_t sel = (gi & 1) ? 0x3232u : 0x1010u;
-            const __half2 sc = bits_h2(__byte_perm(meta[gi / 2], 0u, sel)), lo = bits_h2(__byte_perm(meta[G / 2 + gi / 2], 0u, sel));
-            __half2 c[4];
-            codes_f16(code[gi], c);
-            uint4 u;
-            u.x = h2_bits(__hfma2(c[0], sc, lo)), u.y = h2_bits(__hfma2(c[1], sc, lo));
-            u.z = h2_bits(__hfma2(c[2], sc, lo)), u.w = h2_bits(__hfma2(c[3], sc, lo));
-            *reinterpret_cast<uint4*>(at + (gi >> 1) * Sh::kKChunk + (((4 * (gi & 1) + t) ^ (row & 7)) << 4)) = u;
-          }
-          if (h2_bits(z) & 0x7fff7fffu) {  // a value outside fp16's range becomes its largest
-#pragma unroll 1
-            for (int gi = 0; gi < G; ++gi)
-              clamp_words(reinterpret_cast<uint4*>(at + (gi >> 1) * Sh::kKChunk + (((4 * (gi & 1) + t) ^ (row & 7)) << 4)));
-          }
-        }
-      } else {
-        // lane (g, group of eight o): channels 32 j + 4 g + i of eight tokens, four 16-byte keys each
-        const int o = 4 * w + (lane & 3), g = lane >> 2;
-        const uint8_t* un = raw + (o >> 2) * U::kBytes;
-        const int at = (o & 3) >> 1, hh = o & 1;  // block of 16, half
-        uint32_t code[4][G], sc[4][G], lo[4][G];
-        __half2 z = bits_h2(0u);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int t = (k + o) & 3;
-          lds_words<G>(un + U::kV + 8 * D * at + 4 * D * hh + 4 * G * (4 * g + t), code[k]);
-          lds_words<G>(un + U::kVScale + 32 * G * at + 16 * G * hh + 4 * G * t, sc[k]);
-          lds_words<G>(un + U::kVLow + 32 * G * at + 16 * G * hh + 4 * G * t, lo[k]);
-#pragma unroll
-          for (int gi = 0; gi < G; ++gi)
-            z = __hfma2(__hfma2(bits_h2(0x4b804b80u), bits_h2(sc[k][gi]), bits_h2(lo[k][gi])), bits_h2(0u), z);
-        }
-        // lane g also looks at K of token 8 o + g
-        uint32_t meta[G];
-        lds_words<G>(un + U::kKMeta + 4 * G * ((8 * o + g) & 31), meta);
-        __half2 zk = bits_h2(0u);
-#pragma unroll
-        for (int i = 0; i < G; ++i) zk = __hfma2(bits_h2(meta[i]), bits_h2(0u), zk);
-        const unsigned bad_k = __ballot_sync(0xffffffffu, h2_bits(zk) & 0x7fff7fffu);
-        const bool odd = (h2_bits(z) & 0x7fff7fffu) != 0u;  // a value would not be finite
-        uint32_t bad[G];
-#pragma unroll
-        for (int gi = 0; gi < G; ++gi) bad[gi] = 0u;
-        if (odd) {
-          const __half2 inf = bits_h2(0x7c007c00u);
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-#pragma unroll
-            for (int gi = 0; gi < G; ++gi) {
-              const uint32_t fine = __hlt2_mask(__habs2(bits_h2(sc[k][gi])), inf) & __hlt2_mask(__habs2(bits_h2(lo[k][gi])), inf);
-              sc[k][gi] &= fine, lo[k][gi] &= fine;
-              bad[gi] |= ((~fine & 1u) | (~fine >> 15 & 2u)) << (2 * k);
-            }
-        }
-        if (__any_sync(0xffffffffu, odd || bad_k != 0u)) {
-          if (g == 0) {
-#pragma unroll
-            for (int gi = 0; gi < G; ++gi) sBad[(s * (G + 2) + gi) * 8 + o] = static_cast<uint8_t>(bad[gi]);
-            uint32_t byte = 0u;
-#pragma unroll 1
-            for (int i = 0; i < 8; ++i) byte |= (bad_k >> (4 * i + lane) & 1u) << (chunk_row(8 * o + i) & 7);
-            sBad[(s * (G + 2) + G) * 8 + o] = static_cast<uint8_t>(byte);
-            sBad[(s * (G + 2) + G + 1) * 8 + o] = 1u;
-          }
-          __syncwarp();
-        } else if (g == 0) {
-          // the other warp's groups may be marked: then these are read too
-#pragma unroll
-          for (int gi = 0; gi <= G + 1; ++gi) sBad[(s * (G + 2) + gi) * 8 + o] = 0u;
-        }
-        uint8_t* dst = sV + s * Sh::kVTile;
+        for (int i = 0; i < G / 2; ++i)
+          z = __hfma2(__hfma2(bits_h2(0x4b804b80u), bits_h2(meta[i]), bits_h2(meta[G / 2 + i])), bits_h2(0u), z);
+        const int row = chunk_row(token);
+        uint8_t* at = dst + row * 128;
 #pragma unroll
         for (int gi = 0; gi < G; ++gi) {
-          uint32_t out[4][4];  // [channel i][pair k]
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t x = __byte_perm(code[k][gi / 2], code[k][G / 2 + gi / 2], (gi & 1) ? 0x7632u : 0x5410u);
-            __half2 c[4];
-            codes_f16(x, c);  // channels 0..3 of tokens 2t | 2t + 1
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              out[i][k] = h2_bits(__hfma2(c[i], bits_h2(sc[k][gi]), bits_h2(lo[k][gi])));
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int row = 32 * gi + 4 * g + i;
-            *reinterpret_cast<uint4*>(dst + row * 128 + ((o ^ (row & 7)) << 4)) = make_uint4(out[i][0], out[i][1], out[i][2], out[i][3]);
-          }
+          const uint32_t sel = (gi & 1) ? 0x3232u : 0x1010u;
+          const __half2 sc = bits_h2(__byte_perm(meta[gi / 2], 0u, sel)), lo = bits_h2(__byte_perm(meta[G / 2 + gi / 2], 0u, sel));
+          __half2 c[4];
+          codes_f16(code[gi], c);
+          uint4 u;
+          u.x = h2_bits(__hfma2(c[0], sc, lo)), u.y = h2_bits(__hfma2(c[1], sc, lo));
+          u.z = h2_bits(__hfma2(c[2], sc, lo)), u.w = h2_bits(__hfma2(c[3], sc, lo));
+          *reinterpret_cast<uint4*>(at + (gi >> 1) * Sh::kKChunk + (((4 * (gi & 1) + t) ^ (row & 7)) << 4)) = u;
         }
-        if (odd) {
+        if (h2_bits(z) & 0x7fff7fffu) {  // a value outside fp16's range becomes its largest
 #pragma unroll 1
-          for (int i = 0; i < 4 * G; ++i) {
-            const int row = 32 * (i >> 2) + 4 * g + (i & 3);
-            clamp_words(reinterpret_cast<uint4*>(dst + row * 128 + ((o ^ (row & 7)) << 4)));
-          }
+          for (int gi = 0; gi < G; ++gi)
+            clamp_words(reinterpret_cast<uint4*>(at + (gi >> 1) * Sh::kKChunk + (((4 * (gi & 1) + t) ^ (row & 7)) << 4)));
         }
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(is_v ? &v_full[s] : &k_full[s]);
+        mbar_arrive(&k_full[s]);
+        mbar_arrive(&raw_empty[rs]);
+      }
+    }
+  }
+  } else if (warp >= 12) {
+    // ---------------- rebuild V^T (warps 12 to 15) ----------------
+    reg_dec<kChunkRegsRebuild>();
+    const int w = warp & 3, nt = share.nt;
+    bool ok = true;
+    for (int j = 0; ok && j < nt; ++j) {
+      const int s = j % kS, rs = j % kR;
+      ok = mbar_wait(&raw_full[rs], static_cast<uint32_t>(j / kR) & 1u, kErrKv4Chunk + 2) &&
+           mbar_wait(&v_empty[s], (static_cast<uint32_t>(j / kS) & 1u) ^ 1u, kErrKv4Chunk + 2);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      const uint8_t* raw = sRaw + rs * Sh::kRaw;
+      // lane (g, half h, group of eight o): channels 32 j + 4 g + 2 h + i of eight tokens
+      const int o = 2 * w + (lane & 1), h = lane >> 1 & 1, g = lane >> 2;
+      const uint8_t* un = raw + (o >> 2) * U::kBytes;
+      const int at = (o & 3) >> 1, hh = o & 1;  // block of 16, half
+      uint32_t code[4][G], sc[4][G], lo[4][G];
+      __half2 z = bits_h2(0u);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int t = (k + o) & 3;
+        lds_words<G>(un + U::kV + 8 * D * at + 4 * D * hh + 4 * G * (4 * g + t), code[k]);
+        lds_words<G>(un + U::kVScale + 32 * G * at + 16 * G * hh + 4 * G * t, sc[k]);
+        lds_words<G>(un + U::kVLow + 32 * G * at + 16 * G * hh + 4 * G * t, lo[k]);
+#pragma unroll
+        for (int gi = 0; gi < G; ++gi)
+          z = __hfma2(__hfma2(bits_h2(0x4b804b80u), bits_h2(sc[k][gi]), bits_h2(lo[k][gi])), bits_h2(0u), z);
+      }
+      // lane g also looks at K of token 8 o + g
+      uint32_t meta[G];
+      lds_words<G>(un + U::kKMeta + 4 * G * ((8 * o + g) & 31), meta);
+      __half2 zk = bits_h2(0u);
+#pragma unroll
+      for (int i = 0; i < G; ++i) zk = __hfma2(bits_h2(meta[i]), bits_h2(0u), zk);
+      const unsigned bad_k = __ballot_sync(0xffffffffu, h2_bits(zk) & 0x7fff7fffu);
+      const bool odd = (h2_bits(z) & 0x7fff7fffu) != 0u;  // a value would not be finite
+      uint32_t bad[G];
+#pragma unroll
+      for (int gi = 0; gi < G; ++gi) bad[gi] = 0u;
+      if (odd) {
+        const __half2 inf = bits_h2(0x7c007c00u);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int gi = 0; gi < G; ++gi) {
+            const uint32_t fine = __hlt2_mask(__habs2(bits_h2(sc[k][gi])), inf) & __hlt2_mask(__habs2(bits_h2(lo[k][gi])), inf);
+            sc[k][gi] &= fine, lo[k][gi] &= fine;
+            bad[gi] |= ((~fine & 1u) | (~fine >> 15 & 2u)) << (2 * k);
+          }
+      }
+      if (__any_sync(0xffffffffu, odd || bad_k != 0u)) {
+        if (g == 0 && h == 0) {
+#pragma unroll
+          for (int gi = 0; gi < G; ++gi) sBad[(s * (G + 2) + gi) * 8 + o] = static_cast<uint8_t>(bad[gi]);
+          uint32_t byte = 0u;
+#pragma unroll 1
+          for (int i = 0; i < 8; ++i) byte |= (bad_k >> (4 * i + lane) & 1u) << (chunk_row(8 * o + i) & 7);
+          sBad[(s * (G + 2) + G) * 8 + o] = static_cast<uint8_t>(byte);
+          sBad[(s * (G + 2) + G + 1) * 8 + o] = 1u;
+        }
+        __syncwarp();
+      } else if (g == 0 && h == 0) {
+        // another warp's groups may be marked: then these are read too
+#pragma unroll
+        for (int gi = 0; gi <= G + 1; ++gi) sBad[(s * (G + 2) + gi) * 8 + o] = 0u;
+      }
+      uint8_t* dst = sV + s * Sh::kVTile;
+#pragma unroll
+      for (int gi = 0; gi < G; ++gi) {
+        uint32_t out[2][4];  // [channel i][pair k]
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t x = __byte_perm(code[k][gi / 2], code[k][G / 2 + gi / 2], (gi & 1) ? 0x7632u : 0x5410u);
+          __half2 c[2];
+          codes_f16_low(x >> (8 * h), c);  // channels 2 h, 2 h + 1 of tokens 2t | 2t + 1
+#pragma unroll
+          for (int i = 0; i < 2; ++i) out[i][k] = h2_bits(__hfma2(c[i], bits_h2(sc[k][gi]), bits_h2(lo[k][gi])));
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int row = 32 * gi + 4 * g + 2 * h + i;
+          *reinterpret_cast<uint4*>(dst + row * 128 + ((o ^ (row & 7)) << 4)) = make_uint4(out[i][0], out[i][1], out[i][2], out[i][3]);
+        }
+      }
+      if (odd) {
+#pragma unroll 1
+        for (int i = 0; i < 2 * G; ++i) {
+          const int row = 32 * (i >> 1) + 4 * g + 2 * h + (i & 1);
+          clamp_words(reinterpret_cast<uint4*>(dst + row * 128 + ((o ^ (row & 7)) << 4)));
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&v_full[s]);
         mbar_arrive(&raw_empty[rs]);
       }
     }
@@ -437,15 +515,19 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
     // ---------------- softmax: one row a thread ----------------
     reg_inc<kChunkRegsSoftmax>();
     const int g = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane;
-    const int row = c0 + 128 * g + r;  // among the kv head's rows
-    const bool live = 128 * g + r < nrows;
-    const int tok = row / P.group, head = kvh * P.group + row - tok * P.group;
-    const int ps = live ? len - nq + tok : -1;
+    const int nt = share.nt, ng = share.ng;
+    int ps, pos_lo, pos_hi;  // positions of this row, and of the tile's first and last
     const uint32_t lane_off = static_cast<uint32_t>(quad * 32) << 16;
     float fac;  // log2 score per unit of the products
     {
+      const int c0 = share.c0, nrows = share.nrows, base = share.base;
+      const bool live = 128 * g + r < nrows;
+      const int row = c0 + 128 * g + r, tok = row / P.group, head = share.kvh * P.group + row - tok * P.group;
+      ps = live ? base + tok : -1;
+      pos_lo = base + (c0 + 128 * g) / P.group;
+      pos_hi = base + (c0 + min(nrows, 128 * g + 128) - 1) / P.group;
       uint4 u[D / 8];
-      const uint4* src = reinterpret_cast<const uint4*>(P.q + static_cast<long long>(q0 + tok) * P.ldq + static_cast<long long>(head) * D);
+      const uint4* src = reinterpret_cast<const uint4*>(P.q + static_cast<long long>(share.q0 + tok) * P.ldq + static_cast<long long>(head) * D);
       float mx = 0.0f;
 #pragma unroll
       for (int i = 0; i < D / 8; ++i) {
@@ -481,9 +563,6 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
     }
-    // positions of the tile's first and last row
-    const int pos_lo = len - nq + (c0 + 128 * g) / P.group;
-    const int pos_hi = len - nq + (c0 + min(nrows, 128 * g + 128) - 1) / P.group;
     float m_ref = -INFINITY, l_run = 0.0f;
     uint32_t poison = 0u;  // groups in which a visible token has no finite value
     bool ok = g < ng;
@@ -491,16 +570,14 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
       const int sb = j & 1;
       const uint32_t ph = static_cast<uint32_t>(j >> 1) & 1u;
       const uint32_t s_col = tmem + lane_off + (2 * g + sb) * 64;
-      ok = __all_sync(0xffffffffu, mbar_wait(&s_full(g)[sb], ph, kErrKv4Chunk + 3));
-      if (!ok) break;
-      tc_fence_after();
       // ---- masks: keys of the two units; a unit past the span is hidden ----
       bool plain = true;
       int key0[2];
+      const int4 span = share.span();
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const bool have = 2 * j + i < span.count;
-        key0[i] = have ? kKv4Unit * span.unit(2 * j + i) : 0x40000000;
+        const int u = span.x + 2 * j + i;
+        key0[i] = u < span.w ? kKv4Unit * ChunkShare::unit(span, u) : 0x40000000;
         plain &= key0[i] + 31 <= pos_lo && (P.window <= 0 || pos_hi - key0[i] < P.window || key0[i] + 31 < P.sinks);
       }
       uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
@@ -510,6 +587,9 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
           seen[i] = P.window > 0 ? chunk_seen(ps - key0[i] + 1, ps - P.window - key0[i], P.sinks - key0[i])
                                  : chunk_seen(ps - key0[i] + 1, -1, 0);
       }
+      ok = __all_sync(0xffffffffu, mbar_wait(&s_full(g)[sb], ph, kErrKv4Chunk + 3));
+      if (!ok) break;
+      tc_fence_after();
       float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       float sv[64];
       tmem_ld32(s_col, *reinterpret_cast<float(*)[32]>(&sv[0]));
@@ -578,10 +658,15 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
     if (ok && nt > 0) ok = mbar_wait(o_final(g), 0u, kErrKv4Chunk + 3);
     if (__all_sync(0xffffffffu, ok) && g < ng) {
       tc_fence_after();
-      const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;  // no visible key: zeros
-      uint4* dst = reinterpret_cast<uint4*>(P.out + (static_cast<long long>(q0 + tok) * P.q_heads + head) * D);
+      const bool whole = P.split == 1;
+      const int row = share.c0 + 128 * g + r, tok = row / P.group, head = share.kvh * P.group + row - tok * P.group;
+      const bool live = 128 * g + r < share.nrows;
+      const float inv = !whole ? 1.0f : l_run == 0.0f ? 0.0f : 1.0f / l_run;  // no visible key: zeros
+      uint4* dst = reinterpret_cast<uint4*>(P.out + (static_cast<long long>(share.q0 + tok) * P.q_heads + head) * D);
+      if (!whole && live) P.part_ml[256LL * blockIdx.x + 128 * g + r] = make_float2(m_ref, l_run);
 #pragma unroll
       for (int h = 0; h < D / 32; ++h) {
+        if (nt == 0 && !whole) break;  // (-inf, 0) says that there is nothing
         float o[32];
         if (nt > 0) {
           tmem_ld32(tmem + lane_off + Sh::kOCol + g * D + 32 * h, o);
@@ -591,16 +676,22 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
           for (int c = 0; c < 32; ++c) o[c] = 0.0f;
         }
         const float f = (poison >> h & 1u) ? NAN : inv;
-        if (live) {
+#pragma unroll
+        for (int c = 0; c < 32; ++c) o[c] *= f;
+        if (live && whole) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             uint4 u;
-            u.x = pack_bf16x2(o[8 * i + 0] * f, o[8 * i + 1] * f);
-            u.y = pack_bf16x2(o[8 * i + 2] * f, o[8 * i + 3] * f);
-            u.z = pack_bf16x2(o[8 * i + 4] * f, o[8 * i + 5] * f);
-            u.w = pack_bf16x2(o[8 * i + 6] * f, o[8 * i + 7] * f);
+            u.x = pack_bf16x2(o[8 * i + 0], o[8 * i + 1]);
+            u.y = pack_bf16x2(o[8 * i + 2], o[8 * i + 3]);
+            u.z = pack_bf16x2(o[8 * i + 4], o[8 * i + 5]);
+            u.w = pack_bf16x2(o[8 * i + 6], o[8 * i + 7]);
             dst[4 * h + i] = u;
           }
+        } else if (live) {
+          float4* po = reinterpret_cast<float4*>(P.part_o) + (static_cast<long long>(blockIdx.x) * (D / 4) + 8 * h) * 256 + 128 * g + r;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) po[256 * i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
         }
       }
     }
@@ -613,11 +704,67 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
   }
 }
 
-cudaError_t launch_kv4_chunk(const Kv4AttnParams& p, int head_dim, cudaStream_t stream) {
-  const dim3 grid((p.max_new * p.group + 255) / 256, p.c.kv_heads, p.c.seqs);
-  return head_dim == 128
-             ? launch_pdl(kv4_chunk_kernel<128>, grid, ChunkShape<128>::kThreads, ChunkShape<128>::kSmem, stream, p)
-             : launch_pdl(kv4_chunk_kernel<64>, grid, ChunkShape<64>::kThreads, ChunkShape<64>::kSmem, stream, p);
+// Joins the parts of rows whose keys were shared out (split > 1): out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.
+// A part lies as [d / 4][256 rows][4], so that both the softmax threads, a row each, and the threads here, a
+// row and four channels each, read and write whole lines.  A part that saw no key holds nothing in part_o.
+template <int D>
+__global__ void __launch_bounds__(256) kv4_chunk_join_kernel(const __grid_constant__ Kv4AttnParams P) {
+  constexpr int kBatch = 8;  // parts loaded at once
+  griddep_wait();
+  griddep_launch();
+  const int max_tiles = (P.max_new * P.group + 255) / 256;
+  const int unsplit = static_cast<int>(blockIdx.x) >> 3, r = (static_cast<int>(blockIdx.x) & 7) * 32 + (threadIdx.x & 31);
+  const int four = 8 * blockIdx.y + (threadIdx.x >> 5);
+  const int kvh = unsplit % P.c.kv_heads, item = unsplit / P.c.kv_heads;
+  const int b = item / max_tiles, row = (item - b * max_tiles) * 256 + r;
+  const int q0 = P.c.cu[b], nq = P.c.cu[b + 1] - q0;
+  if (!chunk_in_bounds(P, q0, nq, P.c.lengths[b]) || row >= nq * P.group) return;
+  const float2* ml = P.part_ml + static_cast<long long>(unsplit) * P.split * 256 + r;
+  const float4* po = reinterpret_cast<const float4*>(P.part_o) + (static_cast<long long>(unsplit) * P.split * (D / 4) + four) * 256 + r;
+  float m = -INFINITY, l = 0.0f;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int i0 = 0; i0 < P.split; i0 += kBatch) {
+    float2 x[kBatch];
+    float4 v[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      x[u] = make_float2(-INFINITY, 0.0f);
+      v[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (i0 + u < P.split) x[u] = ml[256 * (i0 + u)], v[u] = po[static_cast<long long>(i0 + u) * (D / 4) * 256];
+    }
+    float mb = m;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) mb = fmaxf(mb, x[u].x);
+    const float back = part_factor(make_float2(m, l), mb);
+    m = mb;
+    l *= back, o.x *= back, o.y *= back, o.z *= back, o.w *= back;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      if (x[u].x == -INFINITY && x[u].y == 0.0f) continue;  // saw no key: v may be anything
+      const float f = part_factor(x[u], m);
+      l = fmaf(f, x[u].y, l);
+      o.x = fmaf(f, v[u].x, o.x), o.y = fmaf(f, v[u].y, o.y), o.z = fmaf(f, v[u].z, o.z), o.w = fmaf(f, v[u].w, o.w);
+    }
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no visible key: zeros
+  const int tok = row / P.group, head = kvh * P.group + row - tok * P.group;
+  *reinterpret_cast<uint2*>(P.out + (static_cast<long long>(q0 + tok) * P.q_heads + head) * D + 4 * four) =
+      make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+}
+
+namespace {
+template <int D>
+cudaError_t launch_chunk(const Kv4AttnParams& p, unsigned unsplit, cudaStream_t stream) {
+  cudaError_t e = launch_pdl(kv4_chunk_kernel<D>, dim3(unsplit * p.split, 1, 1), ChunkShape<D>::kThreads, ChunkShape<D>::kSmem, stream, p);
+  if (e != cudaSuccess || p.split == 1) return e;
+  return launch_pdl(kv4_chunk_join_kernel<D>, dim3(unsplit * 8, D / 32, 1), 256, 0, stream, p);
+}
+}  // namespace
+
+cudaError_t launch_kv4_chunk(Kv4AttnParams p, int head_dim, cudaStream_t stream) {
+  const unsigned max_tiles = (p.max_new * p.group + 255) / 256, unsplit = max_tiles * p.c.kv_heads * p.c.seqs;
+  p.ordered = p.split == 1 && unsplit > static_cast<unsigned>(sm_count()) && max_tiles * p.c.seqs <= kChunkOrdered;
+  return head_dim == 128 ? launch_chunk<128>(p, unsplit, stream) : launch_chunk<64>(p, unsplit, stream);
 }
 
 cudaError_t kv4_chunk_prepare_device() {

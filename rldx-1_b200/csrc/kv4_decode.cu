@@ -20,7 +20,7 @@
 // Work is split evenly over one wave of CTAs, whatever the lengths: a segment is one (sequence, kv
 // head, tile of columns) with the units that it can see, all segments stand in one line and each
 // CTA takes the same share of it, found by a prefix sum over the sequences that every CTA makes
-// for itself.  Inside a CTA each of 8 warps takes every eighth unit with its own bulk-copy ring,
+// for itself.  Inside a CTA each of 4 warps takes every fourth unit with its own bulk-copy ring,
 // running maximum, sum and accumulator, so nothing is exchanged until the warps' results meet in
 // shared memory at a segment's end.  A segment cut between CTAs is joined by a second kernel, in
 // the CTAs' order, so the result does not depend on timing.
@@ -580,13 +580,67 @@ __global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? kDecResident : kDecR
   if (threadIdx.x == 0 && !P.whole && !P.by_segment && !began) P.part_head[cta] = make_int4(0, 0, 0, 1);
 }
 
-// Joins the segments that were cut between CTAs: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s
-// over the parts, eight at a time so that their loads overlap.  Few segments with many parts
+// What a part with reference maximum x.x and sum x.y counts against the maximum m: nothing if it saw no token.
+__device__ __forceinline__ float part_factor(float2 x, float m) {
+  return x.x == -INFINITY && x.y == 0.0f ? 0.0f : ex2_approx(x.x - (m == -INFINITY ? 0.0f : m));
+}
+
+// out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s over parts from, from + step, ..., eight at a time so
+// that their loads overlap: a warp's running maximum, sum and D / 32 channels a lane.  Part i stands in row
+// row(i) of part_o and part_ml.  A part that saw no token may hold anything in part_o.
+template <int D, typename Row>
+__device__ __forceinline__ void join_parts(const Kv4AttnParams& P, Row row, int from, int step, int parts, float& m, float& l,
+                                           float (&o)[D / 32]) {
+  constexpr int kVec = D / 32, kBatch = 8;
+  const int lane = threadIdx.x & 31;
+  m = -INFINITY, l = 0.0f;
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) o[e] = 0.0f;
+  for (int i0 = from; i0 < parts; i0 += kBatch * step) {
+    float2 x[kBatch];
+    float v[kBatch][kVec];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int i = i0 + u * step;
+      x[u] = make_float2(-INFINITY, 0.0f);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) v[u][e] = 0.0f;
+      if (i < parts) {
+        x[u] = P.part_ml[row(i)];
+        const float* src = P.part_o + row(i) * D + lane * kVec;
+        if constexpr (kVec == 4) {
+          const float4 y = *reinterpret_cast<const float4*>(src);
+          v[u][0] = y.x, v[u][1] = y.y, v[u][2] = y.z, v[u][3] = y.w;
+        } else {
+          const float2 y = *reinterpret_cast<const float2*>(src);
+          v[u][0] = y.x, v[u][1] = y.y;
+        }
+      }
+    }
+    float mb = m;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) mb = fmaxf(mb, x[u].x);
+    const float back = part_factor(make_float2(m, l), mb);
+    l *= back;
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) o[e] *= back;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      if (x[u].x == -INFINITY && x[u].y == 0.0f) continue;
+      const float f = part_factor(x[u], mb);
+      l = fmaf(f, x[u].y, l);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) o[e] = fmaf(f, v[u][e], o[e]);
+    }
+    m = mb;
+  }
+}
+// Joins the segments that were cut between CTAs.  Few segments with many parts
 // (P.by_segment): CTA (i, y) takes column y of segment i, its 16 warps every 16th part.  Otherwise CTA i
 // takes the segment that begins in CTA i of the decode kernel and goes on, a warp per column.
 template <int D>
 __global__ void __launch_bounds__(512) kv4_combine_kernel(const __grid_constant__ Kv4AttnParams P, int cols) {
-  constexpr int kVec = D / 32, kBatch = 8;  // channels of a lane, parts loaded at once
+  constexpr int kVec = D / 32;  // channels of a lane
   __shared__ float s_o[16][D], s_l[16], s_m[16];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   griddep_wait();
@@ -604,47 +658,8 @@ __global__ void __launch_bounds__(512) kv4_combine_kernel(const __grid_constant_
   if (col >= ncols) return;
   // the first CTA kept its part as one that goes on, the others as one that began earlier
   auto slot = [&](int i) { return (2LL * (cta + i) + (i == 0 ? 1 : 0)) * cols + col; };
-  auto factor = [](float2 x, float m) { return x.x == -INFINITY && x.y == 0.0f ? 0.0f : ex2_approx(x.x - (m == -INFINITY ? 0.0f : m)); };
-  float m = -INFINITY, l = 0.0f, o[kVec];
-#pragma unroll
-  for (int e = 0; e < kVec; ++e) o[e] = 0.0f;
-  for (int i0 = from; i0 < parts; i0 += kBatch * split) {
-    float2 x[kBatch];
-    float v[kBatch][kVec];
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int i = i0 + u * split;
-      x[u] = make_float2(-INFINITY, 0.0f);
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) v[u][e] = 0.0f;
-      if (i < parts) {
-        x[u] = P.part_ml[slot(i)];
-        const float* src = P.part_o + slot(i) * D + lane * kVec;
-        if constexpr (kVec == 4) {
-          const float4 y = *reinterpret_cast<const float4*>(src);
-          v[u][0] = y.x, v[u][1] = y.y, v[u][2] = y.z, v[u][3] = y.w;
-        } else {
-          const float2 y = *reinterpret_cast<const float2*>(src);
-          v[u][0] = y.x, v[u][1] = y.y;
-        }
-      }
-    }
-    float mb = m;
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) mb = fmaxf(mb, x[u].x);
-    const float back = factor(make_float2(m, l), mb);
-    l *= back;
-#pragma unroll
-    for (int e = 0; e < kVec; ++e) o[e] *= back;
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const float f = factor(x[u], mb);
-      l = fmaf(f, x[u].y, l);
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) o[e] = fmaf(f, v[u][e], o[e]);
-    }
-    m = mb;
-  }
+  float m, l, o[kVec];
+  join_parts<D>(P, slot, from, split, parts, m, l, o);
   if (P.by_segment) {  // the warps' sums meet
 #pragma unroll
     for (int e = 0; e < kVec; ++e) s_o[warp][lane * kVec + e] = o[e];
@@ -658,13 +673,13 @@ __global__ void __launch_bounds__(512) kv4_combine_kernel(const __grid_constant_
     for (int e = 0; e < kVec; ++e) o[e] = 0.0f;
 #pragma unroll
     for (int w = 0; w < 16; ++w) {
-      const float f = factor(make_float2(s_m[w], s_l[w]), m);
+      const float f = part_factor(make_float2(s_m[w], s_l[w]), m);
       l = fmaf(f, s_l[w], l);
 #pragma unroll
       for (int e = 0; e < kVec; ++e) o[e] = fmaf(f, s_o[w][lane * kVec + e], o[e]);
     }
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no visible token: zeros
   const int row = c0 + col, tok = row / P.group;
   const long long orow = static_cast<long long>(head.x + tok) * P.q_heads + head.z * P.group + row - tok * P.group;
   __nv_bfloat16* dst = P.out + orow * D + lane * kVec;
@@ -734,26 +749,53 @@ cudaError_t kv4_prepare_device() {
 
 namespace {
 struct DecodePlan {
-  int cols, ctas, whole;  // cols 0: kv4_chunk_kernel
+  int cols, ctas, whole;  // cols 0: kv4_chunk_kernel, its keys shared by `split` CTAs
+  int split;
   uint64_t part_rows, bytes;  // workspace of unfinished segments
 };
 
-// Columns per CTA, and one wave of resident CTAs (two per SM with 8 columns, one with 16), or
+// Columns per CTA, and one wave of resident CTAs (four per SM with 8 columns, two with 16), or
 // fewer when not every warp could have a unit.  Up to kDecWholeUnits units a segment is left
-// whole: the few rounds that a warp then takes cost less than the join's launch.
+// whole: the few rounds that a warp then takes cost less than the join's launch (one sequence of
+// 705 tokens: 9.2 us whole, 11.1 us cut and joined).
 constexpr int kDecWholeUnits = 48;
-constexpr int kDecMaxRows = 32;  // rows of a kv head and sequence beyond which kv4_chunk_kernel takes over
+// Which kernel, and how many CTAs share the keys of a tile of rows.  In steps of a 16-column tile over one
+// unit (1.2 ns of the whole GPU with d = 128, 0.9 with 64) this file's kernel takes about kDecBase + tiles
+// (units + kDecStart), spread evenly whatever the shape; kv4_chunk_kernel takes kChunkUnit (units + 10) for
+// each wave of its CTAs of 256 rows (kChunkUnit2 with more than 128 rows: two query tiles), however few of a
+// wave there are, and with keys shared out kChunkJoin + kChunkJoinTile for each 128 rows of a part.  d = 128, 8
+// kv heads, us here / there with one CTA a tile / with as many as the rule takes: 1 x 8192 tokens, 96 rows 25
+// / 144 / 22, 256 rows 51 / 186 / 28; 8 x 8192, 64 rows 87 / 147 / -, 128 rows 164 / 148 / 98, 256 rows 320 / 191 /
+// 114; 8 x 512, 256 rows 47 / 22 / -, 28 if two shared; 32 x 2048, 32 rows 55 / 90 / -, 64 rows 101 / 90 / -, 256
+// rows 378 / 114 / -.  Up to kDecMaxRows rows it was faster here at every shape.
+constexpr int kDecMaxRows = 32;
+constexpr long long kDecBase = 5000, kChunkUnit = 500, kChunkUnit2 = 640, kChunkJoin = 2000, kChunkJoinTile = 20;
+constexpr int kChunkShare = 8;  // units of a part at least
 DecodePlan decode_plan(const rldx_kv4_cache& c, int q_heads, int max_new, int max_len, int window, int sinks) {
   DecodePlan p;
-  const int group = q_heads / c.kv_heads;
+  const long long rows = static_cast<long long>(max_new) * (q_heads / c.kv_heads);
   p = {};
-  if (max_new * group > kDecMaxRows) return p;
-  p.cols = max_new * group <= 8 ? 8 : 16;
-  const long long tiles = (static_cast<long long>(max_new) * group + p.cols - 1) / p.cols;
+  p.cols = rows <= 8 ? 8 : 16;
+  const long long tiles = (rows + p.cols - 1) / p.cols;
   long long keys = max_len;
   if (window > 0) keys = std::min<long long>(keys, static_cast<long long>(window) + max_new + std::min(sinks, max_len) + 3 * kKv4Unit);
   const long long units = (keys + kKv4Unit - 1) / kKv4Unit;
   const long long segments = tiles * c.kv_heads * std::min(c.seqs, kDecMaxSeqs);
+  if (rows > kDecMaxRows) {
+    const long long heads = static_cast<long long>(c.kv_heads) * c.seqs, ctas = (rows + 255) / 256 * heads;
+    long long least = kDecBase + tiles * heads * (units + kDecStart);
+    for (int split = 1; split == 1 || (split * ctas <= 2 * sm_count() && units >= split * kChunkShare); ++split) {
+      const long long waves = (split * ctas + sm_count() - 1) / sm_count();
+      const long long cost = waves * (rows > 128 ? kChunkUnit2 : kChunkUnit) * ((units + split - 1) / split + 10) +
+                             (split > 1 ? kChunkJoin + kChunkJoinTile * split * ctas * (rows > 128 ? 2 : 1) : 0);
+      if (cost < least) least = cost, p.cols = 0, p.split = split;
+    }
+    if (p.cols == 0) {
+      p.part_rows = p.split > 1 ? 256ull * ctas * p.split : 0;
+      p.bytes = p.part_rows * (static_cast<uint64_t>(c.head_dim) * 4 + 8);
+      return p;
+    }
+  }
   const int wave = (p.cols == 8 ? kDecResident : kDecResident / 2) * sm_count();
   p.whole = units <= kDecWholeUnits;
   p.ctas = static_cast<int>(std::min<long long>(wave, p.whole ? segments : (units * segments + kDecWarps - 1) / kDecWarps));
@@ -820,6 +862,7 @@ int rldx_kv4_attention(const rldx_kv4_cache* cache, const rldx_kv4_attention_des
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.max_new = a->max_new;
   p.whole = plan.whole;
+  p.split = plan.split;
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + plan.part_rows * d);
   p.part_head = reinterpret_cast<int4*>(p.part_ml + plan.part_rows);

@@ -308,6 +308,70 @@ def test_nan_of_a_hidden_token_stays_hidden(cuda, new):
             assert bool(torch.isnan(out[i].float()).any()) == sees, (window, i)
 
 
+@pytest.mark.parametrize("hq,hkv,d,page", HEADS)
+@pytest.mark.parametrize("new,old", [([40, 1, 0, 17] * 6, [30, 0, 5, 160] * 6), ([200, 0, 9], [1400, 70, 3000]), ([67], [5000]),
+                                     ([530, 31], [0, 600])])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (33, 5), (1100, 0)])
+def test_chunk_forms(cuda, hq, hkv, d, page, new, old, window, sinks):
+    """Many sequences (longest tiles first), and few whose keys are shared out between CTAs and joined."""
+    g = torch.Generator(device=cuda).manual_seed(hq + d + sum(new) + window)
+    lens = [a + b for a, b in zip(new, old)]
+    cache, table, lengths = filled_cache(cuda, lens, hkv, d, page, g, fill=0xFF)
+    q = torch.randn(sum(new), hq, d, device=cuda, generator=g).mul(1.5).to(BF)
+    cu = cumulative(cuda, new)
+    out = ops.kv4_attention(q, cache, table, lengths, cu, max_new=max(new), max_len=max(lens), window=window, sinks=sinks)
+    again = ops.kv4_attention(q, cache, table, lengths, cu, max_new=max(new), max_len=max(lens), window=window, sinks=sinks)
+    torch.cuda.synchronize()
+    assert ops.device_error() == 0
+    assert torch.equal(out, again)
+    # every row would take minutes in 64 bits: the first and last eight of a sequence and every 29th between
+    cum = cu.tolist()
+    for b in range(len(new)):
+        rows = [i for i in range(new[b]) if i < 8 or i >= new[b] - 8 or i % 29 == 0]
+        for i in rows:
+            at = cum[b] + i
+            length = torch.tensor([lens[b] - new[b] + i + 1], dtype=I32, device=cuda)
+            check_attention(q[at: at + 1], cache, table[b: b + 1], length, cumulative(cuda, [1]), out[at: at + 1], window, sinks)
+
+
+@pytest.mark.parametrize("new,old", [([300, 2], [1200, 10]), ([40] * 20, [60] * 20)])
+def test_chunk_nan_stays_hidden(cuda, new, old):
+    """NaN in K and V of one token of the first sequence reaches the rows that see it and no other, whole or shared out."""
+    g = torch.Generator(device=cuda).manual_seed(new[0])
+    d, hkv, hq = 128, 2, 8
+    lens = [a + b for a, b in zip(new, old)]
+    cache, table, lengths = filled_cache(cuda, lens, hkv, d, 64, g, fill=0xFF)
+    for bad in (old[0] + 3, 1):
+        qkv = torch.full((1, 3 * hkv * d), math.nan, device=cuda).to(BF)
+        one = torch.ones(d, device=cuda).to(BF)
+        ops.qkv_rope_append(qkv, one, one, torch.ones(1, d, device=cuda), torch.zeros(1, d, device=cuda),
+                            torch.zeros(1, dtype=I32, device=cuda), cache, table[:1],
+                            torch.tensor([bad + 1], dtype=I32, device=cuda), cumulative(cuda, [1]), q_heads=hkv)
+        q = torch.randn(sum(new), hq, d, device=cuda, generator=g).to(BF)
+        for window in (5, 0):
+            out = ops.kv4_attention(q, cache, table, lengths, cumulative(cuda, new), max_new=max(new), max_len=max(lens), window=window)
+            p = old[0] + torch.arange(new[0], device=cuda)
+            sees = torch.zeros_like(p, dtype=torch.bool)
+            for x in {bad, old[0] + 3}:
+                sees |= (p >= x) & ((p - x < window) if window else torch.ones_like(sees))
+            nan = torch.isnan(out.float())
+            assert torch.equal(nan[: new[0]].all(2).all(1), sees) and torch.equal(nan[: new[0]].any(2).any(1), sees)
+            assert not bool(nan[new[0]:].any())
+
+
+def test_chunk_rows_without_keys(cuda):
+    """Rows before position 0 of a chunk whose keys are shared out see nothing: zeros."""
+    g = torch.Generator(device=cuda).manual_seed(8)
+    cache, table, _ = filled_cache(cuda, [1000], 2, 128, 64, g)
+    new, hidden = 600, 130
+    lengths = torch.tensor([new - hidden], dtype=I32, device=cuda)
+    q = torch.randn(new, 16, 128, device=cuda, generator=g).to(BF)
+    out = ops.kv4_attention(q, cache, table, lengths, cumulative(cuda, [new]), max_new=new, max_len=1000)
+    assert bool((out[:hidden] == 0).all())
+    check_attention(q[hidden: hidden + 40], cache, table, torch.tensor([40], dtype=I32, device=cuda), cumulative(cuda, [40]),
+                    out[hidden: hidden + 40])
+
+
 @pytest.mark.parametrize("new", [1, 30])
 @pytest.mark.parametrize("mag", [1e-30, 1e-6, 1e6, 1e30])
 def test_query_range(cuda, mag, new):
