@@ -11,11 +11,11 @@
 //
 // A cluster of CTAs holds a row in shared memory, so the logits are read once (one bulk copy a CTA).
 // The last token kept is found in one of two ways:
-//   - top-k up to about a thousand: each CTA finds the k / CTAs-th largest of its threads' maxima (four a
-//     thread), by bisection of the ordered bits; the least of these is a lower bound of the k-th
-//     largest logit.  The tokens that reach it, a little more than k, go to rank 0's list.  Up to 128 one
-//     of its warps sorts (bitonic, ordered bits and id in one word), scans and draws from alone; of more
-//     it finds the cut as below and tells the others.
+//   - top-k up to 1536: each CTA finds the k / CTAs-th largest of its threads' maxima (four a thread), by
+//     ranking or by bisection of the ordered bits; the least of these is a lower bound of the k-th largest
+//     logit.  The tokens that reach it, a little more than k, go to rank 0's list, and the other CTAs are
+//     done.  Up to 128 are compared with one another, a thread each; of more rank 0 finds the cut as
+//     below and draws by bins of ids.
 //   - otherwise by histogram: 1024 bins linear in -d (every bin holds a run of the order), then by the
 //     ordered bits of the logit inside the bin where count or weight crosses, until one value is left;
 //     of the tokens that share it the first few by id stay.  Bins hold counts (top-k) or weights
@@ -31,6 +31,7 @@ constexpr int kSampMaxCluster = 8;
 constexpr int kSampMaxSlice = 49152;  // tokens of a CTA: its sums of 16-bit halves stay below 2^32
 constexpr float kSampReach = 22.5f;   // of the bins; exp(-22.2) < 2^-32: weights beyond are 0
 constexpr int kSampList = 2048;       // candidates of a row
+constexpr int kSampFew = 128;         // of them that a thread each can compare with all
 typedef unsigned long long u64;
 constexpr unsigned int kErrSampleTimeout = 0x530;
 
@@ -68,7 +69,7 @@ struct SampleShared {
   u64 found[4];                      // rank 0's answer, written to every CTA
   u64 red[32][2];
   uint32_t red32[32];
-  uint32_t flag;
+  uint32_t flag, count;
   uint64_t loaded;  // the bulk copy
 };
 
@@ -94,6 +95,40 @@ __device__ __forceinline__ void unpack(const uint4& u, const __nv_bfloat16*, flo
   unpack_bf16x2(u.z, x[4], x[5]);
   unpack_bf16x2(u.w, x[6], x[7]);
 }
+// The larger ones of two vectors, halves of a word apart (NaN gives way to any number).
+__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// Four running maxima of a thread: of bf16 as two words.
+struct MaximaBf16 {
+  uint32_t a = 0xff80ff80u, b = 0xff80ff80u;  // -inf
+  __device__ __forceinline__ void add(const uint4& u) {
+    a = max_bf16x2(a, max_bf16x2(u.x, u.y));
+    b = max_bf16x2(b, max_bf16x2(u.z, u.w));
+  }
+  __device__ __forceinline__ void get(float (&x)[4]) const { unpack_bf16x2(a, x[0], x[1]), unpack_bf16x2(b, x[2], x[3]); }
+};
+struct MaximaFloat {
+  float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  __device__ __forceinline__ void add(const uint4& u) {
+    x[0] = fmaxf(x[0], __uint_as_float(u.x)), x[1] = fmaxf(x[1], __uint_as_float(u.y));
+    x[2] = fmaxf(x[2], __uint_as_float(u.z)), x[3] = fmaxf(x[3], __uint_as_float(u.w));
+  }
+  __device__ __forceinline__ void get(float (&y)[4]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = x[i];
+  }
+};
+template <typename T>
+struct MaximaOf {
+  using Type = MaximaBf16;
+};
+template <>
+struct MaximaOf<float> {
+  using Type = MaximaFloat;
+};
 __device__ __forceinline__ void unpack(const uint4& u, const float*, float (&x)[4]) {
   x[0] = __uint_as_float(u.x), x[1] = __uint_as_float(u.y), x[2] = __uint_as_float(u.z), x[3] = __uint_as_float(u.w);
 }
@@ -368,37 +403,6 @@ struct Sampler {
   }
 
   // ---- a few candidates ----
-  // Sorts the first n (a power of two) of a warp's 128 values descending: lane i holds places 4 i .. 4 i + 3.
-  __device__ __forceinline__ static void sort(u64 (&v)[4], int n) {
-    const int i0 = 4 * (threadIdx.x & 31);
-    // of a pair of places a < b, a takes the larger where (a & k) == 0
-    auto meet = [](u64& x, u64& y, bool larger_first) {
-      if ((x < y) == larger_first) {
-        const u64 z = x;
-        x = y, y = z;
-      }
-    };
-#pragma unroll 1
-    for (int k = 2; k <= n; k <<= 1)
-#pragma unroll 1
-      for (int j = k >> 1; j > 0; j >>= 1) {
-        if (j >= 4) {
-          const bool take_max = ((i0 & k) == 0) == ((i0 & j) == 0);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const u64 other = __shfl_xor_sync(0xffffffffu, v[e], j >> 2);
-            v[e] = (v[e] < other) == take_max ? other : v[e];
-          }
-        } else if (j == 2) {
-          meet(v[0], v[2], (i0 & k) == 0);
-          meet(v[1], v[3], (i0 & k) == 0);
-        } else {
-          meet(v[0], v[1], (i0 & k) == 0);
-          meet(v[2], v[3], ((i0 + 2) & k) == 0);
-        }
-      }
-  }
-
   // A value that at least `want` of the CTA's tokens reach (-inf: not found), its low bits dropped.
   __device__ __forceinline__ float reached_by(int want, const float (&best)[4]) {
     uint32_t b[4], at = 0u;
@@ -452,93 +456,138 @@ struct Sampler {
     return at <= order_bits(-INFINITY) ? -INFINITY : order_value(at);
   }
 
-  // The tokens that reach `bound` go to rank 0's list.  Returns their number, or -1 if they are too many.
+  // The tokens that reach `bound` go to rank 0's list, in any order.  Returns their number, or -1 if they are
+  // too many.
   __device__ __forceinline__ int gather_candidates(float bound) {
-    u64 mine = 0, none = 0, all, other;
-    each([&](float x) { mine += x >= bound && x > -INFINITY; });
-    u64 upto = mine;
-    block_scan(upto, none, &all, &other);
-    all_gather(all, 0);
+    if (threadIdx.x == 0) s.count = 0u;
+    __syncthreads();
+    for (int v = threadIdx.x; v < nvec; v += NT) {
+      typename MaximaOf<T>::Type maxima;
+      float best[4];
+      maxima.add(row[v]);
+      maxima.get(best);
+      if (!(fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3])) >= bound)) continue;
+      float x[kVec];
+      load(v, x);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e)
+        if (x[e] >= bound && x[e] > -INFINITY) {
+          const uint32_t at = atomicAdd(&s.count, 1u);
+          if (at < kSampList) s.list[at] = (static_cast<u64>(order_bits(x[e])) << 32) | static_cast<uint32_t>(~(first_id + v * kVec + e));
+        }
+    }
+    __syncthreads();
+    const uint32_t mine = s.count;
+    all_gather(mine, 0);
     u64 base = 0, total = 0;
     for (int r = 0; r < cluster; ++r) {
       if (r < rank) base += slot(r, 0);
       total += slot(r, 0);
     }
-    if (total > kSampList) return -1;
-    if (mine) {
-      uint32_t at = mapa_shared(smem_u32(s.list), 0) + 8 * static_cast<uint32_t>(base + upto - mine);
-      for (int v = threadIdx.x; v < nvec; v += NT) {
-        float x[kVec];
-        load(v, x);
-        bool any = false;
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) any |= x[e] >= bound;
-        if (any) {
-#pragma unroll
-          for (int e = 0; e < kVec; ++e)
-            if (x[e] >= bound && x[e] > -INFINITY) {
-              st_cluster_u64(at, (static_cast<u64>(order_bits(x[e])) << 32) | static_cast<uint32_t>(~(first_id + v * kVec + e)));
-              at += 8;
-            }
-        }
-      }
+    if (total > kSampList) {  // rank 0's part may have run into the row's bins
+      if (rank == 0)
+        for (int i = threadIdx.x; i < kSampBins; i += NT) s.g[i] = 0;
+      cluster_sync();
+      return -1;
+    }
+    if (rank > 0) {  // rank 0's stand where they are
+      const uint32_t at = mapa_shared(smem_u32(s.list), 0) + 8 * static_cast<uint32_t>(base);
+      for (uint32_t i = threadIdx.x; i < mine; i += NT) st_cluster_u64(at + 8 * i, s.list[i]);
     }
     cluster_sync();
     return static_cast<int>(total);
   }
 
-  // The whole draw by one warp from rank 0's n <= 128 candidates, which contain the first top_k tokens of
-  // positive weight.
-  __device__ __forceinline__ void draw_from_list(const SampleParams& P, int r, int n, int top_k, float top_p, u64 least) {
-    constexpr int kE = 4;
-    const int lane = threadIdx.x & 31, p0 = kE * lane;
-    auto power = [](int m) { return m <= 2 ? 2 : 1 << (32 - __clz(m - 1)); };
-    // inclusive sums in the order of places, and of all
-    auto scan = [&](u64 x, u64* all) {
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const u64 y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
+  // The whole draw by rank 0 from its n <= kSampFew candidates, which contain the first top_k tokens of positive
+  // weight: thread i takes candidate i and compares it with all.
+  __device__ __forceinline__ void draw_from_few(const SampleParams& P, int r, int n, int top_k, float top_p, u64 least) {
+    u64* ws = s.list + kSampFew;  // weights
+    const int i = threadIdx.x;
+    const u64 mine = i < n ? s.list[i] : 0;
+    const u64 w = i < n ? weight(order_value(static_cast<uint32_t>(mine >> 32))) : 0;
+    if (i < n) ws[i] = w;
+    __syncthreads();
+    u64 before = 0;  // in the order
+    int place = 0;
+    if (i < n) {
+#pragma unroll 4
+      for (int k = 0; k < n; ++k)
+        if (s.list[k] > mine) before += ws[k], ++place;
+      if (place == min(n, top_k) - 1) s.found[0] = before + w;  // what top-k left
+    }
+    __syncthreads();
+    const u64 level = top_p < 1.0f ? last_below(fmaxf(top_p, 0.0f), s.found[0]) : ~0ull;
+    if (i < n && !(place < top_k && before <= level && w >= least)) ws[i] = 0;
+    __syncthreads();
+    if (i < n && ws[i] > 0) {
+      u64 sum = 0, kept = 0;
+      before = 0;  // in the order of ids (the low word is ~id)
+#pragma unroll 4
+      for (int k = 0; k < n; ++k) {
+        const u64 x = ws[k];
+        sum += x, kept += x > 0;
+        if (static_cast<uint32_t>(s.list[k]) > static_cast<uint32_t>(mine)) before += x;
       }
-      *all = __shfl_sync(0xffffffffu, x, 31);
-      return x;
-    };
-    u64 v[kE], w[kE], sum = 0, whole;
-#pragma unroll
-    for (int e = 0; e < kE; ++e) v[e] = p0 + e < n ? s.list[p0 + e] : 0;
-    sort(v, power(n));
-    n = min(n, top_k);
-#pragma unroll
-    for (int e = 0; e < kE; ++e) {
-      w[e] = p0 + e < n ? weight(order_value(static_cast<uint32_t>(v[e] >> 32))) : 0;
-      sum += w[e];
+      const u64 goal = goal_of(P.u[r], sum);
+      if (before <= goal && goal < before + w) write(P, r, static_cast<int>(~static_cast<uint32_t>(mine)), w, sum, kept);
     }
-    u64 before = scan(sum, &whole) - sum;
-    const u64 level = top_p < 1.0f ? last_below(fmaxf(top_p, 0.0f), whole) : ~0ull;
-    u64 mine = 0, kept, kept_sum;  // the kept ones are a prefix of the order
-    sum = 0;
+  }
+
+  // The draw by rank 0 among its candidates (kE in each thread's registers: logits and ids) above the cut and its
+  // ties: bins of ids, 1024 over the vocabulary and then the ids of one, hold weights and numbers of tied tokens.
+  template <int kE>
+  __device__ __forceinline__ void draw_from_list(const SampleParams& P, int r, const float (&x)[kE], const int (&id)[kE], const Cut& cut,
+                                                 u64 least) {
+    const u64 tie_weight = (cut.ties > 0 && cut.weight >= least) ? cut.weight : 0;
+    const u64 ties = tie_weight ? cut.ties : 0;
+    uint32_t* tied = reinterpret_cast<uint32_t*>(s.g);
+    u64 w[kE], count = 0;
 #pragma unroll
     for (int e = 0; e < kE; ++e) {
-      const bool keep = w[e] > 0 && before <= level && w[e] >= least;
-      before += w[e];
-      if (keep) ++mine, sum += w[e];
-      v[e] = keep ? (v[e] << 32) | (v[e] >> 32) : 0;  // ~id, ordered bits: descending is ascending id
+      w[e] = x[e] > cut.x ? weight(x[e]) : 0;
+      if (w[e] < least) w[e] = 0;
+      count += w[e] > 0;
     }
-    scan(mine, &kept);
-    scan(sum, &kept_sum);
-    sort(v, power(static_cast<int>(kept)));
-    sum = 0;
+    count = block_sum(count);
+    auto reach = [&](u64 above, u64 tied) { return above + min(ties, tied) * tie_weight; };
+    int base = 0, shift = max(0, 22 - __clz(P.vocab - 1));  // bins of 2^shift ids
+    u64 wb = 0, tb = 0, whole = 0, goal = 0;
+    for (bool first = true;; first = false) {
+      for (int i = threadIdx.x; i < kSampBins; i += NT) s.lo[i] = s.hi[i] = tied[i] = 0u;
+      __syncthreads();
 #pragma unroll
-    for (int e = 0; e < kE; ++e) {
-      w[e] = p0 + e < static_cast<int>(kept) ? weight(order_value(static_cast<uint32_t>(v[e]))) : 0;
-      sum += w[e];
-    }
-    before = scan(sum, &whole) - sum;
-    const u64 goal = goal_of(P.u[r], kept_sum);
+      for (int e = 0; e < kE; ++e) {
+        const int bin = (id[e] - base) >> shift;
+        if (id[e] < base || bin >= kSampBins) continue;
+        if (w[e]) add_weight(bin, w[e]);
+        if (ties && x[e] == cut.x) atomicAdd(&tied[bin], 1u);
+      }
+      __syncthreads();
+      constexpr int kPer = kSampBins / NT;
+      const int b0 = threadIdx.x * kPer;
+      u64 ws = 0, ts = 0, all_w, all_t;
 #pragma unroll
-    for (int e = 0; e < kE; ++e) {
-      if (before <= goal && goal < before + w[e]) write(P, r, static_cast<int>(~static_cast<uint32_t>(v[e] >> 32)), w[e], kept_sum, kept);
-      before += w[e];
+      for (int i = 0; i < kPer; ++i) ws += bin_sum(b0 + i), ts += tied[b0 + i];
+      u64 wi = ws, ti = ts;
+      block_scan(wi, ti, &all_w, &all_t);
+      if (first) whole = reach(all_w, all_t), goal = goal_of(P.u[r], whole), count += min(ties, all_t);
+      wi += wb - ws, ti += tb - ts;  // before this thread's bins
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const u64 wn = wi + bin_sum(b0 + i), tn = ti + tied[b0 + i];
+        if (reach(wi, ti) <= goal && goal < reach(wn, tn)) {
+          if (shift == 0) {
+            write(P, r, base + b0 + i, wn > wi ? wn - wi : tie_weight, whole, count);
+          } else {
+            s.found[0] = b0 + i, s.found[1] = wi, s.found[2] = ti;
+          }
+        }
+        wi = wn, ti = tn;
+      }
+      if (shift == 0) return;
+      __syncthreads();
+      base += static_cast<int>(s.found[0]) << shift, wb = s.found[1], tb = s.found[2];
+      shift = 0;
     }
   }
 
@@ -683,12 +732,11 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 1 : 4) sample_kernel(const __g
   __syncthreads();  // the barrier is set up, the edges are written
   const bool ok = mbar_wait(&s.loaded, 0u, kErrSampleTimeout);
   // ---- maximum (NaN is passed over here and weighs nothing below) and, for a greedy row, its first id ----
-  float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-  for (int v = threadIdx.x; v < nvec; v += NT) {
-    float x[kVec];
-    S.load(v, x);
-#pragma unroll
-    for (int e = 0; e < kVec; ++e) best[e & 3] = fmaxf(best[e & 3], x[e]);
+  float best[4];
+  {
+    typename MaximaOf<T>::Type maxima;
+    for (int v = threadIdx.x; v < nvec; v += NT) maxima.add(vecs[v]);
+    maxima.get(best);
   }
   const uint32_t mine = order_bits(fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3])));
   uint32_t m = __reduce_max_sync(0xffffffffu, mine);
@@ -759,39 +807,32 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 1 : 4) sample_kernel(const __g
   Cut cut{};
   if (n < 0) {
     cut = S.template find_cut<false>(in_row, top_k < P.vocab ? top_k : 0, top_p);
-  } else if (n <= 128) {
-    if (rank == 0 && threadIdx.x < 32) S.draw_from_list(P, r, n, top_k, top_p, least);
+  } else if (n <= kSampFew) {
+    if (rank == 0) S.draw_from_few(P, r, n, top_k, top_p, least);
     return;
   } else {
-    // rank 0 finds the cut among the candidates, a few in each thread's registers, and tells the others
-    if (rank == 0) {
-      constexpr int kE = kSampList / NT;
-      float x[kE];
+    if (rank > 0) return;
+    constexpr int kE = kSampList / NT;
+    float x[kE];
+    int id[kE];
 #pragma unroll
-      for (int e = 0; e < kE; ++e) {
-        const int i = threadIdx.x + e * NT;
-        x[e] = i < n ? order_value(static_cast<uint32_t>(s.list[i] >> 32)) : -INFINITY;
-      }
-      __syncthreads();
-      for (int i = threadIdx.x; i < kSampBins; i += NT) s.g[i] = 0;
-      cut = S.template find_cut<true>(
-          [&](auto f) {
-#pragma unroll
-            for (int e = 0; e < kE; ++e) f(x[e]);
-          },
-          top_k, top_p);
-      __syncthreads();  // every warp has read the last answer in `found`
-      if (threadIdx.x < cluster) {
-        const uint32_t at = mapa_shared(smem_u32(s.found), threadIdx.x);
-        st_cluster_u64(at, __float_as_uint(cut.x));
-        st_cluster_u64(at + 8, cut.ties);
-        st_cluster_u64(at + 16, cut.weight);
-      }
+    for (int e = 0; e < kE; ++e) {
+      const int i = threadIdx.x + e * NT;
+      const u64 c = i < n ? s.list[i] : 0;
+      x[e] = i < n ? order_value(static_cast<uint32_t>(c >> 32)) : -INFINITY;
+      id[e] = i < n ? static_cast<int>(~static_cast<uint32_t>(c)) : -1;
     }
-    cluster_sync();
-    cut.x = __uint_as_float(static_cast<uint32_t>(s.found[0]));
-    cut.ties = static_cast<uint32_t>(s.found[1]);
-    cut.weight = s.found[2];
+    __syncthreads();
+    for (int i = threadIdx.x; i < kSampBins; i += NT) s.g[i] = 0;
+    cut = S.template find_cut<true>(
+        [&](auto f) {
+#pragma unroll
+          for (int e = 0; e < kE; ++e) f(x[e]);
+        },
+        top_k, top_p);
+    __syncthreads();  // every warp has read the last answer in `found`
+    S.template draw_from_list<kE>(P, r, x, id, cut, least);
+    return;
   }
   S.draw_from_row(P, r, cut, least);
 }
