@@ -68,6 +68,7 @@ struct SampleShared {
   u64 slots[2][kSampMaxCluster][2];  // all-gather, two phases
   u64 found[4];                      // rank 0's answer, written to every CTA
   u64 red[32][2];
+  u64 warps[16][2];  // sums of a warp's vectors
   uint32_t red32[32];
   uint32_t flag, count;
   uint64_t loaded;  // the bulk copy
@@ -143,13 +144,24 @@ struct Sampler {
   int nvec, first_id;  // vectors held, id of the first one's first token (negative: padding)
   int rank, cluster, phase;
   float top, temp, inv, scale;  // maximum; scaled temperature, its reciprocal and the scale
+  float floor;                  // tokens below weigh 0
 
   __device__ __forceinline__ void load(int v, float (&x)[kVec]) const { unpack(row[v], static_cast<const T*>(nullptr), x); }
+  __device__ __forceinline__ static float largest(const uint4& u) {
+    typename MaximaOf<T>::Type maxima;
+    float x[4];
+    maxima.add(u);
+    maxima.get(x);
+    return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+  }
+  // The tokens of the vectors that hold one of at least `least`.
   template <typename F>
-  __device__ __forceinline__ void each(F f) const {
+  __device__ __forceinline__ void each(float least, F f) const {
     for (int v = threadIdx.x; v < nvec; v += NT) {
+      const uint4 u = row[v];
+      if (!(largest(u) >= least)) continue;
       float x[kVec];
-      load(v, x);
+      unpack(u, static_cast<const T*>(nullptr), x);
 #pragma unroll
       for (int e = 0; e < kVec; ++e) f(x[e]);
     }
@@ -299,18 +311,18 @@ struct Sampler {
 
   // Finds the cut where the count (or weight) of the order passes `level` among the tokens of positive
   // weight above `from` and its ties.  With `share` >= 0 the level comes from the whole weight, which
-  // is returned in *whole.  False: never.  `each` visits the CTA's tokens.
+  // is returned in *whole.  False: never.  `each` visits the CTA's tokens, those of at least its first argument.
   template <bool kAlone, typename Each>
   __device__ __forceinline__ bool find(Each each, bool by_count, u64 level, float share, const Cut& from, Cut* out, u64* whole) {
     clear();
     if (by_count) {
-      each([&](float x) {
+      each(floor, [&](float x) {
         if (!(x > from.x)) return;
         const float d = distance(x);
         if (weighs(d)) atomicAdd(&s.lo[bin_of(d)], 1u);
       });
     } else {
-      each([&](float x) {
+      each(fmaxf(floor, from.x), [&](float x) {
         const float d = distance(x);
         const u64 w = x > from.x ? weight_of(d) : 0;
         if (w) add_weight(bin_of(d), w);
@@ -331,7 +343,7 @@ struct Sampler {
     // the bin's range of ordered bits (first a little more than its range of quotients)
     const float q_hi = -bin * (kSampReach / kSampBins) * 0.9999f + 1e-6f, q_lo = -(bin + 1) * (kSampReach / kSampBins) * 1.0001f - 1e-6f;
     uint32_t lo = 0xffffffffu, hi = 0u;
-    each([&](float x) {
+    each(floor, [&](float x) {
       const float q = (x - top) * scale * inv;
       if (!(q >= q_lo && q <= q_hi)) return;
       if (!(x > from.x)) return;
@@ -356,7 +368,7 @@ struct Sampler {
       const int shift = max(0, 32 - __clz(hi - lo) - 10);
       const float x_lo = order_value(lo), x_hi = order_value(hi);
       clear();
-      each([&](float x) {
+      each(x_lo, [&](float x) {
         if (!(x >= x_lo && x <= x_hi && x > from.x)) return;
         const float d = distance(x);
         if (!weighs(d)) return;
@@ -462,13 +474,10 @@ struct Sampler {
     if (threadIdx.x == 0) s.count = 0u;
     __syncthreads();
     for (int v = threadIdx.x; v < nvec; v += NT) {
-      typename MaximaOf<T>::Type maxima;
-      float best[4];
-      maxima.add(row[v]);
-      maxima.get(best);
-      if (!(fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3])) >= bound)) continue;
+      const uint4 u = row[v];
+      if (!(largest(u) >= bound)) continue;
       float x[kVec];
-      load(v, x);
+      unpack(u, static_cast<const T*>(nullptr), x);
 #pragma unroll
       for (int e = 0; e < kVec; ++e)
         if (x[e] >= bound && x[e] > -INFINITY) {
@@ -607,35 +616,41 @@ struct Sampler {
     const u64 tie_weight = (cut.ties > 0 && cut.weight >= least) ? cut.weight : 0;
     const uint32_t ties = tie_weight ? cut.ties : 0;
     const uint32_t least32 = static_cast<uint32_t>(max(1ull, min(least, 0xffffffffull)));
-    // weights of one vector's kept tokens above the cut; most vectors have none where the cut is high
-    auto kept_of = [&](const float (&x)[kVec], uint32_t (&k)[kVec]) {
-      bool any = false;
+    const float low = fmaxf(cut.x, floor);
+    // weights of one vector's kept tokens above the cut; false: it has none, nor a tied one
+    auto kept_of = [&](const uint4& u, float (&x)[kVec], uint32_t (&k)[kVec]) {
+      if (!(largest(u) >= low)) return false;
+      unpack(u, static_cast<const T*>(nullptr), x);
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) k[e] = 0u, any |= x[e] > cut.x;
-      if (any) {
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-          const uint32_t t = weight32(distance(x[e]));
-          k[e] = x[e] > cut.x && t >= least32 ? t : 0u;
-        }
+      for (int e = 0; e < kVec; ++e) {
+        const uint32_t t = weight32(distance(x[e]));
+        k[e] = x[e] > cut.x && t >= least32 ? t : 0u;
       }
+      return true;
     };
+    // a warp takes consecutive vectors, so that the search below has one warp's to look through
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = (nvec + kWarps - 1) / kWarps;
     u64 sum = 0, num = 0;  // num: count above, and ties in the low half
     uint32_t above = 0u, tied = 0u;
-    for (int v = threadIdx.x; v < nvec; v += NT) {
+    for (int v = warp * share + lane; v < min(nvec, (warp + 1) * share); v += 32) {
       float x[kVec];
       uint32_t k[kVec];
-      load(v, x);
-      kept_of(x, k);
+      if (!kept_of(row[v], x, k)) continue;
 #pragma unroll
       for (int e = 0; e < kVec; ++e) sum += widen(k[e]), above += k[e] > 0u;
       if (ties)
 #pragma unroll
         for (int e = 0; e < kVec; ++e) tied += x[e] == cut.x;
     }
-    num = (static_cast<u64>(above) << 32) | tied;
-    sum = block_sum(sum);
-    num = block_sum(num);
+    above = __reduce_add_sync(0xffffffffu, above), tied = __reduce_add_sync(0xffffffffu, tied);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    __syncthreads();
+    if (lane == 0) s.warps[warp][0] = sum, s.warps[warp][1] = (static_cast<u64>(above) << 32) | tied;
+    __syncthreads();
+    sum = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) sum += s.warps[w][0], num += s.warps[w][1];
     all_gather(sum, num);
     u64 whole = static_cast<u64>(ties) * tie_weight, count = ties;
     for (int k = 0; k < cluster; ++k) whole += slot(k, 0), count += slot(k, 1) >> 32;
@@ -650,21 +665,27 @@ struct Sampler {
       wb = w1, tb = t1;
     }
     if (rank != owner) return;
-    for (int base = 0; base < nvec; base += NT) {
+    int w0 = 0;
+    for (; w0 < kWarps - 1; ++w0) {
+      const u64 w1 = wb + s.warps[w0][0], t1 = tb + static_cast<uint32_t>(s.warps[w0][1]);
+      if (reach(w1, t1) > goal) break;
+      wb = w1, tb = t1;
+    }
+    const int end = min(nvec, (w0 + 1) * share);
+    for (int base = w0 * share; base < end; base += NT) {
       const int v = base + threadIdx.x;
       float x[kVec];
       uint32_t k[kVec];
       u64 ws = 0, ts = 0, all_w, all_t;
-      if (v < nvec) {
-        load(v, x);
-        kept_of(x, k);
+      const bool some = v < end && kept_of(row[v], x, k);
+      if (some) {
 #pragma unroll
         for (int e = 0; e < kVec; ++e) ws += widen(k[e]), ts += ties > 0u && x[e] == cut.x;
       }
       u64 wi = ws, ti = ts;
       block_scan(wi, ti, &all_w, &all_t);
       wi += wb - ws, ti += tb - ts;  // before this vector
-      if (v < nvec && reach(wi, ti) <= goal && goal < reach(wi + ws, ti + ts)) {
+      if (some && reach(wi, ti) <= goal && goal < reach(wi + ws, ti + ts)) {
         bool done = false;
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
@@ -728,7 +749,7 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 1 : 4) sample_kernel(const __g
   // the list holds what the bound lets through, a little more than top_k
   const bool few = !greedy && top_k > 0 && top_k < P.vocab && top_k <= kSampList * 3 / 4;
   for (int i = threadIdx.x; i < kSampBins; i += NT) s.g[i] = 0;
-  Sampler<T, NT> S{s, vecs, nvec, first_id, rank, cluster, 0, 0.0f, 0.0f, 0.0f, 1.0f};
+  Sampler<T, NT> S{s, vecs, nvec, first_id, rank, cluster, 0, 0.0f, 0.0f, 0.0f, 1.0f, -INFINITY};
   __syncthreads();  // the barrier is set up, the edges are written
   const bool ok = mbar_wait(&s.loaded, 0u, kErrSampleTimeout);
   // ---- maximum (NaN is passed over here and weighs nothing below) and, for a greedy row, its first id ----
@@ -797,12 +818,13 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 1 : 4) sample_kernel(const __g
   // the normal numbers
   S.temp = fminf(fmaxf(temp, 1e-30f), 3e38f);
   S.scale = S.temp < 1e-20f ? 18446744073709551616.0f : S.temp > 1e20f ? 5.4210108624275222e-20f : 1.0f;  // 2^64, 2^-64
+  S.floor = S.top - 22.21f * S.temp;  // exp(-22.2) < 2^-32, and room for what this rounds
   S.temp *= S.scale;
   S.inv = __fdiv_rn(1.0f, S.temp);
 
   // w >= min_p 2^32 for whole w
   const u64 least = static_cast<u64>(ceil(static_cast<double>(min_p > 0.0f ? fminf(min_p, 1.0f) : 0.0f) * 4294967296.0));
-  auto in_row = [&](auto f) { S.each(f); };
+  auto in_row = [&](float least, auto f) { S.each(least, f); };
   const int n = few ? S.gather_candidates(order_value(least_bound)) : -1;
   Cut cut{};
   if (n < 0) {
@@ -825,7 +847,7 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 1 : 4) sample_kernel(const __g
     __syncthreads();
     for (int i = threadIdx.x; i < kSampBins; i += NT) s.g[i] = 0;
     cut = S.template find_cut<true>(
-        [&](auto f) {
+        [&](float, auto f) {
 #pragma unroll
           for (int e = 0; e < kE; ++e) f(x[e]);
         },
