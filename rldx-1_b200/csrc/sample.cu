@@ -17,10 +17,12 @@
 //     done.  Up to 128 are compared with one another, a thread each; of more rank 0 finds the cut as
 //     below and draws by bins of ids.
 //   - otherwise by histogram: 1024 bins linear in -d (every bin holds a run of the order), then by the
-//     ordered bits of the logit inside the bin where count or weight crosses, until one value is left;
+//     ordered bits of the logit (16 of bf16) inside the bin where count or weight crosses, until one value is left;
 //     of the tokens that share it the first few by id stay.  Bins hold counts (top-k) or weights
 //     (top-p: the low 16 and high 17 bits of a weight in two 32-bit sums); CTAs add theirs to rank 0's
 //     through distributed shared memory, which finds the crossing and tells the others.
+#include <cfloat>
+
 #include "host_util.h"
 
 namespace rldx {
@@ -134,6 +136,16 @@ __device__ __forceinline__ void unpack(const uint4& u, const float*, float (&x)[
   x[0] = __uint_as_float(u.x), x[1] = __uint_as_float(u.y), x[2] = __uint_as_float(u.z), x[3] = __uint_as_float(u.w);
 }
 
+// The order of the logits of a type: bf16 has 16 bits of it.
+template <typename T>
+__device__ __forceinline__ uint32_t key_bits(float x) {
+  return order_bits(x) >> (sizeof(T) == 2 ? 16 : 0);
+}
+template <typename T>
+__device__ __forceinline__ float key_float(uint32_t k) {
+  return sizeof(T) == 2 ? order_value((k << 16) | ((k >> 15) ? 0u : 0xffffu)) : order_value(k);
+}
+
 // NT threads of one CTA of a row's cluster.
 template <typename T, int NT>
 struct Sampler {
@@ -147,6 +159,8 @@ struct Sampler {
   float floor;                  // tokens below weigh 0
 
   __device__ __forceinline__ void load(int v, float (&x)[kVec]) const { unpack(row[v], static_cast<const T*>(nullptr), x); }
+  __device__ __forceinline__ static uint32_t key_of(float x) { return key_bits<T>(x); }
+  __device__ __forceinline__ static float key_value(uint32_t k) { return key_float<T>(k); }
   __device__ __forceinline__ static float largest(const uint4& u) {
     typename MaximaOf<T>::Type maxima;
     float x[4];
@@ -340,45 +354,27 @@ struct Sampler {
     if (share >= 0.0f) level = last_below(share, *whole);
     const int bin = static_cast<int>(s.found[0]);
     u64 before = s.found[1], sum = s.found[2];
-    // the bin's range of ordered bits (first a little more than its range of quotients)
-    const float q_hi = -bin * (kSampReach / kSampBins) * 0.9999f + 1e-6f, q_lo = -(bin + 1) * (kSampReach / kSampBins) * 1.0001f - 1e-6f;
-    uint32_t lo = 0xffffffffu, hi = 0u;
-    each(floor, [&](float x) {
-      const float q = (x - top) * scale * inv;
-      if (!(q >= q_lo && q <= q_hi)) return;
-      if (!(x > from.x)) return;
-      const float d = distance(x);
-      if (bin_of(d) != bin || !weighs(d)) return;
-      const uint32_t k = order_bits(x);
-      lo = min(lo, k), hi = max(hi, k);
-    });
-    const uint32_t from_key = order_bits(from.x);
-    if (has_ties && tie_bin == bin) lo = min(lo, from_key), hi = max(hi, from_key);
-    lo = __reduce_min_sync(0xffffffffu, lo);
-    hi = __reduce_max_sync(0xffffffffu, hi);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) s.red[threadIdx.x >> 5][0] = lo, s.red[threadIdx.x >> 5][1] = hi;
-    __syncthreads();
-    for (int w = 0; w < kWarps; ++w) lo = min(lo, static_cast<uint32_t>(s.red[w][0])), hi = max(hi, static_cast<uint32_t>(s.red[w][1]));
-    if constexpr (!kAlone) {
-      all_gather(lo, hi);
-      for (int r = 0; r < cluster; ++r) lo = min(lo, static_cast<uint32_t>(slot(r, 0))), hi = max(hi, static_cast<uint32_t>(slot(r, 1)));
-    }
+    // keys that hold the bin's tokens, and a little more than them
+    const float span = scale == 1.0f ? temp : temp / scale, slack = fabsf(top) * 0x1p-20f;
+    const float x_min = top - (bin + 1) * (kSampReach / kSampBins) * span * 1.0001f - slack;
+    const float x_max = fminf(top, top - bin * (kSampReach / kSampBins) * span * 0.9999f + slack);
+    uint32_t lo = key_of(fmaxf(x_min, -FLT_MAX)), hi = key_of(fmaxf(x_max, -FLT_MAX));
+    const uint32_t from_key = key_of(from.x);
     while (lo != hi) {
       const int shift = max(0, 32 - __clz(hi - lo) - 10);
-      const float x_lo = order_value(lo), x_hi = order_value(hi);
+      const float x_lo = key_value(lo), x_hi = key_value(hi);
       clear();
       each(x_lo, [&](float x) {
         if (!(x >= x_lo && x <= x_hi && x > from.x)) return;
         const float d = distance(x);
-        if (!weighs(d)) return;
-        const int b = static_cast<int>((hi - order_bits(x)) >> shift);
+        if (!weighs(d) || bin_of(d) != bin) return;
+        const int b = static_cast<int>((hi - key_of(x)) >> shift);
         if (by_count)
           atomicAdd(&s.lo[b], 1u);
         else
           add_weight(b, weight_of(d));
       });
-      const bool tie_in = has_ties && from_key >= lo && from_key <= hi;
+      const bool tie_in = has_ties && tie_bin == bin && from_key >= lo && from_key <= hi;
       __syncthreads();
       if (rank == 0 && threadIdx.x == 0 && tie_in) s.g[(hi - from_key) >> shift] += tie_sum;
       if (tie_in && !kAlone) cluster_sync();
@@ -389,7 +385,7 @@ struct Sampler {
       const uint32_t width = (1u << shift) - 1u;
       lo = hi - lo > width ? hi - width : lo;
     }
-    out->x = order_value(lo);
+    out->x = key_value(lo);
     out->weight = weight(out->x);
     out->before = before;
     out->ties = static_cast<uint32_t>(by_count ? sum : sum / out->weight);  // find_cut keeps as many as fit

@@ -111,6 +111,45 @@ def test_ties_go_to_the_lowest_id(cuda, dtype, vocab):
     run_and_check(x, u, t=[0.0] * 8)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("vocab", [300, 5000, 33000])
+def test_list_lengths_and_ties_at_the_cut(cuda, dtype, vocab):
+    """Cuts by count from one token to more than any list holds, on values that many tokens share, with top-p and min-p after."""
+    g = torch.Generator(device=cuda).manual_seed(vocab)
+    ks = [1, 2, 90, 100, 127, 128, 129, 200, 1000, 1500, 1536, 1537, 2500]
+    rows = 3 * len(ks)
+    x = torch.randn(rows, vocab, device=cuda, generator=g)
+    x[len(ks): 2 * len(ks)] = (2 * x[len(ks): 2 * len(ks)]).round()  # a few values only
+    x[2 * len(ks):] *= 4
+    u = torch.rand(rows, device=cuda, generator=g).tolist()
+    pick = lambda values: [values[i % len(values)] for i in range(rows)]  # noqa: E731
+    run_and_check(x.to(dtype), u, t=pick([1.0, 0.7, 1.9, 0.25]), k=ks * 3)
+    run_and_check(x.to(dtype), u, t=pick([1.0, 0.7, 1.9]), k=ks * 3, p=pick([0.9, 0.5, 0.999, 0.05, 1.0]), m=pick([0.0, 0.1]))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_masks_of_the_lowest_value_and_large_logits(cuda, dtype):
+    g = torch.Generator(device=cuda).manual_seed(4)
+    vocab, low = 9000, torch.finfo(dtype).min
+    x = torch.randn(10, vocab, device=cuda, generator=g)
+    x[0] = low  # every token masked: all equal
+    x[1, 5:] = low
+    x[2, ::2] = low
+    x[3] = x[3] * 1e30
+    x[4] = x[4] * 100 + 1e6
+    x[5] = x[5] * 100 - 1e6
+    x[6] = -x[6].abs() * 1e-30
+    x[7] = x[7] * 1e-3 - 3e4
+    x[8, : vocab - 2] = -math.inf
+    x[9] = low
+    x[9, 8999] = -low
+    x = x.to(dtype)
+    u = torch.rand(10, device=cuda, generator=g).tolist()
+    for t in (1.0, 0.01, 1e-30, 1e30, 3e38):
+        for k, p in ((0, 0.5), (0, 0.9), (50, 0.9), (4000, 1.0), (4000, 0.7), (0, 1.0)):
+            run_and_check(x, u, t=[t] * 10, k=[k] * 10, p=[p] * 10)
+
+
 def test_special_rows(cuda):
     """Infinities, NaN, rows that a mask empties, values of a type's range, draws at the ends."""
     v = 300
