@@ -11,9 +11,8 @@
 //
 // A cluster of CTAs holds a row in shared memory, so the logits are read once (one bulk copy a CTA).
 // The last token kept is found in one of two ways:
-//   - top-k up to 1536: each CTA finds the k / CTAs-th largest of its threads' maxima (four a thread), by
-//     ranking or by bisection of the ordered bits; the least of these is a lower bound of the k-th largest
-//     logit.  The tokens that reach it, a little more than k, go to rank 0's list, and the other CTAs are
+//   - top-k up to 1536: each CTA finds, by bins, a value that the k / CTAs largest of its threads' maxima (four
+//     a thread) reach; the least of these is a lower bound of the k-th largest logit.  The tokens that reach it, a little more than k, go to rank 0's list, and the other CTAs are
 //     done.  Up to 128 are compared with one another, a thread each; of more rank 0 finds the cut as
 //     below and draws by bins of ids.
 //   - otherwise by histogram: 1024 bins linear in -d (every bin holds a run of the order), then by the
@@ -411,57 +410,35 @@ struct Sampler {
   }
 
   // ---- a few candidates ----
-  // A value that at least `want` of the CTA's tokens reach (-inf: not found), its low bits dropped.
-  __device__ __forceinline__ float reached_by(int want, const float (&best)[4]) {
-    uint32_t b[4], at = 0u;
+  // A value that at least `want` of the CTA's tokens reach, from the threads' four maxima each in bins of the
+  // distance from the CTA's largest; or, if these do not show so many, one below which every token weighs 0.
+  __device__ __forceinline__ float reached_by(int want, const float (&best)[4], float most, float t) {
+    constexpr int kBins = 256;
+    const int i = threadIdx.x, lane = i & 31, warp = i >> 5;
+    if (i < kBins) s.lo[i] = 0u;
+    if (i == 0) s.flag = kBins - 1;
+    __syncthreads();
+    const float per = kBins / (kSampReach * t);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) b[i] = order_bits(best[i]);
-    if (2 * want <= 4 * kWarps) {
-      // few: the want-th largest of the warps' four maxima each
-#pragma unroll
-      for (int i = 0; i < 4; ++i) b[i] = __reduce_max_sync(0xffffffffu, b[i]);
-      if ((threadIdx.x & 31) == 0)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) reinterpret_cast<uint32_t*>(s.list)[4 * (threadIdx.x >> 5) + i] = b[i];
-      __syncthreads();
-      // every warp ranks the 4 kWarps <= 64 values, two a lane, by (value, place)
-      const uint32_t* all = reinterpret_cast<const uint32_t*>(s.list);
-      const int lane = threadIdx.x & 31;
-      uint32_t found = 0u;
-#pragma unroll
-      for (int h = 0; h < (4 * kWarps + 31) / 32; ++h) {
-        const int place = lane + 32 * h;
-        const uint32_t mine = all[place];
-        int rank_of = 0;
-#pragma unroll 8
-        for (int i = 0; i < 4 * kWarps; ++i) rank_of += all[i] > mine || (all[i] == mine && i < place);
-        if (rank_of == want - 1) found = mine;
-      }
-      at = __reduce_max_sync(0xffffffffu, found);
-      __syncthreads();  // the list's place is used again
-    } else {
-      // the want-th largest of the threads' four, 16 bits (exponent and 7 of the mantissa: all that bf16
-      // has), two a round: a warp counts up to 128 for each of three trial values
-#pragma unroll 1
-      for (int bit = 30; bit >= 16; bit -= 2) {
-        uint32_t n = 0u;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          n += (b[i] >= (at | 1u << bit) ? 1u : 0u) + (b[i] >= (at | 2u << bit) ? 1u << 8 : 0u) + (b[i] >= (at | 3u << bit) ? 1u << 16 : 0u);
-        n = __reduce_add_sync(0xffffffffu, n & 0x00ff00ffu) | __reduce_add_sync(0xffffffffu, n & 0x0000ff00u);
-        uint32_t* red = s.red32 + 16 * (bit >> 1 & 1);  // (NT <= 512: 16 warps)
-        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = n;
-        __syncthreads();
-        int n1 = 0, n2 = 0, n3 = 0;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const uint32_t x = red[w];
-          n1 += x & 0xffu, n2 += x >> 8 & 0xffu, n3 += x >> 16;
-        }
-        at |= (n3 >= want ? 3u : n2 >= want ? 2u : n1 >= want ? 1u : 0u) << bit;
-      }
+    for (int e = 0; e < 4; ++e) {
+      const float q = best[e] == most ? 0.0f : (most - best[e]) * per;
+      if (q < kBins) atomicAdd(&s.lo[static_cast<int>(q)], 1u);
     }
-    return at <= order_bits(-INFINITY) ? -INFINITY : order_value(at);
+    __syncthreads();
+    const int n = i < kBins ? s.lo[i] : 0;
+    int upto = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    if (lane == 31) s.red32[warp] = upto;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kBins / 32; ++w) upto += w < warp ? s.red32[w] : 0;
+    if (i < kBins && upto - n < want && want <= upto) s.flag = i;
+    __syncthreads();
+    return most - (s.flag + 1) / per * 1.0001f - fabsf(most) * 0x1p-20f;  // a little below the bin
   }
 
   // The tokens that reach `bound` go to rank 0's list, in any order.  Returns their number, or -1 if they are
@@ -779,7 +756,7 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 1 : 4) sample_kernel(const __g
     for (int w = 0; w < kWarps; ++w) id = min(id, s.red32[w]);
   } else if (few) {
     __syncthreads();
-    bound = S.reached_by((top_k + cluster - 1) / cluster, best);
+    bound = S.reached_by((top_k + cluster - 1) / cluster, best, order_value(m), fminf(fmaxf(temp, 1e-30f), 3e38f));
   }
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   S.all_gather((static_cast<u64>(m) << 32) | static_cast<uint32_t>(~id), (static_cast<u64>(ok ? 0u : 1u) << 32) | order_bits(bound));
