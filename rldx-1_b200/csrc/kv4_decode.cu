@@ -24,6 +24,12 @@
 // running maximum, sum and accumulator, so nothing is exchanged until the warps' results meet in
 // shared memory at a segment's end.  A segment cut between CTAs is joined by a second kernel, in
 // the CTAs' order, so the result does not depend on timing.
+//
+// Measured: 64 sequences of up to 8192 tokens, 16 / 2 heads, d = 128, 120 MB of cache: 30.2 us with the join
+// (27 without), 3.95 TB/s, 0.60 of the copy's rate; 3 x 131077 26 us, 0.56.  Four warps a CTA and four CTAs an
+// SM, 32 KB of copies in flight a CTA: 33.0 us against 35.7 with eight warps and two CTAs.  What is left is the
+// start (lengths, prefix sums, q: about 3 us before the first unit is used), the shared-memory merge at a
+// segment's end and the join's launch (3.5 us).
 #include <type_traits>
 
 #include "host_util.h"
@@ -40,7 +46,7 @@ constexpr float kDecGrow = 2.0f;  // lazy move of the reference maximum (log2 un
 constexpr int kDecMaxSeqs = 1024;  // sequences of one launch (their prefix sums stand in shared memory)
 
 // A segment's start counts as this many units of a CTA's share: its lookups, the wait for its first units
-// and the merge of the one before.
+// and the merge of the one before (64 x 8192: 0 / 6 / 12 / 16 / 24 / 36 units 33.0 / 32.0 / 30.9 / 30.9 / 31.5 / 32.6 us).
 constexpr int kDecStart = 12;
 
 // What a CTA works on: units [u0, u0 + m) of the n that columns [c0, c0 + ncols) of kv head kvh of a

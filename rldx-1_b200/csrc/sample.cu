@@ -12,14 +12,20 @@
 // A cluster of CTAs holds a row in shared memory, so the logits are read once (one bulk copy a CTA).
 // The last token kept is found in one of two ways:
 //   - top-k up to 1536: each CTA finds, by bins, a value that the k / CTAs largest of its threads' maxima (four
-//     a thread) reach; the least of these is a lower bound of the k-th largest logit.  The tokens that reach it, a little more than k, go to rank 0's list, and the other CTAs are
-//     done.  Up to 128 are compared with one another, a thread each; of more rank 0 finds the cut as
-//     below and draws by bins of ids.
+//     a thread) reach; the least of these is a lower bound of the k-th largest logit.  The tokens that reach
+//     it, a little more than k, go to rank 0's list, and the other CTAs are done.  Up to 128 are compared
+//     with one another, a thread each; of more rank 0 finds the cut as below and draws by bins of ids.
 //   - otherwise by histogram: 1024 bins linear in -d (every bin holds a run of the order), then by the
 //     ordered bits of the logit (16 of bf16) inside the bin where count or weight crosses, until one value is left;
 //     of the tokens that share it the first few by id stay.  Bins hold counts (top-k) or weights
 //     (top-p: the low 16 and high 17 bits of a weight in two 32-bit sums); CTAs add theirs to rank 0's
 //     through distributed shared memory, which finds the crossing and tells the others.
+//
+// Measured, bf16 rows of 151680, 1 row / 256 rows in us: greedy 3.1 / 21 (78 MB: 12 at the copy's rate), top-k 20
+// 7.9 / 44, top-k 1000 14.8 / 84, top-k 3000 (by histogram) 22 / 158, temperature alone 11.6 / 86, top-p 0.9 at
+// T = 1, 28914 kept, 27.6 / 197.  Few rows wait on the chain of passes and cluster barriers; many are bound by
+// instructions, the correctly rounded quotient and exponential of every token that can weigh anything
+// (about 40 a token and pass), and by the histogram's atomics.
 #include <cfloat>
 
 #include "host_util.h"
@@ -904,7 +910,9 @@ extern "C" int rldx_sample(const void* logits, int64_t ld, int rows, int vocab, 
   p.logprob = logprob;
   p.kept = kept;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // few CTAs: 512 threads each shorten a row's passes; more than a wave of them: 256, four to an SM
+  // Few CTAs: 512 threads each shorten a row's passes (1 x 151680 bf16, top-k 1000 14.8 us against 19.0, temperature
+  // alone 11.6 against 13.8).  More than two an SM: 256 threads, four CTAs to an SM (256 x 151680, mixed filters, 90 us
+  // against 120 with 512 threads, two to an SM).
   const bool wide = static_cast<long long>(rows) * p.cluster <= 2 * sm_count();
   cudaError_t e;
   if (logits_fp32)
