@@ -130,6 +130,6 @@ __device__ __forceinline__ Kv4Span kv4_span(int length, int nq, int tok_lo, int 
 
 cudaError_t launch_kv4_chunk(Kv4AttnParams p, int head_dim, cudaStream_t stream);
 cudaError_t kv4_chunk_prepare_device();
-cudaError_t launch_kv4_decode(const Kv4AttnParams& p, int head_dim, int cols, int ctas, cudaStream_t stream);
+cudaError_t launch_kv4_decode(const Kv4AttnParams& p, int head_dim, int cols, int warps, int ctas, cudaStream_t stream);
 
 }  // namespace rldx

@@ -20,7 +20,7 @@
 // Work is split evenly over one wave of CTAs, whatever the lengths: a segment is one (sequence, kv
 // head, tile of columns) with the units that it can see, all segments stand in one line and each
 // CTA takes the same share of it, found by a prefix sum over the sequences that every CTA makes
-// for itself.  Inside a CTA each of 4 warps takes every fourth unit with its own bulk-copy ring,
+// for itself.  Inside a CTA each of W = 4 (8) warps takes every W-th unit with its own bulk-copy ring,
 // running maximum, sum and accumulator, so nothing is exchanged until the warps' results meet in
 // shared memory at a segment's end.  A segment cut between CTAs is joined by a second kernel, in
 // the CTAs' order, so the result does not depend on timing.
@@ -38,8 +38,8 @@
 namespace rldx {
 
 namespace {
-constexpr int kDecWarps = 4;
-constexpr int kDecResident = 16 / kDecWarps;  // CTAs of 8 columns per SM (128 registers a thread)
+constexpr int kDecWarps = 4, kDecWarpsWide = 8;  // of a CTA; of one that has a short segment to itself
+constexpr int dec_resident(int warps, int cols) { return 128 / (warps * cols); }  // CTAs per SM (128 registers a thread)
 constexpr int kDecStages = 2;
 constexpr float kDecGrow = 2.0f;  // lazy move of the reference maximum (log2 units)
 
@@ -56,17 +56,17 @@ struct DecSegment {
   Kv4Span span;
 };
 
-template <int D, int NT>
+template <int D, int NT, int W>
 struct DecShape {
   static constexpr int kCols = 8 * NT;
-  static constexpr int kRing = kDecWarps * kDecStages * Kv4Unit<D>::kBytes;
+  static constexpr int kRing = W * kDecStages * Kv4Unit<D>::kBytes;
   static constexpr int kOLd = D + 4;  // floats of one column's partial result
-  static constexpr int kMerge = kDecWarps * kCols * kOLd * 4;
+  static constexpr int kMerge = W * kCols * kOLd * 4;
   static constexpr int kBody = kRing > kMerge ? kRing : kMerge;
-  static constexpr int kMl = kDecWarps * kCols * 8;  // (reference maximum, sum)
+  static constexpr int kMl = W * kCols * 8;  // (reference maximum, sum)
   static constexpr int kQWords = 4 * Kv4Unit<D>::kG + 3;  // a lane's fragments, sums, factors of 8 columns
   static constexpr int kQ = NT * kQWords * 32 * 4;
-  static constexpr size_t kSmem = kBody + kMl + kQ + 8 * kDecWarps * kDecStages + sizeof(DecSegment) + 4 * (kDecMaxSeqs + 1) + 12;
+  static constexpr size_t kSmem = kBody + kMl + kQ + 8 * W * kDecStages + sizeof(DecSegment) + 4 * (kDecMaxSeqs + 1) + 12;
 };
 
 // d += a b, and d = a b (no accumulator to clear).
@@ -134,11 +134,11 @@ __device__ __forceinline__ int sequence_units(const Kv4AttnParams& P, int b, int
   return n * P.c.kv_heads;
 }
 
-template <int D, int NT>
-__global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? kDecResident : kDecResident / 2)
+template <int D, int NT, int W>
+__global__ void __launch_bounds__(32 * W, dec_resident(W, 8 * NT))
     kv4_decode_kernel(const __grid_constant__ Kv4AttnParams P) {
   using U = Kv4Unit<D>;
-  using Sh = DecShape<D, NT>;
+  using Sh = DecShape<D, NT, W>;
   constexpr int G = U::kG;
   constexpr int kCols = Sh::kCols;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -146,12 +146,12 @@ __global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? kDecResident : kDecR
   float2* s_ml = reinterpret_cast<float2*>(smem + Sh::kBody);
   uint32_t* s_q = reinterpret_cast<uint32_t*>(smem + Sh::kBody + Sh::kMl);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Sh::kBody + Sh::kMl + Sh::kQ);
-  DecSegment& sg = *reinterpret_cast<DecSegment*>(bars + kDecWarps * kDecStages);
+  DecSegment& sg = *reinterpret_cast<DecSegment*>(bars + W * kDecStages);
   int* s_before = reinterpret_cast<int*>(&sg + 1);  // [seqs + 1] units before a sequence
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
 
-  if (threadIdx.x < kDecWarps * kDecStages) mbar_init(&bars[threadIdx.x], 1);
+  if (threadIdx.x < W * kDecStages) mbar_init(&bars[threadIdx.x], 1);
   if (threadIdx.x == 0) fence_mbar_init();
   griddep_wait();
   griddep_launch();
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? kDecResident : kDecR
   {
     int* s_warp = reinterpret_cast<int*>(s_ml);
     int before = 0;
-    for (int b0 = 0; b0 < P.c.seqs; b0 += 32 * kDecWarps) {
+    for (int b0 = 0; b0 < P.c.seqs; b0 += 32 * W) {
       const int b = b0 + threadIdx.x;
       const int n = b < P.c.seqs ? sequence_units(P, b, kCols) : 0;
       int inc = n;
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? kDecResident : kDecR
       __syncthreads();
       int mine = before + inc - n;
 #pragma unroll
-      for (int w = 0; w < kDecWarps; ++w) {
+      for (int w = 0; w < W; ++w) {
         if (w < warp) mine += s_warp[w];
         before += s_warp[w];
       }
@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? kDecResident : kDecR
     }
   }
   const int total = s_before[P.c.seqs];
-  const int quota = max(P.whole ? 1 : kDecWarps, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
+  const int quota = max(P.whole ? 1 : W, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
   const int cta = blockIdx.x;
   const int begin = min(total, cta * quota), end = min(total, begin + quota);
   const uint64_t policy = l2_policy_evict_first();
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? kDecResident : kDecR
 
     // lane i holds the i-th of this warp's next 32 units: its index in the pool, and in a ballot
     // whether every column sees every token of it
-    const int mine = (m - warp + kDecWarps - 1) / kDecWarps;
+    const int mine = (m - warp + W - 1) / W;
     int index = -1;
     unsigned clear = 0u;
     auto look = [&](int round) {
@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? kDecResident : kDecR
       index = -1;
       bool all = false;
       if (i < mine) {
-        const int u = span.unit(u0 + warp + kDecWarps * i), key0 = kKv4Unit * u, key1 = key0 + kKv4Unit - 1;
+        const int u = span.unit(u0 + warp + W * i), key0 = kKv4Unit * u, key1 = key0 + kKv4Unit - 1;
         if (span.count > 0) {
           index = kv4_unit_index(P.c, b, kvh, u);
           if (index < 0) record_error(kErrKv4Table);
@@ -401,7 +401,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? kDecResident : kDecR
         }
       }
       if constexpr (!kPlain) {
-        const int key0 = kKv4Unit * span.unit(u0 + warp + kDecWarps * i);
+        const int key0 = kKv4Unit * span.unit(u0 + warp + W * i);
         const bool have = __shfl_sync(0xffffffffu, index, i & 31) >= 0;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -548,16 +548,16 @@ __global__ void __launch_bounds__(32 * kDecWarps, NT == 1 ? kDecResident : kDecR
       began = !whole;
     }
     const long long slot = 2LL * cta + (u0 == 0 ? 1 : 0);  // 0: began in an earlier CTA; 1: goes on in the next
-    for (int i = threadIdx.x; i < ncols * (D / 4); i += 32 * kDecWarps) {
+    for (int i = threadIdx.x; i < ncols * (D / 4); i += 32 * W) {
       const int col = i / (D / 4), ch = i % (D / 4) * 4;
       float mm = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kDecWarps; ++w) mm = fmaxf(mm, s_ml[w * kCols + col].x);
+      for (int w = 0; w < W; ++w) mm = fmaxf(mm, s_ml[w * kCols + col].x);
       const float m_use = mm == -INFINITY ? 0.0f : mm;
       float l = 0.0f;
       float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-      for (int w = 0; w < kDecWarps; ++w) {
+      for (int w = 0; w < W; ++w) {
         const float2 ml = s_ml[w * kCols + col];
         if (ml.x == -INFINITY && ml.y == 0.0f) continue;  // saw no visible token
         const float f = ex2_approx(ml.x - m_use);
@@ -711,7 +711,7 @@ cudaError_t launch_pdl(K kernel, dim3 grid, int threads, size_t smem, cudaStream
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-template <int D, int NT>
+template <int D, int NT, int W>
 cudaError_t launch_decode(const Kv4AttnParams& whole, int ctas, cudaStream_t stream) {
   for (int b0 = 0; b0 < whole.c.seqs; b0 += kDecMaxSeqs) {
     Kv4AttnParams p = whole;
@@ -722,9 +722,9 @@ cudaError_t launch_decode(const Kv4AttnParams& whole, int ctas, cudaStream_t str
     p.tiles = (p.max_new * p.group + 8 * NT - 1) / (8 * NT);
     // a few segments are cut into many parts each: then a CTA of the join per segment and column
     p.by_segment = 16LL * p.tiles * p.c.kv_heads * p.c.seqs < ctas;
-    cudaError_t e = launch_pdl(kv4_decode_kernel<D, NT>, dim3(ctas, 1, 1), 32 * kDecWarps, DecShape<D, NT>::kSmem, stream, p);
+    cudaError_t e = launch_pdl(kv4_decode_kernel<D, NT, W>, dim3(ctas, 1, 1), 32 * W, DecShape<D, NT, W>::kSmem, stream, p);
     if (e != cudaSuccess) return e;
-    if (ctas == 1 || p.whole) continue;
+    if (p.whole) continue;
     e = p.by_segment ? launch_pdl(kv4_combine_kernel<D>, dim3(p.tiles * p.c.kv_heads * p.c.seqs, 8 * NT, 1), 512, 0, stream, p, 8 * NT)
                      : launch_pdl(kv4_combine_kernel<D>, dim3(ctas, 1, 1), 256 * NT, 0, stream, p, 8 * NT);
     if (e != cudaSuccess) return e;
@@ -734,14 +734,22 @@ cudaError_t launch_decode(const Kv4AttnParams& whole, int ctas, cudaStream_t str
 
 template <int D, int NT>
 cudaError_t decode_smem() {
-  return cudaFuncSetAttribute(kv4_decode_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              static_cast<int>(DecShape<D, NT>::kSmem));
+  cudaError_t e = cudaFuncSetAttribute(kv4_decode_kernel<D, NT, kDecWarps>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       static_cast<int>(DecShape<D, NT, kDecWarps>::kSmem));
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(kv4_decode_kernel<D, NT, kDecWarpsWide>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(DecShape<D, NT, kDecWarpsWide>::kSmem));
+  return e;
+}
+template <int D, int NT>
+cudaError_t launch_decode(const Kv4AttnParams& p, int warps, int ctas, cudaStream_t stream) {
+  return warps == kDecWarps ? launch_decode<D, NT, kDecWarps>(p, ctas, stream) : launch_decode<D, NT, kDecWarpsWide>(p, ctas, stream);
 }
 }  // namespace
 
-cudaError_t launch_kv4_decode(const Kv4AttnParams& p, int head_dim, int cols, int ctas, cudaStream_t stream) {
-  if (head_dim == 128) return cols == 8 ? launch_decode<128, 1>(p, ctas, stream) : launch_decode<128, 2>(p, ctas, stream);
-  return cols == 8 ? launch_decode<64, 1>(p, ctas, stream) : launch_decode<64, 2>(p, ctas, stream);
+cudaError_t launch_kv4_decode(const Kv4AttnParams& p, int head_dim, int cols, int warps, int ctas, cudaStream_t stream) {
+  if (head_dim == 128) return cols == 8 ? launch_decode<128, 1>(p, warps, ctas, stream) : launch_decode<128, 2>(p, warps, ctas, stream);
+  return cols == 8 ? launch_decode<64, 1>(p, warps, ctas, stream) : launch_decode<64, 2>(p, warps, ctas, stream);
 }
 
 cudaError_t kv4_prepare_device() {
@@ -756,15 +764,24 @@ cudaError_t kv4_prepare_device() {
 namespace {
 struct DecodePlan {
   int cols, ctas, whole;  // cols 0: kv4_chunk_kernel, its keys shared by `split` CTAs
-  int split;
+  int split, warps;
   uint64_t part_rows, bytes;  // workspace of unfinished segments
 };
 
-// Columns per CTA, and one wave of resident CTAs (four per SM with 8 columns, two with 16), or
-// fewer when not every warp could have a unit.  Up to kDecWholeUnits units a segment is left
-// whole: the few rounds that a warp then takes cost less than the join's launch (one sequence of
-// 705 tokens: 9.2 us whole, 11.1 us cut and joined).
-constexpr int kDecWholeUnits = 48;
+// Columns per CTA, and one wave of resident CTAs (16 warps per SM with 8 columns, 8 with 16), or fewer when not
+// every warp could have a unit.  A short segment is left whole, which spares the join (4 us with its launch):
+//   - up to kDecWholeUnits units where segments are many;
+//   - where a wave holds one each, with eight warps to a CTA, as long as a CTA's own time (4.5 us + 0.125 a unit, 0.09
+//     with d = 64) stays below that of the cut (9 us + 0.00073 a unit and segment), or kDecWholeUnitsShared where
+//     two CTAs share an SM.  us whole / cut, d = 128: 2 segments of 23 units 7.7 / 11.1, of 64 12.2 / 8.8; 128 of
+//     64 13.3 / 16.4, of 256 38.0 / 35.7; 192 with d = 64, of 64 13.2 / 15.0, of 128 22.0 / 21.2.  Four warps a
+//     CTA instead of eight: 2 of 23 9.0, of 48 12.9 against 10.2.
+constexpr int kDecWholeUnits = 48, kDecWholeUnitsShared = 110;
+bool dec_whole(long long segments, long long units, bool wide, int head_dim) {
+  if (!wide) return units <= kDecWholeUnits;
+  if (segments > sm_count()) return units <= kDecWholeUnitsShared;
+  return units <= (head_dim == 64 ? 50 : 36) + segments * (units + kDecStart) / 170;
+}
 // Which kernel, and how many CTAs share the keys of a tile of rows.  In steps of a 16-column tile over one
 // unit (1.2 ns of the whole GPU with d = 128, 0.9 with 64) this file's kernel takes about kDecBase + tiles
 // (units + kDecStart), spread evenly whatever the shape; kv4_chunk_kernel takes kChunkUnit (units + 10) for
@@ -802,10 +819,12 @@ DecodePlan decode_plan(const rldx_kv4_cache& c, int q_heads, int max_new, int ma
       return p;
     }
   }
-  const int wave = (p.cols == 8 ? kDecResident : kDecResident / 2) * sm_count();
-  p.whole = units <= kDecWholeUnits;
+  const bool wide = segments <= dec_resident(kDecWarpsWide, p.cols) * sm_count();
+  p.whole = dec_whole(segments, units, wide, c.head_dim);
+  p.warps = p.whole && wide ? kDecWarpsWide : kDecWarps;
+  const int wave = dec_resident(p.warps, p.cols) * sm_count();
   p.ctas = static_cast<int>(std::min<long long>(wave, p.whole ? segments : (units * segments + kDecWarps - 1) / kDecWarps));
-  p.part_rows = (p.ctas == 1 || p.whole) ? 0 : 2ull * p.ctas * p.cols;
+  p.part_rows = p.whole ? 0 : 2ull * p.ctas * p.cols;
   p.bytes = p.part_rows * (static_cast<uint64_t>(c.head_dim) * 4 + 8) + (p.part_rows ? 16ull * p.ctas : 0);
   return p;
 }
@@ -873,7 +892,7 @@ int rldx_kv4_attention(const rldx_kv4_cache* cache, const rldx_kv4_attention_des
   p.part_ml = reinterpret_cast<float2*>(p.part_o + plan.part_rows * d);
   p.part_head = reinterpret_cast<int4*>(p.part_ml + plan.part_rows);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e = plan.cols == 0 ? launch_kv4_chunk(p, d, st) : launch_kv4_decode(p, d, plan.cols, plan.ctas, st);
+  cudaError_t e = plan.cols == 0 ? launch_kv4_chunk(p, d, st) : launch_kv4_decode(p, d, plan.cols, plan.warps, plan.ctas, st);
   if (e != cudaSuccess) return cuda_fail(e, "kv4_attention launch");
   return RLDX_OK;
 }
