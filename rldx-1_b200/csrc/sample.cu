@@ -253,8 +253,9 @@ struct Sampler {
     for (int i = threadIdx.x; i < kSampBins; i += NT) s.lo[i] = s.hi[i] = 0u;
     __syncthreads();
   }
-  __device__ __forceinline__ void add_weight(int bin, u64 w) {
-    const uint32_t l = static_cast<uint32_t>(w) & 0xffffu, h = static_cast<uint32_t>(w >> 16);
+  __device__ __forceinline__ void add_weight(int bin, uint32_t t) {  // (2^32 - 1 is 2^32)
+    const bool full = t == 0xffffffffu;
+    const uint32_t l = full ? 0u : t & 0xffffu, h = full ? 0x10000u : t >> 16;
     if (l) atomicAdd(&s.lo[bin], l);
     if (h) atomicAdd(&s.hi[bin], h);
   }
@@ -343,8 +344,7 @@ struct Sampler {
     } else {
       each(fmaxf(floor, from.x), [&](float x) {
         const float d = distance(x);
-        const u64 w = x > from.x ? weight_of(d) : 0;
-        if (w) add_weight(bin_of(d), w);
+        add_weight(bin_of(d), x > from.x ? weight32(d) : 0u);
       });
     }
     const bool has_ties = from.ties > 0;  // the ties of the cut so far count as that many tokens
@@ -377,7 +377,7 @@ struct Sampler {
         if (by_count)
           atomicAdd(&s.lo[b], 1u);
         else
-          add_weight(b, weight_of(d));
+          add_weight(b, weight32(d));
       });
       const bool tie_in = has_ties && tie_bin == bin && from_key >= lo && from_key <= hi;
       __syncthreads();
@@ -529,12 +529,14 @@ struct Sampler {
     const u64 tie_weight = (cut.ties > 0 && cut.weight >= least) ? cut.weight : 0;
     const u64 ties = tie_weight ? cut.ties : 0;
     uint32_t* tied = reinterpret_cast<uint32_t*>(s.g);
-    u64 w[kE], count = 0;
+    const uint32_t least32 = static_cast<uint32_t>(max(1ull, min(least, 0xffffffffull)));
+    uint32_t w[kE];
+    u64 count = 0;
 #pragma unroll
     for (int e = 0; e < kE; ++e) {
-      w[e] = x[e] > cut.x ? weight(x[e]) : 0;
-      if (w[e] < least) w[e] = 0;
-      count += w[e] > 0;
+      const uint32_t t = weight32(distance(x[e]));
+      w[e] = x[e] > cut.x && t >= least32 ? t : 0u;
+      count += w[e] > 0u;
     }
     count = block_sum(count);
     auto reach = [&](u64 above, u64 tied) { return above + min(ties, tied) * tie_weight; };
@@ -547,7 +549,7 @@ struct Sampler {
       for (int e = 0; e < kE; ++e) {
         const int bin = (id[e] - base) >> shift;
         if (id[e] < base || bin >= kSampBins) continue;
-        if (w[e]) add_weight(bin, w[e]);
+        add_weight(bin, w[e]);
         if (ties && x[e] == cut.x) atomicAdd(&tied[bin], 1u);
       }
       __syncthreads();
@@ -609,14 +611,20 @@ struct Sampler {
     };
     // a warp takes consecutive vectors, so that the search below has one warp's to look through
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = (nvec + kWarps - 1) / kWarps;
+    const float full = top + 1e-3f * (floor - top);  // tokens below (0.02 T from the top) weigh less than 2^32
     u64 sum = 0, num = 0;  // num: count above, and ties in the low half
     uint32_t above = 0u, tied = 0u;
     for (int v = warp * share + lane; v < min(nvec, (warp + 1) * share); v += 32) {
       float x[kVec];
       uint32_t k[kVec];
-      if (!kept_of(row[v], x, k)) continue;
+      const uint4 u = row[v];
+      if (!kept_of(u, x, k)) continue;
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) sum += widen(k[e]), above += k[e] > 0u;
+      for (int e = 0; e < kVec; ++e) sum += k[e], above += k[e] > 0u;
+      if (largest(u) >= full) {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) sum += k[e] == 0xffffffffu;
+      }
       if (ties)
 #pragma unroll
         for (int e = 0; e < kVec; ++e) tied += x[e] == cut.x;
