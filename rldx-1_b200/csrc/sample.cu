@@ -335,18 +335,13 @@ struct Sampler {
   template <bool kAlone, typename Each>
   __device__ __forceinline__ bool find(Each each, bool by_count, u64 level, float share, const Cut& from, Cut* out, u64* whole) {
     clear();
-    if (by_count) {
-      each(floor, [&](float x) {
-        if (!(x > from.x)) return;
-        const float d = distance(x);
-        if (weighs(d)) atomicAdd(&s.lo[bin_of(d)], 1u);
-      });
-    } else {
-      each(fmaxf(floor, from.x), [&](float x) {
-        const float d = distance(x);
+    each(fmaxf(floor, from.x), [&](float x) {
+      const float d = distance(x);
+      if (!by_count)
         add_weight(bin_of(d), x > from.x ? weight32(d) : 0u);
-      });
-    }
+      else if (x > from.x && weighs(d))
+        atomicAdd(&s.lo[bin_of(d)], 1u);
+    });
     const bool has_ties = from.ties > 0;  // the ties of the cut so far count as that many tokens
     const int tie_bin = has_ties ? bin_of(distance(from.x)) : -1;
     const u64 tie_sum = by_count ? from.ties : from.ties * from.weight;
@@ -402,13 +397,12 @@ struct Sampler {
     Cut cut{}, c;  // below every logit
     cut.x = -INFINITY;
     u64 whole;
-    if (top_k > 0 && find<kAlone>(each, true, static_cast<u64>(top_k) - 1, -1.0f, cut, &c, &whole)) {
-      c.ties = min(c.ties, static_cast<uint32_t>(static_cast<u64>(top_k) - c.before));
-      cut = c;
-    }
     const float share = fmaxf(top_p, 0.0f);
-    if (top_p < 1.0f && find<kAlone>(each, false, 0, share, cut, &c, &whole)) {
-      const u64 fit = (last_below(share, whole) - c.before) / c.weight + 1;
+#pragma unroll 1
+    for (int by_weight = top_k > 0 ? 0 : 1; by_weight < (top_p < 1.0f ? 2 : 1); ++by_weight) {  // (one copy of the code)
+      const u64 last = static_cast<u64>(top_k) - 1;
+      if (!find<kAlone>(each, !by_weight, last, by_weight ? share : -1.0f, cut, &c, &whole)) continue;
+      const u64 fit = by_weight ? (last_below(share, whole) - c.before) / c.weight + 1 : static_cast<u64>(top_k) - c.before;
       c.ties = static_cast<uint32_t>(min(static_cast<u64>(c.ties), fit));
       cut = c;
     }
@@ -521,22 +515,21 @@ struct Sampler {
     }
   }
 
-  // The draw by rank 0 among its candidates (kE in each thread's registers: logits and ids) above the cut and its
+  // The draw by rank 0 among its n candidates (logits, then replaced by what they weigh, and ids) above the cut and its
   // ties: bins of ids, 1024 over the vocabulary and then the ids of one, hold weights and numbers of tied tokens.
-  template <int kE>
-  __device__ __forceinline__ void draw_from_list(const SampleParams& P, int r, const float (&x)[kE], const int (&id)[kE], const Cut& cut,
-                                                 u64 least) {
+  __device__ __forceinline__ void draw_from_list(const SampleParams& P, int r, uint2* list, int n, const Cut& cut, u64 least) {
+    constexpr uint32_t kTied = 0xfffffffeu;  // (weights are at most 2^32 - 256, or 2^32 - 1 for 2^32)
     const u64 tie_weight = (cut.ties > 0 && cut.weight >= least) ? cut.weight : 0;
     const u64 ties = tie_weight ? cut.ties : 0;
     uint32_t* tied = reinterpret_cast<uint32_t*>(s.g);
     const uint32_t least32 = static_cast<uint32_t>(max(1ull, min(least, 0xffffffffull)));
-    uint32_t w[kE];
     u64 count = 0;
-#pragma unroll
-    for (int e = 0; e < kE; ++e) {
-      const uint32_t t = weight32(distance(x[e]));
-      w[e] = x[e] > cut.x && t >= least32 ? t : 0u;
-      count += w[e] > 0u;
+#pragma unroll 1
+    for (int i = threadIdx.x; i < n; i += NT) {
+      const float x = __uint_as_float(list[i].x);
+      const uint32_t t = weight32(distance(x)), w = x > cut.x && t >= least32 ? t : 0u;
+      list[i].x = ties > 0 && x == cut.x ? kTied : w;
+      count += w > 0u;
     }
     count = block_sum(count);
     auto reach = [&](u64 above, u64 tied) { return above + min(ties, tied) * tie_weight; };
@@ -545,12 +538,15 @@ struct Sampler {
     for (bool first = true;; first = false) {
       for (int i = threadIdx.x; i < kSampBins; i += NT) s.lo[i] = s.hi[i] = tied[i] = 0u;
       __syncthreads();
-#pragma unroll
-      for (int e = 0; e < kE; ++e) {
-        const int bin = (id[e] - base) >> shift;
-        if (id[e] < base || bin >= kSampBins) continue;
-        add_weight(bin, w[e]);
-        if (ties && x[e] == cut.x) atomicAdd(&tied[bin], 1u);
+#pragma unroll 1
+      for (int i = threadIdx.x; i < n; i += NT) {
+        const uint2 c = list[i];
+        const int id = static_cast<int>(c.y), bin = (id - base) >> shift;
+        if (id < base || bin >= kSampBins) continue;
+        if (c.x == kTied)
+          atomicAdd(&tied[bin], 1u);
+        else
+          add_weight(bin, c.x);
       }
       __syncthreads();
       constexpr int kPer = kSampBins / NT;
@@ -821,26 +817,22 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 1 : 4) sample_kernel(const __g
     return;
   } else {
     if (rank > 0) return;
-    constexpr int kE = kSampList / NT;
-    float x[kE];
-    int id[kE];
-#pragma unroll
-    for (int e = 0; e < kE; ++e) {
-      const int i = threadIdx.x + e * NT;
-      const u64 c = i < n ? s.list[i] : 0;
-      x[e] = i < n ? order_value(static_cast<uint32_t>(c >> 32)) : -INFINITY;
-      id[e] = i < n ? static_cast<int>(~static_cast<uint32_t>(c)) : -1;
+    // the candidates move to where the logits were
+    uint2* list = reinterpret_cast<uint2*>(vecs);
+    for (int i = threadIdx.x; i < n; i += NT) {
+      const u64 c = s.list[i];
+      list[i] = make_uint2(__float_as_uint(order_value(static_cast<uint32_t>(c >> 32))), ~static_cast<uint32_t>(c));
     }
     __syncthreads();
     for (int i = threadIdx.x; i < kSampBins; i += NT) s.g[i] = 0;
     cut = S.template find_cut<true>(
         [&](float, auto f) {
-#pragma unroll
-          for (int e = 0; e < kE; ++e) f(x[e]);
+#pragma unroll 1
+          for (int i = threadIdx.x; i < n; i += NT) f(__uint_as_float(list[i].x));
         },
         top_k, top_p);
     __syncthreads();  // every warp has read the last answer in `found`
-    S.template draw_from_list<kE>(P, r, x, id, cut, least);
+    S.draw_from_list(P, r, list, n, cut, least);
     return;
   }
   S.draw_from_row(P, r, cut, least);
@@ -850,7 +842,7 @@ template <typename T>
 size_t sample_smem(int vocab, int cluster) {
   const int kVec = 16 / sizeof(T);
   const int per = ((vocab + kVec - 1 + kVec - 1) / kVec + cluster - 1) / cluster;
-  return (sizeof(SampleShared) + 15) / 16 * 16 + static_cast<size_t>(per) * 16;
+  return (sizeof(SampleShared) + 15) / 16 * 16 + std::max<size_t>(static_cast<size_t>(per) * 16, kSampList * 8);  // or the list
 }
 
 template <typename T, int NT>
