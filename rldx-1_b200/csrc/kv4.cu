@@ -34,6 +34,15 @@ __device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
   unpack_bf16x2(u.z, v[4], v[5]);
   unpack_bf16x2(u.w, v[6], v[7]);
 }
+__device__ __forceinline__ void load4(const __nv_bfloat16* p, float2 (&v)[2]) {
+  const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
+  unpack_bf16x2(u.x, v[0].x, v[0].y);
+  unpack_bf16x2(u.y, v[1].x, v[1].y);
+}
+__device__ __forceinline__ void load4(const float* p, float2 (&v)[2]) {
+  const float4 u = __ldg(reinterpret_cast<const float4*>(p));
+  v[0] = make_float2(u.x, u.y), v[1] = make_float2(u.z, u.w);
+}
 __device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
   const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
   v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
@@ -85,33 +94,22 @@ __device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8]) {
   unpack_bf16x2(u.w, v[6], v[7]);
 }
 
-// kN heads of one token, D / 8 lanes with 8 channels of each: v = rope(rms(v) w).  c, s: this lane's part
-// of the rotation's row, s with the sign of rotate_half = cat(-x2, x1).  The heads' steps are
-// independent of one another, so their shuffles overlap.
-template <int D, int kN>
-__device__ __forceinline__ void norm_rope(float (&v)[kN][8], const float (&w)[8], const float (&c)[8], const float (&s)[8],
-                                          float eps) {
+// A head of one token, D / 8 lanes with 8 channels each: v = rope(rms(v) w).  c, s: this lane's part of the
+// rotation's row, s with the sign of rotate_half = cat(-x2, x1).
+template <int D>
+__device__ __forceinline__ void norm_rope(float (&v)[8], const float (&w)[8], const float (&c)[8], const float (&s)[8], float eps) {
   constexpr int kLanes = D / 8;
-  float ss[kN];
+  float ss = 0.0f;
 #pragma unroll
-  for (int r = 0; r < kN; ++r) {
-    ss[r] = 0.0f;
+  for (int e = 0; e < 8; ++e) ss = fmaf(v[e], v[e], ss);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) ss[r] = fmaf(v[r][e], v[r][e], ss[r]);
-  }
+  for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  const float rstd = rsqrtf(ss * (1.0f / D) + eps);
 #pragma unroll
-  for (int o = kLanes / 2; o > 0; o >>= 1)
-#pragma unroll
-    for (int r = 0; r < kN; ++r) ss[r] += __shfl_xor_sync(0xffffffffu, ss[r], o);
-#pragma unroll
-  for (int r = 0; r < kN; ++r) {
-    const float rstd = rsqrtf(ss[r] * (1.0f / D) + eps);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float y = __fmul_rn(__fmul_rn(v[r][e], rstd), w[e]);
-      const float o = __shfl_xor_sync(0xffffffffu, y, kLanes / 2);  // the channel half a head away
-      v[r][e] = __fadd_rn(__fmul_rn(y, c[e]), __fmul_rn(o, s[e]));
-    }
+  for (int e = 0; e < 8; ++e) {
+    const float y = __fmul_rn(__fmul_rn(v[e], rstd), w[e]);
+    const float o = __shfl_xor_sync(0xffffffffu, y, kLanes / 2);  // the channel half a head away
+    v[e] = __fadd_rn(__fmul_rn(y, c[e]), __fmul_rn(o, s[e]));
   }
 }
 
@@ -162,57 +160,92 @@ __global__ void __launch_bounds__(128) kv4_append_kernel(const __grid_constant__
   const int at = static_cast<int>(item % per_token);
   const __nv_bfloat16* src = P.qkv + tok * P.ld + 8 * l;
   int rp = __ldg(P.rope_pos + tok);
-  float w[8], c[8], s[8];
-  load8((of_q ? P.wq : P.wk) + 8 * l, w);
-  auto rotation = [&] {
+  if (of_q) {
+    // a lane's channels: four, and the four half a head away that the rotation pairs them with
+    const int h0 = at * kAppendHeads;
+    uint2 x[kAppendHeads][2];
+#pragma unroll
+    for (int r = 0; r < kAppendHeads; ++r)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        x[r][i] = __ldcs(reinterpret_cast<const uint2*>(P.qkv + tok * P.ld + min(h0 + r, hq - 1) * D + i * (D / 2) + 4 * l));
     if (static_cast<unsigned>(rp) >= static_cast<unsigned>(P.rope_rows)) {
       if (live) record_error(kErrKv4Rope);
       rp = 0;
     }
-    load8(static_cast<const Rope*>(P.cos) + static_cast<long long>(rp) * D + 8 * l, c);
-    load8(static_cast<const Rope*>(P.sin) + static_cast<long long>(rp) * D + 8 * l, s);
-    if (l < kLanes / 2)
+    float2 w[2][2], c[2][2], s[2][2];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] = -s[e];
-  };
-  if (of_q) {
-    uint4 x[kAppendHeads];
-    float v[kAppendHeads][8];
-    const int h0 = at * kAppendHeads;
-#pragma unroll
-    for (int r = 0; r < kAppendHeads; ++r) x[r] = __ldcs(reinterpret_cast<const uint4*>(src + min(h0 + r, hq - 1) * D));
-    rotation();
+    for (int i = 0; i < 2; ++i) {
+      const int ch = i * (D / 2) + 4 * l;
+      load4(P.wq + ch, w[i]);
+      load4(static_cast<const Rope*>(P.cos) + static_cast<long long>(rp) * D + ch, c[i]);
+      load4(static_cast<const Rope*>(P.sin) + static_cast<long long>(rp) * D + ch, s[i]);
+    }
     griddep_launch();
+    float2 v[kAppendHeads][2][2];
+    float ss[kAppendHeads];
 #pragma unroll
-    for (int r = 0; r < kAppendHeads; ++r) unpack8(x[r], v[r]);
-    norm_rope<D, kAppendHeads>(v, w, c, s, P.eps);
+    for (int r = 0; r < kAppendHeads; ++r) {
+      float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int r = 0; r < kAppendHeads; ++r)
-      if (live && h0 + r < hq) {
-        uint4 u;
-        u.x = pack_bf16x2(v[r][0], v[r][1]);
-        u.y = pack_bf16x2(v[r][2], v[r][3]);
-        u.z = pack_bf16x2(v[r][4], v[r][5]);
-        u.w = pack_bf16x2(v[r][6], v[r][7]);
-        *reinterpret_cast<uint4*>(P.q + (static_cast<long long>(tok) * hq + h0 + r) * D + 8 * l) = u;
+      for (int i = 0; i < 2; ++i) {
+        unpack_bf16x2(x[r][i].x, v[r][i][0].x, v[r][i][0].y);
+        unpack_bf16x2(x[r][i].y, v[r][i][1].x, v[r][i][1].y);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) sum = fma_f32x2(v[r][i][e], v[r][i][e], sum);
       }
+      ss[r] = sum.x + sum.y;
+    }
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1)
+#pragma unroll
+      for (int r = 0; r < kAppendHeads; ++r) ss[r] += __shfl_xor_sync(0xffffffffu, ss[r], o);
+#pragma unroll
+    for (int r = 0; r < kAppendHeads; ++r) {
+      const float rstd = rsqrtf(ss[r] * (1.0f / D) + P.eps);
+      const float2 rr = make_float2(rstd, rstd);
+      uint2 u[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float2 y0 = mul_f32x2(mul_f32x2(v[r][0][e], rr), w[0][e]), y1 = mul_f32x2(mul_f32x2(v[r][1][e], rr), w[1][e]);
+        const float2 n = mul_f32x2(y1, s[0][e]);
+        const float2 a = add_f32x2(mul_f32x2(y0, c[0][e]), make_float2(-n.x, -n.y));
+        const float2 b = add_f32x2(mul_f32x2(y1, c[1][e]), mul_f32x2(y0, s[1][e]));
+        (e ? u[0].y : u[0].x) = pack_bf16x2(a.x, a.y);
+        (e ? u[1].y : u[1].x) = pack_bf16x2(b.x, b.y);
+      }
+      if (live && h0 + r < hq)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          *reinterpret_cast<uint2*>(P.q + (static_cast<long long>(tok) * hq + h0 + r) * D + i * (D / 2) + 4 * l) = u[i];
+    }
     return;
+  }
+  float w[8], c[8], s[8];
+  load8(P.wk + 8 * l, w);
+  if (static_cast<unsigned>(rp) >= static_cast<unsigned>(P.rope_rows)) {
+    if (live) record_error(kErrKv4Rope);
+    rp = 0;
   }
   const uint4 xk = __ldcs(reinterpret_cast<const uint4*>(src + (hq + at) * D));
   const uint4 xv = __ldcs(reinterpret_cast<const uint4*>(src + (hq + hkv + at) * D));
   const int *cu = P.c.cu, *lengths = P.c.lengths;
   stage_seqs(P.c, s_seq, &cu, &lengths);
-  rotation();
+  load8(static_cast<const Rope*>(P.cos) + static_cast<long long>(rp) * D + 8 * l, c);
+  load8(static_cast<const Rope*>(P.sin) + static_cast<long long>(rp) * D + 8 * l, s);
+  if (l < kLanes / 2)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[e] = -s[e];
   __syncthreads();
   griddep_launch();
   int tau = 0;
   const int place = live ? kv4_token_place(P.c, cu, lengths, tok, &tau) : -1;
-  float k[1][8], v[8];
-  unpack8(xk, k[0]);
+  float k[8], v[8];
+  unpack8(xk, k);
   unpack8(xv, v);
-  norm_rope<D, 1>(k, w, c, s, P.eps);
+  norm_rope<D>(k, w, c, s, P.eps);
   __half k_scale, k_low, v_scale, v_low;
-  const uint32_t kc = quantise8(k[0], &k_scale, &k_low), vc = quantise8(v, &v_scale, &v_low);
+  const uint32_t kc = quantise8(k, &k_scale, &k_low), vc = quantise8(v, &v_scale, &v_low);
   if (place < 0) return;
   uint8_t* unit = P.c.data + static_cast<long long>(place + at * P.c.units_per_page) * U::kBytes;
   const int j = l / 4, t4 = l % 4;  // group, position in the group
