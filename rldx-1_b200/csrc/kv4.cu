@@ -141,8 +141,9 @@ __device__ __forceinline__ uint32_t quantise8(const float (&v)[8], __half* scale
 // D / 8 lanes own an item: four query heads of a token, or (blocks from q_blocks on) k and v of one kv
 // head.  The rotation's row is read once for an item, all loads are issued before any arithmetic, and
 // every block runs straight-line code of one kind.  8 prompts of up to 1104 tokens, 16 / 2 heads, d = 128,
-// appended and read back: 26 us, 39 with one head an item, 39 with q, k and v heads mixed in a block; two
-// heads an item and more CTAs an SM 27, so instructions and not occupancy bound it (SM 46 % busy, DRAM 20 %).
+// appended and read back: 24.6 us (kv4_read_kernel about 7 of them).  Before the query heads' arithmetic was
+// paired it was 26, and then 39 with one head an item, 39 with q, k and v heads mixed in a block, 27 with two heads an
+// item and more CTAs an SM: instructions and the chain of loads bound it, not occupancy.
 constexpr int kAppendHeads = 4;
 
 template <int D, typename Rope>

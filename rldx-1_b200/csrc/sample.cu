@@ -21,9 +21,9 @@
 //     (top-p: the low 16 and high 17 bits of a weight in two 32-bit sums); CTAs add theirs to rank 0's
 //     through distributed shared memory, which finds the crossing and tells the others.
 //
-// Measured, bf16 rows of 151680, 1 row / 256 rows in us: greedy 3.1 / 21 (78 MB: 12 at the copy's rate), top-k 20
-// 7.9 / 44, top-k 1000 14.8 / 84, top-k 3000 (by histogram) 22 / 158, temperature alone 11.6 / 86, top-p 0.9 at
-// T = 1, 28914 kept, 27.6 / 197.  Few rows wait on the chain of passes and cluster barriers; many are bound by
+// Measured, bf16 rows of 151680, 1 row / 256 rows in us: greedy 3.0 / 21 (78 MB: 12 at the copy's rate), top-k 20
+// 7.9 / 43, top-k 1000 15.5 / 77, top-k 3000 (by histogram) 23 / 160, temperature alone 11.4 / 82, top-p 0.9 at
+// T = 1, 28914 kept, 26.3 / 193.  Few rows wait on the chain of passes and cluster barriers; many are bound by
 // instructions, the correctly rounded quotient and exponential of every token that can weigh anything
 // (about 40 a token and pass), and by the histogram's atomics.
 #include <cfloat>
@@ -910,9 +910,9 @@ extern "C" int rldx_sample(const void* logits, int64_t ld, int rows, int vocab, 
   p.logprob = logprob;
   p.kept = kept;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // Few CTAs: 512 threads each shorten a row's passes (1 x 151680 bf16, top-k 1000 14.8 us against 19.0, temperature
-  // alone 11.6 against 13.8).  More than two an SM: 256 threads, four CTAs to an SM (256 x 151680, mixed filters, 90 us
-  // against 120 with 512 threads, two to an SM).
+  // Few CTAs: 512 threads each shorten a row's passes (1 x 151680 bf16, top-k 1000 14.8 us against 19.0 with 256,
+  // temperature alone 11.6 against 13.8).  More than two an SM: 256 threads, four CTAs to an SM (256 x 151680, mixed
+  // filters, 90 us against 120 with 512 threads, two to an SM, when both were measured; now 86).
   const bool wide = static_cast<long long>(rows) * p.cluster <= 2 * sm_count();
   cudaError_t e;
   if (logits_fp32)
