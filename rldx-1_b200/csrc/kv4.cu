@@ -141,7 +141,7 @@ __device__ __forceinline__ uint32_t quantise8(const float (&v)[8], __half* scale
 // D / 8 lanes own an item: four query heads of a token, or (blocks from q_blocks on) k and v of one kv
 // head.  The rotation's row is read once for an item, all loads are issued before any arithmetic, and
 // every block runs straight-line code of one kind.  8 prompts of up to 1104 tokens, 16 / 2 heads, d = 128,
-// appended and read back: 24.6 us (kv4_read_kernel about 7 of them).  Before the query heads' arithmetic was
+// appended and read back: 23.7 us.  Before the query heads' arithmetic was
 // paired it was 26, and then 39 with one head an item, 39 with q, k and v heads mixed in a block, 27 with two heads an
 // item and more CTAs an SM: instructions and the chain of loads bound it, not occupancy.
 constexpr int kAppendHeads = 4;
@@ -265,7 +265,17 @@ __global__ void __launch_bounds__(128) kv4_append_kernel(const __grid_constant__
   }
 }
 
-// D / 8 lanes own one (token, kv head, K or V) row.
+// 8 channels: scale * code + low, rounded to bf16.
+__device__ __forceinline__ uint4 rebuild8(uint32_t codes, __half scale_h, __half low_h) {
+  const float scale = __half2float(scale_h), low = __half2float(low_h);
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = fmaf(scale, static_cast<float>(codes >> (4 * i) & 15u), low);
+  return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+}
+
+// D / 8 lanes own k and v of one kv head of a token: one search for the token's place serves both, and all
+// loads are issued together.
 template <int D>
 __global__ void __launch_bounds__(128) kv4_read_kernel(const __grid_constant__ Kv4ReadParams P) {
   using U = Kv4Unit<D>;
@@ -278,42 +288,30 @@ __global__ void __launch_bounds__(128) kv4_read_kernel(const __grid_constant__ K
   stage_seqs(P.c, s_seq, &cu, &lengths);
   __syncthreads();
   const long long row = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) / kLanes;
-  if (row >= static_cast<long long>(P.c.tokens) * hkv * 2) return;
+  if (row >= static_cast<long long>(P.c.tokens) * hkv) return;
   const int l = threadIdx.x % kLanes, j = l / 4, t4 = l % 4;
-  const int tok = static_cast<int>(row / (2 * hkv)), which = static_cast<int>(row - static_cast<long long>(tok) * 2 * hkv);
-  const bool is_v = which >= hkv;
-  const int h = is_v ? which - hkv : which;
+  const int tok = static_cast<int>(row / hkv), h = static_cast<int>(row - static_cast<long long>(tok) * hkv);
   int tau;
   const int place = kv4_token_place(P.c, cu, lengths, tok, &tau);
-  uint4 o = make_uint4(0u, 0u, 0u, 0u);
+  uint4 k = make_uint4(0u, 0u, 0u, 0u), v = k;
   if (place >= 0) {
     const uint8_t* unit = P.c.data + static_cast<long long>(place + h * P.c.units_per_page) * U::kBytes;
-    uint32_t codes;
-    float scale, low;
-    if (!is_v) {
-      codes = *reinterpret_cast<const uint32_t*>(unit + tau * U::kRow + 4 * (t4 * U::kG + j));
-      const __half* meta = reinterpret_cast<const __half*>(unit + U::kKMeta + 4 * U::kG * tau);
-      scale = __half2float(meta[j]);
-      low = __half2float(meta[U::kG + j]);
-    } else {
-      const int blk = tau / 16, hh = tau / 8 % 2, t = tau / 2 % 4, e = tau % 2;
-      const uint8_t* at = unit + U::kV + 8 * D * blk + 4 * D * hh + 4 * U::kG * t + 2 * U::kG * e + 2 * j;
-      codes = *reinterpret_cast<const uint16_t*>(at + 16 * U::kG * (2 * t4));
-      codes |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(at + 16 * U::kG * (2 * t4 + 1))) << 16;
-      const int m = 32 * U::kG * blk + 16 * U::kG * hh + 4 * U::kG * t + 4 * j + 2 * e;
-      scale = __half2float(*reinterpret_cast<const __half*>(unit + U::kVScale + m));
-      low = __half2float(*reinterpret_cast<const __half*>(unit + U::kVLow + m));
-    }
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = fmaf(scale, static_cast<float>(codes >> (4 * i) & 15u), low);
-    o.x = pack_bf16x2(v[0], v[1]);
-    o.y = pack_bf16x2(v[2], v[3]);
-    o.z = pack_bf16x2(v[4], v[5]);
-    o.w = pack_bf16x2(v[6], v[7]);
+    const int blk = tau / 16, hh = tau / 8 % 2, t = tau / 2 % 4, e = tau % 2;
+    const uint8_t* at = unit + U::kV + 8 * D * blk + 4 * D * hh + 4 * U::kG * t + 2 * U::kG * e + 2 * j;
+    const int m = 32 * U::kG * blk + 16 * U::kG * hh + 4 * U::kG * t + 4 * j + 2 * e;
+    const __half* meta = reinterpret_cast<const __half*>(unit + U::kKMeta + 4 * U::kG * tau);
+    const uint32_t kc = *reinterpret_cast<const uint32_t*>(unit + tau * U::kRow + 4 * (t4 * U::kG + j));
+    const __half k_scale = meta[j], k_low = meta[U::kG + j];
+    const uint32_t v0 = *reinterpret_cast<const uint16_t*>(at + 16 * U::kG * (2 * t4));
+    const uint32_t v1 = *reinterpret_cast<const uint16_t*>(at + 16 * U::kG * (2 * t4 + 1));
+    const __half v_scale = *reinterpret_cast<const __half*>(unit + U::kVScale + m);
+    const __half v_low = *reinterpret_cast<const __half*>(unit + U::kVLow + m);
+    k = rebuild8(kc, k_scale, k_low);
+    v = rebuild8(v0 | v1 << 16, v_scale, v_low);
   }
-  __nv_bfloat16* dst = (is_v ? P.v : P.k) + (static_cast<long long>(tok) * hkv + h) * D + 8 * l;
-  *reinterpret_cast<uint4*>(dst) = o;
+  const long long to = (static_cast<long long>(tok) * hkv + h) * D + 8 * l;
+  *reinterpret_cast<uint4*>(P.k + to) = k;
+  *reinterpret_cast<uint4*>(P.v + to) = v;
 }
 
 namespace {
@@ -347,7 +345,7 @@ cudaError_t launch_kv4_append(const Kv4AppendParams& p, int head_dim, cudaStream
 }
 
 cudaError_t launch_kv4_read(const Kv4ReadParams& p, int head_dim, cudaStream_t stream) {
-  const unsigned blocks = blocks_of(static_cast<long long>(p.c.tokens) * p.c.kv_heads * 2, head_dim / 8);
+  const unsigned blocks = blocks_of(static_cast<long long>(p.c.tokens) * p.c.kv_heads, head_dim / 8);
   return head_dim == 128 ? launch_blocks<Kv4ReadParams>(kv4_read_kernel<128>, blocks, stream, p)
                          : launch_blocks<Kv4ReadParams>(kv4_read_kernel<64>, blocks, stream, p);
 }
