@@ -20,13 +20,14 @@
 // A value of V that is not finite, of a token that some rows must not see, cannot go through a
 // product with p = 0: it is rebuilt as 0, its place marked, and the rows that do see the token
 // give NaN in the channels of its group (in every channel where K is not finite).
+//
 // Few tiles of rows would leave most SMs idle, so up to two waves' worth of CTAs share a tile's keys evenly
 // and a second kernel joins their parts (the rule and both sides' times: decode_plan).  With more than
 // a wave of tiles each CTA has its own, longest first.
 //
 // Measured: 8 sequences of up to 2300 tokens, up to 1104 of them new, 16 / 2 heads, d = 128: 139 us, 31 % of
 // cuBLAS's bf16 rate (44 us).  No role bounds it alone: without three quarters of K's rebuilding, of V's, or
-// of the exponentials it takes 137, 132 and 130 us.  K's tiles of 64 keys give an MMA of N = 64, P takes S's
+// without nearly all exponentials it takes 138, 133 and 131 us.  K's tiles of 64 keys give an MMA of N = 64, P takes S's
 // place, and the chain S, softmax, P V of the two query tiles covers each other's waits only in part.
 #include "host_util.h"
 #include "kv4.cuh"
