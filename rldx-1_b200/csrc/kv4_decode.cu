@@ -720,8 +720,9 @@ cudaError_t launch_decode(const Kv4AttnParams& whole, int ctas, cudaStream_t str
     p.c.lengths += b0;
     p.c.table += static_cast<long long>(b0) * p.c.table_ld;
     p.tiles = (p.max_new * p.group + 8 * NT - 1) / (8 * NT);
-    // a few segments are cut into many parts each: then a CTA of the join per segment and column
-    p.by_segment = 16LL * p.tiles * p.c.kv_heads * p.c.seqs < ctas;
+    // a few segments are cut into many parts each: then a CTA of the join per segment and column.  A launch that
+    // cuts nothing has no join and no workspace for its segments' heads, however few sequences the last one holds.
+    p.by_segment = !p.whole && 16LL * p.tiles * p.c.kv_heads * p.c.seqs < ctas;
     cudaError_t e = launch_pdl(kv4_decode_kernel<D, NT, W>, dim3(ctas, 1, 1), 32 * W, DecShape<D, NT, W>::kSmem, stream, p);
     if (e != cudaSuccess) return e;
     if (p.whole) continue;
