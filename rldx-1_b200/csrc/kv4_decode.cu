@@ -12,10 +12,14 @@
 // m16n8k16: rows = 16 tokens (K) or 16 channels (V), columns = 8 of the query rows (new token,
 // head of the group) that share a kv head.  q is scaled by a power of two per row to [2^8, 2^9)
 // at its largest, so bf16's range fits fp16 and 32 q sum below 2^14; sums of q go in as a
-// high and a low half.  The products accumulate in fp32, running maximum and sum are fp32; p is
-// rounded to fp16 (2^-11 relative, against bf16's 2^-9 at the output).  A row's reference maximum
-// moves when a score passes it by more than 2 (log2 units), so p <= 4 and p scale <= 4 x 8735
-// stays finite for every scale that the append kernel writes.
+// high and a low half.  The products accumulate in fp32, running maximum and sum are fp32.  p and p scale
+// are rounded to fp16 for the MMA (2^-11 relative each, against bf16's 2^-8 at the output; the row's sum takes
+// the rounded p, so that the weights still add up to one).  That bound holds over fp16's normal numbers, so both
+// are kept at their top: a row's p is held 2^11 times or more, its largest up to 2^15 (kDecSet, kDecMove), and V's scales
+// go in times a power of two that each warp keeps for its units, the largest near 1/2.  What falls below is off by
+// 2^-25 beside 2^11: a token counts with its bits down to 2^-25 of the largest weight, whatever the size of
+// V.  8192 tokens, V of size 1 / 1e-3 / 1e-4 / 1e-5, error against 64 bits (the output's rounding alone 0.0017): 0.0017
+// each; with p <= 4 and the scales as they are 0.0017 / 0.004 / 0.12 / 3.4, for 3 to 5 % less time.
 //
 // Work is split evenly over one wave of CTAs, whatever the lengths: a segment is one (sequence, kv
 // head, tile of columns) with the units that it can see, all segments stand in one line and each
@@ -25,8 +29,8 @@
 // shared memory at a segment's end.  A segment cut between CTAs is joined by a second kernel, in
 // the CTAs' order, so the result does not depend on timing.
 //
-// Measured: 64 sequences of up to 8192 tokens, 16 / 2 heads, d = 128, 120 MB of cache: 30.2 us with the join
-// (27 without), 3.95 TB/s, 0.60 of the copy's rate; 3 x 131077 26 us, 0.56.  Four warps a CTA and four CTAs an
+// Measured: 64 sequences of up to 8192 tokens, 16 / 2 heads, d = 128, 120 MB of cache: 31.7 us with the join,
+// 3.77 TB/s, 0.58 of the copy's rate; 3 x 131077 27.4 us, 0.54.  Four warps a CTA and four CTAs an
 // SM, 32 KB of copies in flight a CTA: 33.0 us against 35.7 with eight warps and two CTAs.  What is left is the
 // start (lengths, prefix sums, q: about 3 us before the first unit is used), the shared-memory merge at a
 // segment's end and the join's launch (3.5 us).
@@ -41,7 +45,9 @@ namespace {
 constexpr int kDecWarps = 4, kDecWarpsWide = 8;  // of a CTA; of one that has a short segment to itself
 constexpr int dec_resident(int warps, int cols) { return 128 / (warps * cols); }  // CTAs per SM (128 registers a thread)
 constexpr int kDecStages = 2;
-constexpr float kDecGrow = 2.0f;  // lazy move of the reference maximum (log2 units)
+// A row's reference (log2 units) stands 11 below the largest score when it is set and is set again once one passes it
+// by more than 15, so that p = 2^(score - reference) is at most 2^15, and 2^11 or more for the largest.
+constexpr float kDecSet = 11.0f, kDecMove = 15.0f;
 
 constexpr int kDecMaxSeqs = 1024;  // sequences of one launch (their prefix sums stand in shared memory)
 
@@ -348,10 +354,26 @@ __global__ void __launch_bounds__(32 * W, dec_resident(W, 8 * NT))
       m_ref[nt][0] = m_ref[nt][1] = -INFINITY;
     }
 
+    // V's scales go in times 2^vexp, which keeps them at 1 or below; a larger one moves it (and O) down, to leave
+    // that one between 1/4 and 1/2.
+    int vexp = 15;
+    __half2 vmul = bits_h2(0x78007800u), vmax = bits_h2(0x02000200u);  // 2^vexp, 2^-vexp
+
     // One unit; kPlain: every column sees every token of it.  The two forms are separate code, so that
     // the plain one carries no masking.
     auto attend = [&](const uint8_t* un, int i, auto flag) {
       constexpr bool kPlain = decltype(flag)::value;
+      // V's scales of the unit: a lane looks at G / 2 words of tokens 2 (lane / 2), + 1
+      __half2 top;
+      {
+        const uint8_t* at = un + U::kVScale + lane * 2 * G;
+        if constexpr (G == 4) {
+          const uint2 x = *reinterpret_cast<const uint2*>(at);
+          top = __hmax2(bits_h2(x.x), bits_h2(x.y));
+        } else {
+          top = bits_h2(*reinterpret_cast<const uint32_t*>(at));
+        }
+      }
       // ---- products of 32 tokens (two tiles of 16), before the column's factor ----
       float sc[2][NT][4];
 #pragma unroll
@@ -403,6 +425,13 @@ __global__ void __launch_bounds__(32 * W, dec_resident(W, 8 * NT))
       if constexpr (!kPlain) {
         const int key0 = kKv4Unit * span.unit(u0 + warp + W * i);
         const bool have = __shfl_sync(0xffffffffu, index, i & 31) >= 0;
+        uint32_t some = 0u;  // the scale of a token that no column sees may be anything
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int key = key0 + (lane & ~1) + e;
+          if (have && key <= span.pos_hi && (P.window <= 0 || span.pos_lo - key < P.window || key < P.sinks)) some |= 0xffffu << (16 * e);
+        }
+        top = bits_h2(h2_bits(top) & some);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -419,20 +448,38 @@ __global__ void __launch_bounds__(32 * W, dec_resident(W, 8 * NT))
               }
           }
       }
-      // ---- running maximum ----
+      // ---- running maximum, and the power of two of V's scales ----
+      const bool large = __hgt2_mask(top, vmax) != 0u;
+      if (__any_sync(0xffffffffu, large)) {
+        const uint32_t t2 = h2_bits(__hmax2(top, bits_h2(0u)));  // halves of at least 0, in the order of their bits
+        const uint32_t most = __reduce_max_sync(0xffffffffu, max(t2 & 0xffffu, t2 >> 16));
+        const int to = min(vexp, max(-14, 13 - static_cast<int>(most >> 10)));
+        const float back = __uint_as_float(static_cast<uint32_t>(127 + to - vexp) << 23);
+        vexp = to;
+        vmul = bits_h2(static_cast<uint32_t>(15 + to) * 0x04000400u);
+        vmax = bits_h2(static_cast<uint32_t>(15 - to) * 0x04000400u);
+#pragma unroll
+        for (int c = 0; c < NT; ++c)
+#pragma unroll
+          for (int j = 0; j < G; ++j)
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[c][j][s][e] *= back;
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float mx[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e)
           mx[e] = fmaxf(fmaxf(sc[0][nt][e], sc[0][nt][e + 2]), fmaxf(sc[1][nt][e], sc[1][nt][e + 2])) * colfac[nt][e];
-        if (__any_sync(0xffffffffu, mx[0] > m_ref[nt][0] + kDecGrow || mx[1] > m_ref[nt][1] + kDecGrow)) {
+        if (__any_sync(0xffffffffu, mx[0] > m_ref[nt][0] + kDecMove || mx[1] > m_ref[nt][1] + kDecMove)) {
           float al[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
 #pragma unroll
             for (int o = 4; o <= 16; o <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], o));
-            const float mm = mx[e] > m_ref[nt][e] ? mx[e] + kDecGrow : m_ref[nt][e];
+            const float mm = fmaxf(m_ref[nt][e], mx[e] - kDecSet);
             al[e] = m_ref[nt][e] == -INFINITY ? 0.0f : ex2_approx(m_ref[nt][e] - mm);
             m_ref[nt][e] = mm;
           }
@@ -483,10 +530,11 @@ __global__ void __launch_bounds__(32 * W, dec_resident(W, 8 * NT))
           const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
           const uint32_t x0 = __byte_perm(v0[j / 2], v0[G / 2 + j / 2], sel), x1 = __byte_perm(v1[j / 2], v1[G / 2 + j / 2], sel);
           const uint32_t y0 = x0 >> 8, y1 = x1 >> 8;
+          const __half2 t0 = __hmul2(bits_h2(s0[j]), vmul), t1 = __hmul2(bits_h2(s1[j]), vmul);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            uint32_t b0 = h2_bits(__hmul2(bits_h2(pb[nt][0]), bits_h2(s0[j])));
-            uint32_t b1 = h2_bits(__hmul2(bits_h2(pb[nt][1]), bits_h2(s1[j])));
+            uint32_t b0 = h2_bits(__hmul2(bits_h2(pb[nt][0]), t0));
+            uint32_t b1 = h2_bits(__hmul2(bits_h2(pb[nt][1]), t1));
             if constexpr (!kPlain) {  // p = 0 stays 0 beside whatever stands in a hidden token's scale
               b0 &= __hneu2_mask(bits_h2(pb[nt][0]), bits_h2(0u));
               b1 &= __hneu2_mask(bits_h2(pb[nt][1]), bits_h2(0u));
@@ -519,6 +567,7 @@ __global__ void __launch_bounds__(32 * W, dec_resident(W, 8 * NT))
     // ---- the warps' results meet in shared memory ----
     __syncthreads();  // every ring is idle
     float* so = reinterpret_cast<float*>(body);
+    const float up = __uint_as_float(static_cast<uint32_t>(127 + 24 - vexp) << 23), up16 = up * 0.0625f;  // 2^24 2^-vexp
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -531,10 +580,10 @@ __global__ void __launch_bounds__(32 * W, dec_resident(W, 8 * NT))
         for (int j = 0; j < G; ++j) {
           const float lw = __shfl_sync(0xffffffffu, low[nt][e], 4 * j + t);
           float4 o;
-          o.x = fmaf(16777216.0f, acc[nt][j][0][e], lw);
-          o.y = fmaf(1048576.0f, acc[nt][j][0][e + 2], lw);
-          o.z = fmaf(16777216.0f, acc[nt][j][1][e], lw);
-          o.w = fmaf(1048576.0f, acc[nt][j][1][e + 2], lw);
+          o.x = fmaf(up, acc[nt][j][0][e], lw);
+          o.y = fmaf(up16, acc[nt][j][0][e + 2], lw);
+          o.z = fmaf(up, acc[nt][j][1][e], lw);
+          o.w = fmaf(up16, acc[nt][j][1][e + 2], lw);
           *reinterpret_cast<float4*>(dst + 32 * j) = o;
         }
       }

@@ -10,7 +10,7 @@ pytestmark = pytest.mark.gpu
 
 import rldx_b200  # noqa: E402,F401
 from rldx_b200 import ops  # noqa: E402
-from test_kv4_gpu import check_attention, cumulative, filled_cache  # noqa: E402
+from test_kv4_gpu import U, check_attention, cumulative, filled_cache, stored  # noqa: E402
 
 BF, F64, I32 = torch.bfloat16, torch.float64, torch.int32
 
@@ -38,3 +38,101 @@ def test_many_sequences(cuda, seqs, hq, hkv, d, longest):
     some = [b for b in range(seqs) if lens[b] and (b < 40 or b % 37 == 0 or b > 1000)]
     rows = cu[:-1][some].long()
     check_attention(q[rows], cache, table[some], lengths[some], cumulative(cuda, [1] * len(some)), out[rows])
+
+
+# ------------------------------------------------------------------------------------------------
+# values and weights of any size
+# ------------------------------------------------------------------------------------------------
+def cache_of(dev, k, v, d, page=64):
+    """A cache of one sequence that holds k, v [n, heads, d] (k is normed per head on the way in)."""
+    n, hkv = k.shape[0], k.shape[1]
+    pages = -(-n // page)
+    cache = ops.kv4_cache(pages, hkv, d, page, device=dev).fill_(0xFF)
+    table, lengths = torch.arange(pages, dtype=I32, device=dev)[None], torch.tensor([n], dtype=I32, device=dev)
+    one, cos, sin = torch.ones(d, device=dev).to(BF), torch.ones(1, d, device=dev), torch.zeros(1, d, device=dev)
+    qkv = torch.cat([torch.zeros_like(k), k, v], 1).flatten(1).to(BF)
+    ops.qkv_rope_append(qkv, one, one, cos, sin, torch.zeros(n, dtype=I32, device=dev), cache, table, lengths,
+                        cumulative(dev, [n]), q_heads=hkv)
+    return cache, table, lengths
+
+
+def check_by_weights(q, cache, table, lengths, out, scale):
+    """Every element of the rows q [new, heads, d] of one sequence, and the rows' norm.
+
+    With w the softmax weights and B = sum_k w_k max_c |v_kc|, what the kernels round moves an element by no more than
+      2^-8 |o|                   the output's rounding to bf16
+      2 x 2^-11 x 2 B            p, and p scale or V rebuilt, to fp16 (numerator and sum; scale code <= 2 max |v|)
+      2^-14 B                    fp32 scores, exponentials and sums
+      2 x 2^-11 S B              K rebuilt to fp16 (chunks), S = sum_c |q_c k_c| scale, of the largest row
+      2^-32 n w_max max |v|      fp16's last bits: p is held at 2^7 and more times the largest weight's 1
+    """
+    n, new = lengths.item(), q.shape[0]
+    k, v = (stored(cache, table, 0, n, w) for w in (0, 1))
+    group = q.shape[1] // k.shape[1]
+    k, v = k.repeat_interleave(group, 1), v.repeat_interleave(group, 1)
+    s = torch.einsum("ihd,khd->ihk", q.to(F64), k) * scale
+    hidden = torch.arange(n, device=q.device) > (n - new + torch.arange(new, device=q.device))[:, None, None]
+    w = s.masked_fill(hidden, -math.inf).softmax(-1)
+    ref = torch.einsum("ihk,khd->ihd", w, v)
+    top = v.abs().amax(-1).t()  # [heads, keys]
+    big = (w * top).sum(-1, keepdim=True)
+    spread = torch.einsum("ihd,khd->ihk", q.to(F64).abs(), k.abs()).amax(-1, keepdim=True) * scale
+    tol = U * ref.abs() + (2.0 ** -9 + 2.0 ** -14 + 2.0 ** -10 * spread) * big
+    tol = tol + 2.0 ** -32 * n * w.amax(-1, keepdim=True) * top.amax(-1)[:, None]
+    err = (out.to(F64) - ref).abs()
+    assert bool((err <= tol).all()), ((err / tol).max().item(), (err.norm() / ref.norm()).item())
+    return (err.norm() / ref.norm()).item()
+
+
+@pytest.mark.parametrize("new", [1, 5, 300])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("size", [1.0, 1e-2, 1e-4, 1e3])
+def test_values_of_any_size(cuda, size, d, new):
+    """V's scales from fp16's last bits to its thousands: the error stays what rounding the output makes it."""
+    g = torch.Generator(device=cuda).manual_seed(d + new)
+    n, hkv, hq = 4001, 2, 16
+    k, v = (torch.randn(n, hkv, d, device=cuda, generator=g) for _ in range(2))
+    cache, table, lengths = cache_of(cuda, k, v * size, d)
+    q = torch.randn(new, hq, d, device=cuda, generator=g).mul(1.5).to(BF)
+    out = ops.kv4_attention(q, cache, table, lengths, cumulative(cuda, [new]), max_new=new, max_len=n)
+    # bf16's rounding alone is 2^-8 / sqrt(3) at most, in the mean over a row
+    assert check_by_weights(q, cache, table, lengths, out, d ** -0.5) <= 2.0 ** -8
+
+
+@pytest.mark.parametrize("new", [1, 5])
+@pytest.mark.parametrize("d", [64, 128])
+def test_values_that_grow_along_the_sequence(cuda, d, new):
+    """Sizes from 1e-4 to 1e3 in one sequence, up, down and mixed: the running power of two follows."""
+    g = torch.Generator(device=cuda).manual_seed(d)
+    n = 3000
+    sizes = 10.0 ** torch.linspace(-4, 3, n, device=cuda)
+    for order in (torch.arange(n), torch.arange(n).flip(0), torch.randperm(n, generator=torch.Generator().manual_seed(1))):
+        k, v = (torch.randn(n, 2, d, device=cuda, generator=g) for _ in range(2))
+        cache, table, lengths = cache_of(cuda, k, v * sizes[order.to(cuda)][:, None, None], d)
+        q = torch.randn(new, 16, d, device=cuda, generator=g).to(BF)
+        out = ops.kv4_attention(q, cache, table, lengths, cumulative(cuda, [new]), max_new=new, max_len=n)
+        check_by_weights(q, cache, table, lengths, out, d ** -0.5)
+
+
+@pytest.mark.parametrize("new", [1, 3])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("bits", [9.3, 17.3, 22.415, 24.415])
+def test_small_weights_beside_a_large_one(cuda, bits, d, new):
+    """The first token takes nearly all weight and holds zeros; the others, 2^-bits of its weight each, make the result."""
+    small_weights(cuda, bits, d, new)
+
+
+def small_weights(cuda, bits, d, new):
+    g = torch.Generator(device=cuda).manual_seed(d)
+    n, hkv, hq = 2000, 2, 16
+    k = torch.randn(1, hkv, d, device=cuda, generator=g).expand(n, hkv, d).clone()
+    k[0] = 1.0 - 2.0 * (torch.arange(d, device=cuda) % 2)
+    v = 0.02 * (1.0 + 0.3 * torch.randn(n, hkv, d, device=cuda, generator=g))
+    v[0] = 0.0
+    cache, table, lengths = cache_of(cuda, k, v, d)
+    q = k[0, 0].to(BF).expand(new, hq, d).contiguous()
+    held = stored(cache, table, 0, n, 0)
+    gap = torch.einsum("d,khd->kh", q[0, 0].to(F64), held[:2])
+    scale = bits * math.log(2.0) / (gap[0] - gap[1]).min().item()  # one kv head at `bits`, the other a little past it
+    out = ops.kv4_attention(q, cache, table, lengths, cumulative(cuda, [new]), max_new=new, max_len=n, scale=scale)
+    check_by_weights(q, cache, table, lengths, out, torch.tensor(scale, dtype=torch.float32).item())
