@@ -3,9 +3,10 @@
 // of 128, and runs over the keys they can see in tiles of 64 (two units):
 //   S = Q K^T (M = 128, N = 64, K = d), P = exp2(S - m), O += P V (M = 128, N = d, K = 64)
 // with S, P and O in tensor memory and the codes rebuilt to fp16 on the way to shared memory:
-// scale code + low in one fp16 fma, whose rounding (2^-11) is far inside the 4-bit step.  q goes to
-// fp16 scaled by a power of two per row (largest in [2^14, 2^15)), p is at most 2^8 by the lazy
-// reference maximum of joint_attention_kernel; sums and maxima are fp32.
+// scale code + low in one fp16 fma, off by 2^-11 of the value.  q goes to
+// fp16 scaled by a power of two per row (largest in [2^14, 2^15)).  p is fp16, off by 2^-11 and by 2^-25 beside a largest
+// of 2^7 to 2^15 (a reference moved lazily, kChunkSet, kChunkMove); sums and maxima are fp32.  With a largest of 1
+// to 2^8 a thousand tokens at 2^-24.4 of the largest weight counted a third too much.
 //
 // Warps: 0 fetches units by bulk copies, 1 issues the MMAs, 2-3 rebuild K, 4-11 do the softmax (one row a
 // thread), 12-15 rebuild V^T; registers move from the first four to the softmax.  The order of
@@ -25,7 +26,7 @@
 // and a second kernel joins their parts (the rule and both sides' times: decode_plan).  With more than
 // a wave of tiles each CTA has its own, longest first.
 //
-// Measured: 8 sequences of up to 2300 tokens, up to 1104 of them new, 16 / 2 heads, d = 128: 139 us, 31 % of
+// Measured: 8 sequences of up to 2300 tokens, up to 1104 of them new, 16 / 2 heads, d = 128: 140 us, 31 % of
 // cuBLAS's bf16 rate (44 us).  No role bounds it alone: without three quarters of K's rebuilding, of V's, or
 // without nearly all exponentials it takes 138, 133 and 131 us.  K's tiles of 64 keys give an MMA of N = 64, P takes S's
 // place, and the chain S, softmax, P V of the two query tiles covers each other's waits only in part.
@@ -35,6 +36,9 @@
 namespace rldx {
 
 namespace {
+// A row's reference (log2 units) stands 7 below the largest score when it is set and is set again once one passes it
+// by more than 15: p = 2^(score - reference) is at most 2^15, and 2^7 or more for the largest.
+constexpr float kChunkSet = 7.0f, kChunkMove = 15.0f;
 constexpr unsigned int kErrKv4Chunk = 0x520;  // + role: a bounded wait ran out
 
 template <int D>
@@ -604,11 +608,11 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
 #pragma unroll
       for (int c = 0; c < 64; ++c) mx4[c & 3] = fmaxf(mx4[c & 3], sv[c]);
       const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * fac;
-      const bool grow = mx > m_ref + kRescaleLog2;
+      const bool grow = mx > m_ref + kChunkMove;
       float alpha = 1.0f;
       if (grow) {
-        alpha = m_ref == -INFINITY ? 0.0f : ex2_approx(m_ref - mx);
-        m_ref = mx;
+        alpha = m_ref == -INFINITY ? 0.0f : ex2_approx(m_ref - (mx - kChunkSet));
+        m_ref = mx - kChunkSet;
         l_run *= alpha;
       }
       if (j > 0 && __any_sync(0xffffffffu, grow)) {  // O holds PV_0 .. PV_{j-1}: scale the rows that moved

@@ -114,15 +114,11 @@ def test_values_that_grow_along_the_sequence(cuda, d, new):
         check_by_weights(q, cache, table, lengths, out, d ** -0.5)
 
 
-@pytest.mark.parametrize("new", [1, 3])
+@pytest.mark.parametrize("new", [1, 3, 300, 2000])
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("bits", [9.3, 17.3, 22.415, 24.415])
 def test_small_weights_beside_a_large_one(cuda, bits, d, new):
     """The first token takes nearly all weight and holds zeros; the others, 2^-bits of its weight each, make the result."""
-    small_weights(cuda, bits, d, new)
-
-
-def small_weights(cuda, bits, d, new):
     g = torch.Generator(device=cuda).manual_seed(d)
     n, hkv, hq = 2000, 2, 16
     k = torch.randn(1, hkv, d, device=cuda, generator=g).expand(n, hkv, d).clone()
