@@ -32,7 +32,9 @@ int rldx_version(void);
 /* Message of the last failed call on this thread ("" if none). */
 const char* rldx_last_error(void);
 
-/* Reads and clears the device-side error word (0 = none).  Synchronizes the device. */
+/* Reads and clears the device-side error (0 = none).  Synchronizes the device.  A wait that ran out comes first,
+ * then what a kernel found in its data, left out and went on from (the cache operators' 0x500 to 0x502; these
+ * stop no other call): both set take two calls. */
 int rldx_get_device_error(unsigned int* code);
 
 /* Bound of every wait inside the kernels, in SM clock cycles (default 4e9, about 2 s at full

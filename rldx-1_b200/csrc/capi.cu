@@ -783,11 +783,16 @@ int rldx_get_device_error(unsigned int* code) {
   if (!code) return set_error(RLDX_ERR_ARG, "null code");
   cudaError_t e = cudaDeviceSynchronize();
   if (e != cudaSuccess) return cuda_fail(e, "cudaDeviceSynchronize");
-  unsigned int v = 0, zero = 0;
+  unsigned int v = 0;
+  const unsigned int zero = 0;
   e = cudaMemcpyFromSymbol(&v, g_rldx_err, sizeof(v));
-  if (e != cudaSuccess) return cuda_fail(e, "read device error");
-  e = cudaMemcpyToSymbol(g_rldx_err, &zero, sizeof(zero));
-  if (e != cudaSuccess) return cuda_fail(e, "clear device error");
+  if (e == cudaSuccess && v) {
+    e = cudaMemcpyToSymbol(g_rldx_err, &zero, sizeof(zero));
+  } else if (e == cudaSuccess) {
+    e = cudaMemcpyFromSymbol(&v, g_rldx_data_err, sizeof(v));
+    if (e == cudaSuccess && v) e = cudaMemcpyToSymbol(g_rldx_data_err, &zero, sizeof(zero));
+  }
+  if (e != cudaSuccess) return cuda_fail(e, "read and clear device error");
   *code = v;
   return RLDX_OK;
 }

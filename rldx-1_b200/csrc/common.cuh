@@ -17,6 +17,9 @@ namespace rldx {
 // Error word shared by every kernel of the library.  The library is built as one translation
 // unit (rldx_b200.cu includes every .cu file), so this is its only definition.
 __device__ unsigned int g_rldx_err = 0;
+// What a kernel found in its data on the device (an index outside its table), left out and went on from.  A
+// word of its own: every wait gives up early once g_rldx_err is set, and such data must not stop other callers.
+__device__ unsigned int g_rldx_data_err = 0;
 
 enum DeviceError : unsigned int {
   kErrNone = 0,
@@ -34,6 +37,9 @@ __device__ long long g_rldx_wait_limit = kWaitLimitCycles;
 
 __device__ __forceinline__ void record_error(unsigned int code) {
   atomicCAS(&g_rldx_err, 0u, code);
+}
+__device__ __forceinline__ void record_data_error(unsigned int code) {
+  atomicCAS(&g_rldx_data_err, 0u, code);
 }
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {

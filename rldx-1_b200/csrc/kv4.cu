@@ -71,7 +71,7 @@ __device__ __forceinline__ int kv4_token_place(const Kv4Cache& c, const int* cu,
   const int pos = lengths[b] - cu[b + 1] + row;
   *tau = pos & (kKv4Unit - 1);
   const int index = pos >= 0 ? kv4_unit_index(c, b, 0, pos / kKv4Unit) : -1;
-  if (index < 0) record_error(kErrKv4Table);
+  if (index < 0) record_data_error(kErrKv4Table);
   return index;
 }
 
@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(128) kv4_append_kernel(const __grid_constant__
       for (int i = 0; i < 2; ++i)
         x[r][i] = __ldcs(reinterpret_cast<const uint2*>(P.qkv + tok * P.ld + min(h0 + r, hq - 1) * D + i * (D / 2) + 4 * l));
     if (static_cast<unsigned>(rp) >= static_cast<unsigned>(P.rope_rows)) {
-      if (live) record_error(kErrKv4Rope);
+      if (live) record_data_error(kErrKv4Rope);
       rp = 0;
     }
     float2 w[2][2], c[2][2], s[2][2];
@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(128) kv4_append_kernel(const __grid_constant__
   float w[8], c[8], s[8];
   load8(P.wk + 8 * l, w);
   if (static_cast<unsigned>(rp) >= static_cast<unsigned>(P.rope_rows)) {
-    if (live) record_error(kErrKv4Rope);
+    if (live) record_data_error(kErrKv4Rope);
     rp = 0;
   }
   const uint4 xk = __ldcs(reinterpret_cast<const uint4*>(src + (hq + at) * D));

@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
     const int b = item / max_tiles, c0 = (item - b * max_tiles) * 256;
     const int q0 = P.c.cu[b], nq = P.c.cu[b + 1] - q0, len = P.c.lengths[b];
     if (!chunk_in_bounds(P, q0, nq, len)) {
-      if (nq != 0 && threadIdx.x == 0) record_error(kErrKv4Bound);
+      if (nq != 0 && threadIdx.x == 0) record_data_error(kErrKv4Bound);
       return;
     }
     const int nrows = min(256, nq * P.group - c0);
@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
       if ((j & 15) == 0) {
         const int u = span.x + 2 * j + lane;
         index = u < span.w ? kv4_unit_index(P.c, b, kvh, ChunkShare::unit(span, u)) : -1;
-        if (u < span.w && index < 0) record_error(kErrKv4Table);
+        if (u < span.w && index < 0) record_data_error(kErrKv4Table);
       }
       const int a = __shfl_sync(0xffffffffu, index, 2 * (j & 15)), c = __shfl_sync(0xffffffffu, index, 2 * (j & 15) + 1);
       const int s = j % kR;

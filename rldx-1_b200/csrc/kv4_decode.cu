@@ -132,7 +132,7 @@ __device__ __forceinline__ int tile_units(const Kv4AttnParams& P, int len, int n
 __device__ __forceinline__ int sequence_units(const Kv4AttnParams& P, int b, int cols) {
   const int q0 = P.c.cu[b], nq = P.c.cu[b + 1] - q0, len = P.c.lengths[b];
   if (nq <= 0 || q0 < 0 || nq > P.max_new || len > P.max_len || q0 + nq > P.c.tokens) {
-    if (nq != 0) record_error(kErrKv4Bound);
+    if (nq != 0) record_data_error(kErrKv4Bound);
     return 0;
   }
   int n = 0;
@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(32 * W, dec_resident(W, 8 * NT))
         const int u = span.unit(u0 + warp + W * i), key0 = kKv4Unit * u, key1 = key0 + kKv4Unit - 1;
         if (span.count > 0) {
           index = kv4_unit_index(P.c, b, kvh, u);
-          if (index < 0) record_error(kErrKv4Table);
+          if (index < 0) record_data_error(kErrKv4Table);
         }
         all = index >= 0 && key1 <= span.pos_lo && (P.window <= 0 || span.pos_hi - key0 < P.window || key1 < P.sinks);
       }

@@ -313,7 +313,8 @@ def swiglu_bias(segments) -> None:
 
 
 def device_error() -> int:
-    """Reads and clears the device-side error word (synchronizes)."""
+    """Reads and clears the device-side error (synchronizes): a wait that ran out first, at the next call what a
+    kernel found in its data and left out."""
     v = C.c_uint(0)
     check(load().rldx_get_device_error(C.byref(v)))
     return int(v.value)
