@@ -661,8 +661,10 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
       if (lane == 0) mbar_arrive(&p_full(g)[sb]);
     }
     if (ok && nt > 0) ok = mbar_wait(o_final(g), 0u, kErrKv4Chunk + 3);
-    if (__all_sync(0xffffffffu, ok) && g < ng) {
+    if (g < ng) {
+      const bool fine = __all_sync(0xffffffffu, ok);  // no wait has run out: else NaN
       tc_fence_after();
+      if (!fine) l_run = NAN;
       const bool whole = P.split == 1;
       const int row = share.c0 + 128 * g + r, tok = row / P.group, head = share.kvh * P.group + row - tok * P.group;
       const bool live = 128 * g + r < share.nrows;
@@ -673,14 +675,14 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
       for (int h = 0; h < D / 32; ++h) {
         if (nt == 0 && !whole) break;  // (-inf, 0) says that there is nothing
         float o[32];
-        if (nt > 0) {
+        if (nt > 0 && fine) {
           tmem_ld32(tmem + lane_off + Sh::kOCol + g * D + 32 * h, o);
           tmem_wait_ld();
         } else {
 #pragma unroll
           for (int c = 0; c < 32; ++c) o[c] = 0.0f;
         }
-        const float f = (poison >> h & 1u) ? NAN : inv;
+        const float f = !fine || (poison >> h & 1u) ? NAN : inv;
 #pragma unroll
         for (int c = 0; c < 32; ++c) o[c] *= f;
         if (live && whole) {

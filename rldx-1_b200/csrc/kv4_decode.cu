@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(32 * W, dec_resident(W, 8 * NT))
   uint64_t* bar = bars + warp * kDecStages;
   bool began = false;  // thread 0: a segment begins here and goes on
   int turn = 0;  // units this warp has fetched into its ring and consumed, over all segments
-  bool ok = true;
+  bool ok = true;  // no wait of this warp has run out: else its ring is not used again and what it has a part in is NaN
 
   for (int at = begin; at < end;) {
     // ---- the segment that unit `at` of the line belongs to ----
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(32 * W, dec_resident(W, 8 * NT))
 
     // lane i holds the i-th of this warp's next 32 units: its index in the pool, and in a ballot
     // whether every column sees every token of it
-    const int mine = (m - warp + W - 1) / W;
+    const int mine = ok ? (m - warp + W - 1) / W : 0;
     int index = -1;
     unsigned clear = 0u;
     auto look = [&](int round) {
@@ -562,7 +562,13 @@ __global__ void __launch_bounds__(32 * W, dec_resident(W, 8 * NT))
         fetch(i + kDecStages, st);
       }
     }
-    if (!ok) settle_issued_copies();
+    if (!ok) {
+      settle_issued_copies();
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) low[nt][e] = NAN;
+    }
 
     // ---- the warps' results meet in shared memory ----
     __syncthreads();  // every ring is idle

@@ -55,3 +55,34 @@ def test_steps_after_it_run_clean(cuda, small_chain):
     assert torch.equal(token, x.argmax(-1))
     assert ops.device_error() == 0x500
     assert ops.device_error() == 0
+
+
+@pytest.mark.parametrize("lens", [[8192] * 48, [60000, 90, 31]])
+def test_rows_of_a_wait_that_ran_out_are_nan(cuda, lens):
+    """Under a bound that a copy from memory may pass, a row is right or NaN, and NaN comes with the wait's code.  (The
+    bound is looked at every 256 polls: on an idle GPU none runs out and every row is right.)"""
+    g = torch.Generator(device=cuda).manual_seed(6)
+    cache, table, lengths = filled_cache(cuda, lens, 2, 128, 64, g)
+    n = len(lens)
+    q = torch.randn(n, 16, 128, device=cuda, generator=g).to(BF)
+    cu = cumulative(cuda, [1] * n)
+    flush = torch.empty(1 << 28, dtype=torch.uint8, device=cuda)
+
+    def attend():
+        flush.fill_(1)  # the cache is not in L2
+        return ops.kv4_attention(q, cache, table, lengths, cu, max_new=1, max_len=max(lens))
+
+    want = attend()
+    assert ops.device_error() == 0
+    limit = ops.get_wait_limit()
+    try:
+        ops.set_wait_limit(1000)
+        for _ in range(10):
+            got = attend()
+            code = ops.device_error()
+            nan = torch.isnan(got.float()).any(2)
+            assert torch.equal(got[~nan], want[~nan])
+            assert code in (0, 0x510) and bool(nan.any()) <= (code == 0x510)
+    finally:
+        ops.set_wait_limit(limit)
+    assert torch.equal(attend(), want) and ops.device_error() == 0
