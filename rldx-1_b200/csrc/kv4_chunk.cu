@@ -20,7 +20,8 @@
 //
 // A value of V that is not finite, of a token that some rows must not see, cannot go through a
 // product with p = 0: it is rebuilt as 0, its place marked, and the rows that do see the token
-// give NaN in the channels of its group (in every channel where K is not finite).
+// give NaN in the channels of its group (in every channel where K is not finite).  A unit without a page
+// is marked the same way and hidden from every row, whatever its place in the ring holds.
 //
 // Few tiles of rows would leave most SMs idle, so up to two waves' worth of CTAs share a tile's keys evenly
 // and a second kernel joins their parts (the rule and both sides' times: decode_plan).  With more than
@@ -57,7 +58,9 @@ struct ChunkShape {
   static constexpr uint32_t kOCol = 256;  // S / P: (2 g + buffer) 64 columns; O of tile g: 256 + g d
   static constexpr uint32_t kTmemCols = 512;
   static constexpr int kBars = 1 + 2 * kRawStages + 4 * kStages + 2 * 7 + 1;
-  static constexpr int kBad = kStages * (kG + 2) * 8;  // marks of what is not finite, a bit per token: V's groups, K; any
+  // Marks of a stage of V: what is not finite, a bit per token, in V's groups and K; then a byte for each eight tokens,
+  // 1: there is any, 2: their unit has no page.  Then a byte a raw stage: which of its units have none.
+  static constexpr int kBad = kStages * (kG + 2) * 8 + 8;
   static constexpr size_t kSmem = 1024 + 2 * kQTile + kStages * (kKTile + kVTile) + kRawStages * kRaw + kBad + 8 * kBars + 16 + 64;
 };
 
@@ -206,6 +209,7 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
   uint8_t* sV = sK + kS * Sh::kKTile;
   uint8_t* sRaw = sV + kS * Sh::kVTile;
   uint8_t* sBad = sRaw + kR * Sh::kRaw;  // [stage][group of V, then K, then any][8] bytes
+  uint8_t* sGone = sBad + kS * (G + 2) * 8;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sBad + Sh::kBad);
   uint64_t* q_full = bars;
   uint64_t* raw_full = bars + 1;
@@ -287,8 +291,8 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
     for (int j = 0; j < nt; ++j) {
       if ((j & 15) == 0) {
         const int u = span.x + 2 * j + lane;
-        index = u < span.w ? kv4_unit_index(P.c, b, kvh, ChunkShare::unit(span, u)) : -1;
-        if (u < span.w && index < 0) record_data_error(kErrKv4Table);
+        index = u < span.w ? kv4_unit_index(P.c, b, kvh, ChunkShare::unit(span, u)) : -2;
+        if (index == -1) record_data_error(kErrKv4Table);
       }
       const int a = __shfl_sync(0xffffffffu, index, 2 * (j & 15)), c = __shfl_sync(0xffffffffu, index, 2 * (j & 15) + 1);
       const int s = j % kR;
@@ -296,6 +300,7 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
         ok = mbar_wait(&raw_empty[s], (static_cast<uint32_t>(j / kR) & 1u) ^ 1u, kErrKv4Chunk);
         if (ok) {
           const int n = (a >= 0) + (c >= 0);
+          sGone[s] = (a == -1 ? 1 : 0) | (c == -1 ? 2 : 0);
           if (n)
             mbar_arrive_expect_tx(&raw_full[s], n * U::kBytes);
           else
@@ -454,6 +459,7 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
       for (int i = 0; i < G; ++i) zk = __hfma2(bits_h2(meta[i]), bits_h2(0u), zk);
       const unsigned bad_k = __ballot_sync(0xffffffffu, h2_bits(zk) & 0x7fff7fffu);
       const bool odd = (h2_bits(z) & 0x7fff7fffu) != 0u;  // a value would not be finite
+      const uint32_t gone = (sGone[rs] >> (w >> 1) & 1u) << 1;  // (a warp's tokens are of one unit)
       uint32_t bad[G];
 #pragma unroll
       for (int gi = 0; gi < G; ++gi) bad[gi] = 0u;
@@ -476,13 +482,14 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
 #pragma unroll 1
           for (int i = 0; i < 8; ++i) byte |= (bad_k >> (4 * i + lane) & 1u) << (chunk_row(8 * o + i) & 7);
           sBad[(s * (G + 2) + G) * 8 + o] = static_cast<uint8_t>(byte);
-          sBad[(s * (G + 2) + G + 1) * 8 + o] = 1u;
+          sBad[(s * (G + 2) + G + 1) * 8 + o] = static_cast<uint8_t>(1u | gone);
         }
         __syncwarp();
       } else if (g == 0 && h == 0) {
         // another warp's groups may be marked: then these are read too
 #pragma unroll
-        for (int gi = 0; gi <= G + 1; ++gi) sBad[(s * (G + 2) + gi) * 8 + o] = 0u;
+        for (int gi = 0; gi <= G; ++gi) sBad[(s * (G + 2) + gi) * 8 + o] = 0u;
+        sBad[(s * (G + 2) + G + 1) * 8 + o] = static_cast<uint8_t>(gone);
       }
       uint8_t* dst = sV + s * Sh::kVTile;
 #pragma unroll
@@ -575,7 +582,12 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
       const int sb = j & 1;
       const uint32_t ph = static_cast<uint32_t>(j >> 1) & 1u;
       const uint32_t s_col = tmem + lane_off + (2 * g + sb) * 64;
-      // ---- masks: keys of the two units; a unit past the span is hidden ----
+      // ---- masks: keys of the two units; a unit past the span is hidden, and one without a page (the marks are
+      // there once V_j is) ----
+      ok = __all_sync(0xffffffffu, mbar_wait(&v_full[j % kS], static_cast<uint32_t>(j / kS) & 1u, kErrKv4Chunk + 3));
+      if (!ok) break;
+      const uint32_t* marks = reinterpret_cast<const uint32_t*>(sBad + (j % kS) * (G + 2) * 8);
+      const uint32_t mark[2] = {marks[2 * G + 2], marks[2 * G + 3]};
       bool plain = true;
       int key0[2];
       const int4 span = share.span();
@@ -585,12 +597,16 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
         key0[i] = u < span.w ? kKv4Unit * ChunkShare::unit(span, u) : 0x40000000;
         plain &= key0[i] + 31 <= pos_lo && (P.window <= 0 || pos_hi - key0[i] < P.window || key0[i] + 31 < P.sinks);
       }
+      plain &= ((mark[0] | mark[1]) & 0x02020202u) == 0u;
       uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
       if (!plain) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
           seen[i] = P.window > 0 ? chunk_seen(ps - key0[i] + 1, ps - P.window - key0[i], P.sinks - key0[i])
                                  : chunk_seen(ps - key0[i] + 1, -1, 0);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (mark[i] & 0x02020202u) seen[i] = 0u;
       }
       ok = __all_sync(0xffffffffu, mbar_wait(&s_full(g)[sb], ph, kErrKv4Chunk + 3));
       if (!ok) break;
@@ -647,11 +663,8 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
       }
       l_run += (sum0.x + sum0.y) + (sum1.x + sum1.y);
       tmem_wait_st();
-      // ---- values that are not finite (the marks are there once V_j is) ----
-      ok = __all_sync(0xffffffffu, mbar_wait(&v_full[j % kS], static_cast<uint32_t>(j / kS) & 1u, kErrKv4Chunk + 3));
-      if (!ok) break;
-      const uint32_t* marks = reinterpret_cast<const uint32_t*>(sBad + (j % kS) * (G + 2) * 8);
-      if (marks[2 * G + 2] | marks[2 * G + 3]) {
+      // ---- values that are not finite ----
+      if (mark[0] | mark[1]) {
 #pragma unroll 1
         for (int gi = 0; gi <= G; ++gi)
           if ((seen[0] & marks[2 * gi]) | (seen[1] & marks[2 * gi + 1])) poison |= gi < G ? 1u << gi : 0xffffffffu;

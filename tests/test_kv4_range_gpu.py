@@ -132,3 +132,45 @@ def test_small_weights_beside_a_large_one(cuda, bits, d, new):
     scale = bits * math.log(2.0) / (gap[0] - gap[1]).min().item()  # one kv head at `bits`, the other a little past it
     out = ops.kv4_attention(q, cache, table, lengths, cumulative(cuda, [new]), max_new=new, max_len=n, scale=scale)
     check_by_weights(q, cache, table, lengths, out, torch.tensor(scale, dtype=torch.float32).item())
+
+
+# ------------------------------------------------------------------------------------------------
+# what only the device can see
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("new,old", [([1], [700]), ([4, 1], [500, 90]), ([300, 2], [1200, 10]), ([40] * 20, [100] * 20),
+                                     ([2000], [0])])
+@pytest.mark.parametrize("window", [0, 200])
+@pytest.mark.parametrize("d", [64, 128])
+def test_tokens_without_a_page_are_hidden(cuda, d, window, new, old):
+    """Pages of the first sequence that its table does not name (-1, or past the pool) count for nothing, whichever kernel
+    runs and whatever was read before: the other tokens' attention, and the code of the table."""
+    g = torch.Generator(device=cuda).manual_seed(d + new[0])
+    lens = [a + b for a, b in zip(new, old)]
+    page, hq, hkv = 32, 16, 2
+    cache, table, lengths = filled_cache(cuda, lens, hkv, d, page, g, fill=0xFF, offset=8.0)
+    held = -(-lens[0] // page)
+    lost = sorted({0, 3, 4, held // 2, held - 2, held - 1} & set(range(held)))
+    torn = table.clone()
+    for i, p in enumerate(lost):
+        torn[0, p] = -1 if i % 2 else cache.shape[0]
+    q = torch.randn(sum(new), hq, d, device=cuda, generator=g).mul(1.5).to(BF)
+    cu = cumulative(cuda, new)
+    assert ops.device_error() == 0
+    out = ops.kv4_attention(q, cache, torn, lengths, cu, max_new=max(new), max_len=max(lens), window=window)
+    assert ops.device_error() == 0x500 and ops.device_error() == 0
+    k, v = (stored(cache, table, 0, lens[0], w) for w in (0, 1))
+    key = torch.arange(lens[0], device=cuda)
+    there = ~torch.isin(key // page, torch.tensor(lost, device=cuda))
+    rows = [i for i in range(new[0]) if i < 40 or i % 29 == 0]
+    pos = old[0] + torch.tensor(rows, device=cuda)[:, None]
+    seen = there & (key <= pos) & ((pos - key < window) if window else True)
+    s = torch.einsum("ihd,khd->ihk", q[rows].to(F64), k.repeat_interleave(hq // hkv, 1)) * d ** -0.5
+    w = s.masked_fill(~seen[:, None], -math.inf).softmax(-1).nan_to_num(0.0)  # no token left: zeros
+    ref = torch.einsum("ihk,khd->ihd", w, v.repeat_interleave(hq // hkv, 1))
+    # as check_attention's: the output's bf16, fp16 of p and of p scale or V, K in fp16, against the largest value
+    tol = U * ref.abs() + 2.0 ** -9 * v.abs().max()
+    assert bool(((out[rows].to(F64) - ref).abs() <= tol).all()), (out[rows].to(F64) - ref).abs().max().item()
+    if len(new) > 1:  # the other sequences have all their pages
+        some = list(range(1, len(new)))
+        last = cu[1:].long()[some] - 1
+        check_attention(q[last], cache, table[some], lengths[some], cumulative(cuda, [1] * len(some)), out[last], window)
