@@ -330,7 +330,7 @@ typedef struct rldx_kv4_cache {
  * mean's root), all in fp32: q to bf16 [tokens, q_heads, head_dim], k and v into the cache.
  * qkv: bf16 rows [q | k | v] with stride ld (a multiple of 8); q_norm, k_norm bf16 [head_dim];
  * rope_cos / rope_sin [rope_rows, head_dim] bf16, or fp32 with rope_fp32; rope_pos [tokens] rows
- * of them. */
+ * of them.  Rows before cu_seqlens[0] or past cu_seqlens[seqs] are stored nowhere (device error 0x502). */
 int rldx_kv4_append(const rldx_kv4_cache* cache, const void* qkv, int64_t ld, int tokens, int q_heads,
                     const void* q_norm, const void* k_norm, const void* rope_cos, const void* rope_sin,
                     int rope_fp32, int rope_rows, const int32_t* rope_pos, void* q_out, float eps, void* stream);

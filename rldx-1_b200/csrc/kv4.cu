@@ -64,12 +64,17 @@ __device__ __forceinline__ int seq_of_row(const int* cu, int seqs, int row) {
 
 constexpr int kKv4SmemSeqs = 1024;  // batches up to this size keep cu and lengths in shared memory
 
-// Where new-token row `row` stands in the cache: index of its unit for head 0 (-1: nowhere, recorded) and
-// its token in the unit; head h's unit is units_per_page h further.
+// Where new-token row `row` stands in the cache: index of its unit for head 0 (-1: nowhere, recorded; a row before
+// the first sequence's or past the last one's is none of theirs) and its token in the unit; head h's unit is
+// units_per_page h further.
 __device__ __forceinline__ int kv4_token_place(const Kv4Cache& c, const int* cu, const int* lengths, int row, int* tau) {
   const int b = seq_of_row(cu, c.seqs, row);
   const int pos = lengths[b] - cu[b + 1] + row;
   *tau = pos & (kKv4Unit - 1);
+  if (row < cu[b] || row >= cu[b + 1]) {
+    record_data_error(kErrKv4Bound);
+    return -1;
+  }
   const int index = pos >= 0 ? kv4_unit_index(c, b, 0, pos / kKv4Unit) : -1;
   if (index < 0) record_data_error(kErrKv4Table);
   return index;

@@ -26,7 +26,7 @@ constexpr int kKv4Unit = 32;  // tokens of a unit and channels of a group
 
 // Data errors of the cache kernels (record_data_error): an entry of the page table (or of lengths, cu_seqlens)
 // names memory outside the pool, a RoPE row is outside its table, a sequence is longer or has
-// more new tokens than the call said.  The access is skipped, the rest left out.
+// more new tokens than the call said or a row to be stored belongs to none.  The access is skipped, the rest left out.
 constexpr unsigned int kErrKv4Table = 0x500;
 constexpr unsigned int kErrKv4Rope = 0x501;
 constexpr unsigned int kErrKv4Bound = 0x502;

@@ -174,3 +174,28 @@ def test_tokens_without_a_page_are_hidden(cuda, d, window, new, old):
         some = list(range(1, len(new)))
         last = cu[1:].long()[some] - 1
         check_attention(q[last], cache, table[some], lengths[some], cumulative(cuda, [1] * len(some)), out[last], window)
+
+
+@pytest.mark.parametrize("seqs", [2, 1030])
+def test_append_stores_rows_of_sequences_only(cuda, seqs):
+    """Rows before the first sequence's and past the last one's change no byte of the cache, where there is a page too."""
+    g = torch.Generator(device=cuda).manual_seed(2)
+    d, hkv, lens = 64, 2, [20] * seqs
+    cache, table, lengths = filled_cache(cuda, lens, hkv, d, 32, g)
+    one, cos, sin = torch.ones(d, device=cuda).to(BF), torch.ones(1, d, device=cuda), torch.zeros(1, d, device=cuda)
+    lengths = lengths + 1  # one new token each, of pages that have room
+    plain, want = cache.clone(), None
+    qkv = torch.randn(seqs + 7, 3 * hkv * d, device=cuda, generator=g).to(BF)
+
+    def append(pool, rows, cu):
+        return ops.qkv_rope_append(rows, one, one, cos, sin, torch.zeros(rows.shape[0], dtype=I32, device=cuda), pool, table,
+                                   lengths, cu, q_heads=hkv)
+
+    want = append(plain, qkv[3:-4], cumulative(cuda, [1] * seqs))
+    assert ops.device_error() == 0
+    q = append(cache, qkv, cumulative(cuda, [1] * seqs) + 3)
+    assert ops.device_error() == 0x502 and ops.device_error() == 0
+    assert torch.equal(cache, plain) and torch.equal(q[3:-4], want)
+    k, v = ops.kv4_read(cache, table, lengths, cumulative(cuda, [1] * seqs) + 3, tokens=seqs + 7)
+    assert ops.device_error() == 0x502 and ops.device_error() == 0
+    assert not bool(k[:3].any()) and not bool(k[-4:].any()) and not bool(v[-4:].any()) and bool(k[3:-4].any(2).all())
