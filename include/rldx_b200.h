@@ -339,7 +339,8 @@ int rldx_kv4_append(const rldx_kv4_cache* cache, const void* qkv, int64_t ld, in
 int rldx_kv4_read(const rldx_kv4_cache* cache, int tokens, void* k, void* v, void* stream);
 
 /* Softmax attention of the new tokens' queries over the cache: the token at position p sees key
- * j <= p, with window > 0 only j > p - window or j < sinks.  A row that sees no key is zero.
+ * j <= p, with window > 0 only j > p - window or j < sinks.  A row that sees no key is zero, and one of no
+ * sequence, or of a sequence that breaks max_new or max_len (device error 0x502).
  * q, out bf16 [tokens, q_heads, head_dim], q with token stride ldq (a multiple of 8); query head
  * h reads kv head h / (q_heads / kv_heads).  max_new / max_len bound the new tokens and the
  * length of a sequence (they size the launch; values on the device may be smaller). */

@@ -103,6 +103,7 @@ struct Kv4AttnParams {
   int4* part_head;  // [CTAs] first row, columns, kv head, parts and first CTA of the segment that a CTA begins,
                     // or (by_segment) of each segment: sequence, tile of columns, kv head
   int by_segment, tiles;
+  int edges;           // this launch holds the batch's first sequence (1), its last (2)
   int split, ordered;  // kv4_chunk_kernel: CTAs that share the keys of a tile of rows; longest tiles first
 };
 
@@ -126,6 +127,14 @@ __device__ __forceinline__ Kv4Span kv4_span(int length, int nq, int tok_lo, int 
   if (s.first <= s.sink_units) s.first = s.sink_units = 0;
   s.count = s.sink_units + s.end - s.first;
   return s;
+}
+
+// Zeros in the output's rows [r0, r1), by thread i of n.
+__device__ __forceinline__ void kv4_zero_rows(const Kv4AttnParams& P, int d, int r0, int r1, int i, int n) {
+  const long long row = static_cast<long long>(P.q_heads) * d / 8;  // vectors of 16 bytes
+  uint4* out = reinterpret_cast<uint4*>(P.out);
+#pragma unroll 1
+  for (long long at = max(r0, 0) * row + i; at < min(r1, P.c.tokens) * row; at += n) out[at] = make_uint4(0u, 0u, 0u, 0u);
 }
 
 cudaError_t launch_kv4_chunk(Kv4AttnParams p, int head_dim, cudaStream_t stream);

@@ -252,9 +252,15 @@ __global__ void __launch_bounds__(ChunkShape<D>::kThreads, 1) kv4_chunk_kernel(c
     if (P.ordered) item = chunk_item_of_rank(P, item, max_tiles, reinterpret_cast<int*>(smem));
     const int b = item / max_tiles, c0 = (item - b * max_tiles) * 256;
     const int q0 = P.c.cu[b], nq = P.c.cu[b + 1] - q0, len = P.c.lengths[b];
-    if (!chunk_in_bounds(P, q0, nq, len)) {
-      if (nq != 0 && threadIdx.x == 0) record_data_error(kErrKv4Bound);
-      return;
+    const bool fine = chunk_in_bounds(P, q0, nq, len);
+    if (blockIdx.x == 0 || !fine) {  // zeros: in rows of no sequence, and of one that breaks the call's bounds
+      if (!fine && nq != 0 && threadIdx.x == 0) record_data_error(kErrKv4Bound);
+      const bool all = !fine && c0 == 0 && part == 0 && unsplit % P.c.kv_heads == 0;
+#pragma unroll 1
+      for (int k = blockIdx.x == 0 ? 0 : 2; k < (all ? 3 : 2); ++k)
+        kv4_zero_rows(P, D, k == 0 ? 0 : k == 1 ? P.c.cu[P.c.seqs] : q0, k == 0 ? P.c.cu[0] : k == 1 ? P.c.tokens : q0 + nq, threadIdx.x,
+                      blockDim.x);
+      if (!fine) return;
     }
     const int nrows = min(256, nq * P.group - c0);
     if (nrows <= 0) return;

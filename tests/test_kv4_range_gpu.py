@@ -176,6 +176,48 @@ def test_tokens_without_a_page_are_hidden(cuda, d, window, new, old):
         check_attention(q[last], cache, table[some], lengths[some], cumulative(cuda, [1] * len(some)), out[last], window)
 
 
+@pytest.mark.parametrize("new,old,max_new,max_len", [
+    ([1, 1, 0, 1, 1], [40, 700, 3, 90, 5], 1, 100),  # the second is longer than the call says
+    ([3, 7, 0, 2], [40, 20, 3, 90], 4, 100),         # the second has more new tokens
+    ([40, 300, 17, 600], [500, 20, 33, 0], 300, 545),  # chunks, the last breaks both
+    ([300, 2100], [100, 0], 300, 3000),              # chunks whose keys are shared out
+])
+def test_rows_that_get_no_attention_are_zero(cuda, new, old, max_new, max_len):
+    """Rows of a sequence that breaks the call's bounds (0x502), and rows before the first or past the last sequence's."""
+    g = torch.Generator(device=cuda).manual_seed(sum(new))
+    d, lens, head, tail = 128, [a + b for a, b in zip(new, old)], 3, 5
+    cache, table, lengths = filled_cache(cuda, lens, 2, d, 64, g, fill=0xFF)
+    cu = cumulative(cuda, new) + head
+    q = torch.randn(head + sum(new) + tail, 16, d, device=cuda, generator=g).to(BF)
+    out = torch.full_like(q, math.nan)
+    ops.kv4_attention(q, cache, table, lengths, cu, max_new=max_new, max_len=max_len, out=out)
+    assert ops.device_error() == 0x502 and ops.device_error() == 0
+    assert bool((out[:head] == 0).all()) and bool((out[-tail:] == 0).all())
+    for b, (n, length) in enumerate(zip(new, lens)):
+        rows = slice(cu[b].item(), cu[b + 1].item())
+        if n > max_new or length > max_len:
+            assert bool((out[rows] == 0).all()), b
+        elif n:
+            assert not bool(torch.isnan(out[rows].float()).any()), b
+            last = rows.stop - 1
+            check_attention(q[last: last + 1], cache, table[b: b + 1], lengths[b: b + 1], cumulative(cuda, [1]), out[last: last + 1])
+
+
+def test_rows_outside_every_launch(cuda):
+    """Batches of several launches: the rows around them are zeroed once, those between are not."""
+    g = torch.Generator(device=cuda).manual_seed(1)
+    seqs = 1030
+    lens = [1 + b % 9 for b in range(seqs)]
+    cache, table, lengths = filled_cache(cuda, lens, 2, 64, 32, g)
+    cu = cumulative(cuda, [1] * seqs) + 2
+    q = torch.randn(seqs + 6, 16, 64, device=cuda, generator=g).to(BF)
+    out = torch.full_like(q, math.nan)
+    ops.kv4_attention(q, cache, table, lengths, cu, max_new=1, max_len=9, out=out)
+    assert ops.device_error() == 0
+    assert bool((out[:2] == 0).all()) and bool((out[-4:] == 0).all())
+    check_attention(q[2:-4], cache, table, lengths, cumulative(cuda, [1] * seqs), out[2:-4])
+
+
 @pytest.mark.parametrize("seqs", [2, 1030])
 def test_append_stores_rows_of_sequences_only(cuda, seqs):
     """Rows before the first sequence's and past the last one's change no byte of the cache, where there is a page too."""
