@@ -139,6 +139,6 @@ __device__ __forceinline__ void kv4_zero_rows(const Kv4AttnParams& P, int d, int
 
 cudaError_t launch_kv4_chunk(Kv4AttnParams p, int head_dim, cudaStream_t stream);
 cudaError_t kv4_chunk_prepare_device();
-cudaError_t launch_kv4_decode(const Kv4AttnParams& p, int head_dim, int cols, int warps, int ctas, cudaStream_t stream);
+cudaError_t launch_kv4_decode(const Kv4AttnParams& p, int head_dim, int cols, int warps, int ctas, int batch, cudaStream_t stream);
 
 }  // namespace rldx

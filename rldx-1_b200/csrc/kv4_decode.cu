@@ -49,7 +49,8 @@ constexpr int kDecStages = 2;
 // by more than 15, so that p = 2^(score - reference) is at most 2^15, and 2^11 or more for the largest.
 constexpr float kDecSet = 11.0f, kDecMove = 15.0f;
 
-constexpr int kDecMaxSeqs = 1024;  // sequences of one launch (their prefix sums stand in shared memory)
+constexpr int kDecMaxSeqs = 1024;        // sequences of one launch (their prefix sums stand in shared memory)
+constexpr long long kDecMaxLine = 1 << 30;  // and units of all their segments (32-bit sums): pages may be shared, so memory sets no bound
 
 // A segment's start counts as this many units of a CTA's share: its lookups, the wait for its first units
 // and the merge of the one before (64 x 8192: 0 / 6 / 12 / 16 / 24 / 36 units 33.0 / 32.0 / 30.9 / 30.9 / 31.5 / 32.6 us).
@@ -784,14 +785,14 @@ cudaError_t launch_pdl(K kernel, dim3 grid, int threads, size_t smem, cudaStream
 }
 
 template <int D, int NT, int W>
-cudaError_t launch_decode(const Kv4AttnParams& whole, int ctas, cudaStream_t stream) {
-  for (int b0 = 0; b0 < whole.c.seqs; b0 += kDecMaxSeqs) {
+cudaError_t launch_decode(const Kv4AttnParams& whole, int ctas, int batch, cudaStream_t stream) {
+  for (int b0 = 0; b0 < whole.c.seqs; b0 += batch) {
     Kv4AttnParams p = whole;
-    p.c.seqs = std::min(kDecMaxSeqs, whole.c.seqs - b0);
+    p.c.seqs = std::min(batch, whole.c.seqs - b0);
     p.c.cu += b0;
     p.c.lengths += b0;
     p.c.table += static_cast<long long>(b0) * p.c.table_ld;
-    p.edges = (b0 == 0 ? 1 : 0) | (b0 + kDecMaxSeqs >= whole.c.seqs ? 2 : 0);
+    p.edges = (b0 == 0 ? 1 : 0) | (b0 + p.c.seqs >= whole.c.seqs ? 2 : 0);
     p.tiles = (p.max_new * p.group + 8 * NT - 1) / (8 * NT);
     // a few segments are cut into many parts each: then a CTA of the join per segment and column.  A launch that
     // cuts nothing has no join and no workspace for its segments' heads, however few sequences the last one holds.
@@ -816,14 +817,16 @@ cudaError_t decode_smem() {
   return e;
 }
 template <int D, int NT>
-cudaError_t launch_decode(const Kv4AttnParams& p, int warps, int ctas, cudaStream_t stream) {
-  return warps == kDecWarps ? launch_decode<D, NT, kDecWarps>(p, ctas, stream) : launch_decode<D, NT, kDecWarpsWide>(p, ctas, stream);
+cudaError_t launch_decode(const Kv4AttnParams& p, int warps, int ctas, int batch, cudaStream_t stream) {
+  return warps == kDecWarps ? launch_decode<D, NT, kDecWarps>(p, ctas, batch, stream)
+                            : launch_decode<D, NT, kDecWarpsWide>(p, ctas, batch, stream);
 }
 }  // namespace
 
-cudaError_t launch_kv4_decode(const Kv4AttnParams& p, int head_dim, int cols, int warps, int ctas, cudaStream_t stream) {
-  if (head_dim == 128) return cols == 8 ? launch_decode<128, 1>(p, warps, ctas, stream) : launch_decode<128, 2>(p, warps, ctas, stream);
-  return cols == 8 ? launch_decode<64, 1>(p, warps, ctas, stream) : launch_decode<64, 2>(p, warps, ctas, stream);
+cudaError_t launch_kv4_decode(const Kv4AttnParams& p, int head_dim, int cols, int warps, int ctas, int batch, cudaStream_t stream) {
+  if (head_dim == 128)
+    return cols == 8 ? launch_decode<128, 1>(p, warps, ctas, batch, stream) : launch_decode<128, 2>(p, warps, ctas, batch, stream);
+  return cols == 8 ? launch_decode<64, 1>(p, warps, ctas, batch, stream) : launch_decode<64, 2>(p, warps, ctas, batch, stream);
 }
 
 cudaError_t kv4_prepare_device() {
@@ -839,6 +842,7 @@ namespace {
 struct DecodePlan {
   int cols, ctas, whole;  // cols 0: kv4_chunk_kernel, its keys shared by `split` CTAs
   int split, warps;
+  int batch;  // sequences of a launch, 0: one alone has too many units
   uint64_t part_rows, bytes;  // workspace of unfinished segments
 };
 
@@ -877,10 +881,12 @@ DecodePlan decode_plan(const rldx_kv4_cache& c, int q_heads, int max_new, int ma
   long long keys = max_len;
   if (window > 0) keys = std::min<long long>(keys, static_cast<long long>(window) + max_new + std::min(sinks, max_len) + 3 * kKv4Unit);
   const long long units = (keys + kKv4Unit - 1) / kKv4Unit;
-  const long long segments = tiles * c.kv_heads * std::min(c.seqs, kDecMaxSeqs);
+  const long long line = tiles * c.kv_heads * ((static_cast<long long>(max_len) + kKv4Unit - 1) / kKv4Unit + kDecStart);
+  p.batch = static_cast<int>(std::min<long long>(kDecMaxSeqs, kDecMaxLine / line));
+  const long long segments = tiles * c.kv_heads * std::min(c.seqs, p.batch);
   if (rows > kDecMaxRows) {
     const long long heads = static_cast<long long>(c.kv_heads) * c.seqs, ctas = (rows + 255) / 256 * heads;
-    long long least = kDecBase + tiles * heads * (units + kDecStart);
+    long long least = p.batch > 0 ? kDecBase + tiles * heads * (units + kDecStart) : INT64_MAX;
     for (int split = 1; split == 1 || (split * ctas <= 2 * sm_count() && units >= split * kChunkShare); ++split) {
       const long long waves = (split * ctas + sm_count() - 1) / sm_count();
       const long long cost = waves * (rows > 128 ? kChunkUnit2 : kChunkUnit) * ((units + split - 1) / split + 10) +
@@ -901,6 +907,13 @@ DecodePlan decode_plan(const rldx_kv4_cache& c, int q_heads, int max_new, int ma
   p.part_rows = p.whole ? 0 : 2ull * p.ctas * p.cols;
   p.bytes = p.part_rows * (static_cast<uint64_t>(c.head_dim) * 4 + 8) + (p.part_rows ? 16ull * p.ctas : 0);
   return p;
+}
+
+int plan_of(const rldx_kv4_cache& c, const rldx_kv4_attention_desc& a, int max_len, DecodePlan* plan) {
+  *plan = decode_plan(c, a.q_heads, a.max_new, max_len, a.window, a.sinks);
+  if (plan->cols > 0 && plan->batch == 0)
+    return set_error(RLDX_ERR_UNSUPPORTED, "kv4_attention: max_len and the heads allow for more than 2^30 units of 32 tokens in a sequence");
+  return RLDX_OK;
 }
 
 int attention_args(const rldx_kv4_cache* cache, const rldx_kv4_attention_desc* a, Kv4AttnParams* p) {
@@ -931,8 +944,10 @@ int rldx_kv4_attention_workspace_size(const rldx_kv4_cache* cache, const rldx_kv
   Kv4AttnParams p;
   int rc = attention_args(cache, a, &p);
   if (rc != RLDX_OK) return rc;
-  *bytes = decode_plan(*cache, a->q_heads, a->max_new, p.max_len, a->window, a->sinks).bytes;
-  return RLDX_OK;
+  DecodePlan plan;
+  rc = plan_of(*cache, *a, p.max_len, &plan);
+  if (rc == RLDX_OK) *bytes = plan.bytes;
+  return rc;
 }
 
 int rldx_kv4_attention(const rldx_kv4_cache* cache, const rldx_kv4_attention_desc* a, void* workspace,
@@ -948,7 +963,9 @@ int rldx_kv4_attention(const rldx_kv4_cache* cache, const rldx_kv4_attention_des
   if (a->ldq < static_cast<int64_t>(a->q_heads) * d || a->ldq % 8)
     return set_error(RLDX_ERR_ARG, "kv4_attention: q rows must be 16-byte aligned and hold every head");
   if (a->tokens == 0) return RLDX_OK;
-  const DecodePlan plan = decode_plan(*cache, a->q_heads, a->max_new, p.max_len, a->window, a->sinks);
+  DecodePlan plan;
+  rc = plan_of(*cache, *a, p.max_len, &plan);
+  if (rc != RLDX_OK) return rc;
   if (plan.bytes > workspace_bytes || (plan.bytes > 0 && (!workspace || !aligned_to(workspace, 16))))
     return set_error(RLDX_ERR_ARG, "kv4_attention: needs a 16-byte aligned workspace of " + std::to_string(plan.bytes) + " bytes");
   p.q = static_cast<const __nv_bfloat16*>(a->q);
@@ -966,7 +983,7 @@ int rldx_kv4_attention(const rldx_kv4_cache* cache, const rldx_kv4_attention_des
   p.part_ml = reinterpret_cast<float2*>(p.part_o + plan.part_rows * d);
   p.part_head = reinterpret_cast<int4*>(p.part_ml + plan.part_rows);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e = plan.cols == 0 ? launch_kv4_chunk(p, d, st) : launch_kv4_decode(p, d, plan.cols, plan.warps, plan.ctas, st);
+  cudaError_t e = plan.cols == 0 ? launch_kv4_chunk(p, d, st) : launch_kv4_decode(p, d, plan.cols, plan.warps, plan.ctas, plan.batch, st);
   if (e != cudaSuccess) return cuda_fail(e, "kv4_attention launch");
   return RLDX_OK;
 }

@@ -241,3 +241,18 @@ def test_append_stores_rows_of_sequences_only(cuda, seqs):
     k, v = ops.kv4_read(cache, table, lengths, cumulative(cuda, [1] * seqs) + 3, tokens=seqs + 7)
     assert ops.device_error() == 0x502 and ops.device_error() == 0
     assert not bool(k[:3].any()) and not bool(k[-4:].any()) and not bool(v[-4:].any()) and bool(k[3:-4].any(2).all())
+
+
+def test_launches_of_few_sequences_where_lengths_may_be_huge(cuda):
+    """A max_len of 368 million tokens leaves two sequences to a launch, whose sums are 32-bit."""
+    g = torch.Generator(device=cuda).manual_seed(3)
+    new, old = [20, 1, 3, 20, 7], [100, 0, 3000, 12, 1]
+    lens = [a + b for a, b in zip(new, old)]
+    cache, table, lengths = filled_cache(cuda, lens, 24, 64, 32, g, fill=0xFF)
+    wide = torch.full((5, 11_500_000), -1, dtype=I32, device=cuda)
+    wide[:, : table.shape[1]] = table
+    q = torch.randn(sum(new), 24, 64, device=cuda, generator=g).mul(1.5).to(BF)
+    cu = cumulative(cuda, new)
+    out = ops.kv4_attention(q, cache, wide, lengths, cu, max_new=20, max_len=wide.shape[1] * 32)
+    assert ops.device_error() == 0
+    check_attention(q, cache, table, lengths, cu, out)
