@@ -115,8 +115,9 @@ class B200TextDecoder:
         return B200KV4Cache(len(self.layers), self.kv_heads, self.head_dim, seqs, max_tokens, page_size, self.device)
 
     def _rmsnorm(self, x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
+        x = x.contiguous()  # one row stride serves input and output
         out = torch.empty_like(x)
-        seg = _lib.ResLnSegment(x.data_ptr(), None, None, None, None, out.data_ptr(), x.shape[0], x.shape[1], x.stride(0),
+        seg = _lib.ResLnSegment(x.data_ptr(), None, None, None, None, out.data_ptr(), x.shape[0], x.shape[1], x.shape[1],
                                 weight.data_ptr())
         _lib.check(_lib.load().rldx_res_rmsnorm(C.byref(seg), 1, self.eps, C.c_void_p(torch.cuda.current_stream().cuda_stream)))
         return out
