@@ -114,6 +114,15 @@ class B200TextDecoder:
     def new_cache(self, seqs: int, max_tokens: int, page_size: int = 64) -> B200KV4Cache:
         return B200KV4Cache(len(self.layers), self.kv_heads, self.head_dim, seqs, max_tokens, page_size, self.device)
 
+    def _here(self, cache: B200KV4Cache, **tensors: Optional[torch.Tensor]) -> None:
+        """Refuses tensors that are not the decoder's device's, or another current device, to whose stream the launches go."""
+        at = self.embed.device
+        for name, t in dict(tensors, cache=cache.table).items():
+            if t is not None and t.device != at:
+                raise ValueError(f"{name} is on {t.device}, the decoder on {at}")
+        if at.type != "cuda" or at.index != torch.cuda.current_device():
+            raise ValueError(f"the decoder is on {at}, which is not the current CUDA device (no CPU path exists)")
+
     def _rmsnorm(self, x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
         x = x.contiguous()  # one row stride serves input and output
         out = torch.empty_like(x)
@@ -130,6 +139,7 @@ class B200TextDecoder:
         of each sequence's last new token."""
         if hidden.shape != (sum(new), self.hidden) or hidden.dtype != BF:
             raise ValueError(f"hidden must be bfloat16 [{sum(new)}, {self.hidden}], got {hidden.dtype} {tuple(hidden.shape)}")
+        self._here(cache, hidden=hidden)
         start = list(cache.tokens)
         cache.extend(new)
         if positions is None:

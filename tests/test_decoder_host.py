@@ -51,3 +51,33 @@ def test_norm_hands_over_rows_of_one_stride(monkeypatch):
         assert (rows, width, ld) == (5, HIDDEN, HIDDEN) and dst == out.data_ptr()
         assert out.shape == (5, HIDDEN) and out.stride() == (HIDDEN, 1)
         assert (src == x.data_ptr()) == x.is_contiguous()
+
+
+def state(cache):
+    return list(cache.tokens), cache.lengths.tolist(), cache.table.tolist(), cache.free_tokens
+
+
+def refused(dec, cache, error, match, hidden, new, **kw):
+    before = state(cache)
+    with pytest.raises(error, match=match):
+        dec.forward(hidden, cache, new, **kw)
+    assert state(cache) == before
+
+
+def test_other_devices_are_refused(monkeypatch):
+    """On the host, before any launch: a CPU decoder, tensors of another device, another current device."""
+    launches = []
+    monkeypatch.setattr(_lib, "load", lambda: launches.append(1))
+    dec = make()
+    cache = dec.new_cache(1, 64)
+    refused(dec, cache, ValueError, "no CPU path", torch.zeros(3, HIDDEN, dtype=BF), [3])
+    meta = torch.zeros(3, HIDDEN, dtype=BF, device="meta")  # stands for another device
+    refused(dec, cache, ValueError, "hidden is on meta", meta, [3])
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    dec.embed = NS(device=torch.device("cuda", 1))  # a decoder of device 1 while 0 is current
+    on_one = NS(shape=(3, HIDDEN), dtype=BF, device=torch.device("cuda", 1))
+    refused(dec, cache, ValueError, "cache is on cpu", on_one, [3])
+    there = NS(tokens=[0], table=NS(device=torch.device("cuda", 1)))
+    with pytest.raises(ValueError, match="not the current CUDA device"):
+        dec.forward(on_one, there, [3])
+    assert not launches
