@@ -55,13 +55,18 @@ class B200KV4Cache:
     def free_tokens(self) -> int:
         return len(self._free) * self.page_size
 
-    def extend(self, new: Sequence[int]) -> None:
-        """Makes room for new[s] more tokens of each sequence: lengths and pages cover them after."""
+    def room(self, new: Sequence[int]) -> list:
+        """Pages that new[s] more tokens of each sequence need; raises where the cache has not so many."""
         if len(new) != self.seqs or any(n < 0 for n in new):
             raise ValueError(f"new must give a count for each of the {self.seqs} sequences")
         need = [-(-(t + n) // self.page_size) - len(h) for t, n, h in zip(self.tokens, new, self._held)]
         if sum(need) > len(self._free):
             raise RuntimeError(f"the cache has {len(self._free)} free pages, {sum(need)} are needed")
+        return need
+
+    def extend(self, new: Sequence[int]) -> None:
+        """Makes room for new[s] more tokens of each sequence: lengths and pages cover them after."""
+        need = self.room(new)
         seq, col, page = [], [], []
         for s, n in enumerate(need):
             for _ in range(n):
@@ -137,16 +142,24 @@ class B200TextDecoder:
         through the layers; keys and values join the cache.  positions [sum(new)]: RoPE rows, the
         tokens' places in their sequences by default.  Returns logits [seqs with new tokens, vocab]
         of each sequence's last new token."""
+        new = [int(n) for n in new]
         if hidden.shape != (sum(new), self.hidden) or hidden.dtype != BF:
             raise ValueError(f"hidden must be bfloat16 [{sum(new)}, {self.hidden}], got {hidden.dtype} {tuple(hidden.shape)}")
-        self._here(cache, hidden=hidden)
+        if len(new) != len(cache.tokens) or min(new) < 0 or max(new) == 0:
+            raise ValueError(f"new must give a count for each of the {len(cache.tokens)} sequences, one of them positive")
         start = list(cache.tokens)
-        cache.extend(new)
         if positions is None:
-            if max(cache.tokens) > self.cos.shape[0]:
-                raise ValueError(f"a sequence of {max(cache.tokens)} tokens is longer than the RoPE tables ({self.cos.shape[0]})")
+            longest = max(s + n for s, n in zip(start, new))
+            if longest > self.cos.shape[0]:
+                raise ValueError(f"a sequence of {longest} tokens is longer than the RoPE tables ({self.cos.shape[0]})")
             positions = torch.cat([torch.arange(s, s + n, dtype=torch.int32) for s, n in zip(start, new)])
+        elif tuple(positions.shape) != (sum(new),):
+            raise ValueError(f"positions must be [{sum(new)}], got {tuple(positions.shape)}")
+        elif positions.device.type == "cpu" and not 0 <= int(positions.min()) <= int(positions.max()) < self.cos.shape[0]:
+            raise ValueError(f"positions must be rows of the RoPE tables ({self.cos.shape[0]})")  # (else device error 0x501)
+        self._here(cache, hidden=hidden)
         positions = positions.to(self.device, torch.int32)
+        cache.extend(new)  # from here on nothing refuses
         cu = torch.tensor([0, *new], dtype=torch.int32).cumsum(0).to(torch.int32).to(self.device)
         max_new, max_len = max(new), max(cache.tokens)
         h = hidden
@@ -173,6 +186,15 @@ class B200TextDecoder:
         rows = [self.embed[torch.as_tensor(p, device=self.device)] if not torch.is_tensor(p) or p.dim() == 1 else
                 p.to(self.device, BF) for p in prompts]
         cache = cache or self.new_cache(n, sum(r.shape[0] for r in rows) + n * max_new_tokens)
+        if cache.seqs != n:
+            raise ValueError(f"the cache has {cache.seqs} sequences, {n} prompts were given")
+        if min(r.shape[0] for r in rows) == 0:
+            raise ValueError("a prompt has no token")
+        if max_new_tokens > 0:  # what would end the run in its middle: all but the last token drawn are run
+            ends = [t + r.shape[0] + max_new_tokens - 1 for t, r in zip(cache.tokens, rows)]
+            if max(ends) > self.cos.shape[0]:
+                raise ValueError(f"a sequence of {max(ends)} tokens is longer than the RoPE tables ({self.cos.shape[0]})")
+            cache.room([e - t for e, t in zip(ends, cache.tokens)])
         u = u.to(self.device, torch.float32).contiguous()
 
         def full(v, dtype):

@@ -81,3 +81,45 @@ def test_other_devices_are_refused(monkeypatch):
     with pytest.raises(ValueError, match="not the current CUDA device"):
         dec.forward(on_one, there, [3])
     assert not launches
+
+
+def test_a_refused_forward_leaves_the_cache_alone():
+    dec = make()
+    cache = dec.new_cache(2, 256)
+    rows = lambda n: torch.zeros(n, HIDDEN, dtype=BF)  # noqa: E731
+    refused(dec, cache, ValueError, "longer than the RoPE tables", rows(ROWS + 4), [3, ROWS + 1])
+    refused(dec, cache, ValueError, "hidden must be", rows(3).float(), [1, 2])
+    refused(dec, cache, ValueError, "hidden must be", rows(4), [1, 2])
+    refused(dec, cache, ValueError, "count for each", rows(3), [3])
+    refused(dec, cache, ValueError, "count for each", rows(3), [4, -1])
+    refused(dec, cache, ValueError, "one of them positive", rows(0), [0, 0])
+    refused(dec, cache, ValueError, "positions must be", rows(3), [1, 2], positions=torch.zeros(2, dtype=torch.int32))
+    for bad in ([0, 1, ROWS], [-1, 0, 1]):
+        refused(dec, cache, ValueError, "rows of the RoPE tables", rows(3), [1, 2], positions=torch.tensor(bad))
+    cache.extend([30, 0])
+    refused(dec, cache, ValueError, "longer than the RoPE tables", rows(11), [11, 0])
+
+
+def test_generate_refuses_what_it_could_not_finish(monkeypatch):
+    """Before the first step: the tables' length, the cache's pages and its sequences for the whole run."""
+    dec = make()
+    monkeypatch.setattr(dec, "forward", lambda *a, **kw: pytest.fail("a step was run"))
+    cache = dec.new_cache(2, 256, page_size=32)
+    before = state(cache)
+
+    def run(prompts, n, cache=cache):
+        return dec.generate(prompts, n, u=torch.zeros(n, len(prompts)), cache=cache)
+
+    with pytest.raises(ValueError, match="longer than the RoPE tables"):
+        run([[1] * 10, [2] * 5], ROWS - 10 + 2)
+    with pytest.raises(ValueError, match="the cache has 2 sequences"):
+        run([[1]], 3)
+    with pytest.raises(ValueError, match="no token"):
+        run([torch.tensor([1]), torch.zeros(0, dtype=torch.long)], 3)
+    small = dec.new_cache(2, 1, page_size=32)  # three pages
+    with pytest.raises(RuntimeError, match="free pages"):
+        run([[1] * 30, [2] * 30], 10, cache=small)
+    assert state(cache) == before and small.tokens == [0, 0]
+    cache.extend([20, 0])
+    with pytest.raises(ValueError, match="longer than the RoPE tables"):
+        run([[1] * 10, [2] * 5], ROWS - 30 + 2)
