@@ -115,6 +115,9 @@ class B200TextDecoder:
                             down=put(m.mlp.down_proj.weight)) for m in layers]
         self.norm, self.embed, self.lm_head = put(norm.weight), put(embed), put(lm_head)
         self.cos, self.sin = (t.detach().to(self.device).contiguous() for t in (cos, sin))
+        if (cos.dim() != 2 or cos.shape[1] != self.head_dim or sin.shape != cos.shape or sin.dtype != cos.dtype or
+                cos.dtype not in (torch.float32, BF)):
+            raise ValueError(f"cos and sin must be [rows, {self.head_dim}], both float32 or both bfloat16")
 
     def new_cache(self, seqs: int, max_tokens: int, page_size: int = 64) -> B200KV4Cache:
         return B200KV4Cache(len(self.layers), self.kv_heads, self.head_dim, seqs, max_tokens, page_size, self.device)
@@ -157,6 +160,9 @@ class B200TextDecoder:
             raise ValueError(f"positions must be [{sum(new)}], got {tuple(positions.shape)}")
         elif positions.device.type == "cpu" and not 0 <= int(positions.min()) <= int(positions.max()) < self.cos.shape[0]:
             raise ValueError(f"positions must be rows of the RoPE tables ({self.cos.shape[0]})")  # (else device error 0x501)
+        if len(cache.pools) != len(self.layers) or any(p.shape[1] != self.kv_heads or p.shape[3] != 40 * self.head_dim
+                                                       for p in cache.pools):
+            raise ValueError(f"the cache is not one of {len(self.layers)} layers of {self.kv_heads} key / value heads of {self.head_dim}")
         self._here(cache, hidden=hidden)
         positions = positions.to(self.device, torch.int32)
         cache.extend(new)  # from here on nothing refuses

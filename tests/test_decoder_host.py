@@ -77,7 +77,7 @@ def test_other_devices_are_refused(monkeypatch):
     dec.embed = NS(device=torch.device("cuda", 1))  # a decoder of device 1 while 0 is current
     on_one = NS(shape=(3, HIDDEN), dtype=BF, device=torch.device("cuda", 1))
     refused(dec, cache, ValueError, "cache is on cpu", on_one, [3])
-    there = NS(tokens=[0], table=NS(device=torch.device("cuda", 1)))
+    there = NS(tokens=[0], table=NS(device=torch.device("cuda", 1)), pools=cache.pools)
     with pytest.raises(ValueError, match="not the current CUDA device"):
         dec.forward(on_one, there, [3])
     assert not launches
@@ -123,3 +123,17 @@ def test_generate_refuses_what_it_could_not_finish(monkeypatch):
     cache.extend([20, 0])
     with pytest.raises(ValueError, match="longer than the RoPE tables"):
         run([[1] * 10, [2] * 5], ROWS - 30 + 2)
+
+
+def test_other_models_caches_and_tables_are_refused():
+    """A cache of fewer layers would run fewer layers; tables of another width would be refused in mid-step."""
+    dec = make()
+    rows = torch.zeros(2, HIDDEN, dtype=BF)
+    for other in (make([layer()]), make([layer()] * 3)):
+        refused(dec, other.new_cache(1, 64), ValueError, "not one of 2 layers", rows, [2])
+    two = layer(k_proj=weight(2 * HEAD, HIDDEN), v_proj=weight(2 * HEAD, HIDDEN))
+    refused(dec, make([two, two]).new_cache(1, 64), ValueError, "1 key / value heads of 64", rows, [2])
+    for cos, sin in ((torch.zeros(9, 32), torch.zeros(9, 32)), (torch.zeros(9, HEAD), torch.zeros(8, HEAD)),
+                     (torch.zeros(9, HEAD).half(), torch.zeros(9, HEAD).half()), (torch.zeros(9, HEAD), torch.zeros(9, HEAD, dtype=BF))):
+        with pytest.raises(ValueError, match="cos and sin must be"):
+            B200TextDecoder([layer()], weight(HIDDEN), torch.zeros(VOCAB, HIDDEN), torch.zeros(VOCAB, HIDDEN), cos, sin, device="cpu")
