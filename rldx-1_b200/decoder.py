@@ -185,7 +185,9 @@ class B200TextDecoder:
                  temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, stop_ids: Sequence[int] = ()):
         """Appends max_new_tokens tokens to each of the prompts (lists of ids, or rows [n, hidden] of
         embeddings that a vision tower has filled in).  u [max_new_tokens, prompts] are the draws'
-        numbers in [0, 1).  Returns a list of id lists; a sequence ends after one of stop_ids."""
+        numbers in [0, 1).  Returns a list of id lists; a sequence ends after one of stop_ids.  A sequence whose logits
+        have no number to draw from (all NaN or -inf) before its end raises RuntimeError, an error that a kernel
+        has recorded on the device RldxError."""
         n = len(prompts)
         if tuple(u.shape) != (max_new_tokens, n):
             raise ValueError(f"u must be [{max_new_tokens}, {n}], got {tuple(u.shape)}")
@@ -214,10 +216,15 @@ class B200TextDecoder:
             tokens.append(token)
             hidden, new = self.embed[token], [1] * n
         out = torch.stack(tokens, 1).tolist() if tokens else [[] for _ in prompts]
-        for ids in out:
+        code = ops.device_error()
+        if code:
+            raise _lib.RldxError(_lib.RLDX_ERR_DEVICE, f"device error 0x{code:x} recorded while tokens were generated, or left by earlier work")
+        for s, ids in enumerate(out):
             end = next((k for k, t in enumerate(ids) if t in stop_ids), None)
             if end is not None:
                 del ids[end + 1:]
+            if -1 in ids:  # (what was run after it began with the last row of the embedding)
+                raise RuntimeError(f"sequence {s} has no logit that is a number at its token {ids.index(-1)}")
         return out
 
 

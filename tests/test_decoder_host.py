@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import rldx_b200  # noqa: F401
-from rldx_b200 import _lib
+from rldx_b200 import _lib, decoder
 from rldx_b200.decoder import B200TextDecoder
 
 BF = torch.bfloat16
@@ -137,3 +137,31 @@ def test_other_models_caches_and_tables_are_refused():
                      (torch.zeros(9, HEAD).half(), torch.zeros(9, HEAD).half()), (torch.zeros(9, HEAD), torch.zeros(9, HEAD, dtype=BF))):
         with pytest.raises(ValueError, match="cos and sin must be"):
             B200TextDecoder([layer()], weight(HIDDEN), torch.zeros(VOCAB, HIDDEN), torch.zeros(VOCAB, HIDDEN), cos, sin, device="cpu")
+
+
+def scripted(monkeypatch, dec, tokens, code=0):
+    """generate() over drawn tokens given per step, with no device."""
+    steps = iter(tokens)
+    monkeypatch.setattr(dec, "forward", lambda hidden, cache, new, *a, **kw: cache.extend(new))
+    monkeypatch.setattr(decoder.ops, "sample", lambda *a, **kw: (torch.tensor(next(steps)), None, None))
+    monkeypatch.setattr(decoder.ops, "device_error", lambda: code)
+
+
+def test_generate_reports_rows_without_a_token(monkeypatch):
+    dec = make()
+    u = torch.zeros(3, 2)
+    scripted(monkeypatch, dec, [[4, 5], [6, -1], [7, 8]])
+    with pytest.raises(RuntimeError, match="sequence 1 has no logit that is a number at its token 1"):
+        dec.generate([[1], [2, 3]], 3, u=u)
+    scripted(monkeypatch, dec, [[4, 9], [6, -1], [7, 8]])  # past its end: of no interest
+    assert dec.generate([[1], [2, 3]], 3, u=u, stop_ids=[9]) == [[4, 6, 7], [9]]
+
+
+def test_generate_reports_device_errors(monkeypatch):
+    dec = make()
+    scripted(monkeypatch, dec, [[4], [5]], code=0x500)
+    with pytest.raises(_lib.RldxError, match="0x500") as e:
+        dec.generate([[1]], 2, u=torch.zeros(2, 1))
+    assert e.value.code == _lib.RLDX_ERR_DEVICE
+    scripted(monkeypatch, dec, [[4], [5]])
+    assert dec.generate([[1]], 2, u=torch.zeros(2, 1)) == [[4, 5]]
