@@ -90,13 +90,30 @@ class B200KV4Cache:
 
 
 class B200TextDecoder:
-    """Qwen3 decoder layers, embedding and output projection over a B200KV4Cache."""
+    """Qwen3 decoder layers, embedding and output projection over a B200KV4Cache.
+
+    Layers in a LayerWrapper that compresses video tokens (B200LLMChain's compress_info) would have to drop tokens from
+    the cache of the layers after it, which no page table here can say: they are refused unless
+    ignore_compression says that no prompt has what the wrapper compresses (it leaves one frame, and text, as
+    they are)."""
 
     def __init__(self, layers, norm, embed: torch.Tensor, lm_head: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *,
-                 window: int = 0, sinks: int = 0, device=None):
+                 window: int = 0, sinks: int = 0, device=None, ignore_compression: bool = False):
+        layers = list(layers)
+        for i, wrap in enumerate(layers):
+            if _raw_layer(wrap) is not wrap and wrap.layer_idx == wrap.internal_projection and not ignore_compression:
+                raise NotImplementedError(f"layer {i} compresses video tokens, which the decoder does not; ignore_compression=True "
+                                          "where no prompt has more than one frame")
         self.device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
         layers = [_raw_layer(layer) for layer in layers]
         a0 = layers[0].self_attn
+        for m in layers:
+            a = m.self_attn
+            if getattr(a, "q_norm", None) is None or getattr(a, "k_norm", None) is None:
+                raise NotImplementedError("a layer without q_norm and k_norm is not bound")
+            if any(getattr(p, "bias", None) is not None for p in (a.q_proj, a.k_proj, a.v_proj, a.o_proj, m.mlp.gate_proj,
+                                                                  m.mlp.up_proj, m.mlp.down_proj)):
+                raise NotImplementedError("Qwen3 projections have no bias; a biased layer is not bound")
         self.head_dim = a0.q_norm.weight.shape[0]
         self.q_heads = a0.q_proj.weight.shape[0] // self.head_dim
         self.kv_heads = a0.k_proj.weight.shape[0] // self.head_dim

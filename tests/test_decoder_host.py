@@ -165,3 +165,20 @@ def test_generate_reports_device_errors(monkeypatch):
     assert e.value.code == _lib.RLDX_ERR_DEVICE
     scripted(monkeypatch, dec, [[4], [5]])
     assert dec.generate([[1]], 2, u=torch.zeros(2, 1)) == [[4, 5]]
+
+
+def test_layers_that_it_does_not_run_are_refused():
+    """Video-token compression, biases and layers without the per-head norms, each of which was left out without a word."""
+    wrapped = [NS(layer=layer(), internal_projection=1, layer_idx=i) for i in range(3)]
+    with pytest.raises(NotImplementedError, match="layer 1 compresses video tokens"):
+        make(wrapped)
+    assert len(make(wrapped, ignore_compression=True).layers) == 3
+    assert len(make(wrapped[:1]).layers) == 1  # this one's wrapper never compresses
+    with pytest.raises(NotImplementedError, match="bias"):
+        make([layer(), layer(v_proj=weight(HKV * HEAD, HIDDEN, bias=torch.zeros(HEAD)))])
+    biased = layer()
+    biased.mlp.down_proj.bias = torch.zeros(HIDDEN)
+    with pytest.raises(NotImplementedError, match="bias"):
+        make([layer(), biased])
+    with pytest.raises(NotImplementedError, match="q_norm"):
+        make([layer(), layer(k_norm=None)])
