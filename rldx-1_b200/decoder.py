@@ -199,9 +199,13 @@ class B200TextDecoder:
         return ops.linear(self._rmsnorm(h[last].contiguous(), self.norm), self.lm_head)
 
     def generate(self, prompts, max_new_tokens: int, *, u: torch.Tensor, cache: Optional[B200KV4Cache] = None,
-                 temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, stop_ids: Sequence[int] = ()):
+                 temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, stop_ids: Sequence[int] = (),
+                 positions: Optional[Sequence] = None, next_positions: Optional[Sequence[int]] = None):
         """Appends max_new_tokens tokens to each of the prompts (lists of ids, or rows [n, hidden] of
-        embeddings that a vision tower has filled in).  u [max_new_tokens, prompts] are the draws'
+        embeddings that a vision tower has filled in).  positions gives each prompt's RoPE rows [n], of
+        tables whose rows stand for whatever the prompt's tokens have (vision tokens do not count up one by one);
+        the new tokens go on at next_positions, by default one past a prompt's largest.  Without it the rows are
+        the tokens' places in their sequences.  u [max_new_tokens, prompts] are the draws'
         numbers in [0, 1).  Returns a list of id lists; a sequence ends after one of stop_ids.  A sequence whose logits
         have no number to draw from (all NaN or -inf) before its end raises RuntimeError, an error that a kernel
         has recorded on the device RldxError."""
@@ -217,9 +221,24 @@ class B200TextDecoder:
             raise ValueError("a prompt has no token")
         if max_new_tokens > 0:  # what would end the run in its middle: all but the last token drawn are run
             ends = [t + r.shape[0] + max_new_tokens - 1 for t, r in zip(cache.tokens, rows)]
-            if max(ends) > self.cos.shape[0]:
+            if positions is None and max(ends) > self.cos.shape[0]:
                 raise ValueError(f"a sequence of {max(ends)} tokens is longer than the RoPE tables ({self.cos.shape[0]})")
             cache.room([e - t for e, t in zip(ends, cache.tokens)])
+        places = follow = None
+        if positions is not None:
+            given = [torch.as_tensor(p).to("cpu", torch.int32) for p in positions]
+            if [tuple(p.shape) for p in given] != [(r.shape[0],) for r in rows]:
+                raise ValueError(f"positions must give {[r.shape[0] for r in rows]} rows, got {[tuple(p.shape) for p in given]}")
+            places = torch.cat(given)
+            follow = torch.tensor([int(p.max()) + 1 for p in given] if next_positions is None else [int(p) for p in next_positions],
+                                  dtype=torch.int32)
+            if follow.shape != (n,):
+                raise ValueError(f"next_positions must be {n} rows")
+            if not (0 <= int(places.min()) and int(places.max()) < self.cos.shape[0] and
+                    (max_new_tokens <= 1 or (int(follow.min()) >= 0 and int(follow.max()) + max_new_tokens - 2 < self.cos.shape[0]))):
+                raise ValueError(f"the positions of the prompts and the new tokens must be rows of the RoPE tables ({self.cos.shape[0]})")
+        elif next_positions is not None:
+            raise ValueError("next_positions go with positions")
         u = u.to(self.device, torch.float32).contiguous()
 
         def full(v, dtype):
@@ -229,9 +248,9 @@ class B200TextDecoder:
                       top_p=full(top_p, torch.float32), min_p=full(min_p, torch.float32))
         hidden, new, tokens = torch.cat(rows), [r.shape[0] for r in rows], []
         for i in range(max_new_tokens):
-            token, _, _ = ops.sample(self.forward(hidden, cache, new), u[i], **limits)
+            token, _, _ = ops.sample(self.forward(hidden, cache, new, places), u[i], **limits)
             tokens.append(token)
-            hidden, new = self.embed[token], [1] * n
+            hidden, new, places = self.embed[token], [1] * n, None if follow is None else follow + i
         out = torch.stack(tokens, 1).tolist() if tokens else [[] for _ in prompts]
         code = ops.device_error()
         if code:

@@ -182,3 +182,28 @@ def test_layers_that_it_does_not_run_are_refused():
         make([layer(), biased])
     with pytest.raises(NotImplementedError, match="q_norm"):
         make([layer(), layer(k_norm=None)])
+
+
+def test_generate_hands_on_positions(monkeypatch):
+    dec = make()
+    seen = []
+
+    def forward(hidden, cache, new, positions=None):
+        seen.append(None if positions is None else positions.tolist())
+        cache.extend(new)
+
+    monkeypatch.setattr(decoder.ops, "sample", lambda *a, **kw: (torch.tensor([1, 2]), None, None))
+    monkeypatch.setattr(decoder.ops, "device_error", lambda: 0)
+    monkeypatch.setattr(dec, "forward", forward)
+    prompts, u = [[5, 6, 7], torch.zeros(2, HIDDEN)], torch.zeros(3, 2)
+    dec.generate(prompts, 3, u=u)
+    dec.generate(prompts, 3, u=u, positions=[[0, 4, 4], torch.tensor([1, 0])])
+    dec.generate(prompts, 3, u=u, positions=[[0, 4, 4], [1, 0]], next_positions=[ROWS - 2, 9])
+    assert seen == [None] * 3 + [[0, 4, 4, 1, 0], [5, 2], [6, 3]] + [[0, 4, 4, 1, 0], [ROWS - 2, 9], [ROWS - 1, 10]]
+    del seen[:]
+    for kw in (dict(positions=[[0, 1, 2], [0]]), dict(positions=[[0, 1, 2]]), dict(positions=[[0, 1, ROWS], [0, 1]]),
+               dict(positions=[[0, -1, 2], [0, 1]]), dict(positions=[[0, 1, ROWS - 2], [0, 1]]), dict(next_positions=[3, 3]),
+               dict(positions=[[0, 1, 2], [0, 1]], next_positions=[3]), dict(positions=[[0, 1, 2], [0, 1]], next_positions=[3, ROWS - 1])):
+        with pytest.raises(ValueError, match="positions"):
+            dec.generate(prompts, 3, u=u, **kw)
+    assert not seen
