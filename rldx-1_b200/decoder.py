@@ -157,10 +157,13 @@ class B200TextDecoder:
         return out
 
     def forward(self, hidden: torch.Tensor, cache: B200KV4Cache, new: Sequence[int],
-                positions: Optional[torch.Tensor] = None) -> torch.Tensor:
+                positions: Optional[torch.Tensor] = None, deepstack_features: Optional[Sequence[torch.Tensor]] = None,
+                deepstack_rows: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Runs the rows `hidden` [sum(new), hidden] (the new tokens of every sequence, in order)
         through the layers; keys and values join the cache.  positions [sum(new)]: RoPE rows, the
-        tokens' places in their sequences by default.  Returns logits [seqs with new tokens, vocab]
+        tokens' places in their sequences by default.  deepstack_features[i] [n, hidden] are added after
+        layer i to the rows deepstack_rows [n] of hidden (a vision tower's, as B200LLMChain takes them), with one
+        rounding to bf16.  Returns logits [seqs with new tokens, vocab]
         of each sequence's last new token."""
         new = [int(n) for n in new]
         if hidden.shape != (sum(new), self.hidden) or hidden.dtype != BF:
@@ -180,13 +183,26 @@ class B200TextDecoder:
         if len(cache.pools) != len(self.layers) or any(p.shape[1] != self.kv_heads or p.shape[3] != 40 * self.head_dim
                                                        for p in cache.pools):
             raise ValueError(f"the cache is not one of {len(self.layers)} layers of {self.kv_heads} key / value heads of {self.head_dim}")
+        features, at = list(deepstack_features or ()), None
+        if features:
+            if deepstack_rows is None:
+                raise ValueError("deepstack_features need deepstack_rows")
+            at = torch.as_tensor(deepstack_rows).to("cpu", torch.int64)  # (looked at on the host: rows outside would fault)
+            if at.dim() != 1 or at.unique().numel() != at.numel() or (at.numel() and not 0 <= int(at.min()) <= int(at.max()) < sum(new)):
+                raise ValueError(f"deepstack_rows must be different rows of the {sum(new)} of hidden")
+            if len(features) > len(self.layers) or any(tuple(f.shape) != (at.numel(), self.hidden) for f in features):
+                raise ValueError(f"deepstack_features must be at most {len(self.layers)} of [{at.numel()}, {self.hidden}]")
+        elif deepstack_rows is not None:
+            raise ValueError("deepstack_rows go with deepstack_features")
         self._here(cache, hidden=hidden)
+        if features:
+            at, features = at.to(self.device), [f.to(self.device, BF) for f in features]
         positions = positions.to(self.device, torch.int32)
         cache.extend(new)  # from here on nothing refuses
         cu = torch.tensor([0, *new], dtype=torch.int32).cumsum(0).to(torch.int32).to(self.device)
         max_new, max_len = max(new), max(cache.tokens)
         h = hidden
-        for w, pool in zip(self.layers, cache.pools):
+        for i, (w, pool) in enumerate(zip(self.layers, cache.pools)):
             qkv = ops.linear(self._rmsnorm(h, w["norm1"]), w["qkv"])
             q = ops.qkv_rope_append(qkv, w["q_norm"], w["k_norm"], self.cos, self.sin, positions, pool, cache.table,
                                     cache.lengths, cu, q_heads=self.q_heads, eps=self.eps)
@@ -195,17 +211,21 @@ class B200TextDecoder:
             h = ops.linear(a.flatten(1), w["o"], add=h)
             gate, up = ops.linear(self._rmsnorm(h, w["norm2"]), w["gate_up"]).chunk(2, 1)
             h = ops.linear(ops.swiglu(gate, up), w["down"], add=h)
+            if i < len(features):
+                h[at] += features[i]
         last = torch.tensor([e - 1 for n, e in zip(new, torch.tensor(new).cumsum(0).tolist()) if n], device=self.device)
         return ops.linear(self._rmsnorm(h[last].contiguous(), self.norm), self.lm_head)
 
     def generate(self, prompts, max_new_tokens: int, *, u: torch.Tensor, cache: Optional[B200KV4Cache] = None,
                  temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, stop_ids: Sequence[int] = (),
-                 positions: Optional[Sequence] = None, next_positions: Optional[Sequence[int]] = None):
+                 positions: Optional[Sequence] = None, next_positions: Optional[Sequence[int]] = None,
+                 deepstack_features: Optional[Sequence[torch.Tensor]] = None, deepstack_rows: Optional[torch.Tensor] = None):
         """Appends max_new_tokens tokens to each of the prompts (lists of ids, or rows [n, hidden] of
         embeddings that a vision tower has filled in).  positions gives each prompt's RoPE rows [n], of
         tables whose rows stand for whatever the prompt's tokens have (vision tokens do not count up one by one);
         the new tokens go on at next_positions, by default one past a prompt's largest.  Without it the rows are
-        the tokens' places in their sequences.  u [max_new_tokens, prompts] are the draws'
+        the tokens' places in their sequences.  deepstack_features and deepstack_rows are forward()'s, of the
+        prompts' rows one after the other.  u [max_new_tokens, prompts] are the draws'
         numbers in [0, 1).  Returns a list of id lists; a sequence ends after one of stop_ids.  A sequence whose logits
         have no number to draw from (all NaN or -inf) before its end raises RuntimeError, an error that a kernel
         has recorded on the device RldxError."""
@@ -246,10 +266,14 @@ class B200TextDecoder:
 
         limits = dict(temperature=full(temperature, torch.float32), top_k=full(top_k, torch.int32),
                       top_p=full(top_p, torch.float32), min_p=full(min_p, torch.float32))
+        deep = {} if deepstack_features is None else dict(deepstack_features=deepstack_features, deepstack_rows=deepstack_rows)
+        if not deep and deepstack_rows is not None:
+            raise ValueError("deepstack_rows go with deepstack_features")
         hidden, new, tokens = torch.cat(rows), [r.shape[0] for r in rows], []
         for i in range(max_new_tokens):
-            token, _, _ = ops.sample(self.forward(hidden, cache, new, places), u[i], **limits)
+            token, _, _ = ops.sample(self.forward(hidden, cache, new, places, **deep), u[i], **limits)
             tokens.append(token)
+            deep = {}
             hidden, new, places = self.embed[token], [1] * n, None if follow is None else follow + i
         out = torch.stack(tokens, 1).tolist() if tokens else [[] for _ in prompts]
         code = ops.device_error()

@@ -207,3 +207,19 @@ def test_generate_hands_on_positions(monkeypatch):
         with pytest.raises(ValueError, match="positions"):
             dec.generate(prompts, 3, u=u, **kw)
     assert not seen
+
+
+def test_deepstack_that_does_not_fit_is_refused():
+    dec = make()
+    cache, rows = dec.new_cache(2, 256), torch.zeros(5, HIDDEN, dtype=BF)
+    f = torch.zeros(2, HIDDEN)
+    for kw, match in ((dict(deepstack_features=[f]), "need deepstack_rows"), (dict(deepstack_rows=torch.tensor([1, 2])), "go with"),
+                      (dict(deepstack_features=[f], deepstack_rows=torch.tensor([1, 5])), "different rows of the 5"),
+                      (dict(deepstack_features=[f], deepstack_rows=torch.tensor([-1, 2])), "different rows"),
+                      (dict(deepstack_features=[f], deepstack_rows=torch.tensor([2, 2])), "different rows"),
+                      (dict(deepstack_features=[f, f, f], deepstack_rows=torch.tensor([1, 2])), "at most 2"),
+                      (dict(deepstack_features=[f, f[:1]], deepstack_rows=torch.tensor([1, 2])), "at most 2"),
+                      (dict(deepstack_features=[f[:, 1:]], deepstack_rows=torch.tensor([1, 2])), "at most 2")):
+        refused(dec, cache, ValueError, match, rows, [2, 3], **kw)
+    with pytest.raises(ValueError, match="go with"):
+        dec.generate([[1], [2]], 2, u=torch.zeros(2, 2), deepstack_rows=torch.tensor([0]))
