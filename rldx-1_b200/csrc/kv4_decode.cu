@@ -909,8 +909,8 @@ DecodePlan decode_plan(const rldx_kv4_cache& c, int q_heads, int max_new, int ma
   return p;
 }
 
-int plan_of(const rldx_kv4_cache& c, const rldx_kv4_attention_desc& a, int max_len, DecodePlan* plan) {
-  *plan = decode_plan(c, a.q_heads, a.max_new, max_len, a.window, a.sinks);
+int plan_of(const rldx_kv4_cache& c, const rldx_kv4_attention_desc& a, const Kv4AttnParams& p, DecodePlan* plan) {
+  *plan = decode_plan(c, a.q_heads, a.max_new, p.max_len, p.window, p.sinks);
   if (plan->cols > 0 && plan->batch == 0)
     return set_error(RLDX_ERR_UNSUPPORTED, "kv4_attention: max_len and the heads allow for more than 2^30 units of 32 tokens in a sequence");
   return RLDX_OK;
@@ -928,6 +928,9 @@ int attention_args(const rldx_kv4_cache* cache, const rldx_kv4_attention_desc* a
   if (static_cast<long long>(a->tokens) * a->q_heads >= (1LL << 31) || static_cast<long long>(a->max_new) * a->q_heads >= (1LL << 19))
     return set_error(RLDX_ERR_UNSUPPORTED, "kv4_attention: too many rows");
   p->max_len = static_cast<int>(std::min<long long>(a->max_len, static_cast<long long>(cache->table_width) * cache->page_size));
+  // a window that no sequence is longer than hides nothing (and its differences of positions would not fit 32 bits)
+  p->window = a->window < p->max_len ? a->window : 0;
+  p->sinks = p->window > 0 ? a->sinks : 0;
   return RLDX_OK;
 }
 }  // namespace
@@ -945,7 +948,7 @@ int rldx_kv4_attention_workspace_size(const rldx_kv4_cache* cache, const rldx_kv
   int rc = attention_args(cache, a, &p);
   if (rc != RLDX_OK) return rc;
   DecodePlan plan;
-  rc = plan_of(*cache, *a, p.max_len, &plan);
+  rc = plan_of(*cache, *a, p, &plan);
   if (rc == RLDX_OK) *bytes = plan.bytes;
   return rc;
 }
@@ -964,7 +967,7 @@ int rldx_kv4_attention(const rldx_kv4_cache* cache, const rldx_kv4_attention_des
     return set_error(RLDX_ERR_ARG, "kv4_attention: q rows must be 16-byte aligned and hold every head");
   if (a->tokens == 0) return RLDX_OK;
   DecodePlan plan;
-  rc = plan_of(*cache, *a, p.max_len, &plan);
+  rc = plan_of(*cache, *a, p, &plan);
   if (rc != RLDX_OK) return rc;
   if (plan.bytes > workspace_bytes || (plan.bytes > 0 && (!workspace || !aligned_to(workspace, 16))))
     return set_error(RLDX_ERR_ARG, "kv4_attention: needs a 16-byte aligned workspace of " + std::to_string(plan.bytes) + " bytes");
@@ -973,8 +976,6 @@ int rldx_kv4_attention(const rldx_kv4_cache* cache, const rldx_kv4_attention_des
   p.out = static_cast<__nv_bfloat16*>(a->out);
   p.q_heads = a->q_heads;
   p.group = a->q_heads / cache->kv_heads;
-  p.window = a->window;
-  p.sinks = a->window > 0 ? a->sinks : 0;
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.max_new = a->max_new;
   p.whole = plan.whole;

@@ -256,3 +256,20 @@ def test_launches_of_few_sequences_where_lengths_may_be_huge(cuda):
     out = ops.kv4_attention(q, cache, wide, lengths, cu, max_new=20, max_len=wide.shape[1] * 32)
     assert ops.device_error() == 0
     check_attention(q, cache, table, lengths, cu, out)
+
+
+@pytest.mark.parametrize("new,hidden", [(6, 4), (90, 40), (600, 130)])
+@pytest.mark.parametrize("window", [999, 1000, 1001, 2 ** 31 - 1])
+@pytest.mark.parametrize("sinks", [0, 3])
+def test_windows_as_long_as_the_sequence_and_longer(cuda, new, hidden, window, sinks):
+    """Such a window hides nothing, with rows before position 0 too (whose positions less the window pass 32 bits)."""
+    g = torch.Generator(device=cuda).manual_seed(8)
+    cache, table, _ = filled_cache(cuda, [1000], 2, 128, 64, g)
+    lengths = torch.tensor([new - hidden], dtype=I32, device=cuda)
+    q = torch.randn(new, 16, 128, device=cuda, generator=g).to(BF)
+    cu = cumulative(cuda, [new])
+    out = ops.kv4_attention(q, cache, table, lengths, cu, max_new=new, max_len=1000, window=window, sinks=sinks)
+    want = ops.kv4_attention(q, cache, table, lengths, cu, max_new=new, max_len=1000)
+    assert bool((out[:hidden] == 0).all()) and ops.device_error() == 0
+    # 999 still runs as a window, whose units may be split in other places
+    assert torch.equal(out, want) or (window == 999 and (out.float() - want.float()).abs().max() <= 2.0 ** -6)
