@@ -76,7 +76,9 @@ __device__ __forceinline__ int chunk_row(int token) {
   return (o << 3) + 2 * (((token >> 1) - o) & 3) + (token & 1);
 }
 
-// Codes of one word as fp16 pairs: its nibbles 0 4 | 1 5, and with those of word >> 8 also 2 6 | 3 7.
+// Codes of one word as fp16 pairs: its nibbles 0 4 | 1 5, and with those of word >> 8 also 2 6 | 3 7.  A half of exponent
+// 2^10 has a last bit of 1, so a nibble in its low bits makes it 1024 + code, and one four bits further up
+// 1024 + 16 code; the difference, or the difference of a sixteenth and 64, is exact.
 __device__ __forceinline__ void codes_f16_low(uint32_t w, __half2 (&c)[2]) {
   c[0] = __hsub2(bits_h2((w & 0x000f000fu) | 0x64006400u), bits_h2(0x64006400u));                                // 1024
   c[1] = __hfma2(bits_h2((w & 0x00f000f0u) | 0x64006400u), bits_h2(0x2c002c00u), bits_h2(0xd400d400u));  // 1/16, -64

@@ -794,8 +794,11 @@ cudaError_t launch_decode(const Kv4AttnParams& whole, int ctas, int batch, cudaS
     p.c.table += static_cast<long long>(b0) * p.c.table_ld;
     p.edges = (b0 == 0 ? 1 : 0) | (b0 + p.c.seqs >= whole.c.seqs ? 2 : 0);
     p.tiles = (p.max_new * p.group + 8 * NT - 1) / (8 * NT);
-    // a few segments are cut into many parts each: then a CTA of the join per segment and column.  A launch that
-    // cuts nothing has no join and no workspace for its segments' heads, however few sequences the last one holds.
+    // A few segments are cut into many parts each: then a CTA of the join per segment and column, instead of one per
+    // CTA of this launch with a warp per column (us, 592 CTAs, 400000 tokens in 2 / 8 / 16 / 24 / 32 / 48 / 74 segments
+    // of d = 128: 32 / 30 / 30 / 33.0 / 33.6 / 36 / 38 against 67 / 40 / 35 / 33.8 / 33.2 / 33 / 32; 60000 tokens in 2 / 16 / 24 /
+    // 32: 14.5 / 13.1 / 15.3 / 15.9 against 47 / 17 / 15.6 / 14.8).  A launch that cuts nothing has no join and no
+    // workspace for its segments' heads, however few sequences the last one holds.
     p.by_segment = !p.whole && 16LL * p.tiles * p.c.kv_heads * p.c.seqs < ctas;
     cudaError_t e = launch_pdl(kv4_decode_kernel<D, NT, W>, dim3(ctas, 1, 1), 32 * W, DecShape<D, NT, W>::kSmem, stream, p);
     if (e != cudaSuccess) return e;

@@ -901,6 +901,10 @@ extern "C" int rldx_sample(const void* logits, int64_t ld, int rows, int vocab, 
   p.ld = ld;
   p.rows = rows;
   p.vocab = vocab;
+  // As many CTAs a row, up to 8, as leave each 4096 tokens or fewer: right for few rows.  The number of rows does not
+  // count yet, and many rows of a middling vocabulary would be faster with fewer (us, bf16, 1 / 2 / 4 / 8 CTAs a row: 1 row,
+  // top-p 0.9, of 4096 15.4 / 15.4 / 15.5 / 15.9, 16384 23 / 18 / 15.5 / 16.3, 32003 34 / 24 / 18 / 16, 151680 - / - / 42 / 29;
+  // 256 rows of 4096 30 / 20 / 36 / 69, 32003 70 / 53 / 62 / 87, 151680 - / - / 257 / 207).
   p.cluster = 1;
   while (p.cluster < kSampMaxCluster && vocab / p.cluster > 4096) p.cluster *= 2;
   p.u = u;
