@@ -27,7 +27,7 @@
 // and a second kernel joins their parts (the rule and both sides' times: decode_plan).  With more than
 // a wave of tiles each CTA has its own, longest first.
 //
-// Measured: 8 sequences of up to 2300 tokens, up to 1104 of them new, 16 / 2 heads, d = 128: 140 us, 31 % of
+// Measured: 8 sequences of up to 2300 tokens, up to 1104 of them new, 16 / 2 heads, d = 128: 138 us, 32 % of
 // cuBLAS's bf16 rate (44 us).  No role bounds it alone: without three quarters of K's rebuilding, of V's, or
 // without nearly all exponentials it takes 138, 133 and 131 us.  K's tiles of 64 keys give an MMA of N = 64, P takes S's
 // place, and the chain S, softmax, P V of the two query tiles covers each other's waits only in part.

@@ -29,9 +29,9 @@
 // shared memory at a segment's end.  A segment cut between CTAs is joined by a second kernel, in
 // the CTAs' order, so the result does not depend on timing.
 //
-// Measured: 64 sequences of up to 8192 tokens, 16 / 2 heads, d = 128, 120 MB of cache: 31.7 us with the join,
-// 3.77 TB/s, 0.58 of the copy's rate; 3 x 131077 27.4 us, 0.54.  Four warps a CTA and four CTAs an
-// SM, 32 KB of copies in flight a CTA: 33.0 us against 35.7 with eight warps and two CTAs.  What is left is the
+// Measured: 64 sequences of up to 8192 tokens, 16 / 2 heads, d = 128, 120 MB of cache: 32.0 us with the join,
+// 3.73 TB/s, 0.57 of the copy's rate; 3 x 131077 27.7 us, 0.53.  Four warps a CTA and four CTAs an
+// SM, 32 KB of copies in flight a CTA: 33.0 us against 35.7 with eight warps and two CTAs, when both were measured.  What is left is the
 // start (lengths, prefix sums, q: about 3 us before the first unit is used), the shared-memory merge at a
 // segment's end and the join's launch (3.5 us).
 #include <type_traits>
@@ -53,7 +53,7 @@ constexpr int kDecMaxSeqs = 1024;        // sequences of one launch (their prefi
 constexpr long long kDecMaxLine = 1 << 30;  // and units of all their segments (32-bit sums): pages may be shared, so memory sets no bound
 
 // A segment's start counts as this many units of a CTA's share: its lookups, the wait for its first units
-// and the merge of the one before (64 x 8192: 0 / 6 / 12 / 16 / 24 / 36 units 33.0 / 32.0 / 30.9 / 30.9 / 31.5 / 32.6 us).
+// and the merge of the one before (64 x 8192: 0 / 6 / 12 / 16 / 24 / 36 units 34.4 / 33.4 / 32.1 / 32.0 / 32.8 / 33.8 us).
 constexpr int kDecStart = 12;
 
 // What a CTA works on: units [u0, u0 + m) of the n that columns [c0, c0 + ncols) of kv head kvh of a
@@ -854,9 +854,9 @@ struct DecodePlan {
 //   - up to kDecWholeUnits units where segments are many;
 //   - where a wave holds one each, with eight warps to a CTA, as long as a CTA's own time (4.5 us + 0.125 a unit, 0.09
 //     with d = 64) stays below that of the cut (9 us + 0.00073 a unit and segment), or kDecWholeUnitsShared where
-//     two CTAs share an SM.  us whole / cut, d = 128: 2 segments of 23 units 7.7 / 11.1, of 64 12.2 / 8.8; 128 of
-//     64 13.3 / 16.4, of 256 38.0 / 35.7; 192 with d = 64, of 64 13.2 / 15.0, of 128 22.0 / 21.2.  Four warps a
-//     CTA instead of eight: 2 of 23 9.0, of 48 12.9 against 10.2.
+//     two CTAs share an SM.  us whole / cut, d = 128: 2 segments of 23 units 7.5 / 8.3, of 48 10.7 / 9.1, of 64 12.7 /
+//     9.6; 128 of 64 14.3 / 17.9, of 134 24.0 / 25.2, of 256 40.2 / 36.9; 192 with d = 64, of 64 14.1 / 15.9, of 92 18.0 /
+//     18.2, of 128 22.9 / 21.9.  Four warps a CTA instead of eight: 2 of 23 8.7, of 48 13.3.
 constexpr int kDecWholeUnits = 48, kDecWholeUnitsShared = 110;
 bool dec_whole(long long segments, long long units, bool wide, int head_dim) {
   if (!wide) return units <= kDecWholeUnits;
@@ -868,10 +868,10 @@ bool dec_whole(long long segments, long long units, bool wide, int head_dim) {
 // (units + kDecStart), spread evenly whatever the shape; kv4_chunk_kernel takes kChunkUnit (units + 10) for
 // each wave of its CTAs of 256 rows (kChunkUnit2 with more than 128 rows: two query tiles), however few of a
 // wave there are, and with keys shared out kChunkJoin + kChunkJoinTile for each 128 rows of a part.  d = 128, 8
-// kv heads, us here / there with one CTA a tile / with as many as the rule takes: 1 x 8192 tokens, 96 rows 25
-// / 144 / 22, 256 rows 51 / 186 / 28; 8 x 8192, 64 rows 87 / 147 / -, 128 rows 164 / 148 / 98, 256 rows 320 / 191 /
-// 114; 8 x 512, 256 rows 47 / 22 / -, 28 if two shared; 32 x 2048, 32 rows 55 / 90 / -, 64 rows 101 / 90 / -, 256
-// rows 378 / 114 / -.  Up to kDecMaxRows rows it was faster here at every shape.
+// kv heads, us here / there with one CTA a tile / with as many as the rule takes: 1 x 8192 tokens, 96 rows 26
+// / 147 / 22, 256 rows 53 / 180 / 29; 8 x 8192, 64 rows 89 / 150 / -, 128 rows 167 / 151 / 92, 256 rows 326 / 185 /
+// 113; 8 x 512, 256 rows 48 / 22 / -, 28 if two shared; 32 x 2048, 32 rows 57 / 87 / -, 64 rows 103 / 88 / -, 256
+// rows 387 / 114 / -.  Up to kDecMaxRows rows it was faster here at every shape.
 constexpr int kDecMaxRows = 32;
 constexpr long long kDecBase = 5000, kChunkUnit = 500, kChunkUnit2 = 640, kChunkJoin = 2000, kChunkJoinTile = 20;
 constexpr int kChunkShare = 8;  // units of a part at least

@@ -23,9 +23,11 @@
 //
 // Measured, bf16 rows of 151680, 1 row / 256 rows in us: greedy 3.0 / 21 (78 MB: 12 at the copy's rate), top-k 20
 // 7.9 / 43, top-k 1000 15.5 / 77, top-k 3000 (by histogram) 23 / 160, temperature alone 11.4 / 82, top-p 0.9 at
-// T = 1, 28914 kept, 26.3 / 193.  Few rows wait on the chain of passes and cluster barriers; many are bound by
-// instructions, the correctly rounded quotient and exponential of every token that can weigh anything
-// (about 40 a token and pass), and by the histogram's atomics.
+// T = 1, 28914 kept, 26.3 / 193.  Few rows wait on the chain of passes and cluster barriers, and so do
+// many: with mixed filters barriers and the fences beside them lead the stalls (2.7 and 1.1 of an issue's), DRAM is at 11
+// % and the busiest unit of an SM at 36 %.  Rows drawn from the list keep one CTA of a cluster after the gather, so top-k
+// 20 takes twice a greedy row; flat rows add a correctly rounded quotient and exponential a token and pass
+// (about 40 instructions) and the histogram's atomics.
 #include <cfloat>
 
 #include "host_util.h"

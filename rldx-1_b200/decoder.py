@@ -14,7 +14,8 @@ and produces tokens, one path through the decoding operators of `rldx_b200.ops`:
     out = decoder.generate(prompts, 64, cache=cache, u=torch.rand(64, 4), temperature=0.7, top_p=0.9)
 
 `decoder_layers` are Qwen3 text decoder layers (the attribute names that B200LLMChain takes), `cos` and
-`sin` their RoPE tables [positions, head_dim].  `python -m rldx_b200.decoder` decodes with random
+`sin` their RoPE tables [positions, head_dim].  Prompts of a vision tower bring positions and deepstack
+features of their own; everything that cannot be run is refused before the cache changes.  `python -m rldx_b200.decoder` decodes with random
 weights.
 """
 

@@ -376,9 +376,10 @@ def kv4_attention(q, cache, table, lengths, cu_seqlens, *, max_new: int, max_len
     """Softmax attention of the new tokens' queries q [tokens, q_heads, head_dim] (bf16, any token
     stride) over the 4-bit cache, grouped-query heads: the token at position p of its sequence sees
     key j <= p, with window > 0 only j > p - window or j < sinks.  A token that sees no key gives
-    zeros, as does a row of no sequence.  max_new and max_len bound the new tokens and the length of any sequence (a launch is
-    sized by them; the device's values may be smaller, larger ones give zeros and record device error 0x502).
-    scale defaults to head_dim ** -0.5.  Returns [tokens, q_heads, head_dim]."""
+    zeros, as does a row of no sequence.  max_new and max_len bound the new tokens and the length of any
+    sequence (a launch is sized by them; the device's values may be smaller, larger ones give zeros and
+    record device error 0x502).  The result keeps its accuracy whatever the size of k and v.  scale
+    defaults to head_dim ** -0.5.  Returns [tokens, q_heads, head_dim]."""
     return _native().kv4_attention(q, cache, table, lengths, cu_seqlens, max_new, max_len, window, sinks, scale, out)
 
 
