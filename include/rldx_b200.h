@@ -674,6 +674,87 @@ int rldx_llm_status(rldx_llm* h, int wait, unsigned int* code);
  * custom_llm_chain.py:138-147).  Requires deepstack_layers > 0 at create. */
 int rldx_llm_set_deepstack(rldx_llm* h, const void* features, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Around a decoder's products: rotary positions, the norms after and before a block, log
+ * probabilities of given tokens.  Arguments are checked before any device work; everything is
+ * asynchronous on stream, with no workspace.
+ * ------------------------------------------------------------------------------------------ */
+enum { RLDX_BF16 = 0, RLDX_F16 = 1, RLDX_F32 = 2 };
+
+/* Angles: pair i of a token's head is turned by p * freqs[i] radians, p the token's position on
+ * the pair's axis.  axes == 1: positions[token].  Else positions[axis * positions_ld + token], and
+ * sections[axis] pairs belong to an axis: side by side in the order of the axes, or interleaved
+ * (pair i to axis i % axes while i < axes * sections[axis], the others to axis 0).  factor
+ * multiplies cos and sin; inverse turns backwards. */
+typedef struct {
+  const void* positions;  /* int32 or int64 */
+  int64_t positions_ld;   /* elements between axes */
+  const double* freqs;    /* [pairs] device */
+  int positions_int64;
+  int axes;               /* 1..4 */
+  int sections[4];
+  int sections_interleaved;
+  int pairs;              /* turned pairs of a head, at most 512 */
+  int interleaved;        /* 0: pairs (i, i + pairs); 1: (2 i, 2 i + 1) */
+  int inverse;
+  float factor;
+} rldx_rope_plan;
+
+/* heads [tokens, heads, head_dim], strides in elements; out may be in (the same strides) */
+typedef struct {
+  const void* in;
+  void* out;
+  int64_t in_tok, in_head, out_tok, out_head;
+  int heads;
+} rldx_rope_heads;
+
+/* Turns one or two groups of heads (q and k) in one launch: fp32 arithmetic on angles reduced in
+ * double, one rounding; values past 2 * pairs of a head are copied. */
+int rldx_rope(const rldx_rope_plan* plan, const rldx_rope_heads* heads, int nheads, int64_t tokens, int head_dim, int dtype,
+              void* stream);
+/* cos and sin rows [tokens, 2 * pairs] of the plan's angles, pair i at i and i + pairs (the tables
+ * that rldx_kv4_append reads). */
+int rldx_rope_rows(const rldx_rope_plan* plan, int64_t tokens, void* cos, void* sin, int dtype, void* stream);
+
+enum { RLDX_NORM_NONE = 0, RLDX_NORM_RMS = 1, RLDX_NORM_LAYER = 2 };
+
+/* residual_out = residual + scale * gate * post(branch);
+ * out = pre(that sum, before its rounding) * (1 + mod_scale) + mod_shift.
+ * Rows [rows, width]; branch and out of type dtype, the residuals of residual_dtype (dtype or
+ * RLDX_F32), the vectors of vector_dtype (dtype or RLDX_F32).  A null weight is one, a null bias
+ * zero, a null gate one; weight_plus_one: weights are 1 + what is given.  ld_gate / ld_scale /
+ * ld_shift: 0, or elements between the vectors of groups of rows_per_group rows.  pre none: out and
+ * all of pre's null.  residual_out may be residual, out may be branch (the same stride). */
+typedef struct {
+  const void* branch;
+  const void* residual;
+  void* residual_out;
+  void* out;
+  int64_t ld_branch, ld_residual, ld_residual_out, ld_out;
+  const void* post_weight;
+  const void* post_bias;
+  const void* gate;
+  const void* pre_weight;
+  const void* pre_bias;
+  const void* mod_scale;
+  const void* mod_shift;
+  int64_t ld_gate, ld_scale, ld_shift;
+  int64_t rows, rows_per_group;
+  int width, post, pre;
+  int dtype, residual_dtype, vector_dtype;
+  int weight_plus_one;
+  float scale, eps;
+} rldx_block_norms_desc;
+int rldx_block_norms(const rldx_block_norms_desc* d, void* stream);
+
+/* Of rows of logits [rows, vocab] (any row stride): logprob of tokens[row], the entropy of the
+ * row's distribution, the token's rank (tokens of a larger logit, or of an equal one and a lower
+ * id), and the top (0..32) tokens in that order with their log probabilities.  A negative token is none:
+ * logprob 0, rank -1.  One past the vocabulary records device error 0x503: logprob NaN, rank -1.  A
+ * row with a NaN or +inf, or of -inf alone, has no distribution: NaN, ranks and ids -1. */
+int rldx_token_logprobs(const void* logits, int64_t ld, int rows, int vocab, int dtype, const int64_t* tokens, int top,
+                        float* logprob, float* entropy, int32_t* rank, int64_t* top_ids, float* top_logprobs, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

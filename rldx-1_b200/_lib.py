@@ -25,6 +25,8 @@ EPI_STORE, EPI_SWIGLU, EPI_QKV, EPI_EULER = 0, 1, 2, 3
 BIAS_NONE, BIAS_FUSED, BIAS_POST_ROUND = 0, 1, 2
 ACT_NONE, ACT_RELU, ACT_SILU, ACT_SWISH = 0, 1, 2, 3
 ROPE_SA_ONLY, ROPE_VL_SA = 0, 1
+DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 0, 1, 2
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
 
 vp = C.c_void_p
 i64 = C.c_int64
@@ -168,6 +170,27 @@ class Kv4AttentionDesc(C.Structure):
                 ("scale", C.c_float)]
 
 
+class RopePlan(C.Structure):
+    _fields_ = [("positions", vp), ("positions_ld", i64), ("freqs", vp), ("positions_int64", C.c_int), ("axes", C.c_int),
+                ("sections", C.c_int * 4), ("sections_interleaved", C.c_int), ("pairs", C.c_int),
+                ("interleaved", C.c_int), ("inverse", C.c_int), ("factor", C.c_float)]
+
+
+class RopeHeads(C.Structure):
+    _fields_ = [("inp", vp), ("out", vp), ("in_tok", i64), ("in_head", i64), ("out_tok", i64), ("out_head", i64),
+                ("heads", C.c_int)]
+
+
+class BlockNormsDesc(C.Structure):
+    _fields_ = [("branch", vp), ("residual", vp), ("residual_out", vp), ("out", vp), ("ld_branch", i64),
+                ("ld_residual", i64), ("ld_residual_out", i64), ("ld_out", i64), ("post_weight", vp), ("post_bias", vp),
+                ("gate", vp), ("pre_weight", vp), ("pre_bias", vp), ("mod_scale", vp), ("mod_shift", vp),
+                ("ld_gate", i64), ("ld_scale", i64), ("ld_shift", i64), ("rows", i64), ("rows_per_group", i64),
+                ("width", C.c_int), ("post", C.c_int), ("pre", C.c_int), ("dtype", C.c_int),
+                ("residual_dtype", C.c_int), ("vector_dtype", C.c_int), ("weight_plus_one", C.c_int),
+                ("scale", C.c_float), ("eps", C.c_float)]
+
+
 class MsatIO(C.Structure):
     _fields_ = [("vl", vp), ("state", vp), ("emb_id", vp), ("init_noise", vp),
                 ("physics_hist", vp), ("physics_noise", vp), ("actions", vp),
@@ -209,6 +232,10 @@ SIGNATURES = {
                                                     C.POINTER(C.c_uint64)]),
     "rldx_kv4_attention": (C.c_int, [C.POINTER(Kv4Cache), C.POINTER(Kv4AttentionDesc), vp, C.c_uint64, vp]),
     "rldx_sample": (C.c_int, [vp, i64, C.c_int, C.c_int, C.c_int, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
+    "rldx_rope": (C.c_int, [C.POINTER(RopePlan), C.POINTER(RopeHeads), C.c_int, i64, C.c_int, C.c_int, vp]),
+    "rldx_rope_rows": (C.c_int, [C.POINTER(RopePlan), i64, vp, vp, C.c_int, vp]),
+    "rldx_block_norms": (C.c_int, [C.POINTER(BlockNormsDesc), vp]),
+    "rldx_token_logprobs": (C.c_int, [vp, i64, C.c_int, C.c_int, C.c_int, vp, C.c_int, vp, vp, vp, vp, vp, vp]),
     "rldx_swiglu": (C.c_int, [vp, vp, i64, vp, i64, i64, C.c_int, vp]),
     "rldx_msat_create": (C.c_int, [C.POINTER(MsatConfig), C.POINTER(MsatWeights), C.POINTER(vp)]),
     "rldx_msat_destroy": (C.c_int, [vp]),
@@ -273,7 +300,7 @@ def load_binding():
     lib = load()
     mod.bind(RldxError, *(C.cast(getattr(lib, name), C.c_void_p).value for name in (
         "rldx_last_error", "rldx_kv4_append", "rldx_kv4_read", "rldx_kv4_attention_workspace_size", "rldx_kv4_attention",
-        "rldx_sample")))
+        "rldx_sample", "rldx_rope", "rldx_rope_rows", "rldx_block_norms", "rldx_token_logprobs")))
     _BINDING = mod
     return mod
 

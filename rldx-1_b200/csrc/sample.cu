@@ -31,6 +31,7 @@
 #include <cfloat>
 
 #include "host_util.h"
+#include "rows.cuh"
 
 namespace rldx {
 
@@ -84,15 +85,6 @@ struct SampleShared {
   uint32_t flag, count;
   uint64_t loaded;  // the bulk copy
 };
-
-// Order of the logits as whole numbers (-0 counts as 0).
-__device__ __forceinline__ uint32_t order_bits(float x) {
-  const uint32_t b = __float_as_uint(x + 0.0f);
-  return (b >> 31) ? ~b : (b | 0x80000000u);
-}
-__device__ __forceinline__ float order_value(uint32_t k) {
-  return __uint_as_float((k >> 31) ? (k & 0x7fffffffu) : ~k);
-}
 
 __device__ __forceinline__ void st_cluster_u64(uint32_t addr, u64 v) {
   asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");

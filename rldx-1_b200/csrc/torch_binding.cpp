@@ -1,5 +1,6 @@
-// Python binding of the token-decoding operators (ops.qkv_rope_append, kv4_read, kv4_attention, sample):
-// checks the tensors, allocates the results and calls the C ABI on the current stream.
+// Python binding of the token-decoding operators (ops.qkv_rope_append, kv4_read, kv4_attention, sample, rope,
+// rope_rows, block_norms, token_logprobs): checks the tensors, allocates the results and calls the C ABI on the
+// current stream.
 //
 // A decode step makes a few launches of some microseconds per layer, so what the host spends on a call
 // counts: the same steps through ctypes took 14 us a call, of which the launch is 3.  The C ABI's entry
@@ -27,6 +28,10 @@ decltype(&rldx_kv4_read) g_read = nullptr;
 decltype(&rldx_kv4_attention_workspace_size) g_workspace = nullptr;
 decltype(&rldx_kv4_attention) g_attention = nullptr;
 decltype(&rldx_sample) g_sample = nullptr;
+decltype(&rldx_rope) g_rope = nullptr;
+decltype(&rldx_rope_rows) g_rope_rows = nullptr;
+decltype(&rldx_block_norms) g_block_norms = nullptr;
+decltype(&rldx_token_logprobs) g_token_logprobs = nullptr;
 PyObject* g_error = nullptr;
 
 // A refusal: TypeError or ValueError with a message.
@@ -131,6 +136,11 @@ rldx_kv4_cache cache_of(const Device& dev, PyObject* const* a) {  // cache, tabl
 
 int rows_of(int64_t n) {
   if (n > INT32_MAX) refuse_value("more than 2^31 rows");
+  return static_cast<int>(n);
+}
+
+int small_count(int64_t n, const char* name) {
+  if (n > INT32_MAX) refuse_value(std::string(name) + " does not fit 32 bits");
   return static_cast<int>(n);
 }
 
@@ -291,14 +301,308 @@ PyObject* sample(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ---- rotary positions, block norms, log probabilities ----
+// These look at shapes, types and layouts before the device, so a wrong call is refused alike on every machine.
+
+int dtype_of(at::ScalarType t, const char* name) {
+  if (t == at::kBFloat16) return RLDX_BF16;
+  if (t == at::kHalf) return RLDX_F16;
+  if (t == at::kFloat) return RLDX_F32;
+  refuse_type(std::string(name) + " must be bfloat16, float16 or float32");
+}
+
+// Whether a tensor of rows (dimension 0; the others densely or in steps below the rows') is apart from another: no byte
+// of one between the first and last of the other, or both of one row stride and in columns of their own.
+struct Span {
+  uintptr_t first;
+  int64_t rows, stride, width, size;  // elements, and bytes of one
+  explicit Span(const at::Tensor& t) : first(reinterpret_cast<uintptr_t>(t.const_data_ptr())), rows(t.size(0)), stride(t.stride(0)), width(1), size(t.element_size()) {
+    for (int64_t i = 1; i < t.dim(); ++i) width += (t.size(i) - 1) * t.stride(i);
+    if (t.numel() == 0) rows = 0;
+  }
+  uintptr_t end() const { return rows ? first + ((rows - 1) * stride + width) * size : first; }
+  bool apart_from(const Span& o) const {
+    if (!rows || !o.rows || end() <= o.first || o.end() <= first) return true;
+    const int64_t row = stride * size, d = static_cast<int64_t>(o.first - first);
+    if (row <= 0 || row != o.stride * o.size || width * size > row || o.width * o.size > row) return false;
+    const int64_t column = ((d % row) + row) % row;  // where o's rows begin in this one's
+    return column >= width * size && column + o.width * o.size <= row;
+  }
+};
+bool same_place(const at::Tensor& a, const at::Tensor& b) {
+  return a.const_data_ptr() == b.const_data_ptr() && a.scalar_type() == b.scalar_type() && a.sizes() == b.sizes() && a.strides() == b.strides();
+}
+// A written tensor may be one of what is read, place for place, and has to be apart from the rest.
+void writes_apart(const at::Tensor& out, const char* name, const at::Tensor* in, const char* in_name) {
+  if (in && !same_place(out, *in) && !Span(out).apart_from(Span(*in)))
+    refuse_value(std::string(name) + " shares memory with " + in_name + ": it may be the same tensor, or one apart from it");
+}
+
+// positions, freqs, sections, interleaved_sections, interleaved, factor, inverse
+struct RopePlan {
+  const at::Tensor *positions, *freqs;
+  int64_t tokens;
+  rldx_rope_plan p = {};
+  explicit RopePlan(PyObject* const* a) : positions(&tensor(a[0], "positions")), freqs(&tensor(a[1], "freqs")) {
+    if (positions->scalar_type() != at::kInt && positions->scalar_type() != at::kLong) refuse_type("positions must be int32 or int64");
+    if (freqs->scalar_type() != at::kDouble) refuse_type("freqs must be float64");
+    if (freqs->dim() != 1 || freqs->size(0) < 1 || !freqs->is_contiguous()) refuse_value("freqs must be a contiguous tensor [pairs]");
+    if (freqs->size(0) > 512) refuse_value("freqs must be of at most 512 pairs");
+    p.pairs = static_cast<int>(freqs->size(0));
+    p.axes = 1;
+    if (a[2] != Py_None) {
+      PyObject* seq = PySequence_Fast(a[2], "sections must be a sequence of whole numbers");
+      if (!seq) throw Raised{};
+      const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq);
+      long v[4] = {0, 0, 0, 0}, sum = 0;
+      for (Py_ssize_t i = 0; i < n && i < 4; ++i) {
+        v[i] = PyLong_AsLong(PySequence_Fast_GET_ITEM(seq, i));
+        if (v[i] == -1 && PyErr_Occurred()) {
+          Py_DECREF(seq);
+          throw Raised{};
+        }
+      }
+      Py_DECREF(seq);
+      if (n < 1 || n > 4) refuse_value("sections must be of 1 to 4 axes");
+      for (int i = 0; i < n; ++i) {
+        if (v[i] < 0 || v[i] > p.pairs) refuse_value("sections must be counts of pairs");
+        p.sections[i] = static_cast<int>(v[i]);
+        sum += v[i];
+      }
+      if (sum != p.pairs) refuse_value("sections must add up to the " + std::to_string(p.pairs) + " pairs of freqs");
+      p.axes = static_cast<int>(n);
+    }
+    const int64_t dim = positions->dim();
+    if (dim != 1 && dim != 2) refuse_value("positions must be [tokens] or [axes, tokens]");
+    if (dim == 1 ? p.axes != 1 : positions->size(0) != p.axes)
+      refuse_value("positions must have " + std::to_string(p.axes) + " axes, as sections say");
+    tokens = positions->size(dim - 1);
+    if (tokens > 1 && positions->stride(dim - 1) != 1) refuse_value("positions of an axis must lie side by side");
+    p.positions_ld = dim == 2 ? positions->stride(0) : 0;
+    p.positions_int64 = positions->scalar_type() == at::kLong;
+    p.sections_interleaved = truth(a[3]);
+    p.interleaved = truth(a[4]);
+    p.factor = static_cast<float>(number(a[5]));
+    p.inverse = truth(a[6]);
+  }
+  static int truth(PyObject* o) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) throw Raised{};
+    return v;
+  }
+  void at(const Device& dev) {
+    dev.has(*positions), dev.has(*freqs);
+    p.positions = positions->const_data_ptr();
+    p.freqs = static_cast<const double*>(freqs->const_data_ptr());
+  }
+};
+
+// q, k, positions, freqs, sections, interleaved_sections, interleaved, factor, inverse, out_q, out_k
+PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded("rope", n, 11, [&] {
+    static const char* const names[2] = {"q", "k"};
+    static const char* const out_names[2] = {"out_q", "out_k"};
+    const at::Tensor* x[2] = {&tensor(a[0], "q"), optional_tensor(a[1], "k")};
+    const at::Tensor* given[2] = {optional_tensor(a[9], "out_q"), optional_tensor(a[10], "out_k")};
+    RopePlan plan(a + 2);
+    const int dtype = dtype_of(x[0]->scalar_type(), "q");
+    if (given[1] && !x[1]) refuse_value("out_k goes with k");
+    for (int i = 0; i < 2; ++i) {
+      if (!x[i]) continue;
+      const at::Tensor& t = *x[i];
+      if (t.scalar_type() != x[0]->scalar_type()) refuse_type("q and k must have one type");
+      if (t.dim() != 3 || t.size(0) != plan.tokens || t.size(2) != x[0]->size(2) || t.stride(2) != 1)
+        refuse_value(std::string(names[i]) + " must be [" + std::to_string(plan.tokens) + " tokens, heads, head_dim] with a head's values side by side");
+      if (t.size(1) < 1) refuse_value(std::string(names[i]) + " has no heads");
+      if (t.size(2) < 2 * plan.p.pairs)
+        refuse_value("a head of " + std::to_string(t.size(2)) + " values has no " + std::to_string(plan.p.pairs) + " pairs");
+      if (given[i]) {
+        if (given[i]->scalar_type() != t.scalar_type()) refuse_type(std::string(out_names[i]) + " must have q's type");
+        if (given[i]->sizes() != t.sizes() || given[i]->stride(2) != 1)
+          refuse_value(std::string(out_names[i]) + " must have the shape of what it takes, a head's values side by side");
+        writes_apart(*given[i], out_names[i], x[i], names[i]);
+        if (x[1 - i] && !Span(*given[i]).apart_from(Span(*x[1 - i])))
+          refuse_value(std::string(out_names[i]) + " shares memory with " + names[1 - i]);
+      }
+    }
+    if (given[0] && given[1] && !Span(*given[0]).apart_from(Span(*given[1]))) refuse_value("out_q and out_k share memory");
+    const Device dev(*x[0]);
+    dev.has(x[1]), dev.has(given[0]), dev.has(given[1]);
+    plan.at(dev);
+    at::Tensor out[2];
+    rldx_rope_heads h[2];
+    int parts = 0;
+    for (int i = 0; i < 2; ++i) {
+      if (!x[i]) continue;
+      const at::Tensor& t = *x[i];
+      out[i] = given[i] ? *given[i] : dev.empty(t.sizes(), t.scalar_type());
+      if (plan.tokens == 0) continue;
+      const bool one = plan.tokens == 1, single = t.size(1) == 1;
+      h[parts++] = {t.const_data_ptr(), out[i].mutable_data_ptr(), one ? 0 : t.stride(0), single ? 0 : t.stride(1),
+                    one ? 0 : out[i].stride(0), single ? 0 : out[i].stride(1), small_count(t.size(1), "heads")};
+    }
+    if (plan.tokens > 0) check(g_rope(&plan.p, h, parts, plan.tokens, small_count(x[0]->size(2), "head_dim"), dtype, dev.stream()));
+    PyObject* both = PyTuple_New(2);
+    if (!both) throw Raised{};
+    PyTuple_SET_ITEM(both, 0, THPVariable_Wrap(out[0]));
+    if (x[1]) {
+      PyTuple_SET_ITEM(both, 1, THPVariable_Wrap(out[1]));
+    } else {
+      Py_INCREF(Py_None);
+      PyTuple_SET_ITEM(both, 1, Py_None);
+    }
+    return both;
+  });
+}
+
+// positions, freqs, sections, interleaved_sections, factor, inverse, type (RLDX_BF16, ...)
+PyObject* rope_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded("rope_rows", n, 7, [&] {
+    PyObject* const whole[7] = {a[0], a[1], a[2], a[3], Py_False, a[4], a[5]};
+    RopePlan plan(whole);
+    const int dtype = small(a[6], "dtype");
+    const at::ScalarType type = dtype == RLDX_BF16 ? at::kBFloat16 : dtype == RLDX_F16 ? at::kHalf : at::kFloat;
+    const Device dev(*plan.positions);
+    plan.at(dev);
+    const at::Tensor cos = dev.empty({plan.tokens, 2 * plan.p.pairs}, type), sin = dev.empty(cos.sizes(), type);
+    if (plan.tokens > 0) check(g_rope_rows(&plan.p, plan.tokens, cos.mutable_data_ptr(), sin.mutable_data_ptr(), dtype, dev.stream()));
+    PyObject* both = PyTuple_New(2);
+    if (!both) throw Raised{};
+    PyTuple_SET_ITEM(both, 0, THPVariable_Wrap(cos));
+    PyTuple_SET_ITEM(both, 1, THPVariable_Wrap(sin));
+    return both;
+  });
+}
+
+// branch, residual, post, post_weight, post_bias, gate, scale, pre, pre_weight, pre_bias, mod_scale, mod_shift,
+// rows_per_group, weight_plus_one, eps, out_residual, out
+PyObject* block_norms(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded("block_norms", n, 17, [&] {
+    const at::Tensor &y = tensor(a[0], "branch"), &h = tensor(a[1], "residual");
+    rldx_block_norms_desc d = {};
+    d.dtype = dtype_of(y.scalar_type(), "branch");
+    d.residual_dtype = dtype_of(h.scalar_type(), "residual");
+    if (d.residual_dtype != d.dtype && d.residual_dtype != RLDX_F32) refuse_type("residual must have branch's type or float32");
+    if (y.dim() != 2 || (y.size(1) > 1 && y.stride(1) != 1)) refuse_value("branch must be a 2-D row-major view");
+    const int64_t rows = y.size(0), width = y.size(1);
+    if (h.sizes() != y.sizes() || (width > 1 && h.stride(1) != 1)) refuse_value("residual must be a row-major view of branch's shape");
+    if (width < 1 || width > 16384) refuse_value("rows must have 1 to 16384 values");
+    d.post = small(a[2], "post"), d.pre = small(a[7], "pre");
+    d.rows = rows, d.width = static_cast<int>(width);
+    d.rows_per_group = integer(a[12]);
+    if (d.rows_per_group < 0) refuse_value("rows_per_group must not be negative");
+    d.scale = static_cast<float>(number(a[6])), d.eps = static_cast<float>(number(a[14]));
+    d.weight_plus_one = RopePlan::truth(a[13]);
+    const int at[7] = {3, 4, 5, 8, 9, 10, 11};
+    static const char* const names[7] = {"post_weight", "post_bias", "gate", "pre_weight", "pre_bias", "mod_scale", "mod_shift"};
+    const void** to[7] = {&d.post_weight, &d.post_bias, &d.gate, &d.pre_weight, &d.pre_bias, &d.mod_scale, &d.mod_shift};
+    int64_t* ld[7] = {nullptr, nullptr, &d.ld_gate, nullptr, nullptr, &d.ld_scale, &d.ld_shift};
+    const at::Tensor* vec[7];
+    const at::Tensor* first = nullptr;
+    d.vector_dtype = d.dtype;
+    for (int i = 0; i < 7; ++i) {
+      vec[i] = optional_tensor(a[at[i]], names[i]);
+      if (!vec[i]) continue;
+      const at::Tensor& v = *vec[i];
+      const int type = dtype_of(v.scalar_type(), names[i]);
+      if (!first) first = vec[i], d.vector_dtype = type;
+      if (type != d.vector_dtype || (type != d.dtype && type != RLDX_F32))
+        refuse_type("weights, biases, gate and modulation must all have branch's type, or all float32");
+      const bool groups = ld[i] && v.dim() == 2;
+      if (!groups && (v.dim() != 1 || v.size(0) != width || (width > 1 && v.stride(0) != 1)))
+        refuse_value(std::string(names[i]) + " must be a contiguous tensor [" + std::to_string(width) + "]" + (ld[i] ? " or row-major [groups, ...]" : ""));
+      if (groups) {
+        if (v.size(1) != width || (width > 1 && v.stride(1) != 1))
+          refuse_value(std::string(names[i]) + " must be row-major [groups, " + std::to_string(width) + "]");
+        if (d.rows_per_group < 1) refuse_value(std::string(names[i]) + " of groups needs rows_per_group");
+        if (v.size(0) != (rows + d.rows_per_group - 1) / d.rows_per_group)
+          refuse_value(std::string(names[i]) + " must have a row for each group of " + std::to_string(d.rows_per_group) + " rows");
+        *ld[i] = v.size(0) > 1 ? v.stride(0) : 0;
+      }
+    }
+    const at::Tensor *given_h = optional_tensor(a[15], "out_residual"), *given_n = optional_tensor(a[16], "out");
+    if (given_n && d.pre == RLDX_NORM_NONE) refuse_value("without a pre norm there is no out");
+    for (int i = 0; i < 2; ++i) {
+      const at::Tensor* t = i ? given_n : given_h;
+      const char* name = i ? "out" : "out_residual";
+      if (!t) continue;
+      if (t->scalar_type() != (i ? y : h).scalar_type()) refuse_type(std::string(name) + " must have the type of " + (i ? "branch" : "residual"));
+      if (t->sizes() != y.sizes() || (width > 1 && t->stride(1) != 1) || (rows > 1 && t->stride(0) < width))
+        refuse_value(std::string(name) + " must be a row-major view of branch's shape");
+      writes_apart(*t, name, &y, "branch");
+      writes_apart(*t, name, &h, "residual");
+      for (int v = 0; v < 7; ++v)
+        if (vec[v] && !Span(*t).apart_from(Span(vec[v]->dim() == 1 ? vec[v]->unsqueeze(0) : *vec[v]))) refuse_value(std::string(name) + " shares memory with " + names[v]);
+    }
+    if (given_h && given_n && !Span(*given_h).apart_from(Span(*given_n))) refuse_value("out_residual and out share memory");
+    const Device dev(y);
+    dev.has(h), dev.has(given_h), dev.has(given_n);
+    for (int i = 0; i < 7; ++i) {
+      dev.has(vec[i]);
+      if (vec[i]) *to[i] = vec[i]->const_data_ptr();
+    }
+    const at::Tensor h_out = given_h ? *given_h : dev.empty(y.sizes(), h.scalar_type());
+    at::Tensor n_out;
+    if (d.pre != RLDX_NORM_NONE) n_out = given_n ? *given_n : dev.empty(y.sizes(), y.scalar_type());
+    d.branch = y.const_data_ptr(), d.residual = h.const_data_ptr(), d.residual_out = h_out.mutable_data_ptr();
+    if (n_out.defined()) d.out = n_out.mutable_data_ptr();
+    auto stride = [&](const at::Tensor& t) { return rows > 1 ? t.stride(0) : width; };
+    d.ld_branch = stride(y), d.ld_residual = stride(h), d.ld_residual_out = stride(h_out), d.ld_out = n_out.defined() ? stride(n_out) : 0;
+    if (rows > 0) check(g_block_norms(&d, dev.stream()));
+    PyObject* both = PyTuple_New(2);
+    if (!both) throw Raised{};
+    PyTuple_SET_ITEM(both, 0, THPVariable_Wrap(h_out));
+    if (n_out.defined()) {
+      PyTuple_SET_ITEM(both, 1, THPVariable_Wrap(n_out));
+    } else {
+      Py_INCREF(Py_None);
+      PyTuple_SET_ITEM(both, 1, Py_None);
+    }
+    return both;
+  });
+}
+
+// logits, tokens, top
+PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded("token_logprobs", n, 3, [&] {
+    const at::Tensor &logits = tensor(a[0], "logits"), &tokens = tensor(a[1], "tokens");
+    const int dtype = dtype_of(logits.scalar_type(), "logits");
+    if (logits.dim() != 2 || (logits.size(1) > 1 && logits.stride(1) != 1)) refuse_value("logits must be a 2-D row-major view");
+    const int64_t rows = logits.size(0), vocab = logits.size(1);
+    if (vocab < 1) refuse_value("logits have no tokens");
+    vector_of(tokens, "tokens", at::kLong, "int64", rows);
+    const int top = small(a[2], "top");
+    if (top < 0 || top > 32 || top > vocab) refuse_value("top must be 0 to 32, and no more than the tokens");
+    const Device dev(logits);
+    dev.has(tokens);
+    const at::Tensor logprob = dev.empty({rows}, at::kFloat), entropy = dev.empty({rows}, at::kFloat), rank = dev.empty({rows}, at::kInt),
+                     ids = dev.empty({rows, top}, at::kLong), values = dev.empty({rows, top}, at::kFloat);
+    if (rows > 0)
+      check(g_token_logprobs(logits.const_data_ptr(), rows > 1 ? logits.stride(0) : vocab, rows_of(rows), rows_of(vocab), dtype,
+                             static_cast<const int64_t*>(tokens.const_data_ptr()), top, static_cast<float*>(logprob.mutable_data_ptr()),
+                             static_cast<float*>(entropy.mutable_data_ptr()), static_cast<int32_t*>(rank.mutable_data_ptr()),
+                             top ? static_cast<int64_t*>(ids.mutable_data_ptr()) : nullptr,
+                             top ? static_cast<float*>(values.mutable_data_ptr()) : nullptr, dev.stream()));
+    PyObject* all = PyTuple_New(5);
+    if (!all) throw Raised{};
+    PyTuple_SET_ITEM(all, 0, THPVariable_Wrap(logprob));
+    PyTuple_SET_ITEM(all, 1, THPVariable_Wrap(entropy));
+    PyTuple_SET_ITEM(all, 2, THPVariable_Wrap(rank));
+    PyTuple_SET_ITEM(all, 3, THPVariable_Wrap(ids));
+    PyTuple_SET_ITEM(all, 4, THPVariable_Wrap(values));
+    return all;
+  });
+}
+
 // error class, then the addresses of the entry points in the order of the globals above
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 7) {
-    PyErr_SetString(PyExc_TypeError, "bind takes the error class and six addresses");
+  constexpr int kEntries = 10;
+  if (n != 1 + kEntries) {
+    PyErr_SetString(PyExc_TypeError, "bind takes the error class and ten addresses");
     return nullptr;
   }
-  void* p[6];
-  for (int i = 0; i < 6; ++i) {
+  void* p[kEntries];
+  for (int i = 0; i < kEntries; ++i) {
     p[i] = PyLong_AsVoidPtr(a[1 + i]);
     if (!p[i]) {
       if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "bind: a null address");
@@ -311,6 +615,10 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   g_workspace = reinterpret_cast<decltype(g_workspace)>(p[3]);
   g_attention = reinterpret_cast<decltype(g_attention)>(p[4]);
   g_sample = reinterpret_cast<decltype(g_sample)>(p[5]);
+  g_rope = reinterpret_cast<decltype(g_rope)>(p[6]);
+  g_rope_rows = reinterpret_cast<decltype(g_rope_rows)>(p[7]);
+  g_block_norms = reinterpret_cast<decltype(g_block_norms)>(p[8]);
+  g_token_logprobs = reinterpret_cast<decltype(g_token_logprobs)>(p[9]);
   Py_INCREF(a[0]);
   Py_XDECREF(g_error);
   g_error = a[0];
@@ -320,7 +628,9 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
 #define RLDX_METHOD(f) \
   { #f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr }
 PyMethodDef g_methods[] = {RLDX_METHOD(bind),          RLDX_METHOD(qkv_rope_append), RLDX_METHOD(kv4_read),
-                           RLDX_METHOD(kv4_attention), RLDX_METHOD(sample),          {nullptr, nullptr, 0, nullptr}};
+                           RLDX_METHOD(kv4_attention), RLDX_METHOD(sample),          RLDX_METHOD(rope),
+                           RLDX_METHOD(rope_rows),     RLDX_METHOD(block_norms),     RLDX_METHOD(token_logprobs),
+                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_torch_binding", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

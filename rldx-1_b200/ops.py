@@ -394,3 +394,64 @@ def sample(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=None):
     a row's draw is the same in every batch.  Returns token [rows] int64, logprob [rows] fp32 (of the
     kept distribution) and kept [rows] int32, the number of tokens that the filters left."""
     return _native().sample(logits, u, temperature, top_k, top_p, min_p)
+
+
+# ------------------------------------------------------------------------------------------------
+# around a decoder's products: rotary positions, the norms after and before a block, log probabilities
+#
+# Checked, allocated and launched like the decoding operators above.  None has a backward: they serve.
+# ------------------------------------------------------------------------------------------------
+_TYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16, torch.float32: _lib.DTYPE_F32}
+_NORMS = {None: _lib.NORM_NONE, "none": _lib.NORM_NONE, "rms": _lib.NORM_RMS, "layer": _lib.NORM_LAYER}
+
+
+def rope(q, k, positions, freqs, *, sections: Optional[Sequence[int]] = None, interleaved_sections: bool = False,
+         interleaved: bool = False, factor: float = 1.0, inverse: bool = False, out_q=None, out_k=None):
+    """Rotary positions without a table: pair i of every head is turned by positions[token] * freqs[i]
+    radians (freqs float64 [pairs], at most 512; positions int32 or int64 [tokens]) and multiplied by factor.
+    q [tokens, q_heads, head_dim] and k [tokens, kv_heads, head_dim] (or None) are bf16, fp16 or fp32 of any
+    token and head strides.  Pairs are (i, i + pairs), or (2 i, 2 i + 1) with interleaved; values of a head past
+    2 pairs pass unchanged.  sections: positions are [axes, tokens] and sections[a] pairs take those of axis a, side by side, or
+    with interleaved_sections pair i those of axis i % axes while i < axes * sections[i % axes] and of axis 0 from there on.
+    inverse turns backwards.  Angles are reduced in double, the rest is fp32 with one rounding.  out_q and
+    out_k may be q and k themselves.  Returns (q, k) rotated."""
+    return _native().rope(q, k, positions, freqs, sections, interleaved_sections, interleaved, factor, inverse, out_q, out_k)
+
+
+def rope_rows(positions, freqs, *, sections: Optional[Sequence[int]] = None, interleaved_sections: bool = False,
+              factor: float = 1.0, inverse: bool = False, dtype=torch.float32):
+    """cos and sin rows [tokens, 2 pairs] of the angles that rope() turns by, each value at i and i + pairs: the
+    tables that qkv_rope_append reads, made for the tokens at hand (rope_pos counts them)."""
+    if dtype not in _TYPES:
+        raise TypeError(f"dtype must be bfloat16, float16 or float32, got {dtype}")
+    return _native().rope_rows(positions, freqs, sections, interleaved_sections, factor, inverse, _TYPES[dtype])
+
+
+def block_norms(branch, residual, *, post: Optional[str] = None, post_weight=None, post_bias=None, gate=None, scale: float = 1.0,
+                pre: Optional[str] = "rms", pre_weight=None, pre_bias=None, mod_scale=None, mod_shift=None, rows_per_group: int = 0,
+                weight_plus_one: bool = False, eps: float = 1e-6, out_residual=None, out=None):
+    """What stands between two blocks, in one pass over rows [rows, width] (width at most 16384):
+
+        residual' = residual + scale * gate * post(branch)
+        out       = pre(residual', unrounded) * (1 + mod_scale) + mod_shift
+
+    post and pre are "rms", "layer" or None ("none").  branch is bf16, fp16 or fp32, residual of that type or fp32; the weights,
+    biases, gate and modulation are all of branch's type or all fp32.  gate, mod_scale and mod_shift are [width], or
+    [groups, width] with row r taking row r // rows_per_group.  weight_plus_one: weights are given as w - 1.  fp32 inside,
+    one rounding a result.  out_residual and out may be residual and branch themselves.  Returns (residual', out); out is None
+    without a pre norm."""
+    if post not in _NORMS or pre not in _NORMS:
+        raise ValueError(f"post and pre must be 'rms', 'layer' or None, got {post!r} and {pre!r}")
+    return _native().block_norms(branch, residual, _NORMS[post], post_weight, post_bias, gate, scale, _NORMS[pre], pre_weight, pre_bias,
+                                 mod_scale, mod_shift, rows_per_group, weight_plus_one, eps, out_residual, out)
+
+
+def token_logprobs(logits, tokens, *, top: int = 0):
+    """Of each row of logits [rows, vocab] (bf16, fp16 or fp32, any row stride), with one read of it: the log probability of
+    tokens[row] (int64), the entropy, the token's rank (how many tokens have a larger logit, or an equal one and a
+    lower id), and the top (at most 32) tokens in that order with their log probabilities.  A negative token is
+    none: logprob 0, rank -1.  A token past the vocabulary records device error 0x503 and gives NaN and -1.  A row that holds NaN or
+    +inf, or nothing but -inf, has no distribution: NaN, rank and ids -1.  Sums are fp32: logprob and entropy are good to a few
+    2^-24 of 1 + their size.  Returns logprob, entropy [rows] fp32, rank [rows] int32, top_ids
+    [rows, top] int64, top_logprobs [rows, top] fp32."""
+    return _native().token_logprobs(logits, tokens, top)
