@@ -7,22 +7,27 @@
 // Everything is fp32 until the two results are rounded, once each; pre takes the sum before its rounding.  The
 // variance is the mean square of what the mean leaves, from registers.
 //
-// A row lies in the registers of a team: 4 to 32 lanes, or as many warps as 16 values a thread ask for.  Bound by memory: y
-// and h are read and h' and n written once; the vectors come from the caches.
+// A row lies in the registers of a team: 4 to 32 lanes, or a few warps, of 16 or 32 values a thread.  The vectors come down
+// to four numbers a value, h' = h + (a y^ + b) and n = c h^ + d with a = scale gate (w + 1), b = scale gate b, c = (w + 1)
+// (1 + mod_scale), d = b (1 + mod_scale) + mod_shift, kept in shared memory: made once by a CTA where all rows share them,
+// else by each team whenever it comes to another group.  A CTA goes over a run of rows, the next of which is on the way
+// while one is normed.  Bound by memory: y and h are read and h' and n written once.
 #include "host_util.h"
 #include "rows.cuh"
 
 namespace rldx {
 
 namespace {
-constexpr int kNormValues = 16;  // of a thread
-constexpr int kNormMaxWidth = 1024 * kNormValues;
+constexpr int kNormMaxWidth = 14336;  // four vectors of it fill the shared memory
+constexpr int kNormBlock = 256;             // threads, of one row or several
+constexpr int kNormShared = 4 * 4 * kNormMaxWidth;
+enum { kNormA = 0, kNormB = 1, kNormC = 2, kNormD = 3 };
 
 struct NormsParams {
   const void* y;
   const void* h;
   void* h_out;
-  void* n_out;  // null: pre is none
+  void* n_out;
   long long ld_y, ld_h, ld_h_out, ld_n;
   const void* post_w;
   const void* post_b;
@@ -31,187 +36,321 @@ struct NormsParams {
   const void* pre_b;
   const void* mod_scale;
   const void* mod_shift;
-  long long ld_gate, ld_scale, ld_shift;  // of the groups' vectors; 0: one for all rows
+  long long ld_gate, ld_scale, ld_shift;  // of the groups' vectors
   long long rows, group;
-  int width, post, pre;      // RLDX_NORM_*
-  int vectors_f32, aligned;  // the vectors' type; V of them may be loaded at once
-  int team, warps;           // lanes of a row (4 to 32), warps of a row
+  int run;                 // rows of a team
+  int width, post, pre;    // RLDX_NORM_*
+  int place[4];            // of a, b, c, d in shared memory (values); -1: a is scale, c one, b and d zero
+  int copy;                // and of a team's own copy of them; 0: one for all
+  int padded;              // values of one of them there
+  int vectors_f32, aligned;  // the vectors' type; four of them may be loaded at once
+  int team, warps;         // lanes of a row (4 to 32), warps of a row
   float scale, eps, plus_one;
 };
 
-template <int V>
-__device__ __forceinline__ void each(float (&x)[V], float v) {
+// Values e .. e + V of a vector (of fp32 or the rows' type) that begins `from` values past base; what is past the width stays.
+template <typename T, int V>
+__device__ __forceinline__ void vector_at(const NormsParams& P, const void* base, long long from, int e, float (&x)[V]) {
+  auto read = [&](auto* p) {
+    using S = std::remove_cv_t<std::remove_reference_t<decltype(*p)>>;
+    p += from + e;
+    if (P.aligned && e + V <= P.width)
+      unpack_row<S, V>(load_shared_by_rows<S, V>(p), x);
+    else
 #pragma unroll
-  for (int i = 0; i < V; ++i) x[i] = v;
+      for (int i = 0; i < V; ++i)
+        if (e + i < P.width) x[i] = to_float(__ldg(p + i));
+  };
+  if (P.vectors_f32)
+    read(static_cast<const float*>(base));
+  else
+    read(static_cast<const T*>(base));
 }
 
-// Values e .. e + V of a vector (of fp32 or the rows' type), `n` of them there.
-template <typename T, int V>
-__device__ __forceinline__ void vector_at(const NormsParams& P, const void* base, long long e, int n, float (&x)[V]) {
-  if (P.vectors_f32) {
-    const float* p = static_cast<const float*>(base) + e;
-    if (P.aligned && n >= V)
-      unpack_row<float, V>(load_shared_by_rows<float, V>(p), x);
-    else
+// kWhole: a vector of V values is there whole or not at all.
+template <typename T, int V, bool kWhole>
+__device__ __forceinline__ Raw<T, V> row_at(const T* p, int n) {
+  Raw<T, V> r = {};
+  if (kWhole ? n > 0 : n >= V) {
+    r = load_once<T, V>(p);
+  } else if constexpr (!kWhole) {
+    T* e = reinterpret_cast<T*>(&r);
 #pragma unroll
-      for (int i = 0; i < V; ++i) x[i] = i < n ? __ldg(p + i) : 0.0f;
-  } else {
-    const T* p = static_cast<const T*>(base) + e;
-    if (P.aligned && n >= V)
-      unpack_row<T, V>(load_shared_by_rows<T, V>(p), x);
-    else
-#pragma unroll
-      for (int i = 0; i < V; ++i) x[i] = i < n ? to_float(__ldg(p + i)) : 0.0f;
+    for (int i = 0; i < V; ++i)
+      if (i < n) e[i] = p[i];
   }
+  return r;
 }
-
-template <typename T, int V>
-__device__ __forceinline__ void row_at(const T* p, int n, float (&x)[V]) {
-  if (n >= V)
-    unpack_row<T, V>(load_once<T, V>(p), x);
-  else
-#pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = i < n ? to_float(p[i]) : 0.0f;
-}
-template <typename T, int V>
+template <typename T, int V, bool kWhole>
 __device__ __forceinline__ void row_to(T* p, int n, const float (&x)[V]) {
-  if (n >= V)
+  if (kWhole ? n > 0 : n >= V) {
     store_once<T, V>(p, pack_row<T, V>(x));
-  else
+  } else if constexpr (!kWhole) {
 #pragma unroll
     for (int i = 0; i < V; ++i)
       if (i < n) p[i] = from_float<T>(x[i]);
+  }
 }
 
-// Sum over a row's team.  Of several warps: each leaves its sum, and all read them after a barrier; two sets of
-// places take turns, so one barrier a sum is enough.
+// Sum over a row's team.  Several warps are all of the CTA: each leaves its sum, and all read them after a barrier; two
+// sets of places take turns, so one barrier a sum is enough.
+template <int kWarps>
 struct TeamSum {
-  float* places;  // [2][warps of the row]
-  int team, warps, warp, barrier, turn;
+  float* places;  // [2][kWarps], zeros past the row's warps
+  int team, warps;
+  int turn = 0;
   __device__ __forceinline__ float operator()(float x) {
-    for (int o = team >> 1; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+      if (o < team) x += __shfl_xor_sync(0xffffffffu, x, o);
     if (warps == 1) return x;
-    float* p = places + turn * warps;
-    turn ^= 1;
-    if ((threadIdx.x & 31) == 0) p[warp] = x;
-    named_bar_sync(barrier, 32 * warps);
-    x = 0.0f;
-    for (int w = 0; w < warps; ++w) x += p[w];
+    float* p = places + turn;
+    turn ^= kWarps;
+    if ((threadIdx.x & 31) == 0) p[threadIdx.x >> 5] = x;
+    __syncthreads();
+    x = p[threadIdx.x & (kWarps - 1)];
+#pragma unroll
+    for (int o = kWarps / 2; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
     return x;
   }
 };
 
-template <typename TY, typename TH, int V>
-__global__ void __launch_bounds__(1024) block_norms_kernel(const __grid_constant__ NormsParams P) {
-  constexpr int K = kNormValues / V;  // vectors of a thread
-  __shared__ float places[2 * 32];
+// Threads that run on an SM at once, from their registers: 80 with vectors of eight and 16 values, 128 else.
+template <typename TY, int V, int E, bool kWhole>
+constexpr int kNormResident = sizeof(TY) == 2 && V == 8 && E == 16 && kWhole ? 768 : 512;
+
+// E values a thread, V at a time.
+template <typename TY, typename TH, int V, int E, bool kWhole, int kThreads>
+__global__ void __launch_bounds__(kThreads, kNormResident<TY, V, E, kWhole> / kThreads) block_norms_kernel(const __grid_constant__ NormsParams P) {
+  constexpr int K = E / V;
+  constexpr int kWarps = kThreads / 32;
+  extern __shared__ __align__(16) float shared[];  // a, b, c, d
+  __shared__ float places[2 * kWarps];
   griddep_wait();
   griddep_launch();
   const int threads = P.warps > 1 ? 32 * P.warps : P.team;  // of a row
-  const int slot = threadIdx.x / threads, at = threadIdx.x - slot * threads;
-  const long long row = static_cast<long long>(blockIdx.x) * (blockDim.x / threads) + slot;
-  const bool real = row < P.rows;
-  TeamSum sum{places + 2 * slot * (P.warps > 1 ? P.warps : 0), P.team, P.warps, at >> 5, 1 + slot, 0};
-  const int D = P.width;
-  const float inv_d = 1.0f / static_cast<float>(D), root_inv_d = rsqrtf(static_cast<float>(D));
-  auto left = [&](int k) { return real ? D - (at + k * threads) * V : 0; };  // values there, V at most
-  auto first = [&](int k) { return (at + k * threads) * V; };
-  float x[K][V], h[K][V];
-  const TY* y = static_cast<const TY*>(P.y) + row * P.ld_y;
-  const TH* hin = static_cast<const TH*>(P.h) + row * P.ld_h;
-#pragma unroll
-  for (int k = 0; k < K; ++k) row_at<TY, V>(y + first(k), left(k), x[k]);
-#pragma unroll
-  for (int k = 0; k < K; ++k) row_at<TH, V>(hin + first(k), left(k), h[k]);
+  const int teams = blockDim.x / threads, slot = threadIdx.x / threads, at = threadIdx.x - slot * threads;
+  if (threadIdx.x < 2 * kWarps) places[threadIdx.x] = 0.0f;
+  TeamSum<kWarps> sum{places, P.team, P.warps};
+  long long row = static_cast<long long>(blockIdx.x) * teams * P.run + slot;
+  const long long row_end = min(P.rows, row - slot + teams * P.run);
+  // Vector k begins at value at V + k step; n(k) values are there, V or more of a whole one.
+  const int step = threads * V, first = at * V, width = P.width;
+  auto n = [&](int k) { return width - first - k * step; };
+  const float inv_d = 1.0f / static_cast<float>(width), root_inv_d = rsqrtf(static_cast<float>(width));
 
-  // mean (of a LayerNorm) and 1 / sqrt of the mean square of what it leaves
-  auto statistics = [&](int kind, float& mean, float& inv) {
-    mean = 0.0f;
-    if (kind == RLDX_NORM_LAYER) {
+  const TY* y_at = static_cast<const TY*>(P.y) + row * P.ld_y + first;
+  const TH* h_at = static_cast<const TH*>(P.h) + row * P.ld_h + first;
+  TH* h_to = static_cast<TH*>(P.h_out) + row * P.ld_h_out + first;
+  TY* n_to = static_cast<TY*>(P.n_out) + row * P.ld_n + first;
+  Raw<TY, V> y[K];
+  Raw<TH, V> h[K];
+  auto load_y = [&](bool real) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) y[k] = row_at<TY, V, kWhole>(y_at + k * step, real ? n(k) : 0);
+    y_at += teams * P.ld_y;
+  };
+  auto load_h = [&](bool real) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) h[k] = row_at<TH, V, kWhole>(h_at + k * step, real ? n(k) : 0);
+    h_at += teams * P.ld_h;
+  };
+  load_y(row < row_end);
+  load_h(row < row_end);
+  // a, b, c, d of group g, by `by` threads of which this is the `me`-th, four values at a time; threads of eight values
+  // read theirs in two halves, each side by side with the other threads' (half: where the second ones begin)
+  float* const mine = shared + slot * P.copy;
+  const int half = V == 8 ? P.padded / 2 : 0;
+  auto make_vectors = [&](long long g, int me, int by) {
+#pragma unroll 2
+    for (int e = 4 * me; e < P.padded; e += 4 * by) {
+      auto values = [&](const void* base, long long ld, float otherwise, float (&v)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = otherwise;
+        if (base) vector_at<TY, 4>(P, base, g * ld, e, v);
+      };
+      const int to = V == 8 ? (e >> 1 & ~3) + (e & 4 ? half : 0) : e;
+      auto put = [&](int which, const float (&v)[4]) {
+        *reinterpret_cast<float4*>(mine + P.place[which] + to) = make_float4(v[0], v[1], v[2], v[3]);
+      };
+      float v[4], w[4];
+      if (P.place[kNormA] >= 0 || P.place[kNormB] >= 0) {
+        float gate[4];
+        values(P.gate, P.ld_gate, 1.0f, gate);
+        values(P.post_w, 0, 1.0f - P.plus_one, v);
+        values(P.post_b, 0, 0.0f, w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) gate[i] *= P.scale, v[i] = gate[i] * (v[i] + P.plus_one), w[i] *= gate[i];
+        if (P.place[kNormA] >= 0) put(kNormA, v);
+        if (P.place[kNormB] >= 0) put(kNormB, w);
+      }
+      if (P.place[kNormC] >= 0 || P.place[kNormD] >= 0) {
+        float scale[4], shift[4];
+        values(P.mod_scale, P.ld_scale, 0.0f, scale);
+        values(P.mod_shift, P.ld_shift, 0.0f, shift);
+        values(P.pre_w, 0, 1.0f - P.plus_one, v);
+        values(P.pre_b, 0, 0.0f, w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] += P.plus_one, v[i] = fmaf(v[i], scale[i], v[i]), w[i] = fmaf(w[i], scale[i], w[i]) + shift[i];
+        if (P.place[kNormC] >= 0) put(kNormC, v);
+        if (P.place[kNormD] >= 0) put(kNormD, w);
+      }
+    }
+  };
+  const bool grouped = P.copy > 0;
+  long long group_end = 0;
+  if (grouped) {
+    const long long g = min(row, P.rows - 1) / P.group;
+    group_end = (g + 1) * P.group;
+    make_vectors(g, at, threads);
+  } else {
+    make_vectors(0, threadIdx.x, blockDim.x);
+  }
+  __syncthreads();
+
+#pragma unroll 1
+  for (int left = P.run; left > 0; --left) {  // (the same count for every team: lanes of a warp stay together)
+    asm volatile("" ::: "memory");  // (a to d are read anew for each row: kept in registers they would take most of them)
+    const bool real = row < row_end, more = left > 1 && row + teams < row_end;
+    float x[K][V];
+#pragma unroll
+    for (int k = 0; k < K; ++k) unpack_row<TY, V>(y[k], x[k]);
+    load_y(more);
+
+    // What is not there counts as v.
+    auto fill = [&](float v) {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        if (n(k) < V)
+#pragma unroll
+          for (int i = 0; i < V; ++i) x[k][i] = !kWhole && i < n(k) ? x[k][i] : v;
+    };
+    // 1 / sqrt of the mean square of x, centred first for a LayerNorm (x is zero where nothing is)
+    auto inverse_size = [&](int kind) {
+      if (kind == RLDX_NORM_LAYER) {
+        float s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int i = 0; i < V; ++i) s += x[k][i];
+        const float mean = sum(s) * inv_d;
+        fill(mean);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int i = 0; i < V; ++i) x[k][i] -= mean;
+      }
       float s = 0.0f;
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < V; ++i) s += x[k][i];  // (zeros where there is nothing)
-      mean = sum(s) * inv_d;
-    }
-    float s = 0.0f;
+        for (int i = 0; i < V; ++i) {
+          const float v = x[k][i] * root_inv_d;  // (a mean, not a sum, of squares stays in range up to 1.8e19)
+          s = fmaf(v, v, s);
+        }
+      return rsqrtf(sum(s) + P.eps);
+    };
+    // f(x, number) with those of a vector in shared memory
+    auto with = [&](int which, auto f) {
+      const int place = P.place[which];
+      if (place < 0) return;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        float v[V];
+        const float* from = mine + place + (V == 8 ? (first + k * step) / 2 : first + k * step);
+        if constexpr (V % 4 == 0) {
+#pragma unroll
+          for (int i = 0; i < V; i += 4) *reinterpret_cast<float4*>(v + i) = *reinterpret_cast<const float4*>(from + (i ? half : 0));
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; ++i) v[i] = from[i];
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[k][i] = f(x[k][i], v[i]);
+      }
+    };
+    auto times = [](float a, float b) { return a * b; };
+    auto plus = [](float a, float b) { return a + b; };
+
+    const float post = P.post != RLDX_NORM_NONE ? inverse_size(P.post) : 1.0f;
+    const float size = P.place[kNormA] < 0 ? P.scale * post : post;
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float d = (x[k][i] - mean) * root_inv_d;  // (a mean, not a sum, of squares stays in range up to 1.8e19)
-        s += i < left(k) ? d * d : 0.0f;
-      }
-    inv = rsqrtf(sum(s) + P.eps);
-  };
-  auto normed = [&](const void* w, const void* b, float mean, float inv) {
+      for (int i = 0; i < V; ++i) x[k][i] *= size;
+    with(kNormA, times);
+    with(kNormB, plus);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      if (left(k) <= 0) continue;
-      float wv[V], bv[V];
-      each(wv, 1.0f), each(bv, 0.0f);
-      if (w) {
-        vector_at<TY, V>(P, w, first(k), left(k), wv);
+      float r[V];
+      unpack_row<TH, V>(h[k], r);
 #pragma unroll
-        for (int i = 0; i < V; ++i) wv[i] += P.plus_one;
+      for (int i = 0; i < V; ++i) x[k][i] += r[i];
+      row_to<TH, V, kWhole>(h_to + k * step, real ? n(k) : 0, x[k]);
+    }
+    load_h(more);
+    if (P.pre != RLDX_NORM_NONE) {  // (the same for every thread)
+      fill(0.0f);
+      const float pre = inverse_size(P.pre);
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[k][i] *= pre;
+      with(kNormC, times);
+      with(kNormD, plus);
+#pragma unroll
+      for (int k = 0; k < K; ++k) row_to<TY, V, kWhole>(n_to + k * step, real ? n(k) : 0, x[k]);
+      n_to += teams * P.ld_n;
+    }
+    h_to += teams * P.ld_h_out;
+    row += teams;
+    const bool next_group = grouped && row >= group_end && left > 1 && row < row_end;
+    if (__any_sync(0xffffffffu, next_group)) {  // (several warps are one team, and agree)
+      const auto wait = [&] {
+        if (P.warps > 1)
+          __syncthreads();
+        else
+          __syncwarp();
+      };
+      wait();  // the last row's numbers have been read
+      if (next_group) {
+        const long long g = min(row, P.rows - 1) / P.group;
+        group_end = (g + 1) * P.group;
+        make_vectors(g, at, threads);
       }
-      if (b) vector_at<TY, V>(P, b, first(k), left(k), bv);
-#pragma unroll
-      for (int i = 0; i < V; ++i) x[k][i] = fmaf((x[k][i] - mean) * inv, wv[i], bv[i]);
+      wait();
     }
-  };
-
-  float mean, inv;
-  if (P.post != RLDX_NORM_NONE) {
-    statistics(P.post, mean, inv);
-    normed(P.post_w, P.post_b, mean, inv);
-  }
-  const long long g = real && P.group > 0 ? row / P.group : 0;
-  TH* hout = static_cast<TH*>(P.h_out) + row * P.ld_h_out;
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    if (left(k) > 0) {
-      float gv[V];
-      each(gv, 1.0f);
-      if (P.gate) vector_at<TY, V>(P, P.gate, g * P.ld_gate + first(k), left(k), gv);
-#pragma unroll
-      for (int i = 0; i < V; ++i) x[k][i] = i < left(k) ? fmaf(P.scale * gv[i], x[k][i], h[k][i]) : 0.0f;
-      row_to<TH, V>(hout + first(k), left(k), x[k]);
-    }
-  }
-  if (P.pre == RLDX_NORM_NONE) return;  // (the same for every thread)
-  statistics(P.pre, mean, inv);
-  normed(P.pre_w, P.pre_b, mean, inv);
-  TY* nout = static_cast<TY*>(P.n_out) + row * P.ld_n;
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    if (left(k) <= 0) continue;
-    if (P.mod_scale) {
-      float sv[V];
-      vector_at<TY, V>(P, P.mod_scale, g * P.ld_scale + first(k), left(k), sv);
-#pragma unroll
-      for (int i = 0; i < V; ++i) x[k][i] = fmaf(x[k][i], sv[i], x[k][i]);
-    }
-    if (P.mod_shift) {
-      float sv[V];
-      vector_at<TY, V>(P, P.mod_shift, g * P.ld_shift + first(k), left(k), sv);
-#pragma unroll
-      for (int i = 0; i < V; ++i) x[k][i] += sv[i];
-    }
-    row_to<TY, V>(nout + first(k), left(k), x[k]);
   }
 }
 
-template <typename TY, typename TH>
-cudaError_t launch_block_norms(const NormsParams& p, int v, unsigned grid, unsigned block, cudaStream_t stream) {
-  if constexpr (sizeof(TY) == 2)
-    if (v == 8) return launch_overlapped(block_norms_kernel<TY, TH, 8>, grid, block, 0, stream, p);
-  switch (v) {
-    case 4: return launch_overlapped(block_norms_kernel<TY, TH, 4>, grid, block, 0, stream, p);
-    case 2: return launch_overlapped(block_norms_kernel<TY, TH, 2>, grid, block, 0, stream, p);
-    default: return launch_overlapped(block_norms_kernel<TY, TH, 1>, grid, block, 0, stream, p);
+template <typename TY, typename TH, int V, int E, bool kWhole, int kThreads>
+cudaError_t launch_norms(NormsParams p, int block, size_t smem, cudaStream_t stream) {
+  // as many teams as run at once, each with its run of rows
+  const int teams = block / (p.warps > 1 ? 32 * p.warps : p.team);
+  const long long resident = static_cast<long long>(sm_count()) * std::max(1, kNormResident<TY, V, E, kWhole> / block) * teams;
+  p.run = static_cast<int>(std::max(1LL, (p.rows + resident - 1) / resident));
+  const long long all_teams = (p.rows + p.run - 1) / p.run;
+  auto* kernel = block_norms_kernel<TY, TH, V, E, kWhole, kThreads>;
+  if (smem > 47 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kNormShared);
+    if (e != cudaSuccess) return e;
   }
+  return launch_overlapped(kernel, static_cast<unsigned>((all_teams + teams - 1) / teams), static_cast<unsigned>(block), smem, stream, p);
+}
+template <typename TY, typename TH, int V, bool kWhole>
+cudaError_t launch_block_norms(const NormsParams& p, int e, int block, size_t smem, cudaStream_t stream) {
+  return e == 16 ? launch_norms<TY, TH, V, 16, kWhole, kNormBlock>(p, block, smem, stream)
+                 : launch_norms<TY, TH, V, 32, kWhole, 2 * kNormBlock>(p, block, smem, stream);
+}
+template <typename TY, typename TH>
+cudaError_t launch_block_norms(const NormsParams& p, int v, int e, int block, size_t smem, cudaStream_t stream) {
+  constexpr int kMost = 16 / sizeof(TY);
+  if (v == kMost)
+    return p.width % kMost == 0 ? launch_block_norms<TY, TH, kMost, true>(p, e, block, smem, stream)
+                                : launch_block_norms<TY, TH, kMost, false>(p, e, block, smem, stream);
+  if constexpr (sizeof(TY) == 2)
+    if (v == 2) return launch_block_norms<TY, TH, 2, false>(p, e, block, smem, stream);
+  return launch_block_norms<TY, TH, 1, true>(p, e, block, smem, stream);
 }
 }  // namespace
 
@@ -240,8 +379,8 @@ extern "C" int rldx_block_norms(const rldx_block_norms_desc* d, void* stream) {
   const int64_t lds[4] = {d->ld_branch, d->ld_residual, d->ld_residual_out, d->pre != RLDX_NORM_NONE ? d->ld_out : d->width};
   if (lds[0] < 0 || lds[1] < 0) return bad("negative strides");  // (0: one row for all)
   if (lds[2] < d->width || lds[3] < d->width) return bad("rows of a result overlap");
-  const bool grouped = d->ld_gate || d->ld_scale || d->ld_shift;
-  if (d->rows_per_group < 0 || (grouped && d->rows_per_group < 1)) return bad("vectors of groups need rows_per_group");
+  const bool grouped = (d->gate && d->ld_gate) || (d->mod_scale && d->ld_scale) || (d->mod_shift && d->ld_shift);
+  if (d->rows_per_group < 0 || ((d->ld_gate || d->ld_scale || d->ld_shift) && d->rows_per_group < 1)) return bad("vectors of groups need rows_per_group");
   for (int64_t ld : {d->ld_gate, d->ld_scale, d->ld_shift})
     if (ld < 0 || (ld > 0 && ld < d->width)) return bad("vectors of groups overlap");
   const void* rows_at[4] = {d->branch, d->residual, d->residual_out, d->out};
@@ -266,35 +405,46 @@ extern "C" int rldx_block_norms(const rldx_block_norms_desc* d, void* stream) {
   p.vectors_f32 = d->vector_dtype == RLDX_F32;
   p.scale = d->scale, p.eps = d->eps, p.plus_one = d->weight_plus_one ? 1.0f : 0.0f;
   // V values at a time: as many as the rows' common alignment allows.  The end of a row that they do not divide goes
-  // value by value, and so do vectors whose own alignment is less.
+  // value by value.
   int v = d->dtype == RLDX_F32 ? 4 : 8;
   auto fits = [](const void* at, int64_t ld, int size, int v) {
     return ld % v == 0 && reinterpret_cast<uintptr_t>(at) % std::min(16, v * size) == 0;
   };
   for (int i = 0; i < 4; ++i)
-    while (v > 1 && !fits(rows_at[i], lds[i], row_size[i], v)) v /= 2;
+    while (v > 1 && !fits(rows_at[i], lds[i], row_size[i], v)) v = v == 8 ? 2 : 1;
   p.aligned = 1;
   const int64_t vector_ld[7] = {0, 0, d->ld_gate, 0, 0, d->ld_scale, d->ld_shift};
   for (int i = 0; i < 7; ++i)
-    if (!fits(vectors[i], vector_ld[i], sv, v)) p.aligned = 0;
-  const int lanes = (d->width + kNormValues - 1) / kNormValues;
+    if (!fits(vectors[i], vector_ld[i], sv, 4)) p.aligned = 0;
+  // 16 values a thread, or 32 where that takes fewer instructions: about 10 a value and 150 a warp and row
+  // (and 16 while rows are too few to fill the SMs, where a row's own time counts)
+  const auto warps_of = [&](int e) { return (d->width + 32 * e - 1) / (32 * e); };
+  const bool few = d->rows * warps_of(16) <= 16LL * sm_count();
+  const int e_values = d->width <= 512 || (d->width <= 16 * kNormBlock && (few || warps_of(16) * 310 <= warps_of(32) * 470)) ? 16 : 32;
+  const int lanes = (d->width + e_values - 1) / e_values;
   p.warps = (lanes + 31) / 32;
   p.team = 4;
   while (p.team < 32 && p.team < lanes) p.team *= 2;
   const int threads = p.warps > 1 ? 32 * p.warps : p.team;
-  const int teams = p.warps > 1 ? std::max(1, 4 / p.warps) : 128 / threads;
-  const unsigned block = static_cast<unsigned>(teams * threads);
-  const unsigned grid = static_cast<unsigned>((d->rows + teams - 1) / teams);
+  const int teams = p.warps > 1 ? 1 : 128 / threads;
+  const int block = teams * threads;
+  const bool held[4] = {d->post_weight || d->gate, d->post_bias != nullptr, d->pre_weight || d->mod_scale, d->pre_bias || d->mod_shift};
+  const int values = threads * e_values;  // of a team's threads, 14336 at most
+  int all = 0;
+  for (int i = 0; i < 4; ++i) p.place[i] = held[i] ? values * all++ : -1;
+  p.padded = all ? values : 0;
+  p.copy = grouped ? values * all : 0;
+  const size_t smem = sizeof(float) * values * all * (grouped ? teams : 1);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool wide = d->residual_dtype == RLDX_F32;
   cudaError_t e;
   if (d->dtype == RLDX_F32)
-    e = launch_block_norms<float, float>(p, v, grid, block, st);
+    e = launch_block_norms<float, float>(p, v, e_values, block, smem, st);
   else if (d->dtype == RLDX_F16)
-    e = wide ? launch_block_norms<__half, float>(p, v, grid, block, st) : launch_block_norms<__half, __half>(p, v, grid, block, st);
+    e = wide ? launch_block_norms<__half, float>(p, v, e_values, block, smem, st) : launch_block_norms<__half, __half>(p, v, e_values, block, smem, st);
   else
-    e = wide ? launch_block_norms<__nv_bfloat16, float>(p, v, grid, block, st)
-             : launch_block_norms<__nv_bfloat16, __nv_bfloat16>(p, v, grid, block, st);
+    e = wide ? launch_block_norms<__nv_bfloat16, float>(p, v, e_values, block, smem, st)
+             : launch_block_norms<__nv_bfloat16, __nv_bfloat16>(p, v, e_values, block, smem, st);
   if (e != cudaSuccess) return cuda_fail(e, "block_norms launch");
   return RLDX_OK;
 }

@@ -79,23 +79,103 @@ struct LogprobsShared {
   int count;
 };
 
+// What differs between the types: a word of -inf, how many leading bits of the fp32 form tell values apart, how far from
+// zero a reference may lie for the short form of the differences, and the value that stands for what is below it there.
 template <typename T>
-struct LogitBits;  // a vector's worth of -inf, and how many leading bits tell values of T apart
+struct Logit;
 template <>
-struct LogitBits<__nv_bfloat16> {
-  static constexpr uint32_t kLowest = 0xff80ff80u;
+struct Logit<__nv_bfloat16> {
+  static constexpr uint32_t kLowest = 0xff80ff80u, kFloor = 0xf14af14au;  // -1e30
   static constexpr int kBits = 16;
+  static constexpr float kNear = 65536.0f;
 };
 template <>
-struct LogitBits<__half> {
-  static constexpr uint32_t kLowest = 0xfc00fc00u;
-  static constexpr int kBits = 19;  // of its fp32 form: sign, 8 exponent and 10 mantissa bits
+struct Logit<__half> {
+  static constexpr uint32_t kLowest = 0xfc00fc00u, kFloor = 0xfbfffbffu;  // -65504
+  static constexpr int kBits = 19;  // sign, 8 exponent and 10 mantissa bits
+  static constexpr float kNear = 32768.0f;
 };
 template <>
-struct LogitBits<float> {
+struct Logit<float> {
   static constexpr uint32_t kLowest = 0xff800000u;
   static constexpr int kBits = 32;
+  static constexpr float kNear = 65536.0f;
 };
+
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b, const __nv_bfloat16*) {
+  uint32_t r;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b, const __half*) {
+  uint32_t r;
+  asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b, const __nv_bfloat16*) {
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b, const __half*) {
+  uint32_t r;
+  asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(uint32_t w, const __nv_bfloat16*) {
+  float2 x;
+  unpack_bf16x2(w, x.x, x.y);
+  return x;
+}
+__device__ __forceinline__ float2 unpack2(uint32_t w, const __half*) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
+// Ones where a > b, added up in halves of a word (whole numbers up to 256 there).
+__device__ __forceinline__ void count2(uint32_t& n, uint32_t a, uint32_t b, const __nv_bfloat16*) {
+  const __nv_bfloat162 r = __hadd2(*reinterpret_cast<__nv_bfloat162*>(&n), __hgt2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b)));
+  n = *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ void count2(uint32_t& n, uint32_t a, uint32_t b, const __half*) {
+  const __half2 r = __hadd2(*reinterpret_cast<__half2*>(&n), __hgt2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b)));
+  n = *reinterpret_cast<const uint32_t*>(&r);
+}
+// The largest value of T below x (x finite).
+__device__ __forceinline__ __nv_bfloat16 below(__nv_bfloat16 x) {
+  const uint16_t b = __bfloat16_as_ushort(x);
+  return __ushort_as_bfloat16((b & 0x7fffu) == 0 ? 0x8001u : b & 0x8000u ? b + 1 : b - 1);
+}
+__device__ __forceinline__ __half below(__half x) {
+  const uint16_t b = __half_as_ushort(x);
+  return __ushort_as_half((b & 0x7fffu) == 0 ? 0x8001u : b & 0x8000u ? b + 1 : b - 1);
+}
+__device__ __forceinline__ float below(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return __uint_as_float((b & 0x7fffffffu) == 0 ? 0x80000001u : b & 0x80000000u ? b + 1 : b - 1);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t both(T x) {
+  if constexpr (sizeof(T) == 4)
+    return __float_as_uint(x);
+  else
+    return 0x10001u * *reinterpret_cast<const uint16_t*>(&x);
+}
+
+// The largest of a vector (NaN gives way).
+template <typename T>
+__device__ __forceinline__ float largest_of(const uint4 (&raw)[kLogpVecs]) {
+  if constexpr (sizeof(T) == 4) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kLogpVecs; ++k)
+      m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(raw[k].x), __uint_as_float(raw[k].y)), fmaxf(__uint_as_float(raw[k].z), __uint_as_float(raw[k].w))));
+    return m;
+  } else {
+    const T* t = nullptr;
+    uint32_t m = Logit<T>::kLowest;
+#pragma unroll
+    for (int k = 0; k < kLogpVecs; ++k) m = max2(m, max2(max2(raw[k].x, raw[k].y, t), max2(raw[k].z, raw[k].w, t), t), t);
+    const float2 x = unpack2(m, t);
+    return fmaxf(x.x, x.y);
+  }
+}
 
 __device__ __forceinline__ u64 key_of(float x, int id) {
   return (static_cast<u64>(order_bits(x)) << 32) | static_cast<uint32_t>(~id);
@@ -156,7 +236,7 @@ __device__ __forceinline__ void prune(LogprobsShared& s, int k) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kLogpThreads) logprobs_kernel(const __grid_constant__ LogprobsParams P) {
+__global__ void __launch_bounds__(kLogpThreads, 3) logprobs_kernel(const __grid_constant__ LogprobsParams P) {
   constexpr int kVec = 16 / sizeof(T);
   constexpr int NT = kLogpThreads, NV = kLogpVecs;
   __shared__ LogprobsShared s;
@@ -167,19 +247,39 @@ __global__ void __launch_bounds__(kLogpThreads) logprobs_kernel(const __grid_con
   griddep_wait();
   griddep_launch();
   const int top = P.top;
-  if (threadIdx.x == 0) s.count = 0, s.bound = 0;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) s.count = 0, s.bound = 0;
   const T* logits = static_cast<const T*>(P.logits) + row * P.ld;
   // vectors on 16-byte boundaries, the first and the last in part of other rows
   const int before = static_cast<int>(reinterpret_cast<uintptr_t>(logits) % 16 / sizeof(T));
   const uint4* vecs = reinterpret_cast<const uint4*>(logits - before);
   const int nvec = static_cast<int>((static_cast<long long>(P.vocab) + before + kVec - 1) / kVec);
   const int per = (nvec + cluster - 1) / cluster;
-  const int v_end = min(nvec, (part + 1) * per);
+  const int v_begin = part * per, v_end = min(nvec, v_begin + per);
+
+  // vector v of this part, -inf in the place of what is not of it
+  auto vec_at = [&](int v) {
+    constexpr uint32_t low = Logit<T>::kLowest;
+    uint4 u = make_uint4(low, low, low, low);
+    if (v < v_end) u = __ldcs(vecs + v);
+    if (v == 0 || v == nvec - 1) {
+      T* e = reinterpret_cast<T*>(&u);
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) {
+        const int id = v * kVec + i - before;
+        if (id < 0 || id >= P.vocab) e[i] = from_float<T>(-INFINITY);
+      }
+    }
+    return u;
+  };
+  uint4 raw[NV];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) raw[k] = vec_at(v_begin + k * NT + tid);
+
   const long long token = P.tokens[row];
   const bool given = token >= 0 && token < P.vocab;
-  const float x_token = given ? to_float(logits[token]) : INFINITY;
-  // equal logits count up to here: before the token, and in this part (what fills up its last chunk is -inf too)
-  const int id_token = given ? static_cast<int>(min(token, static_cast<long long>(v_end) * kVec - before)) : 0;
+  const T t_token = given ? logits[token] : from_float<T>(INFINITY);
+  const float x_token = to_float(t_token);
 
   Partial p{-FLT_MAX, 0.0f, 0.0f};
   float best = -INFINITY;  // this thread's largest logit so far, where it has seen one
@@ -188,59 +288,104 @@ __global__ void __launch_bounds__(kLogpThreads) logprobs_kernel(const __grid_con
   __syncthreads();
 
 #pragma unroll 1
-  for (int base = part * per; base < v_end; base += NT * NV) {
-    uint4 raw[NV];
+  for (int base = v_begin; base < v_end; base += NT * NV) {
+    const float largest = largest_of<T>(raw);
+    if (largest > p.m) move_to(p, largest);
+    // tokens before the given one are those above a value, if all of the chunk comes before it or after it; a
+    // chunk that holds it, and -inf, which fills up vectors, are looked at one by one
+    const long long first = static_cast<long long>(base) * kVec - before, last = static_cast<long long>(min(base + NT * NV, v_end)) * kVec - before;
+    T above = t_token;
+    if (x_token == -INFINITY || (token >= first && token < last)) {
+      const long long end = min(token, last);
+      if (given) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int v = base + k * NT + static_cast<int>(threadIdx.x);
-      if (v < v_end)
-        raw[k] = __ldcs(vecs + v);
-      else
-        raw[k] = make_uint4(LogitBits<T>::kLowest, LogitBits<T>::kLowest, LogitBits<T>::kLowest, LogitBits<T>::kLowest);
-      if (v == 0 || v == nvec - 1) {  // values of other rows
-        T* e = reinterpret_cast<T*>(&raw[k]);
+        for (int k = 0; k < NV; ++k) {
+          Raw<T, kVec> r;
+          r.w[0] = raw[k];
+          float x[kVec];
+          unpack_row<T, kVec>(r, x);
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-          const int id = v * kVec + i - before;
-          if (id < 0 || id >= P.vocab) e[i] = from_float<T>(-INFINITY);
+          for (int i = 0; i < kVec; ++i) {
+            const long long id = first + (k * NT + tid) * kVec + i;
+            better += x[i] > x_token || (x[i] == x_token && id >= 0 && id < end);
+          }
         }
       }
+      above = from_float<T>(INFINITY);
+    } else if (given && last <= token && x_token < INFINITY && x_token == x_token) {
+      above = below(t_token);
     }
-    auto values = [&](int k, float (&x)[kVec]) {
-      Raw<T, kVec> r;
-      r.w[0] = raw[k];
-      unpack_row<T, kVec>(r, x);
-    };
-    float largest = -INFINITY;
+    const uint32_t above2 = both(above);
+    uint32_t count = 0;
+    const T* t = nullptr;
+    const int next = base + NT * NV + tid;
+    if (fabsf(p.m) <= Logit<T>::kNear) {
+      // exp2(x log2 e - c) with c = m log2 e rounded: one product a value, and what the rounding left out, rho, is put right
+      // for all of the chunk.  Of values so far from the reference that they count as nothing it takes a finite one.
+      const float c = p.m * kLog2e;
+      const float rho = fmaf(p.m, kLog2e, -c);
+      const float2 l2 = make_float2(kLog2e, kLog2e), c2 = make_float2(-c, -c);
+      float2 s2 = make_float2(0.0f, 0.0f), t2 = s2;
+      auto add = [&](float2 x) {
+        const float2 d = fma_f32x2(x, l2, c2);
+        const float2 e = make_float2(ex2_approx(d.x), ex2_approx(d.y));
+        s2 = add_f32x2(s2, e);
+        t2 = fma_f32x2(e, d, t2);
+      };
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      float x[kVec];
-      values(k, x);
+      for (int k = 0; k < NV; ++k) {
+        const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+        raw[k] = vec_at(next + k * NT);
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) largest = fmaxf(largest, x[i]);
-    }
-    if (largest > p.m) move_to(p, largest);
-    float chunk_s = 0.0f, chunk_t = 0.0f;  // (short sums: a thread of a long row adds hundreds of values)
+          for (int i = 0; i < 4; i += 2) {
+            const float a = __uint_as_float(w[i]), b = __uint_as_float(w[i + 1]);
+            count += a > __uint_as_float(above2), count += b > __uint_as_float(above2);
+            add(make_float2(max_nan(a, -1e30f), max_nan(b, -1e30f)));
+          }
+        } else {
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      float x[kVec];
-      values(k, x);
-      const int id0 = (base + k * NT + static_cast<int>(threadIdx.x)) * kVec - before;  // (before the row: x is -inf there)
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) {
-        const float d = max_nan((x[i] - p.m) * kLog2e, kLogpLeast), e = ex2_approx(d);
-        chunk_s += e;
-        chunk_t = fmaf(e, d, chunk_t);
-        better += x[i] > x_token || (x[i] == x_token && id0 + i >= 0 && id0 + i < id_token);
+          for (int i = 0; i < 4; ++i) {
+            count2(count, w[i], above2, t);
+            add(unpack2(max2_nan(w[i], Logit<T>::kFloor, t), t));
+          }
+        }
       }
+      const float f = ex2_approx(-rho), sum = f * (s2.x + s2.y);
+      p.s += sum;
+      p.t += fmaf(-rho, sum, f * (t2.x + t2.y));
+    } else {
+      float sum = 0.0f, sum_d = 0.0f;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        Raw<T, kVec> r;
+        r.w[0] = raw[k];
+        raw[k] = vec_at(next + k * NT);
+        float x[kVec];
+        unpack_row<T, kVec>(r, x);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+          const float d = max_nan((x[i] - p.m) * kLog2e, kLogpLeast), e = ex2_approx(d);
+          sum += e;
+          sum_d = fmaf(e, d, sum_d);
+          better += x[i] > to_float(above);
+        }
+      }
+      p.s += sum, p.t += sum_d;
     }
-    p.s += chunk_s, p.t += chunk_t;
+    if constexpr (sizeof(T) == 4) {
+      better += count;
+    } else {
+      const float2 n = unpack2(count, t);
+      better += static_cast<uint32_t>(n.x + n.y);
+    }
+
     if (top == 0) continue;
     const u64 bound = s.bound;  // 0: none yet
     const float bound_x = bound ? order_value(static_cast<uint32_t>(bound >> 32)) : -INFINITY;
     const int bound_id = bound ? static_cast<int>(~static_cast<uint32_t>(bound)) : INT32_MAX;
-    const int id0 = (base + static_cast<int>(threadIdx.x)) * kVec - before;
-    const bool here = base + static_cast<int>(threadIdx.x) < v_end;  // the thread has values in this chunk
+    const int id0 = (base + tid) * kVec - before;
+    const bool here = base + tid < v_end;  // the thread has values in this chunk
     const bool rises = here && (largest > bound_x || (largest == bound_x && id0 <= bound_id));
     const bool earlier = seen;
     const float earlier_best = best;
@@ -252,47 +397,59 @@ __global__ void __launch_bounds__(kLogpThreads) logprobs_kernel(const __grid_con
     int new_id = bound_id;
     if (rising > top) {
       // a new bound: the top-th largest of the threads' maxima
-      constexpr int low = 32 - LogitBits<T>::kBits;
+      constexpr int low = 32 - Logit<T>::kBits;
       const uint32_t bits = seen ? order_bits(best) : 0u;
-      uint32_t t = reached_by(top, 31, low, [&](uint32_t c) { return bits >= c; });
-      if (!(t >> 31)) t |= (1u << low) - 1u;  // (negative values: the bits that the type does not have are ones)
-      const float tx = order_value(t);
+      uint32_t reach = reached_by(top, 31, low, [&](uint32_t c) { return bits >= c; });
+      if (!(reach >> 31)) reach |= (1u << low) - 1u;  // (negative values: the bits that the type does not have are ones)
+      const float tx = order_value(reach);
       if (tx >= bound_x) {
-        const int above = __syncthreads_count(bits > t), tied = __syncthreads_count(bits == t);
+        const int higher = __syncthreads_count(bits > reach), tied = __syncthreads_count(bits == reach);
         new_id = tx > bound_x ? INT32_MAX : bound_id;
         new_x = tx;
-        if (tied > top - above) {
+        if (tied > top - higher) {
           // of those that share the value the lowest ids; one of an earlier chunk counts as lower than any here
           int id = INT32_MAX;
           if (earlier && earlier_best == tx) {
             id = 0;
-          } else if (bits == t) {
-#pragma unroll
+          } else if (bits == reach) {
+#pragma unroll 1
             for (int k = NV - 1; k >= 0; --k) {
+              Raw<T, kVec> r;
+              r.w[0] = vec_at(base + k * NT + tid);
               float x[kVec];
-              values(k, x);
+              unpack_row<T, kVec>(r, x);
 #pragma unroll
               for (int i = kVec - 1; i >= 0; --i) {
                 const int at = id0 + k * NT * kVec + i;
-                if (x[i] == tx && at >= 0 && at < P.vocab) id = at;
+                if (x[i] == tx && base + k * NT + tid < v_end && at >= 0 && at < P.vocab) id = at;
               }
             }
           }
-          const uint32_t order = bits == t ? static_cast<uint32_t>(INT32_MAX - id) : 0u;
-          const uint32_t r = reached_by(top - above, 30, 0, [&](uint32_t c) { return order >= c; });
+          const uint32_t order = bits == reach ? static_cast<uint32_t>(INT32_MAX - id) : 0u;
+          const uint32_t r = reached_by(top - higher, 30, 0, [&](uint32_t c) { return order >= c; });
           new_id = min(new_id, INT32_MAX - static_cast<int>(r));
         }
       }
     }
-    if (rises && largest >= new_x) {
+    // what reaches the bound: a warp reads the vectors of four such threads at a time again
+    uint32_t who = __ballot_sync(0xffffffffu, rises && largest >= new_x);
+    while (who) {
+      int mine = -1;
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
+      for (int g = 0; g < 4; ++g) {
+        if (who && lane >> 3 == g) mine = __ffs(who) - 1;
+        who &= who - 1;
+      }
+      const int v = base + (lane & 7) * NT + warp * 32 + mine;
+      if (mine >= 0 && v < v_end) {
+        Raw<T, kVec> r;
+        r.w[0] = vec_at(v);
         float x[kVec];
-        values(k, x);
+        unpack_row<T, kVec>(r, x);
 #pragma unroll
         for (int i = 0; i < kVec; ++i) {
-          const int id = id0 + k * NT * kVec + i;
-          if ((x[i] > new_x || (x[i] == new_x && id <= new_id)) && id >= 0 && base + k * NT + static_cast<int>(threadIdx.x) < v_end && id < P.vocab) {
+          const int id = v * kVec + i - before;
+          if ((x[i] > new_x || (x[i] == new_x && id <= new_id)) && id >= 0 && id < P.vocab) {
             const int at = atomicAdd(&s.count, 1);
             if (at < kLogpList) s.list[at] = key_of(x[i], id);
           }
@@ -301,7 +458,7 @@ __global__ void __launch_bounds__(kLogpThreads) logprobs_kernel(const __grid_con
     }
     __syncthreads();
     const int listed = s.count;
-    if (threadIdx.x == 0 && (new_x != bound_x || new_id != bound_id)) s.bound = key_of(new_x, new_id);
+    if (tid == 0 && (new_x != bound_x || new_id != bound_id)) s.bound = key_of(new_x, new_id);
     __syncthreads();
     if (listed > kLogpPrune) prune(s, top);
   }
@@ -313,7 +470,6 @@ __global__ void __launch_bounds__(kLogpThreads) logprobs_kernel(const __grid_con
     join(p, q);
   }
   better = __reduce_add_sync(0xffffffffu, better);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (lane == 0) s.warps[warp] = make_float4(p.m, p.s, p.t, __uint_as_float(better));
   __syncthreads();
   // and its list go to rank 0

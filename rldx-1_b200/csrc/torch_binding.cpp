@@ -486,7 +486,7 @@ PyObject* block_norms(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (y.dim() != 2 || (y.size(1) > 1 && y.stride(1) != 1)) refuse_value("branch must be a 2-D row-major view");
     const int64_t rows = y.size(0), width = y.size(1);
     if (h.sizes() != y.sizes() || (width > 1 && h.stride(1) != 1)) refuse_value("residual must be a row-major view of branch's shape");
-    if (width < 1 || width > 16384) refuse_value("rows must have 1 to 16384 values");
+    if (width < 1 || width > 14336) refuse_value("rows must have 1 to 14336 values");
     d.post = small(a[2], "post"), d.pre = small(a[7], "pre");
     d.rows = rows, d.width = static_cast<int>(width);
     d.rows_per_group = integer(a[12]);

@@ -430,7 +430,7 @@ def rope_rows(positions, freqs, *, sections: Optional[Sequence[int]] = None, int
 def block_norms(branch, residual, *, post: Optional[str] = None, post_weight=None, post_bias=None, gate=None, scale: float = 1.0,
                 pre: Optional[str] = "rms", pre_weight=None, pre_bias=None, mod_scale=None, mod_shift=None, rows_per_group: int = 0,
                 weight_plus_one: bool = False, eps: float = 1e-6, out_residual=None, out=None):
-    """What stands between two blocks, in one pass over rows [rows, width] (width at most 16384):
+    """What stands between two blocks, in one pass over rows [rows, width] (width at most 14336):
 
         residual' = residual + scale * gate * post(branch)
         out       = pre(residual', unrounded) * (1 + mod_scale) + mod_shift

@@ -123,8 +123,8 @@ def test_block_norms_refusals():
     refused(ValueError, "residual", h=h[:5])
     refused(ValueError, "row-major", y=torch.zeros(40, 6, dtype=BF).t())
     refused(ValueError, "row-major", y=torch.zeros(2, 6, 40, dtype=BF))
-    refused(ValueError, "16384", y=torch.zeros(1, 16385), h=torch.zeros(1, 16385))
-    refused(ValueError, "16384", y=torch.zeros(1, 0), h=torch.zeros(1, 0))
+    refused(ValueError, "14336", y=torch.zeros(1, 14337), h=torch.zeros(1, 14337))
+    refused(ValueError, "14336", y=torch.zeros(1, 0), h=torch.zeros(1, 0))
     refused(TypeError, "all", gate=v, pre_weight=v.float())
     refused(TypeError, "all", gate=v.half())
     refused(ValueError, "pre_weight", pre_weight=v[:39])
