@@ -7,7 +7,7 @@
 // Everything is fp32 until the two results are rounded, once each; pre takes the sum before its rounding.  The
 // variance is the mean square of what the mean leaves, from registers.
 //
-// A row lies in the registers of a team: 4 to 32 lanes, or a few warps, of 16 or 32 values a thread.  The vectors come down
+// A row lies in the registers of a team: 8 lanes, a warp or several, 16 values a thread.  The vectors come down
 // to four numbers a value, h' = h + (a y^ + b) and n = c h^ + d with a = scale gate (w + 1), b = scale gate b, c = (w + 1)
 // (1 + mod_scale), d = b (1 + mod_scale) + mod_shift, kept in shared memory: made once by a CTA where all rows share them,
 // else by each team whenever it comes to another group.  A CTA goes over a run of rows, the next of which is on the way
@@ -19,8 +19,8 @@ namespace rldx {
 
 namespace {
 constexpr int kNormMaxWidth = 14336;  // four vectors of it fill the shared memory
-constexpr int kNormBlock = 256;             // threads, of one row or several
 constexpr int kNormShared = 4 * 4 * kNormMaxWidth;
+constexpr int kNormValues = 16;       // of a thread
 enum { kNormA = 0, kNormB = 1, kNormC = 2, kNormD = 3 };
 
 struct NormsParams {
@@ -44,7 +44,7 @@ struct NormsParams {
   int copy;                // and of a team's own copy of them; 0: one for all
   int padded;              // values of one of them there
   int vectors_f32, aligned;  // the vectors' type; four of them may be loaded at once
-  int team, warps;         // lanes of a row (4 to 32), warps of a row
+  int warps;               // of a row
   float scale, eps, plus_one;
 };
 
@@ -67,43 +67,17 @@ __device__ __forceinline__ void vector_at(const NormsParams& P, const void* base
     read(static_cast<const T*>(base));
 }
 
-// kWhole: a vector of V values is there whole or not at all.
-template <typename T, int V, bool kWhole>
-__device__ __forceinline__ Raw<T, V> row_at(const T* p, int n) {
-  Raw<T, V> r = {};
-  if (kWhole ? n > 0 : n >= V) {
-    r = load_once<T, V>(p);
-  } else if constexpr (!kWhole) {
-    T* e = reinterpret_cast<T*>(&r);
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (i < n) e[i] = p[i];
-  }
-  return r;
-}
-template <typename T, int V, bool kWhole>
-__device__ __forceinline__ void row_to(T* p, int n, const float (&x)[V]) {
-  if (kWhole ? n > 0 : n >= V) {
-    store_once<T, V>(p, pack_row<T, V>(x));
-  } else if constexpr (!kWhole) {
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (i < n) p[i] = from_float<T>(x[i]);
-  }
-}
-
 // Sum over a row's team.  Several warps are all of the CTA: each leaves its sum, and all read them after a barrier; two
 // sets of places take turns, so one barrier a sum is enough.
-template <int kWarps>
+template <int kLanes, int kWarps>
 struct TeamSum {
   float* places;  // [2][kWarps], zeros past the row's warps
-  int team, warps;
+  bool several;
   int turn = 0;
   __device__ __forceinline__ float operator()(float x) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-      if (o < team) x += __shfl_xor_sync(0xffffffffu, x, o);
-    if (warps == 1) return x;
+    for (int o = kLanes / 2; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    if (kLanes < 32 || !several) return x;
     float* p = places + turn;
     turn ^= kWarps;
     if ((threadIdx.x & 31) == 0) p[threadIdx.x >> 5] = x;
@@ -115,28 +89,28 @@ struct TeamSum {
   }
 };
 
-// Threads that run on an SM at once, from their registers: 80 with vectors of eight and 16 values, 128 else.
-template <typename TY, int V, int E, bool kWhole>
-constexpr int kNormResident = sizeof(TY) == 2 && V == 8 && E == 16 && kWhole ? 768 : 512;
+// Threads that run on an SM at once, from their registers: 80 with vectors of eight, 64 in CTAs of up to 1024, 128 else.
+template <int V, int kThreads>
+constexpr int kNormResident = kThreads > 256 ? 1024 : V == 8 ? 768 : 512;
 
-// E values a thread, V at a time.
-template <typename TY, typename TH, int V, int E, bool kWhole, int kThreads>
-__global__ void __launch_bounds__(kThreads, kNormResident<TY, V, E, kWhole> / kThreads) block_norms_kernel(const __grid_constant__ NormsParams P) {
-  constexpr int K = E / V;
+// V values at a time, which divides the width; kLanes: of a row, or of one of its warps.
+template <typename TY, typename TH, int V, int kLanes, int kThreads>
+__global__ void __launch_bounds__(kThreads, kNormResident<V, kThreads> / kThreads) block_norms_kernel(const __grid_constant__ NormsParams P) {
+  constexpr int E = kNormValues, K = E / V, kStep = kLanes * V;
   constexpr int kWarps = kThreads / 32;
   extern __shared__ __align__(16) float shared[];  // a, b, c, d
   __shared__ float places[2 * kWarps];
   griddep_wait();
   griddep_launch();
-  const int threads = P.warps > 1 ? 32 * P.warps : P.team;  // of a row
-  const int teams = blockDim.x / threads, slot = threadIdx.x / threads, at = threadIdx.x - slot * threads;
+  const int threads = P.warps > 1 ? 32 * P.warps : kLanes;  // of a row
+  const int teams = blockDim.x / threads, slot = P.warps > 1 ? 0 : threadIdx.x / kLanes, at = threadIdx.x - slot * threads;
   if (threadIdx.x < 2 * kWarps) places[threadIdx.x] = 0.0f;
-  TeamSum<kWarps> sum{places, P.team, P.warps};
+  TeamSum<kLanes, kWarps> sum{places, P.warps > 1};
   long long row = static_cast<long long>(blockIdx.x) * teams * P.run + slot;
   const long long row_end = min(P.rows, row - slot + teams * P.run);
-  // Vector k begins at value at V + k step; n(k) values are there, V or more of a whole one.
-  const int step = threads * V, first = at * V, width = P.width;
-  auto n = [&](int k) { return width - first - k * step; };
+  // Vector k of a thread begins at value first + k kStep; `have` of them are there.
+  const int width = P.width, first = at / kLanes * (kLanes * E) + at % kLanes * V;
+  const int have = min(K, max(0, (width - first + kStep - 1) / kStep));
   const float inv_d = 1.0f / static_cast<float>(width), root_inv_d = rsqrtf(static_cast<float>(width));
 
   const TY* y_at = static_cast<const TY*>(P.y) + row * P.ld_y + first;
@@ -145,18 +119,25 @@ __global__ void __launch_bounds__(kThreads, kNormResident<TY, V, E, kWhole> / kT
   TY* n_to = static_cast<TY*>(P.n_out) + row * P.ld_n + first;
   Raw<TY, V> y[K];
   Raw<TH, V> h[K];
-  auto load_y = [&](bool real) {
+  auto load_y = [&](int have) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) y[k] = row_at<TY, V, kWhole>(y_at + k * step, real ? n(k) : 0);
+    for (int k = 0; k < K; ++k) {
+      y[k] = Raw<TY, V>{};
+      if (k < have) y[k] = load_once<TY, V>(y_at + k * kStep);
+    }
     y_at += teams * P.ld_y;
   };
-  auto load_h = [&](bool real) {
+  auto load_h = [&](int have) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) h[k] = row_at<TH, V, kWhole>(h_at + k * step, real ? n(k) : 0);
+    for (int k = 0; k < K; ++k) {
+      h[k] = Raw<TH, V>{};
+      if (k < have) h[k] = load_once<TH, V>(h_at + k * kStep);
+    }
     h_at += teams * P.ld_h;
   };
-  load_y(row < row_end);
-  load_h(row < row_end);
+  load_y(row < row_end ? have : 0);
+  load_h(row < row_end ? have : 0);
+
   // a, b, c, d of group g, by `by` threads of which this is the `me`-th, four values at a time; threads of eight values
   // read theirs in two halves, each side by side with the other threads' (half: where the second ones begin)
   float* const mine = shared + slot * P.copy;
@@ -211,95 +192,88 @@ __global__ void __launch_bounds__(kThreads, kNormResident<TY, V, E, kWhole> / kT
 #pragma unroll 1
   for (int left = P.run; left > 0; --left) {  // (the same count for every team: lanes of a warp stay together)
     asm volatile("" ::: "memory");  // (a to d are read anew for each row: kept in registers they would take most of them)
-    const bool real = row < row_end, more = left > 1 && row + teams < row_end;
-    float x[K][V];
+    const int next = left > 1 && row + teams < row_end ? have : 0, here = row < row_end ? have : 0;
+    float2 x[E / 2];  // two by two, in packed arithmetic
 #pragma unroll
-    for (int k = 0; k < K; ++k) unpack_row<TY, V>(y[k], x[k]);
-    load_y(more);
-
-    // What is not there counts as v.
-    auto fill = [&](float v) {
+    for (int k = 0; k < K; ++k) unpack_row<TY, V>(y[k], *reinterpret_cast<float(*)[V]>(reinterpret_cast<float*>(x) + k * V));
+    load_y(next);
+    auto each = [&](auto f) {
 #pragma unroll
-      for (int k = 0; k < K; ++k)
-        if (n(k) < V)
-#pragma unroll
-          for (int i = 0; i < V; ++i) x[k][i] = !kWhole && i < n(k) ? x[k][i] : v;
+      for (int j = 0; j < E / 2; ++j) x[j] = f(x[j]);
     };
-    // 1 / sqrt of the mean square of x, centred first for a LayerNorm (x is zero where nothing is)
+    auto times = [&](float v) { each([v](float2 a) { return mul_f32x2(a, make_float2(v, v)); }); };
+    // 1 / sqrt of the mean square of x, centred first for a LayerNorm (x is zero where nothing is, and then again)
     auto inverse_size = [&](int kind) {
+      auto total = [&](float2 s) { return sum(s.x + s.y); };
       if (kind == RLDX_NORM_LAYER) {
-        float s = 0.0f;
+        float2 s = x[0];
 #pragma unroll
-        for (int k = 0; k < K; ++k)
+        for (int j = 1; j < E / 2; ++j) s = add_f32x2(s, x[j]);
+        const float mean = total(s) * inv_d;
+        each([mean](float2 a) { return add_f32x2(a, make_float2(-mean, -mean)); });
+        if (have < K) {
+          float* v = reinterpret_cast<float*>(x);
 #pragma unroll
-          for (int i = 0; i < V; ++i) s += x[k][i];
-        const float mean = sum(s) * inv_d;
-        fill(mean);
+          for (int k = 0; k < K; ++k)
+            if (k >= have)
 #pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-          for (int i = 0; i < V; ++i) x[k][i] -= mean;
-      }
-      float s = 0.0f;
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float v = x[k][i] * root_inv_d;  // (a mean, not a sum, of squares stays in range up to 1.8e19)
-          s = fmaf(v, v, s);
+              for (int i = 0; i < V; ++i) v[k * V + i] = 0.0f;
         }
-      return rsqrtf(sum(s) + P.eps);
+      }
+      float2 s = make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int j = 0; j < E / 2; ++j) {
+        const float2 v = mul_f32x2(x[j], make_float2(root_inv_d, root_inv_d));  // (a mean, not a sum, of squares is in range up to 1.8e19)
+        s = fma_f32x2(v, v, s);
+      }
+      return rsqrtf(total(s) + P.eps);
     };
-    // f(x, number) with those of a vector in shared memory
+    // f(x, numbers) with those of a vector in shared memory (a is 0 past the width, and so are b, c and d)
     auto with = [&](int which, auto f) {
       const int place = P.place[which];
       if (place < 0) return;
+      const float* from = mine + place + (V == 8 ? first / 2 : first);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        float v[V];
-        const float* from = mine + place + (V == 8 ? (first + k * step) / 2 : first + k * step);
-        if constexpr (V % 4 == 0) {
-#pragma unroll
-          for (int i = 0; i < V; i += 4) *reinterpret_cast<float4*>(v + i) = *reinterpret_cast<const float4*>(from + (i ? half : 0));
+        float2 v[(V + 1) / 2];
+        if constexpr (V == 1) {
+          if (k % 2 == 0) x[k / 2] = f(x[k / 2], make_float2(from[k * kStep], from[(k + 1) * kStep]));
         } else {
 #pragma unroll
-          for (int i = 0; i < V; ++i) v[i] = from[i];
-        }
+          for (int i = 0; i < V / 4; ++i)
+            *reinterpret_cast<float4*>(v + 2 * i) = *reinterpret_cast<const float4*>(from + (V == 8 ? k * kStep / 2 : k * kStep) + (i ? half : 0));
 #pragma unroll
-        for (int i = 0; i < V; ++i) x[k][i] = f(x[k][i], v[i]);
+          for (int i = 0; i < V / 2; ++i) x[k * V / 2 + i] = f(x[k * V / 2 + i], v[i]);
+        }
       }
     };
-    auto times = [](float a, float b) { return a * b; };
-    auto plus = [](float a, float b) { return a + b; };
+    auto product = [](float2 a, float2 b) { return mul_f32x2(a, b); };
+    auto plus = [](float2 a, float2 b) { return add_f32x2(a, b); };
+    auto vector = [&](int k) -> const float(&)[V] { return *reinterpret_cast<const float(*)[V]>(reinterpret_cast<const float*>(x) + k * V); };
 
     const float post = P.post != RLDX_NORM_NONE ? inverse_size(P.post) : 1.0f;
-    const float size = P.place[kNormA] < 0 ? P.scale * post : post;
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int i = 0; i < V; ++i) x[k][i] *= size;
-    with(kNormA, times);
+    times(P.place[kNormA] < 0 ? P.scale * post : post);
+    with(kNormA, product);
     with(kNormB, plus);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       float r[V];
       unpack_row<TH, V>(h[k], r);
+      float* v = reinterpret_cast<float*>(x) + k * V;
 #pragma unroll
-      for (int i = 0; i < V; ++i) x[k][i] += r[i];
-      row_to<TH, V, kWhole>(h_to + k * step, real ? n(k) : 0, x[k]);
+      for (int i = 0; i < V; ++i) v[i] += r[i];
     }
-    load_h(more);
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (k < here) store_once<TH, V>(h_to + k * kStep, pack_row<TH, V>(vector(k)));
+    load_h(next);
     if (P.pre != RLDX_NORM_NONE) {  // (the same for every thread)
-      fill(0.0f);
-      const float pre = inverse_size(P.pre);
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int i = 0; i < V; ++i) x[k][i] *= pre;
-      with(kNormC, times);
+      times(inverse_size(P.pre));
+      with(kNormC, product);
       with(kNormD, plus);
 #pragma unroll
-      for (int k = 0; k < K; ++k) row_to<TY, V, kWhole>(n_to + k * step, real ? n(k) : 0, x[k]);
+      for (int k = 0; k < K; ++k)
+        if (k < here) store_once<TY, V>(n_to + k * kStep, pack_row<TY, V>(vector(k)));
       n_to += teams * P.ld_n;
     }
     h_to += teams * P.ld_h_out;
@@ -314,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, kNormResident<TY, V, E, kWhole> / kT
       };
       wait();  // the last row's numbers have been read
       if (next_group) {
-        const long long g = min(row, P.rows - 1) / P.group;
+        const long long g = row / P.group;
         group_end = (g + 1) * P.group;
         make_vectors(g, at, threads);
       }
@@ -323,34 +297,41 @@ __global__ void __launch_bounds__(kThreads, kNormResident<TY, V, E, kWhole> / kT
   }
 }
 
-template <typename TY, typename TH, int V, int E, bool kWhole, int kThreads>
-cudaError_t launch_norms(NormsParams p, int block, size_t smem, cudaStream_t stream) {
+template <typename TY, typename TH, int V, int kLanes, int kThreads>
+cudaError_t launch_norms(NormsParams p, int values, cudaStream_t stream) {
   // as many teams as run at once, each with its run of rows
-  const int teams = block / (p.warps > 1 ? 32 * p.warps : p.team);
-  const long long resident = static_cast<long long>(sm_count()) * std::max(1, kNormResident<TY, V, E, kWhole> / block) * teams;
+  const int block = p.warps > 1 ? 32 * p.warps : 128, teams = p.warps > 1 ? 1 : block / kLanes;
+  const long long resident = static_cast<long long>(sm_count()) * std::max(1, kNormResident<V, kThreads> / block) * teams;
   p.run = static_cast<int>(std::max(1LL, (p.rows + resident - 1) / resident));
   const long long all_teams = (p.rows + p.run - 1) / p.run;
-  auto* kernel = block_norms_kernel<TY, TH, V, E, kWhole, kThreads>;
+  const size_t smem = sizeof(float) * values * (p.copy ? teams : 1);
+  auto* kernel = block_norms_kernel<TY, TH, V, kLanes, kThreads>;
   if (smem > 47 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kNormShared);
     if (e != cudaSuccess) return e;
   }
   return launch_overlapped(kernel, static_cast<unsigned>((all_teams + teams - 1) / teams), static_cast<unsigned>(block), smem, stream, p);
 }
-template <typename TY, typename TH, int V, bool kWhole>
-cudaError_t launch_block_norms(const NormsParams& p, int e, int block, size_t smem, cudaStream_t stream) {
-  return e == 16 ? launch_norms<TY, TH, V, 16, kWhole, kNormBlock>(p, block, smem, stream)
-                 : launch_norms<TY, TH, V, 32, kWhole, 2 * kNormBlock>(p, block, smem, stream);
+template <typename TY, typename TH, int V>
+cudaError_t launch_block_norms(NormsParams p, bool grouped, const bool (&held)[4], cudaStream_t stream) {
+  // a row of up to 128 values is 8 lanes', of up to 512 a warp's
+  const int lanes = p.width <= 8 * kNormValues ? 8 : 32;
+  p.warps = (p.width + lanes * kNormValues - 1) / (lanes * kNormValues);
+  p.padded = lanes * p.warps * kNormValues;  // 14336 at most
+  int values = 0;
+  for (int i = 0; i < 4; ++i) {
+    p.place[i] = held[i] ? values : -1;
+    values += held[i] ? p.padded : 0;
+  }
+  if (!values) p.padded = 0;
+  p.copy = grouped ? values : 0;
+  return lanes == 8      ? launch_norms<TY, TH, V, 8, 256>(p, values, stream)
+         : p.warps <= 8 ? launch_norms<TY, TH, V, 32, 256>(p, values, stream)
+                        : launch_norms<TY, TH, V, 32, 1024>(p, values, stream);
 }
 template <typename TY, typename TH>
-cudaError_t launch_block_norms(const NormsParams& p, int v, int e, int block, size_t smem, cudaStream_t stream) {
-  constexpr int kMost = 16 / sizeof(TY);
-  if (v == kMost)
-    return p.width % kMost == 0 ? launch_block_norms<TY, TH, kMost, true>(p, e, block, smem, stream)
-                                : launch_block_norms<TY, TH, kMost, false>(p, e, block, smem, stream);
-  if constexpr (sizeof(TY) == 2)
-    if (v == 2) return launch_block_norms<TY, TH, 2, false>(p, e, block, smem, stream);
-  return launch_block_norms<TY, TH, 1, true>(p, e, block, smem, stream);
+cudaError_t launch_block_norms(const NormsParams& p, bool whole, bool grouped, const bool (&held)[4], cudaStream_t stream) {
+  return whole ? launch_block_norms<TY, TH, 16 / sizeof(TY)>(p, grouped, held, stream) : launch_block_norms<TY, TH, 1>(p, grouped, held, stream);
 }
 }  // namespace
 
@@ -404,47 +385,28 @@ extern "C" int rldx_block_norms(const rldx_block_norms_desc* d, void* stream) {
   p.width = d->width, p.post = d->post, p.pre = d->pre;
   p.vectors_f32 = d->vector_dtype == RLDX_F32;
   p.scale = d->scale, p.eps = d->eps, p.plus_one = d->weight_plus_one ? 1.0f : 0.0f;
-  // V values at a time: as many as the rows' common alignment allows.  The end of a row that they do not divide goes
-  // value by value.
-  int v = d->dtype == RLDX_F32 ? 4 : 8;
+  // 16 bytes of y at a time where the rows' alignment and the width allow it, else one value
+  const int v = 16 / sy;
   auto fits = [](const void* at, int64_t ld, int size, int v) {
     return ld % v == 0 && reinterpret_cast<uintptr_t>(at) % std::min(16, v * size) == 0;
   };
-  for (int i = 0; i < 4; ++i)
-    while (v > 1 && !fits(rows_at[i], lds[i], row_size[i], v)) v = v == 8 ? 2 : 1;
+  bool whole = d->width % v == 0;
+  for (int i = 0; i < 4; ++i) whole &= fits(rows_at[i], lds[i], row_size[i], v);
   p.aligned = 1;
   const int64_t vector_ld[7] = {0, 0, d->ld_gate, 0, 0, d->ld_scale, d->ld_shift};
   for (int i = 0; i < 7; ++i)
     if (!fits(vectors[i], vector_ld[i], sv, 4)) p.aligned = 0;
-  // 16 values a thread, or 32 where that takes fewer instructions: about 10 a value and 150 a warp and row
-  // (and 16 while rows are too few to fill the SMs, where a row's own time counts)
-  const auto warps_of = [&](int e) { return (d->width + 32 * e - 1) / (32 * e); };
-  const bool few = d->rows * warps_of(16) <= 16LL * sm_count();
-  const int e_values = d->width <= 512 || (d->width <= 16 * kNormBlock && (few || warps_of(16) * 310 <= warps_of(32) * 470)) ? 16 : 32;
-  const int lanes = (d->width + e_values - 1) / e_values;
-  p.warps = (lanes + 31) / 32;
-  p.team = 4;
-  while (p.team < 32 && p.team < lanes) p.team *= 2;
-  const int threads = p.warps > 1 ? 32 * p.warps : p.team;
-  const int teams = p.warps > 1 ? 1 : 128 / threads;
-  const int block = teams * threads;
   const bool held[4] = {d->post_weight || d->gate, d->post_bias != nullptr, d->pre_weight || d->mod_scale, d->pre_bias || d->mod_shift};
-  const int values = threads * e_values;  // of a team's threads, 14336 at most
-  int all = 0;
-  for (int i = 0; i < 4; ++i) p.place[i] = held[i] ? values * all++ : -1;
-  p.padded = all ? values : 0;
-  p.copy = grouped ? values * all : 0;
-  const size_t smem = sizeof(float) * values * all * (grouped ? teams : 1);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool wide = d->residual_dtype == RLDX_F32;
   cudaError_t e;
   if (d->dtype == RLDX_F32)
-    e = launch_block_norms<float, float>(p, v, e_values, block, smem, st);
+    e = launch_block_norms<float, float>(p, whole, grouped, held, st);
   else if (d->dtype == RLDX_F16)
-    e = wide ? launch_block_norms<__half, float>(p, v, e_values, block, smem, st) : launch_block_norms<__half, __half>(p, v, e_values, block, smem, st);
+    e = wide ? launch_block_norms<__half, float>(p, whole, grouped, held, st) : launch_block_norms<__half, __half>(p, whole, grouped, held, st);
   else
-    e = wide ? launch_block_norms<__nv_bfloat16, float>(p, v, e_values, block, smem, st)
-             : launch_block_norms<__nv_bfloat16, __nv_bfloat16>(p, v, e_values, block, smem, st);
+    e = wide ? launch_block_norms<__nv_bfloat16, float>(p, whole, grouped, held, st)
+             : launch_block_norms<__nv_bfloat16, __nv_bfloat16>(p, whole, grouped, held, st);
   if (e != cudaSuccess) return cuda_fail(e, "block_norms launch");
   return RLDX_OK;
 }
