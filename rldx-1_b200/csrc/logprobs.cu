@@ -23,12 +23,10 @@ namespace rldx {
 namespace {
 constexpr int kLogpTop = 32;        // alternatives at most
 constexpr int kLogpMaxCluster = 8;
-constexpr int kLogpThreads = 256;
 constexpr int kLogpVecs = 8;        // 16-byte vectors of a thread and chunk
-// A list is cut down to k when it is longer than kLogpPrune after a chunk; a chunk adds the values of at most k threads.
-constexpr int kLogpPrune = 256;
-constexpr int kLogpMaxValues = kLogpVecs * 8;  // of a thread and chunk
-constexpr int kLogpList = kLogpPrune + kLogpTop * kLogpMaxValues;
+// A list is cut down to k before it could overflow: a chunk adds the values of at most k threads.
+constexpr int kLogpRoom = kLogpTop * kLogpVecs * 8;
+constexpr int kLogpList = kLogpRoom + 512;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 constexpr float kLogpLeast = -200.0f;  // of d in powers of two: its exponential is 0 all the same, and times it 0 too
 constexpr int kLogpMaxVocab = 1 << 28;
@@ -74,7 +72,8 @@ struct LogprobsShared {
   u64 top[kLogpMaxCluster][kLogpTop];  // rank 0: every CTA's, in order
   u64 stats[kLogpMaxCluster][2];       // rank 0: m, s, t and the count of better tokens of every CTA
   u64 tops[kLogpMaxCluster];           // rank 0: the lengths of the lists
-  float4 warps[kLogpThreads / 32];
+  float4 warps[16];
+  u64 kept[kLogpTop];
   u64 bound;
   int count;
 };
@@ -200,45 +199,41 @@ __device__ __forceinline__ uint32_t reached_by(int need, int top_bit, int low_bi
   return t;
 }
 
-// Cuts the list down to the k best, s.bound the last of them.  Every thread calls it; s.count > k.
+// Cuts the list down to the k best, s.bound the last of them.  Every thread calls it after a barrier; s.count >= k.
+template <int NT>
 __device__ __forceinline__ void prune(LogprobsShared& s, int k) {
-  constexpr int kEach = (kLogpList + kLogpThreads - 1) / kLogpThreads;
   const int n = min(s.count, kLogpList);
-  u64 mine[kEach];
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const int at = threadIdx.x + i * kLogpThreads;
-    mine[i] = at < n ? s.list[at] : 0;
-  }
+  int* sums = reinterpret_cast<int*>(s.warps);
   // keys differ: the k-th largest, bit by bit
   u64 t = 0;
 #pragma unroll 1
   for (int b = 63; b >= 0; --b) {
     const u64 c = t | (1ull << b);
-    int mine_reach = 0;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) mine_reach += mine[i] >= c;
-    // sums of more than one a thread: by warps, then over them
-    mine_reach = __reduce_add_sync(0xffffffffu, mine_reach);
-    int* sums = reinterpret_cast<int*>(s.warps) + (b & 1) * (kLogpThreads / 32);
-    if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = mine_reach;
+    int reach = 0;
+    for (int i = threadIdx.x; i < n; i += NT) reach += s.list[i] >= c;
+    reach = __reduce_add_sync(0xffffffffu, reach);
+    int* at = sums + (b & 1) * (NT / 32);
+    if ((threadIdx.x & 31) == 0) at[threadIdx.x >> 5] = reach;
     __syncthreads();
     int all = 0;
-    for (int w = 0; w < kLogpThreads / 32; ++w) all += sums[w];
+    for (int w = 0; w < NT / 32; ++w) all += at[w];
     if (all >= k) t = c;
   }
+  __syncthreads();
   if (threadIdx.x == 0) s.count = 0, s.bound = t;
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kEach; ++i)
-    if (mine[i] >= t) s.list[atomicAdd(&s.count, 1)] = mine[i];
+  for (int i = threadIdx.x; i < n; i += NT)
+    if (s.list[i] >= t) s.kept[atomicAdd(&s.count, 1)] = s.list[i];
+  __syncthreads();
+  if (static_cast<int>(threadIdx.x) < k) s.list[threadIdx.x] = s.kept[threadIdx.x];
   __syncthreads();
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kLogpThreads, 3) logprobs_kernel(const __grid_constant__ LogprobsParams P) {
+// NT threads a CTA.
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT, 768 / NT) logprobs_kernel(const __grid_constant__ LogprobsParams P) {
   constexpr int kVec = 16 / sizeof(T);
-  constexpr int NT = kLogpThreads, NV = kLogpVecs;
+  constexpr int NV = kLogpVecs;
   __shared__ LogprobsShared s;
   const int cluster = P.cluster;
   const int part = cluster > 1 ? static_cast<int>(cluster_ctarank()) : 0;
@@ -248,7 +243,7 @@ __global__ void __launch_bounds__(kLogpThreads, 3) logprobs_kernel(const __grid_
   griddep_launch();
   const int top = P.top;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (tid == 0) s.count = 0, s.bound = 0;
+  if (tid == 0) s.count = 0;
   const T* logits = static_cast<const T*>(P.logits) + row * P.ld;
   // vectors on 16-byte boundaries, the first and the last in part of other rows
   const int before = static_cast<int>(reinterpret_cast<uintptr_t>(logits) % 16 / sizeof(T));
@@ -257,11 +252,15 @@ __global__ void __launch_bounds__(kLogpThreads, 3) logprobs_kernel(const __grid_
   const int per = (nvec + cluster - 1) / cluster;
   const int v_begin = part * per, v_end = min(nvec, v_begin + per);
 
-  // vector v of this part, -inf in the place of what is not of it
-  auto vec_at = [&](int v) {
+  // vector v of this part, -inf where there is none
+  auto load_vec = [&](int v) {
     constexpr uint32_t low = Logit<T>::kLowest;
     uint4 u = make_uint4(low, low, low, low);
     if (v < v_end) u = __ldcs(vecs + v);
+    return u;
+  };
+  // and -inf in the place of other rows' values
+  auto cut = [&](uint4& u, int v) {
     if (v == 0 || v == nvec - 1) {
       T* e = reinterpret_cast<T*>(&u);
 #pragma unroll
@@ -270,52 +269,57 @@ __global__ void __launch_bounds__(kLogpThreads, 3) logprobs_kernel(const __grid_
         if (id < 0 || id >= P.vocab) e[i] = from_float<T>(-INFINITY);
       }
     }
-    return u;
   };
   uint4 raw[NV];
 #pragma unroll
-  for (int k = 0; k < NV; ++k) raw[k] = vec_at(v_begin + k * NT + tid);
+  for (int k = 0; k < NV; ++k) raw[k] = load_vec(v_begin + k * NT + tid);
 
   const long long token = P.tokens[row];
   const bool given = token >= 0 && token < P.vocab;
   const T t_token = given ? logits[token] : from_float<T>(INFINITY);
   const float x_token = to_float(t_token);
+  // Tokens before the given one: of vectors before its own those at or above it, of the others those above, and those of
+  // its own vector that equal it and come before it.  Where it is -inf, which also fills up vectors, all are looked at.
+  const bool by_one = given && x_token == -INFINITY;
+  const int v_token = given ? static_cast<int>((token + before) / kVec) : 0;
+  const uint32_t above = both(by_one ? from_float<T>(INFINITY) : t_token);
+  const uint32_t at_or_above = both(given && x_token < INFINITY && !by_one ? below(t_token) : from_float<T>(INFINITY));
+  uint32_t better = 0;
+  if (given && !by_one && tid < kVec && part == v_token / per) {
+    const long long id = static_cast<long long>(v_token) * kVec + tid - before;
+    if (id >= 0 && id < token) better = to_float(logits[id]) == x_token;
+  }
 
   Partial p{-FLT_MAX, 0.0f, 0.0f};
   float best = -INFINITY;  // this thread's largest logit so far, where it has seen one
   bool seen = false;
-  uint32_t better = 0;  // tokens before the given one
+  // What can be among the top: values above bound_x, and those that equal it up to bound_id.  The same for every thread.
+  float bound_x = -INFINITY;
+  int bound_id = INT32_MAX;
+  int room = kLogpList;  // in the list, at least
   __syncthreads();
 
 #pragma unroll 1
   for (int base = v_begin; base < v_end; base += NT * NV) {
+    if (base == 0 || base + NT * NV >= nvec)
+#pragma unroll
+      for (int k = 0; k < NV; ++k) cut(raw[k], base + k * NT + tid);
     const float largest = largest_of<T>(raw);
     if (largest > p.m) move_to(p, largest);
-    // tokens before the given one are those above a value, if all of the chunk comes before it or after it; a
-    // chunk that holds it, and -inf, which fills up vectors, are looked at one by one
-    const long long first = static_cast<long long>(base) * kVec - before, last = static_cast<long long>(min(base + NT * NV, v_end)) * kVec - before;
-    T above = t_token;
-    if (x_token == -INFINITY || (token >= first && token < last)) {
-      const long long end = min(token, last);
-      if (given) {
+    if (by_one) {
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-          Raw<T, kVec> r;
-          r.w[0] = raw[k];
-          float x[kVec];
-          unpack_row<T, kVec>(r, x);
+      for (int k = 0; k < NV; ++k) {
+        Raw<T, kVec> r;
+        r.w[0] = raw[k];
+        float x[kVec];
+        unpack_row<T, kVec>(r, x);
 #pragma unroll
-          for (int i = 0; i < kVec; ++i) {
-            const long long id = first + (k * NT + tid) * kVec + i;
-            better += x[i] > x_token || (x[i] == x_token && id >= 0 && id < end);
-          }
+        for (int i = 0; i < kVec; ++i) {
+          const int v = base + k * NT + tid, id = v * kVec + i - before;
+          better += x[i] > -INFINITY || (x[i] == -INFINITY && v < v_end && id >= 0 && id < token);
         }
       }
-      above = from_float<T>(INFINITY);
-    } else if (given && last <= token && x_token < INFINITY && x_token == x_token) {
-      above = below(t_token);
     }
-    const uint32_t above2 = both(above);
     uint32_t count = 0;
     const T* t = nullptr;
     const int next = base + NT * NV + tid;
@@ -332,24 +336,32 @@ __global__ void __launch_bounds__(kLogpThreads, 3) logprobs_kernel(const __grid_
         s2 = add_f32x2(s2, e);
         t2 = fma_f32x2(e, d, t2);
       };
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
+      auto take = [&](int k) {
         const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
-        raw[k] = vec_at(next + k * NT);
+        raw[k] = load_vec(next + k * NT);
+        const uint32_t limit = base + k * NT + tid < v_token ? at_or_above : above;
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
           for (int i = 0; i < 4; i += 2) {
             const float a = __uint_as_float(w[i]), b = __uint_as_float(w[i + 1]);
-            count += a > __uint_as_float(above2), count += b > __uint_as_float(above2);
+            count += a > __uint_as_float(limit), count += b > __uint_as_float(limit);
             add(make_float2(max_nan(a, -1e30f), max_nan(b, -1e30f)));
           }
         } else {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            count2(count, w[i], above2, t);
+            count2(count, w[i], limit, t);
             add(unpack2(max2_nan(w[i], Logit<T>::kFloor, t), t));
           }
         }
+      };
+      if (base + NT * (NV - 1) < v_end) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) take(k);
+      } else {  // a row's last chunk, or its only one
+#pragma unroll
+        for (int k = 0; k < NV - 1; ++k)
+          if (base + k * NT < v_end) take(k);
       }
       const float f = ex2_approx(-rho), sum = f * (s2.x + s2.y);
       p.s += sum;
@@ -358,17 +370,20 @@ __global__ void __launch_bounds__(kLogpThreads, 3) logprobs_kernel(const __grid_
       float sum = 0.0f, sum_d = 0.0f;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        Raw<T, kVec> r;
+        Raw<T, kVec> r, l;
         r.w[0] = raw[k];
-        raw[k] = vec_at(next + k * NT);
-        float x[kVec];
+        raw[k] = load_vec(next + k * NT);
+        const uint32_t limit = base + k * NT + tid < v_token ? at_or_above : above;
+        l.w[0] = make_uint4(limit, limit, limit, limit);
+        float x[kVec], y[kVec];
         unpack_row<T, kVec>(r, x);
+        unpack_row<T, kVec>(l, y);
 #pragma unroll
         for (int i = 0; i < kVec; ++i) {
           const float d = max_nan((x[i] - p.m) * kLog2e, kLogpLeast), e = ex2_approx(d);
           sum += e;
           sum_d = fmaf(e, d, sum_d);
-          better += x[i] > to_float(above);
+          better += x[i] > y[i];
         }
       }
       p.s += sum, p.t += sum_d;
@@ -381,9 +396,6 @@ __global__ void __launch_bounds__(kLogpThreads, 3) logprobs_kernel(const __grid_
     }
 
     if (top == 0) continue;
-    const u64 bound = s.bound;  // 0: none yet
-    const float bound_x = bound ? order_value(static_cast<uint32_t>(bound >> 32)) : -INFINITY;
-    const int bound_id = bound ? static_cast<int>(~static_cast<uint32_t>(bound)) : INT32_MAX;
     const int id0 = (base + tid) * kVec - before;
     const bool here = base + tid < v_end;  // the thread has values in this chunk
     const bool rises = here && (largest > bound_x || (largest == bound_x && id0 <= bound_id));
@@ -393,8 +405,6 @@ __global__ void __launch_bounds__(kLogpThreads, 3) logprobs_kernel(const __grid_
     seen |= here;
     const int rising = __syncthreads_count(rises);
     if (rising == 0) continue;
-    float new_x = bound_x;
-    int new_id = bound_id;
     if (rising > top) {
       // a new bound: the top-th largest of the threads' maxima
       constexpr int low = 32 - Logit<T>::kBits;
@@ -404,8 +414,8 @@ __global__ void __launch_bounds__(kLogpThreads, 3) logprobs_kernel(const __grid_
       const float tx = order_value(reach);
       if (tx >= bound_x) {
         const int higher = __syncthreads_count(bits > reach), tied = __syncthreads_count(bits == reach);
-        new_id = tx > bound_x ? INT32_MAX : bound_id;
-        new_x = tx;
+        if (tx > bound_x) bound_id = INT32_MAX;
+        bound_x = tx;
         if (tied > top - higher) {
           // of those that share the value the lowest ids; one of an earlier chunk counts as lower than any here
           int id = INT32_MAX;
@@ -415,7 +425,7 @@ __global__ void __launch_bounds__(kLogpThreads, 3) logprobs_kernel(const __grid_
 #pragma unroll 1
             for (int k = NV - 1; k >= 0; --k) {
               Raw<T, kVec> r;
-              r.w[0] = vec_at(base + k * NT + tid);
+              r.w[0] = load_vec(base + k * NT + tid);
               float x[kVec];
               unpack_row<T, kVec>(r, x);
 #pragma unroll
@@ -427,12 +437,26 @@ __global__ void __launch_bounds__(kLogpThreads, 3) logprobs_kernel(const __grid_
           }
           const uint32_t order = bits == reach ? static_cast<uint32_t>(INT32_MAX - id) : 0u;
           const uint32_t r = reached_by(top - higher, 30, 0, [&](uint32_t c) { return order >= c; });
-          new_id = min(new_id, INT32_MAX - static_cast<int>(r));
+          bound_id = min(bound_id, INT32_MAX - static_cast<int>(r));
         }
       }
     }
+    // At most `top` threads add values now, whose bound is as good as that of the list's last.
+    const int added = min(rising, top) * NV * kVec;
+    if (room < added) {  // (counted anew, it is more: a thread seldom adds all its values)
+      __syncthreads();
+      const int free = kLogpList - s.count;
+      if (free < added) {
+        prune<NT>(s, top);
+        if (s.bound > key_of(bound_x, bound_id))
+          bound_x = order_value(static_cast<uint32_t>(s.bound >> 32)), bound_id = static_cast<int>(~static_cast<uint32_t>(s.bound));
+      }
+      room = kLogpList - s.count;
+      __syncthreads();
+    }
+    room -= added;
     // what reaches the bound: a warp reads the vectors of four such threads at a time again
-    uint32_t who = __ballot_sync(0xffffffffu, rises && largest >= new_x);
+    uint32_t who = __ballot_sync(0xffffffffu, rises && largest >= bound_x);
     while (who) {
       int mine = -1;
 #pragma unroll
@@ -443,24 +467,19 @@ __global__ void __launch_bounds__(kLogpThreads, 3) logprobs_kernel(const __grid_
       const int v = base + (lane & 7) * NT + warp * 32 + mine;
       if (mine >= 0 && v < v_end) {
         Raw<T, kVec> r;
-        r.w[0] = vec_at(v);
+        r.w[0] = load_vec(v);
         float x[kVec];
         unpack_row<T, kVec>(r, x);
 #pragma unroll
         for (int i = 0; i < kVec; ++i) {
           const int id = v * kVec + i - before;
-          if ((x[i] > new_x || (x[i] == new_x && id <= new_id)) && id >= 0 && id < P.vocab) {
+          if ((x[i] > bound_x || (x[i] == bound_x && id <= bound_id)) && id >= 0 && id < P.vocab) {
             const int at = atomicAdd(&s.count, 1);
             if (at < kLogpList) s.list[at] = key_of(x[i], id);
           }
         }
       }
     }
-    __syncthreads();
-    const int listed = s.count;
-    if (tid == 0 && (new_x != bound_x || new_id != bound_id)) s.bound = key_of(new_x, new_id);
-    __syncthreads();
-    if (listed > kLogpPrune) prune(s, top);
   }
 
   // the part's sums
@@ -470,13 +489,15 @@ __global__ void __launch_bounds__(kLogpThreads, 3) logprobs_kernel(const __grid_
     join(p, q);
   }
   better = __reduce_add_sync(0xffffffffu, better);
+  __syncthreads();
+  if (s.count > NT) prune<NT>(s, top);  // (NT >= 64 > top)
   if (lane == 0) s.warps[warp] = make_float4(p.m, p.s, p.t, __uint_as_float(better));
   __syncthreads();
   // and its list go to rank 0
   if (cluster > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  const int listed = s.count;  // at most kLogpPrune, a thread each
-  if (static_cast<int>(threadIdx.x) < listed) {
-    const u64 mine = s.list[threadIdx.x];
+  const int listed = s.count;  // a thread each
+  if (tid < listed) {
+    const u64 mine = s.list[tid];
     int place = 0;
     for (int i = 0; i < listed; ++i) place += s.list[i] > mine;
     if (place < top) store_to_first(&s.top[part][place], mine, cluster);
@@ -548,11 +569,11 @@ __global__ void __launch_bounds__(kLogpThreads, 3) logprobs_kernel(const __grid_
   }
 }
 
-template <typename T>
+template <typename T, int NT>
 cudaError_t launch_logprobs(const LogprobsParams& p, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(p.rows) * static_cast<unsigned>(p.cluster), 1, 1);
-  cfg.blockDim = dim3(kLogpThreads, 1, 1);
+  cfg.blockDim = dim3(NT, 1, 1);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -562,7 +583,18 @@ cudaError_t launch_logprobs(const LogprobsParams& p, cudaStream_t stream) {
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = p.cluster > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, logprobs_kernel<T>, p);
+  return cudaLaunchKernelEx(&cfg, logprobs_kernel<T, NT>, p);
+}
+template <typename T>
+cudaError_t launch_logprobs(LogprobsParams p, cudaStream_t stream) {
+  // Threads of a CTA: 64, of many small rows to an SM, where they hold one at a time; else 256.  CTAs of a row: as few as
+  // fill the SMs, and none with less than a vector a thread.
+  const long long vecs = static_cast<long long>(p.vocab) * sizeof(T) / 16;
+  const int nt = vecs <= 64 * kLogpVecs ? 64 : 256;
+  p.cluster = 1;
+  while (p.cluster < kLogpMaxCluster && static_cast<long long>(p.rows) * p.cluster * nt < 768LL * sm_count() && vecs / (2 * p.cluster) >= nt)
+    p.cluster *= 2;
+  return nt == 64 ? launch_logprobs<T, 64>(p, stream) : launch_logprobs<T, 256>(p, stream);
 }
 }  // namespace
 
@@ -589,11 +621,6 @@ extern "C" int rldx_token_logprobs(const void* logits, int64_t ld, int rows, int
   p.tokens = reinterpret_cast<const long long*>(tokens);
   p.logprob = logprob, p.entropy = entropy, p.rank = rank;
   p.top_ids = reinterpret_cast<long long*>(top_ids), p.top_logprobs = top_logprobs;
-  // CTAs of a row: as few as fill the SMs, and none with less than a vector a thread
-  const long long vecs = static_cast<long long>(vocab) * dtype_bytes(dtype) / 16;
-  p.cluster = 1;
-  while (p.cluster < kLogpMaxCluster && static_cast<long long>(rows) * p.cluster < 3LL * sm_count() && vecs / (2 * p.cluster) >= kLogpThreads)
-    p.cluster *= 2;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = dtype == RLDX_F32   ? launch_logprobs<float>(p, st)
                         : dtype == RLDX_F16 ? launch_logprobs<__half>(p, st)
