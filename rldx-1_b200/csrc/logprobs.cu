@@ -8,11 +8,13 @@
 // Sums and statistics are fp32, each thread's relative to the largest logit that it has seen; two of them are joined
 // by moving the smaller reference to the larger.
 //
-// A row is shared out among the CTAs of a cluster, each of which goes over its part in chunks of 32 KB that its threads
-// hold in registers.  The top k of a part: the k-th largest of the threads' maxima is a lower bound of the k-th largest
-// value, so what reaches it is a little more than k tokens, and it comes from at most k threads.  Those go to a list in
-// shared memory as (ordered bits of the logit, ~id), whose order is the answer's.  Bounds only rise, and where more
-// threads share the bounding value than are needed the lowest ids decide, so a row of equal logits lists no more.
+// A row is shared out among the CTAs of a cluster, one where rows are many; each goes over its part in chunks that its
+// threads hold in registers, the next one on the way.
+// The top k of a part: every warp keeps a list of (ordered bits of the logit, ~id), whose order is the answer's.  Threads
+// whose maximum of a chunk reaches the bound show their vectors to their warp, which lists what reaches it; a full list is
+// cut down to its k best, and the last of them is a bound.  So is the k-th largest of 64 maxima, each of a few threads, which
+// two warps find after the chunks 0, 1, 3, 7, ... by counting for each how many are larger: some more than k values reach
+// it.  At the end one warp puts in order what the lists hold of those.
 #include <cfloat>
 
 #include "host_util.h"
@@ -24,9 +26,8 @@ namespace {
 constexpr int kLogpTop = 32;        // alternatives at most
 constexpr int kLogpMaxCluster = 8;
 constexpr int kLogpVecs = 8;        // 16-byte vectors of a thread and chunk
-// A list is cut down to k before it could overflow: a chunk adds the values of at most k threads.
-constexpr int kLogpRoom = kLogpTop * kLogpVecs * 8;
-constexpr int kLogpList = kLogpRoom + 512;
+constexpr int kLogpShown = 4;       // threads that show their vectors at a time
+constexpr int kLogpList = 2 * kLogpShown * kLogpVecs * 8;  // of a warp: room for theirs besides what is left of a full one
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 constexpr float kLogpLeast = -200.0f;  // of d in powers of two: its exponential is 0 all the same, and times it 0 too
 constexpr int kLogpMaxVocab = 1 << 28;
@@ -67,15 +68,21 @@ __device__ __forceinline__ void join(Partial& a, Partial b) {
   a.s += b.s, a.t += b.t;
 }
 
+template <int NT>
 struct LogprobsShared {
-  u64 list[kLogpList];
+  static constexpr int kWarps = NT / 32;
+  u64 list[kWarps][kLogpList];
+  uint4 shown[kWarps][kLogpShown * kLogpVecs];
+  int from[kWarps][kLogpShown];
+  int listed[kWarps];
+  uint4 maxima[64 / 4];
+  uint32_t bound[2];  // of a chunk, and of the next one that finds one
+  float4 sums[kWarps];                 // m, s, t and the count of better tokens of each warp
+  u64 front[NT];                       // of the lists, 32 at most of a warp
+  int fronts;
   u64 top[kLogpMaxCluster][kLogpTop];  // rank 0: every CTA's, in order
   u64 stats[kLogpMaxCluster][2];       // rank 0: m, s, t and the count of better tokens of every CTA
-  u64 tops[kLogpMaxCluster];           // rank 0: the lengths of the lists
-  float4 warps[16];
-  u64 kept[kLogpTop];
-  u64 bound;
-  int count;
+  int tops[kLogpMaxCluster][2];        // rank 0: the lengths of the lists
 };
 
 // What differs between the types: a word of -inf, how many leading bits of the fp32 form tell values apart, how far from
@@ -181,131 +188,218 @@ __device__ __forceinline__ u64 key_of(float x, int id) {
 }
 
 __device__ __forceinline__ u64 pair_of(uint32_t lo, uint32_t hi) { return (static_cast<u64>(hi) << 32) | lo; }
-// Writes to the same place of the cluster's first CTA.
-__device__ __forceinline__ void store_to_first(u64* place, u64 v, int cluster) {
-  if (cluster > 1)
-    st_cluster_u64(mapa_shared(smem_u32(place), 0), v);
-  else
-    *place = v;
-}
-
-// The largest t, in bits top_bit to low_bit, that at least `need` of the threads' numbers reach; 0 where there are fewer.
+// The largest t, in bits 31 to `low`, that `need` of the warp's numbers reach (of those there are at least so many).
+// count(c): of a thread's those that reach c.
 template <typename F>
-__device__ __forceinline__ uint32_t reached_by(int need, int top_bit, int low_bit, F reaches) {
+__device__ __forceinline__ uint32_t warp_reached_by(int need, int low, F count) {
   uint32_t t = 0;
 #pragma unroll 1
-  for (int b = top_bit; b >= low_bit; --b)
-    if (__syncthreads_count(reaches(t | (1u << b))) >= need) t |= 1u << b;
+  for (int b = 31; b >= low; --b)
+    if (static_cast<int>(__reduce_add_sync(0xffffffffu, count(t | (1u << b)))) >= need) t |= 1u << b;
   return t;
 }
-
-// Cuts the list down to the k best, s.bound the last of them.  Every thread calls it after a barrier; s.count >= k.
-template <int NT>
-__device__ __forceinline__ void prune(LogprobsShared& s, int k) {
-  const int n = min(s.count, kLogpList);
-  int* sums = reinterpret_cast<int*>(s.warps);
-  // keys differ: the k-th largest, bit by bit
-  u64 t = 0;
-#pragma unroll 1
-  for (int b = 63; b >= 0; --b) {
-    const u64 c = t | (1ull << b);
-    int reach = 0;
-    for (int i = threadIdx.x; i < n; i += NT) reach += s.list[i] >= c;
-    reach = __reduce_add_sync(0xffffffffu, reach);
-    int* at = sums + (b & 1) * (NT / 32);
-    if ((threadIdx.x & 31) == 0) at[threadIdx.x >> 5] = reach;
-    __syncthreads();
-    int all = 0;
-    for (int w = 0; w < NT / 32; ++w) all += at[w];
-    if (all >= k) t = c;
+// Leaves the keys of a warp's list of n that reach `last`, and returns their number.
+__device__ __forceinline__ int warp_keep(u64* list, int n, u64 last) {
+  const int lane = threadIdx.x & 31;
+  int kept = 0;
+  __syncwarp();
+  for (int base = 0; base < n; base += 32) {
+    const u64 key = base + lane < n ? list[base + lane] : 0;
+    const uint32_t keep = __ballot_sync(0xffffffffu, key >= last);  // (every key has been read by now)
+    if (key >= last) list[kept + __popc(keep & ((1u << lane) - 1u))] = key;
+    kept += __popc(keep);
+    __syncwarp();
   }
-  __syncthreads();
-  if (threadIdx.x == 0) s.count = 0, s.bound = t;
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += NT)
-    if (s.list[i] >= t) s.kept[atomicAdd(&s.count, 1)] = s.list[i];
-  __syncthreads();
-  if (static_cast<int>(threadIdx.x) < k) s.list[threadIdx.x] = s.kept[threadIdx.x];
-  __syncthreads();
+  return kept;
+}
+// Cuts a warp's list of n > k keys down to the k best and returns the last of them.  kBits: as Logit's.
+template <int kBits>
+__device__ __noinline__ u64 warp_prune(u64* list, int n, int k) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+  auto count = [&](auto f) {
+    uint32_t c = 0;
+    for (int i = lane; i < n; i += 32) c += f(static_cast<uint32_t>(list[i] >> 32), static_cast<uint32_t>(list[i]));
+    return c;
+  };
+  uint32_t hi = warp_reached_by(k, 32 - kBits, [&](uint32_t c) { return count([c](uint32_t x, uint32_t) { return x >= c; }); });
+  if (kBits < 32 && !(hi >> 31)) hi |= (1u << (32 - kBits)) - 1u;  // (negative values: the bits that the type does not have are ones)
+  const int left = k - static_cast<int>(__reduce_add_sync(0xffffffffu, count([hi](uint32_t x, uint32_t) { return x > hi; })));
+  const uint32_t lo = warp_reached_by(left, 0, [&](uint32_t c) { return count([hi, c](uint32_t x, uint32_t id) { return x == hi && id >= c; }); });
+  const u64 last = pair_of(lo, hi);
+  warp_keep(list, n, last);
+  return last;
+}
+
+// A row whose sum is good has a distribution: no NaN or +inf, and not -inf alone.
+__device__ __forceinline__ bool good_sum(const Partial& p) { return p.s > 0.0f && p.s < INFINITY; }
+template <typename T>
+__device__ __forceinline__ void finish(const LogprobsParams& P, int row, long long token, float x_token, const Partial& p, uint32_t better) {
+  if ((threadIdx.x & 31) != 0) return;
+  const bool good = good_sum(p), given = token >= 0 && token < P.vocab;
+  const float log_s = logf(p.s);
+  if (token >= P.vocab) record_data_error(kErrLogprobsToken);
+  P.logprob[row] = token < 0 ? 0.0f : given && good ? (x_token - p.m) - log_s : NAN;
+  P.rank[row] = given && good ? static_cast<int>(better) : -1;
+  P.entropy[row] = good ? log_s - kLn2 * (p.t / p.s) : NAN;
+}
+__device__ __forceinline__ void write_top(const LogprobsParams& P, int row, int place, u64 key, const Partial& p) {
+  const long long at = static_cast<long long>(row) * P.top + place;
+  const bool good = good_sum(p);
+  P.top_ids[at] = good ? static_cast<long long>(~static_cast<uint32_t>(key)) : -1;
+  P.top_logprobs[at] = good ? (order_value(static_cast<uint32_t>(key >> 32)) - p.m) - logf(p.s) : NAN;
 }
 
 // NT threads a CTA.
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT, 768 / NT) logprobs_kernel(const __grid_constant__ LogprobsParams P) {
   constexpr int kVec = 16 / sizeof(T);
-  constexpr int NV = kLogpVecs;
-  __shared__ LogprobsShared s;
+  constexpr int NV = kLogpVecs, kWarps = NT / 32;
+  __shared__ LogprobsShared<NT> s;
   const int cluster = P.cluster;
   const int part = cluster > 1 ? static_cast<int>(cluster_ctarank()) : 0;
-  const long long row = blockIdx.x / cluster;
   if (cluster > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // (rank 0 runs before it is written to)
   griddep_wait();
   griddep_launch();
   const int top = P.top;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (tid == 0) s.count = 0;
+  const int row = static_cast<int>(blockIdx.x / cluster);
   const T* logits = static_cast<const T*>(P.logits) + row * P.ld;
-  // vectors on 16-byte boundaries, the first and the last in part of other rows
+  // This part of the row: vectors on 16-byte boundaries, the first and the last of the row in part of other rows.
   const int before = static_cast<int>(reinterpret_cast<uintptr_t>(logits) % 16 / sizeof(T));
   const uint4* vecs = reinterpret_cast<const uint4*>(logits - before);
   const int nvec = static_cast<int>((static_cast<long long>(P.vocab) + before + kVec - 1) / kVec);
   const int per = (nvec + cluster - 1) / cluster;
-  const int v_begin = part * per, v_end = min(nvec, v_begin + per);
-
-  // vector v of this part, -inf where there is none
+  const int begin = min(nvec, part * per), end = min(nvec, begin + per);
+  // vector v, -inf where there is none
   auto load_vec = [&](int v) {
     constexpr uint32_t low = Logit<T>::kLowest;
     uint4 u = make_uint4(low, low, low, low);
-    if (v < v_end) u = __ldcs(vecs + v);
+    if (v < end) u = __ldcs(vecs + v);
     return u;
-  };
-  // and -inf in the place of other rows' values
-  auto cut = [&](uint4& u, int v) {
-    if (v == 0 || v == nvec - 1) {
-      T* e = reinterpret_cast<T*>(&u);
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) {
-        const int id = v * kVec + i - before;
-        if (id < 0 || id >= P.vocab) e[i] = from_float<T>(-INFINITY);
-      }
-    }
   };
   uint4 raw[NV];
 #pragma unroll
-  for (int k = 0; k < NV; ++k) raw[k] = load_vec(v_begin + k * NT + tid);
+  for (int k = 0; k < NV; ++k) raw[k] = load_vec(begin + k * NT + tid);
 
+  // Tokens before the given one: of vectors before its own those at or above it, of the others those above, and those of
+  // its own vector that equal it and come before it.  Where it is -inf, which also fills up vectors, all are looked at.
   const long long token = P.tokens[row];
   const bool given = token >= 0 && token < P.vocab;
   const T t_token = given ? logits[token] : from_float<T>(INFINITY);
   const float x_token = to_float(t_token);
-  // Tokens before the given one: of vectors before its own those at or above it, of the others those above, and those of
-  // its own vector that equal it and come before it.  Where it is -inf, which also fills up vectors, all are looked at.
   const bool by_one = given && x_token == -INFINITY;
   const int v_token = given ? static_cast<int>((token + before) / kVec) : 0;
   const uint32_t above = both(by_one ? from_float<T>(INFINITY) : t_token);
   const uint32_t at_or_above = both(given && x_token < INFINITY && !by_one ? below(t_token) : from_float<T>(INFINITY));
   uint32_t better = 0;
-  if (given && !by_one && tid < kVec && part == v_token / per) {
+  if (given && !by_one && tid < kVec && v_token >= begin && v_token < end) {
     const long long id = static_cast<long long>(v_token) * kVec + tid - before;
     if (id >= 0 && id < token) better = to_float(logits[id]) == x_token;
   }
 
+  if (tid == 0) s.fronts = 0;
+  __syncthreads();
   Partial p{-FLT_MAX, 0.0f, 0.0f};
   float best = -INFINITY;  // this thread's largest logit so far, where it has seen one
   bool seen = false;
-  // What can be among the top: values above bound_x, and those that equal it up to bound_id.  The same for every thread.
+  // What can be among the top: values above bound_x, and those that equal it up to bound_id.  The same for a warp's threads.
   float bound_x = -INFINITY;
   int bound_id = INT32_MAX;
-  int room = kLogpList;  // in the list, at least
-  __syncthreads();
+  int listed = 0;  // by this warp
+  int found = 0;   // bounds, by the CTA
 
 #pragma unroll 1
-  for (int base = v_begin; base < v_end; base += NT * NV) {
-    if (base == 0 || base + NT * NV >= nvec)
+  for (int base = begin, chunk = 0; base < end; base += NT * NV, ++chunk) {
+    if (base == 0 || base + NT * NV >= nvec) {  // values of other rows
 #pragma unroll
-      for (int k = 0; k < NV; ++k) cut(raw[k], base + k * NT + tid);
+      for (int k = 0; k < NV; ++k) {
+        const int v = base + k * NT + tid;
+        if (v == 0 || v == nvec - 1) {
+          T* e = reinterpret_cast<T*>(&raw[k]);
+#pragma unroll
+          for (int i = 0; i < kVec; ++i) {
+            const int id = v * kVec + i - before;
+            if (id < 0 || id >= P.vocab) e[i] = from_float<T>(-INFINITY);
+          }
+        }
+      }
+    }
     const float largest = largest_of<T>(raw);
     if (largest > p.m) move_to(p, largest);
+    if (top > 0) {
+      const int id0 = (base + tid) * kVec - before;
+      const bool here = base + tid < end;  // the thread has values in this chunk
+      best = fmaxf(best, largest);
+      seen |= here;
+      if ((chunk & (chunk + 1)) == 0 && end - begin > top) {
+        // a new bound: the top-th largest of 64 maxima, each of NT / 64 threads
+        uint32_t m = seen ? order_bits(best) : 0u;
+        if (NT > 64) {
+          m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+          m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        }
+        uint32_t* maxima = reinterpret_cast<uint32_t*>(s.maxima);
+        if (tid % (NT / 64) == 0) maxima[tid / (NT / 64)] = m;
+        uint32_t* bound = &s.bound[found++ & 1];
+        if (tid == 0) *bound = 0xffffffffu;
+        __syncthreads();
+        if (tid < 64) {
+          const uint32_t mine = maxima[tid];
+          int larger = 0;
+#pragma unroll 4
+          for (int i = 0; i < 16; ++i) {
+            const uint4 u = s.maxima[i];
+            larger += (u.x > mine) + (u.y > mine) + (u.z > mine) + (u.w > mine);
+          }
+          if (larger < top) atomicMin(bound, mine);
+        }
+        __syncthreads();
+        const float x = order_value(*bound);
+        if (x > bound_x) bound_x = x, bound_id = INT32_MAX;
+      }
+      u64* list = s.list[warp];
+      auto who_reach = [&] { return __ballot_sync(0xffffffffu, here && (largest > bound_x || (largest == bound_x && id0 <= bound_id))); };
+      uint32_t who = who_reach();
+      while (who) {
+        if (listed > kLogpList / 2) {
+          const u64 last = warp_prune<Logit<T>::kBits>(list, listed, top);
+          listed = top;
+          if (last > key_of(bound_x, bound_id)) bound_x = order_value(static_cast<uint32_t>(last >> 32)), bound_id = static_cast<int>(~static_cast<uint32_t>(last));
+          who &= who_reach();
+        }
+        // the first few of these threads show their vectors, and every thread looks at one
+        const int slot = __popc(who & ((1u << lane) - 1u));
+        if ((who >> lane & 1u) && slot < kLogpShown) {
+#pragma unroll
+          for (int k = 0; k < NV; ++k) s.shown[warp][slot * NV + k] = raw[k];
+          s.from[warp][slot] = lane;
+        }
+        if (lane == 0) s.listed[warp] = listed;
+        __syncwarp();
+        if (lane / NV < __popc(who)) {
+          Raw<T, kVec> r;
+          r.w[0] = s.shown[warp][lane];
+          const int v = base + (lane % NV) * NT + warp * 32 + s.from[warp][lane / NV];
+          float x[kVec];
+          unpack_row<T, kVec>(r, x);
+          float m = x[0];
+#pragma unroll
+          for (int i = 1; i < kVec; ++i) m = fmaxf(m, x[i]);
+          if (m >= bound_x && v < end) {
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) {
+              const int id = v * kVec + i - before;
+              if (x[i] > bound_x || (x[i] == bound_x && id <= bound_id && id >= 0 && id < P.vocab)) list[atomicAdd(&s.listed[warp], 1)] = key_of(x[i], id);
+            }
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < kLogpShown; ++g) who &= who - 1;
+        __syncwarp();
+        listed = s.listed[warp];
+      }
+    }
     if (by_one) {
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
@@ -316,13 +410,13 @@ __global__ void __launch_bounds__(NT, 768 / NT) logprobs_kernel(const __grid_con
 #pragma unroll
         for (int i = 0; i < kVec; ++i) {
           const int v = base + k * NT + tid, id = v * kVec + i - before;
-          better += x[i] > -INFINITY || (x[i] == -INFINITY && v < v_end && id >= 0 && id < token);
+          better += x[i] > -INFINITY || (x[i] == -INFINITY && v < end && id >= 0 && id < token);
         }
       }
     }
     uint32_t count = 0;
     const T* t = nullptr;
-    const int next = base + NT * NV + tid;
+    const int next = base + NT * NV + tid;  // on the way while this chunk is summed
     if (fabsf(p.m) <= Logit<T>::kNear) {
       // exp2(x log2 e - c) with c = m log2 e rounded: one product a value, and what the rounding left out, rho, is put right
       // for all of the chunk.  Of values so far from the reference that they count as nothing it takes a finite one.
@@ -355,13 +449,13 @@ __global__ void __launch_bounds__(NT, 768 / NT) logprobs_kernel(const __grid_con
           }
         }
       };
-      if (base + NT * (NV - 1) < v_end) {
+      if (base + NT * (NV - 1) < end) {
 #pragma unroll
         for (int k = 0; k < NV; ++k) take(k);
       } else {  // a row's last chunk, or its only one
 #pragma unroll
         for (int k = 0; k < NV - 1; ++k)
-          if (base + k * NT < v_end) take(k);
+          if (base + k * NT < end) take(k);
       }
       const float f = ex2_approx(-rho), sum = f * (s2.x + s2.y);
       p.s += sum;
@@ -394,178 +488,101 @@ __global__ void __launch_bounds__(NT, 768 / NT) logprobs_kernel(const __grid_con
       const float2 n = unpack2(count, t);
       better += static_cast<uint32_t>(n.x + n.y);
     }
-
-    if (top == 0) continue;
-    const int id0 = (base + tid) * kVec - before;
-    const bool here = base + tid < v_end;  // the thread has values in this chunk
-    const bool rises = here && (largest > bound_x || (largest == bound_x && id0 <= bound_id));
-    const bool earlier = seen;
-    const float earlier_best = best;
-    best = fmaxf(best, largest);
-    seen |= here;
-    const int rising = __syncthreads_count(rises);
-    if (rising == 0) continue;
-    if (rising > top) {
-      // a new bound: the top-th largest of the threads' maxima
-      constexpr int low = 32 - Logit<T>::kBits;
-      const uint32_t bits = seen ? order_bits(best) : 0u;
-      uint32_t reach = reached_by(top, 31, low, [&](uint32_t c) { return bits >= c; });
-      if (!(reach >> 31)) reach |= (1u << low) - 1u;  // (negative values: the bits that the type does not have are ones)
-      const float tx = order_value(reach);
-      if (tx >= bound_x) {
-        const int higher = __syncthreads_count(bits > reach), tied = __syncthreads_count(bits == reach);
-        if (tx > bound_x) bound_id = INT32_MAX;
-        bound_x = tx;
-        if (tied > top - higher) {
-          // of those that share the value the lowest ids; one of an earlier chunk counts as lower than any here
-          int id = INT32_MAX;
-          if (earlier && earlier_best == tx) {
-            id = 0;
-          } else if (bits == reach) {
-#pragma unroll 1
-            for (int k = NV - 1; k >= 0; --k) {
-              Raw<T, kVec> r;
-              r.w[0] = load_vec(base + k * NT + tid);
-              float x[kVec];
-              unpack_row<T, kVec>(r, x);
-#pragma unroll
-              for (int i = kVec - 1; i >= 0; --i) {
-                const int at = id0 + k * NT * kVec + i;
-                if (x[i] == tx && base + k * NT + tid < v_end && at >= 0 && at < P.vocab) id = at;
-              }
-            }
-          }
-          const uint32_t order = bits == reach ? static_cast<uint32_t>(INT32_MAX - id) : 0u;
-          const uint32_t r = reached_by(top - higher, 30, 0, [&](uint32_t c) { return order >= c; });
-          bound_id = min(bound_id, INT32_MAX - static_cast<int>(r));
-        }
-      }
-    }
-    // At most `top` threads add values now, whose bound is as good as that of the list's last.
-    const int added = min(rising, top) * NV * kVec;
-    if (room < added) {  // (counted anew, it is more: a thread seldom adds all its values)
-      __syncthreads();
-      const int free = kLogpList - s.count;
-      if (free < added) {
-        prune<NT>(s, top);
-        if (s.bound > key_of(bound_x, bound_id))
-          bound_x = order_value(static_cast<uint32_t>(s.bound >> 32)), bound_id = static_cast<int>(~static_cast<uint32_t>(s.bound));
-      }
-      room = kLogpList - s.count;
-      __syncthreads();
-    }
-    room -= added;
-    // what reaches the bound: a warp reads the vectors of four such threads at a time again
-    uint32_t who = __ballot_sync(0xffffffffu, rises && largest >= bound_x);
-    while (who) {
-      int mine = -1;
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        if (who && lane >> 3 == g) mine = __ffs(who) - 1;
-        who &= who - 1;
-      }
-      const int v = base + (lane & 7) * NT + warp * 32 + mine;
-      if (mine >= 0 && v < v_end) {
-        Raw<T, kVec> r;
-        r.w[0] = load_vec(v);
-        float x[kVec];
-        unpack_row<T, kVec>(r, x);
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-          const int id = v * kVec + i - before;
-          if ((x[i] > bound_x || (x[i] == bound_x && id <= bound_id)) && id >= 0 && id < P.vocab) {
-            const int at = atomicAdd(&s.count, 1);
-            if (at < kLogpList) s.list[at] = key_of(x[i], id);
-          }
-        }
-      }
-    }
   }
 
-  // the part's sums
+  // The warps leave their sums, and of their lists what reaches the bound, 32 at most; one of them goes on with these.
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const Partial q{__shfl_xor_sync(0xffffffffu, p.m, o), __shfl_xor_sync(0xffffffffu, p.s, o), __shfl_xor_sync(0xffffffffu, p.t, o)};
     join(p, q);
   }
   better = __reduce_add_sync(0xffffffffu, better);
-  __syncthreads();
-  if (s.count > NT) prune<NT>(s, top);  // (NT >= 64 > top)
-  if (lane == 0) s.warps[warp] = make_float4(p.m, p.s, p.t, __uint_as_float(better));
-  __syncthreads();
-  // and its list go to rank 0
-  if (cluster > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  const int listed = s.count;  // a thread each
-  if (tid < listed) {
-    const u64 mine = s.list[tid];
-    int place = 0;
-    for (int i = 0; i < listed; ++i) place += s.list[i] > mine;
-    if (place < top) store_to_first(&s.top[part][place], mine, cluster);
+  if (lane == 0) s.sums[warp] = make_float4(p.m, p.s, p.t, __uint_as_float(better));
+  if (listed > 0) {
+    u64* list = s.list[warp];
+    if (listed > 32) listed = warp_keep(list, listed, key_of(bound_x, bound_id));
+    if (listed > 32) {
+      warp_prune<Logit<T>::kBits>(list, listed, top);
+      listed = top;
+    }
+    int at = 0;
+    if (lane == 0) at = atomicAdd(&s.fronts, listed);
+    at = __shfl_sync(0xffffffffu, at, 0);
+    if (lane < listed) s.front[at + lane] = list[lane];
   }
+  if (cluster > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  __syncthreads();
   if (warp == 0) {
-    const float4 w = lane < NT / 32 ? s.warps[lane] : make_float4(-FLT_MAX, 0.0f, 0.0f, 0.0f);
+    const float4 w = lane < kWarps ? s.sums[lane] : make_float4(-FLT_MAX, 0.0f, 0.0f, 0.0f);
     p = Partial{w.x, w.y, w.z};
     better = __float_as_uint(w.w);
 #pragma unroll
-    for (int o = NT / 64; o > 0; o >>= 1) {
+    for (int o = kWarps / 2; o > 0; o >>= 1) {
       const Partial q{__shfl_xor_sync(0xffffffffu, p.m, o), __shfl_xor_sync(0xffffffffu, p.s, o), __shfl_xor_sync(0xffffffffu, p.t, o)};
       join(p, q);
       better += __shfl_xor_sync(0xffffffffu, better, o);
     }
-    if (lane == 0) {
-      store_to_first(&s.stats[part][0], pair_of(__float_as_uint(p.m), __float_as_uint(p.s)), cluster);
-      store_to_first(&s.stats[part][1], pair_of(__float_as_uint(p.t), better), cluster);
-      store_to_first(&s.tops[part], static_cast<u64>(min(listed, top)), cluster);
+    p = Partial{__shfl_sync(0xffffffffu, p.m, 0), __shfl_sync(0xffffffffu, p.s, 0), __shfl_sync(0xffffffffu, p.t, 0)};
+    better = __shfl_sync(0xffffffffu, better, 0);
+    const int front = s.fronts, n = min(front, top);
+    for (int i = lane; i < front; i += 32) {
+      const u64 mine = s.front[i];
+      int place = 0;
+#pragma unroll 8
+      for (int o = 0; o < front; ++o) place += s.front[o] > mine;
+      if (place < top) {
+        if (cluster > 1)
+          st_cluster_u64(mapa_shared(smem_u32(&s.top[part][place]), 0), mine);
+        else
+          s.top[0][place] = mine;
+      }
+    }
+    __syncwarp();
+    if (cluster > 1) {
+      if (lane == 0) {
+        st_cluster_u64(mapa_shared(smem_u32(&s.stats[part][0]), 0), pair_of(__float_as_uint(p.m), __float_as_uint(p.s)));
+        st_cluster_u64(mapa_shared(smem_u32(&s.stats[part][1]), 0), pair_of(__float_as_uint(p.t), better));
+        st_cluster_u64(mapa_shared(smem_u32(&s.tops[part][0]), 0), static_cast<u64>(n));
+      }
+    } else {
+      finish<T>(P, row, token, x_token, p, better);
+      for (int i = lane; i < top; i += 32) write_top(P, row, i, s.top[0][i], p);
     }
   }
-  if (cluster > 1) {
+  if (cluster > 1) {  // (one row a cluster)
     cluster_sync();
     if (part > 0) return;  // nothing is written to another CTA from here on
-  } else {
-    __syncthreads();
-  }
-
-  // every warp joins the parts
-  p = Partial{-FLT_MAX, 0.0f, 0.0f};
-  better = 0;
-  for (int c = 0; c < cluster; ++c) {
-    const u64 a = s.stats[c][0], b = s.stats[c][1];
-    join(p, Partial{__uint_as_float(static_cast<uint32_t>(a)), __uint_as_float(static_cast<uint32_t>(a >> 32)), __uint_as_float(static_cast<uint32_t>(b))});
-    better += static_cast<uint32_t>(b >> 32);
-  }
-  const bool good = p.s > 0.0f && p.s < INFINITY;  // else NaN or +inf is in the row, or nothing but -inf
-  const float log_s = logf(p.s);
-  if (threadIdx.x == 0) {
-    if (token >= P.vocab) record_data_error(kErrLogprobsToken);
-    P.logprob[row] = token < 0 ? 0.0f : given && good ? (x_token - p.m) - log_s : NAN;
-    P.rank[row] = given && good ? static_cast<int>(better) : -1;
-    P.entropy[row] = good ? log_s - kLn2 * (p.t / p.s) : NAN;
-  }
-  for (int e = threadIdx.x; e < cluster * top; e += NT) {
-    const int c = e / top, i = e - c * top;
-    if (!good) {
-      if (c == 0) P.top_ids[row * top + i] = -1, P.top_logprobs[row * top + i] = NAN;
-      continue;
+    if (warp > 0) return;
+    p = Partial{-FLT_MAX, 0.0f, 0.0f};
+    better = 0;
+    for (int c = 0; c < cluster; ++c) {
+      const u64 a = s.stats[c][0], b = s.stats[c][1];
+      join(p, Partial{__uint_as_float(static_cast<uint32_t>(a)), __uint_as_float(static_cast<uint32_t>(a >> 32)), __uint_as_float(static_cast<uint32_t>(b))});
+      better += static_cast<uint32_t>(b >> 32);
     }
-    if (i >= static_cast<int>(s.tops[c])) continue;
-    const u64 mine = s.top[c][i];
-    int place = i;
-    for (int o = 0; o < cluster; ++o) {
-      if (o == c) continue;
-      int lo = 0, hi = static_cast<int>(s.tops[o]);  // the keys of list o before mine
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (s.top[o][mid] > mine)
-          lo = mid + 1;
-        else
-          hi = mid;
+    finish<T>(P, row, token, x_token, p, better);
+    if (!good_sum(p))  // (its lists may be short)
+      for (int i = lane; i < top; i += 32) write_top(P, row, i, 0, p);
+    for (int e = lane; good_sum(p) && e < cluster * top; e += 32) {
+      const int c = e / top, i = e - c * top;
+      if (i >= s.tops[c][0]) continue;
+      const u64 mine = s.top[c][i];
+      int place = i;
+      for (int o = 0; o < cluster; ++o) {
+        if (o == c) continue;
+        int lo = 0, hi = s.tops[o][0];  // the keys of list o before mine
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          if (s.top[o][mid] > mine)
+            lo = mid + 1;
+          else
+            hi = mid;
+        }
+        place += lo;
       }
-      place += lo;
+      if (place < top) write_top(P, row, place, mine, p);
     }
-    if (place < top) {
-      P.top_ids[row * top + place] = static_cast<long long>(~static_cast<uint32_t>(mine));
-      P.top_logprobs[row * top + place] = (order_value(static_cast<uint32_t>(mine >> 32)) - p.m) - log_s;
-    }
+    return;
   }
 }
 
