@@ -24,7 +24,7 @@ namespace rldx {
 
 namespace {
 constexpr int kLogpTop = 32;        // alternatives at most
-constexpr int kLogpMaxCluster = 8;
+constexpr int kLogpMaxCluster = 16;
 constexpr int kLogpVecs = 8;        // 16-byte vectors of a thread and chunk
 constexpr int kLogpShown = 4;       // threads that show their vectors at a time
 constexpr int kLogpList = 2 * kLogpShown * kLogpVecs * 8;  // of a warp: room for theirs besides what is left of a full one
@@ -61,11 +61,31 @@ __device__ __forceinline__ void move_to(Partial& p, float m) {
   p.s *= f;
   p.m = m;
 }
-__device__ __forceinline__ void join(Partial& a, Partial b) {
-  const float m = fmaxf(a.m, b.m);
-  move_to(a, m);
-  move_to(b, m);
-  a.s += b.s, a.t += b.t;
+// The sums of a warp's threads, and of their counts.  (Called for a warp, a CTA and a cluster: code that runs once a row
+// waits for its instructions more than for anything else, so there is one copy of it.)
+struct Total {
+  Partial p;
+  uint32_t better;
+};
+__device__ __noinline__ Total warp_total(Total x) {
+  move_to(x.p, order_value(__reduce_max_sync(0xffffffffu, order_bits(x.p.m))));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x.p.s += __shfl_xor_sync(0xffffffffu, x.p.s, o), x.p.t += __shfl_xor_sync(0xffffffffu, x.p.t, o);
+  x.better = __reduce_add_sync(0xffffffffu, x.better);
+  return x;
+}
+__device__ __forceinline__ uint4 words_of(const Total& x) {
+  return make_uint4(__float_as_uint(x.p.m), __float_as_uint(x.p.s), __float_as_uint(x.p.t), x.better);
+}
+// The total of n of them in shared memory, for every thread of the warp that asks.
+__device__ __forceinline__ Total total_of(const uint4* words, int n) {
+  const int lane = threadIdx.x & 31;
+  Total x{{-FLT_MAX, 0.0f, 0.0f}, 0};
+  if (lane < n) {
+    const uint4 w = words[lane];
+    x = {{__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z)}, w.w};
+  }
+  return warp_total(x);
 }
 
 template <int NT>
@@ -77,12 +97,16 @@ struct LogprobsShared {
   int listed[kWarps];
   uint4 maxima[64 / 4];
   uint32_t bound[2];  // of a chunk, and of the next one that finds one
-  float4 sums[kWarps];                 // m, s, t and the count of better tokens of each warp
-  u64 front[NT];                       // of the lists, 32 at most of a warp
-  int fronts;
-  u64 top[kLogpMaxCluster][kLogpTop];  // rank 0: every CTA's, in order
-  u64 stats[kLogpMaxCluster][2];       // rank 0: m, s, t and the count of better tokens of every CTA
-  int tops[kLogpMaxCluster][2];        // rank 0: the lengths of the lists
+  uint4 totals[kWarps];                   // of the warps
+  u64 front[NT];                          // of the lists, 32 at most of a warp
+  int fronts, finalists;
+  long long token;
+  float x_token;
+  // rank 0's, of every CTA: the keys that it sends, their number and its bound, its totals
+  u64 sent[kLogpMaxCluster * kLogpTop];
+  uint2 sent_n[kLogpMaxCluster];
+  uint4 sent_totals[kLogpMaxCluster];
+  u64 final[kLogpMaxCluster * kLogpTop];  // those that reach every CTA's bound
 };
 
 // What differs between the types: a word of -inf, how many leading bits of the fp32 form tell values apart, how far from
@@ -233,21 +257,34 @@ __device__ __noinline__ u64 warp_prune(u64* list, int n, int k) {
 
 // A row whose sum is good has a distribution: no NaN or +inf, and not -inf alone.
 __device__ __forceinline__ bool good_sum(const Partial& p) { return p.s > 0.0f && p.s < INFINITY; }
-template <typename T>
-__device__ __forceinline__ void finish(const LogprobsParams& P, int row, long long token, float x_token, const Partial& p, uint32_t better) {
-  if ((threadIdx.x & 31) != 0) return;
-  const bool good = good_sum(p), given = token >= 0 && token < P.vocab;
-  const float log_s = logf(p.s);
+__device__ __forceinline__ void finish(const LogprobsParams& P, int row, long long token, float x_token, const Total& x) {
+  const bool good = good_sum(x.p), given = token >= 0 && token < P.vocab;
+  const float log_s = logf(x.p.s);
   if (token >= P.vocab) record_data_error(kErrLogprobsToken);
-  P.logprob[row] = token < 0 ? 0.0f : given && good ? (x_token - p.m) - log_s : NAN;
-  P.rank[row] = given && good ? static_cast<int>(better) : -1;
-  P.entropy[row] = good ? log_s - kLn2 * (p.t / p.s) : NAN;
+  P.logprob[row] = token < 0 ? 0.0f : given && good ? (x_token - x.p.m) - log_s : NAN;
+  P.rank[row] = given && good ? static_cast<int>(x.better) : -1;
+  P.entropy[row] = good ? log_s - kLn2 * (x.p.t / x.p.s) : NAN;
 }
-__device__ __forceinline__ void write_top(const LogprobsParams& P, int row, int place, u64 key, const Partial& p) {
-  const long long at = static_cast<long long>(row) * P.top + place;
-  const bool good = good_sum(p);
-  P.top_ids[at] = good ? static_cast<long long>(~static_cast<uint32_t>(key)) : -1;
-  P.top_logprobs[at] = good ? (order_value(static_cast<uint32_t>(key >> 32)) - p.m) - logf(p.s) : NAN;
+// How many of n keys are larger.
+__device__ __noinline__ int place_of(const u64* keys, int n, u64 key) {
+  int place = 0;
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) place += keys[i] > key;
+  return place;
+}
+// Writes key i of n, among them the row's top, to its place.  A row without a distribution may have fewer.
+__device__ __forceinline__ void write_top(const LogprobsParams& P, int row, const u64* keys, int n, int i, const Total& x) {
+  const long long at = static_cast<long long>(row) * P.top;
+  if (!good_sum(x.p)) {
+    if (i == 0)
+      for (int k = 0; k < P.top; ++k) P.top_ids[at + k] = -1, P.top_logprobs[at + k] = NAN;
+    return;
+  }
+  if (i >= n) return;
+  const int place = place_of(keys, n, keys[i]);
+  if (place >= P.top) return;
+  P.top_ids[at + place] = static_cast<long long>(~static_cast<uint32_t>(keys[i]));
+  P.top_logprobs[at + place] = (order_value(static_cast<uint32_t>(keys[i] >> 32)) - x.p.m) - logf(x.p.s);
 }
 
 // NT threads a CTA.
@@ -298,7 +335,7 @@ __global__ void __launch_bounds__(NT, 768 / NT) logprobs_kernel(const __grid_con
     if (id >= 0 && id < token) better = to_float(logits[id]) == x_token;
   }
 
-  if (tid == 0) s.fronts = 0;
+  if (tid == 0) s.fronts = 0, s.token = token, s.x_token = x_token;
   __syncthreads();
   Partial p{-FLT_MAX, 0.0f, 0.0f};
   float best = -INFINITY;  // this thread's largest logit so far, where it has seen one
@@ -335,10 +372,8 @@ __global__ void __launch_bounds__(NT, 768 / NT) logprobs_kernel(const __grid_con
       if ((chunk & (chunk + 1)) == 0 && end - begin > top) {
         // a new bound: the top-th largest of 64 maxima, each of NT / 64 threads
         uint32_t m = seen ? order_bits(best) : 0u;
-        if (NT > 64) {
-          m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-          m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        }
+#pragma unroll
+        for (int o = 1; o < NT / 64; o *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
         uint32_t* maxima = reinterpret_cast<uint32_t*>(s.maxima);
         if (tid % (NT / 64) == 0) maxima[tid / (NT / 64)] = m;
         uint32_t* bound = &s.bound[found++ & 1];
@@ -352,7 +387,8 @@ __global__ void __launch_bounds__(NT, 768 / NT) logprobs_kernel(const __grid_con
             const uint4 u = s.maxima[i];
             larger += (u.x > mine) + (u.y > mine) + (u.z > mine) + (u.w > mine);
           }
-          if (larger < top) atomicMin(bound, mine);
+          const uint32_t least = __reduce_min_sync(0xffffffffu, larger < top ? mine : 0xffffffffu);
+          if (lane == 0) atomicMin(bound, least);
         }
         __syncthreads();
         const float x = order_value(*bound);
@@ -422,13 +458,12 @@ __global__ void __launch_bounds__(NT, 768 / NT) logprobs_kernel(const __grid_con
       // for all of the chunk.  Of values so far from the reference that they count as nothing it takes a finite one.
       const float c = p.m * kLog2e;
       const float rho = fmaf(p.m, kLog2e, -c);
-      const float2 l2 = make_float2(kLog2e, kLog2e), c2 = make_float2(-c, -c);
-      float2 s2 = make_float2(0.0f, 0.0f), t2 = s2;
-      auto add = [&](float2 x) {
-        const float2 d = fma_f32x2(x, l2, c2);
-        const float2 e = make_float2(ex2_approx(d.x), ex2_approx(d.y));
-        s2 = add_f32x2(s2, e);
-        t2 = fma_f32x2(e, d, t2);
+      // (one value at a time: packed pairs took 140 us where this takes 126, 2208 rows of 151680 without alternatives)
+      float sum0 = 0.0f, sum1 = 0.0f, dot0 = 0.0f, dot1 = 0.0f;
+      auto add = [&](float x, float& sum, float& dot) {
+        const float d = fmaf(x, kLog2e, -c), e = ex2_approx(d);
+        sum += e;
+        dot = fmaf(e, d, dot);
       };
       auto take = [&](int k) {
         const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
@@ -439,13 +474,16 @@ __global__ void __launch_bounds__(NT, 768 / NT) logprobs_kernel(const __grid_con
           for (int i = 0; i < 4; i += 2) {
             const float a = __uint_as_float(w[i]), b = __uint_as_float(w[i + 1]);
             count += a > __uint_as_float(limit), count += b > __uint_as_float(limit);
-            add(make_float2(max_nan(a, -1e30f), max_nan(b, -1e30f)));
+            add(max_nan(a, -1e30f), sum0, dot0);
+            add(max_nan(b, -1e30f), sum1, dot1);
           }
         } else {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             count2(count, w[i], limit, t);
-            add(unpack2(max2_nan(w[i], Logit<T>::kFloor, t), t));
+            const float2 x = unpack2(max2_nan(w[i], Logit<T>::kFloor, t), t);
+            add(x.x, sum0, dot0);
+            add(x.y, sum1, dot1);
           }
         }
       };
@@ -457,9 +495,9 @@ __global__ void __launch_bounds__(NT, 768 / NT) logprobs_kernel(const __grid_con
         for (int k = 0; k < NV - 1; ++k)
           if (base + k * NT < end) take(k);
       }
-      const float f = ex2_approx(-rho), sum = f * (s2.x + s2.y);
+      const float f = ex2_approx(-rho), sum = f * (sum0 + sum1);
       p.s += sum;
-      p.t += fmaf(-rho, sum, f * (t2.x + t2.y));
+      p.t += fmaf(-rho, sum, f * (dot0 + dot1));
     } else {
       float sum = 0.0f, sum_d = 0.0f;
 #pragma unroll
@@ -490,14 +528,9 @@ __global__ void __launch_bounds__(NT, 768 / NT) logprobs_kernel(const __grid_con
     }
   }
 
-  // The warps leave their sums, and of their lists what reaches the bound, 32 at most; one of them goes on with these.
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const Partial q{__shfl_xor_sync(0xffffffffu, p.m, o), __shfl_xor_sync(0xffffffffu, p.s, o), __shfl_xor_sync(0xffffffffu, p.t, o)};
-    join(p, q);
-  }
-  better = __reduce_add_sync(0xffffffffu, better);
-  if (lane == 0) s.sums[warp] = make_float4(p.m, p.s, p.t, __uint_as_float(better));
+  // The warps leave their totals, and of their lists what reaches the bound, 32 at most.
+  const Total mine = warp_total({p, better});
+  if (lane == 0) s.totals[warp] = words_of(mine);
   if (listed > 0) {
     u64* list = s.list[warp];
     if (listed > 32) listed = warp_keep(list, listed, key_of(bound_x, bound_id));
@@ -512,78 +545,37 @@ __global__ void __launch_bounds__(NT, 768 / NT) logprobs_kernel(const __grid_con
   }
   if (cluster > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   __syncthreads();
-  if (warp == 0) {
-    const float4 w = lane < kWarps ? s.sums[lane] : make_float4(-FLT_MAX, 0.0f, 0.0f, 0.0f);
-    p = Partial{w.x, w.y, w.z};
-    better = __float_as_uint(w.w);
-#pragma unroll
-    for (int o = kWarps / 2; o > 0; o >>= 1) {
-      const Partial q{__shfl_xor_sync(0xffffffffu, p.m, o), __shfl_xor_sync(0xffffffffu, p.s, o), __shfl_xor_sync(0xffffffffu, p.t, o)};
-      join(p, q);
-      better += __shfl_xor_sync(0xffffffffu, better, o);
-    }
-    p = Partial{__shfl_sync(0xffffffffu, p.m, 0), __shfl_sync(0xffffffffu, p.s, 0), __shfl_sync(0xffffffffu, p.t, 0)};
-    better = __shfl_sync(0xffffffffu, better, 0);
-    const int front = s.fronts, n = min(front, top);
-    for (int i = lane; i < front; i += 32) {
-      const u64 mine = s.front[i];
-      int place = 0;
-#pragma unroll 8
-      for (int o = 0; o < front; ++o) place += s.front[o] > mine;
-      if (place < top) {
-        if (cluster > 1)
-          st_cluster_u64(mapa_shared(smem_u32(&s.top[part][place]), 0), mine);
-        else
-          s.top[0][place] = mine;
-      }
-    }
-    __syncwarp();
-    if (cluster > 1) {
-      if (lane == 0) {
-        st_cluster_u64(mapa_shared(smem_u32(&s.stats[part][0]), 0), pair_of(__float_as_uint(p.m), __float_as_uint(p.s)));
-        st_cluster_u64(mapa_shared(smem_u32(&s.stats[part][1]), 0), pair_of(__float_as_uint(p.t), better));
-        st_cluster_u64(mapa_shared(smem_u32(&s.tops[part][0]), 0), static_cast<u64>(n));
-      }
-    } else {
-      finish<T>(P, row, token, x_token, p, better);
-      for (int i = lane; i < top; i += 32) write_top(P, row, i, s.top[0][i], p);
-    }
-  }
-  if (cluster > 1) {  // (one row a cluster)
-    cluster_sync();
-    if (part > 0) return;  // nothing is written to another CTA from here on
-    if (warp > 0) return;
-    p = Partial{-FLT_MAX, 0.0f, 0.0f};
-    better = 0;
-    for (int c = 0; c < cluster; ++c) {
-      const u64 a = s.stats[c][0], b = s.stats[c][1];
-      join(p, Partial{__uint_as_float(static_cast<uint32_t>(a)), __uint_as_float(static_cast<uint32_t>(a >> 32)), __uint_as_float(static_cast<uint32_t>(b))});
-      better += static_cast<uint32_t>(b >> 32);
-    }
-    finish<T>(P, row, token, x_token, p, better);
-    if (!good_sum(p))  // (its lists may be short)
-      for (int i = lane; i < top; i += 32) write_top(P, row, i, 0, p);
-    for (int e = lane; good_sum(p) && e < cluster * top; e += 32) {
-      const int c = e / top, i = e - c * top;
-      if (i >= s.tops[c][0]) continue;
-      const u64 mine = s.top[c][i];
-      int place = i;
-      for (int o = 0; o < cluster; ++o) {
-        if (o == c) continue;
-        int lo = 0, hi = s.tops[o][0];  // the keys of list o before mine
-        while (lo < hi) {
-          const int mid = (lo + hi) >> 1;
-          if (s.top[o][mid] > mine)
-            lo = mid + 1;
-          else
-            hi = mid;
-        }
-        place += lo;
-      }
-      if (place < top) write_top(P, row, place, mine, p);
-    }
+  const Total total = total_of(s.totals, kWarps);
+  const int fronts = s.fronts;
+  if (cluster == 1) {
+    if (tid == 0) finish(P, row, s.token, s.x_token, total);
+    write_top(P, row, s.front, fronts, tid, total);
     return;
   }
+  // Rank 0 gets up to 32 keys of every CTA: all, or where they are more the top ones.
+  if (tid < fronts) {
+    const u64 key = s.front[tid];
+    const int place = fronts > kLogpTop ? place_of(s.front, fronts, key) : tid;
+    if (place < kLogpTop) st_cluster_u64(mapa_shared(smem_u32(&s.sent[part * kLogpTop + place]), 0), key);
+  }
+  if (tid == 0) {
+    const uint4 w = words_of(total);
+    st_cluster_u64(mapa_shared(smem_u32(&s.sent_totals[part]), 0), pair_of(w.x, w.y));
+    st_cluster_u64(mapa_shared(smem_u32(&s.sent_totals[part]) + 8, 0), pair_of(w.z, w.w));
+    st_cluster_u64(mapa_shared(smem_u32(&s.sent_n[part]), 0), pair_of(min(fronts, kLogpTop), found ? s.bound[(found - 1) & 1] : 0u));
+    s.finalists = 0;
+  }
+  cluster_sync();
+  if (part > 0) return;  // nothing is written to another CTA from here on
+  const Total row_total = total_of(s.sent_totals, cluster);
+  if (tid == 0) finish(P, row, s.token, s.x_token, row_total);
+  const uint2 mine_n = lane < cluster ? s.sent_n[lane] : make_uint2(0, 0);
+  const uint32_t row_bound = __reduce_max_sync(0xffffffffu, mine_n.y);
+  for (int e = tid; e < cluster * kLogpTop; e += NT)
+    if (e % kLogpTop < static_cast<int>(s.sent_n[e / kLogpTop].x) && static_cast<uint32_t>(s.sent[e] >> 32) >= row_bound)
+      s.final[atomicAdd(&s.finalists, 1)] = s.sent[e];
+  __syncthreads();
+  for (int e = tid; e < max(s.finalists, 1); e += NT) write_top(P, row, s.final, s.finalists, e, row_total);
 }
 
 template <typename T, int NT>
@@ -602,6 +594,10 @@ cudaError_t launch_logprobs(const LogprobsParams& p, cudaStream_t stream) {
   cfg.numAttrs = p.cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, logprobs_kernel<T, NT>, p);
 }
+template <typename T, int NT>
+cudaError_t logprobs_clusters() {
+  return cudaFuncSetAttribute(logprobs_kernel<T, NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+}
 template <typename T>
 cudaError_t launch_logprobs(LogprobsParams p, cudaStream_t stream) {
   // Threads of a CTA: 64, of many small rows to an SM, where they hold one at a time; else 256.  CTAs of a row: as few as
@@ -609,11 +605,18 @@ cudaError_t launch_logprobs(LogprobsParams p, cudaStream_t stream) {
   const long long vecs = static_cast<long long>(p.vocab) * sizeof(T) / 16;
   const int nt = vecs <= 64 * kLogpVecs ? 64 : 256;
   p.cluster = 1;
-  while (p.cluster < kLogpMaxCluster && static_cast<long long>(p.rows) * p.cluster * nt < 768LL * sm_count() && vecs / (2 * p.cluster) >= nt)
+  while (p.cluster < (nt == 64 ? 8 : kLogpMaxCluster) && static_cast<long long>(p.rows) * p.cluster * nt < 768LL * sm_count() && vecs / (2 * p.cluster) >= nt)
     p.cluster *= 2;
   return nt == 64 ? launch_logprobs<T, 64>(p, stream) : launch_logprobs<T, 256>(p, stream);
 }
 }  // namespace
+
+cudaError_t logprobs_prepare_device() {
+  cudaError_t e = logprobs_clusters<__nv_bfloat16, 256>();
+  if (e == cudaSuccess) e = logprobs_clusters<__half, 256>();
+  if (e == cudaSuccess) e = logprobs_clusters<float, 256>();
+  return e;
+}
 
 }  // namespace rldx
 
