@@ -10,11 +10,13 @@
 //
 // A row is shared out among the CTAs of a cluster, one where rows are many; each goes over its part in chunks that its
 // threads hold in registers, the next one on the way.
-// The top k of a part: every warp keeps a list of (ordered bits of the logit, ~id), whose order is the answer's.  Threads
-// whose maximum of a chunk reaches the bound show their vectors to their warp, which lists what reaches it; a full list is
-// cut down to its k best, and the last of them is a bound.  So is the k-th largest of 64 maxima, each of a few threads, which
-// two warps find after the chunks 0, 1, 3, 7, ... by counting for each how many are larger: some more than k values reach
-// it.  At the end one warp puts in order what the lists hold of those.
+// The top k of a part: after the chunks 0, 1, 3, 7, ... the k-th largest of 64 maxima, each of a few threads', is a bound
+// that some more than k values reach (two warps find it by counting for each how many are larger).  Threads whose maximum
+// of a chunk reaches it queue the vectors that do; at the end the queue's values that reach the last bound are put in order
+// as (ordered bits of the logit, ~id), whose order is the answer's.  -inf is never queued: where fewer than k
+// other values are in a row, the missing places go to the lowest ids of -inf.  A queue that overflows (many values share the
+// bound, or logits rise along the row) is given up for lists of the warps that are cut down to k when they are full:
+// exact whatever the row, and some times slower.
 #include <cfloat>
 
 #include "host_util.h"
@@ -26,7 +28,8 @@ namespace {
 constexpr int kLogpTop = 32;        // alternatives at most
 constexpr int kLogpMaxCluster = 16;
 constexpr int kLogpVecs = 8;        // 16-byte vectors of a thread and chunk
-constexpr int kLogpShown = 4;       // threads that show their vectors at a time
+constexpr int kLogpQueue = 512;     // vectors of a CTA
+constexpr int kLogpShown = 4;       // threads that show their vectors to their warp at a time
 constexpr int kLogpList = 2 * kLogpShown * kLogpVecs * 8;  // of a warp: room for theirs besides what is left of a full one
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 constexpr float kLogpLeast = -200.0f;  // of d in powers of two: its exponential is 0 all the same, and times it 0 too
@@ -91,15 +94,23 @@ __device__ __forceinline__ Total total_of(const uint4* words, int n) {
 template <int NT>
 struct LogprobsShared {
   static constexpr int kWarps = NT / 32;
-  u64 list[kWarps][kLogpList];
-  uint4 shown[kWarps][kLogpShown * kLogpVecs];
-  int from[kWarps][kLogpShown];
-  int listed[kWarps];
+  union {
+    struct {
+      uint4 queue[kLogpQueue];
+      int queue_at[kLogpQueue];  // their places in the row
+    };
+    struct {  // where the queue is not enough
+      u64 list[kWarps][kLogpList];
+      uint4 shown[kWarps][kLogpShown * kLogpVecs];
+      int from[kWarps][kLogpShown];
+      int listed[kWarps];
+    };
+  };
   uint4 maxima[64 / 4];
-  uint32_t bound[2];  // of a chunk, and of the next one that finds one
-  uint4 totals[kWarps];                   // of the warps
-  u64 front[NT];                          // of the lists, 32 at most of a warp
-  int fronts, finalists;
+  uint32_t bound[2];      // of a chunk, and of the next one that finds one
+  uint4 totals[kWarps];   // of the warps
+  u64 front[NT];          // keys that can be among the top
+  int queued, fronts, finalists;
   long long token;
   float x_token;
   // rank 0's, of every CTA: the keys that it sends, their number and its bound, its totals
@@ -158,12 +169,9 @@ __device__ __forceinline__ float2 unpack2(uint32_t w, const __nv_bfloat16*) {
   return x;
 }
 __device__ __forceinline__ float2 unpack2(uint32_t w, const __half*) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
-// Ones where a > b, added up in halves of a word (whole numbers up to 256 there).
-__device__ __forceinline__ void count2(uint32_t& n, uint32_t a, uint32_t b, const __nv_bfloat16*) {
-  const __nv_bfloat162 r = __hadd2(*reinterpret_cast<__nv_bfloat162*>(&n), __hgt2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b)));
-  n = *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ void count2(uint32_t& n, uint32_t a, uint32_t b, const __half*) {
+// Ones where a > b, added up in fp16 in halves of a word (whole numbers up to 2048 there).  bf16 patterns are compared as
+// fp16 ones, whose order is the same up to 2^121 (2208 rows of 151680: 175 us, with bf16 comparisons 184).
+__device__ __forceinline__ void count2(uint32_t& n, uint32_t a, uint32_t b) {
   const __half2 r = __hadd2(*reinterpret_cast<__half2*>(&n), __hgt2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b)));
   n = *reinterpret_cast<const uint32_t*>(&r);
 }
@@ -190,12 +198,21 @@ __device__ __forceinline__ uint32_t both(T x) {
 
 // The largest of a vector (NaN gives way).
 template <typename T>
+__device__ __forceinline__ float largest_of(const uint4& u) {
+  if constexpr (sizeof(T) == 4) {
+    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+  } else {
+    const T* t = nullptr;
+    const float2 x = unpack2(max2(max2(u.x, u.y, t), max2(u.z, u.w, t), t), t);
+    return fmaxf(x.x, x.y);
+  }
+}
+template <typename T>
 __device__ __forceinline__ float largest_of(const uint4 (&raw)[kLogpVecs]) {
   if constexpr (sizeof(T) == 4) {
     float m = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < kLogpVecs; ++k)
-      m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(raw[k].x), __uint_as_float(raw[k].y)), fmaxf(__uint_as_float(raw[k].z), __uint_as_float(raw[k].w))));
+    for (int k = 0; k < kLogpVecs; ++k) m = fmaxf(m, largest_of<T>(raw[k]));
     return m;
   } else {
     const T* t = nullptr;
@@ -205,6 +222,14 @@ __device__ __forceinline__ float largest_of(const uint4 (&raw)[kLogpVecs]) {
     const float2 x = unpack2(m, t);
     return fmaxf(x.x, x.y);
   }
+}
+// -inf in the place of other rows' values; the vector's ids count from `id0`.
+template <typename T>
+__device__ __forceinline__ void cut_vec(uint4& u, int id0, int vocab) {
+  T* e = reinterpret_cast<T*>(&u);
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(16 / sizeof(T)); ++i)
+    if (id0 + i < 0 || id0 + i >= vocab) e[i] = from_float<T>(-INFINITY);
 }
 
 __device__ __forceinline__ u64 key_of(float x, int id) {
@@ -255,6 +280,81 @@ __device__ __noinline__ u64 warp_prune(u64* list, int n, int k) {
   return last;
 }
 
+// Fills s.front with 32 keys at most of every warp, the part's top ones among them, whatever the row: the way of a queue that
+// overflowed.  Every thread calls it.  bound_x: a value that they reach.
+template <typename T, int NT>
+__device__ __noinline__ void list_part(LogprobsShared<NT>& s, int vocab, int top, const uint4* vecs, int before, int begin, int end, int nvec,
+                                       float bound_x) {
+  constexpr int kVec = 16 / sizeof(T), NV = kLogpVecs;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  __syncthreads();  // the queue and the count are done with
+  if (tid == 0) s.fronts = 0;
+  int bound_id = INT32_MAX;  // values that equal bound_x count up to this id
+  int listed = 0;
+  u64* list = s.list[warp];
+#pragma unroll 1
+  for (int base = begin; base < end; base += NT * NV) {
+    uint4 raw[NV];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int v = base + k * NT + tid;
+      constexpr uint32_t low = Logit<T>::kLowest;
+      raw[k] = v < end ? vecs[v] : make_uint4(low, low, low, low);
+      if (v == 0 || v == nvec - 1) cut_vec<T>(raw[k], v * kVec - before, vocab);
+    }
+    float largest = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) largest = fmaxf(largest, largest_of<T>(raw[k]));
+    const int id0 = (base + tid) * kVec - before;
+    auto who_reach = [&] {
+      return __ballot_sync(0xffffffffu, largest > -INFINITY && (largest > bound_x || (largest == bound_x && id0 <= bound_id)));
+    };
+    uint32_t who = who_reach();
+    while (who) {
+      if (listed > kLogpList / 2) {
+        const u64 last = warp_prune<Logit<T>::kBits>(list, listed, top);
+        listed = top;
+        if (last > key_of(bound_x, bound_id)) bound_x = order_value(static_cast<uint32_t>(last >> 32)), bound_id = static_cast<int>(~static_cast<uint32_t>(last));
+        who &= who_reach();
+      }
+      // the first few of these threads show their vectors, and every thread looks at one
+      const int slot = __popc(who & ((1u << lane) - 1u));
+      if ((who >> lane & 1u) && slot < kLogpShown) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) s.shown[warp][slot * NV + k] = raw[k];
+        s.from[warp][slot] = lane;
+      }
+      if (lane == 0) s.listed[warp] = listed;
+      __syncwarp();
+      if (lane / NV < __popc(who)) {
+        Raw<T, kVec> r;
+        r.w[0] = s.shown[warp][lane];
+        const int v = base + (lane % NV) * NT + warp * 32 + s.from[warp][lane / NV];
+        float x[kVec];
+        unpack_row<T, kVec>(r, x);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+          const int id = v * kVec + i - before;
+          if (x[i] > -INFINITY && (x[i] > bound_x || (x[i] == bound_x && id <= bound_id))) list[atomicAdd(&s.listed[warp], 1)] = key_of(x[i], id);
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < kLogpShown; ++g) who &= who - 1;
+      __syncwarp();
+      listed = s.listed[warp];
+    }
+  }
+  if (listed > 32) {
+    warp_prune<Logit<T>::kBits>(list, listed, top);
+    listed = top;
+  }
+  __syncthreads();
+  int at = 0;
+  if (lane == 0) at = atomicAdd(&s.fronts, listed);
+  at = __shfl_sync(0xffffffffu, at, 0);
+  if (lane < listed) s.front[at + lane] = list[lane];
+}
+
 // A row whose sum is good has a distribution: no NaN or +inf, and not -inf alone.
 __device__ __forceinline__ bool good_sum(const Partial& p) { return p.s > 0.0f && p.s < INFINITY; }
 __device__ __forceinline__ void finish(const LogprobsParams& P, int row, long long token, float x_token, const Total& x) {
@@ -272,19 +372,31 @@ __device__ __noinline__ int place_of(const u64* keys, int n, u64 key) {
   for (int i = 0; i < n; ++i) place += keys[i] > key;
   return place;
 }
-// Writes key i of n, among them the row's top, to its place.  A row without a distribution may have fewer.
-__device__ __forceinline__ void write_top(const LogprobsParams& P, int row, const u64* keys, int n, int i, const Total& x) {
+// Writes the row's top of n keys, `i` this thread's first of every `by`.  Where they are fewer the others are the lowest ids of
+// -inf: with less than 32 other values they are among the first 64 (the first warp looks for them).
+template <typename T>
+__device__ __forceinline__ void write_top(const LogprobsParams& P, int row, const u64* keys, int n, int i, int by, const Total& x) {
   const long long at = static_cast<long long>(row) * P.top;
-  if (!good_sum(x.p)) {
-    if (i == 0)
-      for (int k = 0; k < P.top; ++k) P.top_ids[at + k] = -1, P.top_logprobs[at + k] = NAN;
-    return;
+  const bool good = good_sum(x.p);
+  const float log_s = logf(x.p.s);
+  if (good)
+    for (int k = i; k < n; k += by) {
+      const u64 key = keys[k];
+      const int place = place_of(keys, n, key);
+      if (place >= P.top) continue;
+      P.top_ids[at + place] = static_cast<long long>(~static_cast<uint32_t>(key));
+      P.top_logprobs[at + place] = (order_value(static_cast<uint32_t>(key >> 32)) - x.p.m) - log_s;
+    }
+  if ((good && n >= P.top) || threadIdx.x >= 32) return;
+  int place = good ? n : 0;
+  const T* logits = static_cast<const T*>(P.logits) + row * P.ld;
+  for (int base = 0; base < 64; base += 32) {
+    const int id = base + static_cast<int>(threadIdx.x);
+    const uint32_t b = __ballot_sync(0xffffffffu, !good || (id < P.vocab && to_float(logits[id]) == -INFINITY));
+    const int mine = place + __popc(b & ((1u << threadIdx.x) - 1u));
+    if ((b >> threadIdx.x & 1u) && mine < P.top) P.top_ids[at + mine] = good ? id : -1, P.top_logprobs[at + mine] = good ? -INFINITY : NAN;
+    place += __popc(b);
   }
-  if (i >= n) return;
-  const int place = place_of(keys, n, keys[i]);
-  if (place >= P.top) return;
-  P.top_ids[at + place] = static_cast<long long>(~static_cast<uint32_t>(keys[i]));
-  P.top_logprobs[at + place] = (order_value(static_cast<uint32_t>(keys[i] >> 32)) - x.p.m) - logf(x.p.s);
 }
 
 // NT threads a CTA.
@@ -320,31 +432,29 @@ __global__ void __launch_bounds__(NT, 768 / NT) logprobs_kernel(const __grid_con
   for (int k = 0; k < NV; ++k) raw[k] = load_vec(begin + k * NT + tid);
 
   // Tokens before the given one: of vectors before its own those at or above it, of the others those above, and those of
-  // its own vector that equal it and come before it.  Where it is -inf, which also fills up vectors, all are looked at.
+  // its own vector that equal it and come before it.  Where it is -inf, which also fills up vectors, or of a size that is
+  // not compared by its bits, all are looked at.
   const long long token = P.tokens[row];
   const bool given = token >= 0 && token < P.vocab;
   const T t_token = given ? logits[token] : from_float<T>(INFINITY);
   const float x_token = to_float(t_token);
-  const bool by_one = given && x_token == -INFINITY;
+  const bool by_one = given && !(fabsf(x_token) < 1e36f);
   const int v_token = given ? static_cast<int>((token + before) / kVec) : 0;
   const uint32_t above = both(by_one ? from_float<T>(INFINITY) : t_token);
-  const uint32_t at_or_above = both(given && x_token < INFINITY && !by_one ? below(t_token) : from_float<T>(INFINITY));
+  const uint32_t at_or_above = both(given && !by_one ? below(t_token) : from_float<T>(INFINITY));
   uint32_t better = 0;
   if (given && !by_one && tid < kVec && v_token >= begin && v_token < end) {
     const long long id = static_cast<long long>(v_token) * kVec + tid - before;
     if (id >= 0 && id < token) better = to_float(logits[id]) == x_token;
   }
 
-  if (tid == 0) s.fronts = 0, s.token = token, s.x_token = x_token;
+  if (tid == 0) s.fronts = 0, s.queued = 0, s.token = token, s.x_token = x_token;
   __syncthreads();
   Partial p{-FLT_MAX, 0.0f, 0.0f};
   float best = -INFINITY;  // this thread's largest logit so far, where it has seen one
   bool seen = false;
-  // What can be among the top: values above bound_x, and those that equal it up to bound_id.  The same for a warp's threads.
-  float bound_x = -INFINITY;
-  int bound_id = INT32_MAX;
-  int listed = 0;  // by this warp
-  int found = 0;   // bounds, by the CTA
+  float bound_x = -INFINITY;  // what can be among the top reaches it; the same for every thread
+  int found = 0;              // such bounds
 
 #pragma unroll 1
   for (int base = begin, chunk = 0; base < end; base += NT * NV, ++chunk) {
@@ -352,24 +462,16 @@ __global__ void __launch_bounds__(NT, 768 / NT) logprobs_kernel(const __grid_con
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         const int v = base + k * NT + tid;
-        if (v == 0 || v == nvec - 1) {
-          T* e = reinterpret_cast<T*>(&raw[k]);
-#pragma unroll
-          for (int i = 0; i < kVec; ++i) {
-            const int id = v * kVec + i - before;
-            if (id < 0 || id >= P.vocab) e[i] = from_float<T>(-INFINITY);
-          }
-        }
+        if (v == 0 || v == nvec - 1) cut_vec<T>(raw[k], v * kVec - before, P.vocab);
       }
     }
     const float largest = largest_of<T>(raw);
     if (largest > p.m) move_to(p, largest);
     if (top > 0) {
-      const int id0 = (base + tid) * kVec - before;
       const bool here = base + tid < end;  // the thread has values in this chunk
       best = fmaxf(best, largest);
       seen |= here;
-      if ((chunk & (chunk + 1)) == 0 && end - begin > top) {
+      if (((chunk & (chunk + 1)) == 0 || bound_x == -INFINITY) && end - begin > top) {
         // a new bound: the top-th largest of 64 maxima, each of NT / 64 threads
         uint32_t m = seen ? order_bits(best) : 0u;
 #pragma unroll
@@ -392,48 +494,15 @@ __global__ void __launch_bounds__(NT, 768 / NT) logprobs_kernel(const __grid_con
         }
         __syncthreads();
         const float x = order_value(*bound);
-        if (x > bound_x) bound_x = x, bound_id = INT32_MAX;
+        if (x > bound_x) bound_x = x;
       }
-      u64* list = s.list[warp];
-      auto who_reach = [&] { return __ballot_sync(0xffffffffu, here && (largest > bound_x || (largest == bound_x && id0 <= bound_id))); };
-      uint32_t who = who_reach();
-      while (who) {
-        if (listed > kLogpList / 2) {
-          const u64 last = warp_prune<Logit<T>::kBits>(list, listed, top);
-          listed = top;
-          if (last > key_of(bound_x, bound_id)) bound_x = order_value(static_cast<uint32_t>(last >> 32)), bound_id = static_cast<int>(~static_cast<uint32_t>(last));
-          who &= who_reach();
-        }
-        // the first few of these threads show their vectors, and every thread looks at one
-        const int slot = __popc(who & ((1u << lane) - 1u));
-        if ((who >> lane & 1u) && slot < kLogpShown) {
+      if (here && largest >= bound_x && largest > -INFINITY) {
 #pragma unroll
-          for (int k = 0; k < NV; ++k) s.shown[warp][slot * NV + k] = raw[k];
-          s.from[warp][slot] = lane;
-        }
-        if (lane == 0) s.listed[warp] = listed;
-        __syncwarp();
-        if (lane / NV < __popc(who)) {
-          Raw<T, kVec> r;
-          r.w[0] = s.shown[warp][lane];
-          const int v = base + (lane % NV) * NT + warp * 32 + s.from[warp][lane / NV];
-          float x[kVec];
-          unpack_row<T, kVec>(r, x);
-          float m = x[0];
-#pragma unroll
-          for (int i = 1; i < kVec; ++i) m = fmaxf(m, x[i]);
-          if (m >= bound_x && v < end) {
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) {
-              const int id = v * kVec + i - before;
-              if (x[i] > bound_x || (x[i] == bound_x && id <= bound_id && id >= 0 && id < P.vocab)) list[atomicAdd(&s.listed[warp], 1)] = key_of(x[i], id);
-            }
+        for (int k = 0; k < NV; ++k)
+          if (largest_of<T>(raw[k]) >= bound_x && base + k * NT + tid < end) {
+            const int at = atomicAdd(&s.queued, 1);
+            if (at < kLogpQueue) s.queue[at] = raw[k], s.queue_at[at] = base + k * NT + tid;
           }
-        }
-#pragma unroll
-        for (int g = 0; g < kLogpShown; ++g) who &= who - 1;
-        __syncwarp();
-        listed = s.listed[warp];
       }
     }
     if (by_one) {
@@ -446,7 +515,7 @@ __global__ void __launch_bounds__(NT, 768 / NT) logprobs_kernel(const __grid_con
 #pragma unroll
         for (int i = 0; i < kVec; ++i) {
           const int v = base + k * NT + tid, id = v * kVec + i - before;
-          better += x[i] > -INFINITY || (x[i] == -INFINITY && v < end && id >= 0 && id < token);
+          better += x[i] > x_token || (x[i] == x_token && v < end && id >= 0 && id < token);
         }
       }
     }
@@ -480,7 +549,7 @@ __global__ void __launch_bounds__(NT, 768 / NT) logprobs_kernel(const __grid_con
         } else {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            count2(count, w[i], limit, t);
+            count2(count, w[i], limit);
             const float2 x = unpack2(max2_nan(w[i], Logit<T>::kFloor, t), t);
             add(x.x, sum0, dot0);
             add(x.y, sum1, dot1);
@@ -523,7 +592,7 @@ __global__ void __launch_bounds__(NT, 768 / NT) logprobs_kernel(const __grid_con
     if constexpr (sizeof(T) == 4) {
       better += count;
     } else {
-      const float2 n = unpack2(count, t);
+      const float2 n = unpack2(count, static_cast<const __half*>(nullptr));
       better += static_cast<uint32_t>(n.x + n.y);
     }
   }
@@ -531,17 +600,25 @@ __global__ void __launch_bounds__(NT, 768 / NT) logprobs_kernel(const __grid_con
   // The warps leave their totals, and of their lists what reaches the bound, 32 at most.
   const Total mine = warp_total({p, better});
   if (lane == 0) s.totals[warp] = words_of(mine);
-  if (listed > 0) {
-    u64* list = s.list[warp];
-    if (listed > 32) listed = warp_keep(list, listed, key_of(bound_x, bound_id));
-    if (listed > 32) {
-      warp_prune<Logit<T>::kBits>(list, listed, top);
-      listed = top;
-    }
-    int at = 0;
-    if (lane == 0) at = atomicAdd(&s.fronts, listed);
-    at = __shfl_sync(0xffffffffu, at, 0);
-    if (lane < listed) s.front[at + lane] = list[lane];
+  if (top > 0) {
+    __syncthreads();
+    const int queued = s.queued;
+    if (queued <= kLogpQueue)
+      for (int i = tid; i < queued; i += NT) {
+        Raw<T, kVec> r;
+        r.w[0] = s.queue[i];
+        float x[kVec];
+        unpack_row<T, kVec>(r, x);
+        const int id0 = s.queue_at[i] * kVec - before;
+#pragma unroll
+        for (int k = 0; k < kVec; ++k)
+          if (x[k] >= bound_x && x[k] > -INFINITY) {
+            const int at = atomicAdd(&s.fronts, 1);
+            if (at < NT) s.front[at] = key_of(x[k], id0 + k);
+          }
+      }
+    __syncthreads();
+    if (queued > kLogpQueue || s.fronts > NT) list_part<T, NT>(s, P.vocab, top, vecs, before, begin, end, nvec, bound_x);
   }
   if (cluster > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   __syncthreads();
@@ -549,7 +626,7 @@ __global__ void __launch_bounds__(NT, 768 / NT) logprobs_kernel(const __grid_con
   const int fronts = s.fronts;
   if (cluster == 1) {
     if (tid == 0) finish(P, row, s.token, s.x_token, total);
-    write_top(P, row, s.front, fronts, tid, total);
+    if (top > 0) write_top<T>(P, row, s.front, fronts, tid, NT, total);
     return;
   }
   // Rank 0 gets up to 32 keys of every CTA: all, or where they are more the top ones.
@@ -575,7 +652,7 @@ __global__ void __launch_bounds__(NT, 768 / NT) logprobs_kernel(const __grid_con
     if (e % kLogpTop < static_cast<int>(s.sent_n[e / kLogpTop].x) && static_cast<uint32_t>(s.sent[e] >> 32) >= row_bound)
       s.final[atomicAdd(&s.finalists, 1)] = s.sent[e];
   __syncthreads();
-  for (int e = tid; e < max(s.finalists, 1); e += NT) write_top(P, row, s.final, s.finalists, e, row_total);
+  if (top > 0) write_top<T>(P, row, s.final, s.finalists, tid, NT, row_total);
 }
 
 template <typename T, int NT>
