@@ -12,9 +12,13 @@ and produces tokens, one path through the decoding operators of `rldx_b200.ops`:
     cache = B200KV4Cache(layers, kv_heads, head_dim, seqs=4, max_tokens=4096)
     decoder = B200TextDecoder(decoder_layers, norm, embed, lm_head, cos, sin)
     out = decoder.generate(prompts, 64, cache=cache, u=torch.rand(64, 4), temperature=0.7, top_p=0.9)
+    scores = decoder.score(prompts, top=5)   # log probabilities of the prompts' tokens, alternatives
 
 `decoder_layers` are Qwen3 text decoder layers (the attribute names that B200LLMChain takes), `cos` and
-`sin` their RoPE tables [positions, head_dim].  Prompts of a vision tower bring positions and deepstack
+`sin` their RoPE tables [positions, head_dim]; with a B200Rope in their place (rope=) there is no table, positions may be of
+several axes and as far as they like.  Layers with norms behind their blocks too (pre_feedforward_layernorm and
+post_feedforward_layernorm beside the other two), or a residual_scale, run through block_norms, which makes the sum
+and both norms in one pass.  Prompts of a vision tower bring positions and deepstack
 features of their own; everything that cannot be run is refused before the cache changes.  `python -m rldx_b200.decoder` decodes with random
 weights.
 """
@@ -23,14 +27,26 @@ from __future__ import annotations
 
 import argparse
 import ctypes as C
-from typing import Optional, Sequence
+from typing import NamedTuple, Optional, Sequence
 
 import torch
 
 from . import _lib, ops
 from .llm import _raw_layer
+from .rope import B200Rope
 
 BF = torch.bfloat16
+
+
+class Scores(NamedTuple):
+    """What ops.token_logprobs gives of one sequence's tokens: logprob, entropy [n] fp32, rank [n] int32, top_ids [n, top] int64,
+    top_logprobs [n, top] fp32."""
+
+    logprob: torch.Tensor
+    entropy: torch.Tensor
+    rank: torch.Tensor
+    top_ids: torch.Tensor
+    top_logprobs: torch.Tensor
 
 
 class B200KV4Cache:
@@ -98,9 +114,12 @@ class B200TextDecoder:
     ignore_compression says that no prompt has what the wrapper compresses (it leaves one frame, and text, as
     they are)."""
 
-    def __init__(self, layers, norm, embed: torch.Tensor, lm_head: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *,
-                 window: int = 0, sinks: int = 0, device=None, ignore_compression: bool = False):
+    def __init__(self, layers, norm, embed: torch.Tensor, lm_head: torch.Tensor, cos: Optional[torch.Tensor] = None,
+                 sin: Optional[torch.Tensor] = None, *, window: int = 0, sinks: int = 0, device=None, ignore_compression: bool = False,
+                 rope: Optional[B200Rope] = None, residual_scale: float = 1.0):
         layers = list(layers)
+        if (rope is None) == (cos is None) or (cos is None) != (sin is None):
+            raise ValueError("the decoder takes cos and sin, or a rope")
         for i, wrap in enumerate(layers):
             if _raw_layer(wrap) is not wrap and wrap.layer_idx == wrap.internal_projection and not ignore_compression:
                 raise NotImplementedError(f"layer {i} compresses video tokens, which the decoder does not; ignore_compression=True "
@@ -123,15 +142,37 @@ class B200TextDecoder:
         ln = layers[0].input_layernorm
         self.eps = float(getattr(ln, "variance_epsilon", getattr(ln, "eps", 1e-6)))
 
+        # norms behind the blocks as well: then the one behind the attention has the name that else is the MLP's before it
+        after = [getattr(m, "post_feedforward_layernorm", None) is not None for m in layers]
+        if any((getattr(m, "pre_feedforward_layernorm", None) is not None) != b for m, b in zip(layers, after)) or len(set(after)) > 1:
+            raise NotImplementedError("every layer has pre_feedforward_layernorm and post_feedforward_layernorm, or none has")
+        self.after, self.residual_scale = after[0], float(residual_scale)
+        # the sum and the norms around it in one pass; layers without either keep their roundings (a sum in the product)
+        self.fused = self.after or self.residual_scale != 1.0
+
         def put(*w):
             return torch.cat([t.detach() for t in w]).to(self.device, BF).contiguous()
 
-        self.layers = [dict(norm1=put(m.input_layernorm.weight), norm2=put(m.post_attention_layernorm.weight),
+        def behind(m):
+            if not self.after:
+                return {}
+            return dict(post1=put(m.post_attention_layernorm.weight), post2=put(m.post_feedforward_layernorm.weight))
+
+        self.layers = [dict(behind(m), norm1=put(m.input_layernorm.weight),
+                            norm2=put((m.pre_feedforward_layernorm if self.after else m.post_attention_layernorm).weight),
                             qkv=put(m.self_attn.q_proj.weight, m.self_attn.k_proj.weight, m.self_attn.v_proj.weight),
                             q_norm=put(m.self_attn.q_norm.weight), k_norm=put(m.self_attn.k_norm.weight),
                             o=put(m.self_attn.o_proj.weight), gate_up=put(m.mlp.gate_proj.weight, m.mlp.up_proj.weight),
                             down=put(m.mlp.down_proj.weight)) for m in layers]
         self.norm, self.embed, self.lm_head = put(norm.weight), put(embed), put(lm_head)
+        self.rope = rope
+        if rope is not None:
+            if rope.head_dim != self.head_dim or rope.rotary_dim != self.head_dim or rope.interleaved:
+                raise ValueError(f"the rope must turn halves of whole heads of {self.head_dim}")
+            if rope.freqs.device != self.embed.device:
+                raise ValueError(f"the rope is on {rope.freqs.device}, the decoder on {self.embed.device}")
+            self.cos = self.sin = None
+            return
         self.cos, self.sin = (t.detach().to(self.device).contiguous() for t in (cos, sin))
         if (cos.dim() != 2 or cos.shape[1] != self.head_dim or sin.shape != cos.shape or sin.dtype != cos.dtype or
                 cos.dtype not in (torch.float32, BF)):
@@ -157,30 +198,31 @@ class B200TextDecoder:
         _lib.check(_lib.load().rldx_res_rmsnorm(C.byref(seg), 1, self.eps, C.c_void_p(torch.cuda.current_stream().cuda_stream)))
         return out
 
-    def forward(self, hidden: torch.Tensor, cache: B200KV4Cache, new: Sequence[int],
-                positions: Optional[torch.Tensor] = None, deepstack_features: Optional[Sequence[torch.Tensor]] = None,
-                deepstack_rows: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """Runs the rows `hidden` [sum(new), hidden] (the new tokens of every sequence, in order)
-        through the layers; keys and values join the cache.  positions [sum(new)]: RoPE rows, the
-        tokens' places in their sequences by default.  deepstack_features[i] [n, hidden] are added after
-        layer i to the rows deepstack_rows [n] of hidden (a vision tower's, as B200LLMChain takes them), with one
-        rounding to bf16.  Returns logits [seqs with new tokens, vocab]
-        of each sequence's last new token."""
+    def _places(self, start: Sequence[int], new: Sequence[int], positions: Optional[torch.Tensor]) -> torch.Tensor:
+        """The rows of the tables, or the rope's positions [axes, rows], that the new tokens take; refuses others."""
+        rows, tables = sum(new), self.rope is None
+        if positions is None:
+            longest = max(s + n for s, n in zip(start, new))
+            if tables and longest > self.cos.shape[0]:
+                raise ValueError(f"a sequence of {longest} tokens is longer than the RoPE tables ({self.cos.shape[0]})")
+            positions = torch.cat([torch.arange(s, s + n, dtype=torch.int32) for s, n in zip(start, new)])
+        elif tuple(positions.shape) != (rows,) and (tables or tuple(positions.shape) != (self.rope.axes, rows)):
+            raise ValueError(f"positions must be [{rows}]" + ("" if tables else f" or [{self.rope.axes}, {rows}]") + f", got {tuple(positions.shape)}")
+        elif tables and positions.device.type == "cpu" and not 0 <= int(positions.min()) <= int(positions.max()) < self.cos.shape[0]:
+            raise ValueError(f"positions must be rows of the RoPE tables ({self.cos.shape[0]})")  # (else device error 0x501)
+        elif not tables and (positions.dtype.is_floating_point or positions.dtype == torch.bool):
+            raise ValueError("positions must be whole numbers")
+        return positions
+
+    def _run(self, hidden: torch.Tensor, cache: B200KV4Cache, new: Sequence[int], positions: Optional[torch.Tensor] = None,
+             deepstack_features: Optional[Sequence[torch.Tensor]] = None, deepstack_rows: Optional[torch.Tensor] = None):
+        """The rows through the layers; returns f(rows) that gives the final norm of some of them."""
         new = [int(n) for n in new]
         if hidden.shape != (sum(new), self.hidden) or hidden.dtype != BF:
             raise ValueError(f"hidden must be bfloat16 [{sum(new)}, {self.hidden}], got {hidden.dtype} {tuple(hidden.shape)}")
         if len(new) != len(cache.tokens) or min(new) < 0 or max(new) == 0:
             raise ValueError(f"new must give a count for each of the {len(cache.tokens)} sequences, one of them positive")
-        start = list(cache.tokens)
-        if positions is None:
-            longest = max(s + n for s, n in zip(start, new))
-            if longest > self.cos.shape[0]:
-                raise ValueError(f"a sequence of {longest} tokens is longer than the RoPE tables ({self.cos.shape[0]})")
-            positions = torch.cat([torch.arange(s, s + n, dtype=torch.int32) for s, n in zip(start, new)])
-        elif tuple(positions.shape) != (sum(new),):
-            raise ValueError(f"positions must be [{sum(new)}], got {tuple(positions.shape)}")
-        elif positions.device.type == "cpu" and not 0 <= int(positions.min()) <= int(positions.max()) < self.cos.shape[0]:
-            raise ValueError(f"positions must be rows of the RoPE tables ({self.cos.shape[0]})")  # (else device error 0x501)
+        positions = self._places(list(cache.tokens), new, positions)
         if len(cache.pools) != len(self.layers) or any(p.shape[1] != self.kv_heads or p.shape[3] != 40 * self.head_dim
                                                        for p in cache.pools):
             raise ValueError(f"the cache is not one of {len(self.layers)} layers of {self.kv_heads} key / value heads of {self.head_dim}")
@@ -198,36 +240,130 @@ class B200TextDecoder:
         self._here(cache, hidden=hidden)
         if features:
             at, features = at.to(self.device), [f.to(self.device, BF) for f in features]
-        positions = positions.to(self.device, torch.int32)
+        if self.rope is None:
+            cos, sin, positions = self.cos, self.sin, positions.to(self.device, torch.int32)
+        else:  # rows for these tokens alone
+            positions = positions.to(self.device, torch.int64)
+            if self.rope.sections is not None:
+                positions = positions.expand(self.rope.axes, -1)
+            elif positions.dim() == 2:
+                positions = positions[0]
+            cos, sin = self.rope.rows(positions)
+            positions = torch.arange(sum(new), dtype=torch.int32, device=self.device)
         cache.extend(new)  # from here on nothing refuses
         cu = torch.tensor([0, *new], dtype=torch.int32).cumsum(0).to(torch.int32).to(self.device)
         max_new, max_len = max(new), max(cache.tokens)
+
+        def attention(n, w, pool):
+            qkv = ops.linear(n, w["qkv"])
+            q = ops.qkv_rope_append(qkv, w["q_norm"], w["k_norm"], cos, sin, positions, pool, cache.table, cache.lengths, cu,
+                                    q_heads=self.q_heads, eps=self.eps)
+            return ops.kv4_attention(q, pool, cache.table, cache.lengths, cu, max_new=max_new, max_len=max_len, window=self.window,
+                                     sinks=self.sinks).flatten(1)
+
+        def mlp(n, w):
+            gate, up = ops.linear(n, w["gate_up"]).chunk(2, 1)
+            return ops.swiglu(gate, up)
+
         h = hidden
+        if not self.fused:
+            for i, (w, pool) in enumerate(zip(self.layers, cache.pools)):
+                h = ops.linear(attention(self._rmsnorm(h, w["norm1"]), w, pool), w["o"], add=h)
+                h = ops.linear(mlp(self._rmsnorm(h, w["norm2"]), w), w["down"], add=h)
+                if i < len(features):
+                    h[at] += features[i]
+            return lambda rows: self._rmsnorm(h[rows].contiguous(), self.norm)
+
+        def between(y, h, weight, post):
+            """h + residual_scale * post(y), and the norm with `weight` of it."""
+            return ops.block_norms(y, h, post="rms" if self.after else None, post_weight=post, scale=self.residual_scale,
+                                   pre=None if weight is None else "rms", pre_weight=weight, eps=self.eps)
+
+        n = self._rmsnorm(h, self.layers[0]["norm1"])
         for i, (w, pool) in enumerate(zip(self.layers, cache.pools)):
-            qkv = ops.linear(self._rmsnorm(h, w["norm1"]), w["qkv"])
-            q = ops.qkv_rope_append(qkv, w["q_norm"], w["k_norm"], self.cos, self.sin, positions, pool, cache.table,
-                                    cache.lengths, cu, q_heads=self.q_heads, eps=self.eps)
-            a = ops.kv4_attention(q, pool, cache.table, cache.lengths, cu, max_new=max_new, max_len=max_len,
-                                  window=self.window, sinks=self.sinks)
-            h = ops.linear(a.flatten(1), w["o"], add=h)
-            gate, up = ops.linear(self._rmsnorm(h, w["norm2"]), w["gate_up"]).chunk(2, 1)
-            h = ops.linear(ops.swiglu(gate, up), w["down"], add=h)
-            if i < len(features):
+            h, n = between(ops.linear(attention(n, w, pool), w["o"]), h, w["norm2"], w.get("post1"))
+            after = self.layers[i + 1]["norm1"] if i + 1 < len(self.layers) else self.norm
+            joins = i < len(features)  # before the next norm
+            h, n = between(ops.linear(mlp(n, w), w["down"]), h, None if joins else after, w.get("post2"))
+            if joins:
                 h[at] += features[i]
+                n = self._rmsnorm(h, after)
+        return lambda rows: n[rows]
+
+    def forward(self, hidden: torch.Tensor, cache: B200KV4Cache, new: Sequence[int],
+                positions: Optional[torch.Tensor] = None, deepstack_features: Optional[Sequence[torch.Tensor]] = None,
+                deepstack_rows: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Runs the rows `hidden` [sum(new), hidden] (the new tokens of every sequence, in order)
+        through the layers; keys and values join the cache.  positions [sum(new)]: RoPE rows, the
+        tokens' places in their sequences by default; with a rope positions of any size, of one axis for all or [axes, sum(new)].
+        deepstack_features[i] [n, hidden] are added after
+        layer i to the rows deepstack_rows [n] of hidden (a vision tower's, as B200LLMChain takes them), with one
+        rounding to bf16.  Returns logits [seqs with new tokens, vocab]
+        of each sequence's last new token."""
+        normed = self._run(hidden, cache, new, positions, deepstack_features, deepstack_rows)
         last = torch.tensor([e - 1 for n, e in zip(new, torch.tensor(new).cumsum(0).tolist()) if n], device=self.device)
-        return ops.linear(self._rmsnorm(h[last].contiguous(), self.norm), self.lm_head)
+        return ops.linear(normed(last).contiguous(), self.lm_head)
+
+    def score(self, prompts, *, targets: Optional[Sequence] = None, top: int = 0, cache: Optional[B200KV4Cache] = None,
+              positions: Optional[Sequence] = None, deepstack_features: Optional[Sequence[torch.Tensor]] = None,
+              deepstack_rows: Optional[torch.Tensor] = None) -> list:
+        """How likely the prompts' own tokens are: for each prompt (ids, or rows of embeddings) Scores whose entry i is about the
+        token that follows its row i: targets[prompt][i], by default the prompt's next id, and none (-1: logprob 0, rank -1)
+        behind the last one or where the prompt is rows.  Its entropy and `top` (0 to 32) alternatives are there either way.  Logits
+        are made for a few thousand rows at a time.  positions, deepstack_features and deepstack_rows are generate()'s."""
+        ids = [None if torch.is_tensor(p) and p.dim() == 2 else torch.as_tensor(p).to("cpu", torch.int64) for p in prompts]
+        rows = [p.to(self.device, BF) if i is None else self.embed[i.to(self.device)] for p, i in zip(prompts, ids)]
+        new = [r.shape[0] for r in rows]
+        if not prompts or min(new) == 0:
+            raise ValueError("a prompt has no token")
+        if not 0 <= top <= min(32, self.lm_head.shape[0]):
+            raise ValueError(f"top must be 0 to {min(32, self.lm_head.shape[0])}, got {top}")
+        if targets is None:
+            follow = [torch.full((n,), -1) if i is None else torch.cat([i[1:], torch.tensor([-1])]) for i, n in zip(ids, new)]
+        else:
+            follow = [torch.as_tensor(t).to("cpu", torch.int64) for t in targets]
+            if [tuple(t.shape) for t in follow] != [(n,) for n in new]:
+                raise ValueError(f"targets must give {new} tokens, got {[tuple(t.shape) for t in follow]}")
+        follow = torch.cat(follow)
+        if int(follow.max()) >= self.lm_head.shape[0]:
+            raise ValueError(f"targets must be below the {self.lm_head.shape[0]} tokens of lm_head")
+        cache = cache or self.new_cache(len(prompts), sum(new))
+        if cache.seqs != len(prompts):
+            raise ValueError(f"the cache has {cache.seqs} sequences, {len(prompts)} prompts were given")
+        cache.room(new)
+        places = None if positions is None else self._prompt_places(positions, new)[0]
+        normed = self._run(torch.cat(rows), cache, new, places, deepstack_features, deepstack_rows)
+        follow, total, parts = follow.to(self.device), sum(new), []
+        step = max(1, 2 ** 29 // self.lm_head.shape[0])  # a gibibyte of logits
+        for a in range(0, total, step):
+            at = slice(a, min(a + step, total))
+            parts.append(ops.token_logprobs(ops.linear(normed(at).contiguous(), self.lm_head), follow[at], top=top))
+        return [Scores(*part) for part in zip(*(torch.cat(t).split(new) for t in zip(*parts)))]
+
+    def _prompt_places(self, positions: Sequence, new: Sequence[int]):
+        """The prompts' positions, one after the other, and one past each one's largest; refuses other shapes."""
+        given = [torch.as_tensor(p).to("cpu", torch.int32 if self.rope is None else torch.int64) for p in positions]
+        wanted = [(n,) for n in new]
+        if self.rope is not None:  # one position for all axes, or each
+            given = [p.expand(self.rope.axes, -1) if p.dim() == 1 else p for p in given]
+            wanted = [(self.rope.axes, n) for n in new]
+        if [tuple(p.shape) for p in given] != wanted:
+            raise ValueError(f"positions must give {list(new)} rows, got {[tuple(p.shape) for p in given]}")
+        return torch.cat(given, -1), [int(p.max()) + 1 for p in given]
 
     def generate(self, prompts, max_new_tokens: int, *, u: torch.Tensor, cache: Optional[B200KV4Cache] = None,
                  temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, stop_ids: Sequence[int] = (),
                  positions: Optional[Sequence] = None, next_positions: Optional[Sequence[int]] = None,
-                 deepstack_features: Optional[Sequence[torch.Tensor]] = None, deepstack_rows: Optional[torch.Tensor] = None):
+                 deepstack_features: Optional[Sequence[torch.Tensor]] = None, deepstack_rows: Optional[torch.Tensor] = None,
+                 logprobs: Optional[int] = None):
         """Appends max_new_tokens tokens to each of the prompts (lists of ids, or rows [n, hidden] of
         embeddings that a vision tower has filled in).  positions gives each prompt's RoPE rows [n], of
         tables whose rows stand for whatever the prompt's tokens have (vision tokens do not count up one by one);
         the new tokens go on at next_positions, by default one past a prompt's largest.  Without it the rows are
         the tokens' places in their sequences.  deepstack_features and deepstack_rows are forward()'s, of the
         prompts' rows one after the other.  u [max_new_tokens, prompts] are the draws'
-        numbers in [0, 1).  Returns a list of id lists; a sequence ends after one of stop_ids.  A sequence whose logits
+        numbers in [0, 1).  Returns a list of id lists; a sequence ends after one of stop_ids.  With logprobs (0 to 32) it is
+        (ids, scores): of each sequence Scores of its new tokens under the unfiltered logits, with so many alternatives.  A sequence whose logits
         have no number to draw from (all NaN or -inf) before its end raises RuntimeError, an error that a kernel
         has recorded on the device RldxError."""
         n = len(prompts)
@@ -242,20 +378,16 @@ class B200TextDecoder:
             raise ValueError("a prompt has no token")
         if max_new_tokens > 0:  # what would end the run in its middle: all but the last token drawn are run
             ends = [t + r.shape[0] + max_new_tokens - 1 for t, r in zip(cache.tokens, rows)]
-            if positions is None and max(ends) > self.cos.shape[0]:
+            if positions is None and self.rope is None and max(ends) > self.cos.shape[0]:
                 raise ValueError(f"a sequence of {max(ends)} tokens is longer than the RoPE tables ({self.cos.shape[0]})")
             cache.room([e - t for e, t in zip(ends, cache.tokens)])
         places = follow = None
         if positions is not None:
-            given = [torch.as_tensor(p).to("cpu", torch.int32) for p in positions]
-            if [tuple(p.shape) for p in given] != [(r.shape[0],) for r in rows]:
-                raise ValueError(f"positions must give {[r.shape[0] for r in rows]} rows, got {[tuple(p.shape) for p in given]}")
-            places = torch.cat(given)
-            follow = torch.tensor([int(p.max()) + 1 for p in given] if next_positions is None else [int(p) for p in next_positions],
-                                  dtype=torch.int32)
+            places, past = self._prompt_places(positions, [r.shape[0] for r in rows])
+            follow = torch.tensor(past if next_positions is None else [int(p) for p in next_positions], dtype=places.dtype)
             if follow.shape != (n,):
                 raise ValueError(f"next_positions must be {n} rows")
-            if not (0 <= int(places.min()) and int(places.max()) < self.cos.shape[0] and
+            if self.rope is None and not (0 <= int(places.min()) and int(places.max()) < self.cos.shape[0] and
                     (max_new_tokens <= 1 or (int(follow.min()) >= 0 and int(follow.max()) + max_new_tokens - 2 < self.cos.shape[0]))):
                 raise ValueError(f"the positions of the prompts and the new tokens must be rows of the RoPE tables ({self.cos.shape[0]})")
         elif next_positions is not None:
@@ -270,10 +402,15 @@ class B200TextDecoder:
         deep = {} if deepstack_features is None else dict(deepstack_features=deepstack_features, deepstack_rows=deepstack_rows)
         if not deep and deepstack_rows is not None:
             raise ValueError("deepstack_rows go with deepstack_features")
-        hidden, new, tokens = torch.cat(rows), [r.shape[0] for r in rows], []
+        if logprobs is not None and not 0 <= logprobs <= min(32, self.lm_head.shape[0]):
+            raise ValueError(f"logprobs must be 0 to {min(32, self.lm_head.shape[0])}, got {logprobs}")
+        hidden, new, tokens, scores = torch.cat(rows), [r.shape[0] for r in rows], [], []
         for i in range(max_new_tokens):
-            token, _, _ = ops.sample(self.forward(hidden, cache, new, places, **deep), u[i], **limits)
+            logits = self.forward(hidden, cache, new, places, **deep)
+            token, _, _ = ops.sample(logits, u[i], **limits)
             tokens.append(token)
+            if logprobs is not None:
+                scores.append(ops.token_logprobs(logits, token, top=logprobs))
             deep = {}
             hidden, new, places = self.embed[token], [1] * n, None if follow is None else follow + i
         out = torch.stack(tokens, 1).tolist() if tokens else [[] for _ in prompts]
@@ -286,7 +423,13 @@ class B200TextDecoder:
                 del ids[end + 1:]
             if -1 in ids:  # (what was run after it began with the last row of the embedding)
                 raise RuntimeError(f"sequence {s} has no logit that is a number at its token {ids.index(-1)}")
-        return out
+        if logprobs is None:
+            return out
+        if not scores:
+            empty = Scores(*ops.token_logprobs(self.embed.new_empty(0, self.lm_head.shape[0]), torch.empty(0, dtype=torch.int64, device=self.device), top=logprobs))
+            return out, [empty for _ in prompts]
+        steps = [torch.stack(t, 1) for t in zip(*scores)]  # [sequences, tokens, ...]
+        return out, [Scores(*(t[s, : len(ids)] for t in steps)) for s, ids in enumerate(out)]
 
 
 def main() -> None:
@@ -301,6 +444,8 @@ def main() -> None:
     ap.add_argument("--tokens", type=int, default=32)
     ap.add_argument("--window", type=int, default=0)
     ap.add_argument("--sinks", type=int, default=0)
+    ap.add_argument("--rope", action="store_true", help="angles from positions in place of tables")
+    ap.add_argument("--score", action="store_true", help="log probabilities of the prompts' own tokens as well")
     a = ap.parse_args()
     g = torch.Generator(device="cuda").manual_seed(0)
 
@@ -315,9 +460,13 @@ def main() -> None:
                               o_proj=w(a.hidden, hq * d), q_norm=head, k_norm=head),
                  mlp=NS(gate_proj=w(ffn, a.hidden), up_proj=w(ffn, a.hidden), down_proj=w(a.hidden, ffn)))
               for _ in range(a.layers)]
-    inv = 1.0 / (1e6 ** (torch.arange(0, d, 2, device="cuda").float() / d))
-    ang = torch.outer(torch.arange(a.prompt + a.tokens, device="cuda").float(), inv).repeat(1, 2)
-    dec = B200TextDecoder(layers, one, w(a.vocab, a.hidden).weight * 50, w(a.vocab, a.hidden).weight, ang.cos(), ang.sin(),
+    if a.rope:
+        angles = dict(rope=B200Rope(d, theta=1e6))
+    else:
+        inv = 1.0 / (1e6 ** (torch.arange(0, d, 2, device="cuda").float() / d))
+        ang = torch.outer(torch.arange(a.prompt + a.tokens, device="cuda").float(), inv).repeat(1, 2)
+        angles = dict(cos=ang.cos(), sin=ang.sin())
+    dec = B200TextDecoder(layers, one, w(a.vocab, a.hidden).weight * 50, w(a.vocab, a.hidden).weight, **angles,
                           window=a.window, sinks=a.sinks)
     prompts = [torch.randint(a.vocab, (a.prompt - 7 * s,), device="cuda", generator=g).tolist() for s in range(a.seqs)]
     u = torch.rand(a.tokens, a.seqs, generator=torch.Generator().manual_seed(0))
@@ -330,6 +479,13 @@ def main() -> None:
     torch.cuda.synchronize()
     print(f"{a.seqs} sequences, prompts of {a.prompt}: {a.tokens} tokens each in {e0.elapsed_time(e1):.1f} ms; first ids "
           f"{[ids[:6] for ids in out]}")
+    if a.score:
+        dec.score(prompts, top=5)
+        e0.record()
+        scores = dec.score(prompts, top=5)
+        e1.record()
+        torch.cuda.synchronize()
+        print(f"scored in {e0.elapsed_time(e1):.1f} ms; mean log probability {[round(float(x.logprob.mean()), 3) for x in scores]}")
 
 
 if __name__ == "__main__":

@@ -359,3 +359,67 @@ def _(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
     rows = logits.shape[0]
     return (logits.new_empty((rows,), dtype=torch.int64), logits.new_empty((rows,), dtype=torch.float32),
             logits.new_empty((rows,), dtype=torch.int32))
+
+
+# ---------------------------------------------------------------------------------------------
+# around a decoder's products
+# ---------------------------------------------------------------------------------------------
+@torch.library.custom_op("b200msat::rope", mutates_args=())
+def rope(q: Tensor, k: Tensor, positions: Tensor, freqs: Tensor, sections: Optional[List[int]] = None,
+         interleaved_sections: bool = False, interleaved: bool = False, factor: float = 1.0,
+         inverse: bool = False) -> Tuple[Tensor, Tensor]:
+    """q and k [tokens, heads, d] turned by positions * freqs, without a table."""
+    return ops.rope(q, k, positions, freqs, sections=sections, interleaved_sections=interleaved_sections, interleaved=interleaved,
+                    factor=factor, inverse=inverse)
+
+
+@rope.register_fake
+def _(q, k, positions, freqs, sections=None, interleaved_sections=False, interleaved=False, factor=1.0, inverse=False):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+@torch.library.custom_op("b200msat::rope_rows", mutates_args=())
+def rope_rows(positions: Tensor, freqs: Tensor, sections: Optional[List[int]] = None, interleaved_sections: bool = False,
+              factor: float = 1.0, inverse: bool = False, dtype: torch.dtype = torch.float32) -> Tuple[Tensor, Tensor]:
+    """cos and sin rows [tokens, 2 pairs] of positions * freqs."""
+    return ops.rope_rows(positions, freqs, sections=sections, interleaved_sections=interleaved_sections, factor=factor, inverse=inverse,
+                         dtype=dtype)
+
+
+@rope_rows.register_fake
+def _(positions, freqs, sections=None, interleaved_sections=False, factor=1.0, inverse=False, dtype=torch.float32):
+    shape = (positions.shape[-1], 2 * freqs.shape[0])
+    return positions.new_empty(shape, dtype=dtype), positions.new_empty(shape, dtype=dtype)
+
+
+@torch.library.custom_op("b200msat::block_norms", mutates_args=())
+def block_norms(branch: Tensor, residual: Tensor, post: str = "none", post_weight: Optional[Tensor] = None, post_bias: Optional[Tensor] = None,
+                gate: Optional[Tensor] = None, scale: float = 1.0, pre: str = "rms", pre_weight: Optional[Tensor] = None,
+                pre_bias: Optional[Tensor] = None, mod_scale: Optional[Tensor] = None, mod_shift: Optional[Tensor] = None,
+                rows_per_group: int = 0, weight_plus_one: bool = False, eps: float = 1e-6) -> Tuple[Tensor, Tensor]:
+    """residual + scale * gate * post(branch), and pre of it with its modulation (pre is a norm)."""
+    if pre == "none":
+        raise ValueError("without a pre norm there is one result: call ops.block_norms")
+    return ops.block_norms(branch, residual, post=post, post_weight=post_weight, post_bias=post_bias, gate=gate, scale=scale, pre=pre,
+                           pre_weight=pre_weight, pre_bias=pre_bias, mod_scale=mod_scale, mod_shift=mod_shift, rows_per_group=rows_per_group,
+                           weight_plus_one=weight_plus_one, eps=eps)
+
+
+@block_norms.register_fake
+def _(branch, residual, post="none", post_weight=None, post_bias=None, gate=None, scale=1.0, pre="rms", pre_weight=None, pre_bias=None,
+      mod_scale=None, mod_shift=None, rows_per_group=0, weight_plus_one=False, eps=1e-6):
+    return residual.new_empty(branch.shape), branch.new_empty(branch.shape)
+
+
+@torch.library.custom_op("b200msat::token_logprobs", mutates_args=())
+def token_logprobs(logits: Tensor, tokens: Tensor, top: int = 0) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """Of given tokens: logprob, entropy, rank, and the rows' top ids and log probabilities."""
+    return ops.token_logprobs(logits, tokens, top=top)
+
+
+@token_logprobs.register_fake
+def _(logits, tokens, top=0):
+    rows = logits.shape[0]
+    return (logits.new_empty((rows,), dtype=torch.float32), logits.new_empty((rows,), dtype=torch.float32),
+            logits.new_empty((rows,), dtype=torch.int32), logits.new_empty((rows, top), dtype=torch.int64),
+            logits.new_empty((rows, top), dtype=torch.float32))

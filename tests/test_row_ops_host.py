@@ -198,3 +198,72 @@ def test_library_refuses_before_any_device_work(lib):
     assert lp(logits=None) == arg and lp(logits=258) == arg and lp(tokens=None) == arg and lp(out=None) == arg and lp(rows=-1) == arg
     assert lp(vocab=0) == arg and lp(ld=-1) == arg and lp(dtype=3) == no and lp(top=33) == no and lp(top=-1) == no and lp(vocab=1, top=2) == no
     assert lp(vocab=2 ** 28 + 1) == no and lp(rows=2 ** 29) == no
+
+
+def test_fake_shapes():
+    import rldx_b200.torch_ops  # noqa: F401
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        q, k = torch.ops.b200msat.rope(torch.empty(7, 8, 64, dtype=BF), torch.empty(7, 2, 64, dtype=BF), torch.empty(3, 7, dtype=torch.int64),
+                                       torch.empty(32, dtype=F64), [16, 8, 8])
+        assert q.shape == (7, 8, 64) and k.shape == (7, 2, 64) and q.dtype == BF
+        cos, sin = torch.ops.b200msat.rope_rows(torch.empty(3, 7, dtype=torch.int64), torch.empty(32, dtype=F64), [16, 8, 8], dtype=BF)
+        assert cos.shape == sin.shape == (7, 64) and cos.dtype == BF
+        h, n = torch.ops.b200msat.block_norms(torch.empty(5, 40, dtype=BF), torch.empty(5, 40))
+        assert h.dtype == F32 and n.dtype == BF and h.shape == n.shape == (5, 40)
+        out = torch.ops.b200msat.token_logprobs(torch.empty(5, 99, dtype=BF), torch.empty(5, dtype=torch.int64), 3)
+        assert [t.dtype for t in out] == [F32, F32, torch.int32, torch.int64, F32] and out[3].shape == out[4].shape == (5, 3)
+
+
+def test_decoder_refusals():
+    from test_decoder_host import FFN, HEAD, HIDDEN, VOCAB, layer, make, weight
+    from rldx_b200.decoder import B200TextDecoder
+
+    def sandwich():
+        m = layer()
+        m.pre_feedforward_layernorm, m.post_feedforward_layernorm = weight(HIDDEN), weight(HIDDEN)
+        return m
+
+    def build(layers=None, **kw):
+        kw.setdefault("rope", B200Rope(HEAD, device="cpu"))
+        return B200TextDecoder(layers or [layer(), layer()], weight(HIDDEN), torch.zeros(VOCAB, HIDDEN), torch.zeros(VOCAB, HIDDEN), device="cpu", **kw)
+
+    assert not make().fused and not build().fused and build(residual_scale=0.5).fused and build([sandwich(), sandwich()]).after
+    with pytest.raises(NotImplementedError, match="every layer"):
+        build([sandwich(), layer()])
+    half = sandwich()
+    half.post_feedforward_layernorm = None
+    with pytest.raises(NotImplementedError, match="every layer"):
+        build([half, half])
+    with pytest.raises(ValueError, match="cos and sin, or a rope"):
+        build(rope=None)
+    with pytest.raises(ValueError, match="cos and sin, or a rope"):
+        build(cos=torch.zeros(4, HEAD), sin=torch.zeros(4, HEAD))
+    with pytest.raises(ValueError, match="cos and sin, or a rope"):
+        build(rope=None, cos=torch.zeros(4, HEAD))
+    for bad in (B200Rope(HEAD, rotary_dim=32, device="cpu"), B200Rope(HEAD, interleaved=True, device="cpu"), B200Rope(2 * HEAD, device="cpu")):
+        with pytest.raises(ValueError, match="halves of whole heads"):
+            build(rope=bad)
+    dec = build(rope=B200Rope(HEAD, sections=(16, 8, 8), device="cpu"))
+    cache = dec.new_cache(2, 256)
+    rows = torch.zeros(3, HIDDEN, dtype=BF)
+    for at in (torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, dtype=torch.int64), torch.zeros(3)):
+        with pytest.raises(ValueError, match="positions must"):
+            dec.forward(rows, cache, [1, 2], at)
+    u = torch.zeros(2, 2)
+    with pytest.raises(ValueError, match="positions must give"):
+        dec.generate([[1], [2, 3]], 2, u=u, positions=[torch.zeros(3, 1), torch.zeros(2, 2)])
+    with pytest.raises(ValueError, match="logprobs must be"):
+        dec.generate([[1], [2, 3]], 2, u=u, logprobs=33)
+    for kw, match in ((dict(top=33), "top must be"), (dict(top=-1), "top must be"), (dict(targets=[[1], [2]]), "targets must give"),
+                      (dict(targets=[[1], [VOCAB, 2]]), "targets must be below"), (dict(positions=[torch.zeros(4, 1), torch.zeros(3, 2)]), "positions must give"),
+                      (dict(cache=dec.new_cache(3, 256)), "the cache has 3 sequences")):
+        with pytest.raises(ValueError, match=match):
+            dec.score([[1], [2, 3]], **kw)
+    with pytest.raises(ValueError, match="no token"):
+        dec.score([[1], []])
+    with pytest.raises(ValueError, match="no token"):
+        dec.score([])
+    with pytest.raises(RuntimeError, match="free pages"):
+        dec.score([[1], [2] * 200], cache=dec.new_cache(2, 1))
+    assert cache.tokens == [0, 0] and FFN
