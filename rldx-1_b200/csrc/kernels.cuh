@@ -189,6 +189,5 @@ cudaError_t launch_key_mask(uint8_t* kmask, const uint8_t* vl, const uint8_t* p,
 cudaError_t gemm_prepare_device();
 cudaError_t kv4_prepare_device();
 cudaError_t sample_prepare_device();
-cudaError_t logprobs_prepare_device();
 
 }  // namespace rldx

@@ -26,7 +26,7 @@ namespace rldx {
 
 namespace {
 constexpr int kLogpTop = 32;        // alternatives at most
-constexpr int kLogpMaxCluster = 16;
+constexpr int kLogpMaxCluster = 8;
 // 16-byte vectors of a thread and chunk: with four, 64 registers let four CTAs of 256 threads run on an SM (eight and three of
 // them, us: 2208 x 151680 175 against 171, 256 rows 36.2 against 31.6, 64 x 50257 fp32 16.6 against 14.5, one row 6.1 against 6.8)
 constexpr int kLogpVecs = 4;
@@ -673,29 +673,19 @@ cudaError_t launch_logprobs(const LogprobsParams& p, cudaStream_t stream) {
   cfg.numAttrs = p.cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, logprobs_kernel<T, NT>, p);
 }
-template <typename T, int NT>
-cudaError_t logprobs_clusters() {
-  return cudaFuncSetAttribute(logprobs_kernel<T, NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-}
 template <typename T>
 cudaError_t launch_logprobs(LogprobsParams p, cudaStream_t stream) {
-  // Threads of a CTA: 64, of many small rows to an SM, where they hold one at a time; else 256.  CTAs of a row: as few as
-  // fill the SMs, and none with less than a vector a thread.
+  // Threads of a CTA: 64 for rows of up to 8 KB, whose time is mostly the search for the top (8000 x 4096 bf16: 46 us, with 256
+  // 72), else 256.  CTAs of a row: up to 8, until they would take a quarter of the threads that run at once, and none with less
+  // than a vector a thread.  (Up to half of them, us: 64 x 50257 fp32 14.3 against 11.6, 64 x 20000 12.2 against 7.8, 256 x
+  // 151680 31.8 against 33.3; up to 16 CTAs a row: 8 x 151680 17.4 against 11.4, one row 14.6 against 10.5.)
   const long long vecs = static_cast<long long>(p.vocab) * sizeof(T) / 16;
-  const int nt = vecs <= 64 * kLogpVecs ? 64 : 256;
+  const int nt = vecs <= 512 ? 64 : 256;
   p.cluster = 1;
-  while (p.cluster < (nt == 64 ? 8 : kLogpMaxCluster) && static_cast<long long>(p.rows) * p.cluster * nt < 768LL * sm_count() && vecs / (2 * p.cluster) >= nt)
-    p.cluster *= 2;
+  while (p.cluster < kLogpMaxCluster && static_cast<long long>(p.rows) * p.cluster * nt < 384LL * sm_count() && vecs / (2 * p.cluster) >= nt) p.cluster *= 2;
   return nt == 64 ? launch_logprobs<T, 64>(p, stream) : launch_logprobs<T, 256>(p, stream);
 }
 }  // namespace
-
-cudaError_t logprobs_prepare_device() {
-  cudaError_t e = logprobs_clusters<__nv_bfloat16, 256>();
-  if (e == cudaSuccess) e = logprobs_clusters<__half, 256>();
-  if (e == cudaSuccess) e = logprobs_clusters<float, 256>();
-  return e;
-}
 
 }  // namespace rldx
 
