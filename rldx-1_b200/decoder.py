@@ -311,10 +311,9 @@ class B200TextDecoder:
         token that follows its row i: targets[prompt][i], by default the prompt's next id, and none (-1: logprob 0, rank -1)
         behind the last one or where the prompt is rows.  Its entropy and `top` (0 to 32) alternatives are there either way.  Logits
         are made for a few thousand rows at a time.  positions, deepstack_features and deepstack_rows are generate()'s."""
-        ids = [None if torch.is_tensor(p) and p.dim() == 2 else torch.as_tensor(p).to("cpu", torch.int64) for p in prompts]
-        rows = [p.to(self.device, BF) if i is None else self.embed[i.to(self.device)] for p, i in zip(prompts, ids)]
+        ids, rows = zip(*(self._rows(p) for p in prompts)) if len(prompts) else ((), ())
         new = [r.shape[0] for r in rows]
-        if not prompts or min(new) == 0:
+        if not new or min(new) == 0:
             raise ValueError("a prompt has no token")
         if not 0 <= top <= min(32, self.lm_head.shape[0]):
             raise ValueError(f"top must be 0 to {min(32, self.lm_head.shape[0])}, got {top}")
@@ -338,7 +337,16 @@ class B200TextDecoder:
         for a in range(0, total, step):
             at = slice(a, min(a + step, total))
             parts.append(ops.token_logprobs(ops.linear(normed(at).contiguous(), self.lm_head), follow[at], top=top))
-        return [Scores(*part) for part in zip(*(torch.cat(t).split(new) for t in zip(*parts)))]
+        return [Scores(*part) for part in zip(*(torch.cat(t).split(list(new)) for t in zip(*parts)))]
+
+    def _rows(self, prompt):
+        """A prompt's ids (None where it is rows of embeddings) and its rows; refuses ids that the embedding does not have."""
+        if torch.is_tensor(prompt) and prompt.dim() == 2:
+            return None, prompt.to(self.device, BF)
+        ids = torch.as_tensor(prompt).to("cpu", torch.int64)
+        if ids.numel() and not 0 <= int(ids.min()) <= int(ids.max()) < self.embed.shape[0]:  # (looked at on the host: others would fault)
+            raise ValueError(f"a prompt's ids must be among the {self.embed.shape[0]} of the embedding")
+        return ids, self.embed[ids.to(self.device)]
 
     def _prompt_places(self, positions: Sequence, new: Sequence[int]):
         """The prompts' positions, one after the other, and one past each one's largest; refuses other shapes."""
@@ -369,8 +377,7 @@ class B200TextDecoder:
         n = len(prompts)
         if tuple(u.shape) != (max_new_tokens, n):
             raise ValueError(f"u must be [{max_new_tokens}, {n}], got {tuple(u.shape)}")
-        rows = [self.embed[torch.as_tensor(p, device=self.device)] if not torch.is_tensor(p) or p.dim() == 1 else
-                p.to(self.device, BF) for p in prompts]
+        rows = [self._rows(p)[1] for p in prompts]
         cache = cache or self.new_cache(n, sum(r.shape[0] for r in rows) + n * max_new_tokens)
         if cache.seqs != n:
             raise ValueError(f"the cache has {cache.seqs} sequences, {n} prompts were given")

@@ -264,6 +264,11 @@ def test_decoder_refusals():
         dec.score([[1], []])
     with pytest.raises(ValueError, match="no token"):
         dec.score([])
+    for ids in ([VOCAB], [-1], torch.tensor([0, VOCAB])):
+        with pytest.raises(ValueError, match="ids must be among"):
+            dec.score([[1], ids])
+        with pytest.raises(ValueError, match="ids must be among"):
+            dec.generate([[1], ids], 2, u=u)
     with pytest.raises(RuntimeError, match="free pages"):
         dec.score([[1], [2] * 200], cache=dec.new_cache(2, 1))
     assert cache.tokens == [0, 0] and FFN
