@@ -9,9 +9,12 @@
 //
 // A row lies in the registers of a team: 8 lanes, a warp or several, 16 values a thread.  The vectors come down
 // to four numbers a value, h' = h + (a y^ + b) and n = c h^ + d with a = scale gate (w + 1), b = scale gate b, c = (w + 1)
-// (1 + mod_scale), d = b (1 + mod_scale) + mod_shift, kept in shared memory: made once by a CTA where all rows share them,
-// else by each team whenever it comes to another group.  A CTA goes over a run of rows, the next of which is on the way
-// while one is normed.  Bound by memory: y and h are read and h' and n written once.
+// (1 + mod_scale), d = b (1 + mod_scale) + mod_shift, kept in shared memory and made once by a CTA.  Vectors of groups are
+// read beside the rows, as they are, where they have the rows' type and alignment; else each team makes its own four numbers
+// whenever it comes to another group.  A CTA goes over a run of rows, the next of which is on the way while one is
+// normed.  Bound by memory: y and h are read and h' and n written once.
+#include <utility>
+
 #include "host_util.h"
 #include "rows.cuh"
 
@@ -20,7 +23,10 @@ namespace rldx {
 namespace {
 constexpr int kNormMaxWidth = 14336;  // four vectors of it fill the shared memory
 constexpr int kNormShared = 4 * 4 * kNormMaxWidth;
-constexpr int kNormValues = 16;       // of a thread
+// Values of a thread: 16, and 8 of those taken one by one, whose rows are often narrow (100000 x 157 bf16: 75 us with 16, 44 with 8;
+// 4999 x 1001 fp16 with an fp32 stream 18.7 and 16.2; 20000 x 1001 bf16 41 and 43).
+template <int V, int kThreads>
+constexpr int kNormValues = V == 1 && kThreads == 256 ? 8 : 16;
 enum { kNormA = 0, kNormB = 1, kNormC = 2, kNormD = 3 };
 
 struct NormsParams {
@@ -38,6 +44,10 @@ struct NormsParams {
   const void* mod_shift;
   long long ld_gate, ld_scale, ld_shift;  // of the groups' vectors
   long long rows, group;
+  // of groups, read beside the rows (the ones above are null then)
+  const void* row_gate;
+  const void* row_scale;
+  const void* row_shift;
   int run;                 // rows of a team
   int width, post, pre;    // RLDX_NORM_*
   int place[4];            // of a, b, c, d in shared memory (values); -1: a is scale, c one, b and d zero
@@ -89,14 +99,16 @@ struct TeamSum {
   }
 };
 
-// Threads that run on an SM at once, from their registers: 80 with vectors of eight, 64 in CTAs of up to 1024, 128 else.
+// Threads that run on an SM at once, from their registers: 80 with vectors of eight and with single values, 64 in CTAs of up to
+// 1024, 128 else.
 template <int V, int kThreads>
-constexpr int kNormResident = kThreads > 256 ? 1024 : V == 8 ? 768 : 512;
+constexpr int kNormResident = kThreads > 256 ? 1024 : V == 8 || V == 1 ? 768 : 512;  // (V == 0: with vectors of groups)
 
-// V values at a time, which divides the width; kLanes: of a row, or of one of its warps.
-template <typename TY, typename TH, int V, int kLanes, int kThreads>
-__global__ void __launch_bounds__(kThreads, kNormResident<V, kThreads> / kThreads) block_norms_kernel(const __grid_constant__ NormsParams P) {
-  constexpr int E = kNormValues, K = E / V, kStep = kLanes * V;
+// V values at a time, which divides the width; kLanes: of a row, or of one of its warps; kDirect: vectors of groups are
+// read beside the rows.
+template <typename TY, typename TH, int V, int kLanes, int kThreads, bool kDirect>
+__global__ void __launch_bounds__(kThreads, kNormResident<kDirect ? 0 : V, kThreads> / kThreads) block_norms_kernel(const __grid_constant__ NormsParams P) {
+  constexpr int E = kNormValues<V, kThreads>, K = E / V, kStep = kLanes * V;
   constexpr int kWarps = kThreads / 32;
   extern __shared__ __align__(16) float shared[];  // a, b, c, d
   __shared__ float places[2 * kWarps];
@@ -137,6 +149,22 @@ __global__ void __launch_bounds__(kThreads, kNormResident<V, kThreads> / kThread
   };
   load_y(row < row_end ? have : 0);
   load_h(row < row_end ? have : 0);
+  constexpr int kDirectVecs = kDirect ? K : 1;
+  Raw<TY, V> gate[kDirectVecs], scale[kDirectVecs], shift[kDirectVecs];
+  auto load_vector = [&](auto& to, const void* base, long long ld, long long of_row, int have) {
+    if constexpr (kDirect) {
+      if (!base) return;
+      const TY* from = static_cast<const TY*>(base) + static_cast<uint32_t>(of_row) / static_cast<uint32_t>(P.group) * ld + first;
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        if (k < have) to[k] = load_shared_by_rows<TY, V>(from + k * kStep);
+    }
+  };
+  if (row < row_end) {
+    load_vector(gate, P.row_gate, P.ld_gate, row, have);
+    load_vector(scale, P.row_scale, P.ld_scale, row, have);
+    load_vector(shift, P.row_shift, P.ld_shift, row, have);
+  }
 
   // a, b, c, d of group g, by `by` threads of which this is the `me`-th, four values at a time; threads of eight values
   // read theirs in two halves, each side by side with the other threads' (half: where the second ones begin)
@@ -249,12 +277,28 @@ __global__ void __launch_bounds__(kThreads, kNormResident<V, kThreads> / kThread
     };
     auto product = [](float2 a, float2 b) { return mul_f32x2(a, b); };
     auto plus = [](float2 a, float2 b) { return add_f32x2(a, b); };
+    // f(x, numbers) with those of the row's group
+    auto with_group = [&](const void* base, const auto& of, auto f) {
+      if constexpr (kDirect) {
+        if (!base) return;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          if (k >= have) continue;
+          float v[V];
+          unpack_row<TY, V>(of[k], v);
+#pragma unroll
+          for (int i = 0; i < V / 2; ++i) x[k * V / 2 + i] = f(x[k * V / 2 + i], make_float2(v[2 * i], v[2 * i + 1]));
+        }
+      }
+    };
     auto vector = [&](int k) -> const float(&)[V] { return *reinterpret_cast<const float(*)[V]>(reinterpret_cast<const float*>(x) + k * V); };
 
     const float post = P.post != RLDX_NORM_NONE ? inverse_size(P.post) : 1.0f;
     times(P.place[kNormA] < 0 ? P.scale * post : post);
     with(kNormA, product);
     with(kNormB, plus);
+    with_group(P.row_gate, gate, product);
+    load_vector(gate, P.row_gate, P.ld_gate, row + teams, next);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       float r[V];
@@ -271,6 +315,10 @@ __global__ void __launch_bounds__(kThreads, kNormResident<V, kThreads> / kThread
       times(inverse_size(P.pre));
       with(kNormC, product);
       with(kNormD, plus);
+      with_group(P.row_scale, scale, [](float2 a, float2 b) { return fma_f32x2(a, b, a); });
+      with_group(P.row_shift, shift, plus);
+      load_vector(scale, P.row_scale, P.ld_scale, row + teams, next);
+      load_vector(shift, P.row_shift, P.ld_shift, row + teams, next);
 #pragma unroll
       for (int k = 0; k < K; ++k)
         if (k < here) store_once<TY, V>(n_to + k * kStep, pack_row<TY, V>(vector(k)));
@@ -297,15 +345,15 @@ __global__ void __launch_bounds__(kThreads, kNormResident<V, kThreads> / kThread
   }
 }
 
-template <typename TY, typename TH, int V, int kLanes, int kThreads>
+template <typename TY, typename TH, int V, int kLanes, int kThreads, bool kDirect>
 cudaError_t launch_norms(NormsParams p, int values, cudaStream_t stream) {
   // as many teams as run at once, each with its run of rows
   const int block = p.warps > 1 ? 32 * p.warps : 128, teams = p.warps > 1 ? 1 : block / kLanes;
-  const long long resident = static_cast<long long>(sm_count()) * std::max(1, kNormResident<V, kThreads> / block) * teams;
+  const long long resident = static_cast<long long>(sm_count()) * std::max(1, kNormResident<kDirect ? 0 : V, kThreads> / block) * teams;
   p.run = static_cast<int>(std::max(1LL, (p.rows + resident - 1) / resident));
   const long long all_teams = (p.rows + p.run - 1) / p.run;
   const size_t smem = sizeof(float) * values * (p.copy ? teams : 1);
-  auto* kernel = block_norms_kernel<TY, TH, V, kLanes, kThreads>;
+  auto* kernel = block_norms_kernel<TY, TH, V, kLanes, kThreads, kDirect>;
   if (smem > 47 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kNormShared);
     if (e != cudaSuccess) return e;
@@ -313,11 +361,25 @@ cudaError_t launch_norms(NormsParams p, int values, cudaStream_t stream) {
   return launch_overlapped(kernel, static_cast<unsigned>((all_teams + teams - 1) / teams), static_cast<unsigned>(block), smem, stream, p);
 }
 template <typename TY, typename TH, int V>
-cudaError_t launch_block_norms(NormsParams p, bool grouped, const bool (&held)[4], cudaStream_t stream) {
-  // a row of up to 128 values is 8 lanes', of up to 512 a warp's
-  const int lanes = p.width <= 8 * kNormValues ? 8 : 32;
-  p.warps = (p.width + lanes * kNormValues - 1) / (lanes * kNormValues);
-  p.padded = lanes * p.warps * kNormValues;  // 14336 at most
+cudaError_t launch_block_norms(NormsParams p, bool grouped, bool direct, cudaStream_t stream) {
+  // a row of up to 8 lanes' values is theirs, else a warp's or several
+  constexpr int e = kNormValues<V, 256>;
+  const int lanes = p.width <= 8 * e ? 8 : 32;
+  const bool wide = p.width > 256 * e;
+  const int ev = wide ? kNormValues<V, 1024> : e;
+  p.warps = (p.width + lanes * ev - 1) / (lanes * ev);
+  p.padded = lanes * p.warps * ev;  // 14336 at most
+  p.row_gate = p.row_scale = p.row_shift = nullptr;
+  // Read beside the rows, the vectors of groups cost registers and their bytes with every row; made into four numbers, a barrier
+  // and a pass over the row's width with every group (us, 8832 x 2048 bf16, gate and modulation of groups of 1, 4, 16, 50 rows: 50, 40,
+  // 37, 36 against 112, 49, 35, 28; 100000 x 128, groups of 100: 21 against 29).
+  direct = direct && V > 1 && !wide && (lanes == 8 || p.group < 16);
+  if (direct) {
+    if (p.ld_gate) std::swap(p.gate, p.row_gate);
+    if (p.ld_scale || p.ld_shift) std::swap(p.mod_scale, p.row_scale), std::swap(p.mod_shift, p.row_shift);
+    grouped = false;
+  }
+  const bool held[4] = {p.post_w || p.gate, p.post_b != nullptr, p.pre_w || p.mod_scale, p.pre_b || p.mod_shift};
   int values = 0;
   for (int i = 0; i < 4; ++i) {
     p.place[i] = held[i] ? values : -1;
@@ -325,13 +387,15 @@ cudaError_t launch_block_norms(NormsParams p, bool grouped, const bool (&held)[4
   }
   if (!values) p.padded = 0;
   p.copy = grouped ? values : 0;
-  return lanes == 8      ? launch_norms<TY, TH, V, 8, 256>(p, values, stream)
-         : p.warps <= 8 ? launch_norms<TY, TH, V, 32, 256>(p, values, stream)
-                        : launch_norms<TY, TH, V, 32, 1024>(p, values, stream);
+  if constexpr (V > 1)
+    if (direct) return lanes == 8 ? launch_norms<TY, TH, V, 8, 256, true>(p, values, stream) : launch_norms<TY, TH, V, 32, 256, true>(p, values, stream);
+  return lanes == 8 ? launch_norms<TY, TH, V, 8, 256, false>(p, values, stream)
+         : !wide   ? launch_norms<TY, TH, V, 32, 256, false>(p, values, stream)
+                   : launch_norms<TY, TH, V, 32, 1024, false>(p, values, stream);
 }
 template <typename TY, typename TH>
-cudaError_t launch_block_norms(const NormsParams& p, bool whole, bool grouped, const bool (&held)[4], cudaStream_t stream) {
-  return whole ? launch_block_norms<TY, TH, 16 / sizeof(TY)>(p, grouped, held, stream) : launch_block_norms<TY, TH, 1>(p, grouped, held, stream);
+cudaError_t launch_block_norms(const NormsParams& p, bool whole, bool grouped, bool direct, cudaStream_t stream) {
+  return whole ? launch_block_norms<TY, TH, 16 / sizeof(TY)>(p, grouped, direct, stream) : launch_block_norms<TY, TH, 1>(p, grouped, false, stream);
 }
 }  // namespace
 
@@ -381,7 +445,7 @@ extern "C" int rldx_block_norms(const rldx_block_norms_desc* d, void* stream) {
   p.post_w = d->post_weight, p.post_b = d->post_bias, p.gate = d->gate, p.pre_w = d->pre_weight, p.pre_b = d->pre_bias;
   p.mod_scale = d->mod_scale, p.mod_shift = d->mod_shift;
   p.ld_gate = d->ld_gate, p.ld_scale = d->ld_scale, p.ld_shift = d->ld_shift;
-  p.rows = d->rows, p.group = d->rows_per_group;
+  p.rows = d->rows, p.group = std::min(d->rows_per_group, d->rows);  // (fits 31 bits)
   p.width = d->width, p.post = d->post, p.pre = d->pre;
   p.vectors_f32 = d->vector_dtype == RLDX_F32;
   p.scale = d->scale, p.eps = d->eps, p.plus_one = d->weight_plus_one ? 1.0f : 0.0f;
@@ -396,17 +460,18 @@ extern "C" int rldx_block_norms(const rldx_block_norms_desc* d, void* stream) {
   const int64_t vector_ld[7] = {0, 0, d->ld_gate, 0, 0, d->ld_scale, d->ld_shift};
   for (int i = 0; i < 7; ++i)
     if (!fits(vectors[i], vector_ld[i], sv, 4)) p.aligned = 0;
-  const bool held[4] = {d->post_weight || d->gate, d->post_bias != nullptr, d->pre_weight || d->mod_scale, d->pre_bias || d->mod_shift};
+  bool direct = grouped && sv == sy;  // the groups' vectors as the rows
+  for (int i : {2, 5, 6}) direct &= fits(vectors[i], vector_ld[i], sv, v);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool wide = d->residual_dtype == RLDX_F32;
   cudaError_t e;
   if (d->dtype == RLDX_F32)
-    e = launch_block_norms<float, float>(p, whole, grouped, held, st);
+    e = launch_block_norms<float, float>(p, whole, grouped, direct, st);
   else if (d->dtype == RLDX_F16)
-    e = wide ? launch_block_norms<__half, float>(p, whole, grouped, held, st) : launch_block_norms<__half, __half>(p, whole, grouped, held, st);
+    e = wide ? launch_block_norms<__half, float>(p, whole, grouped, direct, st) : launch_block_norms<__half, __half>(p, whole, grouped, direct, st);
   else
-    e = wide ? launch_block_norms<__nv_bfloat16, float>(p, whole, grouped, held, st)
-             : launch_block_norms<__nv_bfloat16, __nv_bfloat16>(p, whole, grouped, held, st);
+    e = wide ? launch_block_norms<__nv_bfloat16, float>(p, whole, grouped, direct, st)
+             : launch_block_norms<__nv_bfloat16, __nv_bfloat16>(p, whole, grouped, direct, st);
   if (e != cudaSuccess) return cuda_fail(e, "block_norms launch");
   return RLDX_OK;
 }

@@ -118,6 +118,22 @@ def test_strides_groups_and_vector_types(cuda, dtype, stream):
     check(one_row.expand(9, -1), rows_of(g, cuda, 9, 200, stream))
 
 
+@pytest.mark.parametrize("dtype,stream", TYPES)
+@pytest.mark.parametrize("width", [8, 128, 512, 1536, 4096, 4104])
+def test_groups_of_few_and_of_many_rows(cuda, dtype, stream, width):
+    """Rows enough that a CTA goes over several, groups that end inside its run, behind it and in each row."""
+    g = torch.Generator(device=cuda).manual_seed(width)
+    n = 9001 if width <= 512 else 2003
+    y, h = rows_of(g, cuda, n, width, dtype), rows_of(g, cuda, n, width, stream, 2.0)
+    for group in (1, 3, 15, 16, 700, n, n + 5, 2 ** 40):
+        count = -(-n // group)
+        wide = (0.5 * torch.randn(count, 2 * width, device=cuda, generator=g)).to(dtype)
+        gate = (0.5 * torch.randn(count, width, device=cuda, generator=g)).to(dtype)
+        check(y, h, post="rms", gate=gate, pre="layer", mod_scale=wide[:, :width], mod_shift=wide[:, width:], rows_per_group=group)
+        check(y, h, gate=gate[0], pre="rms", mod_shift=wide[:, :width], rows_per_group=group)
+        check(y, h, post="layer", post_bias=gate[0], gate=gate, pre=None, rows_per_group=group)
+
+
 @pytest.mark.parametrize("dtype,stream", [(BF, BF), (BF, F32), (F32, F32)])
 @pytest.mark.parametrize("width", [40, 2048, 1001])
 def test_in_place(cuda, dtype, stream, width):
