@@ -12,7 +12,9 @@
 // (1 + mod_scale), d = b (1 + mod_scale) + mod_shift, kept in shared memory and made once by a CTA.  Vectors of groups are
 // read beside the rows, as they are, where they have the rows' type and alignment; else each team makes its own four numbers
 // whenever it comes to another group.  A CTA goes over a run of rows, the next of which is on the way while one is
-// normed.  Bound by memory: y and h are read and h' and n written once.
+// normed.  Bound by memory: y and h are read and h' and n written once.  8832 x 2048 bf16 with norms on both sides takes 26 us
+// (5.6 TB/s; at the copy's rate 22), with channel gates 27, 35968 x 1536 with a modulation of each 562 rows 83 (68), 4999 x
+// 1001 fp16 with an fp32 stream 16.3 (9.2: one value at a time, and 450 instructions a warp and row of 512 values).
 #include <utility>
 
 #include "host_util.h"

@@ -17,6 +17,12 @@
 // other values are in a row, the missing places go to the lowest ids of -inf.  A queue that overflows (many values share the
 // bound, or logits rise along the row) is given up for lists of the warps that are cut down to k when they are full:
 // exact whatever the row, and some times slower.
+//
+// Measured: 2208 x 151680 bf16 with 20 alternatives takes 167 us (670 MB: 4.0 TB/s; at the copy's rate 102), without 129, without a
+// token to count before 120; 1104 x 151680 fp32 134; one row 7.2 with five alternatives; 64 x 50257 fp32 11.7.  Many rows are bound
+// by the instructions of a value (about 8: unpacked, compared, exponential on the special-function unit, two sums); the
+// alternatives add the barriers of the bounds and the end of a row, during which the CTA loads nothing.  512 x 151680: rows of
+// random logits 55 us, flat 120, descending 85, ascending 183, masked but for a few 128 to 193.
 #include <cfloat>
 
 #include "host_util.h"
