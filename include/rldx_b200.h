@@ -33,8 +33,8 @@ int rldx_version(void);
 const char* rldx_last_error(void);
 
 /* Reads and clears the device-side error (0 = none).  Synchronizes the device.  A wait that ran out comes first,
- * then what a kernel found in its data, left out and went on from (the cache operators' 0x500 to 0x502; these
- * stop no other call): both set take two calls. */
+ * then what a kernel found in its data, left out and went on from (the cache operators' 0x500 to 0x502, token_logprobs'
+ * 0x503; these stop no other call): both set take two calls. */
 int rldx_get_device_error(unsigned int* code);
 
 /* Bound of every wait inside the kernels, in SM clock cycles (default 4e9, about 2 s at full
@@ -709,7 +709,8 @@ typedef struct {
 } rldx_rope_heads;
 
 /* Turns one or two groups of heads (q and k) in one launch: fp32 arithmetic on angles reduced in
- * double, one rounding; values past 2 * pairs of a head are copied. */
+ * double, one rounding; values past 2 * pairs of a head are copied.  Inputs may repeat heads or tokens
+ * (strides of 0); outputs share no memory with an input but their own, place for place. */
 int rldx_rope(const rldx_rope_plan* plan, const rldx_rope_heads* heads, int nheads, int64_t tokens, int head_dim, int dtype,
               void* stream);
 /* cos and sin rows [tokens, 2 * pairs] of the plan's angles, pair i at i and i + pairs (the tables
