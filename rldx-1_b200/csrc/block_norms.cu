@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, kNormResident<kDirect ? 0 : V, kThre
       }
       return rsqrtf(total(s) + P.eps);
     };
-    // f(x, numbers) with those of a vector in shared memory (a is 0 past the width, and so are b, c and d)
+    // f(x, numbers) with those of a vector in shared memory (past the width x is 0, and b and d are)
     auto with = [&](int which, auto f) {
       const int place = P.place[which];
       if (place < 0) return;

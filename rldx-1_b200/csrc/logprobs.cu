@@ -117,7 +117,7 @@ struct LogprobsShared {
   uint4 maxima[64 / 4];
   uint32_t bound[2];      // of a chunk, and of the next one that finds one
   uint4 totals[kWarps];   // of the warps
-  u64 front[NT];          // keys that can be among the top
+  u64 front[NT];          // keys that can be among the top, in any order
   int queued, fronts, finalists;
   long long token;
   float x_token;
@@ -611,7 +611,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) logprobs_kernel(const __grid_co
     }
   }
 
-  // The warps leave their totals, and of their lists what reaches the bound, 32 at most.
+  // The warps leave their totals; of the queue's values those that reach the last bound go to the front.
   const Total mine = warp_total({p, better});
   if (lane == 0) s.totals[warp] = words_of(mine);
   if (top > 0) {

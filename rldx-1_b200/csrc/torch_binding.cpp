@@ -515,7 +515,7 @@ PyObject* block_norms(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (v.size(1) != width || (width > 1 && v.stride(1) != 1))
           refuse_value(std::string(names[i]) + " must be row-major [groups, " + std::to_string(width) + "]");
         if (d.rows_per_group < 1) refuse_value(std::string(names[i]) + " of groups needs rows_per_group");
-        if (v.size(0) != (rows + d.rows_per_group - 1) / d.rows_per_group)
+        if (v.size(0) != (rows > 0 ? 1 + (rows - 1) / d.rows_per_group : 0))
           refuse_value(std::string(names[i]) + " must have a row for each group of " + std::to_string(d.rows_per_group) + " rows");
         *ld[i] = v.size(0) > 1 ? v.stride(0) : 0;
       }
