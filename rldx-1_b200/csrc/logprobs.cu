@@ -687,15 +687,23 @@ cudaError_t launch_logprobs(const LogprobsParams& p, cudaStream_t stream) {
 }
 template <typename T>
 cudaError_t launch_logprobs(LogprobsParams p, cudaStream_t stream) {
-  // Threads of a CTA: 64 for rows of up to 8 KB, whose time is mostly the search for the top (8000 x 4096 bf16: 46 us, with 256
-  // 72), else 256.  CTAs of a row: up to 8, until they would take a quarter of the threads that run at once, and none with less
+  // Threads of a CTA.  A row's latency is shortest with 256, the search for its top costs least with 64, so the most threads are
+  // taken with which all rows run at once (1024 threads an SM), or in two turns if the rows are past 8 KB; no more than a row has
+  // vectors, and 256 past 64 KB, where the search no longer counts.  us with 64, 128 and 256, bf16:
+  //   x 4096: 300 rows 15.0  9.8  7.3, 600 rows 14.7  8.8 10.1, 4000 rows 26.3 28.3 42.7
+  //   x 16331: 300 rows 18.8 14.5 11.5, 1200 rows 30.4 26.0 25.7, 4000 rows 59.9 61.4 69.9;  4000 x 40000: 111 111 115
+  // CTAs of a row: up to 8, until they would take a quarter of the threads that run at once, and none with less
   // than a vector a thread.  (Up to half of them, us: 64 x 50257 fp32 14.3 against 11.6, 64 x 20000 12.2 against 7.8, 256 x
   // 151680 31.8 against 33.3; up to 16 CTAs a row: 8 x 151680 17.4 against 11.4, one row 14.6 against 10.5.)
   const long long vecs = static_cast<long long>(p.vocab) * sizeof(T) / 16;
-  const int nt = vecs <= 512 ? 64 : 256;
+  const long long at_once = (vecs <= 512 ? 1024LL : 2048LL) * sm_count();
+  int nt = 256;
+  while (nt > 64 && vecs <= 4096 && (vecs < nt || static_cast<long long>(p.rows) * nt > at_once)) nt /= 2;
   p.cluster = 1;
   while (p.cluster < kLogpMaxCluster && static_cast<long long>(p.rows) * p.cluster * nt < 384LL * sm_count() && vecs / (2 * p.cluster) >= nt) p.cluster *= 2;
-  return nt == 64 ? launch_logprobs<T, 64>(p, stream) : launch_logprobs<T, 256>(p, stream);
+  if (nt == 64) return launch_logprobs<T, 64>(p, stream);
+  if (nt == 128) return launch_logprobs<T, 128>(p, stream);
+  return launch_logprobs<T, 256>(p, stream);
 }
 }  // namespace
 

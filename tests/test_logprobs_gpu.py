@@ -87,6 +87,28 @@ def test_many_rows(cuda, dtype, vocab, rows):
         assert all(torch.equal(a[r: r + 1], b) for a, b in zip(whole[2:4], one[2:4]))
 
 
+@pytest.mark.parametrize("dtype,vocab,shift,rows", [
+    (F32, 511, 0, 5), (F32, 512, 0, 5), (F32, 1023, 1, 5), (F32, 1024, 0, 5), (BF, 4096, 0, 592), (BF, 4096, 0, 593), (BF, 4091, 3, 1184),
+    (F16, 4096, 0, 1185), (F16, 8191, 5, 1185), (BF, 4104, 0, 2368), (BF, 8191, 1, 2369), (F32, 16384, 0, 1200), (F32, 16388, 0, 1200)])
+def test_threads_of_a_row(cuda, dtype, vocab, shift, rows):
+    """The sizes at which a row goes to 64, 128 or 256 threads, from both sides, with rows of each awkward kind among the others."""
+    g = torch.Generator(device=cuda).manual_seed(rows + vocab)
+    x = rows_of(g, cuda, rows, vocab, dtype, spread=3.0, shift=shift)
+    n = torch.arange(vocab, device=cuda).float()
+    for first in {0, rows - 5}:
+        x[first] = 1.25
+        x[first + 1] = 30 * n / vocab
+        x[first + 2, : vocab * 9 // 10] = -math.inf
+        x[first + 3] = torch.finfo(dtype).min
+        x[first + 4] = (x[first + 4].float() * 2).round()
+    if rows > 20:
+        x[rows // 2] = -math.inf
+        x[rows // 2 + 1, vocab - 1] = math.nan
+    tokens = torch.randint(-1, vocab, (rows,), device=cuda, generator=g)
+    for top in (0, 1, 32):
+        check(x, tokens, top)
+
+
 @pytest.mark.parametrize("dtype", [BF, F16, F32])
 @pytest.mark.parametrize("vocab", [40, 3001, 40000, 151680])
 @pytest.mark.parametrize("rows", [12, 480])
