@@ -106,13 +106,61 @@ class B200KV4Cache:
         self.lengths[seq] = 0
 
 
+def _refuse_other_norm(norm, name: str) -> None:
+    """Raises for a norm that is not x / rms(x) * weight.  The weights alone do not say (some count from one), so a module that can
+    be called is asked: a weight taken from the other of the two is off by all of x / rms(x), roundings by a few 2^-8 of the result."""
+    if norm is None:
+        return
+    if getattr(norm, "bias", None) is not None:
+        raise NotImplementedError(f"{name} has a bias, which an RMSNorm has not")
+    if not callable(norm):
+        return
+    w = norm.weight.detach()
+    n = w.shape[0]
+    x = torch.linspace(-1.0, 2.0, n, device=w.device, dtype=torch.float32).to(w.dtype)
+    with torch.no_grad():
+        got = norm(x.expand(2, n))[0].float()
+    x = x.float()
+    hat = x * torch.rsqrt((x * x).mean())
+    want = hat * w.float()
+    if not bool(((got - want).abs() <= 2.0 ** -6 * (want.abs() + hat.abs())).all()):
+        raise NotImplementedError(f"{name} is not x / rms(x) * weight (1 + weight, a mean taken off, or another norm)")
+
+
+def _refuse_other_mlp(layer, i: int) -> None:
+    """Raises for an activation other than SiLU, where the layer has one to ask."""
+    act = getattr(layer.mlp, "act_fn", None)
+    if act is None:
+        return
+    name = act.lower() if isinstance(act, str) else None
+    x = torch.linspace(-8.0, 8.0, 65, device=layer.mlp.gate_proj.weight.device)
+    if name is None:
+        with torch.no_grad():
+            silu = bool(((act(x) - torch.nn.functional.silu(x)).abs() <= 2.0 ** -8 * (1 + x.abs())).all())
+    else:
+        silu = name in ("silu", "swish")
+    if not silu:
+        raise NotImplementedError(f"layer {i}'s MLP does not gate with SiLU")
+
+
+def _refuse_other_attention(layer, i: int) -> None:
+    """Raises for scores other than q k / sqrt(head_dim), where the layer says how it makes them."""
+    a = layer.self_attn
+    scale, d = getattr(a, "scaling", None), a.q_norm.weight.shape[0]
+    if scale is not None and abs(float(scale) * d ** 0.5 - 1) > 1e-5:
+        raise NotImplementedError(f"layer {i}'s attention scales by {float(scale)}, not by head_dim ** -0.5 = {d ** -0.5}")
+    if getattr(a, "attn_logit_softcapping", None) is not None:
+        raise NotImplementedError(f"layer {i}'s attention caps its scores")
+
+
 class B200TextDecoder:
     """Qwen3 decoder layers, embedding and output projection over a B200KV4Cache.
 
     Layers in a LayerWrapper that compresses video tokens (B200LLMChain's compress_info) would have to drop tokens from
     the cache of the layers after it, which no page table here can say: they are refused unless
     ignore_compression says that no prompt has what the wrapper compresses (it leaves one frame, and text, as
-    they are)."""
+    they are).  The norms are x / rms(x) * weight, the MLP's activation SiLU, the scores q k / sqrt(head_dim): layers whose modules
+    say otherwise are refused (norms of 1 + weight among them; their weights alone cannot tell)."""
 
     def __init__(self, layers, norm, embed: torch.Tensor, lm_head: torch.Tensor, cos: Optional[torch.Tensor] = None,
                  sin: Optional[torch.Tensor] = None, *, window: int = 0, sinks: int = 0, device=None, ignore_compression: bool = False,
@@ -134,6 +182,13 @@ class B200TextDecoder:
             if any(getattr(p, "bias", None) is not None for p in (a.q_proj, a.k_proj, a.v_proj, a.o_proj, m.mlp.gate_proj,
                                                                   m.mlp.up_proj, m.mlp.down_proj)):
                 raise NotImplementedError("Qwen3 projections have no bias; a biased layer is not bound")
+        norms = ("input_layernorm", "post_attention_layernorm", "pre_feedforward_layernorm", "post_feedforward_layernorm")
+        for i, m in enumerate(layers):
+            for at, name in [(m, n) for n in norms] + [(m.self_attn, "q_norm"), (m.self_attn, "k_norm")]:
+                _refuse_other_norm(getattr(at, name, None), f"layer {i}'s {name}")
+            _refuse_other_mlp(m, i)
+            _refuse_other_attention(m, i)
+        _refuse_other_norm(norm, "the final norm")
         self.head_dim = a0.q_norm.weight.shape[0]
         self.q_heads = a0.q_proj.weight.shape[0] // self.head_dim
         self.kv_heads = a0.k_proj.weight.shape[0] // self.head_dim
