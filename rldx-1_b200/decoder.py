@@ -106,6 +106,18 @@ class B200KV4Cache:
         self.lengths[seq] = 0
 
 
+def _whole(given, name: str, as_values: bool = False) -> torch.Tensor:
+    """Whole numbers as int64 on the host.  Others are refused, not cut: floats (as_values: those that are not whole) and bools."""
+    t = torch.as_tensor(given)
+    if t.numel():  # (an empty list comes as floats)
+        ok = t.dtype != torch.bool and not t.is_complex()
+        if ok and t.is_floating_point():
+            ok = as_values and bool(((t == t.trunc()) & (t.abs() < 2.0 ** 53)).all())
+        if not ok:
+            raise ValueError(f"{name} must be whole numbers, got {t.dtype}")
+    return t.to("cpu", torch.int64)
+
+
 def _refuse_other_norm(norm, name: str) -> None:
     """Raises for a norm that is not x / rms(x) * weight.  The weights alone do not say (some count from one), so a module that can
     be called is asked: a weight taken from the other of the two is off by all of x / rms(x), roundings by a few 2^-8 of the result."""
@@ -263,8 +275,10 @@ class B200TextDecoder:
             positions = torch.cat([torch.arange(s, s + n, dtype=torch.int32) for s, n in zip(start, new)])
         elif tuple(positions.shape) != (rows,) and (tables or tuple(positions.shape) != (self.rope.axes, rows)):
             raise ValueError(f"positions must be [{rows}]" + ("" if tables else f" or [{self.rope.axes}, {rows}]") + f", got {tuple(positions.shape)}")
-        elif tables and positions.device.type == "cpu" and not 0 <= int(positions.min()) <= int(positions.max()) < self.cos.shape[0]:
-            raise ValueError(f"positions must be rows of the RoPE tables ({self.cos.shape[0]})")  # (else device error 0x501)
+        elif tables and positions.device.type == "cpu":
+            positions = _whole(positions, "positions", True)
+            if not 0 <= int(positions.min()) <= int(positions.max()) < self.cos.shape[0]:
+                raise ValueError(f"positions must be rows of the RoPE tables ({self.cos.shape[0]})")  # (on the device: device error 0x501)
         elif not tables and (positions.dtype.is_floating_point or positions.dtype == torch.bool):
             raise ValueError("positions must be whole numbers")
         return positions
@@ -285,7 +299,7 @@ class B200TextDecoder:
         if features:
             if deepstack_rows is None:
                 raise ValueError("deepstack_features need deepstack_rows")
-            at = torch.as_tensor(deepstack_rows).to("cpu", torch.int64)  # (looked at on the host: rows outside would fault)
+            at = _whole(deepstack_rows, "deepstack_rows", True)  # (looked at on the host: rows outside would fault)
             if at.dim() != 1 or at.unique().numel() != at.numel() or (at.numel() and not 0 <= int(at.min()) <= int(at.max()) < sum(new)):
                 raise ValueError(f"deepstack_rows must be different rows of the {sum(new)} of hidden")
             if len(features) > len(self.layers) or any(tuple(f.shape) != (at.numel(), self.hidden) for f in features):
@@ -296,7 +310,7 @@ class B200TextDecoder:
         if features:
             at, features = at.to(self.device), [f.to(self.device, BF) for f in features]
         if self.rope is None:
-            cos, sin, positions = self.cos, self.sin, positions.to(self.device, torch.int32)
+            cos, sin, positions = self.cos, self.sin, positions.to(torch.int32).to(self.device)
         else:  # rows for these tokens alone
             positions = positions.to(self.device, torch.int64)
             if self.rope.sections is not None:
@@ -375,7 +389,7 @@ class B200TextDecoder:
         if targets is None:
             follow = [torch.full((n,), -1) if i is None else torch.cat([i[1:], torch.tensor([-1])]) for i, n in zip(ids, new)]
         else:
-            follow = [torch.as_tensor(t).to("cpu", torch.int64) for t in targets]
+            follow = [_whole(t, "targets") for t in targets]
             if [tuple(t.shape) for t in follow] != [(n,) for n in new]:
                 raise ValueError(f"targets must give {new} tokens, got {[tuple(t.shape) for t in follow]}")
         follow = torch.cat(follow)
@@ -398,20 +412,23 @@ class B200TextDecoder:
         """A prompt's ids (None where it is rows of embeddings) and its rows; refuses ids that the embedding does not have."""
         if torch.is_tensor(prompt) and prompt.dim() == 2:
             return None, prompt.to(self.device, BF)
-        ids = torch.as_tensor(prompt).to("cpu", torch.int64)
+        ids = _whole(prompt, "a prompt's ids")
+        if ids.dim() != 1:
+            raise ValueError(f"a prompt is ids [n] or rows of embeddings [n, {self.hidden}], got {tuple(ids.shape)}")
         if ids.numel() and not 0 <= int(ids.min()) <= int(ids.max()) < self.embed.shape[0]:  # (looked at on the host: others would fault)
             raise ValueError(f"a prompt's ids must be among the {self.embed.shape[0]} of the embedding")
         return ids, self.embed[ids.to(self.device)]
 
     def _prompt_places(self, positions: Sequence, new: Sequence[int]):
         """The prompts' positions, one after the other, and one past each one's largest; refuses other shapes."""
-        given = [torch.as_tensor(p).to("cpu", torch.int32 if self.rope is None else torch.int64) for p in positions]
+        given = [torch.as_tensor(p) for p in positions]
         wanted = [(n,) for n in new]
         if self.rope is not None:  # one position for all axes, or each
             given = [p.expand(self.rope.axes, -1) if p.dim() == 1 else p for p in given]
             wanted = [(self.rope.axes, n) for n in new]
         if [tuple(p.shape) for p in given] != wanted:
             raise ValueError(f"positions must give {list(new)} rows, got {[tuple(p.shape) for p in given]}")
+        given = [_whole(p, "positions", self.rope is None) for p in given]
         return torch.cat(given, -1), [int(p.max()) + 1 for p in given]
 
     def generate(self, prompts, max_new_tokens: int, *, u: torch.Tensor, cache: Optional[B200KV4Cache] = None,
@@ -446,7 +463,8 @@ class B200TextDecoder:
         places = follow = None
         if positions is not None:
             places, past = self._prompt_places(positions, [r.shape[0] for r in rows])
-            follow = torch.tensor(past if next_positions is None else [int(p) for p in next_positions], dtype=places.dtype)
+            follow = torch.tensor(past) if next_positions is None else \
+                _whole(next_positions if torch.is_tensor(next_positions) else list(next_positions), "next_positions", True)
             if follow.shape != (n,):
                 raise ValueError(f"next_positions must be {n} rows")
             if self.rope is None and not (0 <= int(places.min()) and int(places.max()) < self.cos.shape[0] and

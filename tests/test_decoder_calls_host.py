@@ -1,0 +1,77 @@
+"""B200TextDecoder's calls without a GPU: what they refuse before the cache changes, and what they hand on."""
+
+import math
+
+import pytest
+import torch
+
+import rldx_b200  # noqa: F401
+from rldx_b200 import decoder  # noqa: F401
+from rldx_b200.decoder import B200TextDecoder
+from rldx_b200.rope import B200Rope
+
+from test_decoder_host import BF, HEAD, HIDDEN, ROWS, VOCAB, layer, make, refused, state, weight
+
+
+def roped(**kw):
+    return B200TextDecoder([layer(), layer()], weight(HIDDEN), torch.zeros(VOCAB, HIDDEN), torch.zeros(VOCAB, HIDDEN), device="cpu",
+                           rope=B200Rope(HEAD, sections=(16, 8, 8), device="cpu"), **kw)
+
+
+@pytest.mark.parametrize("build", [make, roped])
+def test_ids_are_whole_numbers(build):
+    """Floats and bools were cut to whole numbers and ran."""
+    dec, u = build(), torch.zeros(2, 2)
+    cache = dec.new_cache(2, 256)
+    before = state(cache)
+    for ids in ([0.4, 3.6], [1.0, 2.0], [math.nan], torch.tensor([1.0]), [True, False], torch.tensor([True, False]), torch.tensor([1 + 2j])):
+        with pytest.raises(ValueError, match="ids must be whole numbers"):
+            dec.generate([[1], ids], 2, u=u, cache=cache)
+        with pytest.raises(ValueError, match="ids must be whole numbers"):
+            dec.score([[1], ids], cache=cache)
+    for ids in (torch.tensor(3), [[1, 2]], torch.zeros(1, 2, HIDDEN, dtype=torch.int64)):
+        with pytest.raises(ValueError, match="a prompt is ids"):
+            dec.generate([[1], ids], 2, u=u, cache=cache)
+    for target in ([0.4, 3.6], [1.0, 2.0], [math.nan, 1.0], [True, False], torch.tensor([1.0, 2.0])):
+        with pytest.raises(ValueError, match="targets must be whole numbers"):
+            dec.score([[1], [2, 3]], targets=[[1], target], cache=cache)
+    assert state(cache) == before
+
+
+def test_positions_are_whole_numbers():
+    u = torch.zeros(2, 2)
+    tables, rope = make(), roped()
+    cache = tables.new_cache(2, 256)
+    before = state(cache)
+    for bad in ([0.5, 1.0], [math.nan, 1.0], [math.inf, 1.0], [True, False], torch.tensor([0.0, 1.5])):
+        for dec in (tables, rope):
+            with pytest.raises(ValueError, match="positions must be whole numbers"):
+                dec.generate([[1], [2, 3]], 2, u=u, positions=[[0], bad], cache=cache)
+            with pytest.raises(ValueError, match="positions must be whole numbers"):
+                dec.score([[1], [2, 3]], positions=[[0], bad], cache=cache)
+        for dec in (tables, rope):
+            with pytest.raises(ValueError, match="next_positions must be whole numbers"):
+                dec.generate([[1], [2, 3]], 2, u=u, positions=[[0], [0, 1]], next_positions=bad, cache=cache)
+        refused(tables, cache, ValueError, "positions must be whole numbers", torch.zeros(2, HIDDEN, dtype=BF), [0, 2], positions=torch.as_tensor(bad))
+        with pytest.raises(ValueError, match="deepstack_rows must be whole numbers"):
+            tables.forward(torch.zeros(2, HIDDEN, dtype=BF), cache, [0, 2], deepstack_features=[torch.zeros(2, HIDDEN)], deepstack_rows=bad)
+    with pytest.raises(ValueError, match="rows of the RoPE tables"):  # (cut to 32 bits it was row 5)
+        tables.generate([[1], [2, 3]], 2, u=u, positions=[[2 ** 32 + 5], [0, 1]], cache=cache)
+    assert state(cache) == before
+
+
+def test_whole_positions_of_any_type_are_handed_on(monkeypatch):
+    dec, seen = make(), []
+
+    def forward(hidden, cache, new, positions=None):
+        seen.append(positions.tolist())
+        cache.extend(new)
+
+    monkeypatch.setattr(decoder.ops, "sample", lambda *a, **kw: (torch.tensor([1, 2]), None, None))
+    monkeypatch.setattr(decoder.ops, "device_error", lambda: 0)
+    monkeypatch.setattr(dec, "forward", forward)
+    for p in ([0.0, 4.0], torch.tensor([0, 4], dtype=torch.uint8), torch.tensor([0, 4], dtype=torch.int32)):
+        for follow in ([5, 9], (5.0, 9.0), iter([5, 9]), torch.tensor([5, 9], dtype=torch.int16), [torch.tensor(5), torch.tensor(9)]):
+            dec.generate([[1], [2, 3]], 2, u=torch.zeros(2, 2), positions=[[ROWS - 1], p], next_positions=follow)
+            assert seen == [[ROWS - 1, 0, 4], [5, 9]]
+            del seen[:]
