@@ -206,6 +206,7 @@ class B200TextDecoder:
         self.kv_heads = a0.k_proj.weight.shape[0] // self.head_dim
         self.hidden = embed.shape[1]
         self.window, self.sinks = int(window), int(sinks)
+        self._refuse_other_shapes(layers, norm, embed, lm_head)
         ln = layers[0].input_layernorm
         self.eps = float(getattr(ln, "variance_epsilon", getattr(ln, "eps", 1e-6)))
 
@@ -244,6 +245,38 @@ class B200TextDecoder:
         if (cos.dim() != 2 or cos.shape[1] != self.head_dim or sin.shape != cos.shape or sin.dtype != cos.dtype or
                 cos.dtype not in (torch.float32, BF)):
             raise ValueError(f"cos and sin must be [rows, {self.head_dim}], both float32 or both bfloat16")
+
+    def _refuse_other_shapes(self, layers, norm, embed, lm_head) -> None:
+        """Raises for a model that a step would refuse at one of its kernels, when the cache has changed."""
+        d, hidden, q, kv = self.head_dim, self.hidden, self.q_heads * self.head_dim, self.kv_heads * self.head_dim
+        if d not in (64, 128) or self.kv_heads < 1 or self.q_heads % self.kv_heads:
+            raise NotImplementedError(f"heads of 64 or 128 values are run, each key / value head's with as many query heads; got {self.q_heads} "
+                                      f"query and {self.kv_heads} key / value heads of {d}")
+        if hidden % 8 or not 8 <= hidden <= 4096:
+            raise NotImplementedError(f"hidden must be a multiple of 8, 4096 at most (the norms' rows), got {hidden}")
+        if self.window < 0 or self.sinks < 0:
+            raise ValueError(f"window and sinks must not be negative, got {self.window} and {self.sinks}")
+
+        def has(t, name, *shape):
+            if tuple(t.shape) != shape:
+                raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+
+        for i, m in enumerate(layers):
+            a, ffn = m.self_attn, m.mlp.gate_proj.weight.shape[0]
+            if ffn % 8 or ffn < 8:
+                raise NotImplementedError(f"layer {i}'s MLP must have a multiple of 8 values, got {ffn}")
+            for at, name, *shape in ((a, "q_proj", q, hidden), (a, "k_proj", kv, hidden), (a, "v_proj", kv, hidden), (a, "o_proj", hidden, q),
+                                     (a, "q_norm", d), (a, "k_norm", d), (m.mlp, "gate_proj", ffn, hidden), (m.mlp, "up_proj", ffn, hidden),
+                                     (m.mlp, "down_proj", hidden, ffn), (m, "input_layernorm", hidden), (m, "post_attention_layernorm", hidden),
+                                     (m, "pre_feedforward_layernorm", hidden), (m, "post_feedforward_layernorm", hidden)):
+                part = getattr(at, name, None)
+                if part is not None:
+                    has(part.weight, f"layer {i}'s {name}", *shape)
+        has(norm.weight, "the final norm", hidden)
+        for t, name in ((embed, "embed"), (lm_head, "lm_head")):
+            has(t, name, t.shape[0], hidden)
+            if t.shape[0] < 1:
+                raise ValueError(f"{name} has no tokens")
 
     def new_cache(self, seqs: int, max_tokens: int, page_size: int = 64) -> B200KV4Cache:
         return B200KV4Cache(len(self.layers), self.kv_heads, self.head_dim, seqs, max_tokens, page_size, self.device)
