@@ -340,6 +340,9 @@ class B200TextDecoder:
         elif deepstack_rows is not None:
             raise ValueError("deepstack_rows go with deepstack_features")
         self._here(cache, hidden=hidden)
+        hidden = hidden.contiguous()  # (what a product adds, and the first norm reads, begins at 16 bytes)
+        if hidden.data_ptr() % 16:
+            hidden = hidden.clone()
         if features:
             at, features = at.to(self.device), [f.to(self.device, BF) for f in features]
         if self.rope is None:

@@ -75,3 +75,36 @@ def test_whole_positions_of_any_type_are_handed_on(monkeypatch):
             dec.generate([[1], [2, 3]], 2, u=torch.zeros(2, 2), positions=[[ROWS - 1], p], next_positions=follow)
             assert seen == [[ROWS - 1, 0, 4], [5, 9]]
             del seen[:]
+
+
+class Stop(Exception):
+    pass
+
+
+def first_norm(monkeypatch, dec):
+    """What a step hands to its first norm, in place of running it."""
+    seen = []
+
+    def norm(x, weight):
+        seen.append(x)
+        raise Stop
+
+    monkeypatch.setattr(dec, "_here", lambda *a, **kw: None)
+    monkeypatch.setattr(dec, "_rmsnorm", norm)
+    return seen
+
+
+@pytest.mark.parametrize("scale", [1.0, 0.5])
+def test_rows_of_any_layout_are_run(monkeypatch, scale):
+    """Columns first or off 16 bytes, they were refused in mid-step: the cache had their tokens."""
+    dec = make(residual_scale=scale)
+    seen = first_norm(monkeypatch, dec)
+    rows = torch.randn(5, HIDDEN).to(BF)
+    off = torch.zeros(5 * HIDDEN + 1, dtype=BF)[1:].view(5, HIDDEN)
+    wide = torch.zeros(5, HIDDEN + 3, dtype=BF)[:, 1: 1 + HIDDEN]
+    for x in (rows, rows.t().contiguous().t(), off.copy_(rows), wide.copy_(rows)):
+        with pytest.raises(Stop):
+            dec.forward(x, dec.new_cache(1, 64), [5])
+        got = seen.pop()
+        assert torch.equal(got, rows) and got.is_contiguous() and got.data_ptr() % 16 == 0
+    assert rows.is_contiguous()
