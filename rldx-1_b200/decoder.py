@@ -348,7 +348,7 @@ class B200TextDecoder:
         if self.rope is None:
             cos, sin, positions = self.cos, self.sin, positions.to(torch.int32).to(self.device)
         else:  # rows for these tokens alone
-            positions = positions.to(self.device, torch.int64)
+            positions = positions.to(self.device, torch.int64).contiguous()  # (an axis' positions side by side)
             if self.rope.sections is not None:
                 positions = positions.expand(self.rope.axes, -1)
             elif positions.dim() == 2:

@@ -108,3 +108,27 @@ def test_rows_of_any_layout_are_run(monkeypatch, scale):
         got = seen.pop()
         assert torch.equal(got, rows) and got.is_contiguous() and got.data_ptr() % 16 == 0
     assert rows.is_contiguous()
+
+
+def test_positions_of_any_layout_reach_the_rope(monkeypatch):
+    """[axes, rows] that lie the other way round, or every other one, were refused; an axis' positions go side by side."""
+    dec, seen = roped(), []
+    first_norm(monkeypatch, dec)
+
+    def rows(positions):
+        seen.append(positions)
+        return torch.zeros(4, HEAD), torch.zeros(4, HEAD)
+
+    monkeypatch.setattr(dec.rope, "rows", rows)
+    at = torch.arange(12).view(3, 4)
+    every = torch.zeros(3, 8, dtype=torch.int32)[:, ::2]
+    for p in (at, at.t().contiguous().t(), every.copy_(at), at.to(torch.int16)):
+        with pytest.raises(Stop):
+            dec.forward(torch.zeros(4, HIDDEN, dtype=BF), dec.new_cache(1, 64), [4], p)
+        got = seen.pop()
+        assert torch.equal(got, at) and got.dtype == torch.int64 and got.stride(1) == 1
+    one = torch.arange(8)[::2]
+    with pytest.raises(Stop):
+        dec.forward(torch.zeros(4, HIDDEN, dtype=BF), dec.new_cache(1, 64), [4], one)
+    got = seen.pop()
+    assert torch.equal(got, one.expand(3, -1)) and got.stride(1) == 1
