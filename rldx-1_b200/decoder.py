@@ -405,6 +405,7 @@ class B200TextDecoder:
         layer i to the rows deepstack_rows [n] of hidden (a vision tower's, as B200LLMChain takes them), with one
         rounding to bf16.  Returns logits [seqs with new tokens, vocab]
         of each sequence's last new token."""
+        new = [int(n) for n in new]
         normed = self._run(hidden, cache, new, positions, deepstack_features, deepstack_rows)
         last = torch.tensor([e - 1 for n, e in zip(new, torch.tensor(new).cumsum(0).tolist()) if n], device=self.device)
         return ops.linear(normed(last).contiguous(), self.lm_head)

@@ -132,3 +132,14 @@ def test_positions_of_any_layout_reach_the_rope(monkeypatch):
         dec.forward(torch.zeros(4, HIDDEN, dtype=BF), dec.new_cache(1, 64), [4], one)
     got = seen.pop()
     assert torch.equal(got, one.expand(3, -1)) and got.stride(1) == 1
+
+
+def test_counts_may_come_from_an_iterator(monkeypatch):
+    """They were used up before the last rows were picked: no logits."""
+    dec, last = make(), []
+    monkeypatch.setattr(dec, "_run", lambda hidden, cache, new, *a: last.append(list(new)) or (lambda rows: last.append(rows.tolist()) or torch.zeros(len(rows), HIDDEN)))
+    monkeypatch.setattr(decoder.ops, "linear", lambda x, w: x)
+    for new in ([2, 0, 3], iter([2, 0, 3]), (n for n in (2, 0, 3)), torch.tensor([2, 0, 3])):
+        assert dec.forward(torch.zeros(5, HIDDEN, dtype=BF), None, new).shape == (2, HIDDEN)
+        assert last == [[2, 0, 3], [1, 4]]
+        del last[:]
