@@ -27,6 +27,7 @@ from __future__ import annotations
 
 import argparse
 import ctypes as C
+import operator
 from typing import NamedTuple, Optional, Sequence
 
 import torch
@@ -421,8 +422,7 @@ class B200TextDecoder:
         new = [r.shape[0] for r in rows]
         if not new or min(new) == 0:
             raise ValueError("a prompt has no token")
-        if not 0 <= top <= min(32, self.lm_head.shape[0]):
-            raise ValueError(f"top must be 0 to {min(32, self.lm_head.shape[0])}, got {top}")
+        top = self._alternatives(top, "top")
         if targets is None:
             follow = [torch.full((n,), -1) if i is None else torch.cat([i[1:], torch.tensor([-1])]) for i, n in zip(ids, new)]
         else:
@@ -444,6 +444,13 @@ class B200TextDecoder:
             at = slice(a, min(a + step, total))
             parts.append(ops.token_logprobs(ops.linear(normed(at).contiguous(), self.lm_head), follow[at], top=top))
         return [Scores(*part) for part in zip(*(torch.cat(t).split(list(new)) for t in zip(*parts)))]
+
+    def _alternatives(self, n, name: str) -> int:
+        """A number of alternatives that token_logprobs takes; refuses others, fractions with a TypeError."""
+        n, most = operator.index(n), min(32, self.lm_head.shape[0])
+        if not 0 <= n <= most:
+            raise ValueError(f"{name} must be 0 to {most}, got {n}")
+        return n
 
     def _rows(self, prompt):
         """A prompt's ids (None where it is rows of embeddings) and its rows; refuses ids that the embedding does not have."""
@@ -519,8 +526,8 @@ class B200TextDecoder:
         deep = {} if deepstack_features is None else dict(deepstack_features=deepstack_features, deepstack_rows=deepstack_rows)
         if not deep and deepstack_rows is not None:
             raise ValueError("deepstack_rows go with deepstack_features")
-        if logprobs is not None and not 0 <= logprobs <= min(32, self.lm_head.shape[0]):
-            raise ValueError(f"logprobs must be 0 to {min(32, self.lm_head.shape[0])}, got {logprobs}")
+        if logprobs is not None:
+            logprobs = self._alternatives(logprobs, "logprobs")
         hidden, new, tokens, scores = torch.cat(rows), [r.shape[0] for r in rows], [], []
         for i in range(max_new_tokens):
             logits = self.forward(hidden, cache, new, places, **deep)

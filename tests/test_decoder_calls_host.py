@@ -143,3 +143,19 @@ def test_counts_may_come_from_an_iterator(monkeypatch):
         assert dec.forward(torch.zeros(5, HIDDEN, dtype=BF), None, new).shape == (2, HIDDEN)
         assert last == [[2, 0, 3], [1, 4]]
         del last[:]
+
+
+@pytest.mark.parametrize("n", [2.5, 2.0, "2", math.nan, None])
+def test_numbers_of_alternatives_are_whole(n, monkeypatch):
+    """A fraction was refused behind the step, which had filled the cache."""
+    dec = make()
+    cache = dec.new_cache(2, 256)
+    before = state(cache)
+    for name in ("_run", "forward"):
+        monkeypatch.setattr(dec, name, lambda *a, **kw: pytest.fail("a step was run"))
+    with pytest.raises(TypeError):
+        dec.score([[1], [2, 3]], top=n, cache=cache)
+    if n is not None:  # (None: no scores)
+        with pytest.raises(TypeError):
+            dec.generate([[1], [2, 3]], 2, u=torch.zeros(2, 2), logprobs=n, cache=cache)
+    assert state(cache) == before
