@@ -417,7 +417,8 @@ class B200TextDecoder:
         """How likely the prompts' own tokens are: for each prompt (ids, or rows of embeddings) Scores whose entry i is about the
         token that follows its row i: targets[prompt][i], by default the prompt's next id, and none (-1: logprob 0, rank -1)
         behind the last one or where the prompt is rows.  Its entropy and `top` (0 to 32) alternatives are there either way.  Logits
-        are made for a few thousand rows at a time.  positions, deepstack_features and deepstack_rows are generate()'s."""
+        are made for a few thousand rows at a time.  positions, deepstack_features and deepstack_rows are generate()'s.  An error that a
+        kernel has recorded on the device raises RldxError."""
         ids, rows = zip(*(self._rows(p) for p in prompts)) if len(prompts) else ((), ())
         new = [r.shape[0] for r in rows]
         if not new or min(new) == 0:
@@ -443,7 +444,14 @@ class B200TextDecoder:
         for a in range(0, total, step):
             at = slice(a, min(a + step, total))
             parts.append(ops.token_logprobs(ops.linear(normed(at).contiguous(), self.lm_head), follow[at], top=top))
+        self._report("tokens were scored")
         return [Scores(*part) for part in zip(*(torch.cat(t).split(list(new)) for t in zip(*parts)))]
+
+    def _report(self, what: str) -> None:
+        """Raises a device error that a kernel has recorded: what came out is not of all the data."""
+        code = ops.device_error()
+        if code:
+            raise _lib.RldxError(_lib.RLDX_ERR_DEVICE, f"device error 0x{code:x} recorded while {what}, or left by earlier work")
 
     def _alternatives(self, n, name: str) -> int:
         """A number of alternatives that token_logprobs takes; refuses others, fractions with a TypeError."""
@@ -538,9 +546,7 @@ class B200TextDecoder:
             deep = {}
             hidden, new, places = self.embed[token], [1] * n, None if follow is None else follow + i
         out = torch.stack(tokens, 1).tolist() if tokens else [[] for _ in prompts]
-        code = ops.device_error()
-        if code:
-            raise _lib.RldxError(_lib.RLDX_ERR_DEVICE, f"device error 0x{code:x} recorded while tokens were generated, or left by earlier work")
+        self._report("tokens were generated")
         for s, ids in enumerate(out):
             end = next((k for k, t in enumerate(ids) if t in stop_ids), None)
             if end is not None:

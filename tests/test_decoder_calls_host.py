@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import rldx_b200  # noqa: F401
-from rldx_b200 import decoder  # noqa: F401
+from rldx_b200 import _lib, decoder
 from rldx_b200.decoder import B200TextDecoder
 from rldx_b200.rope import B200Rope
 
@@ -159,3 +159,35 @@ def test_numbers_of_alternatives_are_whole(n, monkeypatch):
         with pytest.raises(TypeError):
             dec.generate([[1], [2, 3]], 2, u=torch.zeros(2, 2), logprobs=n, cache=cache)
     assert state(cache) == before
+
+
+def scored(monkeypatch, dec, code=0):
+    """score() with no device: logits of zeros, and scores that count the rows."""
+    made = []
+
+    def run(hidden, cache, new, *a):
+        cache.extend(new)
+        return lambda rows: hidden[rows]
+
+    def logprobs(logits, tokens, top):
+        n, first = len(tokens), sum(made)
+        made.append(n)
+        row = torch.arange(first, first + n)
+        return row.float(), row.float(), tokens.int(), row[:, None].expand(n, top), row[:, None].expand(n, top).float()
+
+    monkeypatch.setattr(dec, "_run", run)
+    monkeypatch.setattr(decoder.ops, "linear", lambda x, w: x)
+    monkeypatch.setattr(decoder.ops, "token_logprobs", logprobs)
+    monkeypatch.setattr(decoder.ops, "device_error", lambda: code)
+    return made
+
+
+def test_score_reports_device_errors(monkeypatch):
+    """As generate() does: scores of what a kernel left out came back as if they were whole."""
+    dec = make()
+    scored(monkeypatch, dec, 0x500)
+    with pytest.raises(_lib.RldxError, match="0x500") as e:
+        dec.score([[1], [2, 3]])
+    assert e.value.code == _lib.RLDX_ERR_DEVICE
+    scored(monkeypatch, dec)
+    assert [s.rank.tolist() for s in dec.score([[1], [2, 3]], top=2)] == [[-1], [3, -1]]
