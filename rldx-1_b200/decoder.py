@@ -175,6 +175,8 @@ class B200TextDecoder:
     they are).  The norms are x / rms(x) * weight, the MLP's activation SiLU, the scores q k / sqrt(head_dim): layers whose modules
     say otherwise are refused (norms of 1 + weight among them; their weights alone cannot tell)."""
 
+    score_logits = 2 ** 29  # that score() makes at a time: a gibibyte
+
     def __init__(self, layers, norm, embed: torch.Tensor, lm_head: torch.Tensor, cos: Optional[torch.Tensor] = None,
                  sin: Optional[torch.Tensor] = None, *, window: int = 0, sinks: int = 0, device=None, ignore_compression: bool = False,
                  rope: Optional[B200Rope] = None, residual_scale: float = 1.0):
@@ -440,7 +442,7 @@ class B200TextDecoder:
         places = None if positions is None else self._prompt_places(positions, new)[0]
         normed = self._run(torch.cat(rows), cache, new, places, deepstack_features, deepstack_rows)
         follow, total, parts = follow.to(self.device), sum(new), []
-        step = max(1, 2 ** 29 // self.lm_head.shape[0])  # a gibibyte of logits
+        step = max(1, self.score_logits // self.lm_head.shape[0])
         for a in range(0, total, step):
             at = slice(a, min(a + step, total))
             parts.append(ops.token_logprobs(ops.linear(normed(at).contiguous(), self.lm_head), follow[at], top=top))

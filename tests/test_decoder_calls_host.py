@@ -191,3 +191,15 @@ def test_score_reports_device_errors(monkeypatch):
     assert e.value.code == _lib.RLDX_ERR_DEVICE
     scored(monkeypatch, dec)
     assert [s.rank.tolist() for s in dec.score([[1], [2, 3]], top=2)] == [[-1], [3, -1]]
+
+
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 100])
+def test_scores_of_pieces_join(monkeypatch, rows):
+    """Logits are made for some rows at a time; the pieces end inside prompts."""
+    dec = make()
+    made = scored(monkeypatch, dec)
+    dec.score_logits = rows * VOCAB + VOCAB - 1
+    got = dec.score([[1, 2, 3, 4], [5], [6, 7]], top=2)
+    assert made == [min(rows, 7 - a) for a in range(0, 7, rows)]
+    assert [s.rank.tolist() for s in got] == [[2, 3, 4, -1], [-1], [7, -1]]
+    assert [s.logprob.tolist() for s in got] == [[0, 1, 2, 3], [4], [5, 6]] and [s.top_ids.tolist() for s in got][2] == [[5, 5], [6, 6]]
