@@ -723,6 +723,9 @@ extern "C" int rldx_token_logprobs(const void* logits, int64_t ld, int rows, int
   if (rows == 0) return RLDX_OK;
   if (!logits || !tokens || !logprob || !entropy || !rank || (top && (!top_ids || !top_logprobs))) return bad("null pointer");
   if (reinterpret_cast<uintptr_t>(logits) % dtype_bytes(dtype)) return bad("misaligned logits");
+  auto off = [](const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; };
+  if (off(tokens, 8) || off(logprob, 4) || off(entropy, 4) || off(rank, 4) || (top && (off(top_ids, 8) || off(top_logprobs, 4))))
+    return bad("misaligned tokens or results");
   int rc = ensure_device();
   if (rc != RLDX_OK) return rc;
   LogprobsParams p;
