@@ -423,6 +423,9 @@ PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
         writes_apart(*given[i], out_names[i], x[i], names[i]);
         if (x[1 - i] && !Span(*given[i]).apart_from(Span(*x[1 - i])))
           refuse_value(std::string(out_names[i]) + " shares memory with " + names[1 - i]);
+        for (const at::Tensor* t : {plan.positions, plan.freqs})  // (other blocks read them still)
+          if (!Span(*given[i]).apart_from(Span(*t)))
+            refuse_value(std::string(out_names[i]) + " shares memory with " + (t == plan.freqs ? "freqs" : "positions"));
       }
     }
     if (given[0] && given[1] && !Span(*given[0]).apart_from(Span(*given[1]))) refuse_value("out_q and out_k share memory");

@@ -20,3 +20,18 @@ def test_logprobs_pointers_are_aligned(lib):
     for kw in (dict(tokens=260), dict(tokens=257), dict(logprob=258), dict(entropy=257), dict(rank=258), dict(ids=260), dict(values=258)):
         assert call(**kw) == _lib.RLDX_ERR_ARG, kw
         assert b"misaligned" in lib.rldx_last_error()
+
+
+def test_rope_results_are_apart_from_positions_and_freqs():
+    """A block may turn its tokens while another still reads them."""
+    words = torch.zeros(1024, dtype=torch.int64)
+    heads = words.view(BF)[: 6 * 4 * 64].unflatten(0, (6, 4, 64))
+    q, at, f = torch.zeros(6, 4, 64, dtype=BF), torch.arange(6), torch.ones(32, dtype=F64)
+    for kw, match in ((dict(at=words[:6]), "out_q shares memory with positions"), (dict(at=words[383:389]), "out_q shares memory with positions"),
+                      (dict(at=words[:18].view(3, 6), sections=(16, 8, 8)), "out_q shares memory with positions"),
+                      (dict(f=words[100:132].view(F64)), "out_q shares memory with freqs"), (dict(at=words[384:390]), "CUDA")):
+        place, freqs = kw.pop("at", at), kw.pop("f", f)
+        with pytest.raises(ValueError, match=match):
+            ops.rope(q, None, place, freqs, out_q=heads, **kw)
+    with pytest.raises(ValueError, match="out_k shares memory with freqs"):
+        ops.rope(torch.zeros(6, 4, 64, dtype=BF), q, at, words[100:132].view(F64), out_k=heads)
