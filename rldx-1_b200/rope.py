@@ -25,7 +25,10 @@ def frequencies(rotary_dim: int, theta: float, scaling: Optional[dict] = None):
     """float64 [rotary_dim / 2] radians a position on the CPU, and the factor on cos and sin."""
     i = torch.arange(0, rotary_dim, 2, dtype=torch.float64)
     scaling = dict(scaling or {"type": None})
-    kind, s = scaling.pop("type", None), float(scaling.pop("factor", 1.0))
+    kind, s = scaling.pop("type", None), scaling.pop("factor", None)
+    if kind is None and s is not None:
+        raise ValueError("a scaling's factor needs its type")
+    s = 1.0 if s is None else float(s)
     if not (math.isfinite(theta) and theta > 0 and math.isfinite(s) and s > 0):
         raise ValueError("theta and the scaling's factor must be positive numbers")
     m = 1.0

@@ -35,3 +35,13 @@ def test_rope_results_are_apart_from_positions_and_freqs():
             ops.rope(q, None, place, freqs, out_q=heads, **kw)
     with pytest.raises(ValueError, match="out_k shares memory with freqs"):
         ops.rope(torch.zeros(6, 4, 64, dtype=BF), q, at, words[100:132].view(F64), out_k=heads)
+
+
+def test_a_scalings_factor_needs_its_type():
+    """Without one it divided every frequency."""
+    for scaling in ({"factor": 4.0}, {"type": None, "factor": 4.0}):
+        with pytest.raises(ValueError, match="needs its type"):
+            frequencies(64, 1e4, scaling)
+    for scaling in (None, {}, {"type": None}, {"type": "linear"}):
+        f, m = frequencies(64, 1e4, scaling)
+        assert m == 1.0 and torch.equal(f, frequencies(64, 1e4)[0])
