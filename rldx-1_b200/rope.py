@@ -41,14 +41,16 @@ def frequencies(rotary_dim: int, theta: float, scaling: Optional[dict] = None):
     elif kind == "yarn":
         original = scaling.pop("original", None)
         fast, slow = float(scaling.pop("beta_fast", 32.0)), float(scaling.pop("beta_slow", 1.0))
-        if original is None or not original > 0 or not fast >= slow > 0 or theta == 1.0:
-            raise ValueError("yarn scaling needs the original length, beta_fast >= beta_slow > 0 and theta other than 1")
+        if original is None or not original > 0 or not fast >= slow > 0 or theta <= 1.0:
+            raise ValueError("yarn scaling needs the original length, beta_fast >= beta_slow > 0 and theta above 1")
 
         def pair_of(turns):  # (a real number) that turns so often within the original length
             return rotary_dim * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(theta))
 
         low, high = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), rotary_dim - 1)
         share = ((i / 2 - low) / max(high - low, 0.001)).clamp(0, 1)  # 0: kept, 1: divided
+        if pair_of(slow) < 0:  # not even the fastest pair turns so often
+            share = torch.ones_like(i)
         f = theta ** (-i / rotary_dim)
         f = f / s * share + f * (1 - share)
         m = float(scaling.pop("attention_factor", 0.1 * math.log(s) + 1.0 if s > 1 else 1.0))

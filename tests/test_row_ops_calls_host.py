@@ -45,3 +45,17 @@ def test_a_scalings_factor_needs_its_type():
     for scaling in (None, {}, {"type": None}, {"type": "linear"}):
         f, m = frequencies(64, 1e4, scaling)
         assert m == 1.0 and torch.equal(f, frequencies(64, 1e4)[0])
+
+
+def test_yarn_divides_every_pair_that_turns_too_little():
+    """The fastest pair was kept, however little it turns; with theta below 1 pairs were blended the wrong way round."""
+    f, _ = frequencies(128, 1e6)
+    for kw in (dict(original=5), dict(original=128, beta_fast=32.0, beta_slow=32.0), dict(original=128, beta_fast=64.0, beta_slow=21.0)):
+        assert kw["original"] / (2 * math.pi) < kw.get("beta_slow", 1.0)
+        y, _ = frequencies(128, 1e6, {"type": "yarn", "factor": 8.0, **kw})
+        assert torch.allclose(y, f / 8, rtol=1e-15, atol=0)
+    y, _ = frequencies(128, 1e6, {"type": "yarn", "factor": 8.0, "original": 7})  # one pair turns more than once
+    assert y[0] == f[0] and torch.allclose(y[2:], f[2:] / 8, rtol=1e-15, atol=0)
+    for theta in (0.5, 1.0):
+        with pytest.raises(ValueError, match="theta above 1"):
+            frequencies(128, theta, {"type": "yarn", "factor": 8.0, "original": 4096})
