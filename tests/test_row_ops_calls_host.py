@@ -59,3 +59,12 @@ def test_yarn_divides_every_pair_that_turns_too_little():
     for theta in (0.5, 1.0):
         with pytest.raises(ValueError, match="theta above 1"):
             frequencies(128, theta, {"type": "yarn", "factor": 8.0, "original": 4096})
+
+
+def test_rope_refusals_say_what_is_wrong():
+    q, at, f = torch.zeros(6, 4, 64, dtype=BF), torch.arange(6), torch.ones(32, dtype=F64)
+    for match, kw in (("sections must be a sequence", dict(sections=5)), ("integer", dict(sections=(16.0, 16))), ("real number", dict(factor="two"))):
+        with pytest.raises(TypeError, match=match):
+            ops.rope(q, None, at, f, **kw)
+        with pytest.raises(TypeError, match=match):
+            ops.rope_rows(at, f, **kw)
