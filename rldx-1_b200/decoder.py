@@ -209,6 +209,9 @@ class B200TextDecoder:
         self.kv_heads = a0.k_proj.weight.shape[0] // self.head_dim
         self.hidden = embed.shape[1]
         self.window, self.sinks = int(window), int(sinks)
+        # without a window= here a layer's own is kept to by refusing sequences that are longer than it
+        own = [getattr(m.self_attn, "sliding_window", None) for m in layers]
+        self.reach = min((int(w) for w in own if w is not None and not self.window), default=None)
         self._refuse_other_shapes(layers, norm, embed, lm_head)
         ln = layers[0].input_layernorm
         self.eps = float(getattr(ln, "variance_epsilon", getattr(ln, "eps", 1e-6)))
@@ -301,13 +304,18 @@ class B200TextDecoder:
         _lib.check(_lib.load().rldx_res_rmsnorm(C.byref(seg), 1, self.eps, C.c_void_p(torch.cuda.current_stream().cuda_stream)))
         return out
 
+    def _refuse_longer(self, longest: int, tables: bool) -> None:
+        """Raises for a sequence longer than the RoPE tables, or than a window that its layers have and the decoder was not given."""
+        if tables and longest > self.cos.shape[0]:
+            raise ValueError(f"a sequence of {longest} tokens is longer than the RoPE tables ({self.cos.shape[0]})")
+        if self.reach is not None and longest > self.reach:
+            raise ValueError(f"a sequence of {longest} tokens is longer than a layer's sliding window ({self.reach}): give the decoder its window")
+
     def _places(self, start: Sequence[int], new: Sequence[int], positions: Optional[torch.Tensor]) -> torch.Tensor:
         """The rows of the tables, or the rope's positions [axes, rows], that the new tokens take; refuses others."""
         rows, tables = sum(new), self.rope is None
+        self._refuse_longer(max(s + n for s, n in zip(start, new)), tables and positions is None)
         if positions is None:
-            longest = max(s + n for s, n in zip(start, new))
-            if tables and longest > self.cos.shape[0]:
-                raise ValueError(f"a sequence of {longest} tokens is longer than the RoPE tables ({self.cos.shape[0]})")
             positions = torch.cat([torch.arange(s, s + n, dtype=torch.int32) for s, n in zip(start, new)])
         elif tuple(positions.shape) != (rows,) and (tables or tuple(positions.shape) != (self.rope.axes, rows)):
             raise ValueError(f"positions must be [{rows}]" + ("" if tables else f" or [{self.rope.axes}, {rows}]") + f", got {tuple(positions.shape)}")
@@ -511,8 +519,7 @@ class B200TextDecoder:
             raise ValueError("a prompt has no token")
         if max_new_tokens > 0:  # what would end the run in its middle: all but the last token drawn are run
             ends = [t + r.shape[0] + max_new_tokens - 1 for t, r in zip(cache.tokens, rows)]
-            if positions is None and self.rope is None and max(ends) > self.cos.shape[0]:
-                raise ValueError(f"a sequence of {max(ends)} tokens is longer than the RoPE tables ({self.cos.shape[0]})")
+            self._refuse_longer(max(ends), positions is None and self.rope is None)
             cache.room([e - t for e, t in zip(ends, cache.tokens)])
         places = follow = None
         if positions is not None:

@@ -203,3 +203,22 @@ def test_scores_of_pieces_join(monkeypatch, rows):
     assert made == [min(rows, 7 - a) for a in range(0, 7, rows)]
     assert [s.rank.tolist() for s in got] == [[2, 3, 4, -1], [-1], [7, -1]]
     assert [s.logprob.tolist() for s in got] == [[0, 1, 2, 3], [4], [5, 6]] and [s.top_ids.tolist() for s in got][2] == [[5, 5], [6, 6]]
+
+
+def test_a_layers_own_window_is_not_left_out(monkeypatch):
+    """Layers with a sliding window ran over the whole sequence where the decoder was given none."""
+    def build(*windows, **kw):
+        return make([layer(sliding_window=w) for w in windows], **kw)
+
+    rows = torch.zeros(9, HIDDEN, dtype=BF)
+    for dec in (build(None, 8), build(8, 12), build(8, 8)):
+        cache = dec.new_cache(2, 256)
+        refused(dec, cache, ValueError, r"sliding window \(8\)", rows, [0, 9])
+        refused(dec, cache, ValueError, r"sliding window \(8\)", rows, [0, 9], positions=torch.arange(9))
+        cache.extend([0, 5])
+        refused(dec, cache, ValueError, r"sliding window \(8\)", rows[:4], [0, 4])
+        refused(dec, cache, ValueError, "no CPU path", rows[:3], [0, 3])  # everything else is right
+        with pytest.raises(ValueError, match="sliding window"):
+            dec.generate([[1], [2] * 5], 5, u=torch.zeros(5, 2))
+    for dec in (build(None, None), build(8, 8, window=8), make()):
+        refused(dec, dec.new_cache(2, 256), ValueError, "no CPU path", rows, [0, 9])
