@@ -10,7 +10,8 @@
 // A row lies in the registers of a team: 8 lanes, a warp or several, 16 values a thread.  The vectors come down
 // to four numbers a value, h' = h + (a y^ + b) and n = c h^ + d with a = scale gate (w + 1), b = scale gate b, c = (w + 1)
 // (1 + mod_scale), d = b (1 + mod_scale) + mod_shift, kept in shared memory and made once by a CTA.  Vectors of groups are
-// read beside the rows, as they are, where they have the rows' type and alignment; else each team makes its own four numbers
+// read beside the rows, as they are, where they have the rows' type and alignment, rows are of at most 4096 values
+// and either a group has fewer than 16 rows or a row is 8 lanes' (128 values); else each team makes its own four numbers
 // whenever it comes to another group.  A CTA goes over a run of rows, the next of which is on the way while one is
 // normed.  Bound by memory: y and h are read and h' and n written once.  8832 x 2048 bf16 with norms on both sides takes 26 us
 // (5.6 TB/s; at the copy's rate 22), with channel gates 27, 35968 x 1536 with a modulation of each 562 rows 83 (68), 4999 x

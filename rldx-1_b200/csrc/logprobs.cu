@@ -1,5 +1,5 @@
 // Log probabilities of given tokens under rows of logits, with the entropy of each row, the token's rank and the
-// top alternatives, in one pass over the logits.
+// top alternatives, in one pass over the logits (rows whose queue overflows are gone over again, see below).
 //
 // With M the row's maximum, d_i = x_i - M, S = sum exp(d_i) and T = sum exp(d_i) d_i:
 //   log p_i = d_i - ln S,   H = ln S - T / S  (both terms positive: nothing cancels),

@@ -3,9 +3,9 @@
 // with p the token's position on the pair's axis, f_i radians a position (double) and m a factor.  Pairs are
 // (i, i + r / 2) or (2 i, 2 i + 1) of the head's first r values; the others pass unchanged.
 //
-// Angles: p f_i is reduced to a fraction of a turn in doubles, so a position of a million loses nothing (in fp32 its
-// angle would be off by 0.06), and the sine and cosine of that fraction come in fp32 with the part of it that fp32
-// drops added to first order.  Everything else is fp32 with one rounding to the output's type.
+// Angles: p f_i is reduced to a fraction of a turn in doubles, off by less than 2^-51 |p f_i| (two products and the constant 1 / (2 pi)):
+// below fp32's own 2^-24 up to 2^27 radians.  (In fp32 the angle of a position of a million would be off by 0.06.)  The sine and
+// cosine of that fraction come in fp32 with the part of it that fp32 drops added to first order.  Everything else is fp32 with one rounding to the output's type.
 //
 // A block takes a few tokens: its threads make each token's cos and sin once, in shared memory, while their first
 // values are on the way, then turn the heads, V pairs a thread and step.  Bound by memory: every value is read and
@@ -309,8 +309,8 @@ int rldx_rope(const rldx_rope_plan* plan, const rldx_rope_heads* heads, int nhea
   rc = ensure_device();
   if (rc != RLDX_OK) return rc;
   // Tokens of a block: up to 384 items (us, 256 / 384 / 512 / 1024: 8832 tokens of 16 / 2 heads of 128 13.8 / 13.5 / 13.0 / 15.4, 65536 of
-  // 16 / 16 154 / 154 / 165 / 179, 11524 of 12 / 4 heads of 96 in fp32 21.5 / 23.5 / 23.5 / 28.5), but one while tokens are
-  // fewer than twice the SMs, and turns of 16 KB at most.
+  // 16 / 16 154 / 154 / 165 / 179, 11524 of 12 / 4 heads of 96 in fp32 21.5 / 23.5 / 23.5 / 28.5), but so few that there are two blocks
+  // an SM (one token a block while tokens are fewer than four times the SMs), and turns of 16 KB at most.
   long long tpb = std::max(1LL, std::min<long long>(384 / per_token, 2048 / plan->pairs));
   tpb = std::min(tpb, std::max(1LL, tokens / (2LL * sm_count())));
   p.tokens_per_block = static_cast<int>(tpb);

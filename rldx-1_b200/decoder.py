@@ -16,7 +16,7 @@ and produces tokens, one path through the decoding operators of `rldx_b200.ops`:
 
 `decoder_layers` are Qwen3 text decoder layers (the attribute names that B200LLMChain takes), `cos` and
 `sin` their RoPE tables [positions, head_dim]; with a B200Rope in their place (rope=) there is no table, positions may be of
-several axes and as far as they like.  Layers with norms behind their blocks too (pre_feedforward_layernorm and
+several axes and far ones (as exact as fp32 up to 2^27).  Layers with norms behind their blocks too (pre_feedforward_layernorm and
 post_feedforward_layernorm beside the other two), or a residual_scale, run through block_norms, which makes the sum
 and both norms in one pass.  Prompts of a vision tower bring positions and deepstack
 features of their own; everything that cannot be run is refused before the cache changes.  `python -m rldx_b200.decoder` decodes with random
@@ -411,7 +411,7 @@ class B200TextDecoder:
                 deepstack_rows: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Runs the rows `hidden` [sum(new), hidden] (the new tokens of every sequence, in order)
         through the layers; keys and values join the cache.  positions [sum(new)]: RoPE rows, the
-        tokens' places in their sequences by default; with a rope positions of any size, of one axis for all or [axes, sum(new)].
+        tokens' places in their sequences by default; with a rope any whole numbers, of one axis for all or [axes, sum(new)].
         deepstack_features[i] [n, hidden] are added after
         layer i to the rows deepstack_rows [n] of hidden (a vision tower's, as B200LLMChain takes them), with one
         rounding to bf16.  Returns logits [seqs with new tokens, vocab]

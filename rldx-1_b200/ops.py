@@ -413,8 +413,8 @@ def rope(q, k, positions, freqs, *, sections: Optional[Sequence[int]] = None, in
     token and head strides.  Pairs are (i, i + pairs), or (2 i, 2 i + 1) with interleaved; values of a head past
     2 pairs pass unchanged.  sections: positions are [axes, tokens] and sections[a] pairs take those of axis a, side by side, or
     with interleaved_sections pair i those of axis i % axes while i < axes * sections[i % axes] and of axis 0 from there on.
-    inverse turns backwards.  Angles are reduced in double, the rest is fp32 with one rounding.  out_q and
-    out_k may be q and k themselves.  Returns (q, k) rotated."""
+    inverse turns backwards (the transpose: the factor multiplies again).  Angles are reduced in double (off by less than 2^-51 of the angle: fp32's own accuracy up to 2^27
+    radians), the rest is fp32 with one rounding.  out_q and out_k may be q and k themselves, else share memory with no input.  Returns (q, k) rotated."""
     return _native().rope(q, k, positions, freqs, sections, interleaved_sections, interleaved, factor, inverse, out_q, out_k)
 
 
@@ -447,11 +447,14 @@ def block_norms(branch, residual, *, post: Optional[str] = None, post_weight=Non
 
 
 def token_logprobs(logits, tokens, *, top: int = 0):
-    """Of each row of logits [rows, vocab] (bf16, fp16 or fp32, any row stride), with one read of it: the log probability of
+    """Of each row of logits [rows, vocab] (bf16, fp16 or fp32, any row stride), with one read of it (two where more
+    values than a queue holds could be among the top): the log probability of
     tokens[row] (int64), the entropy, the token's rank (how many tokens have a larger logit, or an equal one and a
     lower id), and the top (at most 32) tokens in that order with their log probabilities.  A negative token is
     none: logprob 0, rank -1.  A token past the vocabulary records device error 0x503 and gives NaN and -1.  A row that holds NaN or
-    +inf, or nothing but -inf, has no distribution: NaN, rank and ids -1.  Sums are fp32: logprob and entropy are good to a few
-    2^-24 of 1 + their size.  Returns logprob, entropy [rows] fp32, rank [rows] int32, top_ids
-    [rows, top] int64, top_logprobs [rows, top] fp32."""
+    +inf, or nothing but -inf, has no distribution: NaN, rank and ids -1.  Sums are fp32: with D the mean and D2 the mean square
+    of how far a drawn token's logit lies below the largest, logprob is good to e = 2^-24 (140 + vocab / 680 + 3 D) and entropy to
+    e (1 + D) + 2^-24 3 D2, besides a few 2^-24 of their own size and of the token's distance
+    from the largest logit.  Returns logprob, entropy [rows] fp32, rank [rows] int32, top_ids [rows, top] int64, top_logprobs
+    [rows, top] fp32."""
     return _native().token_logprobs(logits, tokens, top)

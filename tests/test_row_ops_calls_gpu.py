@@ -147,3 +147,30 @@ def test_rows_of_any_layout(cuda):
         wide = torch.zeros(30, CFG.hidden + 3, dtype=BF, device=cuda)[:, 1: 1 + CFG.hidden]
         for x in (rows.t().contiguous().t(), off.copy_(rows), wide.copy_(rows)):
             assert torch.equal(dec.forward(x, dec.new_cache(1, 64), [30]), want)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_logprobs_are_as_good_as_stated(cuda, dtype):
+    """e = 2^-24 (140 + vocab / 680 + 3 D): 35 units of a weight and of the sums' fixed steps, 6 a chunk of a thread (a sum, and the move of
+    its reference), at most vocab / 4096 + 1 chunks or 16; rows that rise slowly move the reference with every chunk."""
+    vocab = 151680
+    g = torch.Generator(device=cuda).manual_seed(4)
+    rise = torch.linspace(-3, 0, vocab, device=cuda)
+    x = torch.stack([rise, 20 * rise, rise.flip(0), torch.zeros(vocab, device=cuda), 0.01 * torch.randn(vocab, device=cuda, generator=g),
+                     3 * torch.randn(vocab, device=cuda, generator=g), 2000 * rise]).to(dtype)
+    for rows in (x, x.repeat(100, 1)):  # a cluster a row, and one CTA
+        t = torch.randint(vocab, (len(rows),), device=cuda, generator=g)
+        logprob, entropy, _, _, _ = ops.token_logprobs(rows, t)
+        for a in range(0, len(rows), 70):
+            at = slice(a, a + 70)
+            y = rows[at].double()
+            d = y - y.amax(1, keepdim=True)
+            logs = torch.log_softmax(y, 1)
+            p = logs.exp()
+            mean, square = (p * d.abs()).sum(1), (p * d * d).sum(1)
+            e = 2.0 ** -24 * (140 + vocab / 680 + 3 * mean)
+            want = logs.gather(1, t[at, None])[:, 0]
+            few = 4 * 2.0 ** -24
+            assert bool(((logprob[at] - want).abs() <= e + few * (want.abs() + d.gather(1, t[at, None])[:, 0].abs())).all())
+            want = -(p * logs).sum(1)
+            assert bool(((entropy[at] - want).abs() <= e * (1 + mean) + 3 * 2.0 ** -24 * square + few * want).all())
