@@ -132,7 +132,7 @@ def _refuse_other_norm(norm, name: str) -> None:
     n = w.shape[0]
     x = torch.linspace(-1.0, 2.0, n, device=w.device, dtype=torch.float32).to(w.dtype)
     with torch.no_grad():
-        got = norm(x.expand(2, n))[0].float()
+        got = norm(x.repeat(2, 1))[0].float()
     x = x.float()
     hat = x * torch.rsqrt((x * x).mean())
     want = hat * w.float()
